@@ -209,8 +209,106 @@ int paia_gemv_plan_create(int kind, int math, int nops, const paia_gemv_op* ops,
 int paia_gemv_plan_launch(const paia_gemv_plan* plan, void* stream);
 int paia_gemv_plan_destroy(paia_gemv_plan* plan);
 
-/* Device-side error word of the current device (0 = none), set by kernels whose bounded waits gave up; clear != 0
- * resets it. Synchronous. */
+/* ---- Serving operators beside the GEMVs (no reference kernel): a batched decode step's attention, rotary positions and
+ * adapters. They launch with programmatic dependent launch, allocate nothing and never synchronise. Strides are counted
+ * in elements and the innermost dimension is contiguous; 64-bit offsets throughout. Codes: 0, -2 bad argument, >0
+ * cudaError_t. Indices that live on the device (page ids, lengths, positions, adapter ids) are checked by the kernels:
+ * a bad one is never followed to memory and sets a code of paia_gemv_device_error (10 page id, 11 length, 12 position
+ * or sequence, 13 adapter id). */
+
+/* Attention of one new token per sequence over a paged key-value cache (grouped-query: heads / kv_heads query heads
+ * share a kv head). Sequence b holds positions 0 .. lens[b] - 1; position j lies in row j % page_size of page
+ * page_table[b][j / page_size]. For query head h of kv head h / (heads / kv_heads):
+ *   s_j = scale k_scale <q_h, k_j>,  p = softmax(s),  out_h = v_scale sum_j p_j v_j,  lse_h = log sum_j exp s_j
+ * over the last `window` positions (0: all). Statistics and sums are fp32; out is rounded once to bf16. A sequence of
+ * length 0 gives out = 0 and lse = -inf; so does a row whose scores are all -inf. Cache rows outside the range are never
+ * read. A page id outside [0, num_pages) (code 10) reads as zero rows, a length above max_pages page_size is cut to it
+ * and one below 0 is 0 (code 11).
+ * q, out bf16; cache bf16 or e4m3 with a fp32 scale per kv head (value = stored * scale). head_dim 64, 96, 128 or 256;
+ * any page size and page / token / head strides (both [page][token][head] and [page][head][token] caches). q, k and v
+ * 16-byte aligned with strides of whole 16 bytes, out 8-byte aligned with strides of multiples of 4 elements. `workspace`:
+ * paia_gemv_paged_attn_workspace(heads, kv_heads, head_dim) bytes on the launch's device, 16-byte aligned, zeroed once;
+ * every launch leaves it ready for the next, of any batch; launches that may overlap on the GPU (other streams, graphs
+ * replayed at the same time) need a workspace each. */
+typedef struct paia_gemv_attn {
+    const void* q;               /* bf16 [batch][heads][head_dim] */
+    const void* k;               /* cache [num_pages][page_size][kv_heads][head_dim], any strides */
+    const void* v;
+    const int* page_table;       /* [batch][max_pages] */
+    const int* lens;             /* [batch], 4-byte aligned */
+    const float* k_scale;        /* [kv_heads] or NULL (1); e4m3 caches only */
+    const float* v_scale;
+    void* out;                   /* bf16 [batch][heads][head_dim] */
+    float* lse;                  /* [batch][heads] or NULL */
+    void* workspace;
+    long long q_batch, q_head, out_batch, out_head, lse_batch, table_batch;
+    long long k_page, k_token, k_head, v_page, v_token, v_head;
+    int batch, heads, kv_heads, head_dim;
+    int cache;                   /* 0 bf16, 1 e4m3 */
+    int num_pages, page_size, max_pages;
+    int window;
+    float scale;
+} paia_gemv_attn;
+size_t paia_gemv_paged_attn_workspace(int heads, int kv_heads, int head_dim);   /* 0: unsupported sizes */
+int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream);
+
+/* The step between a fused QKV projection and the attention, for any number of tokens: per-head RMS norm of q and k
+ * (where q_norm / k_norm are given), rotation of q and k at each token's own position, q stored, k and v stored into
+ * their cache pages. Token t of sequence seq[t] (NULL: t) at position pos[t] goes to row pos % page_size of page
+ * page_table[seq][pos / page_size]; a token with position -1 is padding: nothing is read or stored for it. With
+ * x' = x / sqrt(mean x^2 + eps) * w, pair i of a head, (x'_i, x'_(i + rot / 2)) or, interleaved, (x'_2i, x'_(2i + 1)),
+ * turns by pos * inv_freq[i]; dimensions from rot on stay. Arithmetic is fp32 (angles fp64; an e4m3 cache's k fp64),
+ * rounded once. inv_freq is fp64 [rot / 2]: theta^(-2i / rot) or any scaled table. e4m3 caches store x / scale[kv head],
+ * at most 448 in magnitude. q_out may be the q part of qkv itself. k_out (NULL: none) receives the rotated keys as bf16
+ * too; k and v may both be NULL (no cache) where k_out is given. head_dim and rot are multiples of 16, head_dim <= 256,
+ * rot <= head_dim. qkv, q_out, k_out, k, v 16-byte aligned with strides of whole 16 bytes. Two tokens of one call must
+ * not name the same sequence and position. */
+typedef struct paia_gemv_rope_cache {
+    const void* qkv;             /* bf16 [tokens][(heads + 2 kv_heads) * head_dim] */
+    const int* pos;              /* [tokens] */
+    const int* seq;              /* [tokens] or NULL */
+    const double* inv_freq;      /* [rot / 2] */
+    const float* q_norm;         /* [head_dim] or NULL */
+    const float* k_norm;
+    const int* page_table;       /* [sequences][max_pages] */
+    const float* k_scale;        /* [kv_heads] or NULL (1); e4m3 caches only */
+    const float* v_scale;
+    void* q_out;                 /* bf16 [tokens][heads][head_dim] */
+    void* k_out;                 /* bf16 [tokens][kv_heads][head_dim] or NULL */
+    void* k;                     /* cache as in paia_gemv_attn */
+    void* v;
+    long long qkv_token, q_token, q_head, ko_token, ko_head, table_seq;
+    long long k_page, k_row, k_head, v_page, v_row, v_head;
+    int tokens, sequences, heads, kv_heads, head_dim, rot;
+    int interleaved;
+    int cache;                   /* 0 bf16, 1 e4m3 */
+    int num_pages, page_size, max_pages;
+    float eps;
+} paia_gemv_rope_cache;
+int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* stream);
+
+/* Low-rank adapters of many requests beside a shared projection (paia_gemv_batched): for every row m with adapter
+ * a = adapter[m],  out[m] = base[m] + scaling[a] B[a] (A[a] x[m]);  rows with adapter -1 get base[m]. Adapter a uses its
+ * first ranks[a] ranks (NULL: all `rank`; 0: none; what lies behind them is not used), scaling NULL is 1, base NULL is 0,
+ * base may be out itself. Sums are fp32, A x is kept in 32 bits between the two products, and out is rounded once to
+ * bf16. An id outside [-1, adapters) (code 13) is treated as -1. rank, K and N are multiples of 8, rank <= 256,
+ * adapters <= 8192. x, A, B, base, out 16-byte aligned with strides of whole 16 bytes. */
+typedef struct paia_gemv_lora_args {
+    const void* x;               /* bf16 [M][K] */
+    const void* a;               /* bf16 [adapters][rank][K] */
+    const void* b;               /* bf16 [adapters][N][rank] */
+    const int* adapter;          /* [M] */
+    const int* ranks;            /* [adapters] or NULL */
+    const float* scaling;        /* [adapters] or NULL */
+    const void* base;            /* bf16 [M][N] or NULL */
+    void* out;                   /* bf16 [M][N] */
+    long long x_row, base_row, out_row, a_adapter, a_row, b_adapter, b_row;
+    int M, N, K, rank, adapters;
+} paia_gemv_lora_args;
+int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream);
+
+/* Device-side error word of the current device (0 = none), set by kernels whose bounded waits gave up (codes below
+ * 10) or that met a bad index in device memory (10 to 13); clear != 0 resets it. Synchronous. */
 int paia_gemv_device_error(int clear);
 
 #ifdef __cplusplus

@@ -21,6 +21,9 @@ int launch_int4_naive(const void* Wq, const void* sc, const void* x, void* y, in
 int launch_int4_dequant(const void* Wq, const void* sc, void* out, int N, int K, cudaStream_t st);
 const Variant* extra_int4(int* n);
 const Variant* extra_int4a(int* n);
+int attn_device_error(int clear);
+int rope_device_error(int clear);
+int lora_device_error(int clear);
 
 // ------------------------------------------------------------------ per-device caches
 namespace {
@@ -831,7 +834,14 @@ int paia_gemv_launch_ex(int kind, int R, int U, int W, int math, int pdl, int ks
 }
 
 // Device-side error word of the current device (0 = none; the codes of the TMA-fed kernels' bounded waits, 6 and 8
-// from the tensor-parallel exchange); clear != 0 resets it. Synchronous (a symbol copy).
-int paia_gemv_device_error(int clear) { return tma_device_error(clear); }
+// from the tensor-parallel exchange), then the serving operators' words (10 to 13, bad indices in device memory);
+// clear != 0 resets them all. Synchronous (symbol copies).
+int paia_gemv_device_error(int clear) {
+    const int words[4] = {tma_device_error(clear), attn_device_error(clear), rope_device_error(clear),
+                          lora_device_error(clear)};
+    for (int w : words)
+        if (w) return w;
+    return 0;
+}
 
 }  // extern "C"

@@ -8,7 +8,8 @@ behaviour (a nonzero return code raises RuntimeError; -1 bad variant, -2 bad sha
 
 Added for the B200 build: `int4_asym` (asymmetric INT4 g128, bf16 scale and zero), an optional fused bias on every
 format (`*_bias`), `variant_info_ex` (the B200 launch configuration a variant maps to), `device_error()`, `layer` and `plan_*` (one
-persistent launch for a sequence of GEMVs), and the tensor-parallel helpers used by paia_gemv.tp. There is no CPU fallback: without the library every op raises.
+persistent launch for a sequence of GEMVs), the tensor-parallel helpers used by paia_gemv.tp and the serving operators used
+by paia_gemv.serve. There is no CPU fallback: without the library every op raises.
 """
 import ctypes
 import os
@@ -122,6 +123,11 @@ class GemvLib:
         lib.paia_gemv_int4_asym_variant_count.restype = I
         lib.paia_gemv_variant_info_ex.restype = I
         lib.paia_gemv_variant_info_ex.argtypes = [I, I, ctypes.POINTER(VariantEx)]
+        for name in ("paia_gemv_paged_attn", "paia_gemv_qkv_rope_cache", "paia_gemv_lora"):
+            getattr(lib, name).restype = I
+            getattr(lib, name).argtypes = [P, P]
+        lib.paia_gemv_paged_attn_workspace.restype = ctypes.c_size_t
+        lib.paia_gemv_paged_attn_workspace.argtypes = [I, I, I]
         lib.paia_gemv_device_error.restype = I
         lib.paia_gemv_device_error.argtypes = [I]
         lib.paia_gemv_version.restype = ctypes.c_char_p
@@ -317,8 +323,27 @@ class GemvLib:
     def plan_destroy(self, plan):
         self._check(self._lib.paia_gemv_plan_destroy(plan), "paia_gemv_plan_destroy")
 
+    # --- serving operators (paia_gemv.serve drives these); args: the bytes of the C struct of the same name, in its
+    # field order (serve.ATTN, serve.ROPE_CACHE, serve.LORA pack them)
+    def paged_attn_workspace(self, heads, kv_heads, head_dim):
+        n = self._lib.paia_gemv_paged_attn_workspace(heads, kv_heads, head_dim)
+        if n == 0:
+            raise RuntimeError(f"paia_gemv_paged_attn_workspace: unsupported sizes (heads={heads}, kv_heads={kv_heads}, "
+                               f"head_dim={head_dim})")
+        return n
+
+    def paged_attn(self, args, stream=None):
+        self._check(self._lib.paia_gemv_paged_attn(args, self._st(stream)), "paia_gemv_paged_attn")
+
+    def qkv_rope_cache(self, args, stream=None):
+        self._check(self._lib.paia_gemv_qkv_rope_cache(args, self._st(stream)), "paia_gemv_qkv_rope_cache")
+
+    def lora(self, args, stream=None):
+        self._check(self._lib.paia_gemv_lora(args, self._st(stream)), "paia_gemv_lora")
+
     def device_error(self, clear=True):
-        """The device-side error word (0 = none) written by kernels whose bounded waits gave up."""
+        """The device-side error word (0 = none): below 10 from kernels whose bounded waits gave up, 10 to 13 from
+        serving operators that met a bad page id, length, position or adapter id."""
         return self._lib.paia_gemv_device_error(1 if clear else 0)
 
 

@@ -1,0 +1,217 @@
+"""CPU (no GPU needed): the serving operators' C structs as paia_gemv.serve packs them, their refusals on the host (code
+-2 before any device is touched) and the checks of the tensor wrappers (ValueError)."""
+import re
+import subprocess
+from pathlib import Path
+
+import pytest
+import torch
+
+ROOT = Path(__file__).resolve().parents[1]
+PTR = 0x10000
+
+
+@pytest.fixture(scope="module")
+def L(lib_path):
+    from paia_gemv import loader
+    return loader.GemvLib(lib_path)
+
+
+def fields(name):
+    """The field names of a struct of the header, in order, and their kinds (P pointer, q, i, f)."""
+    txt = re.sub(r"/\*.*?\*/", "", (ROOT / "include" / "paia_gemv.h").read_text(), flags=re.S)
+    body = re.search(r"typedef struct %s \{(.*?)\}" % name, txt, flags=re.S).group(1)
+    out = []
+    for decl in body.split(";"):
+        decl = decl.strip()
+        if not decl:
+            continue
+        kind = "P" if "*" in decl else "q" if decl.startswith("long long") else "f" if decl.startswith("float") else "i"
+        names = re.sub(r"^(const )?(void|int|float|double|long long)\b", "", decl)
+        out += [(n.strip(" *"), kind) for n in names.split(",")]
+    return out
+
+
+def packed(name, fmt, good, **change):
+    values = dict(good)
+    values.update(change)
+    names = fields(name)
+    assert {n for n, _ in names} == set(values)
+    return fmt.pack(*[values[n] for n, _ in names])
+
+
+ATTN = dict(q=PTR, k=PTR, v=PTR, page_table=PTR, lens=PTR, k_scale=0, v_scale=0, out=PTR, lse=0, workspace=PTR,
+            q_batch=1024, q_head=128, out_batch=1024, out_head=128, lse_batch=8, table_batch=4, k_page=4096, k_token=256,
+            k_head=128, v_page=4096, v_token=256, v_head=128, batch=2, heads=8, kv_heads=2, head_dim=128, cache=0,
+            num_pages=9, page_size=16, max_pages=4, window=0, scale=0.1)
+ROPE = dict(qkv=PTR, pos=PTR, seq=0, inv_freq=PTR, q_norm=0, k_norm=0, page_table=PTR, k_scale=0, v_scale=0, q_out=PTR,
+            k_out=0, k=PTR, v=PTR, qkv_token=1536, q_token=1024, q_head=128, ko_token=0, ko_head=0, table_seq=4,
+            k_page=4096, k_row=256, k_head=128, v_page=4096, v_row=256, v_head=128, tokens=3, sequences=3, heads=8,
+            kv_heads=2, head_dim=128, rot=128, interleaved=0, cache=0, num_pages=9, page_size=16, max_pages=4, eps=1e-6)
+LORA = dict(x=PTR, a=PTR, b=PTR, adapter=PTR, ranks=0, scaling=0, base=0, out=PTR, x_row=64, base_row=0, out_row=64,
+            a_adapter=512, a_row=64, b_adapter=512, b_row=8, M=3, N=64, K=64, rank=8, adapters=2)
+
+
+def test_structs_match_the_header(tmp_path):
+    from paia_gemv import serve
+    names = {"paia_gemv_attn": serve.ATTN, "paia_gemv_rope_cache": serve.ROPE_CACHE, "paia_gemv_lora_args": serve.LORA}
+    for n, fmt in names.items():
+        kinds = "".join(k for _, k in fields(n))
+        spelled = "".join(k * int(c or 1) for c, k in re.findall(r"(\d*)([Pqif])", fmt.format))
+        assert kinds == spelled, n
+    src = tmp_path / "s.c"
+    src.write_text('#include <stdio.h>\n#include "paia_gemv.h"\nint main(void) { printf("'
+                   + " ".join(["%zu"] * 3) + '", ' + ", ".join(f"sizeof({n})" for n in names) + "); return 0; }\n")
+    subprocess.run(["gcc", "-I", str(ROOT / "include"), str(src), "-o", str(tmp_path / "s")], check=True)
+    got = subprocess.run([str(tmp_path / "s")], capture_output=True, text=True, check=True).stdout.split()
+    assert [int(v) for v in got] == [f.size for f in names.values()]
+
+
+@pytest.mark.parametrize("change", [
+    dict(heads=7), dict(heads=0), dict(kv_heads=0), dict(head_dim=80), dict(head_dim=512), dict(batch=-1), dict(cache=2),
+    dict(cache=-1), dict(page_size=0), dict(max_pages=-1), dict(num_pages=-1), dict(window=-1), dict(scale=0.0),
+    dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=0), dict(k=0), dict(v=0),
+    dict(page_table=0), dict(lens=0), dict(out=0), dict(workspace=0), dict(q=PTR + 2), dict(k=PTR + 8), dict(v=PTR + 8),
+    dict(workspace=PTR + 4), dict(out=PTR + 4), dict(lse=PTR + 2), dict(lens=PTR + 2), dict(page_table=PTR + 1),
+    dict(q_batch=1020), dict(q_head=130), dict(out_head=127), dict(k_token=260), dict(v_page=4100), dict(k_head=129),
+    dict(k_scale=PTR), dict(v_scale=PTR), dict(cache=1, k_token=264), dict(cache=1, k_scale=PTR + 1),
+    dict(page_size=65536, max_pages=65536)])
+def test_attention_refusals(L, change):
+    from paia_gemv import serve
+    assert L._lib.paia_gemv_paged_attn(packed("paia_gemv_attn", serve.ATTN, ATTN, **change), None) == -2
+
+
+@pytest.mark.parametrize("change", [
+    dict(tokens=-1), dict(heads=0), dict(kv_heads=0), dict(head_dim=24), dict(head_dim=272), dict(head_dim=0), dict(rot=8),
+    dict(rot=144), dict(rot=-16), dict(cache=3), dict(eps=-1.0), dict(eps=float("nan")), dict(qkv=0), dict(pos=0),
+    dict(q_out=0), dict(inv_freq=0), dict(k=0), dict(v=0), dict(k=0, v=0), dict(page_table=0), dict(sequences=0),
+    dict(num_pages=0), dict(page_size=0), dict(max_pages=0), dict(k_scale=PTR), dict(qkv=PTR + 2), dict(q_out=PTR + 8),
+    dict(k=PTR + 8), dict(k_out=PTR + 4), dict(q_norm=PTR + 4), dict(inv_freq=PTR + 4), dict(pos=PTR + 2),
+    dict(qkv_token=1537), dict(q_token=4), dict(q_head=12), dict(ko_token=4), dict(k_row=260), dict(v_head=3),
+    dict(cache=1, v_row=264)])
+def test_rope_refusals(L, change):
+    from paia_gemv import serve
+    args = packed("paia_gemv_rope_cache", serve.ROPE_CACHE, ROPE, **change)
+    assert L._lib.paia_gemv_qkv_rope_cache(args, None) == -2
+
+
+@pytest.mark.parametrize("change", [
+    dict(M=-1), dict(N=0), dict(N=60), dict(K=0), dict(K=4), dict(K=60), dict(rank=0), dict(rank=12), dict(rank=264),
+    dict(adapters=0), dict(adapters=8193), dict(x=0), dict(a=0), dict(b=0), dict(adapter=0), dict(out=0), dict(x=PTR + 8),
+    dict(a=PTR + 2), dict(b=PTR + 4), dict(base=PTR + 8), dict(out=PTR + 8), dict(adapter=PTR + 2), dict(ranks=PTR + 1),
+    dict(scaling=PTR + 2), dict(x_row=65), dict(base_row=4), dict(out_row=68), dict(a_adapter=4), dict(a_row=66),
+    dict(b_adapter=2), dict(b_row=12)])
+def test_lora_refusals(L, change):
+    from paia_gemv import serve
+    assert L._lib.paia_gemv_lora(packed("paia_gemv_lora_args", serve.LORA, LORA, **change), None) == -2
+
+
+def test_nothing_to_do_and_null(L):
+    from paia_gemv import serve
+    lib = L._lib
+    assert lib.paia_gemv_paged_attn(packed("paia_gemv_attn", serve.ATTN, ATTN, batch=0), None) == 0
+    assert lib.paia_gemv_qkv_rope_cache(packed("paia_gemv_rope_cache", serve.ROPE_CACHE, ROPE, tokens=0), None) == 0
+    assert lib.paia_gemv_lora(packed("paia_gemv_lora_args", serve.LORA, LORA, M=0), None) == 0
+    assert lib.paia_gemv_paged_attn(None, None) == lib.paia_gemv_qkv_rope_cache(None, None) == -2
+    assert lib.paia_gemv_lora(None, None) == -2
+    assert lib.paia_gemv_paged_attn_workspace(8, 3, 128) == lib.paia_gemv_paged_attn_workspace(8, 2, 100) == 0
+    with pytest.raises(RuntimeError):
+        L.paged_attn_workspace(8, 3, 128)
+    with pytest.raises(RuntimeError):
+        L.lora(packed("paia_gemv_lora_args", serve.LORA, LORA, rank=12), 0)
+    assert L.paged_attn_workspace(32, 8, 128) < L.paged_attn_workspace(64, 8, 128) <= 16 << 20
+
+
+def test_wrappers_refuse_tensors_off_the_device(L):
+    from paia_gemv import serve
+    bf, i32 = torch.bfloat16, torch.int32
+    q, pool = torch.zeros(1, 4, 64, dtype=bf), torch.zeros(2, 16, 2, 64, dtype=bf)
+    one = torch.zeros(1, dtype=i32)
+    with pytest.raises(ValueError, match="current CUDA device"):
+        serve.paged_attention(L, q, pool, pool, one.view(1, 1), one, q, torch.zeros(1 << 20, dtype=torch.uint8))
+    with pytest.raises(ValueError, match="current CUDA device"):
+        serve.qkv_rope_cache(L, torch.zeros(1, 8 * 64, dtype=bf), one, torch.ones(32, dtype=torch.float64), q, pool, pool,
+                             one.view(1, 1))
+    with pytest.raises(ValueError, match="current CUDA device"):
+        serve.lora(L, torch.zeros(1, 64, dtype=bf), torch.zeros(1, 8, 64, dtype=bf), torch.zeros(1, 64, 8, dtype=bf), one,
+                   torch.zeros(1, 64, dtype=bf))
+
+
+class OnDevice(torch.Tensor):
+    """A CPU tensor that says it is on CUDA device 0: the wrappers' checks run, nothing is launched."""
+    def get_device(self):
+        return 0
+
+
+def on(t):
+    return t.as_subclass(OnDevice)
+
+
+class Recorder:
+    """Stands in for the library: takes the packed struct."""
+    def __init__(self):
+        self.calls = []
+
+    def paged_attn_workspace(self, heads, kv_heads, head_dim):
+        return 64
+
+    def paged_attn(self, args, stream=None):
+        self.calls.append(args)
+
+    qkv_rope_cache = lora = paged_attn
+
+
+def test_wrapper_checks(monkeypatch):
+    """Every tensor of a call is checked for its type, shape, layout and device before the library sees it."""
+    from paia_gemv import serve
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    bf, i32, rec = torch.bfloat16, torch.int32, Recorder()
+    z = lambda *s, dtype=bf: on(torch.zeros(*s, dtype=dtype))   # noqa: E731
+    good = dict(q=z(3, 4, 64), k_pages=z(5, 16, 2, 64), v_pages=z(5, 16, 2, 64), page_table=z(3, 6, dtype=i32),
+                lens=z(3, dtype=i32), out=z(3, 4, 64), workspace=z(64, dtype=torch.uint8))
+    serve.paged_attention(rec, **good)
+    hnd = z(5, 2, 16, 64).transpose(1, 2)
+    serve.paged_attention(rec, **dict(good, k_pages=hnd, v_pages=hnd), lse=z(3, 4, dtype=torch.float32), window=5)
+    vals = serve.ATTN.unpack(rec.calls[1])
+    names = [n for n, _ in fields("paia_gemv_attn")]
+    got = dict(zip(names, vals))
+    assert (got["batch"], got["heads"], got["kv_heads"], got["head_dim"]) == (3, 4, 2, 64)
+    assert (got["num_pages"], got["page_size"], got["max_pages"], got["window"]) == (5, 16, 6, 5)
+    assert (got["k_page"], got["k_token"], got["k_head"]) == (2 * 16 * 64, 64, 16 * 64)
+    assert abs(got["scale"] - 0.125) < 1e-9 and got["lse"] and not got["k_scale"]
+    f32 = torch.float32
+    for bad in (dict(q=z(3, 4, 64, dtype=f32)), dict(q=z(3, 5, 64)), dict(q=z(4, 64)), dict(q=z(3, 64, 4).transpose(1, 2)),
+                dict(k_pages=z(5, 16, 2, 128)), dict(k_pages=z(5, 16, 128)), dict(v_pages=z(4, 16, 2, 64)),
+                dict(v_pages=z(5, 16, 2, 64, dtype=torch.float8_e4m3fn)), dict(k_pages=z(5, 16, 2, 64, dtype=f32)),
+                dict(page_table=z(2, 6, dtype=i32)), dict(page_table=z(3, 6, dtype=torch.int64)),
+                dict(page_table=z(18, dtype=i32)), dict(lens=z(2, dtype=i32)), dict(lens=z(3, dtype=torch.int64)),
+                dict(lens=z(6, dtype=i32)[::2]), dict(out=z(3, 4, 32)), dict(out=z(3, 4, 64, dtype=f32)),
+                dict(workspace=z(32, dtype=torch.uint8)), dict(k_scale=z(2, dtype=f32)),
+                dict(lse=z(3, 5, dtype=f32)), dict(lse=z(3, 4)), dict(lens=torch.zeros(3, dtype=i32)),
+                dict(v_pages=torch.zeros(5, 16, 2, 64, dtype=bf))):
+        with pytest.raises(ValueError):
+            serve.paged_attention(rec, **dict(good, **bad))
+    good = dict(qkv=z(3, 8 * 64), positions=z(3, dtype=i32), inv_freq=z(32, dtype=torch.float64), q_out=z(3, 4, 64),
+                k_pages=z(5, 16, 2, 64), v_pages=z(5, 16, 2, 64), page_table=z(3, 6, dtype=i32))
+    serve.qkv_rope_cache(rec, **good)
+    serve.qkv_rope_cache(rec, **dict(good, page_table=z(1, 6, dtype=i32)), seq=z(3, dtype=i32))
+    none = dict(good, k_pages=None, v_pages=None, page_table=None)
+    serve.qkv_rope_cache(rec, **none, k_out=z(3, 2, 64), kv_heads=2)
+    for bad in (dict(qkv=z(3, 7 * 64)), dict(qkv=z(2, 8 * 64)), dict(positions=z(2, dtype=i32)),
+                dict(positions=z(3, dtype=torch.int64)), dict(inv_freq=z(32, dtype=f32)), dict(inv_freq=z(4, 8, dtype=torch.float64)),
+                dict(q_out=z(3, 256)), dict(page_table=z(2, 6, dtype=i32)), dict(seq=z(2, dtype=i32)),
+                dict(q_norm=z(64)), dict(k_norm=z(32, dtype=f32)), dict(k_out=z(3, 1, 64)), dict(v_scale=z(2, dtype=f32)),
+                dict(v_pages=z(5, 16, 2, 64).transpose(0, 3))):
+        with pytest.raises(ValueError):
+            serve.qkv_rope_cache(rec, **dict(good, **bad))
+    for bad in (none, dict(none, k_out=z(3, 2, 64)), dict(none, kv_heads=2), dict(good, k_pages=None)):
+        with pytest.raises(ValueError):
+            serve.qkv_rope_cache(rec, **bad)
+    good = dict(x=z(3, 64), a=z(2, 8, 64), b=z(2, 40, 8), adapter=z(3, dtype=i32), out=z(3, 40))
+    serve.lora(rec, **good)
+    for bad in (dict(x=z(3, 32)), dict(x=z(64)), dict(a=z(8, 64)), dict(a=z(2, 8, 64, dtype=f32)), dict(b=z(2, 40, 16)),
+                dict(b=z(1, 40, 8)), dict(adapter=z(2, dtype=i32)), dict(adapter=z(3, dtype=torch.int64)),
+                dict(out=z(3, 48)), dict(base=z(2, 40)), dict(base=z(3, 40, dtype=f32)), dict(scaling=z(3, dtype=f32)),
+                dict(scaling=z(2)), dict(ranks=z(2, dtype=f32)), dict(out=z(40, 3).t())):
+        with pytest.raises(ValueError):
+            serve.lora(rec, **dict(good, **bad))
