@@ -6,18 +6,23 @@
 // Bound: HBM. A step must read 2 len kv_heads head_dim elements once and does 4 flops on each per query head of the
 // group, far below what even mma.sync gives (a group of 8 at 6.5 TB/s of bf16 needs 0.05 PFLOP/s), so everything here
 // serves the stream of cache rows:
-//   split     The launch does not know the lengths. All sequences' tiles of 16 positions form one list (sequence, kv
+//   split     The launch does not know the lengths. All sequences' tiles of 16 or 32 positions form one list (sequence, kv
 //             head, tile), and every CTA takes an equal run of it, so a ragged batch or one long sequence fills the GPU
-//             alike. Each CTA finds its run from lens itself (a block-wide prefix sum).
-//   stream    A warp owns a ring of stages, each the K and V rows of one 16-position tile, filled with cp.async (any
+//             alike. A unit (a sequence's kv head) weighs 14 tiles on top of its own, what its merge and output take:
+//             without that weight the CTAs that got a batch's short and empty sequences finished last (32 ragged
+//             sequences up to 4100: 40 us; weight 3: 31, 14: 23). Each CTA finds its run from lens itself.
+//   stream    A warp owns a ring of stages, each the K and V rows of one tile of positions, filled with cp.async (any
 //             page size and strides, rows outside the range arrive as zeros) and running on across sequences and
-//             heads; no warp waits for another while it streams. 16-byte chunks are XOR-swizzled by row so that
-//             ldmatrix and the 4-byte fragment reads are free of bank conflicts.
-//   math      The group's query heads are the 16 rows of m16n8k16 (S = Q K^T, O += P V). With up to 8 heads, rows 8-15
-//             carry the rounding remainder of P (P = hi + lo, two bf16), so P V is good to 2^-17 at no extra
-//             instruction; a group of 9 to 16 spends a second MMA on it. e4m3 rows become f16 exactly and meet q in f16,
-//             scaled per head by a power of two so that its largest element is in [1, 2) (the elements that lose bits
-//             are below 2^-14 of it); P is f16 there (2^-12). Larger groups are cut into units of 16 heads.
+//             heads; no warp waits for another while it streams. Page ids are looked up for 32 tiles at a time, a tile
+//             per lane. 16-byte chunks are XOR-swizzled by row so that the fragment reads are free of bank conflicts.
+//   math      The group's query heads are rows of the MMAs (S = Q K^T, O += P V).
+//             bf16: m16n8k16. With up to 8 heads, rows 8-15 carry the rounding remainder of P (P = hi + lo, two bf16), so
+//             P V is good to 2^-16 at no extra instruction; a group of 9 to 16 spends a second MMA on it.
+//             e4m3: the stored bytes become f16 exactly and meet q in f16, scaled per head by a power of two so that its
+//             largest element is in [1, 2) (only elements below 2^-14 of it lose bits); P is f16 there (2^-11). The order
+//             of the k dimension and of V's columns is free, so a lane reads its bytes 16 at a time. (The e4m3 form of
+//             mma.sync converts both operands anew at every use on this GPU: 40% more instructions, same time.)
+//             Larger groups are cut into units of 16 heads.
 //   join      At the end of a run's part of a (sequence, head) the CTA's warps merge through shared memory. A part that
 //             is not the whole goes to the workspace, and the last CTA to arrive merges all parts in list order (the
 //             same bits whichever CTA it is) and resets the counter. Nothing ever waits on another CTA.
@@ -27,7 +32,8 @@
 namespace pb2 {
 namespace {
 
-constexpr int kTile = 16;                   // positions per tile: the k extent of one P V MMA
+constexpr int kUnitCost = 10;               // what a unit costs beyond its tiles, in tiles: its queries, merge and output
+constexpr int kJoin = 8;                    // parts of a unit that are joined at a time
 constexpr int kAttnMaxGrid = 4 * 160;       // the workspace holds two parts per CTA of the largest grid
 
 struct AttnParams {
@@ -48,54 +54,69 @@ struct AttnParams {
     int batch, kv_heads, group, chunks;     // chunks: units of at most ROWS heads per kv head
     int num_pages, page_size, max_pages, window;
     int page_shift;                         // log2 of page_size, or -1
+    int whole_blocks;                       // page_size % 16 == 0: 16 positions in a row lie in one page
     float scale_log2;
 };
 
+// A tile is 16 or 32 positions, so that its K and V rows are 8 KB where they can be (e4m3 needs 32 for its MMA).
 template <int HD, int FMT>
 struct AttnTile {
     static constexpr int kEs = FMT == 0 ? 2 : 1;
+    static constexpr int kPos = FMT == 0 && HD >= 96 ? 16 : 32;
     static constexpr int kChunks = HD * kEs / 16;                                // 16-byte chunks per row
     static constexpr int kRow = kChunks <= 4 ? 64 : kChunks <= 8 ? 128 : kChunks <= 16 ? 256 : 512;
-    static constexpr int kMat = kTile * kRow;
+    static constexpr int kMat = kPos * kRow;
     static constexpr int kStage = 2 * kMat;                                      // K rows, then V rows
     static __device__ __forceinline__ uint32_t at(int row, int chunk) {
-        return kRow == 64 ? row * 64 + ((chunk ^ ((row >> 1) & 3)) << 4) : row * kRow + ((chunk ^ (row & 7)) << 4);
+        return row * kRow + ((chunk << 4) ^ key(row));
     }
+    static __device__ __forceinline__ uint32_t key(int row) { return (kRow == 64 ? (row >> 1) & 3 : row & 7) << 4; }
 };
 
-// A place in the list of tiles: tile `tile` of `ntile` of unit u (kv head, chunk of heads) of sequence b.
+// A tile of POS positions in the list: tile `tile` of `ntile` of unit u (kv head, chunk of heads) of sequence b. On the
+// scale by which the list is divided a unit has ntile + kUnitCost places, the sequence's first one is w0.
+template <int POS>
 struct Cursor {
     int b, u, tile, ntile, first, start, len;
+    unsigned w0;
     __device__ __forceinline__ void load(const AttnParams& p) {
-        int n = __ldg(p.lens + b);
-        const long long cap = (long long)p.max_pages * p.page_size;
-        n = n < 0 ? 0 : n;
-        len = n > cap ? (int)cap : n;
+        const int n = __ldg(p.lens + b);
+        len = min(max(n, 0), p.max_pages * p.page_size);
         start = p.window > 0 && len > p.window ? len - p.window : 0;
-        first = start / kTile;
-        ntile = max(1, (len + kTile - 1) / kTile - first);
+        first = start / POS;
+        ntile = max(1, (len + POS - 1) / POS - first);
     }
+    // n tiles on
     __device__ __forceinline__ void advance(const AttnParams& p, int units, int n) {
         tile += n;
-        while (tile >= ntile) {
-            tile -= ntile;
-            if (++u == units) {
-                u = 0;
-                if (++b >= p.batch) { b = p.batch - 1; tile = 0; ntile = 0x7fffffff; return; }
-                load(p);
+        if (tile < ntile) return;
+        unsigned off = (unsigned)u * ntile + tile;
+        while (off >= (unsigned)ntile * units) {
+            if (b + 1 >= p.batch) {                                              // stays there: tile == ntile
+                u = units;
+                tile = ntile;
+                return;
             }
+            off -= (unsigned)ntile * units;
+            w0 += (unsigned)(ntile + kUnitCost) * units;
+            ++b;
+            load(p);
         }
+        u = (int)(off / (unsigned)ntile);
+        tile = (int)(off - (unsigned)u * ntile);
     }
+    __device__ __forceinline__ unsigned unit_place() const { return w0 + (unsigned)u * (ntile + kUnitCost); }
 };
 
-__device__ __forceinline__ int unit_tiles(const AttnParams& p, int b) {
-    Cursor c;
+template <int POS>
+__device__ __forceinline__ int unit_places(const AttnParams& p, int b) {
+    Cursor<POS> c;
     c.b = b;
     c.load(p);
-    return c.ntile;
+    return c.ntile + kUnitCost;
 }
 
-template <int HD, int FMT, int ROWS, int W, int S>
+template <int HD, int FMT, int W, int S>
 struct AttnSmem {
     using T = AttnTile<HD, FMT>;
     static constexpr int kStride = HD + 4;                                       // floats per merged row
@@ -103,167 +124,417 @@ struct AttnSmem {
     static size_t bytes(int rows) { return kRing + (size_t)W * rows * (kStride + 2) * 4; }
 };
 
+// e4m3 fragments. K: word w (of HD / 16) of lane t of a row is at byte k_byte(w, t), read VK words at a time; its four
+// dimensions are the lane's k of step w. V: column g of tile j is dimension v_unit(j / UV, g) + j % UV, read UV bytes at a
+// time.
+template <int HD>
+struct Frag8 {
+    static constexpr int VK = HD % 64 == 0 ? 4 : 2;
+    static constexpr int UV = HD % 128 == 0 ? 16 : HD % 64 == 0 ? 8 : 4;
+    static __device__ __forceinline__ int k_byte(int w, int t) {
+        const int u = w / VK;                                                    // chunk 2 t + u, past 8 chunks + 8
+        return (VK == 2 ? 8 * (t + 4 * u) : HD == 64 ? 16 * t : 128 * (u >> 1) + 16 * (2 * t + (u & 1))) + 4 * (w % VK);
+    }
+    static __device__ __forceinline__ int v_unit(int u, int g) { return (g + 8 * u) * UV; }
+};
+template <int N>                                                                 // N words at byte `b` of a row
+__device__ __forceinline__ void lds_words(uint32_t row, uint32_t key, int b, uint32_t* w) {
+    const uint32_t a = row + ((uint32_t)b ^ key);                                // key: the row's swizzle of 16-byte chunks
+    if (N == 4)
+        asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
+    else if (N == 2)
+        asm volatile("ld.shared.v2.b32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(a) : "memory");
+    else
+        asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
+}
+
 template <int HD, int FMT, int ROWS, int W, int S, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnParams p) {
     using T = AttnTile<HD, FMT>;
-    using SM = AttnSmem<HD, FMT, ROWS, W, S>;
+    using SM = AttnSmem<HD, FMT, W, S>;
+    constexpr int POS = T::kPos, NB = POS / 16;                                  // blocks of 16 positions
     constexpr int KS = HD / 16;                                                  // k steps of Q K^T
     constexpr int NT = HD / 8;                                                   // column tiles of P V
+    constexpr int QR = ROWS == 8 ? 2 : 4;
+    using F8 = Frag8<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
-    __shared__ int scan[W], sh_b, sh_last;
-    __shared__ long long sh_pre;
+    __shared__ int sh_last;
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int units = p.kv_heads * p.chunks;
     const int rows = min(p.group, ROWS);
     float* merge_o = reinterpret_cast<float*>(smem + SM::kRing);                 // [W][rows][kStride]
     float2* merge_ml = reinterpret_cast<float2*>(merge_o + W * rows * SM::kStride);
 
+    pdl_trigger();
     pdl_wait();
-    // ---- this CTA's run [t0, t1) of the list, and the sequence it starts in
-    long long total = 0;
+    // ---- this CTA's run [t0, t1) of the list, and the place it starts at. Every warp finds it for itself, so that none
+    // waits for another: lane i counts the i-th 32nd of the sequences, one scan finds the lane that holds t0, a second
+    // one the sequence among that lane's (a third and more beyond 1024 sequences).
+    Cursor<POS> seg;
+    unsigned t0, t1, per;
     {
-        long long mine = 0;
-        for (int b = tid; b < p.batch; b += W * 32) {
-            const int n = __ldg(p.lens + b);
-            if (blockIdx.x == 0 && (n < 0 || n > (long long)p.max_pages * p.page_size)) serve_error(kErrLength);
-            mine += unit_tiles(p, b);
-        }
-        __shared__ long long sums[W];
-        for (int o = 16; o; o >>= 1) mine += __shfl_xor_sync(~0u, mine, o);
-        if (lane == 0) sums[warp] = mine;
-        __syncthreads();
-        for (int w = 0; w < W; ++w) total += sums[w];
-    }
-    total *= units;
-    long long per = (total + gridDim.x - 1) / gridDim.x;
-    if (per < W) per = W;
-    const long long t0 = per * blockIdx.x;
-    if (t0 >= total) return;
-    const int count = (int)(total - t0 < per ? total - t0 : per);
-    long long carry = 0;                                                         // tiles of the sequences before
-    for (int b0 = 0; b0 < p.batch; b0 += W * 32) {
-        const int b = b0 + tid;
-        const int n = b < p.batch ? unit_tiles(p, b) : 0;
-        int inc = n;
+        const int share = (p.batch + 31) / 32, lo = min(lane * share, p.batch), hi = min(lo + share, p.batch);
+        unsigned mine = 0;
+        for (int b = lo; b < hi; ++b) mine += unit_places<POS>(p, b);
+        unsigned inc = mine;
+#pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(~0u, inc, o);
+            const unsigned y = __shfl_up_sync(~0u, inc, o);
             if (lane >= o) inc += y;
         }
-        if (lane == 31) scan[warp] = inc;
-        __syncthreads();
-        int before = 0, block = 0;
-        for (int w = 0; w < W; ++w) {
-            if (w < warp) before += scan[w];
-            block += scan[w];
-        }
-        const long long lo = (carry + before + inc - n) * units, hi = lo + (long long)n * units;
-        if (n && t0 >= lo && t0 < hi) { sh_b = b; sh_pre = lo; }
-        carry += block;
-        __syncthreads();
-        if (t0 < carry * units) break;
-    }
-    Cursor seg;
-    seg.b = sh_b;
-    seg.load(p);
-    {
-        const long long off = t0 - sh_pre;
-        seg.u = (int)(off / seg.ntile);
-        seg.tile = (int)(off % seg.ntile);
-    }
-
-    // ---- the warp's stream of tiles: list places t0 + warp, t0 + warp + W, ...
-    const int my_tiles = count > warp ? (count - warp + W - 1) / W : 0;
-    const uint32_t ring = sptr(smem) + (uint32_t)(warp * S * T::kStage);
-    Cursor is = seg;                                                             // of the next tile to fetch
-    is.advance(p, units, warp);
-    auto fetch = [&](int stage) {
-        const int p0 = (is.first + is.tile) * kTile;
-        const int head = is.u / p.chunks;
-        const uint32_t kd = ring + stage * T::kStage, vd = kd + T::kMat;
-        // lane r (and r + 16) finds row r's place in the pools
-        const int pos = p0 + (lane & 15);
-        bool ok = pos >= is.start && pos < is.len;
-        long long ko = 0, vo = 0;
-        if (ok) {
-            const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-            const int in = pos - pg * p.page_size;
-            const int id = __ldg(p.table + is.b * p.table_batch + pg);
-            if ((unsigned)id >= (unsigned)p.num_pages) {
-                serve_error(kErrPage);
-                ok = false;
-            } else {
-                ko = id * p.k_page + in * p.k_token + head * p.k_head;
-                vo = id * p.v_page + in * p.v_token + head * p.v_head;
+        const unsigned total = __shfl_sync(~0u, inc, 31) * units;
+        per = max((total + gridDim.x - 1) / gridDim.x, (unsigned)W);
+        if ((unsigned long long)per * blockIdx.x >= total) return;
+        t0 = per * blockIdx.x;
+        t1 = t0 + min(total - t0, per);
+        int from = __ffs(__ballot_sync(~0u, t0 < inc * units)) - 1;
+        unsigned before = __shfl_sync(~0u, inc - mine, from);
+        from *= share;
+        if (share > 1) {
+            const int end = min(from + share, p.batch);
+#pragma unroll 1
+            for (;; from += 32) {
+                const int b = from + lane;
+                const unsigned n = b < end ? unit_places<POS>(p, b) : 0;
+                inc = n;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const unsigned y = __shfl_up_sync(~0u, inc, o);
+                    if (lane >= o) inc += y;
+                }
+                const unsigned hit = __ballot_sync(~0u, t0 < (before + inc) * units);
+                if (hit || from + 32 >= end) {
+                    const int at = hit ? __ffs(hit) - 1 : 31;
+                    from += at;
+                    before += __shfl_sync(~0u, inc - n, at);
+                    break;
+                }
+                before += __shfl_sync(~0u, inc, 31);
             }
         }
-        const unsigned live = __ballot_sync(~0u, ok);
+        seg.b = from;
+        seg.w0 = before * units;
+        seg.load(p);
+        const unsigned off = t0 - seg.w0, each = seg.ntile + kUnitCost;
+        seg.u = (int)(off / each);
+        seg.tile = (int)(off - seg.u * each);
+        if (seg.tile >= seg.ntile) {                                             // behind the tiles of its unit
+            seg.tile = seg.ntile - 1;
+            seg.advance(p, units, 1);
+            if (seg.tile || seg.unit_place() >= t1) return;
+        }
+    }
+
+    // ---- the warp's stream of tiles: the run's tiles warp, warp + W, ... Lane i holds what it takes to fetch the i-th of
+    // 32 of them (for 16-position blocks that straddle pages: only where the tile lies).
+    const uint32_t ring = sptr(smem) + (uint32_t)(warp * S * T::kStage);
+    struct Look { int id[NB], in[NB], head, range; };                            // rows range & 255 .. range >> 8
+    Cursor<POS> is = seg;
+    is.advance(p, units, warp + lane * W);
+    Look now{};
+    int fetched = 0, known = 0, fill = 0;                                        // known: tiles looked up; fill: next stage
+    auto look = [&]() {
+        Look w;
+        const bool valid = is.tile < is.ntile && is.unit_place() + is.tile < t1;
+        known = fetched + __popc(__ballot_sync(~0u, valid));
+        if (valid) {
+            const int p0 = (is.first + is.tile) * POS;
+            w.head = p.chunks == 1 ? is.u : is.u / p.chunks;
+            const int lo = max(is.start - p0, 0), hi = min(is.len - p0, POS);    // hi <= 0: an empty sequence
+            w.range = lo | max(hi, 0) << 8;
 #pragma unroll
-        for (int i = 0; i < (kTile * T::kChunks + 31) / 32; ++i) {
-            const int e = lane + 32 * i;
-            const int row = e / T::kChunks, c = e % T::kChunks;
-            const long long a = __shfl_sync(~0u, ko, row & 15), b = __shfl_sync(~0u, vo, row & 15);
-            const int n = (live >> (row & 15) & 1) ? 16 : 0;
-            if (kTile * T::kChunks % 32 == 0 || e < kTile * T::kChunks) {
-                cp16(kd + T::at(row, c), p.k + (n ? a + c * 16 : 0), n);
-                cp16(vd + T::at(row, c), p.v + (n ? b + c * 16 : 0), n);
+            for (int n = 0; n < NB; ++n) {
+                const int pos = p0 + 16 * n;
+                if (p.whole_blocks) {
+                    const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+                    w.in[n] = pos - pg * p.page_size;
+                    w.id[n] = 0;
+                    if (16 * n < hi && 16 * n + 16 > lo) w.id[n] = __ldg(p.table + is.b * p.table_batch + pg);
+                } else {
+                    w.id[n] = is.b;
+                    w.in[n] = pos;
+                }
+            }
+        }
+        return w;
+    };
+    auto fetch = [&]() {
+        const int src = fetched & 31, head = __shfl_sync(~0u, now.head, src), range = __shfl_sync(~0u, now.range, src);
+        const int lo = range & 255, hi = range >> 8;
+        const uint32_t kd = ring + fill * T::kStage, vd = kd + T::kMat;
+        constexpr int kIters = (POS * T::kChunks + 31) / 32;
+        if (p.whole_blocks) {
+            const uint8_t *kb[NB], *vb[NB];
+            bool bad[NB];
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                int id = __shfl_sync(~0u, now.id[n], src);
+                const int in = __shfl_sync(~0u, now.in[n], src);
+                bad[n] = (unsigned)id >= (unsigned)p.num_pages;
+                if (bad[n]) {
+                    serve_error(kErrPage);
+                    id = 0;
+                }
+                kb[n] = p.k + id * p.k_page + in * p.k_token + head * p.k_head;
+                vb[n] = p.v + id * p.v_page + in * p.v_token + head * p.v_head;
+            }
+            if constexpr (32 % T::kChunks == 0) {
+                constexpr int kStep = 32 / T::kChunks;                           // rows per pass of the warp
+                const int row0 = lane / T::kChunks, c = lane % T::kChunks;
+                const long long lane_k = row0 * p.k_token + c * 16, lane_v = row0 * p.v_token + c * 16;
+#pragma unroll
+                for (int i = 0; i < kIters; ++i) {
+                    const int row = row0 + i * kStep, n = i * kStep / 16;
+                    const bool in = row >= lo && row < hi && !bad[n];
+                    const int bytes = in ? 16 : 0;
+                    cp16(kd + T::at(row, c), in ? kb[n] + lane_k + (i * kStep - 16 * n) * p.k_token : p.k, bytes);
+                    cp16(vd + T::at(row, c), in ? vb[n] + lane_v + (i * kStep - 16 * n) * p.v_token : p.v, bytes);
+                }
+            } else {
+#pragma unroll
+                for (int i = 0; i < kIters; ++i) {
+                    const int e = lane + 32 * i, row = e / T::kChunks, c = e % T::kChunks, n = NB == 1 ? 0 : row >> 4;
+                    const bool in = row >= lo && row < hi && !(n ? bad[NB - 1] : bad[0]);
+                    const int r = row & 15, bytes = in ? 16 : 0;
+                    cp16(kd + T::at(row, c), in ? (n ? kb[NB - 1] : kb[0]) + r * p.k_token + c * 16 : p.k, bytes);
+                    cp16(vd + T::at(row, c), in ? (n ? vb[NB - 1] : vb[0]) + r * p.v_token + c * 16 : p.v, bytes);
+                }
+            }
+        } else {
+            // any page size: lane r looks up row r's page here
+            const int b = __shfl_sync(~0u, now.id[0], src), p0 = __shfl_sync(~0u, now.in[0], src), r = lane % POS;
+            bool ok = r >= lo && r < hi;
+            long long ko = 0, vo = 0;
+            if (ok) {
+                const int pos = p0 + r, pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+                const int id = __ldg(p.table + b * p.table_batch + pg), in = pos - pg * p.page_size;
+                ok = (unsigned)id < (unsigned)p.num_pages;
+                if (ok) {
+                    ko = id * p.k_page + in * p.k_token + head * p.k_head;
+                    vo = id * p.v_page + in * p.v_token + head * p.v_head;
+                } else {
+                    serve_error(kErrPage);
+                }
+            }
+            const unsigned live = __ballot_sync(~0u, ok);
+#pragma unroll 2
+            for (int i = 0; i < kIters; ++i) {
+                const int e = lane + 32 * i, row = e / T::kChunks, c = e % T::kChunks;
+                const long long ka = __shfl_sync(~0u, ko, row), va = __shfl_sync(~0u, vo, row);
+                const bool in = live >> row & 1;
+                cp16(kd + T::at(row, c), in ? p.k + ka + c * 16 : p.k, in ? 16 : 0);
+                cp16(vd + T::at(row, c), in ? p.v + va + c * 16 : p.v, in ? 16 : 0);
+            }
+        }
+        ++fetched;
+        fill = fill + 1 == S ? 0 : fill + 1;
+    };
+    if (blockIdx.x == 0)                                                         // report lengths that were cut
+        for (int b = tid; b < p.batch; b += W * 32) {
+            const int n = __ldg(p.lens + b);
+            if (n < 0 || n > p.max_pages * p.page_size) serve_error(kErrLength);
+        }
+
+    // ---- One loop, so that the fetch and the end of a part are in the code once: step `it` fetches the warp's tile `it`
+    // and works on tile it - (S - 1), after ending the parts (of units) that lie before it.
+    // The next unit's queries are loaded a unit ahead: behind a full ring a load takes as long as the ring's copies.
+    uint32_t qa[KS][QR], qn[KS][QR];
+    auto load_q = [&](int b, int u) {
+        const int hd = p.chunks == 1 ? u : u / p.chunks, r0 = (u - hd * p.chunks) * ROWS, n = min(ROWS, p.group - r0);
+        const __nv_bfloat16* qp = p.q + b * p.q_batch + (long long)(hd * p.group + r0) * p.q_head;
+#pragma unroll
+        for (int h = 0; h < ROWS / 8; ++h) {
+            const bool have = g + 8 * h < n;
+            const __nv_bfloat16* src = qp + (have ? g + 8 * h : 0) * p.q_head;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (FMT == 0) {
+                    const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
+                    qn[s][h] = have ? __ldg(w + 8 * s + t) : 0u;
+                    qn[s][QR / 2 + h] = have ? __ldg(w + 8 * s + 4 + t) : 0u;
+                } else {
+                    const uint2 x = have ? __ldg(reinterpret_cast<const uint2*>(src + F8::k_byte(s, t))) : make_uint2(0u, 0u);
+                    qn[s][h] = x.x;
+                    qn[s][QR / 2 + h] = x.y;
+                }
             }
         }
     };
-    int fetched = 0;
-#pragma unroll
-    for (int s = 0; s < S - 1; ++s) {
-        if (fetched < my_tiles) {
-            fetch(s);
-            is.advance(p, units, W);
-            ++fetched;
+    float acc[NT][4], qscale[2], m[2], l[2];
+    int stage = 0, base = 0, part = 0, head = 0, row0 = 0, nrow = 0;             // base: list places of earlier parts
+#pragma unroll 1
+    for (int it = 0;; ++it) {
+        if (!(it & 31) && fetched == it) {
+            if (it) is.advance(p, units, 32 * W);
+            now = look();
+            if (!it) load_q(seg.b, seg.u);                                       // while the page ids come in
         }
+        if (fetched < known) fetch();
         cp_commit();
-    }
-
-    int stage = 0, base = 0;                                                     // base: list places of earlier parts
-    while (base < count) {
-        const int part = min(seg.ntile - seg.tile, count - base);
-        const int head = seg.u / p.chunks, row0 = (seg.u % p.chunks) * ROWS;
-        const int nrow = min(ROWS, p.group - row0);
-        // ---- the query heads of this unit as A fragments
-        uint32_t qa[KS][ROWS == 8 ? 2 : 4];
-        float qscale[2] = {p.scale_log2, p.scale_log2};
-        {
-            const __nv_bfloat16* qp = p.q + seg.b * p.q_batch + (long long)(head * p.group + row0) * p.q_head;
+        if (it < S - 1) continue;
+        const int place = warp + (it - (S - 1)) * W;
+#pragma unroll 1
+        while (place >= base + part) {
+            if (part) {
+                // ---- the warps' sums of this part, merged in warp order
 #pragma unroll
-            for (int h = 0; h < (ROWS == 8 ? 1 : 2); ++h) {
-                const bool have = g + 8 * h < nrow;
-                const uint32_t* src = reinterpret_cast<const uint32_t*>(qp + (g + 8 * h) * p.q_head);
-                if (FMT == 0) {
+                for (int h = 0; h < ROWS / 8; ++h) {
+                    l[h] += __shfl_xor_sync(~0u, l[h], 1);
+                    l[h] += __shfl_xor_sync(~0u, l[h], 2);
+                    const int r = g + 8 * h;
+                    if (r < nrow) {
+                        if (t == 0) merge_ml[warp * rows + r] = make_float2(m[h], l[h]);
+                        float* o = merge_o + (warp * rows + r) * SM::kStride;
+                        if (FMT == 0) {
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        qa[s][h] = have ? __ldg(src + 8 * s + t) : 0u;
-                        qa[s][(ROWS == 8 ? 1 : 2) + h] = have ? __ldg(src + 8 * s + 4 + t) : 0u;
+                            for (int j = 0; j < NT; ++j)
+                                *reinterpret_cast<float2*>(o + 8 * j + 2 * t) =
+                                    ROWS == 8 ? make_float2(acc[j][0] + acc[j][2], acc[j][1] + acc[j][3])
+                                              : make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
+                        } else {
+#pragma unroll
+                            for (int u = 0; u < NT / F8::UV; ++u)
+#pragma unroll
+                                for (int c = 0; c < 2; ++c)
+#pragma unroll
+                                    for (int i = 0; i < F8::UV; i += 4)
+                                        *reinterpret_cast<float4*>(o + F8::v_unit(u, 2 * t + c) + i) =
+                                            make_float4(acc[u * F8::UV + i][2 * h + c], acc[u * F8::UV + i + 1][2 * h + c],
+                                                        acc[u * F8::UV + i + 2][2 * h + c], acc[u * F8::UV + i + 3][2 * h + c]);
+                        }
                     }
-                } else {
-                    // dimensions 16 s + 4 t .. + 3 are the lane's k of step s (K's words are read the same way)
-                    uint32_t lo[KS], hi[KS];
+                }
+                __syncthreads();
+                const bool whole = part == seg.ntile;
+                const unsigned u0 = seg.unit_place();
+                const float vs = FMT == 1 && p.v_scale ? __ldg(p.v_scale + head) : 1.f;
+                auto store = [&](int r, int d, float4 o, float mm, float ll) {
+                    const float inv = ll > 0.f || ll != ll ? vs / ll : 0.f;
+                    const int hq = head * p.group + row0 + r;
+                    *reinterpret_cast<uint2*>(p.out + seg.b * p.out_batch + hq * p.out_head + d) =
+                        make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
+                    if (p.lse && d == 0)
+                        p.lse[seg.b * p.lse_batch + hq] = ll > 0.f || ll != ll ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
+                };
+                const size_t slot = (size_t)(2 * blockIdx.x + (seg.tile == 0 ? 1 : 0)) * rows;
+#pragma unroll 2
+                for (int e = tid; e < nrow * (HD / 4); e += W * 32) {
+                    const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+                    float mm = -INFINITY, ll = 0.f;
+                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                    for (int w = 0; w < W; ++w) mm = fmaxf(mm, merge_ml[w * rows + r].x);
+                    const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+                    for (int w = 0; w < W; ++w) {
+                        const float2 ml = merge_ml[w * rows + r];
+                        const float f = ex2(ml.x - ref);
+                        const float4 a = *reinterpret_cast<const float4*>(merge_o + (w * rows + r) * SM::kStride + d);
+                        ll += f * ml.y;
+                        o.x += f * a.x;
+                        o.y += f * a.y;
+                        o.z += f * a.z;
+                        o.w += f * a.w;
+                    }
+                    if (whole) {
+                        store(r, d, o, mm, ll);
+                    } else {
+                        if (d == 0) p.part_ml[slot + r] = make_float2(mm, ll);
+                        *reinterpret_cast<float4*>(p.part_o + (slot + r) * HD + d) = o;
+                    }
+                }
+                if (!whole) {
+                    const int c0 = (int)(u0 / per), c1 = (int)((u0 + seg.ntile - 1) / per);   // the CTAs that share the unit
+                    __syncthreads();
+                    if (tid == 0) {
+                        // release this CTA's part (the barrier has ordered it before), acquire those of the CTAs before
+                        unsigned before;
+                        asm volatile("atom.acq_rel.gpu.global.add.u32 %0, [%1], 1;" : "=r"(before) : "l"(p.counters + c0) : "memory");
+                        sh_last = before == (unsigned)(c1 - c0);
+                        if (sh_last) p.counters[c0] = 0u;
+                    }
+                    __syncthreads();
+                    if (sh_last) {
+                        // kJoin parts at a time, all loads of a group in flight together
+#pragma unroll 1
+                        for (int e = tid; e < nrow * (HD / 4); e += W * 32) {
+                            const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+                            float mm = -INFINITY, ll = 0.f;
+                            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                            for (int cb = c0; cb <= c1; cb += kJoin) {
+                                float2 ml[kJoin];
+                                float4 a[kJoin];
+#pragma unroll
+                                for (int i = 0; i < kJoin; ++i) {
+                                    const int c = min(cb + i, c1);
+                                    const size_t sl = (size_t)(2 * c + (c == c0 ? 1 : 0)) * rows + r;
+                                    ml[i] = __ldcg(p.part_ml + sl);
+                                    a[i] = __ldcg(reinterpret_cast<const float4*>(p.part_o + sl * HD + d));
+                                }
+                                float top = mm;
+#pragma unroll
+                                for (int i = 0; i < kJoin; ++i) top = fmaxf(top, ml[i].x);
+                                const float ref = top == -INFINITY ? 0.f : top, f0 = ex2(mm - ref);
+                                mm = top;
+                                ll *= f0;
+                                o = make_float4(o.x * f0, o.y * f0, o.z * f0, o.w * f0);
+#pragma unroll
+                                for (int i = 0; i < kJoin; ++i) {
+                                    const float f = cb + i <= c1 ? ex2(ml[i].x - ref) : 0.f;
+                                    ll += f * ml[i].y;
+                                    o.x += f * a[i].x;
+                                    o.y += f * a[i].y;
+                                    o.z += f * a[i].z;
+                                    o.w += f * a[i].w;
+                                }
+                            }
+                            store(r, d, o, mm, ll);
+                        }
+                    }
+                }
+                __syncthreads();
+                base += part;
+                const unsigned next = seg.unit_place() + seg.ntile + kUnitCost;
+                if (next >= t1) {
+                    cp_wait<0>();
+                    return;
+                }
+                seg.advance(p, units, seg.ntile - seg.tile);
+            }
+            part = (int)min((unsigned)seg.ntile, t1 - seg.unit_place()) - seg.tile;
+            head = p.chunks == 1 ? seg.u : seg.u / p.chunks;
+            row0 = (seg.u - head * p.chunks) * ROWS;
+            nrow = min(ROWS, p.group - row0);
+            // the query heads of this unit as A fragments; those of the next one are on their way
+            qscale[0] = qscale[1] = p.scale_log2;
+#pragma unroll
+            for (int s = 0; s < KS; ++s)
+#pragma unroll
+                for (int i = 0; i < QR; ++i) qa[s][i] = qn[s][i];
+            if (seg.unit_place() + seg.ntile + kUnitCost < t1)
+                load_q(seg.u + 1 < units ? seg.b : seg.b + 1, seg.u + 1 < units ? seg.u + 1 : 0);
+            if (FMT == 1) {
+#pragma unroll
+                for (int h = 0; h < ROWS / 8; ++h) {
                     float top = 0.f;
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        const uint2 w = have ? __ldg(reinterpret_cast<const uint2*>(src) + 4 * s + t) : make_uint2(0, 0);
-                        lo[s] = w.x;
-                        hi[s] = w.y;
-                        top = fmaxf(top, fmaxf(fmaxf(fabsf(bf16_lo(w.x)), fabsf(bf16_hi(w.x))),
-                                               fmaxf(fabsf(bf16_lo(w.y)), fabsf(bf16_hi(w.y)))));
-                    }
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int i = h; i < QR; i += QR / 2)
+                            top = fmaxf(top, fmaxf(fabsf(bf16_lo(qa[s][i])), fabsf(bf16_hi(qa[s][i]))));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                    // 2^e <= top < 2^(e + 1) from the exponent bits; 0, denormals, infinities and NaN stay as they are
+                    // 2^e <= top < 2^(e + 1), from the exponent field; 0, infinities and NaN stay as they are
                     const int ex = (int)(__float_as_uint(top) >> 23);
                     const bool norm = ex > 1 && ex < 253;
                     const float down = norm ? __uint_as_float((uint32_t)(254 - ex) << 23) : 1.f;
                     qscale[h] *= norm ? __uint_as_float((uint32_t)ex << 23) : 1.f;
 #pragma unroll
-                    for (int s = 0; s < KS; ++s) {
-                        qa[s][h] = pack_f16(bf16_lo(lo[s]) * down, bf16_hi(lo[s]) * down);
-                        qa[s][(ROWS == 8 ? 1 : 2) + h] = pack_f16(bf16_lo(hi[s]) * down, bf16_hi(hi[s]) * down);
-                    }
+                    for (int s = 0; s < KS; ++s)
+#pragma unroll
+                        for (int i = h; i < QR; i += QR / 2)
+                            qa[s][i] = pack_f16(bf16_lo(qa[s][i]) * down, bf16_hi(qa[s][i]) * down);
                 }
             }
             if (FMT == 1 && p.k_scale) {
@@ -271,243 +542,165 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 qscale[0] *= ks;
                 qscale[1] *= ks;
             }
-        }
-        float acc[NT][4];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-
-        int k0 = (warp - base % W + W) % W;
-        for (; k0 < part; k0 += W) {
-            cp_wait<S - 2>();
-            __syncwarp();
-            {   // refill the stage that the previous tile has freed
-                const int s = stage == 0 ? S - 1 : stage - 1;
-                if (fetched < my_tiles) {
-                    fetch(s);
-                    is.advance(p, units, W);
-                    ++fetched;
-                }
-                cp_commit();
-            }
-            const uint32_t kd = ring + stage * T::kStage, vd = kd + T::kMat;
-            stage = stage + 1 == S ? 0 : stage + 1;
-            // ---- S = Q K^T: two column tiles of 8 positions
-            float s[2][4] = {{0.f, 0.f, 0.f, 0.f}, {0.f, 0.f, 0.f, 0.f}};
+            for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+            m[0] = m[1] = -INFINITY;
+            l[0] = l[1] = 0.f;
+        }
+        cp_wait<S - 1>();
+        __syncwarp();
+        const uint32_t kd = ring + stage * T::kStage, vd = kd + T::kMat;
+        stage = stage + 1 == S ? 0 : stage + 1;
+        // ---- S = Q K^T: column tiles of 8 positions
+        float s[2 * NB][4];
+#pragma unroll
+        for (int n = 0; n < 2 * NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        if constexpr (FMT == 0) {
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
-                const uint32_t a0 = qa[ks][0], a1 = ROWS == 8 ? 0u : qa[ks][1], a2 = qa[ks][ROWS == 8 ? 1 : 2],
-                               a3 = ROWS == 8 ? 0u : qa[ks][ROWS == 8 ? 0 : 3];
-                if (FMT == 0) {
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
                     uint32_t r[4];
-                    ldsm4(kd + T::at((lane & 7) + (lane >> 4) * 8, 2 * ks + ((lane >> 3) & 1)), r);
-                    mma_bf16(s[0], a0, a1, a2, a3, r[0], r[1]);
-                    mma_bf16(s[1], a0, a1, a2, a3, r[2], r[3]);
-                } else {
+                    ldsm4(kd + T::at(16 * n + (lane & 7) + (lane >> 4) * 8, 2 * ks + ((lane >> 3) & 1)), r);
+                    const uint32_t a1 = ROWS == 8 ? 0u : qa[ks][1], a3 = ROWS == 8 ? 0u : qa[ks][QR - 1];
+                    mma_bf16(s[2 * n], qa[ks][0], a1, qa[ks][QR / 2], a3, r[0], r[1]);
+                    mma_bf16(s[2 * n + 1], qa[ks][0], a1, qa[ks][QR / 2], a3, r[2], r[3]);
+                }
+            }
+        } else {
 #pragma unroll
-                    for (int n = 0; n < 2; ++n) {
-                        const uint32_t w = lds32(kd + T::at(8 * n + g, ks) + 4 * t);
-                        mma_f16(s[n], a0, a1, a2, a3, e4m3x2_f16x2(w), e4m3x2_f16x2(w >> 16));
+            for (int u = 0; u < KS / F8::VK; ++u) {
+#pragma unroll
+                for (int n = 0; n < 2 * NB; ++n) {
+                    uint32_t w[F8::VK];
+                    lds_words<F8::VK>(kd + (8 * n + g) * T::kRow, T::key(g), F8::k_byte(u * F8::VK, t), w);
+#pragma unroll
+                    for (int i = 0; i < F8::VK; ++i) {
+                        const int ks = u * F8::VK + i;
+                        const uint32_t a1 = ROWS == 8 ? 0u : qa[ks][1], a3 = ROWS == 8 ? 0u : qa[ks][QR - 1];
+                        uint32_t lo, hi;
+                        e4m3x4_f16x4(w[i], lo, hi);
+                        mma_f16(s[n], qa[ks][0], a1, qa[ks][QR / 2], a3, lo, hi);
                     }
                 }
             }
-            // ---- running softmax; lane has positions 8 n + 2 t, + 1 of rows g and g + 8
-            const int p0 = (seg.first + seg.tile + k0) * kTile + 2 * t;
-            uint32_t pa[4] = {0u, 0u, 0u, 0u}, pl[4] = {0u, 0u, 0u, 0u};
-            float fix[2] = {1.f, 1.f};
-            bool moved = false;
+        }
+        // ---- running softmax; lane has positions 8 n + 2 t, + 1 of rows g and g + 8
+        const int p0 = (seg.first + seg.tile + place - base) * POS;
+        const bool edge = p0 < seg.start || p0 + POS > seg.len;
+        uint32_t pa[NB][4], pl[NB][4];                                       // P as A fragments
+        float fix[2] = {1.f, 1.f};
+        bool moved = false;
 #pragma unroll
-            for (int h = 0; h < (ROWS == 8 ? 1 : 2); ++h) {
-                float x[4];
-                float top = -INFINITY;
+        for (int h = 0; h < ROWS / 8; ++h) {
+            float x[4 * NB];
+            float top = -INFINITY;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const int pos = p0 + (i >> 1) * 8 + (i & 1);
-                    const bool in = pos >= seg.start && pos < seg.len;
-                    x[i] = in ? s[i >> 1][2 * h + (i & 1)] * qscale[h] : -INFINITY;
-                    top = fmaxf(top, x[i]);
-                }
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
-                top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                if (top > m[h]) {
-                    fix[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
-                    m[h] = top;
-                    moved = true;
-                }
-                const float mm = m[h] == -INFINITY ? 0.f : m[h];
+            for (int i = 0; i < 4 * NB; ++i) {
+                x[i] = s[i >> 1][2 * h + (i & 1)] * qscale[h];
+                const int pos = p0 + (i >> 1) * 8 + 2 * t + (i & 1);
+                if (edge && (pos < seg.start || pos >= seg.len)) x[i] = -INFINITY;
+                top = fmaxf(top, x[i]);
+            }
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
+            top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
+            if (top > m[h]) {
+                fix[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
+                m[h] = top;
+                moved = true;
+            }
+            const float mm = m[h] == -INFINITY ? 0.f : m[h];
+            float sum = 0.f;
 #pragma unroll
-                for (int i = 0; i < 4; ++i) x[i] = ex2(x[i] - mm);
-                l[h] = l[h] * fix[h] + ((x[0] + x[1]) + (x[2] + x[3]));
+            for (int i = 0; i < 4 * NB; ++i) {
+                x[i] = ex2(x[i] - mm);
+                sum += x[i];
+            }
+            l[h] = l[h] * fix[h] + sum;
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
+                const float* y = x + 4 * n;
                 if (FMT == 0) {
-                    pa[h] = pack_bf16(x[0], x[1]);
-                    pa[2 + h] = pack_bf16(x[2], x[3]);
-                    const uint32_t r0 = pack_bf16(x[0] - bf16_lo(pa[h]), x[1] - bf16_hi(pa[h]));
-                    const uint32_t r1 = pack_bf16(x[2] - bf16_lo(pa[2 + h]), x[3] - bf16_hi(pa[2 + h]));
+                    const uint32_t h0 = pack_bf16(y[0], y[1]), h1 = pack_bf16(y[2], y[3]);
+                    const uint32_t r0 = pack_bf16(y[0] - bf16_lo(h0), y[1] - bf16_hi(h0));
+                    const uint32_t r1 = pack_bf16(y[2] - bf16_lo(h1), y[3] - bf16_hi(h1));
+                    pa[n][h] = h0;
+                    pa[n][2 + h] = h1;
                     if (ROWS == 8) {
-                        pa[1] = r0;
-                        pa[3] = r1;
+                        pa[n][1] = r0;
+                        pa[n][3] = r1;
                     } else {
-                        pl[h] = r0;
-                        pl[2 + h] = r1;
+                        pl[n][h] = r0;
+                        pl[n][2 + h] = r1;
                     }
                 } else {
-                    pa[h] = pack_f16(x[0], x[1]);
-                    pa[2 + h] = pack_f16(x[2], x[3]);
+                    pa[n][h] = pack_f16(y[0], y[1]);
+                    pa[n][2 + h] = pack_f16(y[2], y[3]);
+                    if (ROWS == 8) pa[n][1] = pa[n][3] = 0u;
                 }
             }
-            if (__any_sync(~0u, moved)) {
-                const float f1 = ROWS == 8 ? fix[0] : fix[1];                    // rows 8-15: the remainders of 0-7
+        }
+        if (__any_sync(~0u, moved)) {
+            const float f1 = ROWS == 8 ? fix[0] : fix[1];                    // rows 8-15: the remainders of 0-7
 #pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    acc[j][0] *= fix[0];
-                    acc[j][1] *= fix[0];
-                    acc[j][2] *= f1;
-                    acc[j][3] *= f1;
-                }
+            for (int j = 0; j < NT; ++j) {
+                acc[j][0] *= fix[0];
+                acc[j][1] *= fix[0];
+                acc[j][2] *= f1;
+                acc[j][3] *= f1;
             }
-            // ---- O += P V
-            if (FMT == 0) {
+        }
+        // ---- O += P V
+        if (FMT == 0) {
+#pragma unroll
+            for (int n = 0; n < NB; ++n) {
 #pragma unroll
                 for (int j = 0; j < NT; j += 2) {
                     uint32_t r[4];
-                    ldsm4t(vd + T::at((lane & 7) + ((lane >> 3) & 1) * 8, j + (lane >> 4)), r);
-                    mma_bf16(acc[j], pa[0], pa[1], pa[2], pa[3], r[0], r[1]);
-                    mma_bf16(acc[j + 1], pa[0], pa[1], pa[2], pa[3], r[2], r[3]);
+                    ldsm4t(vd + T::at(16 * n + (lane & 7) + ((lane >> 3) & 1) * 8, j + (lane >> 4)), r);
+                    mma_bf16(acc[j], pa[n][0], pa[n][1], pa[n][2], pa[n][3], r[0], r[1]);
+                    mma_bf16(acc[j + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], r[2], r[3]);
                     if (ROWS != 8) {
-                        mma_bf16(acc[j], pl[0], pl[1], pl[2], pl[3], r[0], r[1]);
-                        mma_bf16(acc[j + 1], pl[0], pl[1], pl[2], pl[3], r[2], r[3]);
+                        mma_bf16(acc[j], pl[n][0], pl[n][1], pl[n][2], pl[n][3], r[0], r[1]);
+                        mma_bf16(acc[j + 1], pl[n][0], pl[n][1], pl[n][2], pl[n][3], r[2], r[3]);
                     }
                 }
-            } else {
-                // column c of tile 4 j + i is dimension 32 j + 4 c + i: a lane reads 4 bytes of each of its 4 positions
-#pragma unroll
-                for (int j = 0; j < HD / 32; ++j) {
-                    uint32_t w[4];
-#pragma unroll
-                    for (int i = 0; i < 4; ++i)
-                        w[i] = lds32(vd + T::at(2 * t + (i & 1) + 8 * (i >> 1), 2 * j + (g >> 2)) + 4 * (g & 3));
-                    const uint32_t b01 = __byte_perm(w[0], w[1], 0x5140), b23 = __byte_perm(w[0], w[1], 0x7362);
-                    const uint32_t c01 = __byte_perm(w[2], w[3], 0x5140), c23 = __byte_perm(w[2], w[3], 0x7362);
-                    mma_f16(acc[4 * j + 0], pa[0], pa[1], pa[2], pa[3], e4m3x2_f16x2(b01), e4m3x2_f16x2(c01));
-                    mma_f16(acc[4 * j + 1], pa[0], pa[1], pa[2], pa[3], e4m3x2_f16x2(b01 >> 16), e4m3x2_f16x2(c01 >> 16));
-                    mma_f16(acc[4 * j + 2], pa[0], pa[1], pa[2], pa[3], e4m3x2_f16x2(b23), e4m3x2_f16x2(c23));
-                    mma_f16(acc[4 * j + 3], pa[0], pa[1], pa[2], pa[3], e4m3x2_f16x2(b23 >> 16), e4m3x2_f16x2(c23 >> 16));
-                }
             }
-        }
-
-        // ---- the warps' sums of this part, merged in warp order
+        } else {
 #pragma unroll
-        for (int h = 0; h < (ROWS == 8 ? 1 : 2); ++h) {
-            l[h] += __shfl_xor_sync(~0u, l[h], 1);
-            l[h] += __shfl_xor_sync(~0u, l[h], 2);
-            const int r = g + 8 * h;
-            if (r < nrow) {
-                if (t == 0) merge_ml[warp * rows + r] = make_float2(m[h], l[h]);
-                float* o = merge_o + (warp * rows + r) * SM::kStride;
-                if (FMT == 0) {
+            for (int n = 0; n < NB; ++n) {
 #pragma unroll
-                    for (int j = 0; j < NT; ++j)
-                        *reinterpret_cast<float2*>(o + 8 * j + 2 * t) =
-                            ROWS == 8 ? make_float2(acc[j][0] + acc[j][2], acc[j][1] + acc[j][3])
-                                      : make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
-                } else {
+                for (int u = 0; u < NT / F8::UV; ++u) {
+                    uint32_t w[4][F8::UV / 4];                               // of the lane's four positions
 #pragma unroll
-                    for (int j = 0; j < HD / 32; ++j)
-#pragma unroll
-                        for (int c = 0; c < 2; ++c)
-                            *reinterpret_cast<float4*>(o + 32 * j + 8 * t + 4 * c) =
-                                make_float4(acc[4 * j][2 * h + c], acc[4 * j + 1][2 * h + c], acc[4 * j + 2][2 * h + c],
-                                            acc[4 * j + 3][2 * h + c]);
-                }
-            }
-        }
-        __syncthreads();
-        const bool whole = part == seg.ntile;
-        const long long u0 = t0 + base - seg.tile;                               // the unit's first place in the list
-        const int c0 = (int)(u0 / per), c1 = (int)((u0 + seg.ntile - 1) / per);  // the CTAs that share it
-        const float vs = FMT == 1 && p.v_scale ? __ldg(p.v_scale + head) : 1.f;
-        auto store = [&](int r, int d, float4 o, float mm, float ll) {
-            const float inv = ll > 0.f || ll != ll ? vs / ll : 0.f;
-            const int hq = head * p.group + row0 + r;
-            *reinterpret_cast<uint2*>(p.out + seg.b * p.out_batch + hq * p.out_head + d) =
-                make_uint2(pack_bf16(o.x * inv, o.y * inv), pack_bf16(o.z * inv, o.w * inv));
-            if (p.lse && d == 0)
-                p.lse[seg.b * p.lse_batch + hq] = ll > 0.f || ll != ll ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
-        };
-        const size_t slot = (size_t)(2 * blockIdx.x + (seg.tile == 0 ? 1 : 0)) * rows;
-        for (int e = tid; e < nrow * (HD / 4); e += W * 32) {
-            const int r = e / (HD / 4), d = e % (HD / 4) * 4;
-            float mm = -INFINITY, ll = 0.f;
-            float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-            for (int w = 0; w < W; ++w) mm = fmaxf(mm, merge_ml[w * rows + r].x);
-            const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll
-            for (int w = 0; w < W; ++w) {
-                const float2 ml = merge_ml[w * rows + r];
-                const float f = ex2(ml.x - ref);
-                const float4 a = *reinterpret_cast<const float4*>(merge_o + (w * rows + r) * SM::kStride + d);
-                ll += f * ml.y;
-                o.x += f * a.x;
-                o.y += f * a.y;
-                o.z += f * a.z;
-                o.w += f * a.w;
-            }
-            if (whole) {
-                store(r, d, o, mm, ll);
-            } else {
-                if (d == 0) p.part_ml[slot + r] = make_float2(mm, ll);
-                *reinterpret_cast<float4*>(p.part_o + (slot + r) * HD + d) = o;
-            }
-        }
-        if (!whole) {
-            __syncthreads();
-            if (tid == 0) {
-                __threadfence();
-                const unsigned before = atomicAdd(p.counters + c0, 1u);
-                sh_last = before == (unsigned)(c1 - c0);
-                if (sh_last) p.counters[c0] = 0u;
-                __threadfence();
-            }
-            __syncthreads();
-            if (sh_last) {
-                for (int e = tid; e < nrow * (HD / 4); e += W * 32) {
-                    const int r = e / (HD / 4), d = e % (HD / 4) * 4;
-                    float mm = -INFINITY, ll = 0.f;
-                    float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
-                    for (int c = c0; c <= c1; ++c)
-                        mm = fmaxf(mm, __ldcg(p.part_ml + (size_t)(2 * c + (c == c0 ? 1 : 0)) * rows + r).x);
-                    const float ref = mm == -INFINITY ? 0.f : mm;
-#pragma unroll 4
-                    for (int c = c0; c <= c1; ++c) {
-                        const size_t sl = (size_t)(2 * c + (c == c0 ? 1 : 0)) * rows + r;
-                        const float2 ml = __ldcg(p.part_ml + sl);
-                        const float4 a = __ldcg(reinterpret_cast<const float4*>(p.part_o + sl * HD + d));
-                        const float f = ex2(ml.x - ref);
-                        ll += f * ml.y;
-                        o.x += f * a.x;
-                        o.y += f * a.y;
-                        o.z += f * a.z;
-                        o.w += f * a.w;
+                    for (int i = 0; i < 4; ++i) {
+                        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
+                        lds_words<F8::UV / 4>(vd + (16 * n + row) * T::kRow, T::key(row), F8::v_unit(u, g), w[i]);
                     }
-                    store(r, d, o, mm, ll);
+#pragma unroll
+                    for (int q = 0; q < F8::UV / 4; ++q)
+#pragma unroll
+                        for (int i = 0; i < 2; ++i) {                        // bytes 2 i, 2 i + 1 of each word
+                            const int sel = i ? 0x7362 : 0x5140, j = u * F8::UV + 4 * q + 2 * i;
+                            uint32_t a0, a1, b0, b1;
+                            e4m3x4_f16x4(__byte_perm(w[0][q], w[1][q], sel), a0, a1);
+                            e4m3x4_f16x4(__byte_perm(w[2][q], w[3][q], sel), b0, b1);
+                            mma_f16(acc[j], pa[n][0], pa[n][1], pa[n][2], pa[n][3], a0, b0);
+                            mma_f16(acc[j + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], a1, b1);
+                        }
                 }
             }
         }
-        __syncthreads();
-        base += part;
-        seg.advance(p, units, part);
+        __syncwarp();                                                            // the stage may be filled again
     }
-    cp_wait<0>();
 }
 
 template <int HD, int FMT, int ROWS, int W, int S, int MINB>
 int launch_attn(const AttnParams& p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     const auto fn = paged_attn_kernel<HD, FMT, ROWS, W, S, MINB>;
-    const size_t smem = AttnSmem<HD, FMT, ROWS, W, S>::bytes(p.group < ROWS ? p.group : ROWS);
-    const int rc = serve_allow_smem((const void*)fn, AttnSmem<HD, FMT, ROWS, W, S>::bytes(ROWS), done);
+    const size_t smem = AttnSmem<HD, FMT, W, S>::bytes(p.group < ROWS ? p.group : ROWS);
+    const int rc = serve_allow_smem((const void*)fn, AttnSmem<HD, FMT, W, S>::bytes(ROWS), done);
     if (rc) return rc;
     int grid = sm_count() * MINB;
     if (grid > kAttnMaxGrid) grid = kAttnMaxGrid;
@@ -519,11 +712,12 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
 template <int HD>
 int pick_attn(const AttnParams& p, int fmt, cudaStream_t st) {
     constexpr int W = 4, kB = W * AttnTile<HD, 0>::kStage, kQ = W * AttnTile<HD, 1>::kStage;
+    constexpr auto deep = [](int s) { return s > 12 ? 12 : s; };
     if (p.group <= 8)
-        return fmt == 0 ? launch_attn<HD, 0, 8, W, (HD == 256 ? 196608 : 98304) / kB, HD == 256 ? 1 : 2>(p, st)
-                        : launch_attn<HD, 1, 8, W, (HD == 256 ? 196608 : 98304) / kQ, HD == 256 ? 1 : 2>(p, st);
-    return fmt == 0 ? launch_attn<HD, 0, 16, W, (HD == 256 ? 131072 : 196608) / kB, 1>(p, st)
-                    : launch_attn<HD, 1, 16, W, (HD == 256 ? 131072 : 196608) / kQ, 1>(p, st);
+        return fmt == 0 ? launch_attn<HD, 0, 8, W, deep((HD == 256 ? 196608 : 98304) / kB), HD == 256 ? 1 : 2>(p, st)
+                        : launch_attn<HD, 1, 8, W, deep((HD == 256 ? 196608 : 98304) / kQ), HD == 256 ? 1 : 2>(p, st);
+    return fmt == 0 ? launch_attn<HD, 0, 16, W, deep((HD == 256 ? 131072 : 196608) / kB), 1>(p, st)
+                    : launch_attn<HD, 1, 16, W, deep((HD == 256 ? 131072 : 196608) / kQ), 1>(p, st);
 }
 
 bool attn_sizes(int heads, int kv_heads, int head_dim) {
@@ -548,7 +742,7 @@ extern "C" size_t paia_gemv_paged_attn_workspace(int heads, int kv_heads, int he
 
 extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
     if (!a || !attn_sizes(a->heads, a->kv_heads, a->head_dim)) return -2;
-    if (a->batch < 0 || (a->cache != 0 && a->cache != 1) || a->num_pages < 0 || a->page_size < 1 || a->max_pages < 0 ||
+    if (a->batch < 0 || (a->cache != 0 && a->cache != 1) || a->num_pages < 1 || a->page_size < 1 || a->max_pages < 0 ||
         a->window < 0 || !(a->scale > 0.f) || !(a->scale <= 3.0e38f))
         return -2;
     if (a->batch == 0) return 0;
@@ -562,8 +756,10 @@ extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
         a->v_page % unit || a->v_token % unit || a->v_head % unit)
         return -2;
     if (a->cache == 0 && (a->k_scale || a->v_scale)) return -2;
-    // positions and a unit's tiles are counted in 32 bits
-    if ((long long)a->max_pages * a->page_size > 0x7fffff00ll) return -2;
+    // positions and the list's places are counted in 32 bits
+    const long long cap = (long long)a->max_pages * a->page_size;
+    const int group = a->heads / a->kv_heads, chunks = (group + 15) / 16;
+    if (cap > 0x7fffff00ll || (cap / 16 + 2 + kUnitCost) * a->kv_heads * chunks > 0xfff00000ll / a->batch) return -2;
     AttnParams p{};
     p.q = static_cast<const __nv_bfloat16*>(a->q);
     p.k = static_cast<const uint8_t*>(a->k);
@@ -586,12 +782,13 @@ extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
     p.v_page = a->v_page * es; p.v_token = a->v_token * es; p.v_head = a->v_head * es;
     p.batch = a->batch;
     p.kv_heads = a->kv_heads;
-    p.group = a->heads / a->kv_heads;
-    p.chunks = (p.group + 15) / 16;
+    p.group = group;
+    p.chunks = chunks;
     p.num_pages = a->num_pages;
     p.page_size = a->page_size;
     p.max_pages = a->max_pages;
     p.window = a->window;
+    p.whole_blocks = a->page_size % 16 == 0;
     p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? ilog2(a->page_size) : -1;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);

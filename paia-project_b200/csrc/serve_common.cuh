@@ -90,11 +90,10 @@ __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
     asm("cvt.rn.f16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
     return r;
 }
-// Two e4m3 values (the low 16 bits of v) as f16x2, exactly.
-__device__ __forceinline__ uint32_t e4m3x2_f16x2(uint32_t v) {
-    uint32_t r;
-    asm("{\n\t.reg .b16 h;\n\tcvt.u16.u32 h, %1;\n\tcvt.rn.f16x2.e4m3x2 %0, h;\n\t}" : "=r"(r) : "r"(v));
-    return r;
+// Four e4m3 values as f16, exactly: the low two bytes of v, the high two.
+__device__ __forceinline__ void e4m3x4_f16x4(uint32_t v, uint32_t& lo, uint32_t& hi) {
+    asm("{\n\t.reg .b16 a, b;\n\tmov.b32 {a, b}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, a;\n\tcvt.rn.f16x2.e4m3x2 %1, b;\n\t}"
+        : "=r"(lo), "=r"(hi) : "r"(v));
 }
 
 // Lets kernel `fn` use `smem` bytes of dynamic shared memory on the current device (once per kernel and device).

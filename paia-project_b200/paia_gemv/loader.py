@@ -332,14 +332,20 @@ class GemvLib:
                                f"head_dim={head_dim})")
         return n
 
-    def paged_attn(self, args, stream=None):
-        self._check(self._lib.paia_gemv_paged_attn(args, self._st(stream)), "paia_gemv_paged_attn")
+    def paged_attn(self, args, stream):
+        rc = self._lib.paia_gemv_paged_attn(args, stream)
+        if rc:
+            self._check(rc, "paia_gemv_paged_attn")
 
-    def qkv_rope_cache(self, args, stream=None):
-        self._check(self._lib.paia_gemv_qkv_rope_cache(args, self._st(stream)), "paia_gemv_qkv_rope_cache")
+    def qkv_rope_cache(self, args, stream):
+        rc = self._lib.paia_gemv_qkv_rope_cache(args, stream)
+        if rc:
+            self._check(rc, "paia_gemv_qkv_rope_cache")
 
-    def lora(self, args, stream=None):
-        self._check(self._lib.paia_gemv_lora(args, self._st(stream)), "paia_gemv_lora")
+    def lora(self, args, stream):
+        rc = self._lib.paia_gemv_lora(args, stream)
+        if rc:
+            self._check(rc, "paia_gemv_lora")
 
     def device_error(self, clear=True):
         """The device-side error word (0 = none): below 10 from kernels whose bounded waits gave up, 10 to 13 from

@@ -29,8 +29,8 @@ def _bad(name, t, what):
 
 def _rows(name, t, dtype, shape, dev):
     """t: `shape`, contiguous innermost dimension, any other strides."""
-    if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or (t.stride(-1) != 1 and t.shape[-1] != 1):
-        _bad(name, t, f"{dtype} {shape} on the current CUDA device, contiguous in its last dimension")
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or (t.stride()[-1] != 1 and shape[-1] != 1):
+        _bad(name, t, f"{dtype} {tuple(shape)} on the current CUDA device, contiguous in its last dimension")
     return t.data_ptr()
 
 
@@ -38,7 +38,7 @@ def _flat(name, t, dtype, n, dev):
     """Contiguous [n], or None."""
     if t is None:
         return 0
-    if t.dtype is not dtype or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
+    if t.shape != (n,) or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
         _bad(name, t, f"contiguous {dtype} [{n}] on the current CUDA device")
     return t.data_ptr()
 
@@ -51,24 +51,33 @@ def _device(t, name):
 
 
 def _pools(k, v, kv_heads, head_dim, k_scale, v_scale, dev):
-    """(cache code, num_pages, page_size) of a cache's two pools."""
-    shape = k.shape
+    """(cache code, pool shape) of a cache's two pools."""
+    shape, dtype = k.shape, k.dtype
     if len(shape) != 4 or shape[2] != kv_heads or shape[3] != head_dim:
         _bad("k_pages", k, f"[num_pages, page_size, {kv_heads}, {head_dim}]")
-    if k.dtype is not _BF16 and k.dtype is not _E4M3:
+    if dtype is not _BF16 and dtype is not _E4M3:
         _bad("k_pages", k, "bfloat16 or float8_e4m3fn")
-    _rows("k_pages", k, k.dtype, shape, dev)
-    _rows("v_pages", v, k.dtype, shape, dev)
-    if k.dtype is _BF16 and (k_scale is not None or v_scale is not None):
+    if dtype is _BF16 and (k_scale is not None or v_scale is not None):
         raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
-    return (0 if k.dtype is _BF16 else 1), shape[0], shape[1]
+    if k.get_device() != dev or k.stride()[3] != 1:
+        _bad("k_pages", k, "on the current CUDA device, contiguous in its last dimension")
+    if v.shape != shape or v.dtype is not dtype or v.get_device() != dev or v.stride()[3] != 1:
+        _bad("v_pages", v, f"{dtype} {tuple(shape)} on the current CUDA device, contiguous in its last dimension")
+    return (0 if dtype is _BF16 else 1), shape
+
+
+class AttentionWorkspace:
+    """The workspace of `paged_attention` for these heads (`attention_workspace` makes it)."""
+
+    def __init__(self, buffer, heads, kv_heads, head_dim):
+        self.buffer, self.ptr, self.sizes = buffer, buffer.data_ptr(), (buffer.get_device(), heads, kv_heads, head_dim)
 
 
 def attention_workspace(lib, heads, kv_heads, head_dim, device=None):
     """The zeroed workspace of `paged_attention` for these heads, for batches and lengths of any size. Calls that may
     overlap on the GPU (other streams, graphs replayed at the same time) need one each."""
-    return torch.zeros(lib.paged_attn_workspace(heads, kv_heads, head_dim), dtype=torch.uint8,
-                       device="cuda" if device is None else device)
+    return AttentionWorkspace(torch.zeros(lib.paged_attn_workspace(heads, kv_heads, head_dim), dtype=torch.uint8,
+                                          device="cuda" if device is None else device), heads, kv_heads, head_dim)
 
 
 def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, *, scale=None, window=0, k_scale=None,
@@ -76,31 +85,32 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
     """out[b] = attention of q[b] (bf16 [batch, heads, head_dim]) over the first lens[b] positions of sequence b (the
     last `window` of them where window > 0). out bf16 like q; lse fp32 [batch, heads], natural logarithm, or None. A
     sequence of length 0 gets zeros and -inf. scale: 1 / sqrt(head_dim) by default."""
-    dev = _device(q, "q")
-    if q.dim() != 3:
+    dev, shape, pool = _device(q, "q"), q.shape, k_pages.shape
+    if len(shape) != 3:
         _bad("q", q, "[batch, heads, head_dim]")
-    batch, heads, hd = shape = q.shape
-    kv = k_pages.shape[2] if k_pages.dim() == 4 else 0
+    batch, heads, hd = shape
+    kv = pool[2] if len(pool) == 4 else 0
     if not kv or heads % kv:
         _bad("k_pages", k_pages, f"[num_pages, page_size, kv_heads, {hd}] with kv_heads dividing {heads}")
-    cache, num_pages, page_size = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
-    if page_table.dim() != 2:
+    cache, pool = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
+    ts = page_table.shape
+    if len(ts) != 2 or ts[0] != batch:
         _bad("page_table", page_table, f"[{batch}, max_pages]")
-    table = _rows("page_table", page_table, _I32, (batch, page_table.shape[1]), dev)
-    if (workspace.get_device() != dev or not workspace.is_contiguous()
-            or workspace.numel() * workspace.element_size() < lib.paged_attn_workspace(heads, kv, hd)):
-        _bad("workspace", workspace, f"attention_workspace(lib, {heads}, {kv}, {hd})")
+    table = _rows("page_table", page_table, _I32, ts, dev)
+    if workspace.sizes != (dev, heads, kv, hd):
+        raise ValueError(f"workspace is for (device, heads, kv_heads, head_dim) = {workspace.sizes}, the call for "
+                         f"{(dev, heads, kv, hd)}")
     ks, vs = k_pages.stride(), v_pages.stride()
     qs, os = q.stride(), out.stride()
     lib.paged_attn(ATTN.pack(
         _rows("q", q, _BF16, shape, dev), k_pages.data_ptr(), v_pages.data_ptr(), table,
         _flat("lens", lens, _I32, batch, dev), _flat("k_scale", k_scale, _F32, kv, dev),
         _flat("v_scale", v_scale, _F32, kv, dev), _rows("out", out, _BF16, shape, dev),
-        0 if lse is None else _rows("lse", lse, _F32, (batch, heads), dev), workspace.data_ptr(),
+        0 if lse is None else _rows("lse", lse, _F32, (batch, heads), dev), workspace.ptr,
         qs[0], qs[1], os[0], os[1], 0 if lse is None else lse.stride(0), page_table.stride(0),
         ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        batch, heads, kv, hd, cache, num_pages, page_size, page_table.shape[1], window,
-        hd ** -0.5 if scale is None else scale), stream)
+        batch, heads, kv, hd, cache, pool[0], pool[1], ts[1], window,
+        hd ** -0.5 if scale is None else scale), torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return out
 
 
@@ -125,7 +135,7 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
     tokens, heads, hd = q_out.shape
     if k_pages is not None:
         kv = k_pages.shape[2] if k_pages.dim() == 4 else 0
-        cache, num_pages, page_size = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
+        cache, (num_pages, page_size, _, _) = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
         ks, vs, kp, vp = k_pages.stride(), v_pages.stride(), k_pages.data_ptr(), v_pages.data_ptr()
         if page_table.dim() != 2 or (seq is None and page_table.shape[0] < tokens):
             _bad("page_table", page_table, "[sequences, max_pages]")
@@ -148,7 +158,7 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
         0 if k_out is None else _rows("k_out", k_out, _BF16, (tokens, kv, hd), dev), kp, vp,
         qkv.stride(0), qs[0], qs[1], kos[0], kos[1], ts, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
         tokens, seqs, heads, kv, hd, 2 * half, 1 if interleaved else 0, cache, num_pages, page_size, max_pages, eps),
-        stream)
+        torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return q_out
 
 
@@ -168,5 +178,5 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
         _flat("ranks", ranks, _I32, n_ad, dev), _flat("scaling", scaling, _F32, n_ad, dev),
         0 if base is None else _rows("base", base, _BF16, (m, n), dev), _rows("out", out, _BF16, (m, n), dev),
         x.stride(0), 0 if base is None else base.stride(0), out.stride(0), sa[0], sa[1], sb[0], sb[1],
-        m, n, k, rank, n_ad), stream)
+        m, n, k, rank, n_ad), torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return out

@@ -65,8 +65,9 @@ def attention(q, k, v, table, lens, scale, window=0, ks=None, vs=None):
             lse[i, hs] = torch.logsumexp(s, -1)
             # one exponent's error moves its own term and the sum it is divided by
             e = ds.amax(-1, keepdim=True) * 2 + 2.0 ** -20 + (len(pos) / 16 + 64) * 2 * F32
-            pe = p * (2.0 ** -11 if eight else 2.0 ** -16) + (2.0 ** -24 * torch.exp(s.amax(-1, keepdim=True)
-                                                              - lse[i, hs][:, None]) if eight else 0.0)
+            pe = p * (2.0 ** -11 if eight else 2.0 ** -16)
+            if eight:
+                pe = pe + 2.0 ** -24 * torch.exp(s.amax(-1, keepdim=True) - lse[i, hs][:, None])
             w = 1.0 if vs is None else float(vs[j])
             out[i, hs] = w * (p @ vv[:, j])
             big = p @ vv[:, j].abs()

@@ -69,7 +69,7 @@ def test_structs_match_the_header(tmp_path):
 
 @pytest.mark.parametrize("change", [
     dict(heads=7), dict(heads=0), dict(kv_heads=0), dict(head_dim=80), dict(head_dim=512), dict(batch=-1), dict(cache=2),
-    dict(cache=-1), dict(page_size=0), dict(max_pages=-1), dict(num_pages=-1), dict(window=-1), dict(scale=0.0),
+    dict(cache=-1), dict(page_size=0), dict(max_pages=-1), dict(num_pages=0), dict(window=-1), dict(scale=0.0),
     dict(scale=-1.0), dict(scale=float("nan")), dict(scale=float("inf")), dict(q=0), dict(k=0), dict(v=0),
     dict(page_table=0), dict(lens=0), dict(out=0), dict(workspace=0), dict(q=PTR + 2), dict(k=PTR + 8), dict(v=PTR + 8),
     dict(workspace=PTR + 4), dict(out=PTR + 4), dict(lse=PTR + 2), dict(lens=PTR + 2), dict(page_table=PTR + 1),
@@ -128,7 +128,8 @@ def test_wrappers_refuse_tensors_off_the_device(L):
     q, pool = torch.zeros(1, 4, 64, dtype=bf), torch.zeros(2, 16, 2, 64, dtype=bf)
     one = torch.zeros(1, dtype=i32)
     with pytest.raises(ValueError, match="current CUDA device"):
-        serve.paged_attention(L, q, pool, pool, one.view(1, 1), one, q, torch.zeros(1 << 20, dtype=torch.uint8))
+        serve.paged_attention(L, q, pool, pool, one.view(1, 1), one, q,
+                              serve.AttentionWorkspace(torch.zeros(1 << 20, dtype=torch.uint8), 4, 2, 64))
     with pytest.raises(ValueError, match="current CUDA device"):
         serve.qkv_rope_cache(L, torch.zeros(1, 8 * 64, dtype=bf), one, torch.ones(32, dtype=torch.float64), q, pool, pool,
                              one.view(1, 1))
@@ -152,10 +153,7 @@ class Recorder:
     def __init__(self):
         self.calls = []
 
-    def paged_attn_workspace(self, heads, kv_heads, head_dim):
-        return 64
-
-    def paged_attn(self, args, stream=None):
+    def paged_attn(self, args, stream):
         self.calls.append(args)
 
     qkv_rope_cache = lora = paged_attn
@@ -165,10 +163,11 @@ def test_wrapper_checks(monkeypatch):
     """Every tensor of a call is checked for its type, shape, layout and device before the library sees it."""
     from paia_gemv import serve
     monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
+    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
     bf, i32, rec = torch.bfloat16, torch.int32, Recorder()
     z = lambda *s, dtype=bf: on(torch.zeros(*s, dtype=dtype))   # noqa: E731
     good = dict(q=z(3, 4, 64), k_pages=z(5, 16, 2, 64), v_pages=z(5, 16, 2, 64), page_table=z(3, 6, dtype=i32),
-                lens=z(3, dtype=i32), out=z(3, 4, 64), workspace=z(64, dtype=torch.uint8))
+                lens=z(3, dtype=i32), out=z(3, 4, 64), workspace=serve.AttentionWorkspace(z(64, dtype=torch.uint8), 4, 2, 64))
     serve.paged_attention(rec, **good)
     hnd = z(5, 2, 16, 64).transpose(1, 2)
     serve.paged_attention(rec, **dict(good, k_pages=hnd, v_pages=hnd), lse=z(3, 4, dtype=torch.float32), window=5)
@@ -186,7 +185,8 @@ def test_wrapper_checks(monkeypatch):
                 dict(page_table=z(2, 6, dtype=i32)), dict(page_table=z(3, 6, dtype=torch.int64)),
                 dict(page_table=z(18, dtype=i32)), dict(lens=z(2, dtype=i32)), dict(lens=z(3, dtype=torch.int64)),
                 dict(lens=z(6, dtype=i32)[::2]), dict(out=z(3, 4, 32)), dict(out=z(3, 4, 64, dtype=f32)),
-                dict(workspace=z(32, dtype=torch.uint8)), dict(k_scale=z(2, dtype=f32)),
+                dict(workspace=serve.AttentionWorkspace(z(64, dtype=torch.uint8), 4, 4, 64)),
+                dict(workspace=serve.AttentionWorkspace(torch.zeros(64, dtype=torch.uint8), 4, 2, 64)), dict(k_scale=z(2, dtype=f32)),
                 dict(lse=z(3, 5, dtype=f32)), dict(lse=z(3, 4)), dict(lens=torch.zeros(3, dtype=i32)),
                 dict(v_pages=torch.zeros(5, 16, 2, 64, dtype=bf))):
         with pytest.raises(ValueError):

@@ -146,7 +146,7 @@ def test_attention_same_bits_and_shared_workspace(L):
         b[0]()
     torch.cuda.synchronize()
     assert torch.equal(a[1], first)
-    counters = ws[:2560].view(torch.int32)
+    counters = ws.buffer[:2560].view(torch.int32)
     assert (counters == 0).all()
 
 
