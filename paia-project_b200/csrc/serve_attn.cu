@@ -32,7 +32,7 @@
 namespace pb2 {
 namespace {
 
-constexpr int kUnitCost = 10;               // what a unit costs beyond its tiles, in tiles: its queries, merge and output
+constexpr int kUnitCost = 14;               // what a unit costs beyond its tiles, in tiles: its queries, merge and output
 constexpr int kJoin = 8;                    // parts of a unit that are joined at a time
 constexpr int kAttnMaxGrid = 4 * 160;       // the workspace holds two parts per CTA of the largest grid
 

@@ -9,8 +9,8 @@
 //             finds its cluster's item by a prefix sum, then lists the item's rows; surplus clusters leave at once.
 //   A x       K is cut over the cluster's CTAs and their warps in blocks of 32; MMA rows are ranks, columns the item's
 //             rows. Each lane loads 16 bytes of an A row and of an x row at a time: a block's k order is permuted alike
-//             for both, which the sum does not see. A CTA's warps meet in shared memory, the CTAs through distributed
-//             shared memory, always in the same order, and each CTA then holds all of t in fp32.
+//             for both, which the sum does not see. A CTA's warps meet in shared memory; each CTA stores its share into
+//             every CTA of the cluster (distributed shared memory), and adds all shares in CTA order.
 //   B t       N is cut over the CTAs in groups of 32 columns. t enters the MMA as two bf16 (t = hi + lo, good to 2^-17):
 //             with up to 8 rows hi and lo are rows 0-7 and 8-15 of one MMA, with more they take two. Column c of the
 //             group's tile j is n = 8 (c / 2) + 2 j + c % 2, so that a lane ends up with 8 neighbouring columns of its
@@ -43,15 +43,16 @@ struct LoraParams {
 };
 
 // Shared memory: the adapters' row counts first, then (over them) a rank group's partial sums of the warps
-// [warp][rank 64][row 16]; t of this CTA's share of K [rank][row] fp32; t as bf16 hi and lo [row 16][rank + 8].
+// [warp][rank 64][row 16]; t of every CTA's share of K [CTA][rank][row] fp32 (8 rows where the call has no more); t as
+// bf16 hi and lo [row 16][rank + 8]. Ranks padded to 32.
 __host__ __device__ constexpr size_t lora_parts(int adapters) {
     const size_t counts = (size_t)(adapters + 1) * 4, parts = (size_t)kLoraWarps * kLoraGroup * kLoraRows * 4;
     return ((counts > parts ? counts : parts) + 15) / 16 * 16;
 }
-__host__ __device__ constexpr int lora_pad(int rank) { return (rank + 15) / 16 * 16; }
-inline size_t lora_smem(int adapters, int rank) {
-    const int r = lora_pad(rank);
-    return lora_parts(adapters) + (size_t)r * kLoraRows * 4 + 2 * (size_t)kLoraRows * (r + 8) * 2;
+__host__ __device__ constexpr int lora_pad(int rank) { return (rank + 31) / 32 * 32; }
+inline size_t lora_smem(int adapters, int rank, int M) {
+    const size_t r = (size_t)lora_pad(rank);
+    return lora_parts(adapters) + kLoraCluster * r * (M <= 8 ? 8 : 16) * 4 + 2 * kLoraRows * (r + 8) * 2;
 }
 
 __device__ __forceinline__ int lora_id(const LoraParams& p, int m) {
@@ -74,77 +75,270 @@ __device__ __forceinline__ uint4 first_of(uint4 v, int n) {
     return make_uint4(w[0], w[1], w[2], w[3]);
 }
 
-__global__ void __launch_bounds__(kLoraThreads) lora_kernel(const LoraParams p) {
+// A warp's sums of x (its rows g, g + 8 at x0, x1) times RT 16-rank tiles of A over its blocks of 32 k: all loads of U
+// blocks are in flight together. NT: 1 for up to 8 rows, 2 for more.
+template <int RT, int NT>
+__device__ __forceinline__ void lora_shrink(float* parts, const __nv_bfloat16* x0, const __nv_bfloat16* x1, bool in0,
+                                            bool in1, const __nv_bfloat16* A, long long a_row, int ranks, int K, int b0,
+                                            int b1, int warp, int g, int t) {
+    constexpr int U = RT == 1 ? 4 : RT == 2 || NT == 1 ? 2 : 1;
+    float acc[RT][NT][4];
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+#pragma unroll 1
+    for (int blk = b0 + warp; blk < b1; blk += U * kLoraWarps) {
+        uint4 xv[U][NT], av[U][RT][2];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int k = (blk + u * kLoraWarps) * 32 + 8 * t;
+            const bool ok = blk + u * kLoraWarps < b1 && k < K;
+            xv[u][0] = ok && in0 ? load16(x0 + k) : zero;
+            if (NT == 2) xv[u][NT - 1] = ok && in1 ? load16(x1 + k) : zero;
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int r = 16 * i + 8 * h + g;
+                    av[u][i][h] = ok && r < ranks ? load16(A + r * a_row + k) : zero;
+                }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int i = 0; i < RT; ++i)
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const uint4 p = av[u][i][0], q = av[u][i][1], x = xv[u][j];
+                    mma_bf16(acc[i][j], p.x, q.x, p.y, q.y, x.x, x.y);
+                    mma_bf16(acc[i][j], p.z, q.z, p.w, q.w, x.z, x.w);
+                }
+    }
+#pragma unroll
+    for (int i = 0; i < RT; ++i)
+#pragma unroll
+        for (int j = 0; j < NT; ++j) {
+            float* o = parts + (warp * kLoraGroup + 16 * i + g) * kLoraRows + 8 * j + 2 * t;
+            *reinterpret_cast<float2*>(o) = make_float2(acc[i][j][0], acc[i][j][1]);
+            *reinterpret_cast<float2*>(o + 8 * kLoraRows) = make_float2(acc[i][j][2], acc[i][j][3]);
+        }
+}
+
+// The warp's groups of 32 columns: out = base + B t, U groups at a time, all their loads in flight together. WS: steps of
+// 32 ranks; ONCE: these are all, and t stays in registers. Rows of B behind the last are read as the last (their results
+// are not stored), ranks behind the last as zeros.
+template <int WS, int NT, bool ONCE>
+__device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bfloat16* B, const __nv_bfloat16* t_hi,
+                                            const __nv_bfloat16* t_lo, int stride, const int* sh_rows, int rows, int rank,
+                                            int g0, int g1, int warp, int g, int t) {
+    constexpr int U = WS == 1 ? (NT == 1 ? 3 : 2) : 1;
+    const uint4 zero = make_uint4(0, 0, 0, 0);
+    const int cols = 8 * (g >> 1) + (g & 1);                                     // the lane's column of tile j: + 2 j
+    const bool base_in = p.base != nullptr, ragged = rank & 7;
+    const __nv_bfloat16* base[NT];
+    __nv_bfloat16* out[NT];
+    bool in[NT];
+#pragma unroll
+    for (int h = 0; h < NT; ++h) {
+        in[h] = g + 8 * h < rows;
+        const long long m = sh_rows[in[h] ? g + 8 * h : 0];
+        base[h] = p.base + m * p.base_row + 8 * t;
+        out[h] = p.out + m * p.out_row + 8 * t;
+    }
+    uint4 th[WS][2 * NT];                                                        // hi (and lo) of rows g, g + 8
+    auto load_t = [&](int k0) {
+#pragma unroll
+        for (int s = 0; s < WS; ++s)
+#pragma unroll
+            for (int h = 0; h < NT; ++h) {
+                const int at = (g + 8 * h) * stride + k0 + 32 * s + 8 * t;
+                th[s][h] = k0 + 32 * s < rank ? load16(t_hi + at) : zero;
+                th[s][NT + h] = k0 + 32 * s < rank ? load16(t_lo + at) : zero;
+            }
+    };
+    if (ONCE && rank) load_t(0);
+#pragma unroll 1
+    for (int grp = g0 + warp; grp < g1; grp += U * kLoraWarps) {
+        uint4 bs[U][NT];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int n0 = (grp + u * kLoraWarps) * 32;
+            const bool ok = base_in && grp + u * kLoraWarps < g1 && n0 + 8 * t < p.N;
+#pragma unroll
+            for (int h = 0; h < NT; ++h) bs[u][h] = ok && in[h] ? load16(base[h] + n0) : zero;
+        }
+        float acc[U][4][4];
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.f;
+#pragma unroll 1
+        for (int k0 = 0; k0 < rank; k0 += 32 * WS) {
+            uint4 w[U][WS][4];
+#pragma unroll
+            for (int u = 0; u < U; ++u)
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int n = min((grp + u * kLoraWarps) * 32 + cols + 2 * j, p.N - 1);
+                    const __nv_bfloat16* row = B + (long long)n * p.b_row + k0 + 8 * t;
+#pragma unroll
+                    for (int s = 0; s < WS; ++s) w[u][s][j] = k0 + 32 * s + 8 * t < rank ? load16(row + 32 * s) : zero;
+                }
+            if (!ONCE) load_t(k0);
+            if (ragged) {
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int s = 0; s < WS; ++s)
+#pragma unroll
+                        for (int j = 0; j < 4; ++j) w[u][s][j] = first_of(w[u][s][j], rank - k0 - 32 * s - 8 * t);
+            }
+#pragma unroll
+            for (int s = 0; s < WS; ++s)
+#pragma unroll
+                for (int u = 0; u < U; ++u)
+#pragma unroll
+                    for (int j = 0; j < 4; ++j) {
+                        const uint4 b = w[u][s][j], h0 = th[s][0], h1 = th[s][1];        // one row set: hi over lo
+                        mma_bf16(acc[u][j], h0.x, h1.x, h0.y, h1.y, b.x, b.y);
+                        mma_bf16(acc[u][j], h0.z, h1.z, h0.w, h1.w, b.z, b.w);
+                        if (NT == 2) {
+                            const uint4 l0 = th[s][2 * NT - 2], l1 = th[s][2 * NT - 1];
+                            mma_bf16(acc[u][j], l0.x, l1.x, l0.y, l1.y, b.x, b.y);
+                            mma_bf16(acc[u][j], l0.z, l1.z, l0.w, l1.w, b.z, b.w);
+                        }
+                    }
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const int n0 = (grp + u * kLoraWarps) * 32;
+            if (grp + u * kLoraWarps >= g1 || n0 + 8 * t >= p.N) continue;
+#pragma unroll
+            for (int h = 0; h < NT; ++h) {
+                if (!in[h]) continue;
+                const uint32_t b[4] = {bs[u][h].x, bs[u][h].y, bs[u][h].z, bs[u][h].w};
+                uint32_t o[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const float* a = acc[u][j];
+                    const float v0 = NT == 2 ? a[2 * h] : a[0] + a[2], v1 = NT == 2 ? a[2 * h + 1] : a[1] + a[3];
+                    o[j] = pack_bf16(v0 + bf16_lo(b[j]), v1 + bf16_hi(b[j]));
+                }
+                *reinterpret_cast<uint4*>(out[h] + n0) = make_uint4(o[0], o[1], o[2], o[3]);
+            }
+        }
+    }
+}
+
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int sh_rows[kLoraRows], sh_warp[kLoraWarps], sh_item[3];
+    __shared__ int sh_rows[kLoraRows], sh_warp[kLoraWarps], sh_item[4];
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int me = (int)cluster.block_rank(), item = (int)(blockIdx.x / kLoraCluster);
     int* counts = reinterpret_cast<int*>(smem);
     float* parts = reinterpret_cast<float*>(smem);
     const int rpad = lora_pad(p.rank);
-    float* t_mine = reinterpret_cast<float*>(smem + lora_parts(p.adapters));     // [rank][row]
-    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_mine + rpad * kLoraRows);
+    const int t_rows = p.M <= 8 ? 8 : 16;
+    float* t_all = reinterpret_cast<float*>(smem + lora_parts(p.adapters));      // [CTA][rank][row]
+    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_all + kLoraCluster * rpad * t_rows);
     __nv_bfloat16* t_lo = t_hi + kLoraRows * (rpad + 8);
 
+    pdl_trigger();
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");                // this CTA runs: others may store here
     pdl_wait();
-    // ---- the item: adapter id and which 16 of its rows
-    for (int i = tid; i <= p.adapters; i += kLoraThreads) counts[i] = 0;
+    // ---- the item: adapter id and up to 16 of its rows
     if (tid == 0) sh_item[0] = -1;
-    __syncthreads();
-    for (int m0 = 0; m0 < p.M; m0 += kLoraThreads) {
-        const int m = m0 + tid;
-        const int a = m < p.M ? lora_id(p, m) : -1;
-        const unsigned same = __match_any_sync(~0u, a);
-        if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(counts + a, __popc(same));
-    }
-    __syncthreads();
-    int before = 0;
-    for (int i0 = 0; i0 <= p.adapters; i0 += kLoraThreads) {
-        const int i = i0 + tid;
-        const int n = i <= p.adapters ? (counts[i] + kLoraRows - 1) / kLoraRows : 0;
-        int inc = n;
-        for (int o = 1; o < 32; o <<= 1) {
-            const int y = __shfl_up_sync(~0u, inc, o);
-            if (lane >= o) inc += y;
-        }
-        if (lane == 31) sh_warp[warp] = inc;
+    if (p.M <= kLoraThreads) {
+        // a row per thread; its place among the rows of its adapter, each 16th of which begins an item
+        int* ids = counts;
+        const int mine = tid < p.M ? lora_id(p, tid) : -1;
+        const int my_rank = mine < 0 || mine == p.adapters ? 0 : p.ranks ? __ldg(p.ranks + mine) : p.rank;
+        ids[tid] = mine;
         __syncthreads();
-        int block = 0, pre = 0;
-        for (int w = 0; w < kLoraWarps; ++w) {
-            if (w < warp) pre += sh_warp[w];
-            block += sh_warp[w];
+        int at = 0, total = 0;
+        for (int m = 0; m < p.M; ++m) {
+            const bool same = ids[m] == mine;
+            total += same;
+            at += same && m < tid;
         }
-        const int lo = before + pre + inc - n;
-        if (n && item >= lo && item < lo + n) {
-            sh_item[0] = i;
-            sh_item[1] = (item - lo) * kLoraRows;
-            sh_item[2] = min(kLoraRows, counts[i] - (item - lo) * kLoraRows);
-        }
-        before += block;
-        __syncthreads();
-        if (item < before) break;
-    }
-    const int id = sh_item[0];
-    if (id < 0) return;                                                          // a whole cluster leaves together
-    const int skip = sh_item[1], rows = sh_item[2];
-    for (int m0 = 0, seen = 0; m0 < p.M && seen < skip + rows; m0 += kLoraThreads) {
-        const int m = m0 + tid;
-        const bool mine = m < p.M && lora_id(p, m) == id;
-        const unsigned ball = __ballot_sync(~0u, mine);
+        const bool begins = mine >= 0 && at % kLoraRows == 0;
+        const unsigned ball = __ballot_sync(~0u, begins);
         if (lane == 0) sh_warp[warp] = __popc(ball);
         __syncthreads();
-        int at = seen, block = 0;
-        for (int w = 0; w < kLoraWarps; ++w) {
-            if (w < warp) at += sh_warp[w];
-            block += sh_warp[w];
+        int number = __popc(ball & ((1u << lane) - 1u));
+        for (int w = 0; w < warp; ++w) number += sh_warp[w];
+        if (begins && number == item) {
+            sh_item[0] = mine;
+            sh_item[1] = at;
+            sh_item[2] = min(kLoraRows, total - at);
+            sh_item[3] = my_rank;
         }
-        at += __popc(ball & ((1u << lane) - 1u));
-        if (mine && at >= skip && at < skip + rows) sh_rows[at - skip] = m;
-        seen += block;
         __syncthreads();
+        if (mine >= 0 && mine == sh_item[0] && at >= sh_item[1] && at < sh_item[1] + kLoraRows) sh_rows[at - sh_item[1]] = tid;
+    } else {
+        for (int i = tid; i <= p.adapters; i += kLoraThreads) counts[i] = 0;
+        __syncthreads();
+        for (int m0 = 0; m0 < p.M; m0 += kLoraThreads) {
+            const int m = m0 + tid;
+            const int a = m < p.M ? lora_id(p, m) : -1;
+            const unsigned same = __match_any_sync(~0u, a);
+            if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(counts + a, __popc(same));
+        }
+        __syncthreads();
+        int before = 0;
+        for (int i0 = 0; i0 <= p.adapters; i0 += kLoraThreads) {
+            const int i = i0 + tid;
+            const int n = i <= p.adapters ? (counts[i] + kLoraRows - 1) / kLoraRows : 0;
+            int inc = n;
+            for (int o = 1; o < 32; o <<= 1) {
+                const int y = __shfl_up_sync(~0u, inc, o);
+                if (lane >= o) inc += y;
+            }
+            if (lane == 31) sh_warp[warp] = inc;
+            __syncthreads();
+            int block = 0, pre = 0;
+            for (int w = 0; w < kLoraWarps; ++w) {
+                if (w < warp) pre += sh_warp[w];
+                block += sh_warp[w];
+            }
+            const int lo = before + pre + inc - n;
+            if (n && item >= lo && item < lo + n) {
+                sh_item[0] = i;
+                sh_item[1] = (item - lo) * kLoraRows;
+                sh_item[2] = min(kLoraRows, counts[i] - (item - lo) * kLoraRows);
+            }
+            before += block;
+            __syncthreads();
+            if (item < before) break;
+        }
+        const int found = sh_item[0], skip = found < 0 ? 0 : sh_item[1], want = found < 0 ? 0 : sh_item[2];
+        if (tid == 0 && found >= 0) sh_item[3] = found == p.adapters ? 0 : p.ranks ? __ldg(p.ranks + found) : p.rank;
+        for (int m0 = 0, seen = 0; m0 < p.M && seen < skip + want; m0 += kLoraThreads) {
+            const int m = m0 + tid;
+            const bool mine = m < p.M && lora_id(p, m) == found;
+            const unsigned ball = __ballot_sync(~0u, mine);
+            if (lane == 0) sh_warp[warp] = __popc(ball);
+            __syncthreads();
+            int at = seen, block = 0;
+            for (int w = 0; w < kLoraWarps; ++w) {
+                if (w < warp) at += sh_warp[w];
+                block += sh_warp[w];
+            }
+            at += __popc(ball & ((1u << lane) - 1u));
+            if (mine && at >= skip && at < skip + want) sh_rows[at - skip] = m;
+            seen += block;
+            __syncthreads();
+        }
     }
-    int rank = id == p.adapters ? 0 : p.ranks ? min(max(__ldg(p.ranks + id), 0), p.rank) : p.rank;
+    __syncthreads();
+    const int id = sh_item[0], rows = sh_item[2], rank = min(max(sh_item[3], 0), p.rank);
+    if (id < 0) {                                                                // a whole cluster leaves together
+        asm volatile("barrier.cluster.wait;" ::: "memory");
+        return;
+    }
     const __nv_bfloat16* A = p.a + (long long)(rank ? id : 0) * p.a_adapter;
     const __nv_bfloat16* B = p.b + (long long)(rank ? id : 0) * p.b_adapter;
     // ---- this CTA's columns, in groups of 32
@@ -161,133 +355,82 @@ __global__ void __launch_bounds__(kLoraThreads) lora_kernel(const LoraParams p) 
     }
     __syncthreads();
     const bool wide = rows > 8;
+    const int stride = rpad + 8;
     if (rank) {
-        // ---- t over this CTA's blocks of K, a group of 64 ranks at a time
+        // ---- t over this CTA's blocks of K, a group of up to 64 ranks at a time
         const int blocks = (p.K + 31) / 32;
         const int b0 = (int)((long long)blocks * me / kLoraCluster), b1 = (int)((long long)blocks * (me + 1) / kLoraCluster);
         const __nv_bfloat16* x0 = p.x + (long long)sh_rows[min(g, rows - 1)] * p.x_row;
         const __nv_bfloat16* x1 = p.x + (long long)sh_rows[min(g + 8, rows - 1)] * p.x_row;
+        const bool in0 = g < rows, in1 = g + 8 < rows;
+        const int quads = wide ? 4 : 2;                                          // float4s of rows per rank
+#pragma unroll 1
         for (int r0 = 0; r0 < rank; r0 += kLoraGroup) {
-            const int tiles = (min(rank - r0, kLoraGroup) + 15) / 16;
-            float acc[kLoraGroup / 16][2][4];
-#pragma unroll
-            for (int i = 0; i < kLoraGroup / 16; ++i)
-#pragma unroll
-                for (int j = 0; j < 2; ++j) acc[i][j][0] = acc[i][j][1] = acc[i][j][2] = acc[i][j][3] = 0.f;
-            for (int blk = b0 + warp; blk < b1; blk += kLoraWarps) {
-                const int k = blk * 32 + 8 * t;
-                const bool ok = k < p.K;
-                const uint4 zero = make_uint4(0, 0, 0, 0);
-                const uint4 xa = ok && g < rows ? load16(x0 + k) : zero;
-                const uint4 xb = wide && ok && g + 8 < rows ? load16(x1 + k) : zero;
-#pragma unroll
-                for (int i = 0; i < kLoraGroup / 16; ++i) {
-                    if (i >= tiles) break;
-                    const int r = r0 + 16 * i + g;
-                    const uint4 u = ok && r < rank ? load16(A + (long long)r * p.a_row + k) : zero;
-                    const uint4 v = ok && r + 8 < rank ? load16(A + (long long)(r + 8) * p.a_row + k) : zero;
-                    mma_bf16(acc[i][0], u.x, v.x, u.y, v.y, xa.x, xa.y);
-                    mma_bf16(acc[i][0], u.z, v.z, u.w, v.w, xa.z, xa.w);
-                    if (wide) {
-                        mma_bf16(acc[i][1], u.x, v.x, u.y, v.y, xb.x, xb.y);
-                        mma_bf16(acc[i][1], u.z, v.z, u.w, v.w, xb.z, xb.w);
-                    }
-                }
+            const int n = min(rank - r0, kLoraGroup);
+            const __nv_bfloat16* Ar = A + r0 * p.a_row;
+            if (n <= 16) {
+                if (wide) lora_shrink<1, 2>(parts, x0, x1, in0, in1, Ar, p.a_row, n, p.K, b0, b1, warp, g, t);
+                else lora_shrink<1, 1>(parts, x0, x1, in0, in1, Ar, p.a_row, n, p.K, b0, b1, warp, g, t);
+            } else if (n <= 32) {
+                if (wide) lora_shrink<2, 2>(parts, x0, x1, in0, in1, Ar, p.a_row, n, p.K, b0, b1, warp, g, t);
+                else lora_shrink<2, 1>(parts, x0, x1, in0, in1, Ar, p.a_row, n, p.K, b0, b1, warp, g, t);
+            } else {
+                if (wide) lora_shrink<4, 2>(parts, x0, x1, in0, in1, Ar, p.a_row, n, p.K, b0, b1, warp, g, t);
+                else lora_shrink<4, 1>(parts, x0, x1, in0, in1, Ar, p.a_row, n, p.K, b0, b1, warp, g, t);
             }
-#pragma unroll
-            for (int i = 0; i < kLoraGroup / 16; ++i) {
-                if (i >= tiles) break;
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    float* o = parts + (warp * kLoraGroup + 16 * i + g) * kLoraRows + 8 * j + 2 * t;
-                    *reinterpret_cast<float2*>(o) = make_float2(acc[i][j][0], acc[i][j][1]);
-                    *reinterpret_cast<float2*>(o + 8 * kLoraRows) = make_float2(acc[i][j][2], acc[i][j][3]);
-                }
-            }
+            if (r0 == 0) asm volatile("barrier.cluster.wait;" ::: "memory");     // every CTA of the cluster runs
             __syncthreads();
-            for (int e = tid; e < tiles * 16 * kLoraRows; e += kLoraThreads) {
-                float s = 0.f;
+            const int have = n <= 16 ? 16 : n <= 32 ? 32 : 64;                   // ranks that the warps have stored
+            for (int e = tid; e < min(have, rpad - r0) * quads; e += kLoraThreads) {
+                const int r = e / quads, row = e % quads * 4, at = r * kLoraRows + row;
+                float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                for (int w = 0; w < kLoraWarps; ++w) s += parts[w * kLoraGroup * kLoraRows + e];
-                t_mine[r0 * kLoraRows + e] = s;
+                for (int w = 0; w < kLoraWarps; ++w) {
+                    const float4 y = *reinterpret_cast<const float4*>(parts + w * kLoraGroup * kLoraRows + at);
+                    v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+                }
+                float* to = t_all + (me * rpad + r0 + r) * t_rows + row;
+#pragma unroll
+                for (int c = 0; c < kLoraCluster; ++c) *reinterpret_cast<float4*>(cluster.map_shared_rank(to, c)) = v;
             }
             __syncthreads();
         }
-        // ---- the cluster's sum, scaled, as bf16 hi + lo
-        cluster.sync();
+        // ---- the cluster's sum in CTA order, scaled, as bf16 hi + lo; ranks behind the last are zeros
         const float scale = p.scaling ? __ldg(p.scaling + id) : 1.f;
-        for (int e = tid; e < lora_pad(rank) * kLoraRows; e += kLoraThreads) {
-            float s = 0.f;
+        asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+        for (int e = tid; e < lora_pad(rank) * quads; e += kLoraThreads) {
+            const int r = e / quads, row = e % quads * 4;
+            float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
+            if (r < rank) {
 #pragma unroll
-            for (int c = 0; c < kLoraCluster; ++c) s += *cluster.map_shared_rank(t_mine + e, c);
-            s *= scale;
-            const int r = e / kLoraRows, row = e % kLoraRows;
-            const __nv_bfloat16 hi = __float2bfloat16_rn(s);
-            t_hi[row * (rpad + 8) + r] = hi;
-            t_lo[row * (rpad + 8) + r] = __float2bfloat16_rn(s - __bfloat162float(hi));
+                for (int c = 0; c < kLoraCluster; ++c) {
+                    const float4 y = *reinterpret_cast<const float4*>(t_all + (c * rpad + r) * t_rows + row);
+                    v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
+                }
+            }
+            const float f[4] = {v.x * scale, v.y * scale, v.z * scale, v.w * scale};
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const __nv_bfloat16 hi = __float2bfloat16_rn(f[i]);
+                t_hi[(row + i) * stride + r] = hi;
+                t_lo[(row + i) * stride + r] = __float2bfloat16_rn(f[i] - __bfloat162float(hi));
+            }
         }
         __syncthreads();
-        asm volatile("barrier.cluster.arrive.release;" ::: "memory");    // done with the others' t
+    } else {
+        asm volatile("barrier.cluster.wait;" ::: "memory");
     }
     // ---- columns
-    const int steps = (rank + 15) / 16;
-    for (int grp = g0 + warp; grp < g1; grp += kLoraWarps) {
-        const int n0 = grp * 32;
-        float acc[4][4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
-        for (int s = 0; s < steps; ++s) {
-            // the lane's k of this step: ranks 16 s + 4 t .. + 3
-            const int k = 16 * s + 4 * t;
-            const uint2 h0 = *reinterpret_cast<const uint2*>(t_hi + g * (rpad + 8) + k);
-            const uint2 l0 = *reinterpret_cast<const uint2*>(t_lo + g * (rpad + 8) + k);
-            uint2 h1 = l0, l1 = l0;
-            if (wide) {
-                h1 = *reinterpret_cast<const uint2*>(t_hi + (g + 8) * (rpad + 8) + k);
-                l1 = *reinterpret_cast<const uint2*>(t_lo + (g + 8) * (rpad + 8) + k);
-            }
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const int n = n0 + 8 * (g >> 1) + 2 * j + (g & 1);
-                uint2 w = make_uint2(0u, 0u);
-                if (n < p.N && k < rank) {
-                    w = *reinterpret_cast<const uint2*>(B + (long long)n * p.b_row + k);
-                    if (k + 4 > rank) {
-                        const uint4 f = first_of(make_uint4(w.x, w.y, 0u, 0u), rank - k);
-                        w = make_uint2(f.x, f.y);
-                    }
-                }
-                mma_bf16(acc[j], h0.x, h1.x, h0.y, h1.y, w.x, w.y);
-                if (wide) mma_bf16(acc[j], l0.x, l1.x, l0.y, l1.y, w.x, w.y);
-            }
-        }
-        const int n = n0 + 8 * t;
-        if (n >= p.N) continue;
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-            const int r = g + 8 * h;
-            if (r >= rows) continue;
-            const long long m = sh_rows[r];
-            float o[8];
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                o[2 * j] = wide ? acc[j][2 * h] : acc[j][0] + acc[j][2];
-                o[2 * j + 1] = wide ? acc[j][2 * h + 1] : acc[j][1] + acc[j][3];
-            }
-            if (p.base) {
-                const uint4 v = load16(p.base + m * p.base_row + n);
-                const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-#pragma unroll
-                for (int j = 0; j < 4; ++j) {
-                    o[2 * j] += bf16_lo(w[j]);
-                    o[2 * j + 1] += bf16_hi(w[j]);
-                }
-            }
-            *reinterpret_cast<uint4*>(p.out + m * p.out_row + n) =
-                make_uint4(pack_bf16(o[0], o[1]), pack_bf16(o[2], o[3]), pack_bf16(o[4], o[5]), pack_bf16(o[6], o[7]));
-        }
+    if (rank <= 32) {
+        if (wide) lora_expand<1, 2, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
+        else lora_expand<1, 1, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
+    } else if (rank <= 64) {
+        if (wide) lora_expand<2, 2, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
+        else lora_expand<2, 1, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
+    } else {
+        if (wide) lora_expand<2, 2, false>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
+        else lora_expand<2, 1, false>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
     }
-    if (rank) asm volatile("barrier.cluster.wait.acquire;" ::: "memory");   // t stays until all have read it
 }
 
 }  // namespace
@@ -325,8 +468,8 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     p.rank = a->rank;
     p.adapters = a->adapters;
     static std::atomic<unsigned long long> done{0};
-    const size_t smem = lora_smem(a->adapters, a->rank);
-    const int rc = serve_allow_smem((const void*)lora_kernel, lora_smem(kLoraMaxAdapters, kLoraMaxRank), done);
+    const size_t smem = lora_smem(a->adapters, a->rank, a->M);
+    const int rc = serve_allow_smem((const void*)lora_kernel, lora_smem(kLoraMaxAdapters, kLoraMaxRank, kLoraMaxRank), done);
     if (rc) return rc;
     // at most one item that is not full per adapter that appears (and one for the rows without)
     const long long kinds = a->M < a->adapters + 1 ? a->M : a->adapters + 1;
