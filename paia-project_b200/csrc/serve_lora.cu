@@ -3,7 +3,7 @@
 //   out[m] = base[m] + scaling[a] B[a] t[m],  t[m] = A[a] x[m],  a = adapter[m]
 //
 // Bound: HBM on the adapters' weights (rank (K + N) elements of each adapter that appears), latency where they are few.
-// One launch, a cluster of 8 CTAs per item; an item is one adapter with up to 16 of its rows (rows without an adapter
+// One launch, a cluster of up to 8 CTAs per item; an item is one adapter with up to 16 of its rows (rows without an adapter
 // form items of rank 0 that copy base):
 //   who       The launch does not know which adapters appear. Every CTA counts the rows per adapter in shared memory and
 //             finds its cluster's item by a prefix sum, then lists the item's rows; surplus clusters leave at once.
@@ -15,8 +15,6 @@
 //             with up to 8 rows hi and lo are rows 0-7 and 8-15 of one MMA, with more they take two. Column c of the
 //             group's tile j is n = 8 (c / 2) + 2 j + c % 2, so that a lane ends up with 8 neighbouring columns of its
 //             row: base is read and out written 16 bytes at a time.
-//   B early   The part of B that a CTA will need is requested into L2 as soon as its adapter is known, so its latency
-//             passes while A x is computed.
 #include <cooperative_groups.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
@@ -26,7 +24,7 @@ namespace {
 
 namespace cg = cooperative_groups;
 
-constexpr int kLoraWarps = 8, kLoraThreads = kLoraWarps * 32, kLoraCluster = 8, kLoraRows = 16, kLoraGroup = 64;
+constexpr int kLoraWarps = 8, kLoraThreads = kLoraWarps * 32, kLoraRows = 16, kLoraGroup = 64;
 constexpr int kLoraMaxRank = 256, kLoraMaxAdapters = 8192;
 
 struct LoraParams {
@@ -40,6 +38,7 @@ struct LoraParams {
     __nv_bfloat16* out;
     long long x_row, base_row, out_row, a_adapter, a_row, b_adapter, b_row;
     int M, N, K, rank, adapters;
+    int cluster;                             // CTAs per item: 8, 4, 2 or 1
 };
 
 // Shared memory: the adapters' row counts first, then (over them) a rank group's partial sums of the warps
@@ -50,9 +49,9 @@ __host__ __device__ constexpr size_t lora_parts(int adapters) {
     return ((counts > parts ? counts : parts) + 15) / 16 * 16;
 }
 __host__ __device__ constexpr int lora_pad(int rank) { return (rank + 31) / 32 * 32; }
-inline size_t lora_smem(int adapters, int rank, int M) {
+inline size_t lora_smem(int adapters, int rank, int M, int cluster) {
     const size_t r = (size_t)lora_pad(rank);
-    return lora_parts(adapters) + kLoraCluster * r * (M <= 8 ? 8 : 16) * 4 + 2 * kLoraRows * (r + 8) * 2;
+    return lora_parts(adapters) + cluster * r * (M <= 8 ? 8 : 16) * 4 + 2 * kLoraRows * (r + 8) * 2;
 }
 
 __device__ __forceinline__ int lora_id(const LoraParams& p, int m) {
@@ -133,7 +132,7 @@ template <int WS, int NT, bool ONCE>
 __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bfloat16* B, const __nv_bfloat16* t_hi,
                                             const __nv_bfloat16* t_lo, int stride, const int* sh_rows, int rows, int rank,
                                             int g0, int g1, int warp, int g, int t) {
-    constexpr int U = WS == 1 ? (NT == 1 ? 3 : 2) : 1;
+    constexpr int U = WS == 1 ? 2 : 1;
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const int cols = 8 * (g >> 1) + (g & 1);                                     // the lane's column of tile j: + 2 j
     const bool base_in = p.base != nullptr, ragged = rank & 7;
@@ -234,35 +233,41 @@ __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bflo
 
 __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams p) {
     extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int sh_rows[kLoraRows], sh_warp[kLoraWarps], sh_item[4];
+    __shared__ int sh_rows[kLoraRows], sh_warp[kLoraWarps], sh_item[4], sh_ranks[kLoraThreads];
     const cg::cluster_group cluster = cg::this_cluster();
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int me = (int)cluster.block_rank(), item = (int)(blockIdx.x / kLoraCluster);
+    const int me = (int)cluster.block_rank(), item = (int)(blockIdx.x / p.cluster);
     int* counts = reinterpret_cast<int*>(smem);
     float* parts = reinterpret_cast<float*>(smem);
     const int rpad = lora_pad(p.rank);
     const int t_rows = p.M <= 8 ? 8 : 16;
     float* t_all = reinterpret_cast<float*>(smem + lora_parts(p.adapters));      // [CTA][rank][row]
-    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_all + kLoraCluster * rpad * t_rows);
+    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_all + p.cluster * rpad * t_rows);
     __nv_bfloat16* t_lo = t_hi + kLoraRows * (rpad + 8);
 
     pdl_trigger();
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");                // this CTA runs: others may store here
     pdl_wait();
     // ---- the item: adapter id and up to 16 of its rows
-    if (tid == 0) sh_item[0] = -1;
+    if (tid == 0) {
+        sh_item[0] = -1;
+        sh_item[2] = 0;
+    }
     if (p.M <= kLoraThreads) {
         // a row per thread; its place among the rows of its adapter, each 16th of which begins an item
         int* ids = counts;
         const int mine = tid < p.M ? lora_id(p, tid) : -1;
-        const int my_rank = mine < 0 || mine == p.adapters ? 0 : p.ranks ? __ldg(p.ranks + mine) : p.rank;
+        // ranks: of all adapters where they are few (one latency less), else of the row's
+        sh_ranks[tid] = p.ranks && tid < p.adapters ? __ldg(p.ranks + tid) : p.rank;
+        int my_rank = 0;
+        if (p.adapters > kLoraThreads && mine >= 0 && mine < p.adapters) my_rank = p.ranks ? __ldg(p.ranks + mine) : p.rank;
         ids[tid] = mine;
         __syncthreads();
-        int at = 0, total = 0;
-        for (int m = 0; m < p.M; ++m) {
-            const bool same = ids[m] == mine;
-            total += same;
-            at += same && m < tid;
+        int at = __popc(__match_any_sync(~0u, mine) & ((1u << lane) - 1u));
+#pragma unroll 4
+        for (int m = 0; m < min(warp * 32, p.M); m += 4) {                       // ids behind M are -1
+            const int4 v = *reinterpret_cast<const int4*>(ids + m);
+            at += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
         }
         const bool begins = mine >= 0 && at % kLoraRows == 0;
         const unsigned ball = __ballot_sync(~0u, begins);
@@ -273,11 +278,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
         if (begins && number == item) {
             sh_item[0] = mine;
             sh_item[1] = at;
-            sh_item[2] = min(kLoraRows, total - at);
-            sh_item[3] = my_rank;
+            sh_item[3] = mine == p.adapters ? 0 : p.adapters > kLoraThreads ? my_rank : sh_ranks[mine];
         }
         __syncthreads();
-        if (mine >= 0 && mine == sh_item[0] && at >= sh_item[1] && at < sh_item[1] + kLoraRows) sh_rows[at - sh_item[1]] = tid;
+        if (mine >= 0 && mine == sh_item[0] && at >= sh_item[1] && at < sh_item[1] + kLoraRows) {
+            sh_rows[at - sh_item[1]] = tid;
+            atomicAdd(sh_item + 2, 1);
+        }
     } else {
         for (int i = tid; i <= p.adapters; i += kLoraThreads) counts[i] = 0;
         __syncthreads();
@@ -343,23 +350,13 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
     const __nv_bfloat16* B = p.b + (long long)(rank ? id : 0) * p.b_adapter;
     // ---- this CTA's columns, in groups of 32
     const int groups = (p.N + 31) / 32;
-    const int g0 = (int)((long long)groups * me / kLoraCluster), g1 = (int)((long long)groups * (me + 1) / kLoraCluster);
-    if (rank) {                                                                  // B rows [32 g0, 32 g1) into L2
-        const int n0 = g0 * 32, n1 = min(g1 * 32, p.N);
-        const int per = p.b_row > 0 && p.b_row < 64 ? 64 / (int)p.b_row : 1;     // rows in 128 bytes
-        const int lines = (rank + 63) / 64;                                      // 128-byte pieces of a row
-        for (int e = tid; e < (n1 - n0 + per - 1) / per * lines; e += kLoraThreads) {
-            const __nv_bfloat16* line = B + (long long)(n0 + e / lines * per) * p.b_row + e % lines * 64;
-            asm volatile("prefetch.global.L2 [%0];" :: "l"(line));
-        }
-    }
-    __syncthreads();
+    const int g0 = (int)((long long)groups * me / p.cluster), g1 = (int)((long long)groups * (me + 1) / p.cluster);
     const bool wide = rows > 8;
     const int stride = rpad + 8;
     if (rank) {
         // ---- t over this CTA's blocks of K, a group of up to 64 ranks at a time
         const int blocks = (p.K + 31) / 32;
-        const int b0 = (int)((long long)blocks * me / kLoraCluster), b1 = (int)((long long)blocks * (me + 1) / kLoraCluster);
+        const int b0 = (int)((long long)blocks * me / p.cluster), b1 = (int)((long long)blocks * (me + 1) / p.cluster);
         const __nv_bfloat16* x0 = p.x + (long long)sh_rows[min(g, rows - 1)] * p.x_row;
         const __nv_bfloat16* x1 = p.x + (long long)sh_rows[min(g + 8, rows - 1)] * p.x_row;
         const bool in0 = g < rows, in1 = g + 8 < rows;
@@ -390,8 +387,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
                     v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
                 }
                 float* to = t_all + (me * rpad + r0 + r) * t_rows + row;
-#pragma unroll
-                for (int c = 0; c < kLoraCluster; ++c) *reinterpret_cast<float4*>(cluster.map_shared_rank(to, c)) = v;
+                for (int c = 0; c < p.cluster; ++c) *reinterpret_cast<float4*>(cluster.map_shared_rank(to, c)) = v;
             }
             __syncthreads();
         }
@@ -402,8 +398,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
             const int r = e / quads, row = e % quads * 4;
             float4 v = make_float4(0.f, 0.f, 0.f, 0.f);
             if (r < rank) {
-#pragma unroll
-                for (int c = 0; c < kLoraCluster; ++c) {
+                for (int c = 0; c < p.cluster; ++c) {
                     const float4 y = *reinterpret_cast<const float4*>(t_all + (c * rpad + r) * t_rows + row);
                     v = make_float4(v.x + y.x, v.y + y.y, v.z + y.z, v.w + y.w);
                 }
@@ -468,13 +463,17 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     p.rank = a->rank;
     p.adapters = a->adapters;
     static std::atomic<unsigned long long> done{0};
-    const size_t smem = lora_smem(a->adapters, a->rank, a->M);
-    const int rc = serve_allow_smem((const void*)lora_kernel, lora_smem(kLoraMaxAdapters, kLoraMaxRank, kLoraMaxRank), done);
-    if (rc) return rc;
     // at most one item that is not full per adapter that appears (and one for the rows without)
     const long long kinds = a->M < a->adapters + 1 ? a->M : a->adapters + 1;
     const long long items = (a->M + (kLoraRows - 1) * kinds) / kLoraRows;
-    if (items * kLoraCluster > 0x7fffffffll) return -2;
-    return serve_launch(lora_kernel, p, dim3((unsigned)(items * kLoraCluster)), kLoraThreads, smem,
-                        static_cast<cudaStream_t>(stream), kLoraCluster);
+    // The more items, the fewer CTAs to each: what an item costs beside its weights (finding it, joining t, the ramps) is
+    // paid once per wave, so all items run in one wave of two CTAs per SM where they can.
+    p.cluster = 8;
+    while (p.cluster > 1 && items * p.cluster > 2ll * sm_count()) p.cluster /= 2;
+    if (items * p.cluster > 0x7fffffffll) return -2;
+    const size_t smem = lora_smem(a->adapters, a->rank, a->M, p.cluster);
+    const int rc = serve_allow_smem((const void*)lora_kernel, lora_smem(kLoraMaxAdapters, kLoraMaxRank, 16, 8), done);
+    if (rc) return rc;
+    return serve_launch(lora_kernel, p, dim3((unsigned)(items * p.cluster)), kLoraThreads, smem,
+                        static_cast<cudaStream_t>(stream), p.cluster);
 }

@@ -5,18 +5,20 @@
 // Bound: HBM for prompts (every element is read once and written once), latency for a decode step's few tokens. A head is
 // held by head_dim / 16 lanes (rounded up to a power of two), 16 elements each: 8 from the first half of the rotated
 // dimensions and the 8 they pair with, so a pair never leaves its lane, the mean square takes a few shuffles, and every
-// access is 16 bytes. The angle's sine and cosine are the same for all heads of a token: the CTA computes them once per
-// token into shared memory while its loads of qkv are in flight. The angle is reduced in fp64 (pos * inv_freq reaches
-// 10^5 radians, where fp32 has 2^-8 left) and its sine and cosine are taken in fp32. Rows of an e4m3 cache are normed and
-// rotated in fp64, so that what is stored is the e4m3 value nearest to the exact one even where an fp32 rounding would
-// cross the border between two of its coarse steps; they are few next to q.
+// access is 16 bytes. The sine and cosine of an angle serve all heads of a token: a CTA takes a few tokens at a time, one
+// angle per thread into shared memory (and each token's place in the cache), then passes over their heads, the loads of a
+// pass in flight while the one before it is worked on. (One token at a time, with the weights read at every head: 8192
+// tokens of 48 heads 58.7 us.) The angle is reduced in fp64 (pos * inv_freq reaches 10^5 radians, where fp32 has 2^-8
+// left) and its sine and cosine are taken in fp32. Rows of an e4m3 cache are normed and rotated in fp64, so that what is
+// stored is the e4m3 value nearest to the exact one even where an fp32 rounding would cross the border between two of its
+// coarse steps; they are few next to q.
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 
 namespace pb2 {
 namespace {
 
-constexpr int kRopeThreads = 256;
+constexpr int kRopeThreads = 256, kRopeBatch = 8, kRopeTable = 512;
 
 struct RopeParams {
     const __nv_bfloat16* qkv;
@@ -37,6 +39,7 @@ struct RopeParams {
     int tokens, sequences, heads, kv_heads, head_dim, rot, interleaved;
     int num_pages, page_size, max_pages;
     int slots, per_cta;                      // heads in all (q, k, v), heads per CTA along y
+    int batch;                               // tokens a CTA takes at a time (at most kRopeBatch)
     int lanes_log2;                          // log2 of the lanes per head
     float eps;
 };
@@ -70,8 +73,18 @@ __device__ __forceinline__ uint2 pack8_e4m3(const double* x) {
     return make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
 }
 
-// The 16 elements of a lane in type F: lo and hi are normed (w: the head's weights, null: no norm) and, where they belong
-// to the rotated dimensions, turned by the table cs (cos, then sin, of each pair). Every lane of the warp calls it.
+// 8 consecutive table entries or weights.
+__device__ __forceinline__ void read8(const float* p, float* x) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
+    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
+}
+__device__ __forceinline__ void read8(const double* p, double* x) {
+#pragma unroll
+    for (int i = 0; i < 8; ++i) x[i] = p[i];
+}
+
+// The 16 elements of a lane in type F. Every lane of the warp calls sum_of_squares.
 template <class F>
 struct Head {
     F lo[8], hi[8];
@@ -79,23 +92,18 @@ struct Head {
         unpack8(wl, lo);
         unpack8(wh, hi);
     }
-    __device__ __forceinline__ void norm(const float* w, int d0, int d1, int lanes, int dim, float eps) {
+    __device__ __forceinline__ F sum_of_squares(int lanes) const {
         F sq = 0;
 #pragma unroll
         for (int i = 0; i < 8; ++i) sq += lo[i] * lo[i] + hi[i] * hi[i];
         for (int o = lanes >> 1; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
-        if (!w) return;
-        const F r = (F)1 / sqrt(sq / (F)dim + (F)eps);
+        return sq;
+    }
+    __device__ __forceinline__ void scale(F r, const float* wl, const float* wh) {
 #pragma unroll
-        for (int i = 0; i < 8; i += 4) {
-            const float4 a = __ldg(reinterpret_cast<const float4*>(w + d0 + i));
-            const float4 b = __ldg(reinterpret_cast<const float4*>(w + d1 + i));
-            const float wa[4] = {a.x, a.y, a.z, a.w}, wb[4] = {b.x, b.y, b.z, b.w};
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                lo[i + j] = lo[i + j] * r * (F)wa[j];
-                hi[i + j] = hi[i + j] * r * (F)wb[j];
-            }
+        for (int i = 0; i < 8; ++i) {
+            lo[i] = lo[i] * r * (F)wl[i];
+            hi[i] = hi[i] * r * (F)wh[i];
         }
     }
     static __device__ __forceinline__ void turn(F& x, F& y, F c, F s) {
@@ -103,15 +111,19 @@ struct Head {
         x = a * c - b * s;
         y = b * c + a * s;
     }
-    __device__ __forceinline__ void rotate(const F* cs, int half, int i0, int interleaved) {
+    // cs: cos of the lane's 8 pairs, `half` on: sin
+    __device__ __forceinline__ void rotate(const F* cs, int half, int interleaved) {
+        F c[8], s[8];
+        read8(cs, c);
+        read8(cs + half, s);
         if (!interleaved) {
 #pragma unroll
-            for (int i = 0; i < 8; ++i) turn(lo[i], hi[i], cs[i0 + i], cs[half + i0 + i]);
+            for (int i = 0; i < 8; ++i) turn(lo[i], hi[i], c[i], s[i]);
         } else {
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
-                turn(lo[2 * i], lo[2 * i + 1], cs[i0 + i], cs[half + i0 + i]);
-                turn(hi[2 * i], hi[2 * i + 1], cs[i0 + 4 + i], cs[half + i0 + 4 + i]);
+                turn(lo[2 * i], lo[2 * i + 1], c[i], s[i]);
+                turn(hi[2 * i], hi[2 * i + 1], c[4 + i], s[4 + i]);
             }
         }
     }
@@ -119,86 +131,135 @@ struct Head {
 
 template <int FMT>
 __global__ void __launch_bounds__(kRopeThreads) qkv_rope_kernel(const RopeParams p) {
-    __shared__ float cs[256];                                // cos, then sin, of the token's rot / 2 angles
-    __shared__ double csd[FMT == 1 ? 256 : 1];
+    __shared__ __align__(16) float cs[kRopeTable];           // per token: cos, then sin, of its rot / 2 angles
+    __shared__ __align__(16) double csd[FMT == 1 ? kRopeTable : 2];
+    __shared__ long long k_at[kRopeBatch], v_at[kRopeBatch]; // a token's row in the pools (bytes; -1: none)
+    __shared__ int live_at[kRopeBatch];                      // whether it is a token at all
     const int tid = threadIdx.x, half = p.rot / 2;
     const int lanes = 1 << p.lanes_log2, lane = tid & (lanes - 1), per_pass = kRopeThreads >> p.lanes_log2;
     const int turning = p.rot / 16;                          // lanes that hold rotated dimensions
-    const int first = blockIdx.y * p.per_cta, last = min(first + p.per_cta, p.slots);
+    const int first = blockIdx.y * p.per_cta, here = min(p.per_cta, p.slots - first);    // this CTA's heads of a token
     const bool in = lane < p.head_dim / 16, rotated = lane < turning;
     // the lane's dimensions: two runs of 8, pair by pair (rotate-half), or 16 in a row
     const int d0 = rotated ? (p.interleaved ? 16 : 8) * lane : in ? p.rot + 16 * (lane - turning) : 0;
     const int d1 = rotated && !p.interleaved ? half + 8 * lane : d0 + 8;
-    const int i0 = 8 * lane;                                 // its first pair
-    const bool any_norm = p.q_norm || p.k_norm;
+    float wq[16];                                            // the q heads' weights of the lane's dimensions
+    pdl_trigger();
     pdl_wait();
-    for (int tok = blockIdx.x; tok < p.tokens; tok += gridDim.x) {
-        const int pos = __ldg(p.pos + tok);
-        if (pos == -1) continue;                                                 // padding
-        if (pos < 0) {
-            if (tid == 0) serve_error(kErrPosition);
-            continue;
-        }
-        __syncthreads();                                                         // the table's last readers are done
-        if (tid < half) {
-            const double turns = (double)pos * __ldg(p.inv_freq + tid) * 0.15915494309189533577;
-            const double r = 2.0 * (turns - rint(turns));                        // in half turns
-            if (FMT == 1) {
-                double s, c;
-                sincospi(r, &s, &c);
-                csd[tid] = c;
-                csd[half + tid] = s;
-                cs[tid] = (float)c;
-                cs[half + tid] = (float)s;
-            } else {
-                sincospif((float)r, &cs[half + tid], &cs[tid]);
+    if (p.q_norm && in) {
+        read8(p.q_norm + d0, wq);
+        read8(p.q_norm + d1, wq + 8);
+    }
+    for (int tok0 = blockIdx.x * p.batch; tok0 < p.tokens; tok0 += gridDim.x * p.batch) {
+        const int n = min(p.batch, p.tokens - tok0);
+        // the first pass's loads, before anything that waits
+        int slot = tid >> p.lanes_log2, tok = 0;             // the head (of this CTA's) and the token (of the batch)
+        auto wrap = [&]() {
+            while (slot >= here) {
+                slot -= here;
+                ++tok;
             }
-        }
-        __syncthreads();
-        for (int s0 = first; s0 < last; s0 += per_pass) {
-            const int slot = s0 + (tid >> p.lanes_log2);
-            const bool live = in && slot < last;
-            const __nv_bfloat16* src = p.qkv + tok * p.qkv_token + (long long)slot * p.head_dim;
-            uint4 wl = make_uint4(0, 0, 0, 0), wh = wl;
-            if (live) {
+        };
+        wrap();
+        uint4 wl = make_uint4(0, 0, 0, 0), wh = wl;
+        auto fetch = [&]() {
+            if (in && tok < n) {
+                const __nv_bfloat16* src = p.qkv + (tok0 + tok) * p.qkv_token + (long long)(first + slot) * p.head_dim;
                 wl = *reinterpret_cast<const uint4*>(src + d0);
                 wh = *reinterpret_cast<const uint4*>(src + d1);
             }
-            const bool is_q = slot < p.heads, is_k = !is_q && slot < p.heads + p.kv_heads;
-            const int kvh = is_q ? 0 : is_k ? slot - p.heads : slot - p.heads - p.kv_heads;
-            const float* w = !live ? nullptr : is_q ? p.q_norm : is_k ? p.k_norm : nullptr;
+        };
+        fetch();
+        __syncthreads();                                     // the table's last readers are done
+        if (tid < n) {
+            const int t = tok0 + tid, pos = __ldg(p.pos + t);
+            long long k = -1, v = -1;
+            if (pos < -1) serve_error(kErrPosition);
+            if (pos >= 0 && p.k) {
+                const int sid = p.seq ? __ldg(p.seq + t) : t, pg = pos / p.page_size, row = pos - pg * p.page_size;
+                if ((unsigned)sid >= (unsigned)p.sequences || pg >= p.max_pages) {
+                    serve_error(kErrPosition);
+                } else {
+                    const int id = __ldg(p.table + sid * p.table_seq + pg);
+                    if ((unsigned)id >= (unsigned)p.num_pages) {
+                        serve_error(kErrPage);
+                    } else {
+                        k = id * p.k_page + row * p.k_row;
+                        v = id * p.v_page + row * p.v_row;
+                    }
+                }
+            }
+            live_at[tid] = pos >= 0;                         // -1: padding
+            k_at[tid] = k;
+            v_at[tid] = v;
+        }
+        for (int e = tid; e < n * half; e += kRopeThreads) {
+            const int t = e / half, i = e - t * half;
+            const double turns = (double)__ldg(p.pos + tok0 + t) * __ldg(p.inv_freq + i) * 0.15915494309189533577;
+            const double r = 2.0 * (turns - rint(turns));    // in half turns
+            float* c = cs + t * 2 * half + i;
+            if (FMT == 1) {
+                double s, co;
+                sincospi(r, &s, &co);
+                csd[t * 2 * half + i] = co;
+                csd[t * 2 * half + half + i] = s;
+                c[0] = (float)co;
+                c[half] = (float)s;
+            } else {
+                float s, co;
+                sincospif((float)r, &s, &co);
+                c[0] = co;
+                c[half] = s;
+            }
+        }
+        __syncthreads();
+        for (int pass = 0; pass < n * here; pass += per_pass) {
+            const int head = first + slot, tk = tok;
+            const bool live = in && tk < n && live_at[min(tk, n - 1)];
+            const bool is_q = head < p.heads, is_k = !is_q && head < p.heads + p.kv_heads;
+            const int kvh = is_q ? 0 : is_k ? head - p.heads : head - p.heads - p.kv_heads;
+            const float* table = cs + min(tk, n - 1) * 2 * half + 8 * lane;
             Head<float> x;
             x.load(wl, wh);
-            if (any_norm) x.norm(w, d0, d1, lanes, p.head_dim, p.eps);
-            if (rotated && (is_q || is_k)) x.rotate(cs, half, i0, p.interleaved);
-            Head<double> y;                                                      // a row of an e4m3 cache
+            Head<double> y;                                  // a row of an e4m3 cache
+            if (FMT == 1) y.load(wl, wh);
+            slot += per_pass;
+            wrap();
+            fetch();                                         // of the next pass
+            if (p.q_norm || p.k_norm) {
+                const float r = rsqrtf(x.sum_of_squares(lanes) * (1.f / (float)p.head_dim) + p.eps);
+                if (is_q && p.q_norm) x.scale(r, wq, wq + 8);
+                if (is_k && p.k_norm && in) {
+                    float w[16];
+                    read8(p.k_norm + d0, w);
+                    read8(p.k_norm + d1, w + 8);
+                    x.scale(r, w, w + 8);
+                }
+            }
+            if (rotated && (is_q || is_k)) x.rotate(table, half, p.interleaved);
             if (FMT == 1) {
-                y.load(wl, wh);
-                if (p.k_norm) y.norm(is_k ? w : nullptr, d0, d1, lanes, p.head_dim, p.eps);
-                if (rotated && is_k) y.rotate(csd, half, i0, p.interleaved);
+                if (p.k_norm) {
+                    const double sq = y.sum_of_squares(lanes);
+                    if (is_k && in) {
+                        float w[16];
+                        read8(p.k_norm + d0, w);
+                        read8(p.k_norm + d1, w + 8);
+                        y.scale(1.0 / sqrt(sq / (double)p.head_dim + (double)p.eps), w, w + 8);
+                    }
+                }
+                if (rotated && is_k) y.rotate(csd + min(tk, n - 1) * 2 * half + 8 * lane, half, p.interleaved);
             }
             if (!live) continue;
+            const long long t = tok0 + tk;
             if (is_q || (is_k && p.k_out)) {
-                __nv_bfloat16* dst = is_q ? p.q_out + tok * p.q_token + slot * p.q_head
-                                          : p.k_out + tok * p.ko_token + kvh * p.ko_head;
+                __nv_bfloat16* dst = is_q ? p.q_out + t * p.q_token + head * p.q_head
+                                          : p.k_out + t * p.ko_token + kvh * p.ko_head;
                 *reinterpret_cast<uint4*>(dst + d0) = pack8(x.lo);
                 *reinterpret_cast<uint4*>(dst + d1) = pack8(x.hi);
             }
-            if (is_q || !p.k) continue;
-            const int sid = p.seq ? __ldg(p.seq + tok) : tok;
-            const int pg = pos / p.page_size;
-            if ((unsigned)sid >= (unsigned)p.sequences || pg >= p.max_pages) {
-                serve_error(kErrPosition);
-                continue;
-            }
-            const int id = __ldg(p.table + sid * p.table_seq + pg);
-            if ((unsigned)id >= (unsigned)p.num_pages) {
-                serve_error(kErrPage);
-                continue;
-            }
-            const int row = pos - pg * p.page_size;
-            uint8_t* dst = is_k ? p.k + id * p.k_page + row * p.k_row + kvh * p.k_head
-                                : p.v + id * p.v_page + row * p.v_row + kvh * p.v_head;
+            const long long at = is_k ? k_at[tk] : v_at[tk];
+            if (is_q || at < 0) continue;
+            uint8_t* dst = is_k ? p.k + at + kvh * p.k_head : p.v + at + kvh * p.v_head;
             if (FMT == 0) {
                 *reinterpret_cast<uint4*>(dst + 2 * d0) = pack8(x.lo);
                 *reinterpret_cast<uint4*>(dst + 2 * d1) = pack8(x.hi);
@@ -279,13 +340,22 @@ extern "C" int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* str
     p.eps = a->eps;
     p.slots = a->heads + 2 * a->kv_heads;
     while ((16 << p.lanes_log2) < a->head_dim) ++p.lanes_log2;
-    // Few tokens: their heads are spread over CTAs, a pass of 256 threads each (each computes the token's table anew).
-    const int per_pass = kRopeThreads >> p.lanes_log2, passes = (p.slots + per_pass - 1) / per_pass;
-    const int sms = sm_count();
-    const int y = a->tokens >= 2 * sms ? 1 : passes;
-    p.per_cta = y == 1 ? p.slots : per_pass;
-    const long long want = 8ll * sms;
-    const dim3 grid((unsigned)(a->tokens < want ? a->tokens : want), (unsigned)y);
+    const int sms = sm_count(), per_pass = kRopeThreads >> p.lanes_log2;
+    dim3 grid;
+    if (a->tokens < 2 * sms) {
+        // few tokens: their heads are spread over CTAs, a pass of 256 threads each (each computes the angles anew)
+        p.batch = 1;
+        p.per_cta = per_pass;
+        grid = dim3((unsigned)a->tokens, (unsigned)((p.slots + per_pass - 1) / per_pass));
+    } else {
+        // as many tokens at a time as the table holds, but work for every SM
+        p.batch = a->rot ? kRopeTable / a->rot : kRopeBatch;
+        if (p.batch > kRopeBatch) p.batch = kRopeBatch;
+        while (p.batch > 1 && a->tokens / p.batch < 4 * sms) p.batch /= 2;
+        p.per_cta = p.slots;
+        const int want = (a->tokens + p.batch - 1) / p.batch;
+        grid = dim3((unsigned)(want < 8 * sms ? want : 8 * sms), 1u);
+    }
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return a->cache == 0 ? serve_launch(qkv_rope_kernel<0>, p, grid, kRopeThreads, 0, st)
                          : serve_launch(qkv_rope_kernel<1>, p, grid, kRopeThreads, 0, st);
