@@ -2,23 +2,25 @@
 //
 //   x' = x / sqrt(mean x^2 + eps) * w;  (a, b) -> (a cos - b sin, b cos + a sin) at angle pos * inv_freq[i]
 //
-// Bound: HBM for prompts (every element is read once and written once), latency for a decode step's few tokens. A head is
-// held by head_dim / 16 lanes (rounded up to a power of two), 16 elements each: 8 from the first half of the rotated
-// dimensions and the 8 they pair with, so a pair never leaves its lane, the mean square takes a few shuffles, and every
-// access is 16 bytes. The sine and cosine of an angle serve all heads of a token: a CTA takes a few tokens at a time, one
-// angle per thread into shared memory (and each token's place in the cache), then passes over their heads, the loads of a
-// pass in flight while the one before it is worked on. (One token at a time, with the weights read at every head: 8192
-// tokens of 48 heads 58.7 us.) The angle is reduced in fp64 (pos * inv_freq reaches 10^5 radians, where fp32 has 2^-8
-// left) and its sine and cosine are taken in fp32. Rows of an e4m3 cache are normed and rotated in fp64, so that what is
-// stored is the e4m3 value nearest to the exact one even where an fp32 rounding would cross the border between two of its
-// coarse steps; they are few next to q.
+// Bound: HBM for prompts (every element is read once and written once; instruction issue is close behind), latency for a
+// decode step's few tokens. A head is held by head_dim / 16 lanes (rounded up to a power of two), 16 elements each: 8 from
+// the first half of the rotated dimensions and the 8 they pair with, so a pair never leaves its lane, the mean square takes
+// a few shuffles, and every access is 16 bytes. A warp takes a token (of few tokens, a part of its heads): its lanes
+// compute the token's angles once, each lane keeps the sine and cosine of its 8 pairs and the norm's weights in registers,
+// and the heads then pass by, the next one's loads in flight. Nothing waits on another warp. (CTAs that shared a table of
+// several tokens' angles in shared memory spent 290 instructions per pass where this takes a third: 45 us for 8192 tokens
+// of 48 heads.)
+// The angle is reduced in fp64 (pos * inv_freq reaches 10^5 radians, where fp32 has 2^-8 left) and its sine and cosine
+// are taken in fp32. What an e4m3 cache stores is the e4m3 value nearest to the exact one: where the fp32 result lies so
+// near to the border between two of its coarse steps that fp32's error could cross it (about one element in 10^4), the
+// warp computes its rows again in fp64.
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 
 namespace pb2 {
 namespace {
 
-constexpr int kRopeThreads = 256, kRopeBatch = 8, kRopeTable = 512;
+constexpr int kRopeThreads = 256, kRopeWarps = kRopeThreads / 32;
 
 struct RopeParams {
     const __nv_bfloat16* qkv;
@@ -38,245 +40,355 @@ struct RopeParams {
     long long k_page, k_row, k_head, v_page, v_row, v_head;                      // bytes
     int tokens, sequences, heads, kv_heads, head_dim, rot, interleaved;
     int num_pages, page_size, max_pages;
-    int slots, per_cta;                      // heads in all (q, k, v), heads per CTA along y
-    int batch;                               // tokens a CTA takes at a time (at most kRopeBatch)
+    int slots;                               // heads in all (q, k, v)
+    int parts, part_passes;                  // parts of a token's passes (of 32 / lanes heads), passes in a part
     int lanes_log2;                          // log2 of the lanes per head
     float eps;
 };
 
-template <class F>
-__device__ __forceinline__ void unpack8(uint4 w, F* x) {
-    const uint32_t v[4] = {w.x, w.y, w.z, w.w};
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        x[2 * i] = bf16_lo(v[i]);
-        x[2 * i + 1] = bf16_hi(v[i]);
-    }
-}
 __device__ __forceinline__ uint4 pack8(const float* x) {
     return make_uint4(pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(x[4], x[5]), pack_bf16(x[6], x[7]));
 }
-// e4m3 of x, rounded once to nearest even and cut at 448 (fp64 goes through fp32 rounded to odd, which keeps on which
-// side of a border the value lies on).
+// Two fp32 values in a register pair, and arithmetic on both at once.
+struct F2 {
+    unsigned long long v;
+    __device__ __forceinline__ F2() {}
+    __device__ __forceinline__ F2(float a, float b) { asm("mov.b64 %0, {%1, %2};" : "=l"(v) : "f"(a), "f"(b)); }
+    __device__ __forceinline__ void get(float& a, float& b) const { asm("mov.b64 {%0, %1}, %2;" : "=f"(a), "=f"(b) : "l"(v)); }
+};
+__device__ __forceinline__ F2 mul2(F2 a, F2 b) {
+    F2 d;
+    asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ F2 sub2(F2 a, F2 b) {
+    F2 d;
+    asm("sub.rn.f32x2 %0, %1, %2;" : "=l"(d.v) : "l"(a.v), "l"(b.v));
+    return d;
+}
+__device__ __forceinline__ F2 fma2(F2 a, F2 b, F2 c) {
+    F2 d;
+    asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(d.v) : "l"(a.v), "l"(b.v), "l"(c.v));
+    return d;
+}
+// x in fp32 rounded to odd, which keeps on which side of a border between e4m3 values it lies.
 __device__ __forceinline__ float to_odd(double x) {
     const float f = __double2float_rz(x);
     return (double)f == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-__device__ __forceinline__ uint2 pack8_e4m3(const double* x) {
+// 8 consecutive table entries or weights as 4 pairs.
+__device__ __forceinline__ void read8(const float* p, F2* x) {
+    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
+    x[0] = F2(a.x, a.y);
+    x[1] = F2(a.z, a.w);
+    x[2] = F2(b.x, b.y);
+    x[3] = F2(b.z, b.w);
+}
+
+// The 16 elements of a lane as pairs of neighbours. Every lane of the warp calls sum_of_squares.
+struct Head {
+    F2 lo[4], hi[4];
+    __device__ __forceinline__ void load(uint4 wl, uint4 wh) {
+        const uint32_t a[4] = {wl.x, wl.y, wl.z, wl.w}, b[4] = {wh.x, wh.y, wh.z, wh.w};
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i] = F2(bf16_lo(a[i]), bf16_hi(a[i]));
+            hi[i] = F2(bf16_lo(b[i]), bf16_hi(b[i]));
+        }
+    }
+    __device__ __forceinline__ float sum_of_squares(int lanes) const {
+        F2 s = mul2(lo[0], lo[0]);
+#pragma unroll
+        for (int i = 1; i < 4; ++i) s = fma2(lo[i], lo[i], s);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) s = fma2(hi[i], hi[i], s);
+        float a, b;
+        s.get(a, b);
+        float sq = a + b;
+        for (int o = lanes >> 1; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
+        return sq;
+    }
+    __device__ __forceinline__ void scale(float r, const F2* wl, const F2* wh) {
+        const F2 r2(r, r);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i] = mul2(mul2(lo[i], r2), wl[i]);
+            hi[i] = mul2(mul2(hi[i], r2), wh[i]);
+        }
+    }
+    // c, s: cos and sin of the lane's 8 pairs of dimensions
+    __device__ __forceinline__ void rotate(const F2* c, const F2* s, int interleaved) {
+        if (!interleaved) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const F2 a = lo[i], b = hi[i];
+                lo[i] = sub2(mul2(a, c[i]), mul2(b, s[i]));
+                hi[i] = fma2(a, s[i], mul2(b, c[i]));
+            }
+        } else {                                             // a register pair is a pair of dimensions
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float c0, c1, s0, s1, a, b;
+                c[i].get(c0, c1);
+                s[i].get(s0, s1);
+                F2& x = i < 2 ? lo[2 * i] : hi[2 * i - 4];
+                F2& y = i < 2 ? lo[2 * i + 1] : hi[2 * i - 3];
+                x.get(a, b);
+                x = F2(a * c0 - b * s0, b * c0 + a * s0);
+                y.get(a, b);
+                y = F2(a * c1 - b * s1, b * c1 + a * s1);
+            }
+        }
+    }
+    __device__ __forceinline__ void get(float* l, float* h) const {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            lo[i].get(l[2 * i], l[2 * i + 1]);
+            hi[i].get(h[2 * i], h[2 * i + 1]);
+        }
+    }
+};
+
+__device__ __forceinline__ uint2 pack8_e4m3(const float* x) {
     uint32_t r[4];
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         uint16_t h;
-        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(to_odd(x[2 * i + 1])), "f"(to_odd(x[2 * i])));
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(h) : "f"(x[2 * i + 1]), "f"(x[2 * i]));
         r[i] = h;
     }
     return make_uint2(r[0] | r[1] << 16, r[2] | r[3] << 16);
 }
 
-// 8 consecutive table entries or weights.
-__device__ __forceinline__ void read8(const float* p, float* x) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = a.x; x[1] = a.y; x[2] = a.z; x[3] = a.w;
-    x[4] = b.x; x[5] = b.y; x[6] = b.z; x[7] = b.w;
-}
-__device__ __forceinline__ void read8(const double* p, double* x) {
+// The elements of `todo` (bit i: lo i, bit 8 + i: hi i) of a lane's row of an e4m3 cache again in fp64 from the stored
+// bf16, into the packed bytes v; whole warps call it, a lane's first pair with a bit set per round.
+__device__ __noinline__ void exact_pairs(const RopeParams& p, uint4 wl, uint4 wh, int pos, bool is_k, bool in, bool rotated,
+                                         int lane, int d0, int d1, float scale, unsigned todo, unsigned long long* v) {
+    float x[16];
+    Head raw;
+    raw.load(wl, wh);
+    raw.get(x, x + 8);
+    double r = 1.0;
+    if (p.k_norm) {
+        double sq = 0.0;
 #pragma unroll
-    for (int i = 0; i < 8; ++i) x[i] = p[i];
+        for (int i = 0; i < 16; ++i) sq += (double)(x[i] * x[i]);                // squares of bf16 are exact in fp32
+        for (int o = (1 << p.lanes_log2) >> 1; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
+        if (is_k) r = 1.0 / sqrt(sq / (double)p.head_dim + (double)p.eps);
+    }
+    const bool turns = is_k && rotated;
+    while (__any_sync(~0u, todo != 0)) {
+        if (todo) {
+            const int e = __ffs(todo) - 1;
+            // the pair: elements ia and ib, angle j of the lane
+            const int j = turns && p.interleaved ? e >> 1 : e & 7;
+            const int ia = turns ? (p.interleaved ? 2 * j : j) : e, ib = turns ? (p.interleaved ? 2 * j + 1 : 8 + j) : e;
+            float fa = 0.f, fb = 0.f;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                fa = i == ia ? x[i] : fa;
+                fb = i == ib ? x[i] : fb;
+            }
+            double a = fa, b = fb;
+            if (is_k && p.k_norm) {
+                a = a * r * (double)__ldg(p.k_norm + (ia < 8 ? d0 + ia : d1 + ia - 8));
+                b = b * r * (double)__ldg(p.k_norm + (ib < 8 ? d0 + ib : d1 + ib - 8));
+            }
+            if (turns) {
+                const double t = (double)pos * __ldg(p.inv_freq + 8 * lane + j) * 0.15915494309189533577;
+                double s, c;
+                sincospi(2.0 * (t - rint(t)), &s, &c);
+                const double a0 = a;
+                a = a0 * c - b * s;
+                b = b * c + a0 * s;
+            }
+            uint16_t h;
+            asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;"
+                : "=h"(h) : "f"(to_odd(b / (double)scale)), "f"(to_odd(a / (double)scale)));
+            const int sa = 8 * (ia & 7), sb = 8 * (ib & 7);
+            v[ia >> 3] = (v[ia >> 3] & ~(0xFFull << sa)) | (unsigned long long)(h & 0xFF) << sa;
+            v[ib >> 3] = (v[ib >> 3] & ~(0xFFull << sb)) | (unsigned long long)(h >> 8) << sb;
+            todo &= ~(1u << ia | 1u << ib);
+        }
+    }
 }
 
-// The 16 elements of a lane in type F. Every lane of the warp calls sum_of_squares.
-template <class F>
-struct Head {
-    F lo[8], hi[8];
-    __device__ __forceinline__ void load(uint4 wl, uint4 wh) {
-        unpack8(wl, lo);
-        unpack8(wh, hi);
-    }
-    __device__ __forceinline__ F sum_of_squares(int lanes) const {
-        F sq = 0;
-#pragma unroll
-        for (int i = 0; i < 8; ++i) sq += lo[i] * lo[i] + hi[i] * hi[i];
-        for (int o = lanes >> 1; o; o >>= 1) sq += __shfl_xor_sync(~0u, sq, o);
-        return sq;
-    }
-    __device__ __forceinline__ void scale(F r, const float* wl, const float* wh) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            lo[i] = lo[i] * r * (F)wl[i];
-            hi[i] = hi[i] * r * (F)wh[i];
-        }
-    }
-    static __device__ __forceinline__ void turn(F& x, F& y, F c, F s) {
-        const F a = x, b = y;
-        x = a * c - b * s;
-        y = b * c + a * s;
-    }
-    // cs: cos of the lane's 8 pairs, `half` on: sin
-    __device__ __forceinline__ void rotate(const F* cs, int half, int interleaved) {
-        F c[8], s[8];
-        read8(cs, c);
-        read8(cs + half, s);
-        if (!interleaved) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) turn(lo[i], hi[i], c[i], s[i]);
-        } else {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                turn(lo[2 * i], lo[2 * i + 1], c[i], s[i]);
-                turn(hi[2 * i], hi[2 * i + 1], c[4 + i], s[4 + i]);
-            }
-        }
-    }
-};
+// Index of element i of the 8 that lane `lane` of `lanes` reads: 16 bytes per lane side by side, twice.
+__device__ __forceinline__ int spread(int lane, int i, int lanes) { return (i >> 2) * 4 * lanes + 4 * lane + (i & 3); }
+__device__ __forceinline__ void read_spread(const float* p, int lane, int lanes, F2* x) {
+    const float4 a = *reinterpret_cast<const float4*>(p + 4 * lane);
+    const float4 b = *reinterpret_cast<const float4*>(p + 4 * (lanes + lane));
+    x[0] = F2(a.x, a.y);
+    x[1] = F2(a.z, a.w);
+    x[2] = F2(b.x, b.y);
+    x[3] = F2(b.z, b.w);
+}
 
 template <int FMT>
-__global__ void __launch_bounds__(kRopeThreads) qkv_rope_kernel(const RopeParams p) {
-    __shared__ __align__(16) float cs[kRopeTable];           // per token: cos, then sin, of its rot / 2 angles
-    __shared__ __align__(16) double csd[FMT == 1 ? kRopeTable : 2];
-    __shared__ long long k_at[kRopeBatch], v_at[kRopeBatch]; // a token's row in the pools (bytes; -1: none)
-    __shared__ int live_at[kRopeBatch];                      // whether it is a token at all
-    const int tid = threadIdx.x, half = p.rot / 2;
-    const int lanes = 1 << p.lanes_log2, lane = tid & (lanes - 1), per_pass = kRopeThreads >> p.lanes_log2;
+__global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kernel(const __grid_constant__ RopeParams p) {
+    __shared__ __align__(16) float tables[kRopeWarps][256];  // a warp's cos, then sin, of rot / 2 angles
+    const int warp = threadIdx.x >> 5, wlane = threadIdx.x & 31, half = p.rot / 2;
+    const int lanes = 1 << p.lanes_log2, lane = wlane & (lanes - 1), sub = wlane >> p.lanes_log2, heads_per = 32 >> p.lanes_log2;
     const int turning = p.rot / 16;                          // lanes that hold rotated dimensions
-    const int first = blockIdx.y * p.per_cta, here = min(p.per_cta, p.slots - first);    // this CTA's heads of a token
-    const bool in = lane < p.head_dim / 16, rotated = lane < turning;
+    const bool in = lane < p.head_dim / 16, rotated = lane < turning, any_norm = p.q_norm || p.k_norm;
     // the lane's dimensions: two runs of 8, pair by pair (rotate-half), or 16 in a row
     const int d0 = rotated ? (p.interleaved ? 16 : 8) * lane : in ? p.rot + 16 * (lane - turning) : 0;
     const int d1 = rotated && !p.interleaved ? half + 8 * lane : d0 + 8;
-    float wq[16];                                            // the q heads' weights of the lane's dimensions
+    const float inv_dim = 1.f / (float)p.head_dim;
+    const long long step = (long long)heads_per * p.head_dim;
+    const int units = p.tokens * p.parts, stride = gridDim.x * kRopeWarps;
+    float* table = tables[warp];
+    // the norms' weights as the lanes read them
+    __shared__ __align__(16) float weights[2][512];          // q, k: 8 for d0 of every lane, 8 for d1
     pdl_trigger();
     pdl_wait();
-    if (p.q_norm && in) {
-        read8(p.q_norm + d0, wq);
-        read8(p.q_norm + d1, wq + 8);
-    }
-    for (int tok0 = blockIdx.x * p.batch; tok0 < p.tokens; tok0 += gridDim.x * p.batch) {
-        const int n = min(p.batch, p.tokens - tok0);
-        // the first pass's loads, before anything that waits
-        int slot = tid >> p.lanes_log2, tok = 0;             // the head (of this CTA's) and the token (of the batch)
-        auto wrap = [&]() {
-            while (slot >= here) {
-                slot -= here;
-                ++tok;
-            }
-        };
-        wrap();
-        uint4 wl = make_uint4(0, 0, 0, 0), wh = wl;
-        auto fetch = [&]() {
-            if (in && tok < n) {
-                const __nv_bfloat16* src = p.qkv + (tok0 + tok) * p.qkv_token + (long long)(first + slot) * p.head_dim;
-                wl = *reinterpret_cast<const uint4*>(src + d0);
-                wh = *reinterpret_cast<const uint4*>(src + d1);
-            }
-        };
-        fetch();
-        __syncthreads();                                     // the table's last readers are done
-        if (tid < n) {
-            const int t = tok0 + tid, pos = __ldg(p.pos + t);
-            long long k = -1, v = -1;
-            if (pos < -1) serve_error(kErrPosition);
-            if (pos >= 0 && p.k) {
-                const int sid = p.seq ? __ldg(p.seq + t) : t, pg = pos / p.page_size, row = pos - pg * p.page_size;
-                if ((unsigned)sid >= (unsigned)p.sequences || pg >= p.max_pages) {
-                    serve_error(kErrPosition);
-                } else {
-                    const int id = __ldg(p.table + sid * p.table_seq + pg);
-                    if ((unsigned)id >= (unsigned)p.num_pages) {
-                        serve_error(kErrPage);
-                    } else {
-                        k = id * p.k_page + row * p.k_row;
-                        v = id * p.v_page + row * p.v_row;
-                    }
-                }
-            }
-            live_at[tid] = pos >= 0;                         // -1: padding
-            k_at[tid] = k;
-            v_at[tid] = v;
-        }
-        for (int e = tid; e < n * half; e += kRopeThreads) {
-            const int t = e / half, i = e - t * half;
-            const double turns = (double)__ldg(p.pos + tok0 + t) * __ldg(p.inv_freq + i) * 0.15915494309189533577;
-            const double r = 2.0 * (turns - rint(turns));    // in half turns
-            float* c = cs + t * 2 * half + i;
-            if (FMT == 1) {
-                double s, co;
-                sincospi(r, &s, &co);
-                csd[t * 2 * half + i] = co;
-                csd[t * 2 * half + half + i] = s;
-                c[0] = (float)co;
-                c[half] = (float)s;
-            } else {
-                float s, co;
-                sincospif((float)r, &s, &co);
-                c[0] = co;
-                c[half] = s;
-            }
+    if (any_norm) {
+        for (int e = threadIdx.x; e < 2 * 16 * lanes; e += kRopeThreads) {
+            const int which = e / (16 * lanes), rest = e % (16 * lanes), h = rest / (8 * lanes), l = rest % (8 * lanes) >> 3,
+                      i = rest & 7;
+            const float* w = which ? p.k_norm : p.q_norm;
+            const bool rot = l < turning, is = l < p.head_dim / 16;
+            const int e0 = rot ? (p.interleaved ? 16 : 8) * l : is ? p.rot + 16 * (l - turning) : 0;
+            const int e1 = rot && !p.interleaved ? half + 8 * l : e0 + 8;
+            weights[which][h * 8 * lanes + spread(l, i, lanes)] = w && is ? __ldg(w + (h ? e1 : e0) + i) : 0.f;
         }
         __syncthreads();
-        for (int pass = 0; pass < n * here; pass += per_pass) {
-            const int head = first + slot, tk = tok;
-            const bool live = in && tk < n && live_at[min(tk, n - 1)];
-            const bool is_q = head < p.heads, is_k = !is_q && head < p.heads + p.kv_heads;
-            const int kvh = is_q ? 0 : is_k ? head - p.heads : head - p.heads - p.kv_heads;
-            const float* table = cs + min(tk, n - 1) * 2 * half + 8 * lane;
-            Head<float> x;
-            x.load(wl, wh);
-            Head<double> y;                                  // a row of an e4m3 cache
-            if (FMT == 1) y.load(wl, wh);
-            slot += per_pass;
-            wrap();
-            fetch();                                         // of the next pass
-            if (p.q_norm || p.k_norm) {
-                const float r = rsqrtf(x.sum_of_squares(lanes) * (1.f / (float)p.head_dim) + p.eps);
-                if (is_q && p.q_norm) x.scale(r, wq, wq + 8);
-                if (is_k && p.k_norm && in) {
-                    float w[16];
-                    read8(p.k_norm + d0, w);
-                    read8(p.k_norm + d1, w + 8);
-                    x.scale(r, w, w + 8);
-                }
-            }
-            if (rotated && (is_q || is_k)) x.rotate(table, half, p.interleaved);
-            if (FMT == 1) {
-                if (p.k_norm) {
-                    const double sq = y.sum_of_squares(lanes);
-                    if (is_k && in) {
-                        float w[16];
-                        read8(p.k_norm + d0, w);
-                        read8(p.k_norm + d1, w + 8);
-                        y.scale(1.0 / sqrt(sq / (double)p.head_dim + (double)p.eps), w, w + 8);
-                    }
-                }
-                if (rotated && is_k) y.rotate(csd + min(tk, n - 1) * 2 * half + 8 * lane, half, p.interleaved);
-            }
-            if (!live) continue;
-            const long long t = tok0 + tk;
-            if (is_q || (is_k && p.k_out)) {
-                __nv_bfloat16* dst = is_q ? p.q_out + t * p.q_token + head * p.q_head
-                                          : p.k_out + t * p.ko_token + kvh * p.ko_head;
-                *reinterpret_cast<uint4*>(dst + d0) = pack8(x.lo);
-                *reinterpret_cast<uint4*>(dst + d1) = pack8(x.hi);
-            }
-            const long long at = is_k ? k_at[tk] : v_at[tk];
-            if (is_q || at < 0) continue;
-            uint8_t* dst = is_k ? p.k + at + kvh * p.k_head : p.v + at + kvh * p.v_head;
-            if (FMT == 0) {
-                *reinterpret_cast<uint4*>(dst + 2 * d0) = pack8(x.lo);
-                *reinterpret_cast<uint4*>(dst + 2 * d1) = pack8(x.hi);
+    }
+    int unit = blockIdx.x * kRopeWarps + warp;
+    if (unit >= units) return;
+    uint4 wl = make_uint4(0, 0, 0, 0), wh = wl;
+    auto fetch = [&](const __nv_bfloat16* src, int head) {   // src: the pass's first head
+        if (in && head < p.slots) {
+            wl = *reinterpret_cast<const uint4*>(src + d0);
+            wh = *reinterpret_cast<const uint4*>(src + d1);
+        }
+    };
+    auto pass_at = [&](int u, int& pass) {                   // the first pass of a unit
+        const int tok = u / p.parts;
+        pass = (u - tok * p.parts) * p.part_passes;
+        return p.qkv + tok * p.qkv_token + (long long)(pass * heads_per + sub) * p.head_dim;
+    };
+    int pass;
+    const __nv_bfloat16* src = pass_at(unit, pass);
+    fetch(src, pass * heads_per + sub);
+    for (;;) {
+        const int tok = unit / p.parts, pos = __ldg(p.pos + tok);
+        const int end = min((pass + p.part_passes) * heads_per, p.slots);        // the unit's heads end here
+        const int next = unit + stride;
+        int next_pass = 0;
+        const __nv_bfloat16* next_src = src;
+        if (next < units) next_src = pass_at(next, next_pass);
+        long long k_at = -1, v_at = -1;                      // the token's row in the pools (bytes; -1: none)
+        if (pos < -1 && wlane == 0) serve_error(kErrPosition);
+        if (pos >= 0 && p.k && end > p.heads) {
+            const int sid = p.seq ? __ldg(p.seq + tok) : tok, pg = pos / p.page_size, row = pos - pg * p.page_size;
+            if ((unsigned)sid >= (unsigned)p.sequences || pg >= p.max_pages) {
+                serve_error(kErrPosition);
             } else {
-                const float* sc = is_k ? p.k_scale : p.v_scale;
-                if (sc) {
-                    const double scale = (double)__ldg(sc + kvh);
-#pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        y.lo[i] /= scale;
-                        y.hi[i] /= scale;
-                    }
+                const int id = __ldg(p.table + sid * p.table_seq + pg);
+                if ((unsigned)id >= (unsigned)p.num_pages) {
+                    serve_error(kErrPage);
+                } else {
+                    k_at = id * p.k_page + row * p.k_row;
+                    v_at = id * p.v_page + row * p.v_row;
                 }
-                *reinterpret_cast<uint2*>(dst + d0) = pack8_e4m3(y.lo);
-                *reinterpret_cast<uint2*>(dst + d1) = pack8_e4m3(y.hi);
             }
         }
+        __syncwarp();
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (wlane + 32 * i < half) {
+                const int a = wlane + 32 * i;
+                const double t = (double)pos * __ldg(p.inv_freq + a) * 0.15915494309189533577;
+                const int at = spread(a >> 3, a & 7, turning);                   // lane a / 8's angle a % 8
+                sincospif(2.f * (float)(t - rint(t)), table + half + at, table + at);
+            }
+        __syncwarp();
+        F2 c[4], s[4];
+        if (rotated) {
+            read_spread(table, lane, turning, c);
+            read_spread(table + half, lane, turning, s);
+        }
+        for (int head0 = pass * heads_per; head0 < end; head0 += heads_per) {
+            const int head = head0 + sub;
+            const uint4 rl = wl, rh = wh;
+            Head x;
+            x.load(rl, rh);
+            src += step;
+            if (head0 + heads_per < end) fetch(src, head + heads_per);
+            else if (next < units) fetch(next_src, next_pass * heads_per + sub);
+            const bool live = in && pos >= 0;
+            float r = 1.f;
+            if (any_norm) r = rsqrtf(x.sum_of_squares(lanes) * inv_dim + p.eps);
+            const bool is_q = head < p.heads, is_k = !is_q && head < p.heads + p.kv_heads, have = live && head < end;
+            if (is_q ? p.q_norm != nullptr : is_k && p.k_norm) {
+                F2 w[8];
+                const float* from = weights[is_q ? 0 : 1];
+                read_spread(from, lane, lanes, w);
+                read_spread(from + 8 * lanes, lane, lanes, w + 4);
+                x.scale(r, w, w + 4);
+            }
+            float l[8], h[8], mag[8];                        // |a| + |b| of each rotated pair, |x| and more of the others
+            if (FMT == 1) {
+                x.get(l, h);
+#pragma unroll
+                for (int i = 0; i < 8; ++i)
+                    mag[i] = fabsf(l[i]) + fabsf(h[i]) + (p.interleaved ? fabsf(l[i ^ 1]) + fabsf(h[i ^ 1]) : 0.f);
+            }
+            if (rotated && (is_q || is_k)) x.rotate(c, s, p.interleaved);
+            x.get(l, h);
+            const int kvh = is_k ? head - p.heads : head - p.heads - p.kv_heads;
+            if (have && (is_q || (is_k && p.k_out))) {
+                __nv_bfloat16* dst = is_q ? p.q_out + tok * p.q_token + head * p.q_head
+                                          : p.k_out + tok * p.ko_token + kvh * p.ko_head;
+                *reinterpret_cast<uint4*>(dst + d0) = pack8(l);
+                *reinterpret_cast<uint4*>(dst + d1) = pack8(h);
+            }
+            const bool stored = have && !is_q && k_at >= 0;
+            uint8_t* dst = is_k ? p.k + kvh * p.k_head + k_at : p.v + kvh * p.v_head + v_at;
+            if (FMT == 0) {
+                if (stored) {
+                    *reinterpret_cast<uint4*>(dst + 2 * d0) = pack8(l);
+                    *reinterpret_cast<uint4*>(dst + 2 * d1) = pack8(h);
+                }
+            } else if (__any_sync(~0u, stored)) {
+                // fp32's error in steps of 2^-24 of |a| + |b|: k 20 / 2 for the mean square (a step per addition, halved by
+                // the root), 5 for the root, 2 products, 4 for the angle (2 pi 2^-25) and its sine and cosine, 3 for the
+                // rotation, 2 for the scale: below 2^-19; v 2 for the scale
+                const float* sc = is_k ? p.k_scale : p.v_scale;
+                const float scale = stored && sc ? __ldg(sc + kvh) : 1.f, inv = 1.f / scale;
+                float al[8], ah[8], bl[8], bh[8];
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float el = is_k ? mag[i] * 1.6e-6f : fabsf(l[i]) * 1.3e-7f;
+                    const float eh = is_k ? mag[i] * 1.6e-6f : fabsf(h[i]) * 1.3e-7f;
+                    al[i] = (l[i] - el) * inv;
+                    ah[i] = (h[i] - eh) * inv;
+                    bl[i] = (l[i] + el) * inv;
+                    bh[i] = (h[i] + eh) * inv;
+                }
+                const uint2 a0 = pack8_e4m3(al), a1 = pack8_e4m3(ah), b0 = pack8_e4m3(bl), b1 = pack8_e4m3(bh);
+                unsigned long long v[2] = {a0.x | (unsigned long long)a0.y << 32, a1.x | (unsigned long long)a1.y << 32};
+                const bool unsure = a0.x != b0.x || a0.y != b0.y || a1.x != b1.x || a1.y != b1.y;
+                if (__any_sync(~0u, stored && unsure)) {
+                    unsigned todo = 0;
+                    if (stored && unsure) {
+                        const uint32_t d[4] = {a0.x ^ b0.x, a0.y ^ b0.y, a1.x ^ b1.x, a1.y ^ b1.y};
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) todo |= (d[i >> 2] >> 8 * (i & 3) & 0xFF ? 1u : 0u) << i;
+                    }
+                    exact_pairs(p, rl, rh, pos, is_k, in, rotated, lane, d0, d1, scale, todo, v);
+                }
+                if (stored) {
+                    *reinterpret_cast<unsigned long long*>(dst + d0) = v[0];
+                    *reinterpret_cast<unsigned long long*>(dst + d1) = v[1];
+                }
+            }
+        }
+        if (next >= units) return;
+        unit = next;
+        pass = next_pass;
+        src = next_src;
     }
 }
 
@@ -340,22 +452,17 @@ extern "C" int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* str
     p.eps = a->eps;
     p.slots = a->heads + 2 * a->kv_heads;
     while ((16 << p.lanes_log2) < a->head_dim) ++p.lanes_log2;
-    const int sms = sm_count(), per_pass = kRopeThreads >> p.lanes_log2;
-    dim3 grid;
-    if (a->tokens < 2 * sms) {
-        // few tokens: their heads are spread over CTAs, a pass of 256 threads each (each computes the angles anew)
-        p.batch = 1;
-        p.per_cta = per_pass;
-        grid = dim3((unsigned)a->tokens, (unsigned)((p.slots + per_pass - 1) / per_pass));
-    } else {
-        // as many tokens at a time as the table holds, but work for every SM
-        p.batch = a->rot ? kRopeTable / a->rot : kRopeBatch;
-        if (p.batch > kRopeBatch) p.batch = kRopeBatch;
-        while (p.batch > 1 && a->tokens / p.batch < 4 * sms) p.batch /= 2;
-        p.per_cta = p.slots;
-        const int want = (a->tokens + p.batch - 1) / p.batch;
-        grid = dim3((unsigned)(want < 8 * sms ? want : 8 * sms), 1u);
-    }
+    // Units of four passes where that fills the GPU's warps (24 per SM), shorter ones for fewer tokens.
+    const int heads_per = 32 >> p.lanes_log2, passes = (p.slots + heads_per - 1) / heads_per;
+    const long long warps = (long long)sm_count() * 3 * kRopeWarps;
+    long long parts = (passes + 3) / 4;
+    if (a->tokens * parts < warps) parts = warps / a->tokens < passes ? warps / a->tokens : passes;
+    p.part_passes = (int)((passes + parts - 1) / parts);
+    p.parts = (passes + p.part_passes - 1) / p.part_passes;
+    if ((long long)a->tokens * p.parts > 0x7ff00000ll) return -2;
+    const long long ctas = ((long long)a->tokens * p.parts + kRopeWarps - 1) / kRopeWarps;
+    const long long most = (long long)sm_count() * (a->cache == 0 ? 3 : 2);
+    const dim3 grid((unsigned)(ctas < most ? ctas : most));
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
     return a->cache == 0 ? serve_launch(qkv_rope_kernel<0>, p, grid, kRopeThreads, 0, st)
                          : serve_launch(qkv_rope_kernel<1>, p, grid, kRopeThreads, 0, st);
