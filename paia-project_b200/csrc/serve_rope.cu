@@ -76,15 +76,6 @@ __device__ __forceinline__ float to_odd(double x) {
     const float f = __double2float_rz(x);
     return (double)f == x ? f : __uint_as_float(__float_as_uint(f) | 1u);
 }
-// 8 consecutive table entries or weights as 4 pairs.
-__device__ __forceinline__ void read8(const float* p, F2* x) {
-    const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-    x[0] = F2(a.x, a.y);
-    x[1] = F2(a.z, a.w);
-    x[2] = F2(b.x, b.y);
-    x[3] = F2(b.z, b.w);
-}
-
 // The 16 elements of a lane as pairs of neighbours. Every lane of the warp calls sum_of_squares.
 struct Head {
     F2 lo[4], hi[4];

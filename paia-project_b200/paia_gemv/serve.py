@@ -23,23 +23,20 @@ _BF16, _F32, _F64, _I32, _E4M3 = torch.bfloat16, torch.float32, torch.float64, t
 
 
 def _bad(name, t, what):
-    raise ValueError(f"{name} must be {what}, got " + (f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}"
-                                                       if isinstance(t, torch.Tensor) else repr(t)))
+    raise ValueError(f"{name} must be {what} on the current CUDA device, got "
+                     + (f"{t.dtype} {tuple(t.shape)} strides {t.stride()} on {t.device}"
+                        if isinstance(t, torch.Tensor) else repr(t)))
 
 
-def _rows(name, t, dtype, shape, dev):
-    """t: `shape`, contiguous innermost dimension, any other strides."""
-    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or (t.stride()[-1] != 1 and shape[-1] != 1):
-        _bad(name, t, f"{dtype} {tuple(shape)} on the current CUDA device, contiguous in its last dimension")
-    return t.data_ptr()
+# The checks are written out call by call (a decode step makes them on its critical path): a tensor's shape, type,
+# device and contiguous last dimension, then its pointer and strides into the struct.
 
-
-def _flat(name, t, dtype, n, dev):
-    """Contiguous [n], or None."""
+def _flat(name, t, dtype, shape, dev):
+    """The pointer of a contiguous tensor of this shape; 0 for None."""
     if t is None:
         return 0
-    if t.shape != (n,) or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
-        _bad(name, t, f"contiguous {dtype} [{n}] on the current CUDA device")
+    if t.shape != shape or t.dtype is not dtype or t.get_device() != dev or not t.is_contiguous():
+        _bad(name, t, f"contiguous {dtype} {shape}")
     return t.data_ptr()
 
 
@@ -51,19 +48,20 @@ def _device(t, name):
 
 
 def _pools(k, v, kv_heads, head_dim, k_scale, v_scale, dev):
-    """(cache code, pool shape) of a cache's two pools."""
-    shape, dtype = k.shape, k.dtype
+    """(cache code, pool shape, strides of k, of v) of a cache's two pools."""
+    shape, dtype, ks, vs = k.shape, k.dtype, k.stride(), v.stride()
     if len(shape) != 4 or shape[2] != kv_heads or shape[3] != head_dim:
         _bad("k_pages", k, f"[num_pages, page_size, {kv_heads}, {head_dim}]")
-    if dtype is not _BF16 and dtype is not _E4M3:
+    if dtype is _BF16:
+        if k_scale is not None or v_scale is not None:
+            raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
+    elif dtype is not _E4M3:
         _bad("k_pages", k, "bfloat16 or float8_e4m3fn")
-    if dtype is _BF16 and (k_scale is not None or v_scale is not None):
-        raise ValueError("k_scale and v_scale belong to float8_e4m3fn caches")
-    if k.get_device() != dev or k.stride()[3] != 1:
-        _bad("k_pages", k, "on the current CUDA device, contiguous in its last dimension")
-    if v.shape != shape or v.dtype is not dtype or v.get_device() != dev or v.stride()[3] != 1:
-        _bad("v_pages", v, f"{dtype} {tuple(shape)} on the current CUDA device, contiguous in its last dimension")
-    return (0 if dtype is _BF16 else 1), shape
+    if k.get_device() != dev or ks[3] != 1:
+        _bad("k_pages", k, "contiguous in its last dimension,")
+    if v.shape != shape or v.dtype is not dtype or v.get_device() != dev or vs[3] != 1:
+        _bad("v_pages", v, f"{dtype} {tuple(shape)}, contiguous in its last dimension,")
+    return (0 if dtype is _BF16 else 1), shape, ks, vs
 
 
 class AttentionWorkspace:
@@ -85,32 +83,38 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
     """out[b] = attention of q[b] (bf16 [batch, heads, head_dim]) over the first lens[b] positions of sequence b (the
     last `window` of them where window > 0). out bf16 like q; lse fp32 [batch, heads], natural logarithm, or None. A
     sequence of length 0 gets zeros and -inf. scale: 1 / sqrt(head_dim) by default."""
-    dev, shape, pool = _device(q, "q"), q.shape, k_pages.shape
-    if len(shape) != 3:
-        _bad("q", q, "[batch, heads, head_dim]")
+    dev, shape, qs, os = _device(q, "q"), q.shape, q.stride(), out.stride()
+    if len(shape) != 3 or q.dtype is not _BF16 or (qs[2] != 1 and shape[2] != 1):
+        _bad("q", q, "bfloat16 [batch, heads, head_dim], contiguous in its last dimension,")
+    if out.shape != shape or out.dtype is not _BF16 or out.get_device() != dev or os[2] != 1:
+        _bad("out", out, f"bfloat16 {tuple(shape)}, contiguous in its last dimension,")
     batch, heads, hd = shape
-    kv = pool[2] if len(pool) == 4 else 0
+    kv = k_pages.shape[2] if k_pages.dim() == 4 else 0
     if not kv or heads % kv:
         _bad("k_pages", k_pages, f"[num_pages, page_size, kv_heads, {hd}] with kv_heads dividing {heads}")
-    cache, pool = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
-    ts = page_table.shape
-    if len(ts) != 2 or ts[0] != batch:
-        _bad("page_table", page_table, f"[{batch}, max_pages]")
-    table = _rows("page_table", page_table, _I32, ts, dev)
+    cache, pool, ks, vs = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
+    ts, tst = page_table.shape, page_table.stride()
+    if len(ts) != 2 or ts[0] != batch or page_table.dtype is not _I32 or page_table.get_device() != dev or (
+            tst[1] != 1 and ts[1] != 1):
+        _bad("page_table", page_table, f"int32 [{batch}, max_pages], contiguous in its last dimension,")
+    if lens.shape != (batch,) or lens.dtype is not _I32 or lens.get_device() != dev or not lens.is_contiguous():
+        _bad("lens", lens, f"contiguous int32 [{batch}]")
+    lp = ls = 0
+    if lse is not None:
+        if lse.shape != (batch, heads) or lse.dtype is not _F32 or lse.get_device() != dev or (
+                lse.stride(1) != 1 and heads != 1):
+            _bad("lse", lse, f"float32 [{batch}, {heads}], contiguous in its last dimension,")
+        lp, ls = lse.data_ptr(), lse.stride(0)
     if workspace.sizes != (dev, heads, kv, hd):
         raise ValueError(f"workspace is for (device, heads, kv_heads, head_dim) = {workspace.sizes}, the call for "
                          f"{(dev, heads, kv, hd)}")
-    ks, vs = k_pages.stride(), v_pages.stride()
-    qs, os = q.stride(), out.stride()
     lib.paged_attn(ATTN.pack(
-        _rows("q", q, _BF16, shape, dev), k_pages.data_ptr(), v_pages.data_ptr(), table,
-        _flat("lens", lens, _I32, batch, dev), _flat("k_scale", k_scale, _F32, kv, dev),
-        _flat("v_scale", v_scale, _F32, kv, dev), _rows("out", out, _BF16, shape, dev),
-        0 if lse is None else _rows("lse", lse, _F32, (batch, heads), dev), workspace.ptr,
-        qs[0], qs[1], os[0], os[1], 0 if lse is None else lse.stride(0), page_table.stride(0),
-        ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
-        batch, heads, kv, hd, cache, pool[0], pool[1], ts[1], window,
-        hd ** -0.5 if scale is None else scale), torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+        q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
+        0 if k_scale is None else _flat("k_scale", k_scale, _F32, (kv,), dev),
+        0 if v_scale is None else _flat("v_scale", v_scale, _F32, (kv,), dev), out.data_ptr(), lp, workspace.ptr,
+        qs[0], qs[1], os[0], os[1], ls, tst[0], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        batch, heads, kv, hd, cache, pool[0], pool[1], ts[1], window, hd ** -0.5 if scale is None else scale),
+        torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return out
 
 
@@ -129,34 +133,45 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
     head_dim (`rope_inv_freq`). k_out (bf16 [tokens, kv_heads, head_dim]) gets the rotated k heads as well; without a
     cache (k_pages, v_pages and page_table None) it is required, with kv_heads. Two rows of a call must not name the
     same sequence and position."""
-    dev = _device(qkv, "qkv")
-    if q_out.dim() != 3 or qkv.dim() != 2:
-        _bad("qkv and q_out", q_out, "[tokens, (heads + 2 kv_heads) * head_dim] and [tokens, heads, head_dim]")
+    dev, qs, xs = _device(qkv, "qkv"), q_out.stride(), qkv.stride()
+    if len(qs) != 3 or q_out.dtype is not _BF16 or q_out.get_device() != dev or qs[2] != 1:
+        _bad("q_out", q_out, "bfloat16 [tokens, heads, head_dim], contiguous in its last dimension,")
     tokens, heads, hd = q_out.shape
     if k_pages is not None:
         kv = k_pages.shape[2] if k_pages.dim() == 4 else 0
-        cache, (num_pages, page_size, _, _) = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
-        ks, vs, kp, vp = k_pages.stride(), v_pages.stride(), k_pages.data_ptr(), v_pages.data_ptr()
-        if page_table.dim() != 2 or (seq is None and page_table.shape[0] < tokens):
-            _bad("page_table", page_table, "[sequences, max_pages]")
-        seqs, max_pages = page_table.shape
-        table, ts = _rows("page_table", page_table, _I32, page_table.shape, dev), page_table.stride(0)
+        cache, (num_pages, page_size, _, _), ks, vs = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
+        kp, vp, shape, tst = k_pages.data_ptr(), v_pages.data_ptr(), page_table.shape, page_table.stride()
+        if len(shape) != 2 or page_table.dtype is not _I32 or page_table.get_device() != dev or (
+                tst[1] != 1 and shape[1] != 1) or (seq is None and shape[0] < tokens):
+            _bad("page_table", page_table, "int32 [sequences, max_pages], contiguous in its last dimension,")
+        seqs, max_pages = shape
+        table, ts = page_table.data_ptr(), tst[0]
     else:
         if v_pages is not None or page_table is not None or k_out is None or not kv_heads:
             raise ValueError("without a cache, v_pages and page_table are None and k_out and kv_heads are given")
         kv, cache, num_pages, page_size, seqs, max_pages, table, ts, kp, vp = kv_heads, 0, 0, 1, 0, 0, 0, 0, 0, 0
         ks = vs = (0, 0, 0)
-    qs = q_out.stride()
-    kos = (0, 0) if k_out is None else k_out.stride()
+    if qkv.shape != (tokens, (heads + 2 * kv) * hd) or qkv.dtype is not _BF16 or xs[1] != 1:
+        _bad("qkv", qkv, f"bfloat16 {(tokens, (heads + 2 * kv) * hd)}, contiguous in its last dimension,")
+    if positions.shape != (tokens,) or positions.dtype is not _I32 or positions.get_device() != dev or (
+            not positions.is_contiguous()):
+        _bad("positions", positions, f"contiguous int32 [{tokens}]")
     half = inv_freq.shape[0] if inv_freq.dim() == 1 else -1
+    if inv_freq.dtype is not _F64 or half < 0 or inv_freq.get_device() != dev or not inv_freq.is_contiguous():
+        _bad("inv_freq", inv_freq, "contiguous float64 [rot / 2]")
+    ko = kos = 0
+    if k_out is not None:
+        kos = k_out.stride()
+        if k_out.shape != (tokens, kv, hd) or k_out.dtype is not _BF16 or k_out.get_device() != dev or kos[2] != 1:
+            _bad("k_out", k_out, f"bfloat16 {(tokens, kv, hd)}, contiguous in its last dimension,")
+        ko = k_out.data_ptr()
     lib.qkv_rope_cache(ROPE_CACHE.pack(
-        _rows("qkv", qkv, _BF16, (tokens, (heads + 2 * kv) * hd), dev),
-        _flat("positions", positions, _I32, tokens, dev), _flat("seq", seq, _I32, tokens, dev),
-        _flat("inv_freq", inv_freq, _F64, half, dev), _flat("q_norm", q_norm, _F32, hd, dev),
-        _flat("k_norm", k_norm, _F32, hd, dev), table, _flat("k_scale", k_scale, _F32, kv, dev),
-        _flat("v_scale", v_scale, _F32, kv, dev), _rows("q_out", q_out, _BF16, (tokens, heads, hd), dev),
-        0 if k_out is None else _rows("k_out", k_out, _BF16, (tokens, kv, hd), dev), kp, vp,
-        qkv.stride(0), qs[0], qs[1], kos[0], kos[1], ts, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
+        qkv.data_ptr(), positions.data_ptr(), 0 if seq is None else _flat("seq", seq, _I32, (tokens,), dev),
+        inv_freq.data_ptr(), 0 if q_norm is None else _flat("q_norm", q_norm, _F32, (hd,), dev),
+        0 if k_norm is None else _flat("k_norm", k_norm, _F32, (hd,), dev), table,
+        0 if k_scale is None else _flat("k_scale", k_scale, _F32, (kv,), dev),
+        0 if v_scale is None else _flat("v_scale", v_scale, _F32, (kv,), dev), q_out.data_ptr(), ko, kp, vp,
+        xs[0], qs[0], qs[1], kos[0] if ko else 0, kos[1] if ko else 0, ts, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
         tokens, seqs, heads, kv, hd, 2 * half, 1 if interleaved else 0, cache, num_pages, page_size, max_pages, eps),
         torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return q_out
@@ -166,17 +181,29 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
     """out[m] = base[m] + scaling[i] * b[i] (a[i] x[m]) for i = adapter[m] (int32; -1: out[m] = base[m]). x bf16 [M, K],
     a bf16 [adapters, rank, K], b bf16 [adapters, N, rank], out and base (None: zeros; may be out) bf16 [M, N]; scaling
     fp32 and ranks int32 [adapters] (None: 1 and `rank`): adapter i uses its first ranks[i] ranks."""
-    dev = _device(x, "x")
-    if x.dim() != 2 or a.dim() != 3 or b.dim() != 3:
-        _bad("x, a and b", x, "[M, K], [adapters, rank, K] and [adapters, N, rank]")
+    dev, xs, sa, sb, os = _device(x, "x"), x.stride(), a.stride(), b.stride(), out.stride()
+    if len(xs) != 2 or x.dtype is not _BF16 or xs[1] != 1 or len(sa) != 3 or len(sb) != 3:
+        _bad("x", x, "bfloat16 [M, K], contiguous in its last dimension (a [adapters, rank, K], b [adapters, N, rank]),")
     m, k = x.shape
-    n_ad, rank, n = a.shape[0], a.shape[1], b.shape[1]
-    sa, sb = a.stride(), b.stride()
+    n_ad, rank, ka = a.shape
+    if ka != k or a.dtype is not _BF16 or a.get_device() != dev or sa[2] != 1:
+        _bad("a", a, f"bfloat16 [adapters, rank, {k}], contiguous in its last dimension,")
+    n = b.shape[1]
+    if b.shape != (n_ad, n, rank) or b.dtype is not _BF16 or b.get_device() != dev or sb[2] != 1:
+        _bad("b", b, f"bfloat16 [{n_ad}, N, {rank}], contiguous in its last dimension,")
+    if adapter.shape != (m,) or adapter.dtype is not _I32 or adapter.get_device() != dev or not adapter.is_contiguous():
+        _bad("adapter", adapter, f"contiguous int32 [{m}]")
+    if out.shape != (m, n) or out.dtype is not _BF16 or out.get_device() != dev or os[1] != 1:
+        _bad("out", out, f"bfloat16 {(m, n)}, contiguous in its last dimension,")
+    bp = bs = 0
+    if base is not None:
+        if base.shape != (m, n) or base.dtype is not _BF16 or base.get_device() != dev or base.stride(1) != 1:
+            _bad("base", base, f"bfloat16 {(m, n)}, contiguous in its last dimension,")
+        bp, bs = base.data_ptr(), base.stride(0)
     lib.lora(LORA.pack(
-        _rows("x", x, _BF16, (m, k), dev), _rows("a", a, _BF16, (n_ad, rank, k), dev),
-        _rows("b", b, _BF16, (n_ad, n, rank), dev), _flat("adapter", adapter, _I32, m, dev),
-        _flat("ranks", ranks, _I32, n_ad, dev), _flat("scaling", scaling, _F32, n_ad, dev),
-        0 if base is None else _rows("base", base, _BF16, (m, n), dev), _rows("out", out, _BF16, (m, n), dev),
-        x.stride(0), 0 if base is None else base.stride(0), out.stride(0), sa[0], sa[1], sb[0], sb[1],
-        m, n, k, rank, n_ad), torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+        x.data_ptr(), a.data_ptr(), b.data_ptr(), adapter.data_ptr(),
+        0 if ranks is None else _flat("ranks", ranks, _I32, (n_ad,), dev),
+        0 if scaling is None else _flat("scaling", scaling, _F32, (n_ad,), dev), bp, out.data_ptr(),
+        xs[0], bs, os[0], sa[0], sa[1], sb[0], sb[1], m, n, k, rank, n_ad),
+        torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
     return out
