@@ -8,11 +8,15 @@ at position ctx - 1, so every tensor shape is fixed and a whole token captures a
 device time. The reference measures decode cost per token as a sum of per-op GEMV times
 (paia-bench/bench/analyze_e4.py:177-196); this measures the token itself, GEMVs and the ops between them (torch:
 RMSNorm, scaled-dot-product attention, SiLU x up, residual adds).
+
+`PagedDecodeModel` is the same step for a batch of sequences of different lengths, as a server runs it: batched GEMVs,
+low-rank adapters per request, rotary positions and cache write in one pass (`serve.qkv_rope_cache`), attention over a
+paged cache (`serve.paged_attention`); lengths live on the device, so one captured graph decodes token after token.
 """
 import torch
 import torch.nn.functional as F
 
-from . import quant
+from . import quant, serve
 
 MODELS = {
     "llama31_8b": dict(hidden=4096, heads=32, kv_heads=8, head_dim=128, inter=14336, vocab=128256, layers=32,
@@ -78,6 +82,13 @@ class Projection:
         else:
             L.int4_asym_bias(W, p(self.s), p(self.z), xp, p(self.bias), yp, self.N, self.K, v) \
                 if self.bias is not None else L.int4_asym(W, p(self.s), p(self.z), xp, yp, self.N, self.K, v)
+        return y
+
+    def rows(self, x, y):
+        """y[m] = W x[m] (+ bias) for every row (bf16 [M, K] and [M, N], row-major) through paia_gemv_batched."""
+        p = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+        self.lib.batched(self.kind, p(self.W), p(self.s), p(self.z), x.data_ptr(), p(self.bias), y.data_ptr(),
+                         x.shape[0], self.N, self.K)
         return y
 
     def dequantised(self):
@@ -198,6 +209,108 @@ class DecodeModel:
         return self.logits
 
 
+class PagedDecodeModel:
+    """Synthetic weights of a model's decode path in one format and a paged KV cache for `batch` sequences of up to
+    `max_len` positions (bf16, or float8_e4m3fn with a scale per kv head where cache="fp8"), the first lens[b] of them
+    synthetic. step() decodes one token of every sequence at position lens[b], appends it and raises lens[b].
+    adapters > 0: that many low-rank adapters of rank `rank` on the qkv, o, gate_up and down projections; self.adapter[b]
+    (int32, -1: none) names the one of sequence b. qk_norm: RMS norm of q and k per head before the rotation. A sequence
+    that is full must be retired by its caller; active[b] = False (self.active) makes row b padding: its cache and length
+    stay, its logits are those of an empty context."""
+
+    def __init__(self, lib, model, kind, lens, max_len=1024, page_size=16, cache="bf16", adapters=0, rank=16,
+                 qk_norm=False, layers=None, seed=0, dims=None):
+        cfg = dict(MODELS[model])
+        cfg.update(dims or {})
+        if layers is not None:
+            cfg["layers"] = layers
+        if not lens or max(lens) >= max_len or min(lens) < 0:
+            raise ValueError(f"lens must lie in [0, max_len = {max_len}), got {lens}")
+        self.lib, self.cfg, self.kind, self.page_size, self.max_len = lib, cfg, kind, page_size, max_len
+        H, nh, nkv, hd, I, V = (cfg[k] for k in ("hidden", "heads", "kv_heads", "head_dim", "inter", "vocab"))
+        self.batch = B = len(lens)
+        g = torch.Generator(device="cuda").manual_seed(seed)
+        dev = dict(device="cuda", dtype=torch.bfloat16)
+        self.embed = (torch.randn(V, H, device="cuda", generator=g) * 0.02).to(torch.bfloat16)
+        norm = lambda n: (1.0 + 0.1 * torch.randn(n, device="cuda", generator=g)).to(torch.bfloat16).float()   # noqa: E731
+        sizes = {"qkv": ((nh + 2 * nkv) * hd, H), "o": (H, nh * hd), "gate_up": (2 * I, H), "down": (H, I)}
+        per_seq = -(-max_len // page_size)
+        order = torch.randperm(B * per_seq, device="cuda", generator=g)
+        self.page_table = order.view(B, per_seq).to(torch.int32)
+        dtype = torch.bfloat16 if cache == "bf16" else torch.float8_e4m3fn
+        self.k_scale = self.v_scale = None
+        if cache != "bf16":
+            self.k_scale = torch.full((nkv,), 1 / 32, device="cuda")
+            self.v_scale = torch.full((nkv,), 1 / 32, device="cuda")
+        self.layers = []
+        for _ in range(cfg["layers"]):
+            lay = {"norm1": norm(H), "norm2": norm(H), "q_norm": norm(hd) if qk_norm else None,
+                   "k_norm": norm(hd) if qk_norm else None}
+            for name, (n, k) in sizes.items():
+                lay[name] = Projection(lib, kind, n, k, g, bias=name == "qkv" and cfg["qkv_bias"])
+                if adapters:
+                    lay[name + "_a"] = (torch.randn(adapters, rank, k, device="cuda", generator=g) / k ** 0.5).to(torch.bfloat16)
+                    lay[name + "_b"] = (torch.randn(adapters, n, rank, device="cuda", generator=g) * 0.02).to(torch.bfloat16)
+            for name in ("k", "v"):
+                x = torch.randn(B * per_seq, page_size, nkv, hd, device="cuda", generator=g)
+                lay[name] = (x if cache == "bf16" else x * 32).to(dtype)
+            self.layers.append(lay)
+        self.norm_f = norm(H)
+        self.lm_head = Projection(lib, kind, V, H, g)
+        self.scaling = torch.ones(adapters, device="cuda") if adapters else None
+        self.adapter = torch.full((B,), -1, dtype=torch.int32, device="cuda") if adapters else None
+        self.inv_freq = serve.rope_inv_freq(hd, cfg["rope_theta"])
+        self.workspace = serve.attention_workspace(lib, nh, nkv, hd)
+        # state and activations, at fixed addresses so that the step captures as a CUDA graph
+        self.lens = torch.tensor(lens, dtype=torch.int32, device="cuda")
+        self.active = torch.ones(B, dtype=torch.bool, device="cuda")
+        self.token = torch.zeros(B, device="cuda", dtype=torch.long)
+        self.positions = torch.empty(B, dtype=torch.int32, device="cuda")
+        self.padding = torch.full((B,), -1, dtype=torch.int32, device="cuda")
+        self.seen = torch.empty(B, dtype=torch.int32, device="cuda")
+        buf = lambda n: torch.zeros(B, n, **dev)   # noqa: E731
+        self.h, self.a, self.o, self.d = (buf(H) for _ in range(4))
+        self.qkv, self.gu, self.m, self.logits = buf((nh + 2 * nkv) * hd), buf(2 * I), buf(I), buf(V)
+        self.q, self.attn = torch.zeros(B, nh, hd, **dev), torch.zeros(B, nh, hd, **dev)
+
+    def _project(self, lay, name, x, y):
+        """y = the projection of every row, plus the row's adapter."""
+        lay[name].rows(x, y)
+        if self.adapter is not None:
+            serve.lora(self.lib, x, lay[name + "_a"], lay[name + "_b"], self.adapter, y, base=y, scaling=self.scaling)
+
+    def _rmsnorm(self, w, eps=1e-5):
+        self.a.copy_(F.rms_norm(self.h.float(), (self.h.shape[1],), w, eps))
+
+    def step(self):
+        """One token of every active sequence: reads self.token, writes self.logits and the argmax of each active row
+        into self.token, appends to the cache and raises the lengths."""
+        I = self.cfg["inter"]
+        self.h.copy_(self.embed.index_select(0, self.token))
+        torch.where(self.active, self.lens, self.padding, out=self.positions)      # padding rows: position -1, length 0
+        torch.add(self.positions, 1, out=self.seen)
+        for lay in self.layers:
+            self._rmsnorm(lay["norm1"])
+            self._project(lay, "qkv", self.a, self.qkv)
+            serve.qkv_rope_cache(self.lib, self.qkv, self.positions, self.inv_freq, self.q, lay["k"], lay["v"],
+                                 self.page_table, q_norm=lay["q_norm"], k_norm=lay["k_norm"], k_scale=self.k_scale,
+                                 v_scale=self.v_scale)
+            serve.paged_attention(self.lib, self.q, lay["k"], lay["v"], self.page_table, self.seen, self.attn,
+                                  self.workspace, k_scale=self.k_scale, v_scale=self.v_scale)
+            self._project(lay, "o", self.attn.view(self.batch, -1), self.o)
+            self.h.add_(self.o)
+            self._rmsnorm(lay["norm2"])
+            self._project(lay, "gate_up", self.a, self.gu)
+            torch.mul(F.silu(self.gu[:, :I]), self.gu[:, I:], out=self.m)
+            self._project(lay, "down", self.m, self.d)
+            self.h.add_(self.d)
+        self._rmsnorm(self.norm_f)
+        self.lm_head.rows(self.a, self.logits)
+        self.token.copy_(torch.where(self.active, torch.argmax(self.logits, 1), self.token))
+        self.lens.add_(self.active)
+        return self.logits
+
+
 def time_tokens(model, tokens=20, warmup=3):
     """(device microseconds per token, the token ids decoded): the token step captured as one CUDA graph, replayed
     `tokens` times (each replay decodes the next token from the previous one's argmax)."""
@@ -221,7 +334,7 @@ def time_tokens(model, tokens=20, warmup=3):
         g.replay()
     e1.record()
     torch.cuda.synchronize()
-    ids.append(int(model.token.item()))
+    ids.append(int(model.token[0].item()))
     us = e0.elapsed_time(e1) * 1e3 / tokens
     del g
     return us, ids
