@@ -54,7 +54,7 @@ struct AttnParams {
     int batch, kv_heads, group, chunks;     // chunks: units of at most ROWS heads per kv head
     int num_pages, page_size, max_pages, window;
     int page_shift;                         // log2 of page_size, or -1
-    int whole_blocks;                       // page_size % 16 == 0: 16 positions in a row lie in one page
+    int whole_blocks;                       // 16 positions in a row lie in one page, at strides below 2^27 bytes
     float scale_log2;
 };
 
@@ -121,7 +121,7 @@ struct AttnSmem {
     using T = AttnTile<HD, FMT>;
     static constexpr int kStride = HD + 4;                                       // floats per merged row
     static constexpr size_t kRing = (size_t)W * S * T::kStage;
-    static size_t bytes(int rows) { return kRing + (size_t)W * rows * (kStride + 2) * 4; }
+    static size_t bytes(int rows) { return 512 + kRing + (size_t)W * rows * (kStride + 2) * 4; }
 };
 
 // e4m3 fragments. K: word w (of HD / 16) of lane t of a row is at byte k_byte(w, t), read VK words at a time; its four
@@ -137,9 +137,8 @@ struct Frag8 {
     }
     static __device__ __forceinline__ int v_unit(int u, int g) { return (g + 8 * u) * UV; }
 };
-template <int N>                                                                 // N words at byte `b` of a row
-__device__ __forceinline__ void lds_words(uint32_t row, uint32_t key, int b, uint32_t* w) {
-    const uint32_t a = row + ((uint32_t)b ^ key);                                // key: the row's swizzle of 16-byte chunks
+template <int N>
+__device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
     if (N == 4)
         asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(a) : "memory");
     else if (N == 2)
@@ -162,7 +161,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
     const int units = p.kv_heads * p.chunks;
     const int rows = min(p.group, ROWS);
-    float* merge_o = reinterpret_cast<float*>(smem + SM::kRing);                 // [W][rows][kStride]
+    float* merge_o = reinterpret_cast<float*>(smem + 512 + SM::kRing);                 // [W][rows][kStride]
     float2* merge_ml = reinterpret_cast<float2*>(merge_o + W * rows * SM::kStride);
 
     pdl_trigger();
@@ -227,8 +226,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
 
     // ---- the warp's stream of tiles: the run's tiles warp, warp + W, ... Lane i holds what it takes to fetch the i-th of
     // 32 of them (for 16-position blocks that straddle pages: only where the tile lies).
-    const uint32_t ring = sptr(smem) + (uint32_t)(warp * S * T::kStage);
-    struct Look { int id[NB], in[NB], head, range; };                            // rows range & 255 .. range >> 8
+    const uint32_t ring = ((sptr(smem) + 511) & ~511u) + (uint32_t)(warp * S * T::kStage);
+    struct Look { int id[NB], in[NB], head, range, b, p0; };                     // rows range & 255 .. range >> 8
     Cursor<POS> is = seg;
     is.advance(p, units, warp + lane * W);
     Look now{};
@@ -242,68 +241,70 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
             w.head = p.chunks == 1 ? is.u : is.u / p.chunks;
             const int lo = max(is.start - p0, 0), hi = min(is.len - p0, POS);    // hi <= 0: an empty sequence
             w.range = lo | max(hi, 0) << 8;
+            w.b = is.b;
+            w.p0 = p0;
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
                 const int pos = p0 + 16 * n;
-                if (p.whole_blocks) {
-                    const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-                    w.in[n] = pos - pg * p.page_size;
-                    w.id[n] = 0;
-                    if (16 * n < hi && 16 * n + 16 > lo) w.id[n] = __ldg(p.table + is.b * p.table_batch + pg);
-                } else {
-                    w.id[n] = is.b;
-                    w.in[n] = pos;
-                }
+                const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
+                w.in[n] = pos - pg * p.page_size;
+                w.id[n] = -1;
+                if (p.whole_blocks && w.range == POS << 8) w.id[n] = __ldg(p.table + is.b * p.table_batch + pg);
             }
         }
         return w;
     };
+    // a lane's part of a tile in shared memory: chunk lchunk of rows lrow, lrow + kStep, ...; the swizzle repeats every 8 rows
+    constexpr int kIters = (POS * T::kChunks + 31) / 32;
+    constexpr bool kEven = 32 % T::kChunks == 0;
+    constexpr int kStep = kEven ? 32 / T::kChunks : 1, kOff = kEven ? (kStep < 8 ? 8 / kStep : 1) : kIters;
+    const int lrow = lane / T::kChunks, lchunk = lane % T::kChunks;
+    uint32_t off[kOff];
+#pragma unroll
+    for (int i = 0; i < kOff; ++i)
+        off[i] = kEven ? T::at(lrow + i * kStep, lchunk) : T::at((lane + 32 * i) / T::kChunks, (lane + 32 * i) % T::kChunks);
     auto fetch = [&]() {
         const int src = fetched & 31, head = __shfl_sync(~0u, now.head, src), range = __shfl_sync(~0u, now.range, src);
-        const int lo = range & 255, hi = range >> 8;
         const uint32_t kd = ring + fill * T::kStage, vd = kd + T::kMat;
-        constexpr int kIters = (POS * T::kChunks + 31) / 32;
-        if (p.whole_blocks) {
-            const uint8_t *kb[NB], *vb[NB];
-            bool bad[NB];
+        const uint8_t *kb[NB], *vb[NB];
+        bool fast = p.whole_blocks && range == POS << 8;                         // a whole tile in pages that exist
 #pragma unroll
-            for (int n = 0; n < NB; ++n) {
-                int id = __shfl_sync(~0u, now.id[n], src);
-                const int in = __shfl_sync(~0u, now.in[n], src);
-                bad[n] = (unsigned)id >= (unsigned)p.num_pages;
-                if (bad[n]) {
-                    serve_error(kErrPage);
-                    id = 0;
+        for (int n = 0; n < NB; ++n) {
+            const int id = __shfl_sync(~0u, now.id[n], src), in = __shfl_sync(~0u, now.in[n], src);
+            fast = fast && (unsigned)id < (unsigned)p.num_pages;
+            kb[n] = p.k + id * p.k_page + in * p.k_token + head * p.k_head;
+            vb[n] = p.v + id * p.v_page + in * p.v_token + head * p.v_head;
+        }
+        if (fast) {
+            const unsigned kt = (unsigned)p.k_token, vt = (unsigned)p.v_token;
+            if constexpr (kEven) {
+                const unsigned long long lk = (unsigned long long)lrow * kt + lchunk * 16;
+                const unsigned long long lv = (unsigned long long)lrow * vt + lchunk * 16;
+#pragma unroll
+                for (int n = 0; n < NB; ++n) {
+                    kb[n] += lk;
+                    vb[n] += lv;
                 }
-                kb[n] = p.k + id * p.k_page + in * p.k_token + head * p.k_head;
-                vb[n] = p.v + id * p.v_page + in * p.v_token + head * p.v_head;
-            }
-            if constexpr (32 % T::kChunks == 0) {
-                constexpr int kStep = 32 / T::kChunks;                           // rows per pass of the warp
-                const int row0 = lane / T::kChunks, c = lane % T::kChunks;
-                const long long lane_k = row0 * p.k_token + c * 16, lane_v = row0 * p.v_token + c * 16;
 #pragma unroll
                 for (int i = 0; i < kIters; ++i) {
-                    const int row = row0 + i * kStep, n = i * kStep / 16;
-                    const bool in = row >= lo && row < hi && !bad[n];
-                    const int bytes = in ? 16 : 0;
-                    cp16(kd + T::at(row, c), in ? kb[n] + lane_k + (i * kStep - 16 * n) * p.k_token : p.k, bytes);
-                    cp16(vd + T::at(row, c), in ? vb[n] + lane_v + (i * kStep - 16 * n) * p.v_token : p.v, bytes);
+                    const int n = i * kStep / 16;
+                    const unsigned rows_on = i * kStep - 16 * n;
+                    const uint32_t at = off[i % kOff] + i / kOff * 8 * T::kRow;
+                    cp16(kd + at, kb[n] + (unsigned long long)rows_on * kt);
+                    cp16(vd + at, vb[n] + (unsigned long long)rows_on * vt);
                 }
             } else {
 #pragma unroll
                 for (int i = 0; i < kIters; ++i) {
                     const int e = lane + 32 * i, row = e / T::kChunks, c = e % T::kChunks, n = NB == 1 ? 0 : row >> 4;
-                    const bool in = row >= lo && row < hi && !(n ? bad[NB - 1] : bad[0]);
-                    const int r = row & 15, bytes = in ? 16 : 0;
-                    cp16(kd + T::at(row, c), in ? (n ? kb[NB - 1] : kb[0]) + r * p.k_token + c * 16 : p.k, bytes);
-                    cp16(vd + T::at(row, c), in ? (n ? vb[NB - 1] : vb[0]) + r * p.v_token + c * 16 : p.v, bytes);
+                    cp16(kd + off[i], (n ? kb[NB - 1] : kb[0]) + (unsigned long long)(row & 15) * kt + c * 16);
+                    cp16(vd + off[i], (n ? vb[NB - 1] : vb[0]) + (unsigned long long)(row & 15) * vt + c * 16);
                 }
             }
         } else {
-            // any page size: lane r looks up row r's page here
-            const int b = __shfl_sync(~0u, now.id[0], src), p0 = __shfl_sync(~0u, now.in[0], src), r = lane % POS;
-            bool ok = r >= lo && r < hi;
+            // the ends of a sequence, any page size, pages that do not exist: lane r looks up row r's page here
+            const int b = __shfl_sync(~0u, now.b, src), p0 = __shfl_sync(~0u, now.p0, src), r = lane % POS;
+            bool ok = r >= (range & 255) && r < range >> 8;
             long long ko = 0, vo = 0;
             if (ok) {
                 const int pos = p0 + r, pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
@@ -555,25 +556,28 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
         float s[2 * NB][4];
 #pragma unroll
         for (int n = 0; n < 2 * NB; ++n) s[n][0] = s[n][1] = s[n][2] = s[n][3] = 0.f;
+        // The stage is aligned to the row size, so a fixed step along a row is an XOR of the lane's address.
         if constexpr (FMT == 0) {
+            const uint32_t ka = kd + T::at((lane & 7) + (lane >> 4) * 8, (lane >> 3) & 1);
 #pragma unroll
             for (int ks = 0; ks < KS; ++ks) {
 #pragma unroll
                 for (int n = 0; n < NB; ++n) {
                     uint32_t r[4];
-                    ldsm4(kd + T::at(16 * n + (lane & 7) + (lane >> 4) * 8, 2 * ks + ((lane >> 3) & 1)), r);
+                    ldsm4((ka ^ ks << 5) + 16 * n * T::kRow, r);
                     const uint32_t a1 = ROWS == 8 ? 0u : qa[ks][1], a3 = ROWS == 8 ? 0u : qa[ks][QR - 1];
                     mma_bf16(s[2 * n], qa[ks][0], a1, qa[ks][QR / 2], a3, r[0], r[1]);
                     mma_bf16(s[2 * n + 1], qa[ks][0], a1, qa[ks][QR / 2], a3, r[2], r[3]);
                 }
             }
         } else {
+            const uint32_t ka = kd + g * T::kRow + (F8::k_byte(0, t) ^ T::key(g));
 #pragma unroll
             for (int u = 0; u < KS / F8::VK; ++u) {
 #pragma unroll
                 for (int n = 0; n < 2 * NB; ++n) {
                     uint32_t w[F8::VK];
-                    lds_words<F8::VK>(kd + (8 * n + g) * T::kRow, T::key(g), F8::k_byte(u * F8::VK, t), w);
+                    lds_words<F8::VK>((ka ^ F8::k_byte(u * F8::VK, 0)) + 8 * n * T::kRow, w);
 #pragma unroll
                     for (int i = 0; i < F8::VK; ++i) {
                         const int ks = u * F8::VK + i;
@@ -598,10 +602,16 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
 #pragma unroll
             for (int i = 0; i < 4 * NB; ++i) {
                 x[i] = s[i >> 1][2 * h + (i & 1)] * qscale[h];
-                const int pos = p0 + (i >> 1) * 8 + 2 * t + (i & 1);
-                if (edge && (pos < seg.start || pos >= seg.len)) x[i] = -INFINITY;
-                top = fmaxf(top, x[i]);
             }
+            if (edge) {
+#pragma unroll
+                for (int i = 0; i < 4 * NB; ++i) {
+                    const int pos = p0 + (i >> 1) * 8 + 2 * t + (i & 1);
+                    if (pos < seg.start || pos >= seg.len) x[i] = -INFINITY;
+                }
+            }
+#pragma unroll
+            for (int i = 0; i < 4 * NB; ++i) top = fmaxf(top, x[i]);
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
             if (top > m[h]) {
@@ -652,12 +662,13 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
         }
         // ---- O += P V
         if (FMT == 0) {
+            const uint32_t va = vd + T::at((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
 #pragma unroll
                 for (int j = 0; j < NT; j += 2) {
                     uint32_t r[4];
-                    ldsm4t(vd + T::at(16 * n + (lane & 7) + ((lane >> 3) & 1) * 8, j + (lane >> 4)), r);
+                    ldsm4t((va ^ j << 4) + 16 * n * T::kRow, r);
                     mma_bf16(acc[j], pa[n][0], pa[n][1], pa[n][2], pa[n][3], r[0], r[1]);
                     mma_bf16(acc[j + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], r[2], r[3]);
                     if (ROWS != 8) {
@@ -667,16 +678,16 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 }
             }
         } else {
+            // rows 2 t and 2 t + 1; 8 on the swizzle is the same
+            const uint32_t va[2] = {vd + 2 * t * T::kRow + (F8::v_unit(0, g) ^ T::key(2 * t)),
+                                    vd + (2 * t + 1) * T::kRow + (F8::v_unit(0, g) ^ T::key(2 * t + 1))};
 #pragma unroll
             for (int n = 0; n < NB; ++n) {
 #pragma unroll
                 for (int u = 0; u < NT / F8::UV; ++u) {
                     uint32_t w[4][F8::UV / 4];                               // of the lane's four positions
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const int row = 2 * t + (i & 1) + 8 * (i >> 1);
-                        lds_words<F8::UV / 4>(vd + (16 * n + row) * T::kRow, T::key(row), F8::v_unit(u, g), w[i]);
-                    }
+                    for (int i = 0; i < 4; ++i) lds_words<F8::UV / 4>((va[i & 1] ^ F8::v_unit(u, 0)) + (16 * n + 8 * (i >> 1)) * T::kRow, w[i]);
 #pragma unroll
                     for (int q = 0; q < F8::UV / 4; ++q)
 #pragma unroll
@@ -788,7 +799,8 @@ extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
     p.page_size = a->page_size;
     p.max_pages = a->max_pages;
     p.window = a->window;
-    p.whole_blocks = a->page_size % 16 == 0;
+    const long long far = 1ll << 27;
+    p.whole_blocks = a->page_size % 16 == 0 && p.k_token >= 0 && p.k_token < far && p.v_token >= 0 && p.v_token < far;
     p.page_shift = (a->page_size & (a->page_size - 1)) == 0 ? ilog2(a->page_size) : -1;
     p.scale_log2 = a->scale * 1.4426950408889634f;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
