@@ -338,7 +338,9 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
 
     // ---- One loop, so that the fetch and the end of a part are in the code once: step `it` fetches the warp's tile `it`
     // and works on tile it - (S - 1), after ending the parts (of units) that lie before it.
-    // The next unit's queries are loaded a unit ahead: behind a full ring a load takes as long as the ring's copies.
+    // The next unit's queries are loaded a unit ahead: behind a full ring a load takes as long as the ring's copies. (At
+    // head_dim 256 there are no registers for that.)
+    constexpr bool kAhead = HD < 256;
     uint32_t qa[KS][QR], qn[KS][QR];
     auto load_q = [&](int b, int u) {
         const int hd = p.chunks == 1 ? u : u / p.chunks, r0 = (u - hd * p.chunks) * ROWS, n = min(ROWS, p.group - r0);
@@ -368,7 +370,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
         if (!(it & 31) && fetched == it) {
             if (it) is.advance(p, units, 32 * W);
             now = look();
-            if (!it) load_q(seg.b, seg.u);                                       // while the page ids come in
+            if (kAhead && !it) load_q(seg.b, seg.u);                             // while the page ids come in
         }
         if (fetched < known) fetch();
         cp_commit();
@@ -509,11 +511,12 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
             nrow = min(ROWS, p.group - row0);
             // the query heads of this unit as A fragments; those of the next one are on their way
             qscale[0] = qscale[1] = p.scale_log2;
+            if (!kAhead) load_q(seg.b, seg.u);
 #pragma unroll
             for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int i = 0; i < QR; ++i) qa[s][i] = qn[s][i];
-            if (seg.unit_place() + seg.ntile + kUnitCost < t1)
+            if (kAhead && seg.unit_place() + seg.ntile + kUnitCost < t1)
                 load_q(seg.u + 1 < units ? seg.b : seg.b + 1, seg.u + 1 < units ? seg.u + 1 : 0);
             if (FMT == 1) {
 #pragma unroll
@@ -718,17 +721,14 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
     return serve_launch(fn, p, dim3((unsigned)grid), W * 32, smem, st);
 }
 
-// Four warps per CTA; the ring takes what the merge buffer leaves: two CTAs per SM where 96 KB of ring each is enough
-// (head_dim up to 128, up to 8 heads per unit), else one.
+// Four warps per CTA, two CTAs per SM (head_dim 256: one, its sums fill the registers), two stages per warp: one tile
+// (8 KB, 16 KB at head_dim 256) in flight while one is worked on. Three stages are slower: 1 x 128k 90.2 us against 86.0,
+// 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us.
 template <int HD>
 int pick_attn(const AttnParams& p, int fmt, cudaStream_t st) {
-    constexpr int W = 4, kB = W * AttnTile<HD, 0>::kStage, kQ = W * AttnTile<HD, 1>::kStage;
-    constexpr auto deep = [](int s) { return s > 12 ? 12 : s; };
-    if (p.group <= 8)
-        return fmt == 0 ? launch_attn<HD, 0, 8, W, deep((HD == 256 ? 196608 : 98304) / kB), HD == 256 ? 1 : 2>(p, st)
-                        : launch_attn<HD, 1, 8, W, deep((HD == 256 ? 196608 : 98304) / kQ), HD == 256 ? 1 : 2>(p, st);
-    return fmt == 0 ? launch_attn<HD, 0, 16, W, deep((HD == 256 ? 131072 : 196608) / kB), 1>(p, st)
-                    : launch_attn<HD, 1, 16, W, deep((HD == 256 ? 131072 : 196608) / kQ), 1>(p, st);
+    constexpr int W = 4, S = 2, B = HD == 256 ? 1 : 2;
+    if (p.group <= 8) return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B>(p, st) : launch_attn<HD, 1, 8, W, S, B>(p, st);
+    return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
 }
 
 bool attn_sizes(int heads, int kv_heads, int head_dim) {
