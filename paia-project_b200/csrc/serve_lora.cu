@@ -125,17 +125,46 @@ __device__ __forceinline__ void lora_shrink(float* parts, const __nv_bfloat16* x
         }
 }
 
-// The warp's groups of 32 columns: out = base + B t, U groups at a time, all their loads in flight together. WS: steps of
-// 32 ranks; ONCE: these are all, and t stays in registers. Rows of B behind the last are read as the last (their results
-// are not stored), ranks behind the last as zeros.
-template <int WS, int NT, bool ONCE>
+// What a lane loads of a row of B: V is 16 bytes (of 32 ranks), 8 (of 16) or 4 (of 8), two or one steps of the MMA.
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, bool in, uint4& v) {
+    v = in ? *reinterpret_cast<const uint4*>(p) : make_uint4(0, 0, 0, 0);
+}
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, bool in, uint2& v) {
+    v = in ? *reinterpret_cast<const uint2*>(p) : make_uint2(0, 0);
+}
+__device__ __forceinline__ void load_row(const __nv_bfloat16* p, bool in, uint32_t& v) {
+    v = in ? *reinterpret_cast<const uint32_t*>(p) : 0u;
+}
+__device__ __forceinline__ void cut_row(uint4& v, int n) { v = first_of(v, n); }
+__device__ __forceinline__ void cut_row(uint2& v, int n) {
+    const uint4 w = first_of(make_uint4(v.x, v.y, 0, 0), n);
+    v = make_uint2(w.x, w.y);
+}
+__device__ __forceinline__ void cut_row(uint32_t& v, int n) { v = first_of(make_uint4(v, 0, 0, 0), n).x; }
+// d += [a; c] B: rows g from a, g + 8 from c
+__device__ __forceinline__ void mma_row(float d[4], const uint4& a, const uint4& c, const uint4& b) {
+    mma_bf16(d, a.x, c.x, a.y, c.y, b.x, b.y);
+    mma_bf16(d, a.z, c.z, a.w, c.w, b.z, b.w);
+}
+__device__ __forceinline__ void mma_row(float d[4], const uint2& a, const uint2& c, const uint2& b) {
+    mma_bf16(d, a.x, c.x, a.y, c.y, b.x, b.y);
+}
+__device__ __forceinline__ void mma_row(float d[4], const uint32_t& a, const uint32_t& c, const uint32_t& b) {
+    mma_bf16(d, a, c, 0u, 0u, b, 0u);
+}
+
+// The warp's groups of 32 columns: out = base + B t, U groups at a time, all their loads in flight together (16 bytes of
+// each row per lane would leave three lanes of four idle at rank 8, hence the narrower ones). WS: steps of 2 sizeof(V)
+// ranks; ONCE: these are all, and t stays in registers. Rows of B behind the last are read as the last (their results are
+// not stored), ranks behind the last as zeros.
+template <class V, int WS, int U, int NT, bool ONCE>
 __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bfloat16* B, const __nv_bfloat16* t_hi,
                                             const __nv_bfloat16* t_lo, int stride, const int* sh_rows, int rows, int rank,
                                             int g0, int g1, int warp, int g, int t) {
-    constexpr int U = WS == 1 ? 2 : 1;
+    constexpr int L = sizeof(V) / 2, R = 4 * L;                                  // ranks per lane and step, per step
     const uint4 zero = make_uint4(0, 0, 0, 0);
     const int cols = 8 * (g >> 1) + (g & 1);                                     // the lane's column of tile j: + 2 j
-    const bool base_in = p.base != nullptr, ragged = rank & 7;
+    const bool base_in = p.base != nullptr, ragged = rank % L;
     const __nv_bfloat16* base[NT];
     __nv_bfloat16* out[NT];
     bool in[NT];
@@ -146,15 +175,15 @@ __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bflo
         base[h] = p.base + m * p.base_row + 8 * t;
         out[h] = p.out + m * p.out_row + 8 * t;
     }
-    uint4 th[WS][2 * NT];                                                        // hi (and lo) of rows g, g + 8
+    V th[WS][2 * NT];                                                            // hi (and lo) of rows g, g + 8
     auto load_t = [&](int k0) {
 #pragma unroll
         for (int s = 0; s < WS; ++s)
 #pragma unroll
             for (int h = 0; h < NT; ++h) {
-                const int at = (g + 8 * h) * stride + k0 + 32 * s + 8 * t;
-                th[s][h] = k0 + 32 * s < rank ? load16(t_hi + at) : zero;
-                th[s][NT + h] = k0 + 32 * s < rank ? load16(t_lo + at) : zero;
+                const int at = (g + 8 * h) * stride + k0 + R * s + L * t;
+                load_row(t_hi + at, k0 + R * s < rank, th[s][h]);
+                load_row(t_lo + at, k0 + R * s < rank, th[s][NT + h]);
             }
     };
     if (ONCE && rank) load_t(0);
@@ -168,50 +197,47 @@ __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bflo
 #pragma unroll
             for (int h = 0; h < NT; ++h) bs[u][h] = ok && in[h] ? load16(base[h] + n0) : zero;
         }
-        float acc[U][4][4];
-#pragma unroll
-        for (int u = 0; u < U; ++u)
-#pragma unroll
-            for (int j = 0; j < 4; ++j) acc[u][j][0] = acc[u][j][1] = acc[u][j][2] = acc[u][j][3] = 0.f;
-#pragma unroll 1
-        for (int k0 = 0; k0 < rank; k0 += 32 * WS) {
-            uint4 w[U][WS][4];
+        V w[U][WS][4];
+        auto load_b = [&](int k0) {
 #pragma unroll
             for (int u = 0; u < U; ++u)
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int n = min((grp + u * kLoraWarps) * 32 + cols + 2 * j, p.N - 1);
-                    const __nv_bfloat16* row = B + (long long)n * p.b_row + k0 + 8 * t;
+                    const __nv_bfloat16* row = B + (long long)n * p.b_row + k0 + L * t;
 #pragma unroll
-                    for (int s = 0; s < WS; ++s) w[u][s][j] = k0 + 32 * s + 8 * t < rank ? load16(row + 32 * s) : zero;
+                    for (int s = 0; s < WS; ++s)
+                        load_row(row + R * s, grp + u * kLoraWarps < g1 && k0 + R * s + L * t < rank, w[u][s][j]);
                 }
-            if (!ONCE) load_t(k0);
-            if (ragged) {
+        };
+        if (ONCE) load_b(0);
 #pragma unroll
-                for (int u = 0; u < U; ++u)
+        for (int u = 0; u < U; ++u) {
+            float acc[4][4];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+#pragma unroll 1
+            for (int k0 = 0; k0 < rank; k0 += R * WS) {
+                if (!ONCE) {
+                    static_assert(ONCE || U == 1, "sums of one group are kept over the rounds");
+                    load_b(k0);
+                    load_t(k0);
+                }
+                if (ragged) {
 #pragma unroll
                     for (int s = 0; s < WS; ++s)
 #pragma unroll
-                        for (int j = 0; j < 4; ++j) w[u][s][j] = first_of(w[u][s][j], rank - k0 - 32 * s - 8 * t);
-            }
+                        for (int j = 0; j < 4; ++j) cut_row(w[u][s][j], rank - k0 - R * s - L * t);
+                }
 #pragma unroll
-            for (int s = 0; s < WS; ++s)
-#pragma unroll
-                for (int u = 0; u < U; ++u)
+                for (int s = 0; s < WS; ++s)
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
-                        const uint4 b = w[u][s][j], h0 = th[s][0], h1 = th[s][1];        // one row set: hi over lo
-                        mma_bf16(acc[u][j], h0.x, h1.x, h0.y, h1.y, b.x, b.y);
-                        mma_bf16(acc[u][j], h0.z, h1.z, h0.w, h1.w, b.z, b.w);
-                        if (NT == 2) {
-                            const uint4 l0 = th[s][2 * NT - 2], l1 = th[s][2 * NT - 1];
-                            mma_bf16(acc[u][j], l0.x, l1.x, l0.y, l1.y, b.x, b.y);
-                            mma_bf16(acc[u][j], l0.z, l1.z, l0.w, l1.w, b.z, b.w);
-                        }
+                        mma_row(acc[j], th[s][0], th[s][1], w[u][s][j]);         // one row set: hi over lo; two: hi, then lo
+                        if (NT == 2) mma_row(acc[j], th[s][2 * NT - 2], th[s][2 * NT - 1], w[u][s][j]);
                     }
-        }
-#pragma unroll
-        for (int u = 0; u < U; ++u) {
+                if (ONCE) break;
+            }
             const int n0 = (grp + u * kLoraWarps) * 32;
             if (grp + u * kLoraWarps >= g1 || n0 + 8 * t >= p.N) continue;
 #pragma unroll
@@ -221,7 +247,7 @@ __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bflo
                 uint32_t o[4];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
-                    const float* a = acc[u][j];
+                    const float* a = acc[j];
                     const float v0 = NT == 2 ? a[2 * h] : a[0] + a[2], v1 = NT == 2 ? a[2 * h + 1] : a[1] + a[3];
                     o[j] = pack_bf16(v0 + bf16_lo(b[j]), v1 + bf16_hi(b[j]));
                 }
@@ -416,16 +442,17 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
         asm volatile("barrier.cluster.wait;" ::: "memory");
     }
     // ---- columns
-    if (rank <= 32) {
-        if (wide) lora_expand<1, 2, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
-        else lora_expand<1, 1, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
-    } else if (rank <= 64) {
-        if (wide) lora_expand<2, 2, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
-        else lora_expand<2, 1, true>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
-    } else {
-        if (wide) lora_expand<2, 2, false>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
-        else lora_expand<2, 1, false>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);
-    }
+#define EXPAND(V, WS, U1, U2, ONCE)                                                                                       \
+    do {                                                                                                                  \
+        if (wide) lora_expand<V, WS, U2, 2, ONCE>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);     \
+        else lora_expand<V, WS, U1, 1, ONCE>(p, B, t_hi, t_lo, stride, sh_rows, rows, rank, g0, g1, warp, g, t);          \
+    } while (0)
+    if (rank <= 8) EXPAND(uint32_t, 1, 6, 4, true);
+    else if (rank <= 16) EXPAND(uint2, 1, 4, 3, true);
+    else if (rank <= 32) EXPAND(uint4, 1, 3, 2, true);
+    else if (rank <= 64) EXPAND(uint4, 2, 2, 1, true);
+    else EXPAND(uint4, 2, 1, 1, false);
+#undef EXPAND
 }
 
 }  // namespace
