@@ -225,8 +225,9 @@ int paia_gemv_plan_destroy(paia_gemv_plan* plan);
  * read. A page id outside [0, num_pages) (code 10) reads as zero rows, a length above max_pages page_size is cut to it
  * and one below 0 is 0 (code 11).
  * q, out bf16; cache bf16 or e4m3 with a fp32 scale per kv head (value = stored * scale). head_dim 64, 96, 128 or 256;
- * any page size and page / token / head strides (both [page][token][head] and [page][head][token] caches). q, k and v
- * 16-byte aligned with strides of whole 16 bytes, out 8-byte aligned with strides of multiples of 4 elements. `workspace`:
+ * any page size and page / token / head strides (both [page][token][head] and [page][head][token] caches);
+ * batch * kv_heads * max_pages * page_size / 16 (times the 16-head units of a larger group) below 2^32. q, k and v 16-byte
+ * aligned with strides of whole 16 bytes, out 8-byte aligned with strides of multiples of 4 elements. `workspace`:
  * paia_gemv_paged_attn_workspace(heads, kv_heads, head_dim) bytes on the launch's device, 16-byte aligned, zeroed once;
  * every launch leaves it ready for the next, of any batch; launches that may overlap on the GPU (other streams, graphs
  * replayed at the same time) need a workspace each. */

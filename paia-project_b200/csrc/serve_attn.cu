@@ -767,6 +767,8 @@ extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
         a->v_page % unit || a->v_token % unit || a->v_head % unit)
         return -2;
     if (a->cache == 0 && (a->k_scale || a->v_scale)) return -2;
+    // outputs that would fall on one another
+    if ((a->heads > 1 && a->out_head == 0) || (a->batch > 1 && (a->out_batch == 0 || (a->lse && a->lse_batch == 0)))) return -2;
     // positions and the list's places are counted in 32 bits
     const long long cap = (long long)a->max_pages * a->page_size;
     const int group = a->heads / a->kv_heads, chunks = (group + 15) / 16;

@@ -410,6 +410,13 @@ extern "C" int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* str
         a->q_head % 8 || a->ko_token % 8 || a->ko_head % 8 || a->k_page % unit || a->k_row % unit || a->k_head % unit ||
         a->v_page % unit || a->v_row % unit || a->v_head % unit)
         return -2;
+    // outputs that would fall on one another
+    if ((a->heads > 1 && a->q_head == 0) || (a->tokens > 1 && a->q_token == 0) ||
+        (a->k_out && ((a->kv_heads > 1 && a->ko_head == 0) || (a->tokens > 1 && a->ko_token == 0))) ||
+        (a->k && ((a->kv_heads > 1 && (a->k_head == 0 || a->v_head == 0)) ||
+                  (a->page_size > 1 && (a->k_row == 0 || a->v_row == 0)) ||
+                  (a->num_pages > 1 && (a->k_page == 0 || a->v_page == 0)))))
+        return -2;
     RopeParams p{};
     p.qkv = static_cast<const __nv_bfloat16*>(a->qkv);
     p.pos = a->pos;

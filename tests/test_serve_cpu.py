@@ -1,5 +1,7 @@
 """CPU (no GPU needed): the serving operators' C structs as paia_gemv.serve packs them, their refusals on the host (code
--2 before any device is touched) and the checks of the tensor wrappers (ValueError)."""
+-2 before any device is touched), the checks of the tensor wrappers (ValueError), and a replay of the attention's division
+of work and of the adapters' finding of their rows."""
+import random
 import re
 import subprocess
 from pathlib import Path
@@ -75,7 +77,8 @@ def test_structs_match_the_header(tmp_path):
     dict(workspace=PTR + 4), dict(out=PTR + 4), dict(lse=PTR + 2), dict(lens=PTR + 2), dict(page_table=PTR + 1),
     dict(q_batch=1020), dict(q_head=130), dict(out_head=127), dict(k_token=260), dict(v_page=4100), dict(k_head=129),
     dict(k_scale=PTR), dict(v_scale=PTR), dict(cache=1, k_token=264), dict(cache=1, k_scale=PTR + 1),
-    dict(page_size=65536, max_pages=65536)])
+    dict(page_size=65536, max_pages=65536), dict(batch=1 << 20, max_pages=1 << 16), dict(out_head=0), dict(out_batch=0),
+    dict(lse=PTR, lse_batch=0)])
 def test_attention_refusals(L, change):
     from paia_gemv import serve
     assert L._lib.paia_gemv_paged_attn(packed("paia_gemv_attn", serve.ATTN, ATTN, **change), None) == -2
@@ -88,7 +91,8 @@ def test_attention_refusals(L, change):
     dict(num_pages=0), dict(page_size=0), dict(max_pages=0), dict(k_scale=PTR), dict(qkv=PTR + 2), dict(q_out=PTR + 8),
     dict(k=PTR + 8), dict(k_out=PTR + 4), dict(q_norm=PTR + 4), dict(inv_freq=PTR + 4), dict(pos=PTR + 2),
     dict(qkv_token=1537), dict(q_token=4), dict(q_head=12), dict(ko_token=4), dict(k_row=260), dict(v_head=3),
-    dict(cache=1, v_row=264)])
+    dict(cache=1, v_row=264), dict(q_head=0), dict(q_token=0), dict(k_head=0), dict(v_row=0), dict(k_page=0),
+    dict(k_out=PTR, ko_head=0, ko_token=256), dict(k_out=PTR, ko_head=128, ko_token=0)])
 def test_rope_refusals(L, change):
     from paia_gemv import serve
     args = packed("paia_gemv_rope_cache", serve.ROPE_CACHE, ROPE, **change)
@@ -100,7 +104,7 @@ def test_rope_refusals(L, change):
     dict(adapters=0), dict(adapters=8193), dict(x=0), dict(a=0), dict(b=0), dict(adapter=0), dict(out=0), dict(x=PTR + 8),
     dict(a=PTR + 2), dict(b=PTR + 4), dict(base=PTR + 8), dict(out=PTR + 8), dict(adapter=PTR + 2), dict(ranks=PTR + 1),
     dict(scaling=PTR + 2), dict(x_row=65), dict(base_row=4), dict(out_row=68), dict(a_adapter=4), dict(a_row=66),
-    dict(b_adapter=2), dict(b_row=12)])
+    dict(b_adapter=2), dict(b_row=12), dict(out_row=0)])
 def test_lora_refusals(L, change):
     from paia_gemv import serve
     assert L._lib.paia_gemv_lora(packed("paia_gemv_lora_args", serve.LORA, LORA, **change), None) == -2
@@ -215,3 +219,104 @@ def test_wrapper_checks(monkeypatch):
                 dict(scaling=z(2)), dict(ranks=z(2, dtype=f32)), dict(out=z(40, 3).t())):
         with pytest.raises(ValueError):
             serve.lora(rec, **dict(good, **bad))
+
+
+def attention_division(lens, units, pos, grid, warps, cost, window):
+    """What each CTA of serve_attn.cu works on: {cta: [(sequence, unit, first tile, tiles of the part, tiles of the unit,
+    c0, c1)]}, as the kernel finds it."""
+    def tiles(n):
+        start = n - window if window and n > window else 0
+        return max(1, (n + pos - 1) // pos - start // pos)
+
+    each = [tiles(n) + cost for n in lens]
+    total = sum(each) * units
+    per = max(-(-total // grid), warps)
+    out = {}
+    for cta in range(grid):
+        if per * cta >= total:
+            continue
+        t0 = per * cta
+        t1 = t0 + min(total - t0, per)
+        b, before = 0, 0
+        while t0 >= (before + each[b]) * units:
+            before += each[b]
+            b += 1
+        w0 = before * units
+        u, tile = divmod(t0 - w0, each[b])
+        n = each[b] - cost
+
+        def following(b, u, w0):
+            if u + 1 < units:
+                return b, u + 1, w0
+            return b + 1, 0, w0 + each[b] * units
+
+        if tile >= n:                                           # behind its unit's tiles
+            b, u, w0 = following(b, u, w0)
+            tile = 0
+            if b == len(lens) or w0 + u * each[b] >= t1:
+                continue
+        while True:
+            n, place = each[b] - cost, w0 + u * each[b]
+            part = min(n, t1 - place) - tile
+            assert part > 0
+            out.setdefault(cta, []).append((b, u, tile, part, n, place // per, (place + n - 1) // per))
+            if place + each[b] >= t1:
+                break
+            b, u, w0 = following(b, u, w0)
+            tile = 0
+    return out
+
+
+def test_attention_division_covers_every_tile_once():
+    """Every tile of every unit belongs to one CTA; a unit in parts is counted in by exactly the CTAs c0 .. c1, the counter
+    of c0 and each CTA's two slots of the workspace serve one unit each."""
+    src = (ROOT / "paia-project_b200" / "csrc" / "serve_attn.cu").read_text()
+    cost = int(re.search(r"kUnitCost = (\d+);", src).group(1))
+    rng = random.Random(4)
+    for trial in range(300):
+        lens = [rng.choice([0, 1, rng.randrange(40), rng.randrange(3000)]) for _ in range(rng.choice([1, 2, 7, 40, 90]))]
+        units, pos, grid = rng.choice([1, 2, 8, 13]), rng.choice([16, 32]), rng.choice([1, 5, 148, 296])
+        window = rng.choice([0, 0, 1, 100])
+        work = attention_division(lens, units, pos, grid, 4, cost, window)
+        seen, arrivals, counters, slots = {}, {}, {}, {}
+        for cta, parts in work.items():
+            for b, u, tile, part, n, c0, c1 in parts:
+                for i in range(tile, tile + part):
+                    assert seen.setdefault((b, u, i), cta) == cta
+                if part < n:
+                    arrivals.setdefault((b, u, c0, c1), []).append(cta)
+                    assert counters.setdefault(c0, (b, u)) == (b, u)
+                    slot = (cta, 1 if tile == 0 else 0)
+                    assert slots.setdefault(slot, (b, u)) == (b, u)
+                    assert slot[1] == (1 if cta == c0 else 0)   # where the join looks for it
+                else:
+                    assert c0 == c1 == cta or c0 <= cta <= c1
+        for b, n in enumerate(lens):
+            start = n - window if window and n > window else 0
+            count = max(1, (n + pos - 1) // pos - start // pos)
+            for u in range(units):
+                assert all((b, u, i) in seen for i in range(count)) and (b, u, count) not in seen
+        for (b, u, c0, c1), ctas in arrivals.items():
+            assert sorted(ctas) == list(range(c0, c1 + 1)), (lens, b, u)
+
+
+def test_adapter_items_cover_every_row_once():
+    """The number of clusters that the host launches is enough for any assignment of rows, and the items of up to 16 rows
+    (by order of the row that begins them, or by adapter beyond 256 rows) hold every row once."""
+    rng = random.Random(5)
+    for trial in range(200):
+        adapters = rng.choice([1, 2, 5, 60, 500])
+        m = rng.choice([1, 3, 16, 17, 100, 256, 257, 700])
+        ids = [rng.choice([rng.randrange(adapters), adapters, 0]) for _ in range(m)]
+        kinds = min(m, adapters + 1)
+        items = (m + 15 * kinds) // 16
+        at = [sum(ids[j] == ids[i] for j in range(i)) for i in range(m)]
+        if m <= 256:
+            begins = [i for i in range(m) if at[i] % 16 == 0]
+            rows = [[i for i in range(m) if ids[i] == ids[s] and at[s] <= at[i] < at[s] + 16] for s in begins]
+        else:
+            rows = []
+            for a in range(adapters + 1):
+                mine = [i for i in range(m) if ids[i] == a]
+                rows += [mine[k:k + 16] for k in range(0, len(mine), 16)]
+        assert len(rows) <= items and sorted(i for r in rows for i in r) == list(range(m))
