@@ -123,9 +123,12 @@ class GemvLib:
         lib.paia_gemv_int4_asym_variant_count.restype = I
         lib.paia_gemv_variant_info_ex.restype = I
         lib.paia_gemv_variant_info_ex.argtypes = [I, I, ctypes.POINTER(VariantEx)]
-        for name in ("paia_gemv_paged_attn", "paia_gemv_qkv_rope_cache", "paia_gemv_lora"):
-            getattr(lib, name).restype = I
-            getattr(lib, name).argtypes = [P, P]
+        # serving operators (paia_gemv.serve drives these): the bytes of the C struct and the stream; the return code
+        for name in ("paged_attn", "qkv_rope_cache", "lora"):
+            fn = getattr(lib, "paia_gemv_" + name)
+            fn.restype = I
+            fn.argtypes = [P, P]
+            setattr(self, name, fn)
         lib.paia_gemv_paged_attn_workspace.restype = ctypes.c_size_t
         lib.paia_gemv_paged_attn_workspace.argtypes = [I, I, I]
         lib.paia_gemv_device_error.restype = I
@@ -323,29 +326,13 @@ class GemvLib:
     def plan_destroy(self, plan):
         self._check(self._lib.paia_gemv_plan_destroy(plan), "paia_gemv_plan_destroy")
 
-    # --- serving operators (paia_gemv.serve drives these); args: the bytes of the C struct of the same name, in its
-    # field order (serve.ATTN, serve.ROPE_CACHE, serve.LORA pack them)
+    # --- serving operators (paged_attn, qkv_rope_cache and lora are bound in __init__; paia_gemv.serve packs their structs)
     def paged_attn_workspace(self, heads, kv_heads, head_dim):
         n = self._lib.paia_gemv_paged_attn_workspace(heads, kv_heads, head_dim)
         if n == 0:
             raise RuntimeError(f"paia_gemv_paged_attn_workspace: unsupported sizes (heads={heads}, kv_heads={kv_heads}, "
                                f"head_dim={head_dim})")
         return n
-
-    def paged_attn(self, args, stream):
-        rc = self._lib.paia_gemv_paged_attn(args, stream)
-        if rc:
-            self._check(rc, "paia_gemv_paged_attn")
-
-    def qkv_rope_cache(self, args, stream):
-        rc = self._lib.paia_gemv_qkv_rope_cache(args, stream)
-        if rc:
-            self._check(rc, "paia_gemv_qkv_rope_cache")
-
-    def lora(self, args, stream):
-        rc = self._lib.paia_gemv_lora(args, stream)
-        if rc:
-            self._check(rc, "paia_gemv_lora")
 
     def device_error(self, clear=True):
         """The device-side error word (0 = none): below 10 from kernels whose bounded waits gave up, 10 to 13 from

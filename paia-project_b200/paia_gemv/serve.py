@@ -19,6 +19,10 @@ ATTN = struct.Struct("10P 12q 9i f")
 ROPE_CACHE = struct.Struct("13P 12q 11i f")
 LORA = struct.Struct("8P 7q 5i 4x")
 
+# torch.cuda.current_device() and current_stream() without their Python layers (absent from CPU builds of torch)
+_current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0)
+_pack_attn, _pack_rope, _pack_lora = ATTN.pack, ROPE_CACHE.pack, LORA.pack
 _BF16, _F32, _F64, _I32, _E4M3 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.float8_e4m3fn
 
 
@@ -42,7 +46,7 @@ def _flat(name, t, dtype, shape, dev):
 
 def _device(t, name):
     dev = t.get_device()
-    if dev < 0 or dev != torch.cuda.current_device():
+    if dev < 0 or dev != _current_device():
         raise ValueError(f"{name} is on {t.device}: the operators run on the current CUDA device")
     return dev
 
@@ -108,13 +112,15 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
     if workspace.sizes != (dev, heads, kv, hd):
         raise ValueError(f"workspace is for (device, heads, kv_heads, head_dim) = {workspace.sizes}, the call for "
                          f"{(dev, heads, kv, hd)}")
-    lib.paged_attn(ATTN.pack(
+    rc = lib.paged_attn(_pack_attn(
         q.data_ptr(), k_pages.data_ptr(), v_pages.data_ptr(), page_table.data_ptr(), lens.data_ptr(),
         0 if k_scale is None else _flat("k_scale", k_scale, _F32, (kv,), dev),
         0 if v_scale is None else _flat("v_scale", v_scale, _F32, (kv,), dev), out.data_ptr(), lp, workspace.ptr,
         qs[0], qs[1], os[0], os[1], ls, tst[0], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
         batch, heads, kv, hd, cache, pool[0], pool[1], ts[1], window, hd ** -0.5 if scale is None else scale),
-        torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+        _raw_stream(dev) if stream is None else stream)
+    if rc:
+        lib._check(rc, "paia_gemv_paged_attn")
     return out
 
 
@@ -165,7 +171,7 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
         if k_out.shape != (tokens, kv, hd) or k_out.dtype is not _BF16 or k_out.get_device() != dev or kos[2] != 1:
             _bad("k_out", k_out, f"bfloat16 {(tokens, kv, hd)}, contiguous in its last dimension,")
         ko = k_out.data_ptr()
-    lib.qkv_rope_cache(ROPE_CACHE.pack(
+    rc = lib.qkv_rope_cache(_pack_rope(
         qkv.data_ptr(), positions.data_ptr(), 0 if seq is None else _flat("seq", seq, _I32, (tokens,), dev),
         inv_freq.data_ptr(), 0 if q_norm is None else _flat("q_norm", q_norm, _F32, (hd,), dev),
         0 if k_norm is None else _flat("k_norm", k_norm, _F32, (hd,), dev), table,
@@ -173,7 +179,9 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
         0 if v_scale is None else _flat("v_scale", v_scale, _F32, (kv,), dev), q_out.data_ptr(), ko, kp, vp,
         xs[0], qs[0], qs[1], kos[0] if ko else 0, kos[1] if ko else 0, ts, ks[0], ks[1], ks[2], vs[0], vs[1], vs[2],
         tokens, seqs, heads, kv, hd, 2 * half, 1 if interleaved else 0, cache, num_pages, page_size, max_pages, eps),
-        torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+        _raw_stream(dev) if stream is None else stream)
+    if rc:
+        lib._check(rc, "paia_gemv_qkv_rope_cache")
     return q_out
 
 
@@ -200,10 +208,12 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
         if base.shape != (m, n) or base.dtype is not _BF16 or base.get_device() != dev or base.stride(1) != 1:
             _bad("base", base, f"bfloat16 {(m, n)}, contiguous in its last dimension,")
         bp, bs = base.data_ptr(), base.stride(0)
-    lib.lora(LORA.pack(
+    rc = lib.lora(_pack_lora(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), adapter.data_ptr(),
         0 if ranks is None else _flat("ranks", ranks, _I32, (n_ad,), dev),
         0 if scaling is None else _flat("scaling", scaling, _F32, (n_ad,), dev), bp, out.data_ptr(),
         xs[0], bs, os[0], sa[0], sa[1], sb[0], sb[1], m, n, k, rank, n_ad),
-        torch._C._cuda_getCurrentRawStream(dev) if stream is None else stream)
+        _raw_stream(dev) if stream is None else stream)
+    if rc:
+        lib._check(rc, "paia_gemv_lora")
     return out

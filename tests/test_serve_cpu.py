@@ -122,7 +122,7 @@ def test_nothing_to_do_and_null(L):
     with pytest.raises(RuntimeError):
         L.paged_attn_workspace(8, 3, 128)
     with pytest.raises(RuntimeError):
-        L.lora(packed("paia_gemv_lora_args", serve.LORA, LORA, rank=12), 0)
+        L._check(L.lora(packed("paia_gemv_lora_args", serve.LORA, LORA, rank=12), 0), "paia_gemv_lora")
     assert L.paged_attn_workspace(32, 8, 128) < L.paged_attn_workspace(64, 8, 128) <= 16 << 20
 
 
@@ -159,15 +159,24 @@ class Recorder:
 
     def paged_attn(self, args, stream):
         self.calls.append(args)
+        return 0
 
     qkv_rope_cache = lora = paged_attn
+
+
+def test_wrapper_raises_return_codes(monkeypatch, L):
+    from paia_gemv import serve
+    monkeypatch.setattr(serve, "_current_device", lambda: 0)
+    z = lambda *s, dtype=torch.bfloat16: on(torch.zeros(*s, dtype=dtype))   # noqa: E731
+    with pytest.raises(RuntimeError, match="paia_gemv_lora failed with code -2"):      # rank 12 is no multiple of 8
+        serve.lora(L, z(3, 64), z(2, 12, 64), z(2, 40, 12), z(3, dtype=torch.int32), z(3, 40), stream=0)
 
 
 def test_wrapper_checks(monkeypatch):
     """Every tensor of a call is checked for its type, shape, layout and device before the library sees it."""
     from paia_gemv import serve
-    monkeypatch.setattr(torch.cuda, "current_device", lambda: 0)
-    monkeypatch.setattr(torch._C, "_cuda_getCurrentRawStream", lambda d: 0, raising=False)
+    monkeypatch.setattr(serve, "_current_device", lambda: 0)
+    monkeypatch.setattr(serve, "_raw_stream", lambda d: 0)
     bf, i32, rec = torch.bfloat16, torch.int32, Recorder()
     z = lambda *s, dtype=bf: on(torch.zeros(*s, dtype=dtype))   # noqa: E731
     good = dict(q=z(3, 4, 64), k_pages=z(5, 16, 2, 64), v_pages=z(5, 16, 2, 64), page_table=z(3, 6, dtype=i32),
