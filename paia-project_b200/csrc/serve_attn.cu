@@ -8,9 +8,9 @@
 // serves the stream of cache rows:
 //   split     The launch does not know the lengths. All sequences' tiles of 16 or 32 positions form one list (sequence, kv
 //             head, tile), and every CTA takes an equal run of it, so a ragged batch or one long sequence fills the GPU
-//             alike. A unit (a sequence's kv head) weighs 14 tiles on top of its own, what its merge and output take:
-//             without that weight the CTAs that got a batch's short and empty sequences finished last (32 ragged
-//             sequences up to 4100: 40 us; weight 3: 31, 14: 23). Each CTA finds its run from lens itself.
+//             alike. A unit (a sequence's kv head) weighs 14 tiles on top of its own (in CTAs of four warps), what its merge
+//             and output take: without that weight the CTAs that got a batch's short and empty sequences finished last
+//             (32 ragged sequences up to 4100: 40 us; weight 3: 31, 14: 23). Each CTA finds its run from lens itself.
 //   stream    A warp owns a ring of stages, each the K and V rows of one tile of positions, filled with cp.async (any
 //             page size and strides, rows outside the range arrive as zeros) and running on across sequences and
 //             heads; no warp waits for another while it streams. Page ids are looked up for 32 tiles at a time, a tile
@@ -32,7 +32,8 @@
 namespace pb2 {
 namespace {
 
-constexpr int kUnitCost = 14;               // what a unit costs beyond its tiles, in tiles: its queries, merge and output
+// What a unit costs beyond its tiles, in tiles of a CTA of W warps: its queries, merge and output.
+constexpr int unit_cost(int W) { return W == 4 ? 14 : 6; }
 constexpr int kJoin = 8;                    // parts of a unit that are joined at a time
 constexpr int kAttnMaxGrid = 4 * 160;       // the workspace holds two parts per CTA of the largest grid
 
@@ -74,8 +75,8 @@ struct AttnTile {
 };
 
 // A tile of POS positions in the list: tile `tile` of `ntile` of unit u (kv head, chunk of heads) of sequence b. On the
-// scale by which the list is divided a unit has ntile + kUnitCost places, the sequence's first one is w0.
-template <int POS>
+// scale by which the list is divided a unit has ntile + COST places, the sequence's first one is w0.
+template <int POS, int COST>
 struct Cursor {
     int b, u, tile, ntile, first, start, len;
     unsigned w0;
@@ -98,22 +99,22 @@ struct Cursor {
                 return;
             }
             off -= (unsigned)ntile * units;
-            w0 += (unsigned)(ntile + kUnitCost) * units;
+            w0 += (unsigned)(ntile + COST) * units;
             ++b;
             load(p);
         }
         u = (int)(off / (unsigned)ntile);
         tile = (int)(off - (unsigned)u * ntile);
     }
-    __device__ __forceinline__ unsigned unit_place() const { return w0 + (unsigned)u * (ntile + kUnitCost); }
+    __device__ __forceinline__ unsigned unit_place() const { return w0 + (unsigned)u * (ntile + COST); }
 };
 
-template <int POS>
+template <int POS, int COST>
 __device__ __forceinline__ int unit_places(const AttnParams& p, int b) {
-    Cursor<POS> c;
+    Cursor<POS, COST> c;
     c.b = b;
     c.load(p);
-    return c.ntile + kUnitCost;
+    return c.ntile + COST;
 }
 
 template <int HD, int FMT, int W, int S>
@@ -151,6 +152,7 @@ template <int HD, int FMT, int ROWS, int W, int S, int MINB>
 __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnParams p) {
     using T = AttnTile<HD, FMT>;
     using SM = AttnSmem<HD, FMT, W, S>;
+    constexpr int kUnitCost = unit_cost(W);
     constexpr int POS = T::kPos, NB = POS / 16;                                  // blocks of 16 positions
     constexpr int KS = HD / 16;                                                  // k steps of Q K^T
     constexpr int NT = HD / 8;                                                   // column tiles of P V
@@ -169,12 +171,12 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     // ---- this CTA's run [t0, t1) of the list, and the place it starts at. Every warp finds it for itself, so that none
     // waits for another: lane i counts the i-th 32nd of the sequences, one scan finds the lane that holds t0, a second
     // one the sequence among that lane's (a third and more beyond 1024 sequences).
-    Cursor<POS> seg;
+    Cursor<POS, kUnitCost> seg;
     unsigned t0, t1, per;
     {
         const int share = (p.batch + 31) / 32, lo = min(lane * share, p.batch), hi = min(lo + share, p.batch);
         unsigned mine = 0;
-        for (int b = lo; b < hi; ++b) mine += unit_places<POS>(p, b);
+        for (int b = lo; b < hi; ++b) mine += unit_places<POS, kUnitCost>(p, b);
         unsigned inc = mine;
 #pragma unroll
         for (int o = 1; o < 32; o <<= 1) {
@@ -194,7 +196,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
 #pragma unroll 1
             for (;; from += 32) {
                 const int b = from + lane;
-                const unsigned n = b < end ? unit_places<POS>(p, b) : 0;
+                const unsigned n = b < end ? unit_places<POS, kUnitCost>(p, b) : 0;
                 inc = n;
 #pragma unroll
                 for (int o = 1; o < 32; o <<= 1) {
@@ -228,7 +230,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     // 32 of them (for 16-position blocks that straddle pages: only where the tile lies).
     const uint32_t ring = ((sptr(smem) + 511) & ~511u) + (uint32_t)(warp * S * T::kStage);
     struct Look { int id[NB], in[NB], head, range, b, p0; };                     // rows range & 255 .. range >> 8
-    Cursor<POS> is = seg;
+    Cursor<POS, kUnitCost> is = seg;
     is.advance(p, units, warp + lane * W);
     Look now{};
     int fetched = 0, known = 0, fill = 0;                                        // known: tiles looked up; fill: next stage
@@ -723,12 +725,18 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
 
 // Four warps per CTA, two CTAs per SM (head_dim 256: one, its sums fill the registers), two stages per warp: one tile
 // (8 KB, 16 KB at head_dim 256) in flight while one is worked on. Three stages are slower: 1 x 128k 90.2 us against 86.0,
-// 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us.
+// 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us. Where every CTA gets two units or more,
+// CTAs of two warps, twice as many: fewer warps wait at the end of each short unit (256 x 64 positions 25.2 us with four,
+// 18.6 with two; 128 x 1: 12.8 and 9.1; but 1 x 128k 86 and 95).
 template <int HD>
 int pick_attn(const AttnParams& p, int fmt, cudaStream_t st) {
     constexpr int W = 4, S = 2, B = HD == 256 ? 1 : 2;
-    if (p.group <= 8) return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B>(p, st) : launch_attn<HD, 1, 8, W, S, B>(p, st);
-    return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
+    if (p.group > 8) return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
+    if constexpr (HD < 256) {
+        if ((long long)p.batch * p.kv_heads * p.chunks >= 2ll * B * sm_count())
+            return fmt == 0 ? launch_attn<HD, 0, 8, W / 2, S, 2 * B>(p, st) : launch_attn<HD, 1, 8, W / 2, S, 2 * B>(p, st);
+    }
+    return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B>(p, st) : launch_attn<HD, 1, 8, W, S, B>(p, st);
 }
 
 bool attn_sizes(int heads, int kv_heads, int head_dim) {
@@ -772,7 +780,7 @@ extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
     // positions and the list's places are counted in 32 bits
     const long long cap = (long long)a->max_pages * a->page_size;
     const int group = a->heads / a->kv_heads, chunks = (group + 15) / 16;
-    if (cap > 0x7fffff00ll || (cap / 16 + 2 + kUnitCost) * a->kv_heads * chunks > 0xfff00000ll / a->batch) return -2;
+    if (cap > 0x7fffff00ll || (cap / 16 + 2 + unit_cost(4)) * a->kv_heads * chunks > 0xfff00000ll / a->batch) return -2;
     AttnParams p{};
     p.q = static_cast<const __nv_bfloat16*>(a->q);
     p.k = static_cast<const uint8_t*>(a->k);

@@ -280,13 +280,14 @@ def test_attention_division_covers_every_tile_once():
     """Every tile of every unit belongs to one CTA; a unit in parts is counted in by exactly the CTAs c0 .. c1, the counter
     of c0 and each CTA's two slots of the workspace serve one unit each."""
     src = (ROOT / "paia-project_b200" / "csrc" / "serve_attn.cu").read_text()
-    cost = int(re.search(r"kUnitCost = (\d+);", src).group(1))
+    costs = dict(zip((4, 2), map(int, re.search(r"unit_cost.*W == 4 \? (\d+) : (\d+);", src).groups())))
     rng = random.Random(4)
     for trial in range(300):
         lens = [rng.choice([0, 1, rng.randrange(40), rng.randrange(3000)]) for _ in range(rng.choice([1, 2, 7, 40, 90]))]
         units, pos, grid = rng.choice([1, 2, 8, 13]), rng.choice([16, 32]), rng.choice([1, 5, 148, 296])
         window = rng.choice([0, 0, 1, 100])
-        work = attention_division(lens, units, pos, grid, 4, cost, window)
+        warps = rng.choice([4, 2])
+        work = attention_division(lens, units, pos, grid, warps, costs[warps], window)
         seen, arrivals, counters, slots = {}, {}, {}, {}
         for cta, parts in work.items():
             for b, u, tile, part, n, c0, c1 in parts:
