@@ -308,6 +308,9 @@ typedef struct paia_gemv_lora_args {
 } paia_gemv_lora_args;
 int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream);
 
+/* The calling thread's current CUDA device; -1 where there is none. */
+int paia_gemv_current_device(void);
+
 /* Device-side error word of the current device (0 = none), set by kernels whose bounded waits gave up (codes below
  * 10) or that met a bad index in device memory (10 to 13); clear != 0 resets it. Synchronous. */
 int paia_gemv_device_error(int clear);

@@ -7,13 +7,18 @@ Each csrc/*.cu is compiled to an object in parallel (nvcc, -gencode arch=compute
 no torch headers), then linked into one shared library with a plain C ABI, as the reference's build.sh does
 (src/paia_gemv/build.sh:8-19) but for sm_100a only. The ptxas register/spill report of every kernel is kept in
 build/<arch>/ptxas_report.txt. nvcc cross-compiles, so no GPU is needed.
+
+Beside it, where Python's and torch's headers are there, build/<arch>/_paia_serve.so: the CPython extension that makes
+paia_gemv.serve's calls without their Python overhead (csrc/serve_bind.cpp; it links neither torch nor the library).
 """
 import argparse
+import importlib.util
 import os
 import platform
 import shutil
 import subprocess
 import sys
+import sysconfig
 from concurrent.futures import ThreadPoolExecutor
 from pathlib import Path
 
@@ -22,6 +27,7 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 OUT = HERE / "build" / platform.machine()
 LIB = OUT / "libpaia_gemv.so"
+BIND = OUT / "_paia_serve.so"
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr"]
 
@@ -40,8 +46,26 @@ def _stale(obj, deps):
     return any(d.stat().st_mtime > t for d in deps)
 
 
+def build_bind(force=False):
+    """The extension module; None where the headers or a host compiler are missing (serve then calls through ctypes)."""
+    src = CSRC / "serve_bind.cpp"
+    spec, cxx = importlib.util.find_spec("torch"), shutil.which("g++")
+    inc = [Path(sysconfig.get_paths()["include"])] + ([Path(spec.origin).parent / "include"] if spec and spec.origin else [])
+    if cxx is None or len(inc) < 2 or not (inc[0] / "Python.h").exists() or not (inc[1] / "ATen" / "dlpack.h").exists():
+        return None
+    if force or _stale(BIND, [src, INCLUDE / "paia_gemv.h", Path(__file__)]):
+        cmd = [cxx, "-O2", "-std=c++17", "-shared", "-fPIC", "-Wall", *(f"-I{d}" for d in (*inc, INCLUDE)), str(src), "-o",
+               str(BIND)]
+        r = subprocess.run(cmd, capture_output=True, text=True)
+        if r.returncode != 0:                       # headers of a torch without the exchange functions
+            sys.stderr.write(f"{src.name} not built:\n{r.stderr[:2000]}\n")
+            return None
+    return BIND
+
+
 def build(force=False, verbose=False):
     OUT.mkdir(parents=True, exist_ok=True)
+    build_bind(force)
     srcs = sorted(CSRC.glob("*.cu"))
     headers = sorted(CSRC.glob("*.cuh")) + sorted(CSRC.glob("*.h")) + sorted(INCLUDE.glob("*.h"))
     cc = nvcc()

@@ -833,6 +833,12 @@ int paia_gemv_launch_ex(int kind, int R, int U, int W, int math, int pdl, int ks
     return launch_variant(v, p, o, static_cast<cudaStream_t>(stream));
 }
 
+int paia_gemv_current_device(void) {
+    int d = -1;
+    if (cudaGetDevice(&d) != cudaSuccess) { (void)cudaGetLastError(); return -1; }
+    return d;
+}
+
 // Device-side error word of the current device (0 = none; the codes of the TMA-fed kernels' bounded waits, 6 and 8
 // from the tensor-parallel exchange), then the serving operators' words (10 to 13, bad indices in device memory);
 // clear != 0 resets them all. Synchronous (symbol copies).

@@ -129,6 +129,9 @@ class GemvLib:
             fn.restype = I
             fn.argtypes = [P, P]
             setattr(self, name, fn)
+            setattr(self, name + "_entry", ctypes.cast(fn, P).value)
+        lib.paia_gemv_current_device.restype = I
+        self.device_entry = ctypes.cast(lib.paia_gemv_current_device, P).value
         lib.paia_gemv_paged_attn_workspace.restype = ctypes.c_size_t
         lib.paia_gemv_paged_attn_workspace.argtypes = [I, I, I]
         lib.paia_gemv_device_error.restype = I

@@ -10,14 +10,36 @@ Caches are a pair of tensors [num_pages, page_size, kv_heads, head_dim] (bf16, o
 kv head), in any layout whose head_dim is contiguous: a [num_pages, kv_heads, page_size, head_dim] pool is passed as
 `pool.transpose(1, 2)`. Page tables are int32 [sequences, max_pages]. Tensors live on the current CUDA device.
 """
+import importlib.util
+import platform
 import struct
 
 import torch
+
+from .loader import _PKG_ROOT
 
 # the C structs, field by field (native alignment): include/paia_gemv.h
 ATTN = struct.Struct("10P 12q 9i f")
 ROPE_CACHE = struct.Struct("13P 12q 11i f")
 LORA = struct.Struct("8P 7q 5i 4x")
+
+def _load_bind():
+    """The extension that checks and makes these calls in C (csrc/serve_bind.cpp), or None: without it, and for every
+    call that it does not find exactly as it should be, the code below checks, calls and raises."""
+    path = _PKG_ROOT / "build" / platform.machine() / "_paia_serve.so"
+    api = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
+    if api is None or not path.exists():
+        return None
+    try:
+        spec = importlib.util.spec_from_file_location("_paia_serve", path)
+        mod = importlib.util.module_from_spec(spec)
+        spec.loader.exec_module(mod)
+    except ImportError:
+        return None
+    return mod if mod.init(torch.Tensor, api) else None
+
+
+_bind = _load_bind()
 
 # torch.cuda.current_device() and current_stream() without their Python layers (absent from CPU builds of torch)
 _current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
@@ -87,6 +109,10 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
     """out[b] = attention of q[b] (bf16 [batch, heads, head_dim]) over the first lens[b] positions of sequence b (the
     last `window` of them where window > 0). out bf16 like q; lse fp32 [batch, heads], natural logarithm, or None. A
     sequence of length 0 gets zeros and -inf. scale: 1 / sqrt(head_dim) by default."""
+    if _bind is not None and _bind.paged_attention(
+            lib.paged_attn_entry, lib.device_entry, q, k_pages, v_pages, page_table, lens, out, workspace.ptr,
+            workspace.sizes, scale, window, k_scale, v_scale, lse, stream) == 0:
+        return out
     dev, shape, qs, os = _device(q, "q"), q.shape, q.stride(), out.stride()
     if len(shape) != 3 or q.dtype is not _BF16 or (qs[2] != 1 and shape[2] != 1):
         _bad("q", q, "bfloat16 [batch, heads, head_dim], contiguous in its last dimension,")
@@ -139,6 +165,10 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
     head_dim (`rope_inv_freq`). k_out (bf16 [tokens, kv_heads, head_dim]) gets the rotated k heads as well; without a
     cache (k_pages, v_pages and page_table None) it is required, with kv_heads. Two rows of a call must not name the
     same sequence and position."""
+    if _bind is not None and k_pages is not None and _bind.qkv_rope_cache(
+            lib.qkv_rope_cache_entry, lib.device_entry, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_table, seq,
+            q_norm, k_norm, eps, interleaved, k_scale, v_scale, k_out, stream) == 0:
+        return q_out
     dev, qs, xs = _device(qkv, "qkv"), q_out.stride(), qkv.stride()
     if len(qs) != 3 or q_out.dtype is not _BF16 or q_out.get_device() != dev or qs[2] != 1:
         _bad("q_out", q_out, "bfloat16 [tokens, heads, head_dim], contiguous in its last dimension,")
@@ -189,6 +219,9 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
     """out[m] = base[m] + scaling[i] * b[i] (a[i] x[m]) for i = adapter[m] (int32; -1: out[m] = base[m]). x bf16 [M, K],
     a bf16 [adapters, rank, K], b bf16 [adapters, N, rank], out and base (None: zeros; may be out) bf16 [M, N]; scaling
     fp32 and ranks int32 [adapters] (None: 1 and `rank`): adapter i uses its first ranks[i] ranks."""
+    if _bind is not None and _bind.lora(lib.lora_entry, lib.device_entry, x, a, b, adapter, out, base, scaling, ranks,
+                                        stream) == 0:
+        return out
     dev, xs, sa, sb, os = _device(x, "x"), x.stride(), a.stride(), b.stride(), out.stride()
     if len(xs) != 2 or x.dtype is not _BF16 or xs[1] != 1 or len(sa) != 3 or len(sb) != 3:
         _bad("x", x, "bfloat16 [M, K], contiguous in its last dimension (a [adapters, rank, K], b [adapters, N, rank]),")

@@ -154,6 +154,8 @@ def on(t):
 
 class Recorder:
     """Stands in for the library: takes the packed struct."""
+    paged_attn_entry = qkv_rope_cache_entry = lora_entry = device_entry = 0
+
     def __init__(self):
         self.calls = []
 

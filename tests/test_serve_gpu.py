@@ -32,6 +32,83 @@ def within(got, want, tol, what=""):
     assert not off.numel() or off.max().item() <= 0, (what, off.max().item(), tol.flatten()[off.argmax()].item())
 
 
+@pytest.fixture(params=["extension", "ctypes"])
+def route(request, monkeypatch):
+    """Both ways a call takes: the extension's checks in C, and Python's."""
+    from paia_gemv import serve
+    if request.param == "ctypes":
+        monkeypatch.setattr(serve, "_bind", None)
+    else:
+        assert serve._bind is not None, "csrc/serve_bind.cpp is not built"
+    return request.param
+
+
+def test_both_routes_make_the_same_calls(L, monkeypatch, route):
+    """Strides, optional arguments and dimensions of one, whichever way the call takes."""
+    seen = []
+
+    class Spy:
+        def __getattr__(self, name):
+            return getattr(serve_bind, name)
+
+    from paia_gemv import serve
+    serve_bind = serve._bind
+    if route == "extension":
+        for name in ("paged_attention", "qkv_rope_cache", "lora"):
+            real = getattr(serve_bind, name)
+            setattr(Spy, name, staticmethod(lambda *a, real=real: seen.append(real(*a)) or seen[-1]))
+        monkeypatch.setattr(serve, "_bind", Spy())
+    for lens, heads, kv in (([1], 1, 1), ([40, 0, 300], 6, 2)):
+        for dtype in (BF16, E4M3):
+            call, out, lse, want = attend(L, lens, heads, kv, 64, 16, dtype, hnd=True, window=50)
+            check(out, lse, want, lens)
+    test_attention_strided_and_scaled(L)
+    rope_case(L, 1, 1, 1, 64, 64)
+    rope_case(L, 20, 6, 2, 128, 64, E4M3, inter=True, hnd=True, k_out=True)
+    rope_case(L, 20, 6, 2, 128, 64, norm=False, in_place=True)
+    lora_case(L, 1, 64, 64, 8, 1, [0])
+    lora_case(L, 20, 128, 72, 16, 3, [m % 4 - 1 for m in range(20)], ranks=[3, 16, 9], in_place=True)
+    test_lora_strided(L)
+    if route == "extension":
+        assert seen and set(seen) == {0}                         # the extension made every call itself
+
+
+def test_refusals_on_the_device(L, route):
+    """What a call must not be given raises, whichever way it takes, and nothing is launched."""
+    from paia_gemv import serve
+    z = lambda *s, dtype=BF16: torch.zeros(*s, dtype=dtype, device="cuda")   # noqa: E731
+    i32 = torch.int32
+    ws = serve.attention_workspace(L, 4, 2, 64)
+    good = dict(q=z(3, 4, 64), k_pages=z(5, 16, 2, 64), v_pages=z(5, 16, 2, 64), page_table=z(3, 6, dtype=i32),
+                lens=z(3, dtype=i32), out=torch.ones(3, 4, 64, dtype=BF16, device="cuda"), workspace=ws)
+    for bad, err in ((dict(q=z(3, 4, 64).float()), ValueError), (dict(lens=torch.zeros(3, dtype=i32)), ValueError),
+                     (dict(v_pages=z(4, 16, 2, 64)), ValueError), (dict(k_scale=z(2, dtype=torch.float32)), ValueError),
+                     (dict(page_table=z(3, 6, dtype=torch.int64)), ValueError), (dict(lse=z(3, 4)), ValueError),
+                     (dict(workspace=serve.attention_workspace(L, 4, 4, 64)), ValueError), (dict(window=-1), RuntimeError),
+                     (dict(scale=0.0), RuntimeError), (dict(q=z(3, 4, 68)[:, :, :64]), RuntimeError),
+                     (dict(out=z(3, 1, 64).expand(3, 4, 64)), RuntimeError)):
+        with pytest.raises(err):
+            serve.paged_attention(L, **dict(good, **bad))
+    assert (good["out"] == 1).all()
+    good = dict(qkv=z(3, 8 * 64), positions=z(3, dtype=i32), inv_freq=z(32, dtype=torch.float64), q_out=z(3, 4, 64),
+                k_pages=z(5, 16, 2, 64), v_pages=z(5, 16, 2, 64), page_table=z(3, 6, dtype=i32))
+    for bad, err in ((dict(qkv=z(3, 7 * 64)), ValueError), (dict(inv_freq=z(32, dtype=torch.float32)), ValueError),
+                     (dict(page_table=z(2, 6, dtype=i32)), ValueError), (dict(seq=z(2, dtype=i32)), ValueError),
+                     (dict(q_norm=z(64)), ValueError), (dict(inv_freq=z(40, dtype=torch.float64)), RuntimeError),
+                     (dict(eps=-1.0), RuntimeError)):
+        with pytest.raises(err):
+            serve.qkv_rope_cache(L, **dict(good, **bad))
+    good = dict(x=z(3, 64), a=z(2, 8, 64), b=z(2, 40, 8), adapter=z(3, dtype=i32), out=z(3, 40))
+    for bad, err in ((dict(x=z(3, 32)), ValueError), (dict(b=z(2, 40, 16)), ValueError), (dict(base=z(2, 40)), ValueError),
+                     (dict(adapter=z(3, dtype=torch.int64)), ValueError),
+                     (dict(a=z(2, 12, 64), b=z(2, 40, 12)), RuntimeError),
+                     (dict(out=z(1, 40).expand(3, 40)), RuntimeError)):
+        with pytest.raises(err):
+            serve.lora(L, **dict(good, **bad))
+    torch.cuda.synchronize()
+    assert L.device_error(True) == 0
+
+
 # ------------------------------------------------------------------ attention
 
 def attend(L, lens, heads, kv, hd, page, dtype=BF16, hnd=False, window=0, scale=None, seed=1, q=None, ws=None):
