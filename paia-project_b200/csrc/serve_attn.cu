@@ -25,7 +25,9 @@
 //             Larger groups are cut into units of 16 heads.
 //   join      At the end of a run's part of a (sequence, head) the CTA's warps merge through shared memory. A part that
 //             is not the whole goes to the workspace, and the last CTA to arrive merges all parts in list order (the
-//             same bits whichever CTA it is) and resets the counter. Nothing ever waits on another CTA.
+//             same bits whichever CTA it is) and resets the counter. Nothing ever waits on another CTA. (Small calls:
+//             a cluster per unit, whose CTAs store their parts into the first one's shared memory.)
+#include <cooperative_groups.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 
@@ -34,6 +36,8 @@ namespace {
 
 // What a unit costs beyond its tiles, in tiles of a CTA of W warps: its queries, merge and output.
 constexpr int unit_cost(int W) { return W == 4 ? 14 : 6; }
+constexpr int kAttnSmall = 128;             // tiles per sequence up to which small calls take a cluster per unit
+constexpr int kAttnCluster = 8;             // CTAs per unit of the small calls
 constexpr int kJoin = 8;                    // parts of a unit that are joined at a time
 constexpr int kAttnMaxGrid = 4 * 160;       // the workspace holds two parts per CTA of the largest grid
 
@@ -117,12 +121,18 @@ __device__ __forceinline__ int unit_places(const AttnParams& p, int b) {
     return c.ntile + COST;
 }
 
+// p in the shared memory of the cluster's CTA `cta`.
+template <class V>
+__device__ __forceinline__ V* remote(V* p, int cta) { return cooperative_groups::this_cluster().map_shared_rank(p, cta); }
+
 template <int HD, int FMT, int W, int S>
 struct AttnSmem {
     using T = AttnTile<HD, FMT>;
     static constexpr int kStride = HD + 4;                                       // floats per merged row
     static constexpr size_t kRing = (size_t)W * S * T::kStage;
-    static size_t bytes(int rows) { return 512 + kRing + (size_t)W * rows * (kStride + 2) * 4; }
+    static size_t bytes(int rows, int cluster) {
+        return 512 + kRing + (size_t)W * rows * (kStride + 2) * 4 + (size_t)cluster * rows * (HD + 2) * 4;
+    }
 };
 
 // e4m3 fragments. K: word w (of HD / 16) of lane t of a row is at byte k_byte(w, t), read VK words at a time; its four
@@ -148,7 +158,8 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
 }
 
-template <int HD, int FMT, int ROWS, int W, int S, int MINB>
+// CL: a cluster of kAttnCluster CTAs per unit instead of a run of the list per CTA.
+template <int HD, int FMT, int ROWS, int W, int S, int MINB, bool CL>
 __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnParams p) {
     using T = AttnTile<HD, FMT>;
     using SM = AttnSmem<HD, FMT, W, S>;
@@ -165,15 +176,36 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     const int rows = min(p.group, ROWS);
     float* merge_o = reinterpret_cast<float*>(smem + 512 + SM::kRing);                 // [W][rows][kStride]
     float2* merge_ml = reinterpret_cast<float2*>(merge_o + W * rows * SM::kStride);
+    const int rank = CL ? (int)(blockIdx.x % kAttnCluster) : 0;
+    // CL, in CTA 0: every CTA's part of the unit, [CTA][rows][HD], then (m, l) [CTA][rows]
+    float* join_o = reinterpret_cast<float*>(merge_ml + W * rows);
+    float2* join_ml = reinterpret_cast<float2*>(join_o + kAttnCluster * rows * HD);
 
+    if (CL) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");        // this CTA runs: others may store here
     pdl_trigger();
     pdl_wait();
     // ---- this CTA's run [t0, t1) of the list, and the place it starts at. Every warp finds it for itself, so that none
     // waits for another: lane i counts the i-th 32nd of the sequences, one scan finds the lane that holds t0, a second
     // one the sequence among that lane's (a third and more beyond 1024 sequences).
     Cursor<POS, kUnitCost> seg;
-    unsigned t0, t1, per;
-    {
+    unsigned t0, t1, per = 1;
+    if constexpr (CL) {
+        const int unit = (int)(blockIdx.x / kAttnCluster);
+        seg.b = unit / units;
+        seg.u = unit - seg.b * units;
+        seg.w0 = 0;
+        seg.load(p);
+        seg.w0 = 0u - seg.unit_place();                                          // the unit's tiles are places 0, 1, ...
+        t0 = (unsigned)(seg.ntile * rank + kAttnCluster - 1) / kAttnCluster;     // CTA 0 has one at least
+        t1 = (unsigned)(seg.ntile * (rank + 1) + kAttnCluster - 1) / kAttnCluster;
+        seg.tile = (int)t0;
+        if (t0 == t1) {                                                          // fewer tiles than CTAs: no part
+            asm volatile("barrier.cluster.wait;" ::: "memory");
+            for (int r = tid; r < rows; r += W * 32) *remote(join_ml + rank * rows + r, 0) = make_float2(-INFINITY, 0.f);
+            asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+            return;
+        }
+    } else {
         const int share = (p.batch + 31) / 32, lo = min(lane * share, p.batch), hi = min(lo + share, p.batch);
         unsigned mine = 0;
         for (int b = lo; b < hi; ++b) mine += unit_places<POS, kUnitCost>(p, b);
@@ -422,6 +454,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                         p.lse[seg.b * p.lse_batch + hq] = ll > 0.f || ll != ll ? (mm + log2f(ll)) * 0.69314718055994531f : -INFINITY;
                 };
                 const size_t slot = (size_t)(2 * blockIdx.x + (seg.tile == 0 ? 1 : 0)) * rows;
+                if (CL) asm volatile("barrier.cluster.wait;" ::: "memory");      // CTA 0 runs
 #pragma unroll 2
                 for (int e = tid; e < nrow * (HD / 4); e += W * 32) {
                     const int r = e / (HD / 4), d = e % (HD / 4) * 4;
@@ -441,14 +474,42 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                         o.z += f * a.z;
                         o.w += f * a.w;
                     }
-                    if (whole) {
+                    if constexpr (CL) {
+                        if (d == 0) *remote(join_ml + rank * rows + r, 0) = make_float2(mm, ll);
+                        *remote(reinterpret_cast<float4*>(join_o + (rank * rows + r) * HD + d), 0) = o;
+                    } else if (whole) {
                         store(r, d, o, mm, ll);
                     } else {
                         if (d == 0) p.part_ml[slot + r] = make_float2(mm, ll);
                         *reinterpret_cast<float4*>(p.part_o + (slot + r) * HD + d) = o;
                     }
                 }
-                if (!whole) {
+                if constexpr (CL) {
+                    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+                    for (int e = tid; rank == 0 && e < nrow * (HD / 4); e += W * 32) {
+                        const int r = e / (HD / 4), d = e % (HD / 4) * 4;
+                        float mm = -INFINITY, ll = 0.f;
+                        float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+                        for (int c = 0; c < kAttnCluster; ++c) mm = fmaxf(mm, join_ml[c * rows + r].x);
+                        const float ref = mm == -INFINITY ? 0.f : mm;
+#pragma unroll
+                        for (int c = 0; c < kAttnCluster; ++c) {
+                            const float2 ml = join_ml[c * rows + r];
+                            if (ml.x == -INFINITY) continue;                     // no part, or nothing in it
+                            const float4 a = *reinterpret_cast<const float4*>(join_o + (c * rows + r) * HD + d);
+                            const float f = ex2(ml.x - ref);
+                            ll += f * ml.y;
+                            o.x += f * a.x;
+                            o.y += f * a.y;
+                            o.z += f * a.z;
+                            o.w += f * a.w;
+                        }
+                        store(r, d, o, mm, ll);
+                    }
+                    cp_wait<0>();
+                    return;
+                } else if (!whole) {
                     const int c0 = (int)(u0 / per), c1 = (int)((u0 + seg.ntile - 1) / per);   // the CTAs that share the unit
                     __syncthreads();
                     if (tid == 0) {
@@ -711,13 +772,18 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     }
 }
 
-template <int HD, int FMT, int ROWS, int W, int S, int MINB>
+template <int HD, int FMT, int ROWS, int W, int S, int MINB, bool CL = false>
 int launch_attn(const AttnParams& p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
-    const auto fn = paged_attn_kernel<HD, FMT, ROWS, W, S, MINB>;
-    const size_t smem = AttnSmem<HD, FMT, W, S>::bytes(p.group < ROWS ? p.group : ROWS);
-    const int rc = serve_allow_smem((const void*)fn, AttnSmem<HD, FMT, W, S>::bytes(ROWS), done);
+    const auto fn = paged_attn_kernel<HD, FMT, ROWS, W, S, MINB, CL>;
+    using SM = AttnSmem<HD, FMT, W, S>;
+    constexpr int C = CL ? kAttnCluster : 0;
+    const int rc = serve_allow_smem((const void*)fn, SM::bytes(ROWS, C), done);
     if (rc) return rc;
+    const size_t smem = SM::bytes(p.group < ROWS ? p.group : ROWS, C);
+    if (CL)
+        return serve_launch(fn, p, dim3((unsigned)(p.batch * p.kv_heads * p.chunks * kAttnCluster)), W * 32, smem, st,
+                            kAttnCluster);
     int grid = sm_count() * MINB;
     if (grid > kAttnMaxGrid) grid = kAttnMaxGrid;
     return serve_launch(fn, p, dim3((unsigned)grid), W * 32, smem, st);
@@ -727,13 +793,20 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
 // (8 KB, 16 KB at head_dim 256) in flight while one is worked on. Three stages are slower: 1 x 128k 90.2 us against 86.0,
 // 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us. Where every CTA gets two units or more,
 // CTAs of two warps, twice as many: fewer warps wait at the end of each short unit (256 x 64 positions 25.2 us with four,
-// 18.6 with two; 128 x 1: 12.8 and 9.1; but 1 x 128k 86 and 95).
+// 18.6 with two; 128 x 1: 12.8 and 9.1; but 1 x 128k 86 and 95). Where a cluster of CTAs per unit leaves every CTA an SM of
+// its own and the table holds at most 128 tiles per sequence, that: the parts join through distributed shared memory
+// instead of the workspace (1 x 1024 positions 5.4 us against 7.5, 1 x 2048 7.0 and 8.8; 1 x 4096 9.8 and 9.6).
 template <int HD>
 int pick_attn(const AttnParams& p, int fmt, cudaStream_t st) {
     constexpr int W = 4, S = 2, B = HD == 256 ? 1 : 2;
     if (p.group > 8) return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
     if constexpr (HD < 256) {
-        if ((long long)p.batch * p.kv_heads * p.chunks >= 2ll * B * sm_count())
+        const long long n = (long long)p.batch * p.kv_heads * p.chunks;
+        const int cap = p.max_pages * p.page_size, most = p.window && p.window < cap ? p.window : cap;
+        const int pos = fmt == 0 ? AttnTile<HD, 0>::kPos : AttnTile<HD, 1>::kPos;
+        if (n * kAttnCluster <= sm_count() && (most + pos - 1) / pos <= kAttnSmall)
+            return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B, true>(p, st) : launch_attn<HD, 1, 8, W, S, B, true>(p, st);
+        if (n >= 2ll * B * sm_count())
             return fmt == 0 ? launch_attn<HD, 0, 8, W / 2, S, 2 * B>(p, st) : launch_attn<HD, 1, 8, W / 2, S, 2 * B>(p, st);
     }
     return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B>(p, st) : launch_attn<HD, 1, 8, W, S, B>(p, st);

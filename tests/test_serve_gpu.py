@@ -168,6 +168,21 @@ def test_attention_lengths(L, lens):
     check(out, lse, want, lens)
 
 
+@pytest.mark.parametrize("n", [0, 1, 15, 16, 17, 40, 100, 255, 1000, 2048, 2049, 4096, 4100])
+def test_attention_small_calls(L, n):
+    """One or two sequences of few heads (a cluster of CTAs per unit) around the lengths where parts fall empty and where
+    another division takes over."""
+    for heads, kv, hd, dtype, lens in ((8, 2, 128, BF16, [n]), (7, 1, 64, E4M3, [n, 3]), (8, 8, 96, BF16, [5, n]),
+                                       (4, 4, 128, E4M3, [n])):
+        call, out, lse, want = attend(L, lens, heads, kv, hd, 16, dtype)
+        check(out, lse, want, lens)
+        first = out.clone()
+        for _ in range(3):
+            call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
+
+
 @pytest.mark.parametrize("window", [1, 7, 16, 100, 1024])
 def test_attention_window(L, window):
     lens = [1, window, window + 1, 3000, 0, 777]
