@@ -221,9 +221,10 @@ int paia_gemv_plan_destroy(paia_gemv_plan* plan);
  * page_table[b][j / page_size]. For query head h of kv head h / (heads / kv_heads):
  *   s_j = scale k_scale <q_h, k_j>,  p = softmax(s),  out_h = v_scale sum_j p_j v_j,  lse_h = log sum_j exp s_j
  * over the last `window` positions (0: all). Statistics and sums are fp32; out is rounded once to bf16. A sequence of
- * length 0 gives out = 0 and lse = -inf; so does a row whose scores are all -inf. Cache rows outside the range are never
- * read. A page id outside [0, num_pages) (code 10) reads as zero rows, a length above max_pages page_size is cut to it
- * and one below 0 is 0 (code 11).
+ * length 0 gives out = 0 and lse = -inf; so does a row whose scores are all -inf. A NaN or an infinity that is read makes
+ * what it reaches NaN or infinite (a score of -inf has no weight). Cache rows outside the range are never read. A page id
+ * outside [0, num_pages) (code 10) reads as zero rows, a length above max_pages page_size is cut to it and one below 0 is
+ * 0 (code 11).
  * q, out bf16; cache bf16 or e4m3 with a fp32 scale per kv head (value = stored * scale). head_dim 64, 96, 128 or 256;
  * any page size and page / token / head strides (both [page][token][head] and [page][head][token] caches);
  * batch * kv_heads * max_pages * page_size / 16 (times the 16-head units of a larger group) below 2^32. q, k and v 16-byte
@@ -292,8 +293,9 @@ int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* stream);
  * a = adapter[m],  out[m] = base[m] + scaling[a] B[a] (A[a] x[m]);  rows with adapter -1 get base[m]. Adapter a uses its
  * first ranks[a] ranks (NULL: all `rank`; 0: none; what lies behind them is not used), scaling NULL is 1, base NULL is 0,
  * base may be out itself. Sums are fp32, A x is kept in 32 bits between the two products, and out is rounded once to
- * bf16. An id outside [-1, adapters) (code 13) is treated as -1. rank, K and N are multiples of 8, rank <= 256,
- * adapters <= 8192. x, A, B, base, out 16-byte aligned with strides of whole 16 bytes. */
+ * bf16. A NaN or an infinity in x, A or B makes what it reaches NaN or infinite. An id outside [-1, adapters) (code 13) is
+ * treated as -1. rank, K and N are multiples of 8, rank <= 256, adapters <= 8192. x, A, B, base, out 16-byte aligned with
+ * strides of whole 16 bytes. */
 typedef struct paia_gemv_lora_args {
     const void* x;               /* bf16 [M][K] */
     const void* a;               /* bf16 [adapters][rank][K] */

@@ -500,7 +500,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
 #pragma unroll
                         for (int c = 0; c < kAttnCluster; ++c) {
                             const float2 ml = join_ml[c * rows + r];
-                            if (ml.x == -INFINITY) continue;                     // no part, or nothing in it
+                            if (ml.y == 0.f) continue;                           // no part, or nothing in it (NaN is)
                             const float4 a = *reinterpret_cast<const float4*>(join_o + (c * rows + r) * HD + d);
                             const float f = ex2(ml.x - ref);
                             ll += f * ml.y;

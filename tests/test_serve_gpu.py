@@ -183,6 +183,40 @@ def test_attention_small_calls(L, n):
         assert torch.equal(out, first)
 
 
+@pytest.mark.parametrize("heads,kv,hd,dtype", [(8, 2, 128, BF16), (4, 4, 64, E4M3), (16, 1, 128, BF16), (4, 2, 256, BF16)])
+@pytest.mark.parametrize("lens", [[17], [40, 3000], [3] * 200])
+def test_attention_nan_stays_nan(L, heads, kv, hd, dtype, lens):
+    """A NaN query makes its own head NaN in every division of the work; a NaN key in a part of its own (the last of 17
+    positions) makes its kv head's outputs NaN; nothing else changes."""
+    from paia_gemv import serve
+    g = gen(9)
+    k, v, table = C.paged(lens, kv, hd, 16, dtype, "cuda", g)
+    q = torch.randn(len(lens), heads, hd, generator=g, device="cuda").to(BF16)
+    n = torch.tensor(lens, dtype=torch.int32, device="cuda")
+    ws = serve.attention_workspace(L, heads, kv, hd)
+
+    def run():
+        out, lse = torch.empty_like(q), torch.empty(q.shape[:2], device="cuda")
+        serve.paged_attention(L, q, k, v, table, n, out, ws, lse=lse)
+        return out, lse
+    clean, clean_lse = run()
+    q[0, 1, 5] = math.nan
+    out, lse = run()
+    assert out[0, 1].isnan().all() and lse[0, 1].isnan()
+    out[0, 1], lse[0, 1] = clean[0, 1], clean_lse[0, 1]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+    q[0, 1, 5] = 0.0
+    clean, clean_lse = run()
+    at = lens[0] - 1
+    k.view(torch.uint8 if dtype is E4M3 else torch.int16)[table[0, at // 16], at % 16, kv - 1, 3] = \
+        0x7F if dtype is E4M3 else 0x7FFF
+    out, lse = run()
+    hit = slice(heads - heads // kv, heads)
+    assert out[0, hit].isnan().all() and lse[0, hit].isnan().all()
+    out[0, hit], lse[0, hit] = clean[0, hit], clean_lse[0, hit]
+    assert torch.equal(out, clean) and torch.equal(lse, clean_lse)
+
+
 @pytest.mark.parametrize("window", [1, 7, 16, 100, 1024])
 def test_attention_window(L, window):
     lens = [1, window, window + 1, 3000, 0, 777]
