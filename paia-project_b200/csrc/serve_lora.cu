@@ -5,8 +5,10 @@
 // Bound: HBM on the adapters' weights (rank (K + N) elements of each adapter that appears), latency where they are few.
 // One launch, a cluster of up to 8 CTAs per item; an item is one adapter with up to 16 of its rows (rows without an adapter
 // form items of rank 0 that copy base):
-//   who       The launch does not know which adapters appear. Every CTA counts the rows per adapter in shared memory and
-//             finds its cluster's item by a prefix sum, then lists the item's rows; surplus clusters leave at once.
+//   who       The launch does not know which adapters appear. Up to 256 rows: a row per thread, which finds its place
+//             among the rows of its adapter. More: every CTA counts the rows per adapter in shared memory and finds its
+//             item by a prefix sum, then lists the item's rows; where there are more items than CTAs it takes a run of
+//             them, and the search goes on where it stopped. Surplus clusters leave at once.
 //   A x       K is cut over the cluster's CTAs and their warps in blocks of 32; MMA rows are ranks, columns the item's
 //             rows. Each lane loads 16 bytes of an A row and of an x row at a time: a block's k order is permuted alike
 //             for both, which the sum does not see. A CTA's warps meet in shared memory; each CTA stores its share into
@@ -16,7 +18,9 @@
 //             group's tile j is n = 8 (c / 2) + 2 j + c % 2, so that a lane ends up with 8 neighbouring columns of its
 //             row: base is read and out written 16 bytes at a time.
 // Measured: 128 rows of as many adapters of rank 64, K 14336, N 4096: 53 us (5.8 TB/s). 61 rows of 24 adapters of mixed
-// rank up to 32, K 4096, N 28672: 18.5 us, phases that each wait for memory once. 8 rows, rank 16, K 4096, N 6144: 6.1 us.
+// rank up to 32, K 4096, N 28672: 18.7 us, phases that each wait for memory once. 8 rows, rank 16, K 4096, N 6144: 6.1 us.
+// A prompt's rows of one adapter of rank 16, K = N = 4096: 8192 in 67 us, 32768 in 241 (a search of all rows for every
+// item: 90 and 716).
 #include <cooperative_groups.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
@@ -41,28 +45,27 @@ struct LoraParams {
     long long x_row, base_row, out_row, a_adapter, a_row, b_adapter, b_row;
     int M, N, K, rank, adapters;
     int cluster;                             // CTAs per item: 8, 4, 2 or 1
+    int run;                                 // M > 256 and cluster 1: the items are shared out over the grid's CTAs
 };
 
-// Shared memory: the adapters' row counts first, then (over them) a rank group's partial sums of the warps
-// [warp][rank 64][row 16]; t of every CTA's share of K [CTA][rank][row] fp32 (8 rows where the call has no more); t as
-// bf16 hi and lo [row 16][rank + 8]. Ranks padded to 32.
-__host__ __device__ constexpr size_t lora_parts(int adapters) {
-    const size_t counts = (size_t)(adapters + 1) * 4, parts = (size_t)kLoraWarps * kLoraGroup * kLoraRows * 4;
-    return ((counts > parts ? counts : parts) + 15) / 16 * 16;
-}
+// Shared memory: a rank group's partial sums of the warps [warp][rank 64][row 16]; t of every CTA's share of K
+// [CTA][rank][row] fp32 (8 rows where the call has no more); t as bf16 hi and lo [row 16][rank + 8], ranks padded to 32;
+// with more than 256 rows the adapters' row counts.
+constexpr size_t kLoraParts = (size_t)kLoraWarps * kLoraGroup * kLoraRows * 4;
 __host__ __device__ constexpr int lora_pad(int rank) { return (rank + 31) / 32 * 32; }
 inline size_t lora_smem(int adapters, int rank, int M, int cluster) {
     const size_t r = (size_t)lora_pad(rank);
-    return lora_parts(adapters) + cluster * r * (M <= 8 ? 8 : 16) * 4 + 2 * kLoraRows * (r + 8) * 2;
+    return kLoraParts + cluster * r * (M <= 8 ? 8 : 16) * 4 + 2 * kLoraRows * (r + 8) * 2 +
+           (M > kLoraThreads ? (size_t)(adapters + 1) * 4 : 0);
 }
 
-__device__ __forceinline__ int lora_id(const LoraParams& p, int m) {
-    int a = __ldg(p.adapter + m);
+// The count that a row's adapter id belongs to: the last one is of the rows without an adapter.
+__device__ __forceinline__ int lora_id(const LoraParams& p, int a) {
     if (a < -1 || a >= p.adapters) {
         serve_error(kErrAdapter);
         a = -1;
     }
-    return a < 0 ? p.adapters : a;                                               // the last count: no adapter
+    return a < 0 ? p.adapters : a;
 }
 __device__ __forceinline__ uint4 load16(const __nv_bfloat16* p) { return *reinterpret_cast<const uint4*>(p); }
 // The first n of 8 bf16 values, zeros behind.
@@ -259,121 +262,38 @@ __device__ __forceinline__ void lora_expand(const LoraParams& p, const __nv_bflo
     }
 }
 
-__global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams p) {
-    extern __shared__ __align__(16) uint8_t smem[];
-    __shared__ int sh_rows[kLoraRows], sh_warp[kLoraWarps], sh_item[4], sh_ranks[kLoraThreads];
-    const cg::cluster_group cluster = cg::this_cluster();
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
-    const int me = (int)cluster.block_rank(), item = (int)(blockIdx.x / p.cluster);
-    int* counts = reinterpret_cast<int*>(smem);
-    float* parts = reinterpret_cast<float*>(smem);
-    const int rpad = lora_pad(p.rank);
-    const int t_rows = p.M <= 8 ? 8 : 16;
-    float* t_all = reinterpret_cast<float*>(smem + lora_parts(p.adapters));      // [CTA][rank][row]
-    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_all + p.cluster * rpad * t_rows);
-    __nv_bfloat16* t_lo = t_hi + kLoraRows * (rpad + 8);
-
-    pdl_trigger();
-    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");                // this CTA runs: others may store here
-    pdl_wait();
-    // ---- the item: adapter id and up to 16 of its rows
-    if (tid == 0) {
-        sh_item[0] = -1;
-        sh_item[2] = 0;
+// The running total of n over the CTA's threads before this one; `all`: of all of them.
+__device__ __forceinline__ int cta_before(int n, int* sh_warp, int warp, int lane, int& all) {
+    int inc = n;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const int y = __shfl_up_sync(~0u, inc, o);
+        if (lane >= o) inc += y;
     }
-    if (p.M <= kLoraThreads) {
-        // a row per thread; its place among the rows of its adapter, each 16th of which begins an item
-        int* ids = counts;
-        const int mine = tid < p.M ? lora_id(p, tid) : -1;
-        // ranks: of all adapters where they are few (one latency less), else of the row's
-        sh_ranks[tid] = p.ranks && tid < p.adapters ? __ldg(p.ranks + tid) : p.rank;
-        int my_rank = 0;
-        if (p.adapters > kLoraThreads && mine >= 0 && mine < p.adapters) my_rank = p.ranks ? __ldg(p.ranks + mine) : p.rank;
-        ids[tid] = mine;
-        __syncthreads();
-        int at = __popc(__match_any_sync(~0u, mine) & ((1u << lane) - 1u));
-#pragma unroll 4
-        for (int m = 0; m < min(warp * 32, p.M); m += 4) {                       // ids behind M are -1
-            const int4 v = *reinterpret_cast<const int4*>(ids + m);
-            at += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
-        }
-        const bool begins = mine >= 0 && at % kLoraRows == 0;
-        const unsigned ball = __ballot_sync(~0u, begins);
-        if (lane == 0) sh_warp[warp] = __popc(ball);
-        __syncthreads();
-        int number = __popc(ball & ((1u << lane) - 1u));
-        for (int w = 0; w < warp; ++w) number += sh_warp[w];
-        if (begins && number == item) {
-            sh_item[0] = mine;
-            sh_item[1] = at;
-            sh_item[3] = mine == p.adapters ? 0 : p.adapters > kLoraThreads ? my_rank : sh_ranks[mine];
-        }
-        __syncthreads();
-        if (mine >= 0 && mine == sh_item[0] && at >= sh_item[1] && at < sh_item[1] + kLoraRows) {
-            sh_rows[at - sh_item[1]] = tid;
-            atomicAdd(sh_item + 2, 1);
-        }
-    } else {
-        for (int i = tid; i <= p.adapters; i += kLoraThreads) counts[i] = 0;
-        __syncthreads();
-        for (int m0 = 0; m0 < p.M; m0 += kLoraThreads) {
-            const int m = m0 + tid;
-            const int a = m < p.M ? lora_id(p, m) : -1;
-            const unsigned same = __match_any_sync(~0u, a);
-            if (a >= 0 && lane == __ffs(same) - 1) atomicAdd(counts + a, __popc(same));
-        }
-        __syncthreads();
-        int before = 0;
-        for (int i0 = 0; i0 <= p.adapters; i0 += kLoraThreads) {
-            const int i = i0 + tid;
-            const int n = i <= p.adapters ? (counts[i] + kLoraRows - 1) / kLoraRows : 0;
-            int inc = n;
-            for (int o = 1; o < 32; o <<= 1) {
-                const int y = __shfl_up_sync(~0u, inc, o);
-                if (lane >= o) inc += y;
-            }
-            if (lane == 31) sh_warp[warp] = inc;
-            __syncthreads();
-            int block = 0, pre = 0;
-            for (int w = 0; w < kLoraWarps; ++w) {
-                if (w < warp) pre += sh_warp[w];
-                block += sh_warp[w];
-            }
-            const int lo = before + pre + inc - n;
-            if (n && item >= lo && item < lo + n) {
-                sh_item[0] = i;
-                sh_item[1] = (item - lo) * kLoraRows;
-                sh_item[2] = min(kLoraRows, counts[i] - (item - lo) * kLoraRows);
-            }
-            before += block;
-            __syncthreads();
-            if (item < before) break;
-        }
-        const int found = sh_item[0], skip = found < 0 ? 0 : sh_item[1], want = found < 0 ? 0 : sh_item[2];
-        if (tid == 0 && found >= 0) sh_item[3] = found == p.adapters ? 0 : p.ranks ? __ldg(p.ranks + found) : p.rank;
-        for (int m0 = 0, seen = 0; m0 < p.M && seen < skip + want; m0 += kLoraThreads) {
-            const int m = m0 + tid;
-            const bool mine = m < p.M && lora_id(p, m) == found;
-            const unsigned ball = __ballot_sync(~0u, mine);
-            if (lane == 0) sh_warp[warp] = __popc(ball);
-            __syncthreads();
-            int at = seen, block = 0;
-            for (int w = 0; w < kLoraWarps; ++w) {
-                if (w < warp) at += sh_warp[w];
-                block += sh_warp[w];
-            }
-            at += __popc(ball & ((1u << lane) - 1u));
-            if (mine && at >= skip && at < skip + want) sh_rows[at - skip] = m;
-            seen += block;
-            __syncthreads();
-        }
+    if (lane == 31) sh_warp[warp] = inc;
+    __syncthreads();
+    int pre = 0;
+    all = 0;
+#pragma unroll
+    for (int w = 0; w < kLoraWarps; ++w) {
+        if (w < warp) pre += sh_warp[w];
+        all += sh_warp[w];
     }
     __syncthreads();
-    const int id = sh_item[0], rows = sh_item[2], rank = min(max(sh_item[3], 0), p.rank);
-    if (id < 0) {                                                                // a whole cluster leaves together
-        asm volatile("barrier.cluster.wait;" ::: "memory");
-        return;
-    }
+    return pre + inc - n;
+}
+
+// One item: the rows sh_rows of adapter `id` (rank 0: copies of base). The cluster has arrived at its barrier once before.
+__device__ __forceinline__ void lora_item(const LoraParams& p, uint8_t* smem, const int* sh_rows, int id, int rows,
+                                          int rank) {
+    const cg::cluster_group cluster = cg::this_cluster();
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5, g = lane >> 2, t = lane & 3;
+    const int me = (int)cluster.block_rank();
+    float* parts = reinterpret_cast<float*>(smem);
+    const int rpad = lora_pad(p.rank), t_rows = p.M <= 8 ? 8 : 16;
+    float* t_all = reinterpret_cast<float*>(smem + kLoraParts);                  // [CTA][rank][row]
+    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_all + p.cluster * rpad * t_rows);
+    __nv_bfloat16* t_lo = t_hi + kLoraRows * (rpad + 8);
     const __nv_bfloat16* A = p.a + (long long)(rank ? id : 0) * p.a_adapter;
     const __nv_bfloat16* B = p.b + (long long)(rank ? id : 0) * p.b_adapter;
     // ---- this CTA's columns, in groups of 32
@@ -457,6 +377,159 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
 #undef EXPAND
 }
 
+// MANY: more than 256 rows.
+template <bool MANY>
+__global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams p) {
+    extern __shared__ __align__(16) uint8_t smem[];
+    __shared__ int sh_rows[kLoraRows], sh_warp[4 * kLoraWarps], sh_item[4], sh_ranks[kLoraThreads];
+    __shared__ int sh_end, sh_scan[3];                       // MANY: the items' end; where the search for rows goes on
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    int item = (int)(blockIdx.x / p.cluster);
+    const int rpad = lora_pad(p.rank), t_rows = p.M <= 8 ? 8 : 16;
+    int* counts = reinterpret_cast<int*>(smem + kLoraParts + p.cluster * rpad * t_rows * 4 + 4 * kLoraRows * (rpad + 8));
+
+    pdl_trigger();
+    asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");                // this CTA runs: others may store here
+    pdl_wait();
+    // ---- the item: adapter id and up to 16 of its rows
+    if (tid == 0) {
+        sh_item[0] = -1;
+        sh_item[2] = 0;
+    }
+    auto load_ids = [&](int m0, int* a) {                    // 1024 rows' ids, four per thread
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const int m = m0 + j * kLoraThreads + tid;
+            a[j] = m < p.M ? __ldg(p.adapter + m) : -1;
+        }
+    };
+    if constexpr (!MANY) {
+        // a row per thread; its place among the rows of its adapter, each 16th of which begins an item
+        int* ids = reinterpret_cast<int*>(smem);
+        const int mine = tid < p.M ? lora_id(p, __ldg(p.adapter + tid)) : -1;
+        // ranks: of all adapters where they are few (one latency less), else of the row's
+        sh_ranks[tid] = p.ranks && tid < p.adapters ? __ldg(p.ranks + tid) : p.rank;
+        int my_rank = 0;
+        if (p.adapters > kLoraThreads && mine >= 0 && mine < p.adapters) my_rank = p.ranks ? __ldg(p.ranks + mine) : p.rank;
+        ids[tid] = mine;
+        __syncthreads();
+        int at = __popc(__match_any_sync(~0u, mine) & ((1u << lane) - 1u));
+#pragma unroll 4
+        for (int m = 0; m < min(warp * 32, p.M); m += 4) {                       // ids behind M are -1
+            const int4 v = *reinterpret_cast<const int4*>(ids + m);
+            at += (v.x == mine) + (v.y == mine) + (v.z == mine) + (v.w == mine);
+        }
+        const bool begins = mine >= 0 && at % kLoraRows == 0;
+        const unsigned ball = __ballot_sync(~0u, begins);
+        if (lane == 0) sh_warp[warp] = __popc(ball);
+        __syncthreads();
+        int number = __popc(ball & ((1u << lane) - 1u));
+        for (int w = 0; w < warp; ++w) number += sh_warp[w];
+        if (begins && number == item) {
+            sh_item[0] = mine;
+            sh_item[1] = at;
+            sh_item[3] = mine == p.adapters ? 0 : p.adapters > kLoraThreads ? my_rank : sh_ranks[mine];
+        }
+        __syncthreads();
+        if (mine >= 0 && mine == sh_item[0] && at >= sh_item[1] && at < sh_item[1] + kLoraRows) {
+            sh_rows[at - sh_item[1]] = tid;
+            atomicAdd(sh_item + 2, 1);
+        }
+    } else {
+        for (int i = tid; i <= p.adapters; i += kLoraThreads) counts[i] = 0;
+        __syncthreads();
+        for (int m0 = 0; m0 < p.M; m0 += 4 * kLoraThreads) {
+            int a[4];
+            load_ids(m0, a);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const int x = m0 + j * kLoraThreads + tid < p.M ? lora_id(p, a[j]) : -1;
+                const unsigned same = __match_any_sync(~0u, x);
+                if (x >= 0 && lane == __ffs(same) - 1) atomicAdd(counts + x, __popc(same));
+            }
+        }
+        __syncthreads();
+        if (p.run) {                                                             // this CTA's share of the items
+            int items = 0, all;
+            for (int i0 = 0; i0 <= p.adapters; i0 += kLoraThreads) {
+                const int i = i0 + tid;
+                cta_before(i <= p.adapters ? (counts[i] + kLoraRows - 1) / kLoraRows : 0, sh_warp, warp, lane, all);
+                items += all;
+            }
+            item = (int)((long long)items * blockIdx.x / gridDim.x);
+            if (tid == 0) sh_end = (int)((long long)items * (blockIdx.x + 1) / gridDim.x);
+        } else if (tid == 0) {
+            sh_end = item + 1;
+        }
+        if (tid == 0) sh_scan[0] = -1;                                           // adapter, row, rows of it before that
+        __syncthreads();
+    }
+#pragma unroll 1
+    for (;; ++item) {
+        if (MANY && item < sh_end) {
+            int before = 0;
+            for (int i0 = 0; i0 <= p.adapters && before <= item; i0 += kLoraThreads) {
+                const int i = i0 + tid;
+                const int n = i <= p.adapters ? (counts[i] + kLoraRows - 1) / kLoraRows : 0;
+                int all;
+                const int lo = before + cta_before(n, sh_warp, warp, lane, all);
+                if (n && item >= lo && item < lo + n) {
+                    sh_item[0] = i;
+                    sh_item[1] = (item - lo) * kLoraRows;
+                    sh_item[2] = min(kLoraRows, counts[i] - (item - lo) * kLoraRows);
+                    sh_item[3] = i == p.adapters ? 0 : p.ranks ? __ldg(p.ranks + i) : p.rank;
+                }
+                before += all;
+            }
+            __syncthreads();
+            // its rows, from where the last item of the same adapter ended
+            const int found = sh_item[0], skip = sh_item[1], want = found < 0 ? 0 : sh_item[2];
+            const bool on = found == sh_scan[0];
+            int seen = on ? sh_scan[2] : 0;
+            for (int m0 = on ? sh_scan[1] : 0; want && seen < skip + want; m0 += 4 * kLoraThreads) {
+                int a[4], v = 0;
+                load_ids(m0, a);
+                unsigned ball[4];
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    ball[j] = __ballot_sync(~0u, m0 + j * kLoraThreads + tid < p.M && lora_id(p, a[j]) == found);
+                    if (lane == j) v = __popc(ball[j]);
+                }
+                if (lane < 4) sh_warp[lane * kLoraWarps + warp] = v;             // matches of 32 rows each, in row order
+                __syncthreads();
+                const int mine = sh_warp[lane];
+                int inc = mine;
+#pragma unroll
+                for (int o = 1; o < 32; o <<= 1) {
+                    const int y = __shfl_up_sync(~0u, inc, o);
+                    if (lane >= o) inc += y;
+                }
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    const int at = seen + __shfl_sync(~0u, inc - mine, j * kLoraWarps + warp) +
+                                   __popc(ball[j] & ((1u << lane) - 1u));
+                    if ((ball[j] >> lane & 1) && at >= skip && at < skip + want)
+                        sh_rows[at - skip] = m0 + j * kLoraThreads + tid;
+                }
+                if (tid == 0) sh_scan[0] = found, sh_scan[1] = m0, sh_scan[2] = seen;
+                seen += __shfl_sync(~0u, inc, 31);
+                __syncthreads();
+            }
+        }
+        __syncthreads();
+        const int id = sh_item[0], rows = sh_item[2], rank = min(max(sh_item[3], 0), p.rank);
+        if (id < 0 || (MANY && item >= sh_end)) {                       // a whole cluster leaves together
+            asm volatile("barrier.cluster.wait;" ::: "memory");
+            return;
+        }
+        lora_item(p, smem, sh_rows, id, rows, rank);
+        if (!MANY || item + 1 >= sh_end) return;
+        __syncthreads();                                                         // shared memory is free again
+        if (tid == 0) sh_item[0] = -1;
+        asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");
+    }
+}
+
 }  // namespace
 
 int lora_device_error(int clear) { return serve_error_word(clear); }
@@ -467,7 +540,7 @@ using namespace pb2;
 
 extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     if (!a || a->M < 0 || a->N < 8 || a->K < 8 || a->N % 8 || a->K % 8 || a->rank < 8 || a->rank % 8 ||
-        a->rank > kLoraMaxRank || a->adapters < 1 || a->adapters > kLoraMaxAdapters)
+        a->M > 1 << 30 || a->rank > kLoraMaxRank || a->adapters < 1 || a->adapters > kLoraMaxAdapters)
         return -2;
     if (a->M == 0) return 0;
     if (!a->x || !a->a || !a->b || !a->adapter || !a->out) return -2;
@@ -492,7 +565,7 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     p.M = a->M; p.N = a->N; p.K = a->K;
     p.rank = a->rank;
     p.adapters = a->adapters;
-    static std::atomic<unsigned long long> done{0};
+    static std::atomic<unsigned long long> done[2]{};
     // at most one item that is not full per adapter that appears (and one for the rows without)
     const long long kinds = a->M < a->adapters + 1 ? a->M : a->adapters + 1;
     const long long items = (a->M + (kLoraRows - 1) * kinds) / kLoraRows;
@@ -501,9 +574,13 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     p.cluster = 8;
     while (p.cluster > 1 && items * p.cluster > 2ll * sm_count()) p.cluster /= 2;
     if (items * p.cluster > 0x7fffffffll) return -2;
+    p.run = a->M > kLoraThreads && p.cluster == 1;
+    const long long most = p.run && items > 2ll * sm_count() ? 2ll * sm_count() : items;
     const size_t smem = lora_smem(a->adapters, a->rank, a->M, p.cluster);
-    const int rc = serve_allow_smem((const void*)lora_kernel, lora_smem(kLoraMaxAdapters, kLoraMaxRank, 16, 8), done);
+    const auto fn = a->M > kLoraThreads ? lora_kernel<true> : lora_kernel<false>;
+    const int rc = serve_allow_smem((const void*)fn, lora_smem(kLoraMaxAdapters, kLoraMaxRank, kLoraThreads + 1, 8),
+                                    done[a->M > kLoraThreads]);
     if (rc) return rc;
-    return serve_launch(lora_kernel, p, dim3((unsigned)(items * p.cluster)), kLoraThreads, smem,
+    return serve_launch(fn, p, dim3((unsigned)(most * p.cluster)), kLoraThreads, smem,
                         static_cast<cudaStream_t>(stream), p.cluster);
 }

@@ -541,6 +541,15 @@ def test_lora_many_adapters_and_rows(L):
     lora_case(L, 3000, 64, 72, 8, 2, [(m * m) % 3 - 1 for m in range(3000)])
 
 
+@pytest.mark.parametrize("M,bank,rank,ids", [
+    (257, 1, 8, lambda m: 0), (2500, 3, 16, lambda m: m % 4 - 1), (6000, 1, 24, lambda m: 0),
+    (5200, 700, 8, lambda m: m * m % 701 - 1), (9000, 300, 8, lambda m: 299 if m > 1000 else m % 7),
+    (20000, 5, 72, lambda m: -1 if m % 11 else m % 5), (400, 8192, 256, lambda m: (m * 41) % 8192)])
+def test_lora_prompt_rows(L, M, bank, rank, ids):
+    """More items than CTAs: each takes a run of them, over adapters of one row and of thousands."""
+    lora_case(L, M, 40, 24, rank, bank, [ids(m) for m in range(M)])
+
+
 def test_lora_strided(L):
     from paia_gemv import serve
     g = gen(8)
