@@ -15,21 +15,23 @@
 //             page size and strides, rows outside the range arrive as zeros) and running on across sequences and
 //             heads; no warp waits for another while it streams. Page ids are looked up for 32 tiles at a time, a tile
 //             per lane. 16-byte chunks are XOR-swizzled by row so that the fragment reads are free of bank conflicts.
-//   math      The group's query heads are rows of the MMAs (S = Q K^T, O += P V).
+//   math      S = Q K^T and O += P V, the group's query heads as rows of the MMAs.
 //             bf16: m16n8k16. With up to 8 heads, rows 8-15 carry the rounding remainder of P (P = hi + lo, two bf16), so
 //             P V is good to 2^-16 at no extra instruction; a group of 9 to 16 spends a second MMA on it.
 //             e4m3: the stored bytes become f16 exactly and meet q in f16, scaled per head by a power of two so that its
-//             largest element is in [1, 2) (only elements below 2^-14 of it lose bits); P is f16 there (2^-11). The order
-//             of the k dimension and of V's columns is free, so a lane reads its bytes 16 at a time. (The e4m3 form of
-//             mma.sync was no shorter way: 17% more instructions, 64 sequences of 8192 in 270 us where this took 257
-//             at the time.)
+//             largest element is in [1, 2) (only elements below 2^-14 of it lose bits); P is f16 there (2^-11). P has no
+//             remainder to fill rows 8-15 with, so the second product is taken as O^T += V^T P^T, dims as rows: half
+//             the MMAs and sums (16 sequences of 4096 at head_dim 256: 31 us where rows of heads spilled and took 64).
+//             The order of the k dimension and of V's columns is free, so a lane reads its bytes 16 at a time. (The
+//             e4m3 form of mma.sync was no shorter way: 17% more instructions, 64 sequences of 8192 in 270 us where
+//             this took 257 at the time.)
 //             Larger groups are cut into units of 16 heads.
 //   join      At the end of a run's part of a (sequence, head) the CTA's warps merge through shared memory. A part that
 //             is not the whole goes to the workspace, and the last CTA to arrive merges all parts in list order (the
 //             same bits whichever CTA it is) and resets the counter; no CTA waits for another. Small calls take a
 //             cluster per unit instead, whose CTAs store their parts into the first one's shared memory.
 // Measured (head_dim 128): one sequence of 131072 positions, 32/8 heads, bf16: 87.6 us, 6.1 TB/s; 64 sequences of 8192,
-// 16/8 heads, e4m3: 169 us, 6.4 TB/s, while the SM clock holds (as much bound by instruction issue); one sequence of 1024:
+// 16/8 heads, e4m3: 164 us, 6.5 TB/s, while the SM clock holds (as much bound by instruction issue); one sequence of 1024:
 // 5.8 us.
 #include <cooperative_groups.h>
 #include "paia_gemv.h"
@@ -67,11 +69,11 @@ struct AttnParams {
     float scale_log2;
 };
 
-// A tile is 16 or 32 positions, so that its K and V rows are 8 KB where they can be (e4m3 needs 32 for its MMA).
-template <int HD, int FMT>
+// A tile is 16 or 32 positions, so that its K and V rows are 8 KB where they can be.
+template <int HD, int FMT, int ROWS>
 struct AttnTile {
     static constexpr int kEs = FMT == 0 ? 2 : 1;
-    static constexpr int kPos = FMT == 0 && HD >= 96 ? 16 : 32;
+    static constexpr int kPos = (FMT == 0 && HD >= 96) || (HD == 256 && ROWS == 8) ? 16 : 32;
     static constexpr int kChunks = HD * kEs / 16;                                // 16-byte chunks per row
     static constexpr int kRow = kChunks <= 4 ? 64 : kChunks <= 8 ? 128 : kChunks <= 16 ? 256 : 512;
     static constexpr int kMat = kPos * kRow;
@@ -129,9 +131,9 @@ __device__ __forceinline__ int unit_places(const AttnParams& p, int b) {
 template <class V>
 __device__ __forceinline__ V* remote(V* p, int cta) { return cooperative_groups::this_cluster().map_shared_rank(p, cta); }
 
-template <int HD, int FMT, int W, int S>
+template <int HD, int FMT, int ROWS, int W, int S>
 struct AttnSmem {
-    using T = AttnTile<HD, FMT>;
+    using T = AttnTile<HD, FMT, ROWS>;
     static constexpr int kStride = HD + 4;                                       // floats per merged row
     static constexpr size_t kRing = (size_t)W * S * T::kStage;
     static size_t bytes(int rows, int cluster) {
@@ -165,13 +167,13 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
 // CL: a cluster of kAttnCluster CTAs per unit instead of a run of the list per CTA.
 template <int HD, int FMT, int ROWS, int W, int S, int MINB, bool CL>
 __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnParams p) {
-    using T = AttnTile<HD, FMT>;
-    using SM = AttnSmem<HD, FMT, W, S>;
+    using T = AttnTile<HD, FMT, ROWS>;
+    using SM = AttnSmem<HD, FMT, ROWS, W, S>;
     constexpr int kUnitCost = unit_cost(W);
     constexpr int POS = T::kPos, NB = POS / 16;                                  // blocks of 16 positions
     constexpr int KS = HD / 16;                                                  // k steps of Q K^T
     constexpr int NT = HD / 8;                                                   // column tiles of P V
-    constexpr int QR = ROWS == 8 ? 2 : 4;
+    constexpr int QR = ROWS == 8 ? 2 : 4, HB = ROWS / 8;                         // HB: blocks of 8 heads
     using F8 = Frag8<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int sh_last;
@@ -401,7 +403,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
             }
         }
     };
-    float acc[NT][4], qscale[2], m[2], l[2];
+    // tiles of 16 x 8. bf16: heads x dims (up to 8 heads: rows 8-15 are their remainders); e4m3: dims x heads
+    float acc[FMT == 0 ? NT : NT / 2 * HB][4], qscale[2], m[2], l[2];
     int stage = 0, base = 0, part = 0, head = 0, row0 = 0, nrow = 0;             // base: list places of earlier parts
 #pragma unroll 1
     for (int it = 0;; ++it) {
@@ -423,25 +426,30 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                     l[h] += __shfl_xor_sync(~0u, l[h], 1);
                     l[h] += __shfl_xor_sync(~0u, l[h], 2);
                     const int r = g + 8 * h;
-                    if (r < nrow) {
-                        if (t == 0) merge_ml[warp * rows + r] = make_float2(m[h], l[h]);
+                    if (r < nrow && t == 0) merge_ml[warp * rows + r] = make_float2(m[h], l[h]);
+                    if (FMT == 0) {
                         float* o = merge_o + (warp * rows + r) * SM::kStride;
-                        if (FMT == 0) {
+                        if (r < nrow) {
 #pragma unroll
                             for (int j = 0; j < NT; ++j)
                                 *reinterpret_cast<float2*>(o + 8 * j + 2 * t) =
                                     ROWS == 8 ? make_float2(acc[j][0] + acc[j][2], acc[j][1] + acc[j][3])
                                               : make_float2(acc[j][2 * h], acc[j][2 * h + 1]);
-                        } else {
+                        }
+                    } else {
+#pragma unroll
+                        for (int c = 0; c < 2; ++c) {
+                            if (8 * h + 2 * t + c >= nrow) continue;
+                            float* o = merge_o + (warp * rows + 8 * h + 2 * t + c) * SM::kStride;
 #pragma unroll
                             for (int u = 0; u < NT / F8::UV; ++u)
 #pragma unroll
-                                for (int c = 0; c < 2; ++c)
-#pragma unroll
-                                    for (int i = 0; i < F8::UV; i += 4)
-                                        *reinterpret_cast<float4*>(o + F8::v_unit(u, 2 * t + c) + i) =
-                                            make_float4(acc[u * F8::UV + i][2 * h + c], acc[u * F8::UV + i + 1][2 * h + c],
-                                                        acc[u * F8::UV + i + 2][2 * h + c], acc[u * F8::UV + i + 3][2 * h + c]);
+                                for (int i = 0; i < F8::UV; i += 4) {
+                                    const int j = (u * F8::UV + i) / 2;
+                                    const float *x = acc[j * HB + h], *y = acc[(j + 1) * HB + h];
+                                    *reinterpret_cast<float4*>(o + F8::v_unit(u, g) + i) =
+                                        make_float4(x[c], x[2 + c], y[c], y[2 + c]);
+                                }
                         }
                     }
                 }
@@ -614,7 +622,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 qscale[1] *= ks;
             }
 #pragma unroll
-            for (int j = 0; j < NT; ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
+            for (int j = 0; j < (FMT == 0 ? NT : NT / 2 * HB); ++j) acc[j][0] = acc[j][1] = acc[j][2] = acc[j][3] = 0.f;
             m[0] = m[1] = -INFINITY;
             l[0] = l[1] = 0.f;
         }
@@ -662,7 +670,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
         // ---- running softmax; lane has positions 8 n + 2 t, + 1 of rows g and g + 8
         const int p0 = (seg.first + seg.tile + place - base) * POS;
         const bool edge = p0 < seg.start || p0 + POS > seg.len;
-        uint32_t pa[NB][4], pl[NB][4];                                       // P as A fragments
+        uint32_t pa[NB][4], pl[NB][4];                                       // P as A fragments (e4m3: two B fragments)
         float fix[2] = {1.f, 1.f};
         bool moved = false;
 #pragma unroll
@@ -716,21 +724,35 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 } else {
                     pa[n][h] = pack_f16(y[0], y[1]);
                     pa[n][2 + h] = pack_f16(y[2], y[3]);
-                    if (ROWS == 8) pa[n][1] = pa[n][3] = 0u;
                 }
             }
         }
         if (__any_sync(~0u, moved)) {
-            const float f1 = ROWS == 8 ? fix[0] : fix[1];                    // rows 8-15: the remainders of 0-7
+            if (FMT == 0) {
+                const float f1 = ROWS == 8 ? fix[0] : fix[1];                // rows 8-15: the remainders of 0-7
 #pragma unroll
-            for (int j = 0; j < NT; ++j) {
-                acc[j][0] *= fix[0];
-                acc[j][1] *= fix[0];
-                acc[j][2] *= f1;
-                acc[j][3] *= f1;
+                for (int j = 0; j < NT; ++j) {
+                    acc[j][0] *= fix[0];
+                    acc[j][1] *= fix[0];
+                    acc[j][2] *= f1;
+                    acc[j][3] *= f1;
+                }
+            } else {
+#pragma unroll
+                for (int h = 0; h < HB; ++h) {
+                    const float f0 = __shfl_sync(~0u, fix[h], 8 * t), f1 = __shfl_sync(~0u, fix[h], 8 * t + 4);
+#pragma unroll
+                    for (int j = 0; j < NT / 2; ++j) {
+                        float* x = acc[j * HB + h];
+                        x[0] *= f0;
+                        x[1] *= f1;
+                        x[2] *= f0;
+                        x[3] *= f1;
+                    }
+                }
             }
         }
-        // ---- O += P V
+        // ---- O += P V (e4m3: O^T += V^T P^T)
         if (FMT == 0) {
             const uint32_t va = vd + T::at((lane & 7) + ((lane >> 3) & 1) * 8, lane >> 4);
 #pragma unroll
@@ -766,8 +788,8 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                             uint32_t a0, a1, b0, b1;
                             e4m3x4_f16x4(__byte_perm(w[0][q], w[1][q], sel), a0, a1);
                             e4m3x4_f16x4(__byte_perm(w[2][q], w[3][q], sel), b0, b1);
-                            mma_f16(acc[j], pa[n][0], pa[n][1], pa[n][2], pa[n][3], a0, b0);
-                            mma_f16(acc[j + 1], pa[n][0], pa[n][1], pa[n][2], pa[n][3], a1, b1);
+#pragma unroll
+                            for (int h = 0; h < HB; ++h) mma_f16(acc[j / 2 * HB + h], a0, a1, b0, b1, pa[n][h], pa[n][2 + h]);
                         }
                 }
             }
@@ -780,7 +802,7 @@ template <int HD, int FMT, int ROWS, int W, int S, int MINB, bool CL = false>
 int launch_attn(const AttnParams& p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     const auto fn = paged_attn_kernel<HD, FMT, ROWS, W, S, MINB, CL>;
-    using SM = AttnSmem<HD, FMT, W, S>;
+    using SM = AttnSmem<HD, FMT, ROWS, W, S>;
     constexpr int C = CL ? kAttnCluster : 0;
     const int rc = serve_allow_smem((const void*)fn, SM::bytes(ROWS, C), done);
     if (rc) return rc;
@@ -793,27 +815,28 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
     return serve_launch(fn, p, dim3((unsigned)grid), W * 32, smem, st);
 }
 
-// Four warps per CTA, two CTAs per SM (head_dim 256: one, its sums fill the registers), two stages per warp: one tile
-// (8 KB, 16 KB at head_dim 256) in flight while one is worked on. Three stages are slower: 1 x 128k 90.2 us against 86.0,
+// Four warps per CTA, two CTAs per SM (one at head_dim 256 in bf16 or with more than 8 heads: its sums fill the registers),
+// two stages per warp: one tile (8 KB; where there is one CTA 16 KB) in flight while one is worked on. Three stages are slower: 1 x 128k 90.2 us against 86.0,
 // 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us. Where every CTA gets two units or more,
 // CTAs of two warps, twice as many: fewer warps wait at the end of each short unit (256 x 64 positions 25.2 us with four,
 // 18.6 with two; 128 x 1: 12.8 and 9.1; but 1 x 128k 86 and 95). Where a cluster of CTAs per unit leaves every CTA an SM of
 // its own and the table holds at most 128 tiles per sequence, that: the parts join through distributed shared memory
-// instead of the workspace (1 x 1024 positions 5.4 us against 7.5, 1 x 2048 7.0 and 8.8; 1 x 4096 9.8 and 9.6).
+// instead of the workspace (1 x 1024 positions 5.4 us against 7.5, 1 x 2048 7.0 and 8.8; 1 x 4096 9.8 and 9.6; at head_dim
+// 256 1 x 1024 7.6 and 10.4).
 template <int HD>
 int pick_attn(const AttnParams& p, int fmt, cudaStream_t st) {
     constexpr int W = 4, S = 2, B = HD == 256 ? 1 : 2;
     if (p.group > 8) return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
+    const long long n = (long long)p.batch * p.kv_heads * p.chunks;
+    const int cap = p.max_pages * p.page_size, most = p.window && p.window < cap ? p.window : cap;
+    const int pos = fmt == 0 ? AttnTile<HD, 0, 8>::kPos : AttnTile<HD, 1, 8>::kPos;
+    if (n * kAttnCluster <= sm_count() && (most + pos - 1) / pos <= kAttnSmall)
+        return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B, true>(p, st) : launch_attn<HD, 1, 8, W, S, B, true>(p, st);
     if constexpr (HD < 256) {
-        const long long n = (long long)p.batch * p.kv_heads * p.chunks;
-        const int cap = p.max_pages * p.page_size, most = p.window && p.window < cap ? p.window : cap;
-        const int pos = fmt == 0 ? AttnTile<HD, 0>::kPos : AttnTile<HD, 1>::kPos;
-        if (n * kAttnCluster <= sm_count() && (most + pos - 1) / pos <= kAttnSmall)
-            return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B, true>(p, st) : launch_attn<HD, 1, 8, W, S, B, true>(p, st);
         if (n >= 2ll * B * sm_count())
             return fmt == 0 ? launch_attn<HD, 0, 8, W / 2, S, 2 * B>(p, st) : launch_attn<HD, 1, 8, W / 2, S, 2 * B>(p, st);
     }
-    return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B>(p, st) : launch_attn<HD, 1, 8, W, S, B>(p, st);
+    return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B>(p, st) : launch_attn<HD, 1, 8, W, S, 2>(p, st);
 }
 
 bool attn_sizes(int heads, int kv_heads, int head_dim) {

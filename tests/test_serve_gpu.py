@@ -173,7 +173,7 @@ def test_attention_small_calls(L, n):
     """One or two sequences of few heads (a cluster of CTAs per unit) around the lengths where parts fall empty and where
     another division takes over."""
     for heads, kv, hd, dtype, lens in ((8, 2, 128, BF16, [n]), (7, 1, 64, E4M3, [n, 3]), (8, 8, 96, BF16, [5, n]),
-                                       (4, 4, 128, E4M3, [n])):
+                                       (4, 4, 128, E4M3, [n]), (16, 2, 256, BF16, [n]), (12, 2, 256, E4M3, [n, 1])):
         call, out, lse, want = attend(L, lens, heads, kv, hd, 16, dtype)
         check(out, lse, want, lens)
         first = out.clone()
