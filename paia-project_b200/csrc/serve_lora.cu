@@ -22,6 +22,7 @@
 // A prompt's rows of one adapter of rank 16, K = N = 4096: 8192 in 67 us, 32768 in 241 (a search of all rows for every
 // item: 90 and 716).
 #include <cooperative_groups.h>
+#include <math.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 
@@ -44,19 +45,19 @@ struct LoraParams {
     __nv_bfloat16* out;
     long long x_row, base_row, out_row, a_adapter, a_row, b_adapter, b_row;
     int M, N, K, rank, adapters;
-    int cluster;                             // CTAs per item: 8, 4, 2 or 1
+    int cluster;                             // CTAs per item: 1 to 8
     int run;                                 // M > 256 and cluster 1: the items are shared out over the grid's CTAs
 };
 
-// Shared memory: a rank group's partial sums of the warps [warp][rank 64][row 16]; t of every CTA's share of K
-// [CTA][rank][row] fp32 (8 rows where the call has no more); t as bf16 hi and lo [row 16][rank + 8], ranks padded to 32;
-// with more than 256 rows the adapters' row counts.
+// Shared memory: a rank group's partial sums of the warps [warp][rank 64][row 16], then (over them) t as bf16 hi and lo
+// [row 16][rank + 8], ranks padded to 32; t of every CTA's share of K [CTA][rank][row] fp32 (8 rows where the call has no
+// more); with more than 256 rows the adapters' row counts.
 constexpr size_t kLoraParts = (size_t)kLoraWarps * kLoraGroup * kLoraRows * 4;
 __host__ __device__ constexpr int lora_pad(int rank) { return (rank + 31) / 32 * 32; }
+static_assert(kLoraParts >= 2 * kLoraRows * (kLoraMaxRank + 8) * 2, "t fits over the partial sums");
 inline size_t lora_smem(int adapters, int rank, int M, int cluster) {
     const size_t r = (size_t)lora_pad(rank);
-    return kLoraParts + cluster * r * (M <= 8 ? 8 : 16) * 4 + 2 * kLoraRows * (r + 8) * 2 +
-           (M > kLoraThreads ? (size_t)(adapters + 1) * 4 : 0);
+    return kLoraParts + cluster * r * (M <= 8 ? 8 : 16) * 4 + (M > kLoraThreads ? (size_t)(adapters + 1) * 4 : 0);
 }
 
 // The count that a row's adapter id belongs to: the last one is of the rows without an adapter.
@@ -292,7 +293,7 @@ __device__ __forceinline__ void lora_item(const LoraParams& p, uint8_t* smem, co
     float* parts = reinterpret_cast<float*>(smem);
     const int rpad = lora_pad(p.rank), t_rows = p.M <= 8 ? 8 : 16;
     float* t_all = reinterpret_cast<float*>(smem + kLoraParts);                  // [CTA][rank][row]
-    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(t_all + p.cluster * rpad * t_rows);
+    __nv_bfloat16* t_hi = reinterpret_cast<__nv_bfloat16*>(smem);                // the partial sums are done with by then
     __nv_bfloat16* t_lo = t_hi + kLoraRows * (rpad + 8);
     const __nv_bfloat16* A = p.a + (long long)(rank ? id : 0) * p.a_adapter;
     const __nv_bfloat16* B = p.b + (long long)(rank ? id : 0) * p.b_adapter;
@@ -386,7 +387,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     int item = (int)(blockIdx.x / p.cluster);
     const int rpad = lora_pad(p.rank), t_rows = p.M <= 8 ? 8 : 16;
-    int* counts = reinterpret_cast<int*>(smem + kLoraParts + p.cluster * rpad * t_rows * 4 + 4 * kLoraRows * (rpad + 8));
+    int* counts = reinterpret_cast<int*>(smem + kLoraParts + p.cluster * rpad * t_rows * 4);
 
     pdl_trigger();
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");                // this CTA runs: others may store here
@@ -530,6 +531,29 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
     }
 }
 
+constexpr size_t kLoraHalf = 110 * 1024;    // shared memory with which two CTAs fit on an SM; 8 KB more, and they do not
+// How many clusters of this size run at once on the current device, with one or two CTAs of this shared memory per SM.
+int lora_wave(void (*fn)(const LoraParams), int cluster, size_t smem) {
+    static std::atomic<int> known[64][9][2];
+    const int two = smem <= kLoraHalf;
+    int d = 0, n = 0;
+    if (cudaGetDevice(&d) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (d < 64 && (n = known[d][cluster][two].load(std::memory_order_relaxed))) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3(kLoraThreads);
+    cfg.dynamicSmemBytes = two ? kLoraHalf : kLoraHalf + 8 * 1024;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (d < 64) known[d][cluster][two].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 }  // namespace
 
 int lora_device_error(int clear) { return serve_error_word(clear); }
@@ -569,18 +593,26 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     // at most one item that is not full per adapter that appears (and one for the rows without)
     const long long kinds = a->M < a->adapters + 1 ? a->M : a->adapters + 1;
     const long long items = (a->M + (kLoraRows - 1) * kinds) / kLoraRows;
-    // The more items, the fewer CTAs to each: what an item costs beside its weights (finding it, joining t, the ramps) is
-    // paid once per wave, so all items run in one wave of two CTAs per SM where they can.
-    p.cluster = 8;
-    while (p.cluster > 1 && items * p.cluster > 2ll * sm_count()) p.cluster /= 2;
-    if (items * p.cluster > 0x7fffffffll) return -2;
-    p.run = a->M > kLoraThreads && p.cluster == 1;
-    const long long most = p.run && items > 2ll * sm_count() ? 2ll * sm_count() : items;
-    const size_t smem = lora_smem(a->adapters, a->rank, a->M, p.cluster);
     const auto fn = a->M > kLoraThreads ? lora_kernel<true> : lora_kernel<false>;
     const int rc = serve_allow_smem((const void*)fn, lora_smem(kLoraMaxAdapters, kLoraMaxRank, kLoraThreads + 1, 8),
                                     done[a->M > kLoraThreads]);
     if (rc) return rc;
+    // The more items, the fewer CTAs to each: what an item costs beside its weights (finding it, joining t, the ramps) is
+    // paid once per wave, so all items run in one wave where they can. A cluster stays within a GPC, so this is less than
+    // the SMs hold: with 37 items of rank 16, N 6144, clusters of 8 take 13.1 us, of 6 7.8; with 74 items 4 and 3: 17.0 and
+    // 11.9; with 148 items 2 and 1: 16.9 and 21.2. (7 fit no more items than 8: 24.5 us for 37 of rank 64, 6 take 16.9.)
+    // Which adapters the rows have is not known here: where there is one for every row, every row may have its own; where
+    // they have to share, they are taken to fall evenly (61 rows of 24 of 32 adapters: 18.8 us so, 20.6 for the worst case).
+    const double even = (double)kinds * (1.0 - pow(1.0 - 1.0 / (double)kinds, (double)a->M));
+    const long long likely = a->M <= a->adapters ? items : (a->M + (long long)((kLoraRows - 1) * even)) / kLoraRows;
+    for (p.cluster = 8; p.cluster > 1; --p.cluster)
+        if (p.cluster != 7 && likely <= lora_wave(fn, p.cluster, lora_smem(a->adapters, a->rank, a->M, p.cluster))) break;
+    if (items * p.cluster > 0x7fffffffll) return -2;
+    p.run = a->M > kLoraThreads && p.cluster == 1;
+    const long long most = p.run && items > 2ll * sm_count() ? 2ll * sm_count() : items;
+    // Where an SM per CTA is enough, so much shared memory that no two share one: 12 items of rank 64 9.0 us, else 11.0.
+    size_t smem = lora_smem(a->adapters, a->rank, a->M, p.cluster);
+    if (smem <= kLoraHalf && likely <= lora_wave(fn, p.cluster, kLoraHalf + 1)) smem = kLoraHalf + 8 * 1024;
     return serve_launch(fn, p, dim3((unsigned)(most * p.cluster)), kLoraThreads, smem,
                         static_cast<cudaStream_t>(stream), p.cluster);
 }

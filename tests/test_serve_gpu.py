@@ -587,3 +587,10 @@ def test_lora_same_bits_whoever_shares_the_batch(L):
     one = lora_case(L, 12, 520, 520, 16, 4, [2] * 12)
     for _ in range(3):
         assert torch.equal(one, lora_case(L, 12, 520, 520, 16, 4, [2] * 12))
+
+
+@pytest.mark.parametrize("M", [33, 37, 43, 52, 65, 86, 129, 148, 149])
+@pytest.mark.parametrize("rank", [16, 256])
+def test_lora_every_cluster_size(L, M, rank):
+    """As many adapters as rows: 8 CTAs per item down to one, with K and N that do not divide by them."""
+    lora_case(L, M, 1000, 1208, rank, M, [(7 * m) % M for m in range(M)])
