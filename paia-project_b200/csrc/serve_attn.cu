@@ -32,7 +32,7 @@
 //             cluster per unit instead, whose CTAs store their parts into the first one's shared memory.
 // Measured (head_dim 128): one sequence of 131072 positions, 32/8 heads, bf16: 87.6 us, 6.1 TB/s; 64 sequences of 8192,
 // 16/8 heads, e4m3: 164 us, 6.5 TB/s, while the SM clock holds (as much bound by instruction issue); one sequence of 1024:
-// 5.8 us.
+// 5.3 us.
 #include <cooperative_groups.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
@@ -42,8 +42,8 @@ namespace {
 
 // What a unit costs beyond its tiles, in tiles of a CTA of W warps: its queries, merge and output.
 constexpr int unit_cost(int W) { return W == 4 ? 14 : 6; }
-constexpr int kAttnSmall = 128;             // tiles per sequence up to which small calls take a cluster per unit
-constexpr int kAttnCluster = 8;             // CTAs per unit of the small calls
+constexpr int kAttnCluster = 8;             // most CTAs per unit of the small calls
+constexpr int kAttnSmall = 16;              // tiles per CTA up to which small calls take a cluster per unit
 constexpr int kJoin = 8;                    // parts of a unit that are joined at a time
 constexpr int kAttnMaxGrid = 4 * 160;       // the workspace holds two parts per CTA of the largest grid
 
@@ -65,6 +65,7 @@ struct AttnParams {
     int batch, kv_heads, group, chunks;     // chunks: units of at most ROWS heads per kv head
     int num_pages, page_size, max_pages, window;
     int page_shift;                         // log2 of page_size, or -1
+    int cluster_log2;                       // log2 of the CTAs per unit of a small call
     int whole_blocks;                       // 16 positions in a row lie in one page, at strides below 2^27 bytes
     float scale_log2;
 };
@@ -164,7 +165,7 @@ __device__ __forceinline__ void lds_words(uint32_t a, uint32_t* w) {
         asm volatile("ld.shared.b32 %0, [%1];" : "=r"(w[0]) : "r"(a) : "memory");
 }
 
-// CL: a cluster of kAttnCluster CTAs per unit instead of a run of the list per CTA.
+// CL: a cluster of CTAs per unit instead of a run of the list per CTA.
 template <int HD, int FMT, int ROWS, int W, int S, int MINB, bool CL>
 __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnParams p) {
     using T = AttnTile<HD, FMT, ROWS>;
@@ -182,10 +183,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     const int rows = min(p.group, ROWS);
     float* merge_o = reinterpret_cast<float*>(smem + 512 + SM::kRing);                 // [W][rows][kStride]
     float2* merge_ml = reinterpret_cast<float2*>(merge_o + W * rows * SM::kStride);
-    const int rank = CL ? (int)(blockIdx.x % kAttnCluster) : 0;
+    const int cl = CL ? 1 << p.cluster_log2 : 0, rank = CL ? (int)blockIdx.x & (cl - 1) : 0;
     // CL, in CTA 0: every CTA's part of the unit, [CTA][rows][HD], then (m, l) [CTA][rows]
     float* join_o = reinterpret_cast<float*>(merge_ml + W * rows);
-    float2* join_ml = reinterpret_cast<float2*>(join_o + kAttnCluster * rows * HD);
+    float2* join_ml = reinterpret_cast<float2*>(join_o + cl * rows * HD);
 
     if (CL) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");        // this CTA runs: others may store here
     pdl_trigger();
@@ -196,14 +197,14 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     Cursor<POS, kUnitCost> seg;
     unsigned t0, t1, per = 1;
     if constexpr (CL) {
-        const int unit = (int)(blockIdx.x / kAttnCluster);
+        const int unit = (int)(blockIdx.x >> p.cluster_log2);
         seg.b = unit / units;
         seg.u = unit - seg.b * units;
         seg.w0 = 0;
         seg.load(p);
         seg.w0 = 0u - seg.unit_place();                                          // the unit's tiles are places 0, 1, ...
-        t0 = (unsigned)(seg.ntile * rank + kAttnCluster - 1) / kAttnCluster;     // CTA 0 has one at least
-        t1 = (unsigned)(seg.ntile * (rank + 1) + kAttnCluster - 1) / kAttnCluster;
+        t0 = (unsigned)(seg.ntile * rank + cl - 1) >> p.cluster_log2;            // CTA 0 has one at least
+        t1 = (unsigned)(seg.ntile * (rank + 1) + cl - 1) >> p.cluster_log2;
         seg.tile = (int)t0;
         if (t0 == t1) {                                                          // fewer tiles than CTAs: no part
             asm volatile("barrier.cluster.wait;" ::: "memory");
@@ -503,11 +504,12 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                         float mm = -INFINITY, ll = 0.f;
                         float4 o = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-                        for (int c = 0; c < kAttnCluster; ++c) mm = fmaxf(mm, join_ml[c * rows + r].x);
+                        for (int c = 0; c < kAttnCluster; ++c)
+                            if (c < cl) mm = fmaxf(mm, join_ml[c * rows + r].x);
                         const float ref = mm == -INFINITY ? 0.f : mm;
 #pragma unroll
                         for (int c = 0; c < kAttnCluster; ++c) {
-                            const float2 ml = join_ml[c * rows + r];
+                            const float2 ml = c < cl ? join_ml[c * rows + r] : make_float2(0.f, 0.f);
                             if (ml.y == 0.f) continue;                           // no part, or nothing in it (NaN is)
                             const float4 a = *reinterpret_cast<const float4*>(join_o + (c * rows + r) * HD + d);
                             const float f = ex2(ml.x - ref);
@@ -803,34 +805,42 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
     static std::atomic<unsigned long long> done{0};
     const auto fn = paged_attn_kernel<HD, FMT, ROWS, W, S, MINB, CL>;
     using SM = AttnSmem<HD, FMT, ROWS, W, S>;
-    constexpr int C = CL ? kAttnCluster : 0;
-    const int rc = serve_allow_smem((const void*)fn, SM::bytes(ROWS, C), done);
+    const size_t most = SM::bytes(ROWS, CL ? kAttnCluster : 0);
+    const int rc = serve_allow_smem((const void*)fn, CL && most < kSmemAlone ? kSmemAlone : most, done);
     if (rc) return rc;
-    const size_t smem = SM::bytes(p.group < ROWS ? p.group : ROWS, C);
-    if (CL)
-        return serve_launch(fn, p, dim3((unsigned)(p.batch * p.kv_heads * p.chunks * kAttnCluster)), W * 32, smem, st,
-                            kAttnCluster);
+    const int cluster = 1 << p.cluster_log2;
+    size_t smem = SM::bytes(p.group < ROWS ? p.group : ROWS, CL ? cluster : 0);
+    if constexpr (CL) {
+        // An SM per CTA where they suffice: 4 x 1024 positions 7.0 us, else 7.6.
+        static std::atomic<int> known[4][64];
+        const int n = p.batch * p.kv_heads * p.chunks;
+        if (smem < kSmemAlone && n <= serve_clusters(fn, cluster, W * 32, kSmemAlone, known[p.cluster_log2]))
+            smem = kSmemAlone;
+        return serve_launch(fn, p, dim3((unsigned)(n * cluster)), W * 32, smem, st, cluster);
+    }
     int grid = sm_count() * MINB;
     if (grid > kAttnMaxGrid) grid = kAttnMaxGrid;
     return serve_launch(fn, p, dim3((unsigned)grid), W * 32, smem, st);
 }
 
 // Four warps per CTA, two CTAs per SM (one at head_dim 256 in bf16 or with more than 8 heads: its sums fill the registers),
-// two stages per warp: one tile (8 KB; where there is one CTA 16 KB) in flight while one is worked on. Three stages are slower: 1 x 128k 90.2 us against 86.0,
-// 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us. Where every CTA gets two units or more,
-// CTAs of two warps, twice as many: fewer warps wait at the end of each short unit (256 x 64 positions 25.2 us with four,
-// 18.6 with two; 128 x 1: 12.8 and 9.1; but 1 x 128k 86 and 95). Where a cluster of CTAs per unit leaves every CTA an SM of
-// its own and the table holds at most 128 tiles per sequence, that: the parts join through distributed shared memory
-// instead of the workspace (1 x 1024 positions 5.4 us against 7.5, 1 x 2048 7.0 and 8.8; 1 x 4096 9.8 and 9.6; at head_dim
-// 256 1 x 1024 7.6 and 10.4).
+// two stages per warp: one tile (8 KB; where there is one CTA 16 KB) in flight while one is worked on. Three stages are
+// slower: 1 x 128k 90.2 us against 86.0, 32 ragged 23.4 against 21.9; six warps with fewer registers each spill: 101 us. Where
+// every CTA gets two units or more, CTAs of two warps, twice as many: fewer warps wait at the end of each short unit (256 x
+// 64 positions 25.2 us with four, 18.6 with two; 128 x 1: 12.8 and 9.1; but 1 x 128k 86 and 95). Where the units are so few that a cluster of 8, 4 or 2
+// CTAs for each leaves SMs enough, and the table holds at most 16 tiles per sequence for each of them, that: the parts join
+// through distributed shared memory instead of the workspace (8 kv heads: 1 x 1024 positions 5.3 us against 7.5, 1 x 2048
+// 6.8 and 8.8, 4 x 256 4.8 and 6.6, 4 x 1024 7.0 and 8.3, 8 x 256 5.5 and 7.5; with 32 tiles per CTA 1 x 4096 9.9 and 9.7,
+// 4 x 2048 11.9 and 11.3; at head_dim 256 1 x 1024 7.6 and 10.4).
 template <int HD>
-int pick_attn(const AttnParams& p, int fmt, cudaStream_t st) {
+int pick_attn(AttnParams& p, int fmt, cudaStream_t st) {
     constexpr int W = 4, S = 2, B = HD == 256 ? 1 : 2;
     if (p.group > 8) return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
     const long long n = (long long)p.batch * p.kv_heads * p.chunks;
     const int cap = p.max_pages * p.page_size, most = p.window && p.window < cap ? p.window : cap;
     const int pos = fmt == 0 ? AttnTile<HD, 0, 8>::kPos : AttnTile<HD, 1, 8>::kPos;
-    if (n * kAttnCluster <= sm_count() && (most + pos - 1) / pos <= kAttnSmall)
+    for (p.cluster_log2 = ilog2(kAttnCluster); p.cluster_log2 && n << p.cluster_log2 > sm_count();) --p.cluster_log2;
+    if (p.cluster_log2 && (most + pos - 1) / pos <= kAttnSmall << p.cluster_log2)
         return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B, true>(p, st) : launch_attn<HD, 1, 8, W, S, B, true>(p, st);
     if constexpr (HD < 256) {
         if (n >= 2ll * B * sm_count())

@@ -134,6 +134,31 @@ inline int serve_launch(void (*fn)(const P), const P& p, dim3 grid, int threads,
     return 0;
 }
 
+// Two CTAs fit on an SM with up to kSmemHalf bytes of dynamic shared memory each; with kSmemAlone a CTA has it to itself.
+constexpr size_t kSmemHalf = 110 * 1024, kSmemAlone = 118 * 1024;
+
+// How many clusters of kernel `fn` run at once on the current device (a cluster stays within a GPC, so it is less than the
+// SMs hold); known: 64 zeros to begin with, the answers by device.
+template <class P>
+inline int serve_clusters(void (*fn)(const P), int cluster, int threads, size_t smem, std::atomic<int>* known) {
+    int d = 0, n = 0;
+    if (cudaGetDevice(&d) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (d < 64 && (n = known[d].load(std::memory_order_relaxed))) return n;
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)cluster);
+    cfg.blockDim = dim3((unsigned)threads);
+    cfg.dynamicSmemBytes = smem;
+    cudaLaunchAttribute attr;
+    attr.id = cudaLaunchAttributeClusterDimension;
+    attr.val.clusterDim.x = (unsigned)cluster;
+    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
+    cfg.attrs = &attr;
+    cfg.numAttrs = 1;
+    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
+    if (d < 64) known[d].store(n, std::memory_order_relaxed);
+    return n;
+}
+
 inline bool aligned_to(const void* p, unsigned a) { return (reinterpret_cast<uintptr_t>(p) & (uintptr_t)(a - 1)) == 0; }
 
 int attn_device_error(int clear);

@@ -531,27 +531,11 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
     }
 }
 
-constexpr size_t kLoraHalf = 110 * 1024;    // shared memory with which two CTAs fit on an SM; 8 KB more, and they do not
-// How many clusters of this size run at once on the current device, with one or two CTAs of this shared memory per SM.
+// How many clusters of this size run at once, with one or two CTAs of this shared memory per SM.
 int lora_wave(void (*fn)(const LoraParams), int cluster, size_t smem) {
-    static std::atomic<int> known[64][9][2];
-    const int two = smem <= kLoraHalf;
-    int d = 0, n = 0;
-    if (cudaGetDevice(&d) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
-    if (d < 64 && (n = known[d][cluster][two].load(std::memory_order_relaxed))) return n;
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)cluster);
-    cfg.blockDim = dim3(kLoraThreads);
-    cfg.dynamicSmemBytes = two ? kLoraHalf : kLoraHalf + 8 * 1024;
-    cudaLaunchAttribute attr;
-    attr.id = cudaLaunchAttributeClusterDimension;
-    attr.val.clusterDim.x = (unsigned)cluster;
-    attr.val.clusterDim.y = attr.val.clusterDim.z = 1;
-    cfg.attrs = &attr;
-    cfg.numAttrs = 1;
-    if (cudaOccupancyMaxActiveClusters(&n, fn, &cfg) != cudaSuccess) { (void)cudaGetLastError(); return 0; }
-    if (d < 64) known[d][cluster][two].store(n, std::memory_order_relaxed);
-    return n;
+    static std::atomic<int> known[9][2][64];
+    const int two = smem <= kSmemHalf;
+    return serve_clusters(fn, cluster, kLoraThreads, two ? kSmemHalf : kSmemAlone, known[cluster][two]);
 }
 
 }  // namespace
@@ -612,7 +596,7 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
     const long long most = p.run && items > 2ll * sm_count() ? 2ll * sm_count() : items;
     // Where an SM per CTA is enough, so much shared memory that no two share one: 12 items of rank 64 9.0 us, else 11.0.
     size_t smem = lora_smem(a->adapters, a->rank, a->M, p.cluster);
-    if (smem <= kLoraHalf && likely <= lora_wave(fn, p.cluster, kLoraHalf + 1)) smem = kLoraHalf + 8 * 1024;
+    if (smem <= kSmemHalf && likely <= lora_wave(fn, p.cluster, kSmemAlone)) smem = kSmemAlone;
     return serve_launch(fn, p, dim3((unsigned)(most * p.cluster)), kLoraThreads, smem,
                         static_cast<cudaStream_t>(stream), p.cluster);
 }

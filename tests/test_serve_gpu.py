@@ -183,6 +183,21 @@ def test_attention_small_calls(L, n):
         assert torch.equal(out, first)
 
 
+@pytest.mark.parametrize("batch", [9, 14, 17, 19, 33, 37, 38, 74, 75])
+@pytest.mark.parametrize("hd,dtype", [(128, BF16), (64, BF16), (128, E4M3), (256, E4M3)])
+def test_attention_cluster_sizes(L, batch, hd, dtype):
+    """Clusters of 8, 4 and 2 CTAs per unit and none, for units from none to as many tiles as they take."""
+    most = 500 if hd >= 128 else 1000
+    lens = [(97 * i * i + 31 * i) % most if i % 7 else 0 for i in range(batch)]
+    lens[-1] = most
+    call, out, lse, want = attend(L, lens, 5, 1, hd, 16, dtype)
+    check(out, lse, want, lens)
+    first = out.clone()
+    call()
+    torch.cuda.synchronize()
+    assert torch.equal(out, first)
+
+
 @pytest.mark.parametrize("heads,kv,hd,dtype", [(8, 2, 128, BF16), (4, 4, 64, E4M3), (16, 1, 128, BF16), (4, 2, 256, BF16)])
 @pytest.mark.parametrize("lens", [[17], [40, 3000], [3] * 200])
 def test_attention_nan_stays_nan(L, heads, kv, hd, dtype, lens):
