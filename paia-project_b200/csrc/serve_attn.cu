@@ -808,16 +808,23 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
     const size_t most = SM::bytes(ROWS, CL ? kAttnCluster : 0);
     const int rc = serve_allow_smem((const void*)fn, CL && most < kSmemAlone ? kSmemAlone : most, done);
     if (rc) return rc;
-    const int cluster = 1 << p.cluster_log2;
-    size_t smem = SM::bytes(p.group < ROWS ? p.group : ROWS, CL ? cluster : 0);
+    const int rows = p.group < ROWS ? p.group : ROWS;
     if constexpr (CL) {
-        // An SM per CTA where they suffice: 4 x 1024 positions 7.0 us, else 7.6.
+        // An SM per CTA where they suffice: 4 x 1024 positions 7.0 us, else 7.6. Where the shared memory leaves no choice,
+        // so few CTAs per unit that all run at once.
         static std::atomic<int> known[4][64];
         const int n = p.batch * p.kv_heads * p.chunks;
-        if (smem < kSmemAlone && n <= serve_clusters(fn, cluster, W * 32, kSmemAlone, known[p.cluster_log2]))
-            smem = kSmemAlone;
-        return serve_launch(fn, p, dim3((unsigned)(n * cluster)), W * 32, smem, st, cluster);
+        AttnParams q = p;
+        for (;; --q.cluster_log2) {
+            const int cluster = 1 << q.cluster_log2;
+            const size_t smem = SM::bytes(rows, cluster);
+            const bool fits = n <= serve_clusters(fn, cluster, W * 32, smem > kSmemAlone ? smem : kSmemAlone, known[q.cluster_log2]);
+            if (smem > kSmemHalf && !fits && q.cluster_log2 > 1) continue;
+            return serve_launch(fn, q, dim3((unsigned)(n * cluster)), W * 32, fits && smem < kSmemAlone ? kSmemAlone : smem,
+                                st, cluster);
+        }
     }
+    const size_t smem = SM::bytes(rows, 0);
     int grid = sm_count() * MINB;
     if (grid > kAttnMaxGrid) grid = kAttnMaxGrid;
     return serve_launch(fn, p, dim3((unsigned)grid), W * 32, smem, st);
@@ -831,17 +838,23 @@ int launch_attn(const AttnParams& p, cudaStream_t st) {
 // CTAs for each leaves SMs enough, and the table holds at most 16 tiles per sequence for each of them, that: the parts join
 // through distributed shared memory instead of the workspace (8 kv heads: 1 x 1024 positions 5.3 us against 7.5, 1 x 2048
 // 6.8 and 8.8, 4 x 256 4.8 and 6.6, 4 x 1024 7.0 and 8.3, 8 x 256 5.5 and 7.5; with 32 tiles per CTA 1 x 4096 9.9 and 9.7,
-// 4 x 2048 11.9 and 11.3; at head_dim 256 1 x 1024 7.6 and 10.4).
+// 4 x 2048 11.9 and 11.3; at head_dim 256 1 x 1024 7.6 and 10.4; 2 kv heads of 16 query heads each 1 x 1024 8.4 and 12.9).
 template <int HD>
 int pick_attn(AttnParams& p, int fmt, cudaStream_t st) {
     constexpr int W = 4, S = 2, B = HD == 256 ? 1 : 2;
-    if (p.group > 8) return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
     const long long n = (long long)p.batch * p.kv_heads * p.chunks;
     const int cap = p.max_pages * p.page_size, most = p.window && p.window < cap ? p.window : cap;
     const int pos = fmt == 0 ? AttnTile<HD, 0, 8>::kPos : AttnTile<HD, 1, 8>::kPos;
     for (p.cluster_log2 = ilog2(kAttnCluster); p.cluster_log2 && n << p.cluster_log2 > sm_count();) --p.cluster_log2;
-    if (p.cluster_log2 && (most + pos - 1) / pos <= kAttnSmall << p.cluster_log2)
-        return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B, true>(p, st) : launch_attn<HD, 1, 8, W, S, B, true>(p, st);
+    const bool small = p.cluster_log2 && (most + pos - 1) / pos <= kAttnSmall << p.cluster_log2;
+    if (p.group > 8) {
+        if constexpr (HD < 256) {                            // (at 256 a cluster's parts do not fit beside the ring)
+            if (small)
+                return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B, true>(p, st) : launch_attn<HD, 1, 16, W, S, B, true>(p, st);
+        }
+        return fmt == 0 ? launch_attn<HD, 0, 16, W, S, B>(p, st) : launch_attn<HD, 1, 16, W, S, B>(p, st);
+    }
+    if (small) return fmt == 0 ? launch_attn<HD, 0, 8, W, S, B, true>(p, st) : launch_attn<HD, 1, 8, W, S, B, true>(p, st);
     if constexpr (HD < 256) {
         if (n >= 2ll * B * sm_count())
             return fmt == 0 ? launch_attn<HD, 0, 8, W / 2, S, 2 * B>(p, st) : launch_attn<HD, 1, 8, W / 2, S, 2 * B>(p, st);

@@ -190,12 +190,13 @@ def test_attention_cluster_sizes(L, batch, hd, dtype):
     most = 500 if hd >= 128 else 1000
     lens = [(97 * i * i + 31 * i) % most if i % 7 else 0 for i in range(batch)]
     lens[-1] = most
-    call, out, lse, want = attend(L, lens, 5, 1, hd, 16, dtype)
-    check(out, lse, want, lens)
-    first = out.clone()
-    call()
-    torch.cuda.synchronize()
-    assert torch.equal(out, first)
+    for heads in (5, 14, 20):                                     # one unit of 8 rows, one of 16, two of 16
+        call, out, lse, want = attend(L, lens, heads, 1, hd, 16, dtype)
+        check(out, lse, want, lens)
+        first = out.clone()
+        call()
+        torch.cuda.synchronize()
+        assert torch.equal(out, first)
 
 
 @pytest.mark.parametrize("heads,kv,hd,dtype", [(8, 2, 128, BF16), (4, 4, 64, E4M3), (16, 1, 128, BF16), (4, 2, 256, BF16)])
