@@ -332,3 +332,55 @@ def test_adapter_items_cover_every_row_once():
                 mine = [i for i in range(m) if ids[i] == a]
                 rows += [mine[k:k + 16] for k in range(0, len(mine), 16)]
         assert len(rows) <= items and sorted(i for r in rows for i in r) == list(range(m))
+
+
+def adapter_run(counts, key, m, item, end):
+    """(adapter, rows) of each item of a CTA's run [item, end), as the kernel searches for them 1024 rows at a time."""
+    scan, out = (-1, 0, 0), []
+    while item < end:
+        before, found = 0, None
+        for a, c in enumerate(counts):
+            n = (c + 15) // 16
+            if before <= item < before + n:
+                found = (a, (item - before) * 16, min(16, c - (item - before) * 16))
+            before += n
+        if found is None:
+            break
+        a, skip, want = found
+        m0, seen = scan[1:] if scan[0] == a else (0, 0)
+        rows = {}
+        while seen < skip + want:
+            assert m0 < m
+            mine = [r for r in range(m0, min(m0 + 1024, m)) if key[r] == a]
+            rows.update({seen + i - skip: r for i, r in enumerate(mine) if skip <= seen + i < skip + want})
+            scan = (a, m0, seen)
+            seen, m0 = seen + len(mine), m0 + 1024
+        out.append((a, [rows[i] for i in range(want)]))
+        item += 1
+    return out
+
+
+def test_adapter_runs_cover_every_row_once():
+    """More than 256 rows: the CTAs' runs of items hold every row once, under its adapter and in order, whatever the grid."""
+    rng = random.Random(6)
+    for trial in range(40):
+        m, adapters, grid = rng.choice([257, 1024, 1025, 4000]), rng.choice([1, 2, 7, 300]), rng.choice([1, 7, 64, 296])
+        key = [rng.randrange(adapters + 1) if trial % 2 else min(r * r % (adapters + 3), adapters) for r in range(m)]
+        counts = [key.count(a) for a in range(adapters + 1)]
+        items = sum((c + 15) // 16 for c in counts)
+        got = []
+        for cta in range(grid):
+            got += adapter_run(counts, key, m, items * cta // grid, items * (cta + 1) // grid)
+        assert len(got) == items and sorted(r for _, rows in got for r in rows) == list(range(m))
+        for a, rows in got:
+            assert rows == sorted(rows) and all(key[r] == a for r in rows)
+
+
+def test_attention_clusters_cover_every_tile_once():
+    """A small call's CTAs take neighbouring runs of their unit's tiles; the first has one at least."""
+    for log2 in (1, 2, 3):
+        c = 1 << log2
+        for n in range(1, 300):
+            runs = [((n * r + c - 1) >> log2, (n * (r + 1) + c - 1) >> log2) for r in range(c)]
+            assert runs[0][0] == 0 and runs[0][1] > 0 and runs[-1][1] == n
+            assert all(x[1] == y[0] for x, y in zip(runs, runs[1:]))
