@@ -292,10 +292,10 @@ int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* stream);
 /* Low-rank adapters of many requests beside a shared projection (paia_gemv_batched): for every row m with adapter
  * a = adapter[m],  out[m] = base[m] + scaling[a] B[a] (A[a] x[m]);  rows with adapter -1 get base[m]. Adapter a uses its
  * first ranks[a] ranks (NULL: all `rank`; 0: none; what lies behind them is not used), scaling NULL is 1, base NULL is 0,
- * base may be out itself. Sums are fp32, A x is kept in 32 bits between the two products, and out is rounded once to
- * bf16. A NaN or an infinity in x, A or B makes what it reaches NaN or infinite. An id outside [-1, adapters) (code 13) is
- * treated as -1. rank, K and N are multiples of 8, rank <= 256, adapters <= 8192, M <= 2^30. x, A, B, base, out
- * 16-byte aligned with strides of whole 16 bytes. */
+ * base may be out itself, x may not overlap out. Sums are fp32, A x is kept in 32 bits between the two products, and out
+ * is rounded once to bf16. A NaN or an infinity in x, A or B makes what it reaches NaN or infinite. An id outside
+ * [-1, adapters) (code 13) is treated as -1. rank, K and N are multiples of 8, rank <= 256, adapters <= 8192, M <= 2^30.
+ * x, A, B, base, out 16-byte aligned with strides of whole 16 bytes. */
 typedef struct paia_gemv_lora_args {
     const void* x;               /* bf16 [M][K] */
     const void* a;               /* bf16 [adapters][rank][K] */

@@ -557,7 +557,7 @@ extern "C" int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream) {
         a->x_row % 8 || a->base_row % 8 || a->out_row % 8 || a->a_adapter % 8 || a->a_row % 8 || a->b_adapter % 8 ||
         a->b_row % 8)
         return -2;
-    if (a->M > 1 && a->out_row == 0) return -2;
+    if ((a->M > 1 && a->out_row == 0) || a->x == a->out) return -2;                // rows on one another; x read after writes
     LoraParams p{};
     p.x = static_cast<const __nv_bfloat16*>(a->x);
     p.a = static_cast<const __nv_bfloat16*>(a->a);

@@ -217,8 +217,8 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
 
 def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, stream=None):
     """out[m] = base[m] + scaling[i] * b[i] (a[i] x[m]) for i = adapter[m] (int32; -1: out[m] = base[m]). x bf16 [M, K],
-    a bf16 [adapters, rank, K], b bf16 [adapters, N, rank], out and base (None: zeros; may be out) bf16 [M, N]; scaling
-    fp32 and ranks int32 [adapters] (None: 1 and `rank`): adapter i uses its first ranks[i] ranks."""
+    a bf16 [adapters, rank, K], b bf16 [adapters, N, rank], out (apart from x) and base (None: zeros; may be out) bf16
+    [M, N]; scaling fp32 and ranks int32 [adapters] (None: 1 and `rank`): adapter i uses its first ranks[i] ranks."""
     if _bind is not None and _bind.lora(lib.lora_entry, lib.device_entry, x, a, b, adapter, out, base, scaling, ranks,
                                         stream) == 0:
         return out

@@ -50,7 +50,7 @@ ROPE = dict(qkv=PTR, pos=PTR, seq=0, inv_freq=PTR, q_norm=0, k_norm=0, page_tabl
             k_out=0, k=PTR, v=PTR, qkv_token=1536, q_token=1024, q_head=128, ko_token=0, ko_head=0, table_seq=4,
             k_page=4096, k_row=256, k_head=128, v_page=4096, v_row=256, v_head=128, tokens=3, sequences=3, heads=8,
             kv_heads=2, head_dim=128, rot=128, interleaved=0, cache=0, num_pages=9, page_size=16, max_pages=4, eps=1e-6)
-LORA = dict(x=PTR, a=PTR, b=PTR, adapter=PTR, ranks=0, scaling=0, base=0, out=PTR, x_row=64, base_row=0, out_row=64,
+LORA = dict(x=PTR, a=PTR, b=PTR, adapter=PTR, ranks=0, scaling=0, base=0, out=2 * PTR, x_row=64, base_row=0, out_row=64,
             a_adapter=512, a_row=64, b_adapter=512, b_row=8, M=3, N=64, K=64, rank=8, adapters=2)
 
 
@@ -104,7 +104,7 @@ def test_rope_refusals(L, change):
     dict(adapters=0), dict(adapters=8193), dict(x=0), dict(a=0), dict(b=0), dict(adapter=0), dict(out=0), dict(x=PTR + 8),
     dict(a=PTR + 2), dict(b=PTR + 4), dict(base=PTR + 8), dict(out=PTR + 8), dict(adapter=PTR + 2), dict(ranks=PTR + 1),
     dict(scaling=PTR + 2), dict(x_row=65), dict(base_row=4), dict(out_row=68), dict(a_adapter=4), dict(a_row=66),
-    dict(b_adapter=2), dict(b_row=12), dict(out_row=0)])
+    dict(b_adapter=2), dict(b_row=12), dict(out_row=0), dict(out=PTR), dict(M=(1 << 30) + 1)])
 def test_lora_refusals(L, change):
     from paia_gemv import serve
     assert L._lib.paia_gemv_lora(packed("paia_gemv_lora_args", serve.LORA, LORA, **change), None) == -2
