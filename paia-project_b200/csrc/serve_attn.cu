@@ -19,7 +19,11 @@
 //             bf16: m16n8k16. With up to 8 heads, rows 8-15 carry the rounding remainder of P (P = hi + lo, two bf16), so
 //             P V is good to 2^-16 at no extra instruction; a group of 9 to 16 spends a second MMA on it.
 //             e4m3: the stored bytes become f16 exactly and meet q in f16, scaled per head by a power of two so that its
-//             largest element is in [1, 2) (only elements below 2^-14 of it lose bits); P is f16 there (2^-11). P has no
+//             largest element is in [1, 2) (only elements below 2^-14 of it lose bits); P is f16 there too, each rounded by
+//             2^-11 of its value: far below the output's own 2^-8, and on their own, so that over many positions they
+//             cancel. P is kept 2^15 times as large (m is the running maximum less 15; l and O are scaled alike and
+//             the join sees only differences of m), which f16 holds, so that this goes down to 2^-29 of the largest P
+//             and nothing above 2^-40 is dropped: many small ones can outweigh a large one whose v is small. P has no
 //             remainder to fill rows 8-15 with, so the second product is taken as O^T += V^T P^T, dims as rows: half
 //             the MMAs and sums (16 sequences of 4096 at head_dim 256: 31 us where rows of heads spilled and took 64).
 //             The order of the k dimension and of V's columns is free, so a lane reads its bytes 16 at a time. (The
@@ -175,6 +179,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     constexpr int KS = HD / 16;                                                  // k steps of Q K^T
     constexpr int NT = HD / 8;                                                   // column tiles of P V
     constexpr int QR = ROWS == 8 ? 2 : 4, HB = ROWS / 8;                         // HB: blocks of 8 heads
+    constexpr float kLift = FMT == 0 ? 0.f : 15.f;                               // m is the largest score less this
     using F8 = Frag8<HD>;
     extern __shared__ __align__(128) uint8_t smem[];
     __shared__ int sh_last;
@@ -694,9 +699,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
             for (int i = 0; i < 4 * NB; ++i) top = fmaxf(top, x[i]);
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
             top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-            if (top > m[h]) {
-                fix[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - top);
-                m[h] = top;
+            if (top - m[h] > kLift) {                                        // (-inf - -inf is no reason)
+                const float to = fabsf(top) < 8388608.f ? top - kLift : top; // beyond 2^23 the difference may round up
+                fix[h] = m[h] == -INFINITY ? 0.f : ex2(m[h] - to);
+                m[h] = to;
                 moved = true;
             }
             const float mm = m[h] == -INFINITY ? 0.f : m[h];

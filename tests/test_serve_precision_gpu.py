@@ -1,0 +1,103 @@
+"""How exactly the serving operators compute what they keep in fewer than 32 bits, at inputs that show it: probabilities and
+queries of an e4m3 cache's attention (f16 next to the stored bytes)."""
+import math
+
+import pytest
+import torch
+
+import serve_cases as C
+from serve_cases import BF16, E4M3, F32, HALF
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture(scope="module")
+def L():
+    if not torch.cuda.is_available():
+        pytest.skip("no CUDA device")
+    from paia_gemv import load_lib
+    lib = load_lib()
+    lib.device_error(True)
+    return lib
+
+
+def gen(seed):
+    return torch.Generator(device="cuda").manual_seed(seed)
+
+
+def within(got, want, tol, what=""):
+    assert torch.isfinite(got).all(), what
+    off = (got.double() - want).abs() - tol
+    assert not off.numel() or off.max().item() <= 0, (what, off.max().item(), tol.flatten()[off.argmax()].item())
+
+
+def attention8(q, k, v, table, lens, scale):
+    """(out, lse, bound of out, bound of lse) of an e4m3 cache without scales, as serve_cases.attention, but with what f16
+    may lose told apart by size: a probability is rounded by 2^-11 of its value down to 2^-29 of the largest and is off by
+    2^-40 of that below (f16's half step of 2^-25 under 2^15), a query element exact (8 bits) down to 2^-29 of its head's
+    largest and off by 2^-40 of that below."""
+    f = torch.float64
+    b, h, hd = q.shape
+    kv, page = k.shape[2], k.shape[1]
+    out, lse = torch.zeros(b, h, hd, dtype=f, device=q.device), torch.zeros(b, h, dtype=f, device=q.device)
+    tol, tol_lse = torch.zeros_like(out), torch.zeros_like(lse)
+    for i, n in enumerate(lens):
+        pos = torch.arange(n, device=q.device)
+        rows = table[i].long()[pos // page]
+        kk, vv = k[rows, pos % page].to(f), v[rows, pos % page].to(f)
+        for j in range(kv):
+            hs = slice(j * (h // kv), (j + 1) * (h // kv))
+            qq = q[i, hs].to(f)
+            s = scale * (qq @ kk[:, j].T)
+            ds = scale * (hd + 16) * F32 * (qq.abs() @ kk[:, j].abs().T) + 4 * F32 * s.abs()
+            ds = ds + scale * 2.0 ** -40 * qq.abs().amax(-1, keepdim=True) * kk[:, j].abs().sum(-1)
+            p = torch.softmax(s, -1)
+            z = torch.logsumexp(s, -1)
+            # an exponent's error moves its own term and the sum that it is divided by: ds of the term, and of the sum the
+            # terms' ds by their weight
+            e = ds + (p * ds).sum(-1, keepdim=True) + 2.0 ** -20 + (n / 16 + 64) * 2 * F32
+            e = e + 2 * F32 * (s.amax(-1, keepdim=True) - s + 16)            # the difference that ex2 is taken of
+            pe = p * 2.0 ** -11 + 2.0 ** -40 * torch.exp(s.amax(-1) - z)[:, None]
+            out[i, hs] = p @ vv[:, j]
+            tol[i, hs] = ((p * e + pe) @ vv[:, j].abs()) * (1 + 2.0 ** -7) + HALF[BF16] * out[i, hs].abs() + 1e-38
+            lse[i, hs] = z
+            tol_lse[i, hs] = ((p * ds).sum(-1) + 2.0 ** -20 + (n / 16 + 64) * F32
+                              + 4 * F32 * (z.abs() + s.abs().amax(-1) + 16))
+    return out, lse, tol, tol_lse
+
+
+def call(L, q, k, v, table, lens, scale):
+    from paia_gemv import serve
+    b, h, hd = q.shape
+    out, lse = torch.empty_like(q), torch.empty(b, h, device="cuda")
+    serve.paged_attention(L, q, k, v, table, torch.tensor(lens, dtype=torch.int32, device="cuda"), out,
+                          serve.attention_workspace(L, h, k.shape[2], hd), scale=scale, lse=lse)
+    torch.cuda.synchronize()
+    assert L.device_error(True) == 0
+    want = attention8(q, k, v, table, lens, scale)
+    within(out, want[0], want[2], "out")
+    within(lse, want[1], want[3], "lse")
+
+
+SHAPES = [(8, 2, 128), (4, 2, 64), (6, 1, 96), (4, 2, 256), (32, 2, 128), (12, 1, 64), (16, 1, 256)]
+
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+@pytest.mark.parametrize("gap", [0, 8, 14, 16, 18, 19.5])
+def test_e4m3_small_probabilities_beside_a_large_one(L, heads, kv, hd, gap):
+    """One position whose score lies `gap` above the others' middle and whose v is 0, at the front, in the middle and at the
+    end: the output is what the small probabilities leave."""
+    lens = [4000, 3001, 2500, 300, 40]
+    g = gen(21)
+    k, v, table = C.paged(lens, kv, hd, 16, E4M3, "cuda", g)
+    scale = max(gap, 1) / 2048.0
+    q = torch.randn(len(lens), heads, hd, generator=g, device="cuda")
+    q = (q / (scale * 30 * math.sqrt(hd))).to(BF16)               # the other scores: N(0, 1)
+    q[:, :, 0] = 8.0
+    k[..., 0] = 0.0
+    for b, at in enumerate((0, 1500, 2499, 150, 39)):
+        pg = table[b, at // 16].item()
+        k[pg, at % 16] = 0.0
+        k[pg, at % 16, :, 0] = 256.0 if gap else 0.0              # score 8 * 256 * scale = gap
+        v[pg, at % 16] = 0.0
+    call(L, q, k, v, table, lens, scale)
