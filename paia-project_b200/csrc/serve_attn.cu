@@ -19,12 +19,13 @@
 //             bf16: m16n8k16. With up to 8 heads, rows 8-15 carry the rounding remainder of P (P = hi + lo, two bf16), so
 //             P V is good to 2^-16 at no extra instruction; a group of 9 to 16 spends a second MMA on it.
 //             e4m3: the stored bytes become f16 exactly and meet q in f16, scaled per head by a power of two so that its
-//             largest element is in [1, 2) (only elements below 2^-14 of it lose bits); P is f16 there too, each rounded by
-//             2^-11 of its value: far below the output's own 2^-8, and on their own, so that over many positions they
-//             cancel. P is kept 2^15 times as large (m is the running maximum less 15; l and O are scaled alike and
-//             the join sees only differences of m), which f16 holds, so that this goes down to 2^-29 of the largest P
-//             and nothing above 2^-40 is dropped: many small ones can outweigh a large one whose v is small. P has no
-//             remainder to fill rows 8-15 with, so the second product is taken as O^T += V^T P^T, dims as rows: half
+//             largest element is in [2^15, 2^16): an element's 8 bits stay whole down to 2^-32 of the largest, and what
+//             is off below that is 2^-40 of it. P is f16 there too, each rounded by 2^-11 of its value: far below the
+//             output's own 2^-8, and on their own, so that over many positions they cancel. P is kept 2^15 times as
+//             large (m is the running maximum less 15; l and O are scaled alike and the join sees only differences of
+//             m), which f16 holds, so that this goes down to 2^-29 of the largest P and nothing above 2^-40 is dropped:
+//             many small ones can outweigh a large one whose v is small. P has no remainder to fill rows 8-15 with, so
+//             the second product is taken as O^T += V^T P^T, dims as rows: half
 //             the MMAs and sums (16 sequences of 4096 at head_dim 256: 31 us where rows of heads spilled and took 64).
 //             The order of the k dimension and of V's columns is free, so a lane reads its bytes 16 at a time. (The
 //             e4m3 form of mma.sync was no shorter way: 17% more instructions, 64 sequences of 8192 in 270 us where
@@ -611,11 +612,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                             top = fmaxf(top, fmaxf(fabsf(bf16_lo(qa[s][i])), fabsf(bf16_hi(qa[s][i]))));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 1));
                     top = fmaxf(top, __shfl_xor_sync(~0u, top, 2));
-                    // 2^e <= top < 2^(e + 1), from the exponent field; 0, infinities and NaN stay as they are
-                    const int ex = (int)(__float_as_uint(top) >> 23);
-                    const bool norm = ex > 1 && ex < 253;
-                    const float down = norm ? __uint_as_float((uint32_t)(254 - ex) << 23) : 1.f;
-                    qscale[h] *= norm ? __uint_as_float((uint32_t)ex << 23) : 1.f;
+                    // times 2^(up - 127), by top's exponent field (a tiny one: as far as a normal factor goes)
+                    const int up = min(253, 269 - (int)(__float_as_uint(top) >> 23));
+                    const float down = __uint_as_float((uint32_t)up << 23);
+                    qscale[h] *= __uint_as_float((uint32_t)(254 - up) << 23);
 #pragma unroll
                     for (int s = 0; s < KS; ++s)
 #pragma unroll

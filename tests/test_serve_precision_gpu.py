@@ -34,7 +34,7 @@ def within(got, want, tol, what=""):
 def attention8(q, k, v, table, lens, scale):
     """(out, lse, bound of out, bound of lse) of an e4m3 cache without scales, as serve_cases.attention, but with what f16
     may lose told apart by size: a probability is rounded by 2^-11 of its value down to 2^-29 of the largest and is off by
-    2^-40 of that below (f16's half step of 2^-25 under 2^15), a query element exact (8 bits) down to 2^-29 of its head's
+    2^-40 of that below (f16's half step of 2^-25 under 2^15), a query element exact (8 bits) down to 2^-32 of its head's
     largest and off by 2^-40 of that below."""
     f = torch.float64
     b, h, hd = q.shape
@@ -101,3 +101,26 @@ def test_e4m3_small_probabilities_beside_a_large_one(L, heads, kv, hd, gap):
         k[pg, at % 16, :, 0] = 256.0 if gap else 0.0              # score 8 * 256 * scale = gap
         v[pg, at % 16] = 0.0
     call(L, q, k, v, table, lens, scale)
+
+
+@pytest.mark.parametrize("heads,kv,hd", SHAPES)
+@pytest.mark.parametrize("small", [0, 10, 16, 20, 24])
+def test_e4m3_small_query_elements_beside_a_large_one(L, heads, kv, hd, small):
+    """A query whose largest element meets zeros in every key: the scores come from elements 2^-small times as large."""
+    lens = [2100, 500, 33]
+    g = gen(22)
+    k, v, table = C.paged(lens, kv, hd, 16, E4M3, "cuda", g)
+    q = (torch.randn(len(lens), heads, hd, generator=g, device="cuda") * 2.0 ** -small).to(BF16)
+    q[:, :, 0] = 5.0
+    k[..., 0] = 0.0
+    call(L, q, k, v, table, lens, 2.0 ** small / 30 / math.sqrt(hd))
+
+
+@pytest.mark.parametrize("size", [-120, -60, -20, 40, 100])
+def test_e4m3_queries_of_any_size(L, size):
+    """Scores of ordinary size from queries that f16 could not hold, and scale to match."""
+    lens = [700, 40]
+    g = gen(23)
+    k, v, table = C.paged(lens, 2, 128, 16, E4M3, "cuda", g)
+    q = (torch.randn(2, 8, 128, generator=g, device="cuda") * 2.0 ** size).to(BF16)
+    call(L, q, k, v, table, lens, 2.0 ** -size / 30 / math.sqrt(128))
