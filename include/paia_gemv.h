@@ -210,8 +210,9 @@ int paia_gemv_plan_launch(const paia_gemv_plan* plan, void* stream);
 int paia_gemv_plan_destroy(paia_gemv_plan* plan);
 
 /* ---- Serving operators beside the GEMVs (no reference kernel): a batched decode step's attention, rotary positions and
- * adapters. They launch with programmatic dependent launch, allocate nothing and never synchronise. Strides are counted
- * in elements and the innermost dimension is contiguous; 64-bit offsets throughout. Codes: 0, -2 bad argument, >0
+ * adapters. They launch with programmatic dependent launch (they touch memory, and let the next kernel start, only once the
+ * kernel before them is done), allocate nothing and never synchronise. Strides are counted in elements and the innermost
+ * dimension is contiguous; 64-bit offsets throughout. Codes: 0, -2 bad argument, >0
  * cudaError_t. Indices that live on the device (page ids, lengths, positions, adapter ids) are checked by the kernels:
  * a bad one is never followed to memory and sets a code of paia_gemv_device_error (10 page id, 11 length, 12 position
  * or sequence, 13 adapter id). */

@@ -195,8 +195,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     float2* join_ml = reinterpret_cast<float2*>(join_o + cl * rows * HD);
 
     if (CL) asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");        // this CTA runs: others may store here
-    pdl_trigger();
-    pdl_wait();
+    pdl_wait_and_trigger();
     // ---- this CTA's run [t0, t1) of the list, and the place it starts at. Every warp finds it for itself, so that none
     // waits for another: lane i counts the i-th 32nd of the sequences, one scan finds the lane that holds t0, a second
     // one the sequence among that lane's (a third and more beyond 1024 sequences).

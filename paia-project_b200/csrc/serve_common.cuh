@@ -28,10 +28,14 @@ static inline int serve_error_word(int clear) {
     return v;
 }
 
-// The operators launch with programmatic dependent launch: everything a kernel reads before pdl_wait() must not come
-// from the kernel before it on the stream.
-__device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-__device__ __forceinline__ void pdl_trigger() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+// The operators launch with programmatic dependent launch. The kernel before on the stream is done, and what it wrote is
+// visible, behind the wait: nothing that a caller may have written is read before it. The trigger comes after it and never
+// before: the next kernel may then read some of its inputs at once (a GEMV its weights and bias), and is promised that every
+// kernel but the one immediately before it is done.
+__device__ __forceinline__ void pdl_wait_and_trigger() {
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
 
 __device__ __forceinline__ uint32_t sptr(const void* p) { return (uint32_t)__cvta_generic_to_shared(p); }
 

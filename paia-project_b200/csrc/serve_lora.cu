@@ -389,9 +389,8 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
     const int rpad = lora_pad(p.rank), t_rows = p.M <= 8 ? 8 : 16;
     int* counts = reinterpret_cast<int*>(smem + kLoraParts + p.cluster * rpad * t_rows * 4);
 
-    pdl_trigger();
     asm volatile("barrier.cluster.arrive.relaxed;" ::: "memory");                // this CTA runs: others may store here
-    pdl_wait();
+    pdl_wait_and_trigger();
     // ---- the item: adapter id and up to 16 of its rows
     if (tid == 0) {
         sh_item[0] = -1;

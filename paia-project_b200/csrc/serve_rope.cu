@@ -231,8 +231,7 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
     float* table = tables[warp];
     // the norms' weights as the lanes read them
     __shared__ __align__(16) float weights[2][512];          // q, k: 8 for d0 of every lane, 8 for d1
-    pdl_trigger();
-    pdl_wait();
+    pdl_wait_and_trigger();
     if (any_norm) {
         for (int e = threadIdx.x; e < 2 * 16 * lanes; e += kRopeThreads) {
             const int which = e / (16 * lanes), rest = e % (16 * lanes), h = rest / (8 * lanes), l = rest % (8 * lanes) >> 3,
