@@ -97,7 +97,7 @@ struct Cursor {
     int b, u, tile, ntile, first, start, len;
     unsigned w0;
     __device__ __forceinline__ void load(const AttnParams& p) {
-        const int n = __ldg(p.lens + b);
+        const int n = p.lens[b];
         len = min(max(n, 0), p.max_pages * p.page_size);
         start = p.window > 0 && len > p.window ? len - p.window : 0;
         first = start / POS;
@@ -295,7 +295,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 const int pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
                 w.in[n] = pos - pg * p.page_size;
                 w.id[n] = -1;
-                if (p.whole_blocks && w.range == POS << 8) w.id[n] = __ldg(p.table + is.b * p.table_batch + pg);
+                if (p.whole_blocks && w.range == POS << 8) w.id[n] = p.table[is.b * p.table_batch + pg];
             }
         }
         return w;
@@ -354,7 +354,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
             long long ko = 0, vo = 0;
             if (ok) {
                 const int pos = p0 + r, pg = p.page_shift >= 0 ? pos >> p.page_shift : pos / p.page_size;
-                const int id = __ldg(p.table + b * p.table_batch + pg), in = pos - pg * p.page_size;
+                const int id = p.table[b * p.table_batch + pg], in = pos - pg * p.page_size;
                 ok = (unsigned)id < (unsigned)p.num_pages;
                 if (ok) {
                     ko = id * p.k_page + in * p.k_token + head * p.k_head;
@@ -378,7 +378,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
     };
     if (blockIdx.x == 0)                                                         // report lengths that were cut
         for (int b = tid; b < p.batch; b += W * 32) {
-            const int n = __ldg(p.lens + b);
+            const int n = p.lens[b];
             if (n < 0 || n > p.max_pages * p.page_size) serve_error(kErrLength);
         }
 
@@ -399,10 +399,10 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
             for (int s = 0; s < KS; ++s) {
                 if (FMT == 0) {
                     const uint32_t* w = reinterpret_cast<const uint32_t*>(src);
-                    qn[s][h] = have ? __ldg(w + 8 * s + t) : 0u;
-                    qn[s][QR / 2 + h] = have ? __ldg(w + 8 * s + 4 + t) : 0u;
+                    qn[s][h] = have ? w[8 * s + t] : 0u;
+                    qn[s][QR / 2 + h] = have ? w[8 * s + 4 + t] : 0u;
                 } else {
-                    const uint2 x = have ? __ldg(reinterpret_cast<const uint2*>(src + F8::k_byte(s, t))) : make_uint2(0u, 0u);
+                    const uint2 x = have ? *reinterpret_cast<const uint2*>(src + F8::k_byte(s, t)) : make_uint2(0u, 0u);
                     qn[s][h] = x.x;
                     qn[s][QR / 2 + h] = x.y;
                 }
@@ -462,7 +462,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 __syncthreads();
                 const bool whole = part == seg.ntile;
                 const unsigned u0 = seg.unit_place();
-                const float vs = FMT == 1 && p.v_scale ? __ldg(p.v_scale + head) : 1.f;
+                const float vs = FMT == 1 && p.v_scale ? p.v_scale[head] : 1.f;
                 auto store = [&](int r, int d, float4 o, float mm, float ll) {
                     const float inv = ll > 0.f || ll != ll ? vs / ll : 0.f;
                     const int hq = head * p.group + row0 + r;
@@ -623,7 +623,7 @@ __global__ void __launch_bounds__(W * 32, MINB) paged_attn_kernel(const AttnPara
                 }
             }
             if (FMT == 1 && p.k_scale) {
-                const float ks = __ldg(p.k_scale + head);
+                const float ks = p.k_scale[head];
                 qscale[0] *= ks;
                 qscale[1] *= ks;
             }

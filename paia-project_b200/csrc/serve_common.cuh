@@ -29,9 +29,10 @@ static inline int serve_error_word(int clear) {
 }
 
 // The operators launch with programmatic dependent launch. The kernel before on the stream is done, and what it wrote is
-// visible, behind the wait: nothing that a caller may have written is read before it. The trigger comes after it and never
-// before: the next kernel may then read some of its inputs at once (a GEMV its weights and bias), and is promised that every
-// kernel but the one immediately before it is done.
+// visible, behind the wait: nothing that a caller may have written is read before it, and what is read is loaded plainly. (A
+// load through the read-only path, __ldg, promises memory that stays unchanged for the kernel's whole life, which here begins
+// before the wait.) The trigger comes after the wait and never before: the next kernel may then read some of its inputs at
+// once (a GEMV its weights and bias), and is promised that every kernel but the one immediately before it is done.
 __device__ __forceinline__ void pdl_wait_and_trigger() {
     asm volatile("griddepcontrol.wait;" ::: "memory");
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

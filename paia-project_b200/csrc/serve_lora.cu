@@ -341,7 +341,7 @@ __device__ __forceinline__ void lora_item(const LoraParams& p, uint8_t* smem, co
             __syncthreads();
         }
         // ---- the cluster's sum in CTA order, scaled, as bf16 hi + lo; ranks behind the last are zeros
-        const float scale = p.scaling ? __ldg(p.scaling + id) : 1.f;
+        const float scale = p.scaling ? p.scaling[id] : 1.f;
         asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
         for (int e = tid; e < lora_pad(rank) * quads; e += kLoraThreads) {
             const int r = e / quads, row = e % quads * 4;
@@ -400,17 +400,17 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int m = m0 + j * kLoraThreads + tid;
-            a[j] = m < p.M ? __ldg(p.adapter + m) : -1;
+            a[j] = m < p.M ? p.adapter[m] : -1;
         }
     };
     if constexpr (!MANY) {
         // a row per thread; its place among the rows of its adapter, each 16th of which begins an item
         int* ids = reinterpret_cast<int*>(smem);
-        const int mine = tid < p.M ? lora_id(p, __ldg(p.adapter + tid)) : -1;
+        const int mine = tid < p.M ? lora_id(p, p.adapter[tid]) : -1;
         // ranks: of all adapters where they are few (one latency less), else of the row's
-        sh_ranks[tid] = p.ranks && tid < p.adapters ? __ldg(p.ranks + tid) : p.rank;
+        sh_ranks[tid] = p.ranks && tid < p.adapters ? p.ranks[tid] : p.rank;
         int my_rank = 0;
-        if (p.adapters > kLoraThreads && mine >= 0 && mine < p.adapters) my_rank = p.ranks ? __ldg(p.ranks + mine) : p.rank;
+        if (p.adapters > kLoraThreads && mine >= 0 && mine < p.adapters) my_rank = p.ranks ? p.ranks[mine] : p.rank;
         ids[tid] = mine;
         __syncthreads();
         int at = __popc(__match_any_sync(~0u, mine) & ((1u << lane) - 1u));
@@ -477,7 +477,7 @@ __global__ void __launch_bounds__(kLoraThreads, 2) lora_kernel(const LoraParams 
                     sh_item[0] = i;
                     sh_item[1] = (item - lo) * kLoraRows;
                     sh_item[2] = min(kLoraRows, counts[i] - (item - lo) * kLoraRows);
-                    sh_item[3] = i == p.adapters ? 0 : p.ranks ? __ldg(p.ranks + i) : p.rank;
+                    sh_item[3] = i == p.adapters ? 0 : p.ranks ? p.ranks[i] : p.rank;
                 }
                 before += all;
             }

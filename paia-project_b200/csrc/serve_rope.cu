@@ -182,11 +182,11 @@ __device__ __noinline__ void exact_pairs(const RopeParams& p, uint4 wl, uint4 wh
             }
             double a = fa, b = fb;
             if (is_k && p.k_norm) {
-                a = a * r * (double)__ldg(p.k_norm + (ia < 8 ? d0 + ia : d1 + ia - 8));
-                b = b * r * (double)__ldg(p.k_norm + (ib < 8 ? d0 + ib : d1 + ib - 8));
+                a = a * r * (double)p.k_norm[ia < 8 ? d0 + ia : d1 + ia - 8];
+                b = b * r * (double)p.k_norm[ib < 8 ? d0 + ib : d1 + ib - 8];
             }
             if (turns) {
-                const double t = (double)pos * __ldg(p.inv_freq + 8 * lane + j) * 0.15915494309189533577;
+                const double t = (double)pos * p.inv_freq[8 * lane + j] * 0.15915494309189533577;
                 double s, c;
                 sincospi(2.0 * (t - rint(t)), &s, &c);
                 const double a0 = a;
@@ -240,7 +240,7 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
             const bool rot = l < turning, is = l < p.head_dim / 16;
             const int e0 = rot ? (p.interleaved ? 16 : 8) * l : is ? p.rot + 16 * (l - turning) : 0;
             const int e1 = rot && !p.interleaved ? half + 8 * l : e0 + 8;
-            weights[which][h * 8 * lanes + spread(l, i, lanes)] = w && is ? __ldg(w + (h ? e1 : e0) + i) : 0.f;
+            weights[which][h * 8 * lanes + spread(l, i, lanes)] = w && is ? w[(h ? e1 : e0) + i] : 0.f;
         }
         __syncthreads();
     }
@@ -262,7 +262,7 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
     const __nv_bfloat16* src = pass_at(unit, pass);
     fetch(src, pass * heads_per + sub);
     for (;;) {
-        const int tok = unit / p.parts, pos = __ldg(p.pos + tok);
+        const int tok = unit / p.parts, pos = p.pos[tok];
         const int end = min((pass + p.part_passes) * heads_per, p.slots);        // the unit's heads end here
         const int next = unit + stride;
         int next_pass = 0;
@@ -271,11 +271,11 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
         long long k_at = -1, v_at = -1;                      // the token's row in the pools (bytes; -1: none)
         if (pos < -1 && wlane == 0) serve_error(kErrPosition);
         if (pos >= 0 && p.k && end > p.heads) {
-            const int sid = p.seq ? __ldg(p.seq + tok) : tok, pg = pos / p.page_size, row = pos - pg * p.page_size;
+            const int sid = p.seq ? p.seq[tok] : tok, pg = pos / p.page_size, row = pos - pg * p.page_size;
             if ((unsigned)sid >= (unsigned)p.sequences || pg >= p.max_pages) {
                 serve_error(kErrPosition);
             } else {
-                const int id = __ldg(p.table + sid * p.table_seq + pg);
+                const int id = p.table[sid * p.table_seq + pg];
                 if ((unsigned)id >= (unsigned)p.num_pages) {
                     serve_error(kErrPage);
                 } else {
@@ -289,7 +289,7 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
         for (int i = 0; i < 4; ++i)
             if (wlane + 32 * i < half) {
                 const int a = wlane + 32 * i;
-                const double t = (double)pos * __ldg(p.inv_freq + a) * 0.15915494309189533577;
+                const double t = (double)pos * p.inv_freq[a] * 0.15915494309189533577;
                 const int at = spread(a >> 3, a & 7, turning);                   // lane a / 8's angle a % 8
                 sincospif(2.f * (float)(t - rint(t)), table + half + at, table + at);
             }
@@ -346,7 +346,7 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
                 // the root), 5 for the root, 2 products, 4 for the angle (2 pi 2^-25) and its sine and cosine, 3 for the
                 // rotation, 2 for the scale: below 2^-19; v 2 for the scale
                 const float* sc = is_k ? p.k_scale : p.v_scale;
-                const float scale = stored && sc ? __ldg(sc + kvh) : 1.f, inv = 1.f / scale;
+                const float scale = stored && sc ? sc[kvh] : 1.f, inv = 1.f / scale;
                 float al[8], ah[8], bl[8], bh[8];
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {

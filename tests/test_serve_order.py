@@ -1,5 +1,6 @@
 """What a serving operator promises the kernels around it on the stream, under programmatic dependent launch: it triggers
-the next kernel only behind its own wait. (On the CPU: from the source.)"""
+the next kernel only behind its own wait, and reads by loads that see what the kernel before it wrote. (On the CPU: from the
+source.)"""
 import re
 from pathlib import Path
 
@@ -26,3 +27,10 @@ def test_trigger_comes_after_the_wait():
             body = src[at:]
             head = body[:body.index("pdl_wait_and_trigger();")]
             assert not re.search(r"\breturn;", re.sub(r"\[&\]\([^)]*\) \{.*?\n    \};", "", head, flags=re.S)), name
+
+
+def test_no_load_promises_unchanged_memory():
+    """The kernels live while the kernel before them still writes lengths, page tables, queries, positions and adapter ids:
+    the read-only path is not for them, neither asked for nor left to the compiler (restrict)."""
+    for name in ("serve_common.cuh", "serve_attn.cu", "serve_rope.cu", "serve_lora.cu"):
+        assert not re.search(r"__ldg|\.nc\b|__restrict", code(name)), name
