@@ -438,14 +438,15 @@ __global__ void __launch_bounds__(NW * 32, 1) gemv_kernel(const Params p) {
 
     grid_dependency_wait();
 
-    // Stage x (and, for INT4, the sum of each 32-element chunk of x) in shared memory.
+    // Stage x (and, for INT4, the sum of each 32-element chunk of x) in shared memory, by plain loads: the read-only path
+    // promises memory that stays unchanged for the kernel's whole life, and the kernel before may have written x in it.
     if constexpr (I4) {
         const int nc = p.K >> 5;
         for (int c = tid; c < nc; c += NW * 32) {
             const uint4* src = reinterpret_cast<const uint4*>(p.x + (size_t)c * 32);
             uint4 v[4];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = __ldg(src + i);
+            for (int i = 0; i < 4; ++i) v[i] = src[i];
             float sum = 0.f;
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -458,7 +459,7 @@ __global__ void __launch_bounds__(NW * 32, 1) gemv_kernel(const Params p) {
     } else {
         const int n16 = p.K >> 3;
         for (int i = tid; i < n16; i += NW * 32)
-            reinterpret_cast<uint4*>(xs)[i] = __ldg(reinterpret_cast<const uint4*>(p.x) + i);
+            reinterpret_cast<uint4*>(xs)[i] = reinterpret_cast<const uint4*>(p.x)[i];
     }
     __syncthreads();
     launch_dependents();

@@ -34,3 +34,10 @@ def test_no_load_promises_unchanged_memory():
     the read-only path is not for them, neither asked for nor left to the compiler (restrict)."""
     for name in ("serve_common.cuh", "serve_attn.cu", "serve_rope.cu", "serve_lora.cu"):
         assert not re.search(r"__ldg|\.nc\b|__restrict", code(name)), name
+
+
+def test_gemv_reads_x_plainly():
+    """The same holds for x of the GEMVs, which is read behind their wait. (Weights, scales and bias are read ahead of it and
+    are the caller's to leave alone: their loads take the read-only path, in helpers that know nothing of x.)"""
+    for name in ("gemv_kernel.cuh", "gemv_mma.cuh", "gemv_tma.cuh"):
+        assert "__ldg" not in code(name), name
