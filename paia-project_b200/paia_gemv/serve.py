@@ -16,7 +16,7 @@ import struct
 
 import torch
 
-from .loader import _PKG_ROOT
+from .loader import _PKG_ROOT, load_lib
 
 # the C structs, field by field (native alignment): include/paia_gemv.h
 ATTN = struct.Struct("10P 12q 9i f")
@@ -91,9 +91,16 @@ def _pools(k, v, kv_heads, head_dim, k_scale, v_scale, dev):
 
 
 class AttentionWorkspace:
-    """The workspace of `paged_attention` for these heads (`attention_workspace` makes it)."""
+    """The workspace of `paged_attention` for these heads over a buffer of the caller's: contiguous uint8 on a CUDA device,
+    16-byte aligned, of at least lib.paged_attn_workspace(heads, kv_heads, head_dim) bytes, all zero before its first call.
+    (`attention_workspace` makes both.) A buffer elsewhere is refused by the call, as any other tensor."""
 
-    def __init__(self, buffer, heads, kv_heads, head_dim):
+    def __init__(self, buffer, heads, kv_heads, head_dim, lib=None):
+        if buffer.is_cuda:                                       # what no call checks again
+            need = (load_lib() if lib is None else lib).paged_attn_workspace(heads, kv_heads, head_dim)
+            if buffer.dtype is not torch.uint8 or not buffer.is_contiguous() or buffer.numel() < need or (
+                    buffer.data_ptr() % 16):
+                _bad("buffer", buffer, f"contiguous uint8 of at least {need} bytes, 16-byte aligned,")
         self.buffer, self.ptr, self.sizes = buffer, buffer.data_ptr(), (buffer.get_device(), heads, kv_heads, head_dim)
 
 
@@ -101,7 +108,7 @@ def attention_workspace(lib, heads, kv_heads, head_dim, device=None):
     """The zeroed workspace of `paged_attention` for these heads, for batches and lengths of any size. Calls that may
     overlap on the GPU (other streams, graphs replayed at the same time) need one each."""
     return AttentionWorkspace(torch.zeros(lib.paged_attn_workspace(heads, kv_heads, head_dim), dtype=torch.uint8,
-                                          device="cuda" if device is None else device), heads, kv_heads, head_dim)
+                                          device="cuda" if device is None else device), heads, kv_heads, head_dim, lib)
 
 
 def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, *, scale=None, window=0, k_scale=None,

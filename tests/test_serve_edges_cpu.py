@@ -1,0 +1,36 @@
+"""CPU (no GPU needed): refusals and host-side decisions of the serving operators that the calls of test_serve_cpu.py do not
+reach."""
+import pytest
+import torch
+
+
+@pytest.fixture(scope="module")
+def L(lib_path):
+    from paia_gemv import loader
+    return loader.GemvLib(lib_path)
+
+
+class OnCuda(torch.Tensor):
+    """A CPU tensor that says it is on CUDA device 0: host-side checks run, nothing is launched."""
+    is_cuda = property(lambda self: True)
+
+    def get_device(self):
+        return 0
+
+
+@pytest.mark.parametrize("heads,kv,hd", [(4, 2, 64), (32, 8, 128), (64, 2, 256), (40, 2, 96)])
+def test_workspace_over_a_buffer(L, heads, kv, hd):
+    """A workspace over a caller's own buffer holds what the kernel may write, or is refused."""
+    from paia_gemv import serve
+    need = L.paged_attn_workspace(heads, kv, hd)
+    buf = lambda n, dtype=torch.uint8: torch.zeros(n, dtype=dtype).as_subclass(OnCuda)   # noqa: E731
+    whole = buf(need + 16)
+    at = -whole.data_ptr() % 16
+    ws = serve.AttentionWorkspace(whole[at:at + need], heads, kv, hd, L)
+    assert ws.ptr % 16 == 0 and ws.sizes == (0, heads, kv, hd)
+    for bad in (whole[at:at + need - 1], buf(64), buf(0), whole[at + 1:at + 1 + need], buf(2 * need + 32)[::2],
+                buf(need, torch.int8), buf(need, torch.float32)):
+        with pytest.raises(ValueError, match="buffer must be"):
+            serve.AttentionWorkspace(bad, heads, kv, hd, L)
+    with pytest.raises(RuntimeError):                            # heads that the attention does not take
+        serve.AttentionWorkspace(whole, heads + 1, kv, hd, L)
