@@ -314,8 +314,10 @@ int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream);
 /* The calling thread's current CUDA device; -1 where there is none. */
 int paia_gemv_current_device(void);
 
-/* Device-side error word of the current device (0 = none), set by kernels whose bounded waits gave up (codes below
- * 10) or that met a bad index in device memory (10 to 13); clear != 0 resets it. Synchronous. */
+/* Device-side error words of the current device: one of the GEMVs, set by kernels whose bounded waits gave up (codes below
+ * 10), and one of each serving operator, set by the first bad index that it met in device memory (10 to 13). Returns the
+ * first of them that is set (0 = none; -1: they cannot be read); clear != 0 resets that one alone, so calls until 0 return
+ * them all. Synchronous; wait for the kernels in question first. */
 int paia_gemv_device_error(int clear);
 
 #ifdef __cplusplus

@@ -839,14 +839,13 @@ int paia_gemv_current_device(void) {
     return d;
 }
 
-// Device-side error word of the current device (0 = none; the codes of the TMA-fed kernels' bounded waits, 6 and 8
-// from the tensor-parallel exchange), then the serving operators' words (10 to 13, bad indices in device memory);
-// clear != 0 resets them all. Synchronous (symbol copies).
+// The first error word of the current device that is set (0 = none): the codes of the TMA-fed kernels' bounded waits, 6 and
+// 8 from the tensor-parallel exchange, then a word of each serving operator (10 to 13, bad indices in device memory).
+// clear != 0 resets the word that is returned and leaves the others for the next call. Synchronous (symbol copies).
 int paia_gemv_device_error(int clear) {
-    const int words[4] = {tma_device_error(clear), attn_device_error(clear), rope_device_error(clear),
-                          lora_device_error(clear)};
-    for (int w : words)
-        if (w) return w;
+    int (*const words[4])(int) = {tma_device_error, attn_device_error, rope_device_error, lora_device_error};
+    for (auto word : words)
+        if (const int w = word(clear)) return w;
     return 0;
 }
 

@@ -338,8 +338,9 @@ class GemvLib:
         return n
 
     def device_error(self, clear=True):
-        """The device-side error word (0 = none): below 10 from kernels whose bounded waits gave up, 10 to 13 from
-        serving operators that met a bad page id, length, position or adapter id."""
+        """The first device-side error word that is set (0 = none): below 10 from kernels whose bounded waits gave up, 10
+        to 13 from serving operators that met a bad page id, length, position or adapter id (a word each: call until 0 to
+        see them all)."""
         return self._lib.paia_gemv_device_error(1 if clear else 0)
 
 
