@@ -8,7 +8,7 @@ no torch headers), then linked into one shared library with a plain C ABI, as th
 (src/paia_gemv/build.sh:8-19) but for sm_100a only. The ptxas register/spill report of every kernel is kept in
 build/<arch>/ptxas_report.txt. nvcc cross-compiles, so no GPU is needed.
 
-Beside it, where Python's and torch's headers are there, build/<arch>/_paia_serve.so: the CPython extension that makes
+Beside it, where Python's and torch's headers are there, build/<arch>/_paia_serve.<tag>.so: the CPython extension that makes
 paia_gemv.serve's calls without their Python overhead (csrc/serve_bind.cpp; it links neither torch nor the library).
 """
 import argparse
@@ -27,7 +27,7 @@ CSRC = HERE / "csrc"
 INCLUDE = HERE.parent / "include"
 OUT = HERE / "build" / platform.machine()
 LIB = OUT / "libpaia_gemv.so"
-BIND = OUT / "_paia_serve.so"
+BIND = OUT / ("_paia_serve" + sysconfig.get_config_var("EXT_SUFFIX"))        # of this interpreter alone
 GENCODE = ["-gencode", "arch=compute_100a,code=sm_100a"]
 FLAGS = ["-O3", "-std=c++17", "-lineinfo", "-Xcompiler", "-fPIC", "-Xptxas", "-v", "--expt-relaxed-constexpr"]
 

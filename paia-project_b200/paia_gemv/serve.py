@@ -13,6 +13,7 @@ kv head), in any layout whose head_dim is contiguous: a [num_pages, kv_heads, pa
 import importlib.util
 import platform
 import struct
+import sysconfig
 
 import torch
 
@@ -25,8 +26,9 @@ LORA = struct.Struct("8P 7q 5i 4x")
 
 def _load_bind():
     """The extension that checks and makes these calls in C (csrc/serve_bind.cpp), or None: without it, and for every
-    call that it does not find exactly as it should be, the code below checks, calls and raises."""
-    path = _PKG_ROOT / "build" / platform.machine() / "_paia_serve.so"
+    call that it does not find exactly as it should be, the code below checks, calls and raises. One built for another
+    interpreter (its name says which) is not looked at."""
+    path = _PKG_ROOT / "build" / platform.machine() / ("_paia_serve" + sysconfig.get_config_var("EXT_SUFFIX"))
     api = getattr(torch.Tensor, "__dlpack_c_exchange_api__", None)
     if api is None or not path.exists():
         return None

@@ -1,5 +1,9 @@
 """CPU (no GPU needed): refusals and host-side decisions of the serving operators that the calls of test_serve_cpu.py do not
 reach."""
+import platform
+import shutil
+import sysconfig
+
 import pytest
 import torch
 
@@ -34,3 +38,17 @@ def test_workspace_over_a_buffer(L, heads, kv, hd):
             serve.AttentionWorkspace(bad, heads, kv, hd, L)
     with pytest.raises(RuntimeError):                            # heads that the attention does not take
         serve.AttentionWorkspace(whole, heads + 1, kv, hd, L)
+
+
+def test_extension_of_another_interpreter_is_not_loaded(L, monkeypatch, tmp_path):
+    """The extension's name carries the interpreter that it was built for, and only this one's is loaded."""
+    from paia_gemv import serve
+    if serve._bind is None:
+        pytest.skip("the extension is not built")
+    assert serve._bind.__file__.endswith("_paia_serve" + sysconfig.get_config_var("EXT_SUFFIX"))
+    monkeypatch.setattr(serve, "_PKG_ROOT", tmp_path)
+    at = tmp_path / "build" / platform.machine()
+    at.mkdir(parents=True)
+    for name in ("_paia_serve.so", "_paia_serve.cpython-31-x86_64-linux-gnu.so"):
+        shutil.copy(serve._bind.__file__, at / name)
+    assert serve._load_bind() is None
