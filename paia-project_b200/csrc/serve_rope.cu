@@ -13,7 +13,7 @@
 // The angle is reduced in fp64 (pos * inv_freq reaches 10^5 radians, where fp32 has 2^-8 left) and its sine and cosine
 // are taken in fp32. What an e4m3 cache stores is the e4m3 value nearest to the exact one: where the fp32 result lies so
 // near to the border between two of its coarse steps that fp32's error could cross it (about one element in 10^4), the
-// warp computes its rows again in fp64.
+// pair is computed again in fp64.
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 
@@ -153,8 +153,8 @@ __device__ __forceinline__ uint2 pack8_e4m3(const float* x) {
 
 // The elements of `todo` (bit i: lo i, bit 8 + i: hi i) of a lane's row of an e4m3 cache again in fp64 from the stored
 // bf16, into the packed bytes v; whole warps call it, a lane's first pair with a bit set per round.
-__device__ __noinline__ void exact_pairs(const RopeParams& p, uint4 wl, uint4 wh, int pos, bool is_k, bool in, bool rotated,
-                                         int lane, int d0, int d1, float scale, unsigned todo, unsigned long long* v) {
+__device__ __noinline__ void exact_pairs(const RopeParams& p, uint4 wl, uint4 wh, int pos, bool is_k, bool rotated, int lane,
+                                         int d0, int d1, float scale, unsigned todo, unsigned long long* v) {
     float x[16];
     Head raw;
     raw.load(wl, wh);
@@ -343,8 +343,9 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
                 }
             } else if (__any_sync(~0u, stored)) {
                 // fp32's error in steps of 2^-24 of |a| + |b|: k 20 / 2 for the mean square (a step per addition, halved by
-                // the root), 5 for the root, 2 products, 4 for the angle (2 pi 2^-25) and its sine and cosine, 3 for the
-                // rotation, 2 for the scale: below 2^-19; v 2 for the scale
+                // the root), 4 for rsqrtf, 2 products, 4 for the angle (2 pi 2^-25) and its sine and cosine, 2 for the
+                // rotation, 3 for l - el, 1 / scale and their product: 25, 1.5e-6. v has only the last three, and
+                // every pair of a bf16 and a scale beside a border has been replayed: 1.3e-7 finds them all
                 const float* sc = is_k ? p.k_scale : p.v_scale;
                 const float scale = stored && sc ? sc[kvh] : 1.f, inv = 1.f / scale;
                 float al[8], ah[8], bl[8], bh[8];
@@ -367,7 +368,7 @@ __global__ void __launch_bounds__(kRopeThreads, FMT == 0 ? 3 : 2) qkv_rope_kerne
 #pragma unroll
                         for (int i = 0; i < 16; ++i) todo |= (d[i >> 2] >> 8 * (i & 3) & 0xFF ? 1u : 0u) << i;
                     }
-                    exact_pairs(p, rl, rh, pos, is_k, in, rotated, lane, d0, d1, scale, todo, v);
+                    exact_pairs(p, rl, rh, pos, is_k, rotated, lane, d0, d1, scale, todo, v);
                 }
                 if (stored) {
                     *reinterpret_cast<unsigned long long*>(dst + d0) = v[0];

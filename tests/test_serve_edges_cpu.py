@@ -1,11 +1,15 @@
 """CPU (no GPU needed): refusals and host-side decisions of the serving operators that the calls of test_serve_cpu.py do not
 reach."""
 import platform
+import re
 import shutil
 import sysconfig
+from pathlib import Path
 
 import pytest
 import torch
+
+ROOT = Path(__file__).resolve().parents[1]
 
 
 @pytest.fixture(scope="module")
@@ -52,3 +56,29 @@ def test_extension_of_another_interpreter_is_not_loaded(L, monkeypatch, tmp_path
     for name in ("_paia_serve.so", "_paia_serve.cpython-31-x86_64-linux-gnu.so"):
         shutil.copy(serve._bind.__file__, at / name)
     assert serve._load_bind() is None
+
+
+def test_value_brackets_find_every_border():
+    """What an e4m3 cache stores of v: the fp32 quotients of v less and plus a margin, by the reciprocal of the scale. Where
+    both round to one e4m3 value that is the value nearest to the exact quotient, for every bf16 mantissa and every scale
+    within eight fp32 steps of putting it on a border (beyond them the margin is not needed)."""
+    src = (ROOT / "paia-project_b200" / "csrc" / "serve_rope.cu").read_text()
+    margin = torch.tensor(float(re.search(r"fabsf\(l\[i\]\) \* ([\d.e-]+)f;", src).group(1)))
+
+    def nearest(x):                                              # of a binade from 1 on, or of the subnormal values
+        step = torch.where(x >= 0.25, 2.0 ** -3, 2.0 ** -9).double()
+        return torch.round(x.double() / step) * step
+
+    normal = (2 * torch.arange(8, 16).double() + 1) / 16
+    for m, step in ((normal, 2.0 ** -3), ((2 * torch.arange(8).double() + 1) * 2.0 ** -10, 2.0 ** -9)):
+        v = (1 + torch.arange(128) / 128).float()[:, None, None].expand(128, 8, 17)
+        s = (v[:, :, 0].double() / m).float()
+        s = (s[..., None].view(torch.int32) + torch.arange(-8, 9, dtype=torch.int32)).view(torch.float32)
+        off, inv = v * margin, 1 / s
+        lo, hi = nearest((v - off) * inv), nearest((v + off) * inv)
+        d = v.double() - m[None, :, None] * s.double()          # exact: 5 bits by 24
+        below = (m - step / 2)[None, :, None].expand_as(d)
+        tie = torch.where(torch.round(below / step) % 2 == 0, below, below + step)
+        want = torch.where(d < 0, below, torch.where(d > 0, below + step, tie))
+        assert ((lo == hi) <= (lo == want)).all() and ((lo <= want) & (want <= hi)).all()
+        assert (lo != hi).any() and (lo == hi).any()

@@ -1,5 +1,5 @@
 """How exactly the serving operators compute what they keep in fewer than 32 bits, at inputs that show it: probabilities and
-queries of an e4m3 cache's attention (f16 next to the stored bytes)."""
+queries of an e4m3 cache's attention (f16 next to the stored bytes), and the bytes that an e4m3 cache stores."""
 import math
 
 import pytest
@@ -124,3 +124,111 @@ def test_e4m3_queries_of_any_size(L, size):
     k, v, table = C.paged(lens, 2, 128, 16, E4M3, "cuda", g)
     q = (torch.randn(2, 8, 128, generator=g, device="cuda") * 2.0 ** size).to(BF16)
     call(L, q, k, v, table, lens, 2.0 ** -size / 30 / math.sqrt(128))
+
+
+# ------------------------------------------------------------------ what an e4m3 cache stores
+
+def nearest8(x):
+    """The e4m3 value nearest to x (ties to even, at most 448), and how far x is from the next border between two of them."""
+    a = x.abs().clamp(max=448.0)
+    _, e = torch.frexp(a)
+    step = torch.ldexp(torch.ones_like(a), (e - 4).clamp(min=-9))
+    r = a / step
+    far = torch.where(x.abs() >= 448, torch.full_like(a, math.inf), ((r - torch.floor(r)) - 0.5).abs() * step)
+    return torch.sign(x) * torch.round(r) * step, far
+
+
+def same_bytes(pool, want, unsure=None):
+    """The stored values (pool [..., hd]) are the nearest ones, but where the exact value is too near a border to tell."""
+    value, far = nearest8(want)
+    sure = torch.ones_like(far, dtype=torch.bool) if unsure is None else far > unsure
+    assert sure.double().mean().item() > 0.99
+    bad = (pool.double() != value) & sure
+    assert not bad.any(), (int(bad.sum()), pool.double()[bad][:4].tolist(), want[bad][:4].tolist())
+    return int((far < 1e-5 * value.abs()).sum())
+
+
+def borders(g):
+    """(l, scale) pairs whose quotient lies on a border between two e4m3 values or a few fp32 steps beside it: every bf16
+    mantissa against every border of a binade and every subnormal one."""
+    l = 1 + torch.arange(128, dtype=torch.float64) / 128
+    normal = (2 * torch.arange(8, 16, dtype=torch.float64) + 1) / 16
+    m = torch.cat([normal, normal * 2.0 ** -6, normal * 2.0 ** 7, (2 * torch.arange(8, dtype=torch.float64) + 1) * 2.0 ** -10])
+    s = (l[:, None] / m).float()
+    s = s[..., None].view(torch.int32) + torch.arange(-3, 4, dtype=torch.int32)
+    s, two = s.view(torch.float32), torch.exp2(torch.randint(-9, 9, s.shape, generator=g).double())
+    return (l[:, None, None] * two).reshape(-1), (s * two.float()).reshape(-1)
+
+
+def test_e4m3_rows_at_borders(L):
+    """Keys and values that are not turned (position 0, no norm), exactly on the borders and beside them."""
+    from paia_gemv import serve
+    l, s = borders(torch.Generator().manual_seed(3))
+    kv, hd = len(l), 16
+    sign = torch.where(torch.arange(hd) % 3 == 1, -1.0, 1.0).double()
+    rows = (l[:, None] * sign).to(BF16)
+    assert torch.equal(rows.double(), l[:, None] * sign)
+    qkv = torch.cat([torch.zeros(hd, dtype=BF16), rows.reshape(-1), rows.reshape(-1)])[None].cuda()
+    k = torch.zeros(1, 1, kv, hd, dtype=E4M3, device="cuda")
+    v = torch.zeros_like(k)
+    zero = torch.zeros(1, dtype=torch.int32, device="cuda")
+    sc = s.cuda()
+    serve.qkv_rope_cache(L, qkv, zero, serve.rope_inv_freq(16, 1e4), torch.empty(1, 1, hd, dtype=BF16, device="cuda"), k, v,
+                         zero.view(1, 1), k_scale=sc, v_scale=sc)
+    want = (rows.double() / s.double()[:, None]).cuda()
+    assert same_bytes(v[0, 0], want) > 0 and same_bytes(k[0, 0], want) > 0
+    assert L.device_error(True) == 0
+
+
+@pytest.mark.parametrize("hd,rot", [(128, 128), (64, 32), (96, 96), (256, 256), (80, 16)])
+@pytest.mark.parametrize("inter", [False, True])
+@pytest.mark.parametrize("norm", [False, True])
+def test_e4m3_rows_are_the_nearest_values(L, hd, rot, inter, norm):
+    """Turned and normed keys, and values, of many tokens; then of one token whose scales put an element of every key head
+    on a border or a few fp32 steps beside it."""
+    from paia_gemv import serve
+    g = gen(31)
+    eps = 2.0 ** -17
+    freq = serve.rope_inv_freq(rot, 10000.0)
+    kn = 1 + 0.2 * torch.randn(hd, generator=g, device="cuda") if norm else None
+
+    def run(qkv, pos, kv, ks, vs):
+        n = len(pos)
+        k = torch.zeros(n, 1, kv, hd, dtype=E4M3, device="cuda")
+        v = torch.zeros_like(k)
+        table = torch.arange(n, dtype=torch.int32, device="cuda")[:, None].expand(n, int(pos.max()) + 1).contiguous()
+        serve.qkv_rope_cache(L, qkv, pos, freq, torch.empty(n, 1, hd, dtype=BF16, device="cuda"), k, v, table, k_norm=kn,
+                             eps=eps, interleaved=inter, k_scale=ks, v_scale=vs)
+        torch.cuda.synchronize()
+        assert L.device_error(True) == 0
+        return k[:, 0], v[:, 0]
+
+    def exact(qkv, pos, kv):
+        (_, wk, wv), (_, mk, _) = C.rope(qkv, pos, freq, 1, kv, hd, None, kn, eps, inter)
+        # fp64: some steps of 2^-53 of the pair, and the angle's own step
+        return wk, wv, mk * (2.0 ** -46 + pos.double().abs()[:, None, None] * 2.0 ** -50)
+
+    kv, n = 3, 400
+    qkv = (3 * torch.randn(n, (1 + 2 * kv) * hd, generator=g, device="cuda")).to(BF16)
+    pos = torch.randint(0, 900, (n,), generator=g, device="cuda", dtype=torch.int32)
+    ks, vs = (1 + 0.2 * torch.rand(2, kv, generator=g, device="cuda")) / 20
+    k, v = run(qkv, pos, kv, ks, vs)
+    wk, wv, ek = exact(qkv, pos, kv)
+    same_bytes(k, wk / ks.double()[:, None], ek / ks.double()[:, None])
+    same_bytes(v, wv / vs.double()[:, None])
+
+    kv = 4096
+    qkv = (3 * torch.randn(1, (1 + 2 * kv) * hd, generator=g, device="cuda")).to(BF16)
+    pos = torch.tensor([777], dtype=torch.int32, device="cuda")
+    wk, wv, ek = exact(qkv, pos, kv)
+    at = torch.randint(0, hd, (kv,), generator=g, device="cuda")
+    border = (2 * torch.randint(8, 16, (kv,), generator=g, device="cuda").double() + 1) / 16
+    scales = []
+    for w in (wk[0], wv[0]):
+        x = w[torch.arange(kv, device="cuda"), at].abs().clamp(min=2.0 ** -10)
+        step = torch.randint(-4, 5, (kv,), generator=g, device="cuda", dtype=torch.int32)
+        scales.append(((x / border).float().view(torch.int32) + step).view(torch.float32))
+    ks, vs = scales
+    k, v = run(qkv, pos, kv, ks, vs)
+    hit = same_bytes(k[0], wk[0] / ks.double()[:, None], ek[0] / ks.double()[:, None])
+    assert same_bytes(v[0], wv[0] / vs.double()[:, None]) > kv // 2 and hit > kv // 2
