@@ -1,6 +1,7 @@
 """CPU (no GPU needed): refusals and host-side decisions of the serving operators that the calls of test_serve_cpu.py do not
 reach."""
 import platform
+import random
 import re
 import shutil
 import sysconfig
@@ -58,6 +59,46 @@ def test_extension_of_another_interpreter_is_not_loaded(L, monkeypatch, tmp_path
     assert serve._load_bind() is None
 
 
+def scans(each, units, t0):
+    """(sequence, places before it) of place t0, as every warp of the attention finds it: lane i adds up the i-th share of
+    the sequences, one scan over the lanes finds the share, scans of 32 of its sequences at a time the sequence."""
+    batch = len(each)
+    share = (batch + 31) // 32
+    mine = [sum(each[min(i * share, batch):min(min(i * share, batch) + share, batch)]) for i in range(32)]
+    inc = [sum(mine[:i + 1]) for i in range(32)]
+    lane = next(i for i in range(32) if t0 < inc[i] * units)
+    before, at = inc[lane] - mine[lane], lane * share
+    if share > 1:
+        end = min(at + share, batch)
+        while True:
+            n = [each[at + i] if at + i < end else 0 for i in range(32)]
+            inc = [sum(n[:i + 1]) for i in range(32)]
+            hits = [i for i in range(32) if t0 < (before + inc[i]) * units]
+            if hits or at + 32 >= end:
+                i = hits[0] if hits else 31
+                at, before = at + i, before + inc[i] - n[i]
+                break
+            before, at = before + inc[31], at + 32
+    return at, before
+
+
+@pytest.mark.parametrize("batch", [1, 31, 32, 33, 64, 65, 700, 1023, 1024, 1025, 1056, 1057, 1100, 2048, 2049, 2100, 3300, 5000])
+def test_attention_start_is_found_at_any_batch(batch):
+    """Beyond 1024 sequences a lane's share is more than 32: the scans go on over it."""
+    rng = random.Random(batch)
+    for units in (1, 3, 8):
+        each = [rng.choice([7, 8, 1 + 14, rng.randrange(7, 400)]) for _ in range(batch)]
+        starts, place = [], 0
+        for n in each:
+            starts.append(place)
+            place += n * units
+        per = max(-(-place // rng.choice([148, 296, 592])), 4)
+        for t0 in sorted({t for t in range(0, place, per)} | {0, place - 1} | {rng.choice(starts) for _ in range(20)}
+                         | {max(rng.choice(starts) - 1, 0) for _ in range(20)}):
+            b, before = scans(each, units, t0)
+            assert before * units == starts[b] <= t0 < starts[b] + each[b] * units
+
+
 def test_value_brackets_find_every_border():
     """What an e4m3 cache stores of v: the fp32 quotients of v less and plus a margin, by the reciprocal of the scale. Where
     both round to one e4m3 value that is the value nearest to the exact quotient, for every bf16 mantissa and every scale
@@ -82,3 +123,27 @@ def test_value_brackets_find_every_border():
         want = torch.where(d < 0, below, torch.where(d > 0, below + step, tie))
         assert ((lo == hi) <= (lo == want)).all() and ((lo <= want) & (want <= hi)).all()
         assert (lo != hi).any() and (lo == hi).any()
+
+
+def test_registers_and_spills():
+    """ptxas's report of the serving kernels: two CTAs of the attention fit an SM wherever they are launched so, and only
+    known instances spill, none by more than it does: head_dim 256 (its sums fill the registers), 16 heads beside an e4m3
+    cache at head_dim 128, and the adapters' search among more than 256 rows (a few bytes)."""
+    from test_compile_report import load_reports
+    rows = [r for r in load_reports() if r["file"].startswith("serve_")]
+    assert len(rows) >= 36 + 2 + 2
+    seen = 0
+    for r in rows:
+        spills = r["spill_st"] + r["spill_ld"]
+        m = re.search(r"paged_attn_kernelILi(\d+)ELi(\d)ELi(\d+)ELi(\d)ELi(\d)ELi(\d)ELb(\d)E", r["fn"])
+        if m:
+            hd, fmt, heads, warps, _, ctas, _ = map(int, m.groups())
+            seen += 1
+            assert r["regs"] * warps * 32 * ctas <= 65536, r
+            known = 700 if hd == 256 else 300 if (hd, fmt, heads) == (128, 1, 16) else 0
+            assert spills <= known and r["stack"] <= known, r
+        elif "lora_kernel" in r["fn"]:
+            assert spills <= 64 and r["regs"] * 512 <= 65536, r
+        else:
+            assert "qkv_rope_kernel" in r["fn"] and spills == 0 and r["stack"] <= 16, r   # (a frame for the settled bytes)
+    assert seen >= 36
