@@ -210,25 +210,27 @@ int paia_gemv_plan_launch(const paia_gemv_plan* plan, void* stream);
 int paia_gemv_plan_destroy(paia_gemv_plan* plan);
 
 /* ---- Serving operators beside the GEMVs (no reference kernel): a batched decode step's attention, rotary positions and
- * adapters. They launch with programmatic dependent launch (they touch memory, and let the next kernel start, only once the
- * kernel before them is done), allocate nothing and never synchronise. Strides are counted in elements and the innermost
- * dimension is contiguous; 64-bit offsets throughout. Codes: 0, -2 bad argument, >0
- * cudaError_t. Indices that live on the device (page ids, lengths, positions, adapter ids) are checked by the kernels:
- * a bad one is never followed to memory and sets a code of paia_gemv_device_error (10 page id, 11 length, 12 position
- * or sequence, 13 adapter id). */
+ * adapters. They launch with programmatic dependent launch (they touch memory, and let the next kernel start, only once
+ * the kernel before them is done), allocate nothing and never synchronise. Strides are counted in elements and the
+ * innermost dimension is contiguous; 64-bit offsets throughout. Codes: 0, -2 bad argument, >0 cudaError_t. Indices on
+ * the device (page ids, lengths, positions, adapter ids) are checked by the kernels: a bad one is never followed to
+ * memory and sets a code of paia_gemv_device_error (10 page id, 11 length, 12 position or sequence, 13 adapter id). */
 
 /* Attention of one new token per sequence over a paged key-value cache (grouped-query: heads / kv_heads query heads
  * share a kv head). Sequence b holds positions 0 .. lens[b] - 1; position j lies in row j % page_size of page
  * page_table[b][j / page_size]. For query head h of kv head h / (heads / kv_heads):
  *   s_j = scale k_scale <q_h, k_j>,  p = softmax(s),  out_h = v_scale sum_j p_j v_j,  lse_h = log sum_j exp s_j
- * over the last `window` positions (0: all). Statistics and sums are fp32; out is rounded once to bf16. A sequence of
- * length 0 gives out = 0 and lse = -inf; so does a row whose scores are all -inf. A NaN or an infinity that is read makes
- * what it reaches NaN or infinite (a score of -inf has no weight). Cache rows outside the range are never read. A page id
- * outside [0, num_pages) (code 10) reads as zero rows, a length above max_pages page_size is cut to it and one below 0 is
- * 0 (code 11).
+ * over the last `window` positions (0: all). Scores, statistics and sums are fp32; p enters its product with v as two
+ * bf16 (2^-16 of each p), out is rounded once to bf16. Beside an e4m3 cache p is one f16 (2^-11 of each p, independent
+ * from position to position, and 2^-40 of the largest) and q too (exact down to 2^-32 of its head's largest element). A
+ * sequence of length 0 gives out = 0 and lse = -inf; so does a row whose scores are all -inf. A NaN or an infinity that
+ * is read makes what it reaches NaN or infinite (a score of -inf has no weight). Cache rows outside the range are never
+ * read. A page id outside [0, num_pages) (code 10) reads as zero rows, a length above max_pages page_size is cut to it
+ * and one below 0 is 0 (code 11).
  * q, out bf16; cache bf16 or e4m3 with a fp32 scale per kv head (value = stored * scale). head_dim 64, 96, 128 or 256;
- * any page size and page / token / head strides (both [page][token][head] and [page][head][token] caches);
- * batch * kv_heads * max_pages * page_size / 16 (times the 16-head units of a larger group) below 2^32. q, k and v 16-byte
+ * any page size and page / token / head strides (both [page][token][head] and [page][head][token] caches). Positions and
+ * places of the work list are counted in 32 bits: max_pages * page_size <= 2^31 - 256, and batch * kv_heads * ceil(heads
+ * / kv_heads / 16) * (max_pages * page_size / 16 + 16) <= 2^32 - 2^20 (else -2); heads <= 65536. q, k and v 16-byte
  * aligned with strides of whole 16 bytes, out 8-byte aligned with strides of multiples of 4 elements. `workspace`:
  * paia_gemv_paged_attn_workspace(heads, kv_heads, head_dim) bytes on the launch's device, 16-byte aligned, zeroed once;
  * every launch leaves it ready for the next, of any batch; launches that may overlap on the GPU (other streams, graphs
@@ -258,14 +260,15 @@ int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream);
 /* The step between a fused QKV projection and the attention, for any number of tokens: per-head RMS norm of q and k
  * (where q_norm / k_norm are given), rotation of q and k at each token's own position, q stored, k and v stored into
  * their cache pages. Token t of sequence seq[t] (NULL: t) at position pos[t] goes to row pos % page_size of page
- * page_table[seq][pos / page_size]; a token with position -1 is padding: nothing is read or stored for it. With
- * x' = x / sqrt(mean x^2 + eps) * w, pair i of a head, (x'_i, x'_(i + rot / 2)) or, interleaved, (x'_2i, x'_(2i + 1)),
- * turns by pos * inv_freq[i]; dimensions from rot on stay. Arithmetic is fp32 (angles fp64; an e4m3 cache's k fp64),
- * rounded once. inv_freq is fp64 [rot / 2]: theta^(-2i / rot) or any scaled table. e4m3 caches store x / scale[kv head],
- * at most 448 in magnitude. q_out may be the q part of qkv itself. k_out (NULL: none) receives the rotated keys as bf16
- * too; k and v may both be NULL (no cache) where k_out is given. head_dim and rot are multiples of 16, head_dim <= 256,
- * rot <= head_dim. qkv, q_out, k_out, k, v 16-byte aligned with strides of whole 16 bytes. Two tokens of one call must
- * not name the same sequence and position. */
+ * page_table[seq][pos / page_size]; a token with position -1 is padding: nothing is stored for it and its row is not
+ * used (but has to be memory that can be read). With x' = x / sqrt(mean x^2 + eps) * w, pair i of a head, (x'_i, x'_(i +
+ * rot / 2)) or, interleaved, (x'_2i, x'_(2i + 1)), turns by pos * inv_freq[i]; dimensions from rot on stay. Arithmetic
+ * is fp32 (angles are reduced in fp64), rounded once. inv_freq is fp64 [rot / 2]: theta^(-2i / rot) or any scaled table.
+ * e4m3 caches store the value nearest to x / scale[kv head] (what fp32 cannot settle is computed in fp64), at most 448
+ * in magnitude; NaN stays NaN. q_out may be the q part of qkv itself. k_out (NULL: none) receives the rotated keys as
+ * bf16 too; k and v may both be NULL (no cache) where k_out is given. head_dim and rot are multiples of 16, head_dim <=
+ * 256, rot <= head_dim. qkv, q_out, k_out, k, v 16-byte aligned with strides of whole 16 bytes. Two tokens of one call
+ * must not name the same sequence and position. */
 typedef struct paia_gemv_rope_cache {
     const void* qkv;             /* bf16 [tokens][(heads + 2 kv_heads) * head_dim] */
     const int* pos;              /* [tokens] */
@@ -292,11 +295,13 @@ int paia_gemv_qkv_rope_cache(const paia_gemv_rope_cache* a, void* stream);
 
 /* Low-rank adapters of many requests beside a shared projection (paia_gemv_batched): for every row m with adapter
  * a = adapter[m],  out[m] = base[m] + scaling[a] B[a] (A[a] x[m]);  rows with adapter -1 get base[m]. Adapter a uses its
- * first ranks[a] ranks (NULL: all `rank`; 0: none; what lies behind them is not used), scaling NULL is 1, base NULL is 0,
- * base may be out itself, x may not overlap out. Sums are fp32, A x is kept in 32 bits between the two products, and out
- * is rounded once to bf16. A NaN or an infinity in x, A or B makes what it reaches NaN or infinite. An id outside
- * [-1, adapters) (code 13) is treated as -1. rank, K and N are multiples of 8, rank <= 256, adapters <= 8192, M <= 2^30.
- * x, A, B, base, out 16-byte aligned with strides of whole 16 bytes. */
+ * first ranks[a] ranks (NULL: all `rank`; 0: none; what lies behind them is not used), scaling NULL is 1, base NULL is
+ * 0, base may be out itself, x may not overlap out. Sums are fp32; scaling A x enters the second product as two bf16
+ * (2^-16 of it), and out is rounded once to bf16. The division of K, and with it the last bits of a row, follows the
+ * whole call (M, adapters, how many rows share an adapter); the same call gives the same bits. A NaN or an infinity in
+ * x, A or B makes what it reaches NaN or infinite. An id outside [-1, adapters) (code 13) is treated as -1. rank, K and
+ * N are multiples of 8, rank <= 256, adapters <= 8192, M <= 2^30. x, A, B, base, out 16-byte aligned with strides of
+ * whole 16 bytes. */
 typedef struct paia_gemv_lora_args {
     const void* x;               /* bf16 [M][K] */
     const void* a;               /* bf16 [adapters][rank][K] */

@@ -147,3 +147,18 @@ def test_registers_and_spills():
         else:
             assert "qkv_rope_kernel" in r["fn"] and spills == 0 and r["stack"] <= 16, r   # (a frame for the settled bytes)
     assert seen >= 36
+
+
+@pytest.mark.parametrize("change", [
+    dict(batch=1 << 19, heads=4096, kv_heads=4096, max_pages=1, page_size=16), dict(max_pages=1, page_size=0x7FFFFF01),
+    dict(batch=1 << 28, heads=2, kv_heads=1, max_pages=0), dict(batch=1 << 24, heads=512, kv_heads=1, max_pages=0)])
+def test_attention_size_limits(L, change):
+    """The limits that the header gives for positions and places: short tables count 16 places per unit."""
+    import test_serve_cpu as T
+    from paia_gemv import serve
+    a = dict(T.ATTN, q_batch=0, **change)
+    places = a["batch"] * a["kv_heads"] * -(-(a["heads"] // a["kv_heads"]) // 16) * (a["max_pages"] * a["page_size"] // 16 + 16)
+    assert a["max_pages"] * a["page_size"] > 2 ** 31 - 256 or places > 2 ** 32 - 2 ** 20
+    assert L._lib.paia_gemv_paged_attn(T.packed("paia_gemv_attn", serve.ATTN, a), None) == -2
+    if a["batch"] > 2:                                           # its own size alone is what is refused
+        assert L._lib.paia_gemv_paged_attn(T.packed("paia_gemv_attn", serve.ATTN, dict(a, batch=0)), None) == 0
