@@ -68,6 +68,11 @@ def _flat(name, t, dtype, shape, dev):
     return t.data_ptr()
 
 
+def _strides(t):
+    """The strides of a tensor, 0 along a dimension of one: never used, and free to be anything in torch."""
+    return tuple(0 if n == 1 else s for n, s in zip(t.shape, t.stride()))
+
+
 def _device(t, name):
     dev = t.get_device()
     if dev < 0 or dev != _current_device():
@@ -77,7 +82,7 @@ def _device(t, name):
 
 def _pools(k, v, kv_heads, head_dim, k_scale, v_scale, dev):
     """(cache code, pool shape, strides of k, of v) of a cache's two pools."""
-    shape, dtype, ks, vs = k.shape, k.dtype, k.stride(), v.stride()
+    shape, dtype, ks, vs = k.shape, k.dtype, _strides(k), _strides(v)
     if len(shape) != 4 or shape[2] != kv_heads or shape[3] != head_dim:
         _bad("k_pages", k, f"[num_pages, page_size, {kv_heads}, {head_dim}]")
     if dtype is _BF16:
@@ -122,7 +127,7 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
             lib.paged_attn_entry, lib.device_entry, q, k_pages, v_pages, page_table, lens, out, workspace.ptr,
             workspace.sizes, scale, window, k_scale, v_scale, lse, stream) == 0:
         return out
-    dev, shape, qs, os = _device(q, "q"), q.shape, q.stride(), out.stride()
+    dev, shape, qs, os = _device(q, "q"), q.shape, _strides(q), _strides(out)
     if len(shape) != 3 or q.dtype is not _BF16 or (qs[2] != 1 and shape[2] != 1):
         _bad("q", q, "bfloat16 [batch, heads, head_dim], contiguous in its last dimension,")
     if out.shape != shape or out.dtype is not _BF16 or out.get_device() != dev or os[2] != 1:
@@ -132,7 +137,7 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
     if not kv or heads % kv:
         _bad("k_pages", k_pages, f"[num_pages, page_size, kv_heads, {hd}] with kv_heads dividing {heads}")
     cache, pool, ks, vs = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
-    ts, tst = page_table.shape, page_table.stride()
+    ts, tst = page_table.shape, _strides(page_table)
     if len(ts) != 2 or ts[0] != batch or page_table.dtype is not _I32 or page_table.get_device() != dev or (
             tst[1] != 1 and ts[1] != 1):
         _bad("page_table", page_table, f"int32 [{batch}, max_pages], contiguous in its last dimension,")
@@ -143,7 +148,7 @@ def paged_attention(lib, q, k_pages, v_pages, page_table, lens, out, workspace, 
         if lse.shape != (batch, heads) or lse.dtype is not _F32 or lse.get_device() != dev or (
                 lse.stride(1) != 1 and heads != 1):
             _bad("lse", lse, f"float32 [{batch}, {heads}], contiguous in its last dimension,")
-        lp, ls = lse.data_ptr(), lse.stride(0)
+        lp, ls = lse.data_ptr(), _strides(lse)[0]
     if workspace.sizes != (dev, heads, kv, hd):
         raise ValueError(f"workspace is for (device, heads, kv_heads, head_dim) = {workspace.sizes}, the call for "
                          f"{(dev, heads, kv, hd)}")
@@ -178,14 +183,14 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
             lib.qkv_rope_cache_entry, lib.device_entry, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_table, seq,
             q_norm, k_norm, eps, interleaved, k_scale, v_scale, k_out, stream) == 0:
         return q_out
-    dev, qs, xs = _device(qkv, "qkv"), q_out.stride(), qkv.stride()
+    dev, qs, xs = _device(qkv, "qkv"), _strides(q_out), _strides(qkv)
     if len(qs) != 3 or q_out.dtype is not _BF16 or q_out.get_device() != dev or qs[2] != 1:
         _bad("q_out", q_out, "bfloat16 [tokens, heads, head_dim], contiguous in its last dimension,")
     tokens, heads, hd = q_out.shape
     if k_pages is not None:
         kv = k_pages.shape[2] if k_pages.dim() == 4 else 0
         cache, (num_pages, page_size, _, _), ks, vs = _pools(k_pages, v_pages, kv, hd, k_scale, v_scale, dev)
-        kp, vp, shape, tst = k_pages.data_ptr(), v_pages.data_ptr(), page_table.shape, page_table.stride()
+        kp, vp, shape, tst = k_pages.data_ptr(), v_pages.data_ptr(), page_table.shape, _strides(page_table)
         if len(shape) != 2 or page_table.dtype is not _I32 or page_table.get_device() != dev or (
                 tst[1] != 1 and shape[1] != 1) or (seq is None and shape[0] < tokens):
             _bad("page_table", page_table, "int32 [sequences, max_pages], contiguous in its last dimension,")
@@ -206,7 +211,7 @@ def qkv_rope_cache(lib, qkv, positions, inv_freq, q_out, k_pages, v_pages, page_
         _bad("inv_freq", inv_freq, "contiguous float64 [rot / 2]")
     ko = kos = 0
     if k_out is not None:
-        kos = k_out.stride()
+        kos = _strides(k_out)
         if k_out.shape != (tokens, kv, hd) or k_out.dtype is not _BF16 or k_out.get_device() != dev or kos[2] != 1:
             _bad("k_out", k_out, f"bfloat16 {(tokens, kv, hd)}, contiguous in its last dimension,")
         ko = k_out.data_ptr()
@@ -231,7 +236,7 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
     if _bind is not None and _bind.lora(lib.lora_entry, lib.device_entry, x, a, b, adapter, out, base, scaling, ranks,
                                         stream) == 0:
         return out
-    dev, xs, sa, sb, os = _device(x, "x"), x.stride(), a.stride(), b.stride(), out.stride()
+    dev, xs, sa, sb, os = _device(x, "x"), _strides(x), _strides(a), _strides(b), _strides(out)
     if len(xs) != 2 or x.dtype is not _BF16 or xs[1] != 1 or len(sa) != 3 or len(sb) != 3:
         _bad("x", x, "bfloat16 [M, K], contiguous in its last dimension (a [adapters, rank, K], b [adapters, N, rank]),")
     m, k = x.shape
@@ -249,7 +254,7 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
     if base is not None:
         if base.shape != (m, n) or base.dtype is not _BF16 or base.get_device() != dev or base.stride(1) != 1:
             _bad("base", base, f"bfloat16 {(m, n)}, contiguous in its last dimension,")
-        bp, bs = base.data_ptr(), base.stride(0)
+        bp, bs = base.data_ptr(), _strides(base)[0]
     rc = lib.lora(_pack_lora(
         x.data_ptr(), a.data_ptr(), b.data_ptr(), adapter.data_ptr(),
         0 if ranks is None else _flat("ranks", ranks, _I32, (n_ad,), dev),

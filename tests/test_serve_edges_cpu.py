@@ -162,3 +162,37 @@ def test_attention_size_limits(L, change):
     assert L._lib.paia_gemv_paged_attn(T.packed("paia_gemv_attn", serve.ATTN, a), None) == -2
     if a["batch"] > 2:                                           # its own size alone is what is refused
         assert L._lib.paia_gemv_paged_attn(T.packed("paia_gemv_attn", serve.ATTN, dict(a, batch=0)), None) == 0
+
+
+def test_strides_of_one_do_not_count(monkeypatch):
+    """Python's route: the stride of a dimension of one may be anything (a row of a wider buffer, one head of many) and the
+    struct holds 0 for it, as the extension's route has it."""
+    import test_serve_cpu as T
+    from paia_gemv import serve
+    monkeypatch.setattr(serve, "_bind", None)
+    monkeypatch.setattr(serve, "_current_device", lambda: 0)
+    monkeypatch.setattr(serve, "_raw_stream", lambda d: 0)
+    rec = T.Recorder()
+
+    def odd(*shape, dtype=torch.bfloat16):
+        """Zeros of this shape whose dimensions of one have the stride 13."""
+        t = torch.zeros(shape, dtype=dtype)
+        return T.on(t.as_strided(shape, [13 if n == 1 else s for n, s in zip(shape, t.stride())]))
+
+    def packed(name, fmt):
+        return dict(zip([n for n, _ in T.fields(name)], fmt.unpack(rec.calls[-1])))
+    i32, f32 = torch.int32, torch.float32
+    serve.paged_attention(rec, odd(1, 1, 64), odd(1, 1, 1, 64), odd(1, 1, 1, 64), odd(1, 6, dtype=i32), odd(1, dtype=i32),
+                          odd(1, 1, 64), serve.AttentionWorkspace(odd(64, dtype=torch.uint8), 1, 1, 64),
+                          lse=odd(1, 1, dtype=f32))
+    got = packed("paia_gemv_attn", serve.ATTN)
+    assert not any(v for n, v in got.items() if n.split("_")[0] in "qkv" and n.split("_")[-1] in ("batch", "head", "page", "token"))
+    assert got["out_batch"] == got["out_head"] == got["lse_batch"] == got["table_batch"] == 0
+    serve.qkv_rope_cache(rec, odd(1, 3 * 64), odd(1, dtype=i32), odd(32, dtype=torch.float64), odd(1, 1, 64), odd(1, 1, 1, 64),
+                         odd(1, 1, 1, 64), odd(1, 1, dtype=i32), k_out=odd(1, 1, 64))
+    got = packed("paia_gemv_rope_cache", serve.ROPE_CACHE)
+    assert not any(got[n] for n in ("qkv_token", "q_token", "q_head", "ko_token", "ko_head", "table_seq", "k_page", "k_row",
+                                    "k_head", "v_page", "v_row", "v_head"))
+    serve.lora(rec, odd(1, 64), odd(1, 8, 64), odd(1, 40, 8), odd(1, dtype=i32), odd(1, 40), base=odd(1, 40))
+    got = packed("paia_gemv_lora_args", serve.LORA)
+    assert not any(got[n] for n in ("x_row", "base_row", "out_row", "a_adapter", "b_adapter")) and got["a_row"] == 64
