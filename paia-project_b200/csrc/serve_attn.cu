@@ -893,7 +893,7 @@ extern "C" int paia_gemv_paged_attn(const paia_gemv_attn* a, void* stream) {
         a->window < 0 || !(a->scale > 0.f) || !(a->scale <= 3.0e38f))
         return -2;
     if (a->batch == 0) return 0;
-    if (!a->q || !a->k || !a->v || !a->page_table || !a->lens || !a->out || !a->workspace) return -2;
+    if (!a->q || !a->k || !a->v || (!a->page_table && a->max_pages) || !a->lens || !a->out || !a->workspace) return -2;
     const int es = a->cache == 0 ? 2 : 1;
     const long long unit = 16 / es;
     if (!aligned_to(a->q, 16) || !aligned_to(a->k, 16) || !aligned_to(a->v, 16) || !aligned_to(a->workspace, 16) ||

@@ -73,6 +73,21 @@ def test_attention_of_more_than_1024_sequences(L, n, heads, kv, hd, dtype):
     assert (out[~live] == 0).all() and (lse[~live] == -math.inf).all()
 
 
+@pytest.mark.parametrize("n", [1, 40, 700])
+@pytest.mark.parametrize("dtype", [BF16, E4M3])
+def test_attention_without_pages(L, n, dtype):
+    """A page table of no columns: every sequence is empty, and a length above 0 is cut to that (code 11)."""
+    from paia_gemv import serve
+    pool = torch.full((1, 16, 2, 64), math.nan, device="cuda").to(dtype)
+    q = torch.ones(n, 8, 64, dtype=BF16, device="cuda")
+    out, lse = torch.full_like(q, 7.0), torch.full((n, 8), 7.0, device="cuda")
+    ws = serve.attention_workspace(L, 8, 2, 64)
+    for lens, code in ((i32([0] * n), 0), (i32([0] * (n - 1) + [5]), 11)):
+        serve.paged_attention(L, q, pool, pool, torch.empty(n, 0, dtype=torch.int32, device="cuda"), lens, out.fill_(7), ws, lse=lse)
+        torch.cuda.synchronize()
+        assert L.device_error(True) == code and (out == 0).all() and (lse == -math.inf).all()
+
+
 # ------------------------------------------------------------------ infinities and NaN
 
 SPLITS = [[17], [40, 3000], [3] * 200]                           # a cluster per unit, the list, CTAs of two warps
