@@ -70,7 +70,8 @@ def _flat(name, t, dtype, shape, dev):
 
 def _strides(t):
     """The strides of a tensor, 0 along a dimension of one: never used, and free to be anything in torch."""
-    return tuple(0 if n == 1 else s for n, s in zip(t.shape, t.stride()))
+    shape, strides = t.shape, t.stride()
+    return tuple([0 if n == 1 else s for n, s in zip(shape, strides)]) if 1 in shape else strides
 
 
 def _device(t, name):
