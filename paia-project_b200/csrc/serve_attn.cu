@@ -26,7 +26,8 @@
 //             m), which f16 holds, so that this goes down to 2^-29 of the largest P and nothing above 2^-40 is dropped:
 //             many small ones can outweigh a large one whose v is small. P has no remainder to fill rows 8-15 with, so
 //             the second product is taken as O^T += V^T P^T, dims as rows: half
-//             the MMAs and sums (16 sequences of 4096 at head_dim 256: 31 us where rows of heads spilled and took 64).
+//             the MMAs and sums (16 sequences of 4096 at head_dim 256: 31 us where rows of heads spilled and took 64 at the
+//             time; 33 now).
 //             The order of the k dimension and of V's columns is free, so a lane reads its bytes 16 at a time. (The
 //             e4m3 form of mma.sync was no shorter way: 17% more instructions, 64 sequences of 8192 in 270 us where
 //             this took 257 at the time.)
@@ -35,9 +36,9 @@
 //             is not the whole goes to the workspace, and the last CTA to arrive merges all parts in list order (the
 //             same bits whichever CTA it is) and resets the counter; no CTA waits for another. Small calls take a
 //             cluster per unit instead, whose CTAs store their parts into the first one's shared memory.
-// Measured (head_dim 128): one sequence of 131072 positions, 32/8 heads, bf16: 87.6 us, 6.1 TB/s; 64 sequences of 8192,
-// 16/8 heads, e4m3: 164 us, 6.5 TB/s, while the SM clock holds (as much bound by instruction issue); one sequence of 1024:
-// 5.3 us.
+// Measured (head_dim 128): one sequence of 131072 positions, 32/8 heads, bf16: 87.3 us, 6.1 TB/s; 64 sequences of 8192,
+// 32/8 heads, e4m3: 165 us, 6.5 TB/s, while the SM clock holds (as much bound by instruction issue); one sequence of 1024:
+// 5.5 us.
 #include <cooperative_groups.h>
 #include "paia_gemv.h"
 #include "serve_common.cuh"

@@ -17,9 +17,9 @@
 //             with up to 8 rows hi and lo are rows 0-7 and 8-15 of one MMA, with more they take two. Column c of the
 //             group's tile j is n = 8 (c / 2) + 2 j + c % 2, so that a lane ends up with 8 neighbouring columns of its
 //             row: base is read and out written 16 bytes at a time.
-// Measured: 128 rows of as many adapters of rank 64, K 14336, N 4096: 53 us (5.8 TB/s). 61 rows of 24 adapters of mixed
-// rank up to 32, K 4096, N 28672: 18.7 us, phases that each wait for memory once. 8 rows, rank 16, K 4096, N 6144: 6.1 us.
-// A prompt's rows of one adapter of rank 16, K = N = 4096: 8192 in 67 us, 32768 in 241 (a search of all rows for every
+// Measured: 128 rows of as many adapters of rank 64, K 14336, N 4096: 52.5 us (5.9 TB/s). 61 rows of 24 adapters of mixed
+// rank up to 32, K 4096, N 28672: 18.8 us, phases that each wait for memory once. 8 rows, rank 16, K 4096, N 6144: 6.0 us.
+// A prompt's rows of one adapter of rank 16, K = N = 4096: 8192 in 68 us, 32768 in 240 (a search of all rows for every
 // item: 90 and 716).
 #include <cooperative_groups.h>
 #include <math.h>

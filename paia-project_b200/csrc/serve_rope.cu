@@ -9,7 +9,8 @@
 // compute the token's angles once, each lane keeps the sine and cosine of its 8 pairs and the norm's weights in registers,
 // and the heads then pass by, the next one's loads in flight. Nothing waits on another warp. (CTAs that shared a table of
 // several tokens' angles in shared memory: 45 us for 8192 tokens of 48 heads of 128, 97 with an e4m3 cache.)
-// Measured: those 8192 tokens in 43.9 us (4.6 TB/s read and written), 64 with an e4m3 cache; one token in 3.3 us.
+// Measured: those 8192 tokens in 44.0 us (4.6 TB/s read and written), 64 with an e4m3 cache; one token in 3.1 us on the
+// device.
 // The angle is reduced in fp64 (pos * inv_freq reaches 10^5 radians, where fp32 has 2^-8 left) and its sine and cosine
 // are taken in fp32. What an e4m3 cache stores is the e4m3 value nearest to the exact one: where the fp32 result lies so
 // near to the border between two of its coarse steps that fp32's error could cross it (about one element in 10^4), the
