@@ -316,11 +316,99 @@ typedef struct paia_gemv_lora_args {
 } paia_gemv_lora_args;
 int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream);
 
+/* ---- A feed-forward block with experts (no reference kernel): choosing each token's experts, the experts' products, and the
+ * weighted sum, norms and residual around them. The rules of the serving operators above hold here too. A bad index on the
+ * device (code 14) is never followed to memory. */
+
+/* Token t's experts are the top_k of its `experts` logits (bf16 or fp32), in falling order, ties to the lowest index, NaN
+ * last. scoring 0, softmax: ordered by the logits; weights scale e^l_j / sum of e^l over the chosen (renormalise) or over all
+ * experts; 0 where every logit is -inf. scoring 1, sigmoid: ordered by s_e + bias[e], s = 1 / (1 + e^-l), in fp64; weights
+ * scale s_j, over the sum of the chosen s where renormalise (0 where that sum is 0). Weights are fp32. The chosen (t, j),
+ * numbered t top_k + j, are grouped by expert in the order of their numbers: expert e's stand at places offsets[e] ..
+ * offsets[e + 1] - 1, places[t][j] is where (t, j) stands and rows[place] its token. A token with pos[t] < 0 is padding: it
+ * has ids and places -1, weights 0 and no place. rows behind offsets[experts] stay as they were. experts <= 1024, top_k <=
+ * 32, tokens <= 2^24. `workspace`: paia_gemv_route_workspace(experts) bytes, 16-byte aligned, of any content; calls that may
+ * overlap on the GPU need one each. */
+typedef struct paia_gemv_route_args {
+    const void* logits;          /* [tokens][experts] */
+    const float* bias;           /* [experts] or NULL; scoring 1 only */
+    const int* pos;              /* [tokens] or NULL */
+    float* weights;              /* [tokens][top_k] */
+    int* ids;                    /* [tokens][top_k] */
+    int* places;                 /* [tokens][top_k] */
+    int* rows;                   /* [tokens * top_k] */
+    int* offsets;                /* [experts + 1] */
+    void* workspace;
+    long long logits_row;
+    int tokens, experts, top_k;
+    int logits_type;             /* 0 bf16, 1 fp32 */
+    int scoring;                 /* 0 softmax, 1 sigmoid */
+    int renormalise;
+    float scale;
+} paia_gemv_route_args;
+size_t paia_gemv_route_workspace(int experts);               /* 0: unsupported */
+int paia_gemv_route(const paia_gemv_route_args* a, void* stream);
+
+/* Products of grouped rows with their expert's weights W[e] [N][K]: for i in offsets[e] .. offsets[e + 1] - 1,
+ *   out[i] = W[e] x[rows[i]]   (rows NULL: x[i]),  or with silu, W[e] = [gate; up] of N / 2 rows each:  silu(gate x) * (up x).
+ * kind 0: W bf16; kind 1: W e4m3 with a fp32 scale per row, W[e][n] = scales[e][n] * stored. Products are exact, sums fp32,
+ * out is rounded once to bf16; how K is divided follows from the whole call, and the same call gives the same bits. A NaN or
+ * an infinity in a row of x or of W makes what it reaches NaN or infinite and nothing else. Rows of out that belong to no
+ * expert stay as they were. An offset below the one before it or outside [0, M] cuts its group short and a row of x outside
+ * [0, x_rows) reads as zeros (code 14); a bounded wait inside the kernel that gives up sets code 15. K is a multiple of 8
+ * (kind 1: 16), experts <= 1024, M <= 2^28, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of
+ * whole 16 bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed
+ * once; every launch leaves it ready for the next, of any sizes; launches that may overlap on the GPU need one each. */
+typedef struct paia_gemv_expert_args {
+    const void* w;               /* [experts][N][K] */
+    const float* scales;         /* [experts][N]; kind 1 only */
+    const void* x;               /* bf16 [x_rows][K] */
+    const int* rows;             /* [M] or NULL */
+    const int* offsets;          /* [experts + 1] */
+    void* out;                   /* bf16 [M][N], silu: [M][N / 2] */
+    void* workspace;
+    long long w_expert, w_row, x_row, out_row, scale_expert;
+    int experts, M, N, K, x_rows;
+    int kind;                    /* 0 bf16, 1 e4m3 */
+    int silu;
+    int pad;
+} paia_gemv_expert_args;
+size_t paia_gemv_expert_workspace(void);
+int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* stream);
+
+/* The end of a block and the norm before the next one, for every token t:
+ *   y = x[t], or with top_k: sum_j weights[t][j] x[places[t][j]] in the order of j (a place of -1 adds nothing)
+ *   y = y / sqrt(mean y^2 + eps) * post     (post given)
+ *   y = y * gate                            (gate given: bf16, per element (gate_col 1) or per row (gate_col 0), gate_row 0:
+ *                                            the same for every token)
+ *   h_out[t] = bf16(h[t] + scale * y),   out[t] = h_out[t] / sqrt(mean h_out[t]^2 + eps) * pre   (pre and out given)
+ * With x NULL only the norm of h is taken (h_out NULL, no post, gate, top_k). Arithmetic is fp32 (squares beyond its range
+ * are infinite), each output rounded once. h_out may be h itself; otherwise outputs overlap nothing. A place outside
+ * [-1, x_rows) is left out (code 14). hidden is a multiple of 8 up to 32768, top_k <= 64. x, h, h_out, out, post, pre and a
+ * gate per element 16-byte aligned, rows at strides of whole 16 bytes. */
+typedef struct paia_gemv_block_norm_args {
+    const void* x;               /* bf16 [x_rows][hidden] or NULL */
+    const void* h;               /* bf16 [tokens][hidden] */
+    void* h_out;                 /* bf16 [tokens][hidden] */
+    void* out;                   /* bf16 [tokens][hidden] or NULL */
+    const int* places;           /* [tokens][top_k] */
+    const float* weights;        /* [tokens][top_k] */
+    const float* post;           /* [hidden] or NULL */
+    const float* pre;            /* [hidden] or NULL */
+    const void* gate;            /* or NULL */
+    long long x_row, h_row, h_out_row, out_row, places_row, weights_row, gate_row;
+    int tokens, hidden, top_k, x_rows, gate_col;
+    float eps, scale;
+    int pad;
+} paia_gemv_block_norm_args;
+int paia_gemv_block_norm(const paia_gemv_block_norm_args* a, void* stream);
+
 /* The calling thread's current CUDA device; -1 where there is none. */
 int paia_gemv_current_device(void);
 
 /* Device-side error words of the current device: one of the GEMVs, set by kernels whose bounded waits gave up (codes below
- * 10), and one of each serving operator, set by the first bad index that it met in device memory (10 to 13). Returns the
+ * 10), and one of each serving operator, set by the first bad index that it met in device memory (10 to 14; 15: a bounded wait of
+ * paia_gemv_expert_matmul gave up). Returns the
  * first of them that is set (0 = none; -1: they cannot be read); clear != 0 resets that one alone, so calls until 0 return
  * them all. Synchronous; wait for the kernels in question first. */
 int paia_gemv_device_error(int clear);

@@ -24,6 +24,9 @@ const Variant* extra_int4a(int* n);
 int attn_device_error(int clear);
 int rope_device_error(int clear);
 int lora_device_error(int clear);
+int route_device_error(int clear);
+int experts_device_error(int clear);
+int norm_device_error(int clear);
 
 // ------------------------------------------------------------------ per-device caches
 namespace {
@@ -90,10 +93,7 @@ int max_ctas_per_sm(KernelFn fn, int threads, size_t smem) {
 }
 
 // cuTensorMapEncodeTiled through the runtime's driver entry point (no link against the driver library).
-using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
-                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
-                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
-static EncodeTiledFn encode_tiled() {
+EncodeTiledFn encode_tiled() {
     static const EncodeTiledFn fn = []() -> EncodeTiledFn {
         void* f = nullptr;
         cudaDriverEntryPointQueryResult q = cudaDriverEntryPointSymbolNotFound;
@@ -840,10 +840,12 @@ int paia_gemv_current_device(void) {
 }
 
 // The first error word of the current device that is set (0 = none): the codes of the TMA-fed kernels' bounded waits, 6 and
-// 8 from the tensor-parallel exchange, then a word of each serving operator (10 to 13, bad indices in device memory).
+// 8 from the tensor-parallel exchange, then a word of each serving operator (10 to 14, bad indices in device memory; 15, a
+// bounded wait of the experts' products).
 // clear != 0 resets the word that is returned and leaves the others for the next call. Synchronous (symbol copies).
 int paia_gemv_device_error(int clear) {
-    int (*const words[4])(int) = {tma_device_error, attn_device_error, rope_device_error, lora_device_error};
+    int (*const words[])(int) = {tma_device_error, attn_device_error, rope_device_error, lora_device_error,
+                                 route_device_error, experts_device_error, norm_device_error};
     for (auto word : words)
         if (const int w = word(clear)) return w;
     return 0;

@@ -41,6 +41,11 @@ int max_ctas_per_sm(KernelFn fn, int threads, size_t smem);  // occupancy, cache
 size_t sm_smem_bytes();                                      // shared memory per SM, less one CTA's reservation
 size_t max_dyn_smem();                                       // opt-in shared memory per block, current device
 
+using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
+                                   const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
+                                   CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled();                                // cuTensorMapEncodeTiled; nullptr where the driver lacks it
+
 inline int ilog2(int v) { int l = 0; while ((1 << (l + 1)) <= v) ++l; return l; }
 
 // Warps per row: enough that every warp still has >= U steps of its row (K-split for long rows), and enough that the

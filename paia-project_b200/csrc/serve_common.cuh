@@ -1,5 +1,4 @@
-// Shared by the serving operators (serve_attn.cu, serve_rope.cu, serve_lora.cu): the device error word, PTX helpers and
-// the launch. Like the GEMVs they allocate nothing, never synchronise and launch on the caller's stream.
+// Shared by the serving operators (serve_*.cu): the device error word, PTX helpers and the launch. Like the GEMVs they allocate nothing, never synchronise and launch on the caller's stream.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>
@@ -10,10 +9,10 @@
 
 namespace pb2 {
 
-// First invalid value a kernel met in device-side indices (page tables, lengths, positions, adapter ids), one word per
-// translation unit; paia_gemv_device_error reports and clears it. Apart from the GEMVs' word of bounded waits: an entry
+// First invalid value a kernel met in device-side indices (page tables, lengths, positions, adapter ids, routing), one word
+// per translation unit; paia_gemv_device_error reports and clears it. Apart from the GEMVs' word of bounded waits: an entry
 // there makes their waits give up early, and a bad index here is no reason for that.
-constexpr int kErrPage = 10, kErrLength = 11, kErrPosition = 12, kErrAdapter = 13;
+constexpr int kErrPage = 10, kErrLength = 11, kErrPosition = 12, kErrAdapter = 13, kErrRouting = 14, kErrServeWait = 15;
 static __device__ int g_serve_error;
 
 __device__ __forceinline__ void serve_error(int code) { atomicCAS(&g_serve_error, 0, code); }
@@ -170,5 +169,8 @@ inline bool aligned_to(const void* p, unsigned a) { return (reinterpret_cast<uin
 int attn_device_error(int clear);
 int rope_device_error(int clear);
 int lora_device_error(int clear);
+int route_device_error(int clear);
+int experts_device_error(int clear);
+int norm_device_error(int clear);
 
 }  // namespace pb2

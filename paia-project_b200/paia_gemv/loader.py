@@ -124,7 +124,7 @@ class GemvLib:
         lib.paia_gemv_variant_info_ex.restype = I
         lib.paia_gemv_variant_info_ex.argtypes = [I, I, ctypes.POINTER(VariantEx)]
         # serving operators (paia_gemv.serve drives these): the bytes of the C struct and the stream; the return code
-        for name in ("paged_attn", "qkv_rope_cache", "lora"):
+        for name in ("paged_attn", "qkv_rope_cache", "lora", "route", "expert_matmul", "block_norm"):
             fn = getattr(lib, "paia_gemv_" + name)
             fn.restype = I
             fn.argtypes = [P, P]
@@ -134,6 +134,9 @@ class GemvLib:
         self.device_entry = ctypes.cast(lib.paia_gemv_current_device, P).value
         lib.paia_gemv_paged_attn_workspace.restype = ctypes.c_size_t
         lib.paia_gemv_paged_attn_workspace.argtypes = [I, I, I]
+        lib.paia_gemv_route_workspace.restype = ctypes.c_size_t
+        lib.paia_gemv_route_workspace.argtypes = [I]
+        lib.paia_gemv_expert_workspace.restype = ctypes.c_size_t
         lib.paia_gemv_device_error.restype = I
         lib.paia_gemv_device_error.argtypes = [I]
         lib.paia_gemv_version.restype = ctypes.c_char_p
@@ -329,7 +332,8 @@ class GemvLib:
     def plan_destroy(self, plan):
         self._check(self._lib.paia_gemv_plan_destroy(plan), "paia_gemv_plan_destroy")
 
-    # --- serving operators (paged_attn, qkv_rope_cache and lora are bound in __init__; paia_gemv.serve packs their structs)
+    # --- serving operators (paged_attn, qkv_rope_cache, lora, route, expert_matmul and block_norm are bound in __init__;
+    # paia_gemv.serve packs their structs)
     def paged_attn_workspace(self, heads, kv_heads, head_dim):
         n = self._lib.paia_gemv_paged_attn_workspace(heads, kv_heads, head_dim)
         if n == 0:
@@ -337,10 +341,19 @@ class GemvLib:
                                f"head_dim={head_dim})")
         return n
 
+    def route_workspace(self, experts):
+        n = self._lib.paia_gemv_route_workspace(experts)
+        if n == 0:
+            raise RuntimeError(f"paia_gemv_route_workspace: unsupported number of experts {experts}")
+        return n
+
+    def expert_workspace(self):
+        return self._lib.paia_gemv_expert_workspace()
+
     def device_error(self, clear=True):
         """The first device-side error word that is set (0 = none): below 10 from kernels whose bounded waits gave up, 10
-        to 13 from serving operators that met a bad page id, length, position or adapter id (a word each: call until 0 to
-        see them all)."""
+        to 14 from serving operators that met a bad page id, length, position, adapter id or routing index, 15 from a
+        bounded wait of expert_matmul (a word each: call until 0 to see them all)."""
         return self._lib.paia_gemv_device_error(1 if clear else 0)
 
 

@@ -5,6 +5,9 @@ outputs are written in place, nothing is allocated and nothing synchronises, so 
     qkv_rope_cache   per-head norm, rotary positions and cache write of a fused QKV projection's rows
     paged_attention  attention of one new token per sequence over the paged cache
     lora             the low-rank adapters of many requests, added to a shared projection
+    route            each token's experts and their weights, and the tokens grouped by expert (a `routing`)
+    expert_matmul    the products of each group with its expert's weights
+    block_norm       a block's (weighted) output, normed, gated and added to the residual, and the norm before the next one
 
 Caches are a pair of tensors [num_pages, page_size, kv_heads, head_dim] (bf16, or float8_e4m3fn with a fp32 scale per
 kv head), in any layout whose head_dim is contiguous: a [num_pages, kv_heads, page_size, head_dim] pool is passed as
@@ -23,6 +26,9 @@ from .loader import _PKG_ROOT, load_lib
 ATTN = struct.Struct("10P 12q 9i f")
 ROPE_CACHE = struct.Struct("13P 12q 11i f")
 LORA = struct.Struct("8P 7q 5i 4x")
+ROUTE = struct.Struct("9P q 6i f 4x")
+EXPERTS = struct.Struct("7P 5q 8i")
+BLOCK_NORM = struct.Struct("9P 7q 5i 2f i")
 
 def _load_bind():
     """The extension that checks and makes these calls in C (csrc/serve_bind.cpp), or None: without it, and for every
@@ -47,7 +53,9 @@ _bind = _load_bind()
 _current_device = getattr(torch._C, "_cuda_getDevice", lambda: -1)
 _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", lambda device: 0)
 _pack_attn, _pack_rope, _pack_lora = ATTN.pack, ROPE_CACHE.pack, LORA.pack
+_pack_route, _pack_experts, _pack_norm = ROUTE.pack, EXPERTS.pack, BLOCK_NORM.pack
 _BF16, _F32, _F64, _I32, _E4M3 = torch.bfloat16, torch.float32, torch.float64, torch.int32, torch.float8_e4m3fn
+_U8 = torch.uint8
 
 
 def _bad(name, t, what):
@@ -265,3 +273,194 @@ def lora(lib, x, a, b, adapter, out, *, base=None, scaling=None, ranks=None, str
     if rc:
         lib._check(rc, "paia_gemv_lora")
     return out
+
+
+class Routing:
+    """Where `route` writes for up to `tokens` tokens: weights fp32 [tokens, top_k], experts and places int32 [tokens, top_k],
+    rows int32 [tokens * top_k], offsets int32 [experts + 1], on one CUDA device, and its workspace. (`routing` makes one.)
+    first(n) is the same for the first n tokens, over the same memory."""
+
+    def __init__(self, lib, weights, experts, places, rows, offsets, workspace):
+        self.lib, self.weights, self.experts, self.places, self.rows = lib, weights, experts, places, rows
+        self.offsets, self.workspace = offsets, workspace
+        dev, (tokens, top_k), n = weights.get_device(), weights.shape, offsets.shape[0] - 1
+        need = lib.route_workspace(n) if weights.is_cuda else 0
+        for name, t, dtype, shape in (("weights", weights, _F32, (tokens, top_k)), ("experts", experts, _I32, (tokens, top_k)),
+                                      ("places", places, _I32, (tokens, top_k)), ("rows", rows, _I32, (tokens * top_k,)),
+                                      ("offsets", offsets, _I32, (n + 1,)), ("workspace", workspace, _U8, workspace.shape)):
+            if t.dtype is not dtype or t.shape != shape or t.get_device() != dev or not t.is_contiguous():
+                _bad(name, t, f"contiguous {dtype} {shape}")
+        if workspace.numel() < need or workspace.data_ptr() % 16:
+            _bad("workspace", workspace, f"contiguous uint8 of at least {need} bytes, 16-byte aligned,")
+        self.ptrs = tuple(t.data_ptr() for t in (weights, experts, places, rows, offsets, workspace))
+        self.sizes = (dev, tokens, n, top_k)
+
+    def first(self, n):
+        k = self.sizes[3]
+        return Routing(self.lib, self.weights[:n], self.experts[:n], self.places[:n], self.rows[:n * k], self.offsets,
+                       self.workspace)
+
+
+def routing(lib, tokens, experts, top_k, device=None):
+    """A `Routing` for up to `tokens` tokens. Calls that may overlap on the GPU need one each."""
+    dev = "cuda" if device is None else device
+    i32 = lambda *shape: torch.zeros(*shape, dtype=_I32, device=dev)   # noqa: E731
+    return Routing(lib, torch.zeros(tokens, top_k, dtype=_F32, device=dev), i32(tokens, top_k), i32(tokens, top_k),
+                   i32(tokens * top_k), i32(experts + 1), torch.zeros(lib.route_workspace(experts), dtype=_U8, device=dev))
+
+
+_SCORING = {"softmax": 0, "sigmoid": 1}
+
+
+def route(lib, logits, routing, *, scoring="softmax", bias=None, renormalise=True, scale=1.0, positions=None, stream=None):
+    """Each token's top_k experts by its logits (bf16 or fp32 [tokens, experts]), in falling order (ties to the lowest index),
+    their weights (times `scale`), and the tokens grouped by expert, into `routing`. scoring "softmax": weights e^l over the
+    sum of the chosen (renormalise) or of all; "sigmoid": ordered by sigmoid(l) + bias (fp32 [experts] or None), weights
+    sigmoid(l), over the sum of the chosen where renormalise. positions (int32 [tokens], None: all live): rows below 0 are
+    padding, with experts and places -1 and no place among the rows."""
+    if _bind is not None and hasattr(_bind, "route") and _bind.route(lib.route_entry, lib.device_entry, logits, routing.ptrs, routing.sizes, scoring, bias,
+                                         renormalise, scale, positions, stream) == 0:
+        return routing
+    dev, ls = _device(logits, "logits"), _strides(logits)
+    sizes = routing.sizes
+    if logits.dtype not in (_BF16, _F32) or logits.shape != sizes[1:3] or (ls[1] != 1 and sizes[2] != 1):
+        _bad("logits", logits, f"bfloat16 or float32 {sizes[1:3]}, contiguous in its last dimension,")
+    if sizes[0] != dev:
+        raise ValueError(f"routing is on device {sizes[0]}, the call on {dev}")
+    if scoring not in _SCORING:
+        raise ValueError(f"scoring must be one of {tuple(_SCORING)}, got {scoring!r}")
+    if bias is not None and scoring != "sigmoid":
+        raise ValueError("bias belongs to sigmoid scoring")
+    weights, experts, places, rows, offsets, workspace = routing.ptrs
+    rc = lib.route(_pack_route(
+        logits.data_ptr(), _flat("bias", bias, _F32, (sizes[2],), dev), _flat("positions", positions, _I32, (sizes[1],), dev),
+        weights, experts, places, rows, offsets, workspace, ls[0], sizes[1], sizes[2], sizes[3],
+        0 if logits.dtype is _BF16 else 1, _SCORING[scoring], 1 if renormalise else 0, scale),
+        _raw_stream(dev) if stream is None else stream)
+    if rc:
+        lib._check(rc, "paia_gemv_route")
+    return routing
+
+
+class ExpertWorkspace:
+    """The workspace of `expert_matmul` over a buffer of the caller's: contiguous uint8 on a CUDA device, 16-byte aligned, of
+    at least lib.expert_workspace() bytes, all zero before its first call. (`expert_workspace` makes both.)"""
+
+    def __init__(self, buffer, lib=None):
+        if buffer.is_cuda:
+            need = (load_lib() if lib is None else lib).expert_workspace()
+            if buffer.dtype is not _U8 or not buffer.is_contiguous() or buffer.numel() < need or buffer.data_ptr() % 16:
+                _bad("buffer", buffer, f"contiguous uint8 of at least {need} bytes, 16-byte aligned,")
+        self.buffer, self.ptr, self.device = buffer, buffer.data_ptr(), buffer.get_device()
+
+
+def expert_workspace(lib, device=None):
+    """The zeroed workspace of `expert_matmul`, for calls of any sizes. Calls that may overlap on the GPU need one each."""
+    return ExpertWorkspace(torch.zeros(lib.expert_workspace(), dtype=_U8, device="cuda" if device is None else device), lib)
+
+
+def expert_matmul(lib, w, x, offsets, out, workspace, *, scales=None, rows=None, silu=False, stream=None):
+    """out[i] = w[e] x[rows[i]] for i in offsets[e] .. offsets[e + 1] - 1 of every expert e (int32 [experts + 1]; `route`
+    makes offsets and rows). w [experts, N, K] bf16, or e4m3 (float8_e4m3fn or its bytes as uint8) with scales fp32
+    [experts, N]; x bf16 [rows, K]; rows int32 [M] (None: x[i]); out bf16 [M, N] (apart from x). silu: w[e] holds [gate; up]
+    and out [M, N / 2] gets silu(gate x) * (up x). Rows of out that belong to no expert stay as they were."""
+    if _bind is not None and hasattr(_bind, "route") and _bind.expert_matmul(lib.expert_matmul_entry, lib.device_entry, w, x, offsets, out, workspace.ptr,
+                                                 workspace.device, scales, rows, silu, stream) == 0:
+        return out
+    dev, sw, xs, os = _device(x, "x"), _strides(w), _strides(x), _strides(out)
+    if len(xs) != 2 or x.dtype is not _BF16 or xs[1] != 1:
+        _bad("x", x, "bfloat16 [rows, K], contiguous in its last dimension,")
+    kind = 0 if w.dtype is _BF16 else 1
+    if len(sw) != 3 or w.dtype not in (_BF16, _E4M3, _U8) or w.get_device() != dev or sw[2] != 1 or w.shape[2] != x.shape[1]:
+        _bad("w", w, f"bfloat16, float8_e4m3fn or uint8 [experts, N, {x.shape[1]}], contiguous in its last dimension,")
+    e, n, k = w.shape
+    ss = (0, 1)
+    if kind == 1:
+        if scales is None or scales.shape != (e, n) or scales.dtype is not _F32 or scales.get_device() != dev:
+            _bad("scales", scales, f"float32 {(e, n)}")
+        ss = _strides(scales)
+        if ss[1] != 1 and n != 1:
+            _bad("scales", scales, f"float32 {(e, n)}, contiguous in its last dimension,")
+    elif scales is not None:
+        raise ValueError("scales belong to e4m3 weights")
+    if silu and n % 2:
+        raise ValueError(f"with silu w holds gate and up: N must be even, got {n}")
+    cols = n // 2 if silu else n
+    if len(os) != 2 or out.shape[1] != cols or out.dtype is not _BF16 or out.get_device() != dev or (os[1] != 1 and cols != 1):
+        _bad("out", out, f"bfloat16 [M, {cols}], contiguous in its last dimension,")
+    m = out.shape[0]
+    if offsets.shape != (e + 1,) or offsets.dtype is not _I32 or offsets.get_device() != dev or not offsets.is_contiguous():
+        _bad("offsets", offsets, f"contiguous int32 [{e + 1}]")
+    if rows is None and x.shape[0] < m:
+        _bad("x", x, f"bfloat16 [at least {m}, {k}] where rows is None")
+    if workspace.device != dev:
+        raise ValueError(f"workspace is on device {workspace.device}, the call on {dev}")
+    rc = lib.expert_matmul(_pack_experts(
+        w.data_ptr(), 0 if scales is None else scales.data_ptr(), x.data_ptr(), _flat("rows", rows, _I32, (m,), dev),
+        offsets.data_ptr(), out.data_ptr(), workspace.ptr, sw[0], sw[1] if n > 1 else k, xs[0], os[0], ss[0], e, m, n, k,
+        x.shape[0], kind, 1 if silu else 0, 0), _raw_stream(dev) if stream is None else stream)
+    if rc:
+        lib._check(rc, "paia_gemv_expert_matmul")
+    return out
+
+
+def block_norm(lib, h, x=None, h_out=None, *, out=None, places=None, weights=None, post=None, gate=None, scale=1.0, pre=None,
+               eps=1e-5, stream=None):
+    """h_out[t] = h[t] + scale * gate * norm(y[t]), y[t] = x[t], or sum_j weights[t, j] x[places[t, j]] (int32 and fp32
+    [tokens, top_k]; a place of -1 adds nothing), norm(y) = y / sqrt(mean y^2 + eps) * post (post fp32 [hidden]; None: y as
+    it is); out[t] = h_out[t] / sqrt(mean h_out[t]^2 + eps) * pre where out and pre (fp32 [hidden]) are given. h, x, h_out,
+    out bf16 [.., hidden]; h_out may be h. gate bf16 [hidden], [tokens, 1] or [tokens, hidden]. Without x (and h_out): the
+    norm of h alone."""
+    if _bind is not None and hasattr(_bind, "route") and _bind.block_norm(lib.block_norm_entry, lib.device_entry, h, x, h_out, out, places, weights, post,
+                                              gate, scale, pre, eps, stream) == 0:
+        return out if h_out is None else h_out
+    dev, hs = _device(h, "h"), _strides(h)
+    if len(hs) != 2 or h.dtype is not _BF16 or hs[1] != 1:
+        _bad("h", h, "bfloat16 [tokens, hidden], contiguous in its last dimension,")
+    t, hid = h.shape
+
+    def like(name, v, n):
+        if v is None:
+            return 0, 0
+        s = _strides(v)
+        if len(s) != 2 or (v.shape[0] < t if n is None else v.shape[0] != n) or v.shape[1] != hid or v.dtype is not _BF16 or (
+                v.get_device() != dev or s[1] != 1):
+            _bad(name, v, f"bfloat16 [{'rows' if n is None else n}, {hid}], contiguous in its last dimension,")
+        return v.data_ptr(), s[0]
+
+    top_k, ps, wts = 0, 0, 0
+    if places is not None:
+        if len(places.shape) != 2 or places.shape[0] != t or places.dtype is not _I32 or places.get_device() != dev or (
+                places.stride(1) != 1 and places.shape[1] != 1):
+            _bad("places", places, f"int32 [{t}, top_k], contiguous in its last dimension,")
+        top_k = places.shape[1]
+        if weights is None or weights.shape != places.shape or weights.dtype is not _F32 or weights.get_device() != dev or (
+                weights.stride(1) != 1 and top_k != 1):
+            _bad("weights", weights, f"float32 {(t, top_k)}, contiguous in its last dimension,")
+        ps, wts = _strides(places)[0], _strides(weights)[0]
+    elif weights is not None:
+        raise ValueError("weights belong to places")
+    if x is not None and x.dim() == 2 and places is not None:
+        if x.shape[1] != hid or x.dtype is not _BF16 or x.get_device() != dev or _strides(x)[1] != 1:
+            _bad("x", x, f"bfloat16 [rows, {hid}], contiguous in its last dimension,")
+        xp, xs = x.data_ptr(), _strides(x)[0]
+    else:
+        xp, xs = like("x", x, None)
+    op, os = like("h_out", h_out, t)
+    np, ns = like("out", out, t)
+    gp = gs = gc = 0
+    if gate is not None:
+        shape, s = gate.shape, _strides(gate)
+        if gate.dtype is not _BF16 or gate.get_device() != dev or shape not in ((hid,), (t, 1), (t, hid)) or (
+                s[-1] != 1 and shape[-1] != 1):
+            _bad("gate", gate, f"bfloat16 {(hid,)}, {(t, 1)} or {(t, hid)}, contiguous in its last dimension,")
+        gp, gs, gc = gate.data_ptr(), s[0] if len(s) == 2 else 0, 1 if shape[-1] == hid else 0
+    if (x is None) != (h_out is None):
+        raise ValueError("x and h_out go together")
+    rc = lib.block_norm(_pack_norm(
+        xp, h.data_ptr(), op, np, 0 if places is None else places.data_ptr(), 0 if weights is None else weights.data_ptr(),
+        _flat("post", post, _F32, (hid,), dev), _flat("pre", pre, _F32, (hid,), dev), gp, xs, hs[0], os, ns, ps, wts, gs, t, hid,
+        top_k, 0 if x is None else x.shape[0], gc, eps, scale, 0), _raw_stream(dev) if stream is None else stream)
+    if rc:
+        lib._check(rc, "paia_gemv_block_norm")
+    return out if h_out is None else h_out
