@@ -2,17 +2,19 @@
 // to expert e,  out[i] = W_e x[rows[i]]  (or silu(gate) * up of the two halves of W_e x), W bf16 or e4m3 with a scale per row.
 //
 // Bound: HBM where an expert has few rows (every used expert's weights once), the tensor cores where it has many. One kernel
-// serves both, with the weights as the 128 rows of a tcgen05 product and the tokens as its 16 to 256 columns, so that few
-// tokens waste nothing but columns:
-//   tile     128 rows of W_e (silu: 64 of gate and their 64 of up) x a block of tokens x all of K, in chunks of 64 of K.
-//   stream   W by TMA into 128-byte rows (e4m3: 64), x by cp.async (gathered rows, any stride) into the same swizzled form;
-//            a ring of as many stages as shared memory holds.
+// serves both, with the weights as the rows of a tcgen05 product and the tokens as its 16 to 256 columns, so that few tokens
+// waste nothing but columns:
+//   tile     128 rows of W_e (silu: 64 of gate and their 64 of up) x a block of tokens x all of K, in units of 128 bytes of a
+//            row of W. Blocks of more than 128 tokens take two CTAs (a cluster) and 256 rows: each brings its own rows and
+//            half of the tokens, which cuts what an SM has to fetch per product by a third.
+//   stream   W by TMA, x too where its rows are in order; gathered rows by cp.async into the same swizzled form (TMA's own
+//            gather of four rows took 58 cycles each). A ring of as many stages of one or more units as shared memory holds.
 //   math     bf16 x bf16 in fp32 accumulators in tensor memory, two tiles' worth, so that one is stored while the next is
 //            summed. e4m3 becomes bf16 exactly, in registers, and meets x from tensor memory; its row's scale is applied
 //            to the sum, so x is never rounded.
 //   split    The launch does not know the groups. All tiles form one list (expert, rows of W, block of tokens) that every
 //            CTA finds from the offsets. Whole rounds of one tile per CTA are taken as they come; what is left over, up to
-//            two rounds, is cut into equal runs of chunks. A tile cut by a run's end leaves its parts in the workspace and
+//            two rounds, is cut into equal runs of units. A tile cut by a run's end leaves its parts in the workspace and
 //            the last CTA to arrive joins them in the order of K (the same bits whichever it is); no CTA waits for another.
 // Every wait on a barrier is bounded; one that gives up sets code 15 and the CTA stops.
 #include "paia_gemv.h"
@@ -23,84 +25,107 @@ namespace {
 
 constexpr int kExpMaxExperts = 1024;
 constexpr int kExpMaxGrid = 160;                     // the workspace holds two parts per CTA of the largest grid
-constexpr int kExpRows = 128;                        // of W per tile
-constexpr int kExpK = 64;                            // of K per stage
-constexpr int kExpMinRun = 8;                        // chunks per CTA, at least, where a list is cut
-constexpr int kExpMaxStages = 20;
-constexpr int kExpEpilogue = 4, kExpLoaders = 8, kExpConverters = 12;        // first warps of the roles
+constexpr int kExpRows = 128;                        // of W per CTA and tile
+constexpr int kExpUnit = kExpRows * 128;             // bytes of W per unit: 128 of each row
+constexpr int kExpMinRun = 8;                        // units per CTA, at least, where a list is cut
+constexpr int kExpMaxStages = 12;
+constexpr int kExpX = 2, kExpEpilogue = 4, kExpGather = 8, kExpConverters = 12;      // first warps of the roles
+constexpr int kExpLag = 2;                           // stages that a gathering thread has in flight before it looks back
 
-template <int FMT>
+// FMT 0: bf16, 1: e4m3. CG CTAs per tile.
+template <int FMT, int CG>
 struct Exp {
-    static constexpr int kMaxTokens = FMT == 0 ? 256 : 192;      // e4m3 keeps a quarter of tensor memory for converted W
-    static constexpr int kWBytes = kExpRows * kExpK * (FMT == 0 ? 2 : 1);
+    static constexpr int kK = FMT == 0 ? 64 : 128;               // of K per unit
+    static constexpr int kXTiles = kK / 64;                      // of x per unit, 128 bytes a row
     static constexpr int kThreads = FMT == 0 ? 384 : 640;
-    static constexpr int kABase = 384;                           // e4m3: four buffers of converted W, 32 columns each
+    static constexpr int kABufs = CG == 1 ? 4 : 2;               // buffers of converted W, 64 columns each
+    static constexpr int kABase = 512 - 64 * kABufs;
 };
 
 struct alignas(64) ExpertParams {
-    CUtensorMap w;
+    CUtensorMap w, x_map;                            // x_map: where rows are in order
     const __nv_bfloat16* x;
     const int* rows;
     const int* offsets;
     const float* scales;
     __nv_bfloat16* out;
-    unsigned int* counters;                          // one per cut tile: parts that have arrived
+    unsigned int* counters;                          // one per cut tile and CTA of it: parts that have arrived
     float* parts;                                    // [2 grid][tokens][128]
     long long x_row, out_row, scale_expert;
-    int experts, n, k, m, x_rows;                    // n: rows of W_e (silu: of gate)
-    int chunks, row_tiles;                           // of K; tiles along n
-    int tokens, stages;                              // columns per tile, ring
+    int experts, n, m, k, x_rows;                    // n: rows of W_e (silu: of gate)
+    int units, row_tiles;                            // of K; tiles along n
+    int tokens;                                      // columns per tile
+    int stages, sub;                                 // ring, units per stage
 };
 
-// Shared memory: ring of W and of x, then the silu exchange, the barriers and three words per expert.
+// Shared memory: ring of stages (their W, then their x), then the silu exchange, the barriers and three words per expert.
 struct ExpBars {
-    uint64_t w[kExpMaxStages], x[kExpMaxStages], empty[kExpMaxStages], d[2], d_empty[2], a[4], a_empty[4], drained;
+    uint64_t full[kExpMaxStages], empty[kExpMaxStages], peer[kExpMaxStages];
+    uint64_t d[2], d_empty[2], a[4], a_empty[4], drained;
     uint32_t tmem;
     int dead, last;
     int part[32];
 };
 constexpr int kExpExchange = 2 * 4 * 8 * 32 * 4;     // [2][warp][column][lane] floats
-template <int FMT>
-constexpr size_t exp_smem(int tokens, int stages, int experts) {
-    return 1024 + (size_t)stages * (Exp<FMT>::kWBytes + tokens * 128) + kExpExchange + sizeof(ExpBars) + 12 * (size_t)(experts + 1);
-}
+constexpr size_t exp_fixed_smem(int experts) { return 1024 + kExpExchange + sizeof(ExpBars) + 12 * (size_t)(experts + 1); }
 
-// One run of chunks of one tile.
+// A place in a ring.
+struct ExpRing {
+    int slot;
+    uint32_t phase;
+    int stages;
+    bool full;                                       // it has been filled once
+    __device__ __forceinline__ explicit ExpRing(int n) : slot(0), phase(0), stages(n), full(false) {}
+    __device__ __forceinline__ void step() {
+        if (++slot == stages) {
+            slot = 0;
+            phase ^= 1u;
+            full = true;
+        }
+    }
+};
+
+// One run of units of one tile.
 struct ExpPart {
     int tile, e, row_tile, k0, k1;
     int row0, m;                                     // rows of out
 };
 
+// The parts of this CTA (pair), in order.
+template <int CG>
 struct ExpWalk {
     const ExpertParams& p;
-    const int* off;                                  // first row of each expert
+    const int* off;                                  // first row of each expert, then (from experts + 1) its end
     const int* first;                                // first tile of each expert
-    int total, cut, units, workers, at, end, next_whole;
+    int total, cut, work, workers, at, end, next_whole, step;
     __device__ __forceinline__ ExpWalk(const ExpertParams& p_, const int* off_, const int* first_) : p(p_), off(off_), first(first_) {
-        const int g = (int)gridDim.x, c = (int)blockIdx.x;
+        const int g = (int)gridDim.x / CG, c = (int)blockIdx.x / CG;
         total = first[p.experts];
         int rounds = total / g;
         cut = total - rounds * g;
         if (cut && rounds) cut += g;
-        units = cut * p.chunks;
-        workers = min(g, max(1, units / kExpMinRun));
+        work = cut * p.units;
+        workers = min(g, max(1, work / kExpMinRun));
         at = c < workers ? bound(c) : 0;
         end = c < workers ? bound(c + 1) : 0;
         next_whole = cut + c;
+        step = g;
     }
-    __device__ __forceinline__ int bound(int c) const { return (int)((long long)c * units / workers); }
-    __device__ __forceinline__ int owner(int unit) const { return (int)((((long long)unit + 1) * workers - 1) / units); }
+    __device__ __forceinline__ int bound(int c) const { return (int)((long long)c * work / workers); }
+    __device__ __forceinline__ int owner(int unit) const { return (int)((((long long)unit + 1) * workers - 1) / work); }
+    // where owner c's part of a cut tile lies among the parts: its run begins in the tile, or ends there
+    __device__ __forceinline__ int place(int c, int tile) const { return 2 * c + (tile != bound(c) / p.units); }
     __device__ __forceinline__ bool next(ExpPart& s) {
         if (at < end) {
-            s.tile = at / p.chunks;
-            s.k0 = at - s.tile * p.chunks;
-            s.k1 = min(p.chunks, s.k0 + end - at);
+            s.tile = at / p.units;
+            s.k0 = at - s.tile * p.units;
+            s.k1 = min(p.units, s.k0 + end - at);
             at += s.k1 - s.k0;
         } else if (next_whole < total) {
             s.tile = next_whole;
             s.k0 = 0;
-            s.k1 = p.chunks;
-            next_whole += (int)gridDim.x;
+            s.k1 = p.units;
+            next_whole += step;
         } else {
             return false;
         }
@@ -111,29 +136,34 @@ struct ExpWalk {
             else hi = mid;
         }
         s.e = lo;
-        // an expert's blocks of tokens are as equal as multiples of 16 can be, and next to one another in the list: the CTAs
-        // that take them read the same rows of W
+        // an expert's blocks of tokens are as equal as multiples of 16 (32) can be, and next to one another in the list: the
+        // CTAs that take them read the same rows of W
         const int local = s.tile - first[lo], blocks = (first[lo + 1] - first[lo]) / p.row_tiles;
         const int all = off[lo + p.experts + 1] - off[lo];
-        const int per = ((all + blocks - 1) / blocks + 15) & ~15;
+        const int per = round_up((all + blocks - 1) / blocks);
         s.row_tile = local / blocks;
         const int b = local - s.row_tile * blocks;
         s.row0 = off[lo] + b * per;
         s.m = min(per, all - b * per);
         return true;
     }
+    static __device__ __forceinline__ int round_up(int n) { return (n + 16 * CG - 1) & ~(16 * CG - 1); }
 };
 
-// Four e4m3 as bf16, exactly: the exponent's field moves and 2^120 makes up for the bias (subnormals among them).
-__device__ __forceinline__ uint32_t e4m3_half(uint32_t t) {
-    uint32_t r;
-    const uint32_t u = (t >> 4 & 0x07f007f0u) | (t & 0x80008000u);
-    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(u), "r"(0x7b807b80u));
+// Two e4m3 as bf16, exactly: with a byte of its sign above each (prmt), the exponent's field moves by a shift, and 2^120 makes
+// up for the bias (subnormals among them). Eight instructions on the integer pipe for four values took twice as long as the
+// stream from HBM; these are four.
+template <int SEL>
+__device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
+    uint32_t t, r;
+    asm("prmt.b32 %0, %1, 0, %2;" : "=r"(t) : "r"(w), "n"(SEL));
+    asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t * 16u & 0x87f087f0u), "r"(0x7b807b80u));
     return r;
 }
-__device__ __forceinline__ uint32_t e4m3_nan(uint32_t t, uint32_t r) {
-    if ((t & 0x7f00u) == 0x7f00u) r = (r & 0xffff0000u) | 0x7fffu;
-    if ((t & 0x7f000000u) == 0x7f000000u) r = (r & 0xffffu) | 0x7fff0000u;
+// r's halves that came from bytes lo and hi of w, NaN where those are
+__device__ __forceinline__ uint32_t e4m3_nan(uint32_t w, int lo, int hi, uint32_t r) {
+    if ((w >> 8 * lo & 0x7f) == 0x7f) r = (r & 0xffff0000u) | 0x7fffu;
+    if ((w >> 8 * hi & 0x7f) == 0x7f) r = (r & 0xffffu) | 0x7fff0000u;
     return r;
 }
 __device__ __forceinline__ void e4m3x16_bf16(uint4 v, uint32_t r[8]) {
@@ -141,15 +171,15 @@ __device__ __forceinline__ void e4m3x16_bf16(uint4 v, uint32_t r[8]) {
     uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
-        r[2 * i] = e4m3_half(__byte_perm(w[i], 0, 0x1404));
-        r[2 * i + 1] = e4m3_half(__byte_perm(w[i], 0, 0x3424));
+        r[2 * i] = e4m3x2_bf16<0x9180>(w[i]);
+        r[2 * i + 1] = e4m3x2_bf16<0xb3a2>(w[i]);
         odd |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
     }
     if (odd & 0x80808080u) {                                     // a NaN among them
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            r[2 * i] = e4m3_nan(__byte_perm(w[i], 0, 0x1404), r[2 * i]);
-            r[2 * i + 1] = e4m3_nan(__byte_perm(w[i], 0, 0x3424), r[2 * i + 1]);
+            r[2 * i] = e4m3_nan(w[i], 0, 1, r[2 * i]);
+            r[2 * i + 1] = e4m3_nan(w[i], 2, 3, r[2 * i + 1]);
         }
     }
 }
@@ -214,28 +244,32 @@ __device__ void list_tiles(const ExpertParams& p, int* off, int* first, int* par
     __syncthreads();
 }
 
-template <int FMT, bool SILU>
-__global__ void __launch_bounds__(Exp<FMT>::kThreads, 1) expert_kernel(const __grid_constant__ ExpertParams p) {
+template <int FMT, bool SILU, int CG>
+__global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const __grid_constant__ ExpertParams p) {
+    using T = Exp<FMT, CG>;
     extern __shared__ uint8_t raw[];
-    uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(raw) + 1023) & ~(uintptr_t)1023);
-    constexpr int WB = Exp<FMT>::kWBytes;
-    const int ST = p.stages, xb = p.tokens * 128;
-    const uint32_t wring = sptr(smem), xring = wring + ST * WB;
-    float* exchange = reinterpret_cast<float*>(smem + (size_t)ST * (WB + xb));
+    // (the same offset in both CTAs of a cluster)
+    const uint32_t ring = (sptr(raw) + 1023) & ~1023u;
+    uint8_t* smem = raw + (ring - sptr(raw));
+    constexpr int XT = T::kXTiles, K = T::kK;
+    const int sub = p.sub, xb = p.tokens / CG * 128;             // bytes of one tile of x
+    const int stage = sub * (kExpUnit + XT * xb);
+    float* exchange = reinterpret_cast<float*>(smem + (size_t)p.stages * stage);
     ExpBars& bars = *reinterpret_cast<ExpBars*>(reinterpret_cast<uint8_t*>(exchange) + kExpExchange);
     int* first = reinterpret_cast<int*>(&bars + 1);
     int* off = first + p.experts + 1;
     volatile int* dead = &bars.dead;
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+    const uint32_t rank = CG == 1 ? 0 : cluster_rank();
     if (threadIdx.x == 0) {
-        for (int s = 0; s < ST; ++s) {
-            bar_init(sptr(&bars.w[s]), 1);
-            bar_init(sptr(&bars.x[s]), 128);
+        for (int s = 0; s < p.stages; ++s) {
+            bar_init(sptr(&bars.full[s]), 1 + (p.rows ? 128 : 1));
             bar_init(sptr(&bars.empty[s]), 1);
+            bar_init(sptr(&bars.peer[s]), 1);
         }
         for (int i = 0; i < 2; ++i) {
             bar_init(sptr(&bars.d[i]), 1);
-            bar_init(sptr(&bars.d_empty[i]), 128);
+            bar_init(sptr(&bars.d_empty[i]), 4 * CG);
         }
         for (int i = 0; i < 4; ++i) {
             bar_init(sptr(&bars.a[i]), 128);
@@ -245,110 +279,199 @@ __global__ void __launch_bounds__(Exp<FMT>::kThreads, 1) expert_kernel(const __g
         bars.dead = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
     }
-    if (warp == 1) tmem_alloc(sptr(&bars.tmem), 512);
+    if (warp == 1) tmem_alloc<CG>(sptr(&bars.tmem), 512);
+    __syncwarp();
     tc5_fence_before();
-    __syncthreads();
+    if (CG == 1) __syncthreads();
+    else cluster_barrier();
     tc5_fence_after();
     pdl_wait_and_trigger();
     list_tiles(p, off, first, bars.part);
     const uint32_t tmem = bars.tmem;
-    ExpWalk walk(p, off, first);
+    ExpWalk<CG> walk(p, off, first);
     ExpPart s;
-    int it = 0;                                                  // stages so far, across parts
-    const auto slot = [&](int i) { return i % ST; };
-    const auto phase = [&](int i) { return (uint32_t)(i / ST & 1); };
+    ExpRing at(p.stages);
+    const uint32_t bar_full = sptr(bars.full), bar_empty = sptr(bars.empty), bar_peer = sptr(bars.peer), bar_a = sptr(bars.a),
+                   bar_a_empty = sptr(bars.a_empty);
+    bool ok = true;
+    const auto wait = [&](uint32_t bar, uint32_t phase) { return ok = bar_wait(bar, phase, dead); };
     if (warp == 0) {
         // ---- W
-        if (lane == 0) {
-            bool ok = true;
-            while (ok && walk.next(s))
-                for (int c = s.k0; c < s.k1; ++c, ++it) {
-                    const int b = slot(it);
-                    if (it >= ST && !(ok = bar_wait(sptr(&bars.empty[b]), phase(it) ^ 1u, dead))) break;
-                    bar_expect(sptr(&bars.w[b]), WB);
-                    if (SILU) tma_4d(wring + b * WB, &p.w, c * kExpK, s.row_tile * 64, 0, s.e, sptr(&bars.w[b]));
-                    else tma_3d(wring + b * WB, &p.w, c * kExpK, s.row_tile * kExpRows, s.e, sptr(&bars.w[b]));
+        if (elect_one()) {
+            while (ok && walk.next(s)) {
+                const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
+                for (int k = s.k0; k < s.k1; k += sub, at.step()) {
+                    if (at.full && !wait(bar_empty + 8 * at.slot, at.phase ^ 1u)) break;
+                    const int n = min(sub, s.k1 - k);
+                    const uint32_t bar = bar_full + 8 * at.slot, to = ring + at.slot * stage;
+                    bar_expect(bar, n * kExpUnit);
+                    for (int u = 0; u < n; ++u) {
+                        if (SILU) tma_4d(to + u * kExpUnit, &p.w, (k + u) * K, y, 0, s.e, bar);
+                        else tma_3d(to + u * kExpUnit, &p.w, (k + u) * K, y, s.e, bar);
+                    }
                 }
-            if (!ok) {                                           // its copies in flight
+            }
+            if (!ok) {                                           // copies in flight: one phase of every stage
                 const uint64_t t0 = wait_clock_ns();
-                for (int i = max(0, it - ST); i < it; ++i)
-                    while (!bar_test(sptr(&bars.w[slot(i)]), phase(i)) && wait_clock_ns() - t0 < 1000000000ull) {}
+                for (int i = 0; i < p.stages; ++i, at.step())
+                    while (!bar_test(bar_full + 8 * at.slot, at.phase ^ 1u) && wait_clock_ns() - t0 < 1000000000ull) {}
             }
         }
-    } else if (warp == 1) {
-        // ---- products
-        if (lane == 0) {
-            bool ok = true;
-            int tile = 0;
-            for (; ok && walk.next(s); ++tile) {
-                const int buf = tile & 1;
-                if (tile >= 2 && !(ok = bar_wait(sptr(&bars.d_empty[buf]), (tile / 2 & 1) ^ 1u, dead))) break;
-                tc5_fence_after();
-                const uint32_t d = tmem + buf * p.tokens;
-                const uint32_t shape = tc5_bf16_shape((s.m + 15) & ~15);
-                for (int c = s.k0; c < s.k1; ++c, ++it) {
-                    const int b = slot(it);
-                    if (!(ok = bar_wait(sptr(&bars.x[b]), phase(it), dead))) break;
-                    const uint64_t xo = tc5_operand(xring + b * xb);
-                    if (FMT == 0) {
-                        if (!(ok = bar_wait(sptr(&bars.w[b]), phase(it), dead))) break;
-                        async_proxy_fence();
-                        tc5_fence_after();
-                        const uint64_t wo = tc5_operand(wring + b * WB);
-#pragma unroll
-                        for (int i = 0; i < kExpK / 16; ++i) tc5_mma(d, wo + 2 * i, xo + 2 * i, shape, c > s.k0 || i > 0);
-                    } else {
-                        const int ab = it & 3;
-                        if (!(ok = bar_wait(sptr(&bars.a[ab]), it / 4 & 1, dead))) break;
-                        async_proxy_fence();
-                        tc5_fence_after();
-#pragma unroll
-                        for (int i = 0; i < kExpK / 16; ++i)
-                            tc5_mma_t(d, tmem + Exp<FMT>::kABase + 32 * ab + 8 * i, xo + 2 * i, shape, c > s.k0 || i > 0);
-                        tc5_commit(sptr(&bars.a_empty[ab]));
-                    }
-                    tc5_commit(sptr(&bars.empty[b]));
+    } else if (warp == kExpX) {
+        // ---- x, rows in order
+        if (!p.rows && elect_one()) {
+            while (ok && walk.next(s)) {
+                const int row = s.row0 + (int)rank * (walk.round_up(s.m) / CG);
+                for (int k = s.k0; k < s.k1; k += sub, at.step()) {
+                    if (at.full && !wait(bar_empty + 8 * at.slot, at.phase ^ 1u)) break;
+                    const int n = XT * min(sub, s.k1 - k);
+                    const uint32_t bar = bar_full + 8 * at.slot, to = ring + at.slot * stage + sub * kExpUnit;
+                    bar_expect(bar, n * xb);
+                    for (int u = 0; u < n; ++u) tma_2d(to + u * xb, &p.x_map, k * K + 64 * u, row, bar);
                 }
-                if (ok) tc5_commit(sptr(&bars.d[buf]));
             }
-            if (!ok) {                                           // its products in flight
-                tc5_commit(sptr(&bars.drained));
+        }
+    } else if (warp >= kExpGather && warp < kExpConverters && p.rows) {
+        // ---- x, gathered: a thread has 16-byte piece `piece` of rows r0 + 16 i
+        const int t = threadIdx.x - kExpGather * 32, r0 = t >> 3, piece = t & 7;
+        const uint32_t to0 = ring + sub * kExpUnit + r0 * 128 + ((piece ^ (r0 & 7)) << 4);
+        int behind = 0;                                          // stages issued and not yet passed on
+        ExpRing back(p.stages);
+        while (ok && walk.next(s)) {
+            const int half = CG == 1 ? s.m : walk.round_up(s.m) / 2, skip = (int)rank * half, mine = min(half, s.m - skip);
+            const __nv_bfloat16* src[8];                         // nullptr: no such row, zeros
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int r = r0 + 16 * i;
+                src[i] = nullptr;
+                if (r < mine) {
+                    const int from = p.rows[s.row0 + skip + r];
+                    if (from >= 0 && from < p.x_rows) src[i] = p.x + from * p.x_row + piece * 8;
+                    else serve_error(kErrRouting);
+                }
+            }
+            for (int k = s.k0; k < s.k1; k += sub) {
+                if (at.full && !wait(bar_empty + 8 * at.slot, at.phase ^ 1u)) break;
+                const int n = XT * min(sub, s.k1 - k);
+                for (int u = 0; u < n; ++u) {
+                    const uint32_t to = to0 + at.slot * stage + u * xb;
+                    const int from = k * K + 64 * u;
+                    const bool in = from + piece * 8 < p.k;      // zeros behind the end of K
+#pragma unroll
+                    for (int i = 0; i < 8; ++i) {
+                        if (16 * i >= mine) break;
+                        const bool got = in && src[i];
+                        if (r0 + 16 * i < mine) cp16(to + i * 2048, got ? src[i] + from : p.x, got ? 16 : 0);
+                    }
+                }
+                cp_commit();
+                at.step();
+                if (++behind > kExpLag) {
+                    cp_wait<kExpLag>();
+                    async_proxy_fence();
+                    bar_arrive(bar_full + 8 * back.slot);
+                    back.step();
+                    --behind;
+                }
+            }
+        }
+        cp_wait<0>();
+        async_proxy_fence();
+        for (; behind > 0; --behind, back.step()) bar_arrive(bar_full + 8 * back.slot);
+    } else if (warp == 1) {
+        // ---- products, where a stage (e4m3: a buffer of converted W, and with it the stage) is there; the second CTA of a pair
+        // tells the first
+        if (elect_one()) {
+            const bool leader = rank == 0;
+            const int tokens = p.tokens;
+            int ab = 0;                                          // e4m3: buffer of converted W, its phase
+            uint32_t ap = 0;
+            for (int tile = 0; ok && walk.next(s); ++tile) {
+                const int buf = tile & 1;
+                if (leader && tile >= 2 && !wait(sptr(&bars.d_empty[buf]), (tile / 2 & 1) ^ 1u)) break;
+                tc5_fence_after();
+                const uint32_t d = tmem + buf * tokens;
+                const uint32_t shape = tc5_bf16_shape<CG>(walk.round_up(s.m));
+                uint32_t add = 0;
+                for (int k = s.k0; ok && k < s.k1; k += sub) {
+                    const int n = min(sub, s.k1 - k);
+                    const uint32_t w = ring + at.slot * stage;
+                    uint64_t wo = tc5_operand(w), xo = tc5_operand(w + sub * kExpUnit);
+                    for (int u = 0; u < n; ++u) {
+                        if (FMT == 1 || u == 0) {
+                            const int i = FMT == 0 ? at.slot : ab;
+                            const uint32_t phase = FMT == 0 ? at.phase : ap;
+                            if (!wait((FMT == 0 ? bar_full : bar_a) + 8 * i, phase)) break;
+                            if (CG == 2 && leader && !wait(bar_peer + 8 * i, phase)) break;
+                            if (CG == 2 && !leader) bar_arrive_at(bar_peer + 8 * i, 0);
+                            tc5_fence_after();
+                        }
+                        if (CG == 1 || leader) {
+#pragma unroll
+                            for (int j = 0; j < XT; ++j, xo += xb >> 4) {
+#pragma unroll
+                                for (int q = 0; q < 4; ++q) {
+                                    if (FMT == 0) tc5_mma<CG>(d, wo + 2 * q, xo + 2 * q, shape, add);
+                                    else tc5_mma_t<CG>(d, tmem + T::kABase + 64 * ab + 32 * j + 8 * q, xo + 2 * q, shape, add);
+                                    add = 1;
+                                }
+                            }
+                            wo += kExpUnit >> 4;
+                            if (FMT == 1) tc5_commit<CG>(bar_a_empty + 8 * ab);
+                        }
+                        if (FMT == 1 && ++ab == T::kABufs) {
+                            ab = 0;
+                            ap ^= 1u;
+                        }
+                    }
+                    if (ok && leader) tc5_commit<CG>(bar_empty + 8 * at.slot);
+                    at.step();
+                }
+                if (ok && leader) tc5_commit<CG>(sptr(&bars.d[buf]));
+            }
+            if (!ok && leader) {                                 // products in flight
+                tc5_commit<CG>(sptr(&bars.drained));
                 const uint64_t t0 = wait_clock_ns();
                 while (!bar_test(sptr(&bars.drained), 0) && wait_clock_ns() - t0 < 1000000000ull) {}
             }
         }
-    } else if (warp >= kExpEpilogue && warp < kExpLoaders) {
+    } else if (warp >= kExpEpilogue && warp < kExpGather) {
         // ---- results
         const int q = warp - kExpEpilogue, row = q * 32 + lane;
         int step = 0;                                            // exchanges so far
-        bool ok = true;
         for (int tile = 0; ok && walk.next(s); ++tile) {
             const int buf = tile & 1;
             if (!(ok = all_of(__all_sync(0xffffffffu, bar_wait(sptr(&bars.d[buf]), tile / 2 & 1, dead))))) break;
             tc5_fence_after();
             const uint32_t d = tmem + buf * p.tokens + ((uint32_t)(q * 32) << 16);
-            const bool whole = s.k0 == 0 && s.k1 == p.chunks;
+            const auto release = [&]() {                         // the accumulators may be overwritten
+                tc5_fence_before();
+                __syncwarp();
+                if (lane == 0) {
+                    if (CG == 1) bar_arrive(sptr(&bars.d_empty[buf]));
+                    else bar_arrive_at(sptr(&bars.d_empty[buf]), 0);
+                }
+            };
+            const bool whole = s.k0 == 0 && s.k1 == p.units;
             int c0 = 0, c1 = 0;
             bool mine = true;
             if (!whole) {
-                c0 = walk.owner(s.tile * p.chunks);
-                c1 = walk.owner((s.tile + 1) * p.chunks - 1);
-                const int my = 2 * blockIdx.x + (s.tile != walk.bound(blockIdx.x) / p.chunks);
-                float* to = p.parts + ((size_t)my * p.tokens) * kExpRows + row;
+                c0 = walk.owner(s.tile * p.units);
+                c1 = walk.owner((s.tile + 1) * p.units - 1);
+                float* to = p.parts + ((size_t)(walk.place(blockIdx.x / CG, s.tile) * CG + rank) * p.tokens) * kExpRows + row;
                 for (int c = 0; c < s.m; c += 16) {
                     float v[16];
                     tmem_load16(d + c, v);
 #pragma unroll
                     for (int i = 0; i < 16; ++i) to[(c + i) * kExpRows] = v[i];
                 }
-                tc5_fence_before();
-                bar_arrive(sptr(&bars.d_empty[buf]));
+                release();
                 __threadfence();
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (row == 0) {
-                    const unsigned n = atomicAdd(&p.counters[s.tile], 1u);
-                    const bool last = n == (unsigned)(c1 - c0);
-                    if (last) p.counters[s.tile] = 0;
+                    unsigned int* counter = p.counters + s.tile * CG + rank;
+                    const bool last = atomicAdd(counter, 1u) == (unsigned)(c1 - c0);
+                    if (last) *counter = 0;
                     bars.last = last;
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
@@ -357,7 +480,8 @@ __global__ void __launch_bounds__(Exp<FMT>::kThreads, 1) expert_kernel(const __g
                 asm volatile("bar.sync 1, 128;" ::: "memory");   // bars.last has been read
             }
             if (mine) {
-                const int n = SILU ? s.row_tile * 64 + (q & 1) * 32 + lane : s.row_tile * kExpRows + row;
+                const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
+                const int n = SILU ? y + (q & 1) * 32 + lane : y + row;
                 float scale = 1.f;
                 if (FMT == 1 && n < p.n) scale = p.scales[s.e * p.scale_expert + n + (SILU && q >= 2 ? p.n : 0)];
                 for (int c = 0; c < s.m; c += 16) {
@@ -368,8 +492,7 @@ __global__ void __launch_bounds__(Exp<FMT>::kThreads, 1) expert_kernel(const __g
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
                         for (int o = c0; o <= c1; ++o) {
-                            const int at = 2 * o + (s.tile != walk.bound(o) / p.chunks);
-                            const float* from = p.parts + ((size_t)at * p.tokens + c) * kExpRows + row;
+                            const float* from = p.parts + ((size_t)(walk.place(o, s.tile) * CG + rank) * p.tokens + c) * kExpRows + row;
 #pragma unroll
                             for (int i = 0; i < 16; ++i) v[i] += __ldcg(from + i * kExpRows);
                         }
@@ -398,120 +521,119 @@ __global__ void __launch_bounds__(Exp<FMT>::kThreads, 1) expert_kernel(const __g
                     }
                 }
             }
-            if (whole) {
-                tc5_fence_before();
-                bar_arrive(sptr(&bars.d_empty[buf]));
-            }
+            if (whole) release();
         }
-    } else if (warp >= kExpLoaders && warp < kExpLoaders + 4) {
-        // ---- x: a thread has 16-byte piece `piece` of rows r0 + 16 i
-        const int t = threadIdx.x - kExpLoaders * 32, r0 = t >> 3, piece = t & 7;
-        const uint32_t dst0 = xring + r0 * 128 + ((piece ^ (r0 & 7)) << 4);
-        bool ok = true;
-        while (ok && walk.next(s)) {
-            int src[Exp<FMT>::kMaxTokens / 16];
+    } else if (FMT == 1 && warp >= kExpConverters) {
+        // ---- e4m3 -> bf16: two groups of four warps take the units in turn, a row per thread
+        const int group = (warp - kExpConverters) >> 2, row = (warp & 3) * 32 + lane;
+        const uint32_t key = (row & 7) << 4;
+        int turn = 0, ab = 0;
+        uint32_t ap = 1;                                         // the first round of buffers is free
+        const auto wait_all = [&](uint32_t bar, uint32_t phase) { return ok = __all_sync(0xffffffffu, bar_wait(bar, phase, dead)); };
+        while (ok && walk.next(s))
+            for (int k = s.k0; ok && k < s.k1; k += sub, at.step()) {
+                const int n = min(sub, s.k1 - k);
+                for (int u = 0; u < n; ++u, turn ^= 1) {
+                    if (turn == group) {
+                        if (!wait_all(bar_full + 8 * at.slot, at.phase)) break;
+                        const uint32_t from = ring + at.slot * stage + u * kExpUnit + row * 128;
+                        const uint32_t to = tmem + T::kABase + 64 * ab + ((uint32_t)((warp & 3) * 32) << 16);
+                        uint4 v[8];
 #pragma unroll
-            for (int i = 0; i < Exp<FMT>::kMaxTokens / 16; ++i) {
-                const int r = r0 + 16 * i;
-                src[i] = -1;
-                if (r < s.m) {
-                    src[i] = p.rows ? p.rows[s.row0 + r] : s.row0 + r;
-                    if (src[i] < 0 || src[i] >= p.x_rows) {
-                        serve_error(kErrRouting);
-                        src[i] = -1;
+                        for (int i = 0; i < 8; ++i)
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
+                                         : "r"(from + ((i << 4) ^ key)));
+                        uint32_t r[32];
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e4m3x16_bf16(v[i], r + 8 * i);
+                        if (!wait_all(bar_a_empty + 8 * ab, ap)) break;
+                        tc5_fence_after();
+                        tmem_store32(to, r);
+#pragma unroll
+                        for (int i = 0; i < 4; ++i) e4m3x16_bf16(v[4 + i], r + 8 * i);
+                        tmem_store32(to + 32, r);
+                        tmem_store_wait();
+                        tc5_fence_before();
+                        bar_arrive(bar_a + 8 * ab);
+                    }
+                    if (++ab == T::kABufs) {
+                        ab = 0;
+                        ap ^= 1u;
                     }
                 }
-            }
-            for (int c = s.k0; c < s.k1; ++c, ++it) {
-                const int b = slot(it);
-                if (it >= ST && !(ok = bar_wait(sptr(&bars.empty[b]), phase(it) ^ 1u, dead))) break;
-                const int k = c * kExpK + piece * 8;
-                const bool in = k < p.k;
-#pragma unroll
-                for (int i = 0; i < Exp<FMT>::kMaxTokens / 16; ++i) {
-                    if (16 * i >= s.m) break;
-                    const bool got = in && src[i] >= 0;
-                    cp16(dst0 + b * xb + i * 2048, p.x + (got ? src[i] * p.x_row + k : 0), got ? 16 : 0);
-                }
-                cp_arrive(sptr(&bars.x[b]));
-            }
-        }
-        cp_commit();
-        cp_wait<0>();
-    } else if (FMT == 1 && warp >= kExpConverters) {
-        // ---- e4m3 -> bf16: two groups of four warps take the stages in turn, a row per thread
-        const int group = (warp - kExpConverters) >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t src0 = wring + row * 64, key = (row >> 1 & 3) << 4;
-        bool ok = true;
-        while (ok && walk.next(s))
-            for (int c = s.k0; c < s.k1; ++c, ++it) {
-                if ((it & 1) != group) continue;
-                const int b = slot(it), ab = it & 3;
-                if (!(ok = __all_sync(0xffffffffu, bar_wait(sptr(&bars.w[b]), phase(it), dead)))) break;
-                uint32_t r[32];
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    uint4 v;
-                    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];"
-                                 : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(src0 + b * WB + ((i << 4) ^ key)) : "memory");
-                    e4m3x16_bf16(v, r + 8 * i);
-                }
-                if (it >= 4 && !(ok = __all_sync(0xffffffffu, bar_wait(sptr(&bars.a_empty[ab]), (it / 4 & 1) ^ 1u, dead)))) break;
-                tc5_fence_after();
-                tmem_store32(tmem + Exp<FMT>::kABase + 32 * ab + ((uint32_t)((warp & 3) * 32) << 16), r);
-                tc5_fence_before();
-                bar_arrive(sptr(&bars.a[ab]));
             }
     }
     __syncwarp();
     tc5_fence_before();
-    __syncthreads();
+    if (CG == 1) __syncthreads();
+    else cluster_barrier();                                      // (the other CTA's arrivals here are done)
     if (warp == 1) {
         tc5_fence_after();
-        tmem_free(tmem, 512);
+        tmem_free<CG>(tmem, 512);
     }
 }
 
-// The map of W [experts][rows][K]: 64 of K x 128 rows (silu: 64 of gate and 64 of up) per copy; rows and K behind the end
-// arrive as zeros.
-bool map_weights(ExpertParams& p, int fmt, bool silu, const paia_gemv_expert_args* a) {
+// The maps. W [experts][rows][K]: 128 bytes of 128 rows (silu: of 64 of gate and 64 of up) per copy; rows and K behind the end
+// arrive as zeros. x [rows][K]: 64 values of the rows that a CTA brings of a block.
+bool map_operands(ExpertParams& p, int fmt, bool silu, int cg, const paia_gemv_expert_args* a) {
     const EncodeTiledFn fn = encode_tiled();
     if (!fn) return false;
     const cuuint64_t es = fmt == 0 ? 2 : 1, row = (cuuint64_t)a->w_row * es;
     const cuuint64_t expert = a->experts > 1 ? (cuuint64_t)a->w_expert * es : row;
     const cuuint32_t one[4] = {1, 1, 1, 1};
-    const CUtensorMapDataType type = fmt == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8;
-    const CUtensorMapSwizzle swizzle = fmt == 0 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_64B;
     const cuuint64_t dims[4] = {(cuuint64_t)a->K, (cuuint64_t)p.n, silu ? 2u : (cuuint64_t)a->experts, (cuuint64_t)a->experts};
     const cuuint64_t strides[3] = {row, silu ? row * (cuuint64_t)p.n : expert, expert};
-    const cuuint32_t box[4] = {kExpK, silu ? 64u : 128u, silu ? 2u : 1u, 1};
-    return fn(&p.w, type, silu ? 4 : 3, const_cast<void*>(a->w), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, swizzle,
-              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint32_t box[4] = {fmt == 0 ? 64u : 128u, silu ? 64u : 128u, silu ? 2u : 1u, 1};
+    if (fn(&p.w, fmt == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, silu ? 4 : 3,
+           const_cast<void*>(a->w), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+           CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
+        return false;
+    if (p.rows) return true;
+    const cuuint64_t x_dims[2] = {(cuuint64_t)a->K, (cuuint64_t)a->x_rows};
+    const cuuint64_t x_stride[1] = {a->x_rows > 1 ? (cuuint64_t)a->x_row * 2 : ((cuuint64_t)a->K * 2 + 15) / 16 * 16};
+    const cuuint32_t x_box[2] = {64, (cuuint32_t)(p.tokens / cg)};
+    return fn(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a->x), x_dims, x_stride, x_box, one,
+              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+}
+
+template <int FMT, bool SILU, int CG>
+int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t st) {
+    using T = Exp<FMT, CG>;
+    const int unit = kExpUnit + T::kXTiles * (p.tokens / CG * 128);
+    const size_t most = max_dyn_smem(), fixed = exp_fixed_smem(a->experts);
+    if (most < fixed) return -2;
+    const int depth = (int)((most - fixed) / unit);              // in units
+    // Few tokens: larger stages, for fewer waits.
+    p.sub = depth >= 10 ? 2 : 1;
+    p.stages = depth / p.sub < kExpMaxStages ? depth / p.sub : kExpMaxStages;
+    if (p.stages < kExpLag + 2) return -2;
+    const size_t smem = fixed + (size_t)p.stages * p.sub * unit;
+    p.units = (a->K + T::kK - 1) / T::kK;
+    const int rows = CG * (SILU ? 64 : kExpRows);
+    p.row_tiles = (p.n + rows - 1) / rows;
+    if (((long long)a->M / p.tokens + a->experts) * p.row_tiles > 0x7fff0000ll) return -2;
+    if (!map_operands(p, FMT, SILU, CG, a)) return -2;
+    static std::atomic<unsigned long long> done{0};
+    const int rc = serve_allow_smem((const void*)expert_kernel<FMT, SILU, CG>, most, done);
+    if (rc) return rc;
+    const int grid = (sm_count() < kExpMaxGrid ? sm_count() : kExpMaxGrid) / CG * CG;
+    return serve_launch(expert_kernel<FMT, SILU, CG>, p, dim3((unsigned)grid), T::kThreads, smem > kSmemAlone ? smem : kSmemAlone, st, CG);
 }
 
 template <int FMT, bool SILU>
-int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t st) {
-    if (!map_weights(p, FMT, SILU, a)) return -2;
+int pick_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t st) {
     // Blocks of twice the tokens that an expert has on average: smaller ones read W more often, larger ones leave the ring
     // fewer stages.
     const long long want = 2ll * ((a->M + a->experts - 1) / a->experts);
     p.tokens = 16;
-    while (p.tokens < Exp<FMT>::kMaxTokens && p.tokens < want && p.tokens < a->M) p.tokens *= 2;
-    if (p.tokens > Exp<FMT>::kMaxTokens) p.tokens = Exp<FMT>::kMaxTokens;
-    const size_t most = max_dyn_smem();
-    for (p.stages = kExpMaxStages; p.stages > 3 && exp_smem<FMT>(p.tokens, p.stages, a->experts) > most;) --p.stages;
-    const size_t smem = exp_smem<FMT>(p.tokens, p.stages, a->experts);
-    if (smem > most) return -2;
-    p.row_tiles = (p.n + (SILU ? 64 : kExpRows) - 1) / (SILU ? 64 : kExpRows);
-    if (((long long)a->M / p.tokens + a->experts) * p.row_tiles > 0x7fff0000ll) return -2;
-    static std::atomic<unsigned long long> done{0};
-    const int rc = serve_allow_smem((const void*)expert_kernel<FMT, SILU>, most, done);
-    if (rc) return rc;
-    const int grid = sm_count() < kExpMaxGrid ? sm_count() : kExpMaxGrid;
-    return serve_launch(expert_kernel<FMT, SILU>, p, dim3((unsigned)grid), Exp<FMT>::kThreads, smem > kSmemAlone ? smem : kSmemAlone, st);
+    while (p.tokens < 256 && p.tokens < want && p.tokens < a->M) p.tokens *= 2;
+    if (p.tokens <= 128) return launch_experts<FMT, SILU, 1>(p, a, st);
+    p.tokens = FMT == 0 ? 256 : 192;                 // (e4m3 keeps columns for converted W)
+    return launch_experts<FMT, SILU, 2>(p, a, st);
 }
 
-constexpr size_t kExpCounters = 2 * kExpMaxGrid * 4;
+constexpr size_t kExpCounters = 2 * kExpMaxGrid * 4;                 // (a cut list has fewer than two tiles per CTA or pair)
 
 }  // namespace
 
@@ -522,7 +644,7 @@ int experts_device_error(int clear) { return serve_error_word(clear); }
 using namespace pb2;
 
 extern "C" size_t paia_gemv_expert_workspace(void) {
-    return kExpCounters + (size_t)2 * kExpMaxGrid * kExpRows * Exp<0>::kMaxTokens * 4;
+    return kExpCounters + (size_t)2 * kExpMaxGrid * kExpRows * 256 * 4;
 }
 
 extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* stream) {
@@ -540,23 +662,22 @@ extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* str
     if ((a->M > 1 && a->out_row == 0) || a->out == a->x) return -2;
     if (a->M == 0) return 0;
     ExpertParams p{};
-    p.x = static_cast<const __nv_bfloat16*>(a->x);
     p.rows = a->rows;
     p.offsets = a->offsets;
     p.scales = a->scales;
     p.out = static_cast<__nv_bfloat16*>(a->out);
     p.counters = static_cast<unsigned int*>(a->workspace);
     p.parts = reinterpret_cast<float*>(static_cast<uint8_t*>(a->workspace) + kExpCounters);
+    p.x = static_cast<const __nv_bfloat16*>(a->x);
     p.x_row = a->x_row;
+    p.k = a->K;
     p.out_row = a->out_row;
     p.scale_expert = a->scale_expert;
     p.experts = a->experts;
     p.n = a->silu ? a->N / 2 : a->N;
-    p.k = a->K;
     p.m = a->M;
     p.x_rows = a->x_rows;
-    p.chunks = (a->K + kExpK - 1) / kExpK;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->kind == 0) return a->silu ? launch_experts<0, true>(p, a, st) : launch_experts<0, false>(p, a, st);
-    return a->silu ? launch_experts<1, true>(p, a, st) : launch_experts<1, false>(p, a, st);
+    if (a->kind == 0) return a->silu ? pick_experts<0, true>(p, a, st) : pick_experts<0, false>(p, a, st);
+    return a->silu ? pick_experts<1, true>(p, a, st) : pick_experts<1, false>(p, a, st);
 }

@@ -11,6 +11,12 @@ __device__ __forceinline__ uint64_t wait_clock_ns() {
     return t;
 }
 
+// One thread of the warp, the same at every call.
+__device__ __forceinline__ bool elect_one() {
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p;\n\telect.sync _|p, 0xffffffff;\n\tselp.u32 %0, 1, 0, p;\n\t}" : "=r"(r));
+    return r != 0;
+}
 __device__ __forceinline__ void bar_init(uint32_t bar, int count) {
     asm volatile("mbarrier.init.shared.b64 [%0], %1;" :: "r"(bar), "r"(count) : "memory");
 }
@@ -26,30 +32,45 @@ __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
-// Waits for phase `parity` for at most 2 s, or until *dead is set; then sets *dead and the error word and returns false.
+// An arrival on the barrier at `bar` of the cluster's CTA `cta`. It passes on that operands are in this CTA's shared or tensor
+// memory, where this SM's own tensor cores read them; it does not publish this thread's writes to the other CTA (an arrival
+// that does takes 1600 cycles).
+__device__ __forceinline__ void bar_arrive_at(uint32_t bar, uint32_t cta) {
+    asm volatile("{\n\t.reg .b32 a;\n\tmapa.shared::cluster.u32 a, %0, %1;\n\tmbarrier.arrive.shared::cluster.b64 _, [a];\n\t}"
+                 :: "r"(bar), "r"(cta) : "memory");
+}
+__device__ __forceinline__ uint32_t cluster_rank() {
+    uint32_t r;
+    asm volatile("mov.u32 %0, %%cluster_ctarank;" : "=r"(r));
+    return r;
+}
+__device__ __forceinline__ void cluster_barrier() {
+    asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
+}
+// Waits for phase `parity` for at most 2 s or so, or until *dead is set; then sets *dead and the error word and returns false.
+// (The clock is looked at now and then: reading the timer takes longer than most waits.)
 __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile int* dead) {
-    if (bar_test(bar, parity)) return true;
-    const uint64_t t0 = wait_clock_ns();
-    for (int i = 0;; ++i) {
+    uint64_t t0 = 0;
+    for (int i = 1;; ++i) {
         if (bar_test(bar, parity)) return true;
-        if ((i & 63) == 63) {
-            if (*dead) return false;
-            if (wait_clock_ns() - t0 > 2000000000ull) {
-                *dead = 1;
-                serve_error(kErrServeWait);
-                return false;
-            }
+        if (i & 255) continue;
+        if (*dead) return false;
+        if (!t0) t0 = wait_clock_ns();
+        if (wait_clock_ns() - t0 > 2000000000ull) {
+            *dead = 1;
+            serve_error(kErrServeWait);
+            return false;
         }
     }
 }
 
-// cp.async pieces of this thread so far: one arrival on `bar` (counted in its arrivals) once they have landed.
-__device__ __forceinline__ void cp_arrive(uint32_t bar) {
-    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" :: "r"(bar) : "memory");
-}
-// What other threads wrote to shared memory, and this thread has seen through a barrier, is seen by the tensor cores.
+// What this thread has written to shared memory is seen by the tensor cores behind its next arrival on a barrier.
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
+__device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
+    asm volatile("cp.async.bulk.tensor.2d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3}], [%4];"
+                 :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(bar) : "memory");
+}
 __device__ __forceinline__ void tma_3d(uint32_t dst, const void* map, int x, int y, int z, uint32_t bar) {
     asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];"
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(bar) : "memory");
@@ -59,19 +80,34 @@ __device__ __forceinline__ void tma_4d(uint32_t dst, const void* map, int x, int
                  :: "r"(dst), "l"(reinterpret_cast<uint64_t>(map)), "r"(x), "r"(y), "r"(z), "r"(w), "r"(bar) : "memory");
 }
 
-// Tensor memory: 512 columns of 128 lanes x 32 bits per SM. A whole warp allocates and frees.
+// Tensor memory: 512 columns of 128 lanes x 32 bits per SM. A whole warp allocates and frees. CG: how many CTAs work on one
+// product, 1, or 2 of a cluster (each with its half of the rows of A and D, and half of the columns of B).
+template <int CG>
 __device__ __forceinline__ void tmem_alloc(uint32_t slot, int columns) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(slot), "r"(columns) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    if (CG == 1) {
+        asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(slot), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;");
+    } else {
+        asm volatile("tcgen05.alloc.cta_group::2.sync.aligned.shared::cta.b32 [%0], %1;" :: "r"(slot), "r"(columns) : "memory");
+        asm volatile("tcgen05.relinquish_alloc_permit.cta_group::2.sync.aligned;");
+    }
 }
+template <int CG>
 __device__ __forceinline__ void tmem_free(uint32_t addr, int columns) {
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
+    if (CG == 1) asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
+    else asm volatile("tcgen05.dealloc.cta_group::2.sync.aligned.b32 %0, %1;" :: "r"(addr), "r"(columns));
 }
 __device__ __forceinline__ void tc5_fence_before() { asm volatile("tcgen05.fence::before_thread_sync;" ::: "memory"); }
 __device__ __forceinline__ void tc5_fence_after() { asm volatile("tcgen05.fence::after_thread_sync;" ::: "memory"); }
-// An arrival on `bar` once every product that this thread has issued is done.
+// An arrival on `bar` (of both CTAs) once every product that this thread has issued is done.
+template <int CG>
 __device__ __forceinline__ void tc5_commit(uint32_t bar) {
-    asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+    if (CG == 1)
+        asm volatile("tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];" :: "r"(bar) : "memory");
+    else
+        asm volatile("{\n\t.reg .b16 both;\n\tmov.b16 both, 3;\n\t"
+                     "tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.multicast::cluster.b64 [%0], both;\n\t}"
+                     :: "r"(bar) : "memory");
 }
 
 // A K-major operand of 64 16-bit values per row in shared memory, rows of 128 bytes with 16-byte pieces XOR-swizzled by
@@ -79,21 +115,30 @@ __device__ __forceinline__ void tc5_commit(uint32_t bar) {
 __device__ __forceinline__ uint64_t tc5_operand(uint32_t addr) {
     return (uint64_t)(addr >> 4 & 0x3fff) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
 }
-// bf16 x bf16 -> fp32, both K-major, 128 rows, n columns (a multiple of 16 up to 256).
+// bf16 x bf16 -> fp32, both K-major, 128 CG rows, n columns (a multiple of 16, of 32 for two CTAs, up to 256).
+template <int CG>
 __device__ __forceinline__ uint32_t tc5_bf16_shape(int n) {
-    return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (128u >> 4) << 24;
+    return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(CG * 128 >> 4) << 24;
 }
 // D (+)= A B, A in shared memory
-__device__ __forceinline__ void tc5_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"((uint32_t)add) : "memory");
+template <int CG>
+__device__ __forceinline__ void tc5_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
+    if (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
+                     :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"(add) : "memory");
 }
 // D (+)= A B, A in tensor memory (lane = row, a column holds two neighbours along K)
-__device__ __forceinline__ void tc5_mma_t(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, bool add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\t"
-                 "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                 :: "r"(d), "r"(a), "l"(b), "r"(shape), "r"((uint32_t)add) : "memory");
+template <int CG>
+__device__ __forceinline__ void tc5_mma_t(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, uint32_t add) {
+    if (CG == 1)
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+    else
+        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "l"(b), "r"(shape), "r"(add) : "memory");
 }
 // 16 columns of the warp's 32 lanes: a row per lane
 __device__ __forceinline__ void tmem_load16(uint32_t addr, float v[16]) {
@@ -106,10 +151,10 @@ __device__ __forceinline__ void tmem_load16(uint32_t addr, float v[16]) {
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = __uint_as_float(r[i]);
 }
+__device__ __forceinline__ void tmem_store_wait() { asm volatile("tcgen05.wait::st.sync.aligned;" ::: "memory"); }
 __device__ __forceinline__ void tmem_store32(uint32_t addr, const uint32_t r[32]) {
     asm volatile("tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8, %9, %10, %11, %12, %13, %14, %15, "
-                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};\n\t"
-                 "tcgen05.wait::st.sync.aligned;"
+                 "%16, %17, %18, %19, %20, %21, %22, %23, %24, %25, %26, %27, %28, %29, %30, %31, %32};"
                  :: "r"(addr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]),
                     "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]),
                     "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]), "r"(r[25]), "r"(r[26]),
