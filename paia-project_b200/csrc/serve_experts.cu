@@ -30,14 +30,13 @@ constexpr int kExpUnit = kExpRows * 128;             // bytes of W per unit: 128
 constexpr int kExpMinRun = 8;                        // units per CTA, at least, where a list is cut
 constexpr int kExpMaxStages = 12;
 constexpr int kExpX = 2, kExpEpilogue = 4, kExpGather = 8, kExpConverters = 12;      // first warps of the roles
-constexpr int kExpLag = 2;                           // stages that a gathering thread has in flight before it looks back
 
 // FMT 0: bf16, 1: e4m3. CG CTAs per tile.
 template <int FMT, int CG>
 struct Exp {
     static constexpr int kK = FMT == 0 ? 64 : 128;               // of K per unit
     static constexpr int kXTiles = kK / 64;                      // of x per unit, 128 bytes a row
-    static constexpr int kThreads = FMT == 0 ? 384 : 640;
+    static constexpr int kThreads = FMT == 0 ? 384 : 896;
     static constexpr int kABufs = CG == 1 ? 4 : 2;               // buffers of converted W, 64 columns each
     static constexpr int kABase = 512 - 64 * kABufs;
 };
@@ -272,7 +271,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             bar_init(sptr(&bars.d_empty[i]), 4 * CG);
         }
         for (int i = 0; i < 4; ++i) {
-            bar_init(sptr(&bars.a[i]), 128);
+            bar_init(sptr(&bars.a[i]), 256);
             bar_init(sptr(&bars.a_empty[i]), 1);
         }
         bar_init(sptr(&bars.drained), 1);
@@ -335,8 +334,6 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         // ---- x, gathered: a thread has 16-byte piece `piece` of rows r0 + 16 i
         const int t = threadIdx.x - kExpGather * 32, r0 = t >> 3, piece = t & 7;
         const uint32_t to0 = ring + sub * kExpUnit + r0 * 128 + ((piece ^ (r0 & 7)) << 4);
-        int behind = 0;                                          // stages issued and not yet passed on
-        ExpRing back(p.stages);
         while (ok && walk.next(s)) {
             const int half = CG == 1 ? s.m : walk.round_up(s.m) / 2, skip = (int)rank * half, mine = min(half, s.m - skip);
             const __nv_bfloat16* src[8];                         // nullptr: no such row, zeros
@@ -364,20 +361,12 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                         if (r0 + 16 * i < mine) cp16(to + i * 2048, got ? src[i] + from : p.x, got ? 16 : 0);
                     }
                 }
-                cp_commit();
+                cp_arrive(bar_full + 8 * at.slot);
                 at.step();
-                if (++behind > kExpLag) {
-                    cp_wait<kExpLag>();
-                    async_proxy_fence();
-                    bar_arrive(bar_full + 8 * back.slot);
-                    back.step();
-                    --behind;
-                }
             }
         }
+        cp_commit();
         cp_wait<0>();
-        async_proxy_fence();
-        for (; behind > 0; --behind, back.step()) bar_arrive(bar_full + 8 * back.slot);
     } else if (warp == 1) {
         // ---- products, where a stage (e4m3: a buffer of converted W, and with it the stage) is there; the second CTA of a pair
         // tells the first
@@ -402,6 +391,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                             const int i = FMT == 0 ? at.slot : ab;
                             const uint32_t phase = FMT == 0 ? at.phase : ap;
                             if (!wait((FMT == 0 ? bar_full : bar_a) + 8 * i, phase)) break;
+                            async_proxy_fence();
                             if (CG == 2 && leader && !wait(bar_peer + 8 * i, phase)) break;
                             if (CG == 2 && !leader) bar_arrive_at(bar_peer + 8 * i, 0);
                             tc5_fence_after();
@@ -524,9 +514,11 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             if (whole) release();
         }
     } else if (FMT == 1 && warp >= kExpConverters) {
-        // ---- e4m3 -> bf16: two groups of four warps take the units in turn, a row per thread
-        const int group = (warp - kExpConverters) >> 2, row = (warp & 3) * 32 + lane;
-        const uint32_t key = (row & 7) << 4;
+        // ---- e4m3 -> bf16: two groups of eight warps take the units in turn, a row's half per thread. (With one group of eight
+        // the units waited for each other's latency: 1000 cycles each, of which the integer pipe was busy for 560.)
+        const int group = (warp - kExpConverters) >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
+        const uint32_t key = (row & 7) << 4, from0 = ring + row * 128;
+        const uint32_t to0 = tmem + T::kABase + 32 * half + ((uint32_t)((warp & 3) * 32) << 16);
         int turn = 0, ab = 0;
         uint32_t ap = 1;                                         // the first round of buffers is free
         const auto wait_all = [&](uint32_t bar, uint32_t phase) { return ok = __all_sync(0xffffffffu, bar_wait(bar, phase, dead)); };
@@ -536,22 +528,18 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 for (int u = 0; u < n; ++u, turn ^= 1) {
                     if (turn == group) {
                         if (!wait_all(bar_full + 8 * at.slot, at.phase)) break;
-                        const uint32_t from = ring + at.slot * stage + u * kExpUnit + row * 128;
-                        const uint32_t to = tmem + T::kABase + 64 * ab + ((uint32_t)((warp & 3) * 32) << 16);
-                        uint4 v[8];
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v[i].x), "=r"(v[i].y), "=r"(v[i].z), "=r"(v[i].w)
-                                         : "r"(from + ((i << 4) ^ key)));
+                        const uint32_t from = from0 + at.slot * stage + u * kExpUnit;
                         uint32_t r[32];
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) e4m3x16_bf16(v[i], r + 8 * i);
+                        for (int i = 0; i < 4; ++i) {
+                            uint4 v;
+                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
+                                         : "r"(from + (((4 * half + i) << 4) ^ key)));
+                            e4m3x16_bf16(v, r + 8 * i);
+                        }
                         if (!wait_all(bar_a_empty + 8 * ab, ap)) break;
                         tc5_fence_after();
-                        tmem_store32(to, r);
-#pragma unroll
-                        for (int i = 0; i < 4; ++i) e4m3x16_bf16(v[4 + i], r + 8 * i);
-                        tmem_store32(to + 32, r);
+                        tmem_store32(to0 + 64 * ab, r);
                         tmem_store_wait();
                         tc5_fence_before();
                         bar_arrive(bar_a + 8 * ab);
@@ -607,7 +595,7 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t
     // Few tokens: larger stages, for fewer waits.
     p.sub = depth >= 10 ? 2 : 1;
     p.stages = depth / p.sub < kExpMaxStages ? depth / p.sub : kExpMaxStages;
-    if (p.stages < kExpLag + 2) return -2;
+    if (p.stages < 2) return -2;
     const size_t smem = fixed + (size_t)p.stages * p.sub * unit;
     p.units = (a->K + T::kK - 1) / T::kK;
     const int rows = CG * (SILU ? 64 : kExpRows);

@@ -28,7 +28,8 @@ __device__ __forceinline__ void bar_expect(uint32_t bar, uint32_t bytes) {
 }
 __device__ __forceinline__ bool bar_test(uint32_t bar, uint32_t parity) {
     uint32_t done;
-    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+    // (asleep for up to 10 us, so that the waiting warps leave the issue slots to the others)
+    asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.shared.b64 p, [%1], %2, 10000;\n\tselp.u32 %0, 1, 0, p;\n\t}"
                  : "=r"(done) : "r"(bar), "r"(parity) : "memory");
     return done != 0;
 }
@@ -53,7 +54,7 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     uint64_t t0 = 0;
     for (int i = 1;; ++i) {
         if (bar_test(bar, parity)) return true;
-        if (i & 255) continue;
+        if (i & 15) continue;
         if (*dead) return false;
         if (!t0) t0 = wait_clock_ns();
         if (wait_clock_ns() - t0 > 2000000000ull) {
@@ -64,7 +65,11 @@ __device__ __forceinline__ bool bar_wait(uint32_t bar, uint32_t parity, volatile
     }
 }
 
-// What this thread has written to shared memory is seen by the tensor cores behind its next arrival on a barrier.
+// One arrival on `bar` (counted in its arrivals) once every cp.async of this thread so far has landed.
+__device__ __forceinline__ void cp_arrive(uint32_t bar) {
+    asm volatile("cp.async.mbarrier.arrive.noinc.shared.b64 [%0];" :: "r"(bar) : "memory");
+}
+// What threads wrote to shared memory, and this one has seen through a barrier, is seen by the products that it issues next.
 __device__ __forceinline__ void async_proxy_fence() { asm volatile("fence.proxy.async.shared::cta;" ::: "memory"); }
 
 __device__ __forceinline__ void tma_2d(uint32_t dst, const void* map, int x, int y, uint32_t bar) {
