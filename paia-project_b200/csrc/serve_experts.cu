@@ -10,8 +10,9 @@
 //   stream   W by TMA, x too where its rows are in order; gathered rows by cp.async into the same swizzled form (TMA's own
 //            gather of four rows took 58 cycles each). A ring of as many stages of one or more units as shared memory holds.
 //   math     bf16 x bf16 in fp32 accumulators in tensor memory, two tiles' worth, so that one is stored while the next is
-//            summed. e4m3 becomes bf16 exactly, in registers, and meets x from tensor memory; its row's scale is applied
-//            to the sum, so x is never rounded.
+//            summed. e4m3 with few tokens: the bytes as they are, and x as four e4m3 terms (split_kernel), each a column of
+//            its own: x is exact down to 2^-26 of its row's largest, what is off below that is 2^-34 of it. With many: W
+//            becomes bf16 exactly, in registers, and meets x from tensor memory. Its row's scale is applied to the sum.
 //   split    The launch does not know the groups. All tiles form one list (expert, rows of W, block of tokens) that every
 //            CTA finds from the offsets. Whole rounds of one tile per CTA are taken as they come; what is left over, up to
 //            two rounds, is cut into equal runs of units. A tile cut by a run's end leaves its parts in the workspace and
@@ -31,12 +32,18 @@ constexpr int kExpMinRun = 8;                        // units per CTA, at least,
 constexpr int kExpMaxStages = 12;
 constexpr int kExpX = 2, kExpEpilogue = 4, kExpGather = 8, kExpConverters = 12;      // first warps of the roles
 
-// FMT 0: bf16, 1: e4m3. CG CTAs per tile.
+// How W meets x. bf16: both are; split: e4m3 W as it is, x as four e4m3 terms; converted: e4m3 W as bf16.
+enum { kBf16W, kSplit, kConverted };
+constexpr int kExpSplitTokens = 64;                  // per block
+constexpr size_t kExpSplitBytes = 48 << 20;          // of the workspace
+
+// CG CTAs per tile.
 template <int FMT, int CG>
 struct Exp {
-    static constexpr int kK = FMT == 0 ? 64 : 128;               // of K per unit
-    static constexpr int kXTiles = kK / 64;                      // of x per unit, 128 bytes a row
-    static constexpr int kThreads = FMT == 0 ? 384 : 896;
+    static constexpr int kK = FMT == kBf16W ? 64 : 128;          // of K per unit
+    static constexpr int kXTiles = FMT == kConverted ? 2 : 1;    // of x per unit, 128 bytes a row
+    static constexpr int kCols = FMT == kSplit ? 4 : 1;          // columns per token
+    static constexpr int kThreads = FMT == kConverted ? 896 : 384;
     static constexpr int kABufs = CG == 1 ? 4 : 2;               // buffers of converted W, 64 columns each
     static constexpr int kABase = 512 - 64 * kABufs;
 };
@@ -49,7 +56,8 @@ struct alignas(64) ExpertParams {
     const float* scales;
     __nv_bfloat16* out;
     unsigned int* counters;                          // one per cut tile and CTA of it: parts that have arrived
-    float* parts;                                    // [2 grid][tokens][128]
+    float* parts;                                    // [2 grid][columns][128]
+    const float* x_scale;                            // split: [m], of each row's terms
     long long x_row, out_row, scale_expert;
     int experts, n, m, k, x_rows;                    // n: rows of W_e (silu: of gate)
     int units, row_tiles;                            // of K; tiles along n
@@ -159,28 +167,31 @@ __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
     asm("mul.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(t * 16u & 0x87f087f0u), "r"(0x7b807b80u));
     return r;
 }
-// r's halves that came from bytes lo and hi of w, NaN where those are
-__device__ __forceinline__ uint32_t e4m3_nan(uint32_t w, int lo, int hi, uint32_t r) {
-    if ((w >> 8 * lo & 0x7f) == 0x7f) r = (r & 0xffff0000u) | 0x7fffu;
-    if ((w >> 8 * hi & 0x7f) == 0x7f) r = (r & 0xffffu) | 0x7fff0000u;
-    return r;
-}
-__device__ __forceinline__ void e4m3x16_bf16(uint4 v, uint32_t r[8]) {
+// 16 of them from shared memory; a set top bit of a byte of `odd`: a NaN was among them (and came out as 480).
+__device__ __forceinline__ void e4m3x16_bf16(uint32_t from, uint32_t r[8], uint32_t& odd) {
+    uint4 v;
+    asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(from));
     const uint32_t w[4] = {v.x, v.y, v.z, v.w};
-    uint32_t odd = 0;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
         r[2 * i] = e4m3x2_bf16<0x9180>(w[i]);
         r[2 * i + 1] = e4m3x2_bf16<0xb3a2>(w[i]);
         odd |= (w[i] & 0x7f7f7f7fu) + 0x01010101u;
     }
-    if (odd & 0x80808080u) {                                     // a NaN among them
+}
+// 64 of a row (pieces first .. first + 3 of its eight) once more into the 32 columns at `to`, NaN where they are. Out of the
+// way: with it in the converting loop the loop no longer fitted where instructions are fetched from in time (128 against 123 us).
+__device__ __noinline__ void e4m3_row_with_nan(uint32_t row, uint32_t key, int first, uint32_t to) {
+    uint32_t r[32];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            r[2 * i] = e4m3_nan(w[i], 0, 1, r[2 * i]);
-            r[2 * i + 1] = e4m3_nan(w[i], 2, 3, r[2 * i + 1]);
-        }
+    for (int i = 0; i < 32; ++i) {
+        uint32_t w;
+        asm volatile("ld.shared.u16 %0, [%1];" : "=r"(w) : "r"(row + (((first + i / 8) << 4) ^ key) + 2 * (i & 7)));
+        r[i] = e4m3x2_bf16<0x9180>(w);
+        if ((w & 0x7f) == 0x7f) r[i] = (r[i] & 0xffff0000u) | 0x7fffu;
+        if ((w & 0x7f00) == 0x7f00) r[i] = (r[i] & 0xffffu) | 0x7fff0000u;
     }
+    tmem_store32(to, r);
 }
 
 // silu(g) u
@@ -251,7 +262,9 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     const uint32_t ring = (sptr(raw) + 1023) & ~1023u;
     uint8_t* smem = raw + (ring - sptr(raw));
     constexpr int XT = T::kXTiles, K = T::kK;
-    const int sub = p.sub, xb = p.tokens / CG * 128;             // bytes of one tile of x
+    constexpr bool CONV = FMT == kConverted;
+    constexpr int C = T::kCols;
+    const int sub = p.sub, cols = p.tokens * C, xb = cols / CG * 128;    // bytes of one tile of x
     const int stage = sub * (kExpUnit + XT * xb);
     float* exchange = reinterpret_cast<float*>(smem + (size_t)p.stages * stage);
     ExpBars& bars = *reinterpret_cast<ExpBars*>(reinterpret_cast<uint8_t*>(exchange) + kExpExchange);
@@ -271,7 +284,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             bar_init(sptr(&bars.d_empty[i]), 4 * CG);
         }
         for (int i = 0; i < 4; ++i) {
-            bar_init(sptr(&bars.a[i]), 256);
+            bar_init(sptr(&bars.a[i]), 8);
             bar_init(sptr(&bars.a_empty[i]), 1);
         }
         bar_init(sptr(&bars.drained), 1);
@@ -320,13 +333,13 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         // ---- x, rows in order
         if (!p.rows && elect_one()) {
             while (ok && walk.next(s)) {
-                const int row = s.row0 + (int)rank * (walk.round_up(s.m) / CG);
+                const int row = C * s.row0 + (int)rank * (walk.round_up(s.m) / CG);
                 for (int k = s.k0; k < s.k1; k += sub, at.step()) {
                     if (at.full && !wait(bar_empty + 8 * at.slot, at.phase ^ 1u)) break;
                     const int n = XT * min(sub, s.k1 - k);
                     const uint32_t bar = bar_full + 8 * at.slot, to = ring + at.slot * stage + sub * kExpUnit;
                     bar_expect(bar, n * xb);
-                    for (int u = 0; u < n; ++u) tma_2d(to + u * xb, &p.x_map, k * K + 64 * u, row, bar);
+                    for (int u = 0; u < n; ++u) tma_2d(to + u * xb, &p.x_map, k * K + K / XT * u, row, bar);
                 }
             }
         }
@@ -348,7 +361,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 }
             }
             for (int k = s.k0; k < s.k1; k += sub) {
-                if (at.full && !wait(bar_empty + 8 * at.slot, at.phase ^ 1u)) break;
+                if (at.full && !(ok = __all_sync(0xffffffffu, bar_wait(bar_empty + 8 * at.slot, at.phase ^ 1u, dead)))) break;
                 const int n = XT * min(sub, s.k1 - k);
                 for (int u = 0; u < n; ++u) {
                     const uint32_t to = to0 + at.slot * stage + u * xb;
@@ -372,26 +385,26 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         // tells the first
         if (elect_one()) {
             const bool leader = rank == 0;
-            const int tokens = p.tokens;
+            const bool gathered = p.rows != nullptr;
             int ab = 0;                                          // e4m3: buffer of converted W, its phase
             uint32_t ap = 0;
             for (int tile = 0; ok && walk.next(s); ++tile) {
                 const int buf = tile & 1;
                 if (leader && tile >= 2 && !wait(sptr(&bars.d_empty[buf]), (tile / 2 & 1) ^ 1u)) break;
                 tc5_fence_after();
-                const uint32_t d = tmem + buf * tokens;
-                const uint32_t shape = tc5_bf16_shape<CG>(walk.round_up(s.m));
+                const uint32_t d = tmem + buf * cols;
+                const uint32_t shape = FMT == kSplit ? tc5_e4m3_shape<CG>((4 * s.m + 15) & ~15) : tc5_bf16_shape<CG>(walk.round_up(s.m));
                 uint32_t add = 0;
                 for (int k = s.k0; ok && k < s.k1; k += sub) {
                     const int n = min(sub, s.k1 - k);
                     const uint32_t w = ring + at.slot * stage;
                     uint64_t wo = tc5_operand(w), xo = tc5_operand(w + sub * kExpUnit);
                     for (int u = 0; u < n; ++u) {
-                        if (FMT == 1 || u == 0) {
-                            const int i = FMT == 0 ? at.slot : ab;
-                            const uint32_t phase = FMT == 0 ? at.phase : ap;
-                            if (!wait((FMT == 0 ? bar_full : bar_a) + 8 * i, phase)) break;
-                            async_proxy_fence();
+                        if (CONV || u == 0) {
+                            const int i = CONV ? ab : at.slot;
+                            const uint32_t phase = CONV ? ap : at.phase;
+                            if (!wait((CONV ? bar_a : bar_full) + 8 * i, phase)) break;
+                            if (gathered) async_proxy_fence();
                             if (CG == 2 && leader && !wait(bar_peer + 8 * i, phase)) break;
                             if (CG == 2 && !leader) bar_arrive_at(bar_peer + 8 * i, 0);
                             tc5_fence_after();
@@ -401,15 +414,16 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                             for (int j = 0; j < XT; ++j, xo += xb >> 4) {
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
-                                    if (FMT == 0) tc5_mma<CG>(d, wo + 2 * q, xo + 2 * q, shape, add);
+                                    if (FMT == kBf16W) tc5_mma<CG>(d, wo + 2 * q, xo + 2 * q, shape, add);
+                                    else if (FMT == kSplit) tc5_mma_e4m3(d, wo + 2 * q, xo + 2 * q, shape, add);
                                     else tc5_mma_t<CG>(d, tmem + T::kABase + 64 * ab + 32 * j + 8 * q, xo + 2 * q, shape, add);
                                     add = 1;
                                 }
                             }
                             wo += kExpUnit >> 4;
-                            if (FMT == 1) tc5_commit<CG>(bar_a_empty + 8 * ab);
+                            if (CONV) tc5_commit<CG>(bar_a_empty + 8 * ab);
                         }
-                        if (FMT == 1 && ++ab == T::kABufs) {
+                        if (CONV && ++ab == T::kABufs) {
                             ab = 0;
                             ap ^= 1u;
                         }
@@ -433,7 +447,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             const int buf = tile & 1;
             if (!(ok = all_of(__all_sync(0xffffffffu, bar_wait(sptr(&bars.d[buf]), tile / 2 & 1, dead))))) break;
             tc5_fence_after();
-            const uint32_t d = tmem + buf * p.tokens + ((uint32_t)(q * 32) << 16);
+            const uint32_t d = tmem + buf * cols + ((uint32_t)(q * 32) << 16);
             const auto release = [&]() {                         // the accumulators may be overwritten
                 tc5_fence_before();
                 __syncwarp();
@@ -448,8 +462,8 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             if (!whole) {
                 c0 = walk.owner(s.tile * p.units);
                 c1 = walk.owner((s.tile + 1) * p.units - 1);
-                float* to = p.parts + ((size_t)(walk.place(blockIdx.x / CG, s.tile) * CG + rank) * p.tokens) * kExpRows + row;
-                for (int c = 0; c < s.m; c += 16) {
+                float* to = p.parts + ((size_t)(walk.place(blockIdx.x / CG, s.tile) * CG + rank) * cols) * kExpRows + row;
+                for (int c = 0; c < C * s.m; c += 16) {
                     float v[16];
                     tmem_load16(d + c, v);
 #pragma unroll
@@ -473,47 +487,55 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
                 const int n = SILU ? y + (q & 1) * 32 + lane : y + row;
                 float scale = 1.f;
-                if (FMT == 1 && n < p.n) scale = p.scales[s.e * p.scale_expert + n + (SILU && q >= 2 ? p.n : 0)];
-                for (int c = 0; c < s.m; c += 16) {
+                if (FMT != kBf16W && n < p.n) scale = p.scales[s.e * p.scale_expert + n + (SILU && q >= 2 ? p.n : 0)];
+                constexpr int W = 16 / C;                        // tokens per step
+                for (int t = 0; t < s.m; t += W) {
                     float v[16];
                     if (whole) {
-                        tmem_load16(d + c, v);
+                        tmem_load16(d + C * t, v);
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
                         for (int o = c0; o <= c1; ++o) {
-                            const float* from = p.parts + ((size_t)(walk.place(o, s.tile) * CG + rank) * p.tokens + c) * kExpRows + row;
+                            const float* from = p.parts + ((size_t)(walk.place(o, s.tile) * CG + rank) * cols + C * t) * kExpRows + row;
 #pragma unroll
                             for (int i = 0; i < 16; ++i) v[i] += __ldcg(from + i * kExpRows);
                         }
                     }
-                    if (FMT == 1)
+                    if (FMT == kSplit)
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) v[i] *= scale;
-                    __nv_bfloat16* to = p.out + (long long)(s.row0 + c) * p.out_row + n;
+                        for (int i = 0; i < W; ++i) {
+                            const float f = t + i < s.m ? p.x_scale[s.row0 + t + i] : 0.f;
+                            v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * f;
+                        }
+                    if (FMT != kBf16W)
+#pragma unroll
+                        for (int i = 0; i < W; ++i) v[i] *= scale;
+                    __nv_bfloat16* to = p.out + (long long)(s.row0 + t) * p.out_row + n;
                     if (SILU) {
-                        // the warp with gate keeps columns 0-7, the one with the same rows of up 8-15
+                        // the warp with gate keeps the first half of the tokens, the one with the same rows of up the second
+                        constexpr int H = W / 2;
                         float* x = exchange + (step++ & 1) * (4 * 8 * 32);
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) x[(q * 8 + i) * 32 + lane] = q < 2 ? v[8 + i] : v[i];
+                        for (int i = 0; i < H; ++i) x[(q * 8 + i) * 32 + lane] = q < 2 ? v[H + i] : v[i];
                         asm volatile("bar.sync %0, 64;" :: "r"(2 + (q & 1)) : "memory");
                         const float* y = x + (q ^ 2) * 8 * 32 + lane;
 #pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const int col = i + (q < 2 ? 0 : 8);
-                            const float r = q < 2 ? silu_mul(v[i], y[i * 32]) : silu_mul(y[i * 32], v[8 + i]);
-                            if (c + col < s.m && n < p.n) to[col * p.out_row] = __float2bfloat16_rn(r);
+                        for (int i = 0; i < H; ++i) {
+                            const int at = i + (q < 2 ? 0 : H);
+                            const float r = q < 2 ? silu_mul(v[i], y[i * 32]) : silu_mul(y[i * 32], v[H + i]);
+                            if (t + at < s.m && n < p.n) to[at * p.out_row] = __float2bfloat16_rn(r);
                         }
                     } else {
 #pragma unroll
-                        for (int i = 0; i < 16; ++i)
-                            if (c + i < s.m && n < p.n) to[i * p.out_row] = __float2bfloat16_rn(v[i]);
+                        for (int i = 0; i < W; ++i)
+                            if (t + i < s.m && n < p.n) to[i * p.out_row] = __float2bfloat16_rn(v[i]);
                     }
                 }
             }
             if (whole) release();
         }
-    } else if (FMT == 1 && warp >= kExpConverters) {
+    } else if (CONV && warp >= kExpConverters) {
         // ---- e4m3 -> bf16: two groups of eight warps take the units in turn, a row's half per thread. (With one group of eight
         // the units waited for each other's latency: 1000 cycles each, of which the integer pipe was busy for 560.)
         const int group = (warp - kExpConverters) >> 3, half = warp >> 2 & 1, row = (warp & 3) * 32 + lane;
@@ -529,20 +551,17 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     if (turn == group) {
                         if (!wait_all(bar_full + 8 * at.slot, at.phase)) break;
                         const uint32_t from = from0 + at.slot * stage + u * kExpUnit;
-                        uint32_t r[32];
+                        uint32_t r[32], odd = 0;
 #pragma unroll
-                        for (int i = 0; i < 4; ++i) {
-                            uint4 v;
-                            asm volatile("ld.shared.v4.b32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w)
-                                         : "r"(from + (((4 * half + i) << 4) ^ key)));
-                            e4m3x16_bf16(v, r + 8 * i);
-                        }
+                        for (int i = 0; i < 4; ++i) e4m3x16_bf16(from + (((4 * half + i) << 4) ^ key), r + 8 * i, odd);
                         if (!wait_all(bar_a_empty + 8 * ab, ap)) break;
                         tc5_fence_after();
                         tmem_store32(to0 + 64 * ab, r);
+                        if (__any_sync(0xffffffffu, odd & 0x80808080u)) e4m3_row_with_nan(from, key, 4 * half, to0 + 64 * ab);
                         tmem_store_wait();
                         tc5_fence_before();
-                        bar_arrive(bar_a + 8 * ab);
+                        __syncwarp();
+                        if (lane == 0) bar_arrive(bar_a + 8 * ab);
                     }
                     if (++ab == T::kABufs) {
                         ab = 0;
@@ -561,39 +580,106 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     }
 }
 
+// x of every row of out, in their order, as four e4m3 terms of 128-byte aligned rows [m][4][k] and a power of two by which
+// they are to be multiplied: v = x / scale lies below 256, and v = t0 + t1 + 2^-16 (t2 + t3), each term the nearest to what is
+// left. A row that holds a NaN or an infinity is NaN, one that is not there zero.
+struct SplitParams {
+    const __nv_bfloat16* x;
+    const int* rows;
+    uint8_t* terms;
+    float* scale;
+    long long x_row;
+    int k, x_rows;
+};
+constexpr int kSplitThreads = 256;
+__global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams p) {
+    __shared__ uint32_t part[kSplitThreads / 32];
+    pdl_wait_and_trigger();
+    const int i = blockIdx.x, from = p.rows ? p.rows[i] : i;
+    uint8_t* to = p.terms + (size_t)i * 4 * p.k;
+    const bool there = from >= 0 && from < p.x_rows;
+    if (!there && threadIdx.x == 0) serve_error(kErrRouting);
+    const __nv_bfloat16* x = p.x + (there ? from * p.x_row : 0);
+    uint32_t top = 0;                                            // the largest magnitude, as bits
+    for (int c = threadIdx.x * 8; there && c < p.k; c += kSplitThreads * 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w = (&v.x)[j] & 0x7fff7fffu;
+            top = max(top, max(w & 0xffffu, w >> 16));
+        }
+    }
+    top = __reduce_max_sync(0xffffffffu, top);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+    __syncthreads();
+#pragma unroll
+    for (int j = 0; j < kSplitThreads / 32; ++j) top = max(top, part[j]);
+    // 2^e is the largest's power of two; x 2^(7 - e) in two factors, since the whole may pass fp32's range
+    const bool bad = top >= 0x7f80u;
+    const int e = bad || top == 0 ? 7 : max((int)(top >> 7), 1) - 127, f = 7 - e;
+    const float f0 = ldexpf(1.f, f / 2), f1 = ldexpf(1.f, f - f / 2);
+    if (threadIdx.x == 0) p.scale[i] = ldexpf(1.f, -f);
+    for (int c = threadIdx.x * 8; c < p.k; c += kSplitThreads * 8) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (there) v = *reinterpret_cast<const uint4*>(x + c);
+        uint32_t term[4][2];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            float a = bf16_lo((&v.x)[j]) * f0 * f1, b = bf16_hi((&v.x)[j]) * f0 * f1;
+#pragma unroll
+            for (int t = 0; t < 4; ++t) {
+                if (t == 2) { a *= 0x1p16f; b *= 0x1p16f; }
+                uint16_t q;
+                uint32_t h;
+                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"(b), "f"(a));
+                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(q));
+                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
+                a -= back.x;
+                b -= back.y;
+                if (bad) q = 0x7f7f;
+                term[t][j >> 1] = j & 1 ? term[t][j >> 1] | (uint32_t)q << 16 : q;
+            }
+        }
+#pragma unroll
+        for (int t = 0; t < 4; ++t) *reinterpret_cast<uint2*>(to + (size_t)t * p.k + c) = make_uint2(term[t][0], term[t][1]);
+    }
+}
+
 // The maps. W [experts][rows][K]: 128 bytes of 128 rows (silu: of 64 of gate and 64 of up) per copy; rows and K behind the end
-// arrive as zeros. x [rows][K]: 64 values of the rows that a CTA brings of a block.
-bool map_operands(ExpertParams& p, int fmt, bool silu, int cg, const paia_gemv_expert_args* a) {
+// arrive as zeros. x [rows][K] (split: its terms): 128 bytes of the rows that a CTA brings of a block.
+template <int FMT, bool SILU, int CG>
+bool map_operands(ExpertParams& p, const void* x, long long x_row, int x_rows, const paia_gemv_expert_args* a) {
     const EncodeTiledFn fn = encode_tiled();
     if (!fn) return false;
-    const cuuint64_t es = fmt == 0 ? 2 : 1, row = (cuuint64_t)a->w_row * es;
+    const cuuint64_t es = FMT == kBf16W ? 2 : 1, row = (cuuint64_t)a->w_row * es;
     const cuuint64_t expert = a->experts > 1 ? (cuuint64_t)a->w_expert * es : row;
     const cuuint32_t one[4] = {1, 1, 1, 1};
-    const cuuint64_t dims[4] = {(cuuint64_t)a->K, (cuuint64_t)p.n, silu ? 2u : (cuuint64_t)a->experts, (cuuint64_t)a->experts};
-    const cuuint64_t strides[3] = {row, silu ? row * (cuuint64_t)p.n : expert, expert};
-    const cuuint32_t box[4] = {fmt == 0 ? 64u : 128u, silu ? 64u : 128u, silu ? 2u : 1u, 1};
-    if (fn(&p.w, fmt == 0 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, silu ? 4 : 3,
+    const cuuint64_t dims[4] = {(cuuint64_t)a->K, (cuuint64_t)p.n, SILU ? 2u : (cuuint64_t)a->experts, (cuuint64_t)a->experts};
+    const cuuint64_t strides[3] = {row, SILU ? row * (cuuint64_t)p.n : expert, expert};
+    const cuuint32_t box[4] = {(cuuint32_t)(128 / es), SILU ? 64u : 128u, SILU ? 2u : 1u, 1};
+    if (fn(&p.w, FMT == kBf16W ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_UINT8, SILU ? 4 : 3,
            const_cast<void*>(a->w), dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
            CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) != CUDA_SUCCESS)
         return false;
     if (p.rows) return true;
-    const cuuint64_t x_dims[2] = {(cuuint64_t)a->K, (cuuint64_t)a->x_rows};
-    const cuuint64_t x_stride[1] = {a->x_rows > 1 ? (cuuint64_t)a->x_row * 2 : ((cuuint64_t)a->K * 2 + 15) / 16 * 16};
-    const cuuint32_t x_box[2] = {64, (cuuint32_t)(p.tokens / cg)};
-    return fn(&p.x_map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(a->x), x_dims, x_stride, x_box, one,
-              CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-              CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
+    const cuuint64_t xes = FMT == kSplit ? 1 : 2;
+    const cuuint64_t x_dims[2] = {(cuuint64_t)a->K, (cuuint64_t)x_rows};
+    const cuuint64_t x_stride[1] = {x_rows > 1 ? (cuuint64_t)x_row * xes : ((cuuint64_t)a->K * xes + 15) / 16 * 16};
+    const cuuint32_t x_box[2] = {(cuuint32_t)(128 / xes), (cuuint32_t)(p.tokens * Exp<FMT, CG>::kCols / CG)};
+    return fn(&p.x_map, FMT == kSplit ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x),
+              x_dims, x_stride, x_box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+              CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
 }
 
 template <int FMT, bool SILU, int CG>
-int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t st) {
+int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* terms, cudaStream_t st) {
     using T = Exp<FMT, CG>;
-    const int unit = kExpUnit + T::kXTiles * (p.tokens / CG * 128);
+    const int unit = kExpUnit + T::kXTiles * (p.tokens * T::kCols / CG * 128);
     const size_t most = max_dyn_smem(), fixed = exp_fixed_smem(a->experts);
     if (most < fixed) return -2;
     const int depth = (int)((most - fixed) / unit);              // in units
     // Few tokens: larger stages, for fewer waits.
-    p.sub = depth >= 10 ? 2 : 1;
+    p.sub = depth >= 8 ? 2 : 1;
     p.stages = depth / p.sub < kExpMaxStages ? depth / p.sub : kExpMaxStages;
     if (p.stages < 2) return -2;
     const size_t smem = fixed + (size_t)p.stages * p.sub * unit;
@@ -601,7 +687,21 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t
     const int rows = CG * (SILU ? 64 : kExpRows);
     p.row_tiles = (p.n + rows - 1) / rows;
     if (((long long)a->M / p.tokens + a->experts) * p.row_tiles > 0x7fff0000ll) return -2;
-    if (!map_operands(p, FMT, SILU, CG, a)) return -2;
+    const void* x = p.x;
+    long long x_row = p.x_row;
+    int x_rows = p.x_rows;
+    if (FMT == kSplit) {
+        SplitParams q{p.x, p.rows, terms, reinterpret_cast<float*>(terms + (size_t)a->M * 4 * p.k), p.x_row, p.k, p.x_rows};
+        p.x_scale = q.scale;
+        p.rows = nullptr;
+        x = terms;
+        x_row = p.k;
+        x_rows = 4 * a->M;
+        if (!map_operands<FMT, SILU, CG>(p, x, x_row, x_rows, a)) return -2;
+        if (const int rc = serve_launch(split_kernel, q, dim3((unsigned)a->M), kSplitThreads, 0, st)) return rc;
+    } else if (!map_operands<FMT, SILU, CG>(p, x, x_row, x_rows, a)) {
+        return -2;
+    }
     static std::atomic<unsigned long long> done{0};
     const int rc = serve_allow_smem((const void*)expert_kernel<FMT, SILU, CG>, most, done);
     if (rc) return rc;
@@ -609,18 +709,25 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t
     return serve_launch(expert_kernel<FMT, SILU, CG>, p, dim3((unsigned)grid), T::kThreads, smem > kSmemAlone ? smem : kSmemAlone, st, CG);
 }
 
-template <int FMT, bool SILU>
-int pick_experts(ExpertParams& p, const paia_gemv_expert_args* a, cudaStream_t st) {
+template <bool SILU>
+int pick_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* terms, cudaStream_t st) {
     // Blocks of twice the tokens that an expert has on average: smaller ones read W more often, larger ones leave the ring
     // fewer stages.
     const long long want = 2ll * ((a->M + a->experts - 1) / a->experts);
     p.tokens = 16;
     while (p.tokens < 256 && p.tokens < want && p.tokens < a->M) p.tokens *= 2;
-    if (p.tokens <= 128) return launch_experts<FMT, SILU, 1>(p, a, st);
-    p.tokens = FMT == 0 ? 256 : 192;                 // (e4m3 keeps columns for converted W)
-    return launch_experts<FMT, SILU, 2>(p, a, st);
+    if (a->kind == 0) {
+        if (p.tokens <= 128) return launch_experts<kBf16W, SILU, 1>(p, a, terms, st);
+        return launch_experts<kBf16W, SILU, 2>(p, a, terms, st);
+    }
+    if (p.tokens <= kExpSplitTokens && (size_t)a->M * (4 * (size_t)a->K + 4) <= kExpSplitBytes)
+        return launch_experts<kSplit, SILU, 1>(p, a, terms, st);
+    if (p.tokens <= 128) return launch_experts<kConverted, SILU, 1>(p, a, terms, st);
+    p.tokens = 192;                                  // (converted W takes columns of tensor memory)
+    return launch_experts<kConverted, SILU, 2>(p, a, terms, st);
 }
 
+constexpr size_t kExpParts = (size_t)2 * kExpMaxGrid * kExpRows * 256 * 4;
 constexpr size_t kExpCounters = 2 * kExpMaxGrid * 4;                 // (a cut list has fewer than two tiles per CTA or pair)
 
 }  // namespace
@@ -632,7 +739,7 @@ int experts_device_error(int clear) { return serve_error_word(clear); }
 using namespace pb2;
 
 extern "C" size_t paia_gemv_expert_workspace(void) {
-    return kExpCounters + (size_t)2 * kExpMaxGrid * kExpRows * 256 * 4;
+    return kExpCounters + kExpParts + kExpSplitBytes;
 }
 
 extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* stream) {
@@ -666,6 +773,6 @@ extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* str
     p.m = a->M;
     p.x_rows = a->x_rows;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (a->kind == 0) return a->silu ? pick_experts<0, true>(p, a, st) : pick_experts<0, false>(p, a, st);
-    return a->silu ? pick_experts<1, true>(p, a, st) : pick_experts<1, false>(p, a, st);
+    uint8_t* terms = static_cast<uint8_t*>(a->workspace) + kExpCounters + kExpParts;
+    return a->silu ? pick_experts<true>(p, a, terms, st) : pick_experts<false>(p, a, terms, st);
 }

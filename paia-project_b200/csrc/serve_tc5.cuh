@@ -125,6 +125,16 @@ template <int CG>
 __device__ __forceinline__ uint32_t tc5_bf16_shape(int n) {
     return 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(n >> 3) << 17 | (uint32_t)(CG * 128 >> 4) << 24;
 }
+// e4m3 x e4m3 -> fp32
+template <int CG>
+__device__ __forceinline__ uint32_t tc5_e4m3_shape(int n) {
+    return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(CG * 128 >> 4) << 24;
+}
+// D (+)= A B of e4m3, 32 of K
+__device__ __forceinline__ void tc5_mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
+                 :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+}
 // D (+)= A B, A in shared memory
 template <int CG>
 __device__ __forceinline__ void tc5_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
