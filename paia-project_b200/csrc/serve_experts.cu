@@ -111,6 +111,8 @@ struct ExpWalk {
         int rounds = total / g;
         cut = total - rounds * g;
         if (cut && rounds) cut += g;
+        // less than a round that keeps most CTAs busy: whole tiles, no joins
+        else if (4 * cut >= 3 * g) cut = 0;
         work = cut * p.units;
         workers = min(g, max(1, work / kExpMinRun));
         at = c < workers ? bound(c) : 0;
@@ -349,29 +351,41 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         const uint32_t to0 = ring + sub * kExpUnit + r0 * 128 + ((piece ^ (r0 & 7)) << 4);
         while (ok && walk.next(s)) {
             const int half = CG == 1 ? s.m : walk.round_up(s.m) / 2, skip = (int)rank * half, mine = min(half, s.m - skip);
-            const __nv_bfloat16* src[8];                         // nullptr: no such row, zeros
+            const __nv_bfloat16* src[8];                         // (a row that is not in the block: any)
+            int gone = 0;                                        // bit i: row i is nowhere: zeros
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int r = r0 + 16 * i;
-                src[i] = nullptr;
+                int from = 0;
                 if (r < mine) {
-                    const int from = p.rows[s.row0 + skip + r];
-                    if (from >= 0 && from < p.x_rows) src[i] = p.x + from * p.x_row + piece * 8;
-                    else serve_error(kErrRouting);
+                    from = p.rows[s.row0 + skip + r];
+                    if (from < 0 || from >= p.x_rows) {
+                        serve_error(kErrRouting);
+                        from = 0;
+                        gone |= 1 << i;
+                    }
                 }
+                src[i] = p.x + from * p.x_row + piece * 8;
             }
+            const bool plain = !__any_sync(0xffffffffu, gone);
+            const int steps = (mine + 15) >> 4;
             for (int k = s.k0; k < s.k1; k += sub) {
                 if (at.full && !(ok = __all_sync(0xffffffffu, bar_wait(bar_empty + 8 * at.slot, at.phase ^ 1u, dead)))) break;
                 const int n = XT * min(sub, s.k1 - k);
                 for (int u = 0; u < n; ++u) {
                     const uint32_t to = to0 + at.slot * stage + u * xb;
                     const int from = k * K + 64 * u;
-                    const bool in = from + piece * 8 < p.k;      // zeros behind the end of K
+                    if (plain && from + 64 <= p.k) {
 #pragma unroll
-                    for (int i = 0; i < 8; ++i) {
-                        if (16 * i >= mine) break;
-                        const bool got = in && src[i];
-                        if (r0 + 16 * i < mine) cp16(to + i * 2048, got ? src[i] + from : p.x, got ? 16 : 0);
+                        for (int i = 0; i < 8; ++i)
+                            if (i < steps) cp16(to + i * 2048, src[i] + from);
+                    } else {
+                        const bool in = from + piece * 8 < p.k;  // zeros behind the end of K
+#pragma unroll
+                        for (int i = 0; i < 8; ++i) {
+                            const bool got = in && !(gone >> i & 1);
+                            if (i < steps) cp16(to + i * 2048, got ? src[i] + from : p.x, got ? 16 : 0);
+                        }
                     }
                 }
                 cp_arrive(bar_full + 8 * at.slot);
