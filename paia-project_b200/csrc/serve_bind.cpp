@@ -17,7 +17,7 @@ PyObject* g_tensor = nullptr;                    // torch.Tensor
 using Call = int (*)(const void*, void*);
 using Device = int (*)(void);
 
-enum Kind { kBf16, kF32, kF64, kI32, kE4m3 };
+enum Kind { kBf16, kF32, kF64, kI32, kE4m3, kU8 };
 
 bool is_kind(const DLDataType& t, Kind k) {
     if (t.lanes != 1) return false;
@@ -26,6 +26,7 @@ bool is_kind(const DLDataType& t, Kind k) {
         case kF32: return t.code == kDLFloat && t.bits == 32;
         case kF64: return t.code == kDLFloat && t.bits == 64;
         case kI32: return t.code == kDLInt && t.bits == 32;
+        case kU8: return t.code == kDLUInt && t.bits == 8;
         default: return t.code == kDLFloat8_e4m3fn && t.bits == 8;
     }
 }
@@ -289,6 +290,163 @@ PyObject* lora(PyObject*, PyObject* const* a, Py_ssize_t n) {
     return PyErr_Occurred() ? none() : PyLong_FromLong(address<Call>(a[0])(&s, stream));
 }
 
+// The integers of a tuple of n.
+bool integers(PyObject* o, int n, long long* v) {
+    if (!PyTuple_CheckExact(o) || PyTuple_GET_SIZE(o) != n) return false;
+    for (int i = 0; i < n; ++i)
+        if (!integer(PyTuple_GET_ITEM(o, i), v + i)) return false;
+    return true;
+}
+
+// (entry, device, logits, routing pointers (weights, experts, places, rows, offsets, workspace), routing sizes (device, tokens,
+//  experts, top_k), scoring, bias, renormalise, scale, positions, stream)
+PyObject* route(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 11) return none();
+    const int dev = current(a[0], a[1]);
+    Arg x, bias, pos;
+    long long ptr[6], size[4];
+    const void *bp, *pp;
+    double scale = 0.0;
+    paia_gemv_route_args s{};
+    if (dev < 0 || !x.read(a[2], dev) || x.t.ndim != 2 || !x.dense_last() || !integers(a[3], 6, ptr) || !integers(a[4], 4, size) ||
+        size[0] != dev || x.n(0) != size[1] || x.n(1) != size[2] || !small(size[1]) || !small(size[2]) || !small(size[3]))
+        return none();
+    s.logits_type = is_kind(x.t.dtype, kBf16) ? 0 : is_kind(x.t.dtype, kF32) ? 1 : -1;
+    if (s.logits_type < 0 || !PyUnicode_CheckExact(a[5])) return none();
+    s.scoring = PyUnicode_CompareWithASCIIString(a[5], "softmax") == 0 ? 0
+                : PyUnicode_CompareWithASCIIString(a[5], "sigmoid") == 0 ? 1 : -1;
+    if (s.scoring < 0 || !bias.flat(a[6], dev, kF32, size[2], &bp) || (bp && !s.scoring) ||
+        !pos.flat(a[9], dev, kI32, size[1], &pp) || !number(a[8], &scale))
+        return none();
+    const int renorm = PyObject_IsTrue(a[7]);
+    void* stream = nullptr;
+    if (renorm < 0 || !stream_of(a[10], dev, &stream)) return none();
+    s.logits = x.ptr();
+    s.bias = static_cast<const float*>(bp);
+    s.pos = static_cast<const int*>(pp);
+    s.weights = reinterpret_cast<float*>((uintptr_t)ptr[0]);
+    s.ids = reinterpret_cast<int*>((uintptr_t)ptr[1]);
+    s.places = reinterpret_cast<int*>((uintptr_t)ptr[2]);
+    s.rows = reinterpret_cast<int*>((uintptr_t)ptr[3]);
+    s.offsets = reinterpret_cast<int*>((uintptr_t)ptr[4]);
+    s.workspace = reinterpret_cast<void*>((uintptr_t)ptr[5]);
+    s.logits_row = x.stride(0);
+    s.tokens = (int)size[1];
+    s.experts = (int)size[2];
+    s.top_k = (int)size[3];
+    s.renormalise = renorm;
+    s.scale = (float)scale;
+    return PyErr_Occurred() ? none() : PyLong_FromLong(address<Call>(a[0])(&s, stream));
+}
+
+// (entry, device, w, x, offsets, out, workspace pointer, workspace device, scales, rows, silu, stream)
+PyObject* expert_matmul(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 12) return none();
+    const int dev = current(a[0], a[1]);
+    Arg w, x, off, out, sc, rows;
+    const void *op, *rp;
+    long long ws_dev = -1;
+    paia_gemv_expert_args s{};
+    if (dev < 0 || !w.read(a[2], dev) || w.t.ndim != 3 || !w.dense_last() || !x.is(a[3], dev, kBf16, 2) || !x.dense_last() ||
+        !out.is(a[5], dev, kBf16, 2) || !out.dense_last() || !integer(a[7], &ws_dev) || ws_dev != dev)
+        return none();
+    s.kind = is_kind(w.t.dtype, kBf16) ? 0 : is_kind(w.t.dtype, kE4m3) || is_kind(w.t.dtype, kU8) ? 1 : -1;
+    const int silu = PyObject_IsTrue(a[10]);
+    const long long e = w.n(0), rn = w.n(1), k = w.n(2), m = out.n(0), cols = silu > 0 ? rn / 2 : rn;
+    if (s.kind < 0 || silu < 0 || !small(e) || !small(rn) || !small(k) || !small(m) || !small(x.n(0)) || x.n(1) != k ||
+        out.n(1) != cols || (silu && rn % 2) || !off.flat(a[4], dev, kI32, e + 1, &op) || !op ||
+        !rows.flat(a[9], dev, kI32, m, &rp) || (!rp && x.n(0) < m))
+        return none();
+    if (s.kind == 1) {
+        if (!sc.is(a[8], dev, kF32, 2) || sc.n(0) != e || sc.n(1) != rn || !sc.dense_last()) return none();
+        s.scales = static_cast<const float*>(sc.ptr());
+        s.scale_expert = sc.stride(0);
+    } else if (a[8] != Py_None) {
+        return none();
+    }
+    void* stream = nullptr;
+    if (!stream_of(a[11], dev, &stream)) return none();
+    s.w = w.ptr();
+    s.x = x.ptr();
+    s.rows = static_cast<const int*>(rp);
+    s.offsets = static_cast<const int*>(op);
+    s.out = out.ptr();
+    s.workspace = address<void*>(a[6]);
+    s.w_expert = w.stride(0);
+    s.w_row = rn > 1 ? w.stride(1) : k;
+    s.x_row = x.stride(0);
+    s.out_row = out.stride(0);
+    s.experts = (int)e;
+    s.M = (int)m;
+    s.N = (int)rn;
+    s.K = (int)k;
+    s.x_rows = (int)x.n(0);
+    s.silu = silu;
+    return PyErr_Occurred() ? none() : PyLong_FromLong(address<Call>(a[0])(&s, stream));
+}
+
+// (entry, device, h, x, h_out, out, places, weights, post, gate, scale, pre, eps, stream)
+PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    if (n != 14) return none();
+    const int dev = current(a[0], a[1]);
+    Arg h, x, ho, out, pl, wt, post, pre, gate;
+    const void *qp, *np;
+    double scale = 0.0, eps = 0.0;
+    paia_gemv_block_norm_args s{};
+    if (dev < 0 || !h.is(a[2], dev, kBf16, 2) || !h.dense_last() || (a[3] == Py_None) != (a[4] == Py_None)) return none();
+    const long long t = h.n(0), hid = h.n(1);
+    if (!small(t) || !small(hid) || !post.flat(a[8], dev, kF32, hid, &qp) || !pre.flat(a[11], dev, kF32, hid, &np) ||
+        !number(a[10], &scale) || !number(a[12], &eps))
+        return none();
+    if (a[6] != Py_None) {
+        if (!pl.is(a[6], dev, kI32, 2) || !wt.is(a[7], dev, kF32, 2) || pl.n(0) != t || wt.n(0) != t || wt.n(1) != pl.n(1) ||
+            !small(pl.n(1)) || !pl.dense_last() || !wt.dense_last())
+            return none();
+        s.places = static_cast<const int*>(pl.ptr());
+        s.weights = static_cast<const float*>(wt.ptr());
+        s.places_row = pl.stride(0);
+        s.weights_row = wt.stride(0);
+        s.top_k = (int)pl.n(1);
+    } else if (a[7] != Py_None) {
+        return none();
+    }
+    if (a[3] != Py_None) {
+        if (!x.is(a[3], dev, kBf16, 2) || !ho.is(a[4], dev, kBf16, 2) || x.n(1) != hid || !small(x.n(0)) || ho.n(0) != t ||
+            ho.n(1) != hid || !x.dense_last() || !ho.dense_last() || (!s.places && x.n(0) < t))
+            return none();
+        s.x = x.ptr();
+        s.x_row = x.stride(0);
+        s.x_rows = (int)x.n(0);
+        s.h_out = ho.ptr();
+        s.h_out_row = ho.stride(0);
+    }
+    if (a[5] != Py_None) {
+        if (!out.is(a[5], dev, kBf16, 2) || out.n(0) != t || out.n(1) != hid || !out.dense_last()) return none();
+        s.out = out.ptr();
+        s.out_row = out.stride(0);
+    }
+    if (a[9] != Py_None) {
+        if (!gate.read(a[9], dev) || !is_kind(gate.t.dtype, kBf16) || gate.t.ndim < 1 || gate.t.ndim > 2 || !gate.dense_last())
+            return none();
+        const long long cols = gate.n(gate.t.ndim - 1);
+        if (!(gate.t.ndim == 1 ? cols == hid : gate.n(0) == t && (cols == hid || cols == 1))) return none();
+        s.gate = gate.ptr();
+        s.gate_row = gate.t.ndim == 2 ? gate.stride(0) : 0;
+        s.gate_col = cols == hid;
+    }
+    void* stream = nullptr;
+    if (!stream_of(a[13], dev, &stream)) return none();
+    s.h = h.ptr();
+    s.h_row = h.stride(0);
+    s.post = static_cast<const float*>(qp);
+    s.pre = static_cast<const float*>(np);
+    s.tokens = (int)t;
+    s.hidden = (int)hid;
+    s.eps = (float)eps;
+    s.scale = (float)scale;
+    return PyErr_Occurred() ? none() : PyLong_FromLong(address<Call>(a[0])(&s, stream));
+}
+
 // (torch.Tensor, its __dlpack_c_exchange_api__ capsule) -> whether calls can be made
 PyObject* init(PyObject*, PyObject* const* a, Py_ssize_t n) {
     if (n != 2 || !PyCapsule_IsValid(a[1], "dlpack_exchange_api")) Py_RETURN_FALSE;
@@ -307,6 +465,9 @@ PyMethodDef kMethods[] = {
     {"paged_attention", (PyCFunction)(void (*)(void))paged_attention, METH_FASTCALL, nullptr},
     {"qkv_rope_cache", (PyCFunction)(void (*)(void))qkv_rope_cache, METH_FASTCALL, nullptr},
     {"lora", (PyCFunction)(void (*)(void))lora, METH_FASTCALL, nullptr},
+    {"route", (PyCFunction)(void (*)(void))route, METH_FASTCALL, nullptr},
+    {"expert_matmul", (PyCFunction)(void (*)(void))expert_matmul, METH_FASTCALL, nullptr},
+    {"block_norm", (PyCFunction)(void (*)(void))block_norm, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr}};
 PyModuleDef kModule = {PyModuleDef_HEAD_INIT, "_paia_serve", nullptr, -1, kMethods, nullptr, nullptr, nullptr, nullptr};
 

@@ -761,15 +761,15 @@ extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* str
         (a->kind != 0 && a->kind != 1) || (a->silu && a->N % 2))
         return -2;
     const int unit = a->kind == 0 ? 8 : 16;
-    if (a->K % unit || a->K > 1 << 20 || a->M > 1 << 28) return -2;
-    if (!a->w || !a->offsets || !a->workspace || (a->M && (!a->x || !a->out)) || !a->scales != !a->kind) return -2;
+    if (a->K % unit || a->K > 1 << 20 || a->M > 1 << 28 || !a->scales != !a->kind) return -2;
+    if (a->M == 0) return 0;
+    if (!a->w || !a->offsets || !a->workspace || !a->x || !a->out) return -2;
     if (!aligned_to(a->w, 16) || !aligned_to(a->x, 16) || !aligned_to(a->out, 2) || !aligned_to(a->rows, 4) ||
         !aligned_to(a->offsets, 4) || !aligned_to(a->scales, 4) || !aligned_to(a->workspace, 16) || a->w_row % unit ||
         a->w_expert % unit || a->x_row % 8 || a->w_row < a->K || (a->experts > 1 && a->w_expert < 1))
         return -2;
-    if (!a->rows && a->x_rows < a->M) return -2;
+    if (a->x_rows < (a->rows ? 1 : a->M)) return -2;
     if ((a->M > 1 && a->out_row == 0) || a->out == a->x) return -2;
-    if (a->M == 0) return 0;
     ExpertParams p{};
     p.rows = a->rows;
     p.offsets = a->offsets;

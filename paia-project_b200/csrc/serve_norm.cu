@@ -13,6 +13,9 @@
 namespace pb2 {
 namespace {
 
+constexpr int kNormMaxHidden = 32768;
+constexpr int kNormThreads = 512;                    // per row, at most
+
 struct NormParams {
     const __nv_bfloat16* x;
     const __nv_bfloat16* h;
@@ -52,9 +55,9 @@ __device__ __forceinline__ float cta_sum(float v, float* part) {
     return v;
 }
 
-// V pieces of a row per thread.
-template <int V, int THREADS>
-__global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormParams p) {
+// V pieces of a row per thread; B rows of a sum on their way together.
+template <int V, int B>
+__global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const NormParams p) {
     __shared__ float part[2][32];
     pdl_wait_and_trigger();
     const int n = (int)blockDim.x;
@@ -69,21 +72,36 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormParams p)
             for (int e = 0; e < 8; ++e) y[i][e] = 0.f;
         }
         if (p.top_k) {
-            for (int j = 0; j < p.top_k; ++j) {
-                const int at = p.places[t * p.places_row + j];
-                const float w = p.weights[t * p.weights_row + j];
-                if (at < 0 || at >= p.x_rows) {                  // -1: this place is empty
-                    if (at != -1 && threadIdx.x == 0) serve_error(kErrRouting);
-                    continue;
+            for (int j0 = 0; j0 < p.top_k; j0 += B) {
+                int at[B];
+                float w[B];
+#pragma unroll
+                for (int b = 0; b < B; ++b) {
+                    at[b] = j0 + b < p.top_k ? p.places[t * p.places_row + j0 + b] : -1;
+                    w[b] = j0 + b < p.top_k ? p.weights[t * p.weights_row + j0 + b] : 0.f;
                 }
+#pragma unroll
+                for (int b = 0; b < B; ++b)
+                    if (at[b] < -1 || at[b] >= p.x_rows) {       // -1: this place is empty
+                        if (threadIdx.x == 0) serve_error(kErrRouting);
+                        at[b] = -1;
+                    }
 #pragma unroll
                 for (int i = 0; i < V; ++i) {
                     const int c = threadIdx.x + i * n;
                     if (c >= p.vecs) continue;
-                    float f[8];
-                    unpack8(*reinterpret_cast<const uint4*>(p.x + at * p.x_row + 8 * c), f);
+                    uint4 v[B];
 #pragma unroll
-                    for (int e = 0; e < 8; ++e) y[i][e] = fmaf(w, f[e], y[i][e]);
+                    for (int b = 0; b < B; ++b)
+                        if (at[b] >= 0) v[b] = *reinterpret_cast<const uint4*>(p.x + at[b] * p.x_row + 8 * c);
+#pragma unroll
+                    for (int b = 0; b < B; ++b)
+                        if (at[b] >= 0) {
+                            float f[8];
+                            unpack8(v[b], f);
+#pragma unroll
+                            for (int e = 0; e < 8; ++e) y[i][e] = fmaf(w[b], f[e], y[i][e]);
+                        }
                 }
             }
         } else if (p.x) {
@@ -164,13 +182,28 @@ __global__ void __launch_bounds__(THREADS) block_norm_kernel(const NormParams p)
     }
 }
 
-constexpr int kNormMaxHidden = 32768;
-
-template <int V, int THREADS>
+template <int V, int B>
 int launch_norm(const NormParams& p, cudaStream_t st) {
-    int threads = ((p.vecs + V - 1) / V + 31) / 32 * 32;
-    const long long most = (long long)sm_count() * (2048 / threads);
-    return serve_launch(block_norm_kernel<V, THREADS>, p, dim3((unsigned)(p.tokens < most ? p.tokens : most)), threads, 0, st);
+    const int threads = ((p.vecs + V - 1) / V + 31) / 32 * 32;
+    static std::atomic<int> known[64];
+    int d = 0, per_sm = 0;
+    if (cudaGetDevice(&d) == cudaSuccess && d < 64) per_sm = known[d].load(std::memory_order_relaxed);
+    if (!per_sm) {                                   // CTAs of the largest size that an SM holds, smaller ones in proportion
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, block_norm_kernel<V, B>, kNormThreads, 0) != cudaSuccess || per_sm < 1) {
+            (void)cudaGetLastError();
+            per_sm = 1;
+        }
+        if (d < 64) known[d].store(per_sm, std::memory_order_relaxed);
+    }
+    const long long most = (long long)sm_count() * (per_sm * kNormThreads / threads);
+    return serve_launch(block_norm_kernel<V, B>, p, dim3((unsigned)(p.tokens < most ? p.tokens : most)), threads, 0, st);
+}
+
+// Few tokens: a token's rows on their way together (61 tokens of 8 rows of 4096: 4.1 us, one after another 5.0). Many: half
+// the registers and so twice the CTAs of an SM, which hide one another's loads.
+template <int V, int B>
+int pick_norm(const NormParams& p, cudaStream_t st) {
+    return p.top_k > 1 && p.tokens <= 2 * sm_count() ? launch_norm<V, B>(p, st) : launch_norm<V, 1>(p, st);
 }
 
 }  // namespace
@@ -219,8 +252,8 @@ extern "C" int paia_gemv_block_norm(const paia_gemv_block_norm_args* a, void* st
     p.scale = a->scale;
     p.inv_hidden = 1.f / (float)a->hidden;
     const cudaStream_t st = static_cast<cudaStream_t>(stream);
-    if (p.vecs <= 512) return launch_norm<1, 512>(p, st);
-    if (p.vecs <= 1024) return launch_norm<2, 512>(p, st);
-    if (p.vecs <= 2048) return launch_norm<4, 512>(p, st);
-    return launch_norm<8, 512>(p, st);
+    if (p.vecs <= 512) return pick_norm<1, 8>(p, st);
+    if (p.vecs <= 1024) return pick_norm<2, 4>(p, st);
+    if (p.vecs <= 2048) return pick_norm<4, 2>(p, st);
+    return launch_norm<8, 1>(p, st);
 }

@@ -1,8 +1,9 @@
 // Choosing each token's experts and grouping the tokens by expert (paia_gemv_route).
 //
 // softmax: a token's experts are those of its top_k largest logits; weights e^(l - m) over the chosen or over all.
-// sigmoid: ordered by s + bias, s = 1 / (1 + e^-l), computed in fp64 so that the choice is that of the real numbers wherever
-// they differ by more than 2^-50; weights s (/ their sum). Ties go to the lowest index in both.
+// sigmoid: ordered by s + bias, s = 1 / (1 + e^-l), as fp64 has it; weights s (/ their sum). fp32 decides where neighbours in
+// the order are further apart than it can be off, which is nearly always; else the token is done again in fp64 (250 tokens
+// of 256 experts, all of them in fp64: 18.4 us). Ties go to the lowest index in both.
 //
 // The chosen (token, place) pairs, "slots", are grouped by expert in the order of their numbers (token * top_k + place): the
 // same bits on every run, without atomics.
@@ -22,10 +23,11 @@
 namespace pb2 {
 namespace {
 
-constexpr int kRouteWarps = 16;
-constexpr int kRouteThreads = kRouteWarps * 32;
+template <bool ONE>
+constexpr int kRouteWarps = ONE ? 16 : 32;           // per CTA of the one-launch form, and of the other
+constexpr int kPlaceThreads = 1024;
 constexpr int kRouteCluster = 8;                     // most CTAs of the one-launch form
-constexpr int kRouteClusterTokens = 1024;
+constexpr int kRouteClusterTokens = 256;            // (500 of 256 experts: 13.8 us here, 11 in two launches; 250: 9.2)
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopK = 32;
 constexpr int kRouteMaxGrid = 160;                   // the workspace holds the counts of this many CTAs
@@ -78,29 +80,13 @@ __device__ __forceinline__ float logit(const RouteParams& p, int t, int e) {
     return p.bf16 ? __bfloat162float(static_cast<const __nv_bfloat16*>(p.logits)[at]) : static_cast<const float*>(p.logits)[at];
 }
 
-// Token t's experts: lane j < top_k returns the j-th (its weight in w).
-template <int L, bool SIG>
-__device__ __forceinline__ int choose(const RouteParams& p, int t, int lane, float& w) {
-    using Key = typename std::conditional<SIG, unsigned long long, uint32_t>::type;
-    Key key[L];
-#pragma unroll
-    for (int i = 0; i < L; ++i) {
-        const int e = lane + 32 * i;
-        key[i] = 0;
-        if (e < p.n_experts) {
-            const float l = logit(p, t, e);
-            if constexpr (SIG) {
-                const double s = 1.0 / (1.0 + exp(-(double)l));
-                key[i] = key_of(p.bias ? s + (double)p.bias[e] : s);
-            } else {
-                key[i] = key_of(l);
-            }
-        }
-    }
-    float total = 0.f, top = 0.f;
+// The `n` largest of the warp's keys (key[i] of lane l: expert l + 32 i), in falling order, ties to the lowest index: lane
+// j < n returns the j-th's expert. each(j, key) is called by all lanes.
+template <int L, class Key, class Each>
+__device__ __forceinline__ int largest(Key key[L], int n, int lane, const Each& each) {
     int mine = 0;
-    Key got = 0;
-    for (int j = 0; j < p.top_k; ++j) {
+#pragma unroll 1
+    for (int j = 0; j < n; ++j) {
         Key best = key[0];
         int at = 0;
 #pragma unroll
@@ -108,29 +94,73 @@ __device__ __forceinline__ int choose(const RouteParams& p, int t, int lane, flo
             if (key[i] > best) { best = key[i]; at = i; }
         const Key m = warp_max(best);
         const int e = (int)__reduce_min_sync(0xffffffffu, best == m ? (uint32_t)(lane + 32 * at) : 0xffffffffu);
-        if constexpr (!SIG) {
-            if (j == 0) {
-                top = of_key(m);
-                if (!p.renorm) {
-#pragma unroll
-                    for (int i = 0; i < L; ++i)
-                        if (key[i]) total += expf(of_key(key[i]) - top);
-                }
-            }
-        }
+        each(j, m);
 #pragma unroll
         for (int i = 0; i < L; ++i) key[i] = lane + 32 * i == e ? 0 : key[i];
-        if (lane == j) { mine = e; got = m; }
+        if (lane == j) mine = e;
+    }
+    return mine;
+}
+
+// Token t's experts: lane j < top_k returns the j-th (its weight in w).
+template <int L, bool SIG>
+__device__ __forceinline__ int choose(const RouteParams& p, int t, int lane, float& w) {
+    float l[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) l[i] = lane + 32 * i < p.n_experts ? logit(p, t, lane + 32 * i) : 0.f;
+    uint32_t key[L];
+#pragma unroll
+    for (int i = 0; i < L; ++i) {
+        const int e = lane + 32 * i;
+        float f = l[i];
+        if constexpr (SIG) {
+            f = __fdividef(1.f, 1.f + __expf(-f));
+            if (p.bias && e < p.n_experts) f += p.bias[e];
+        }
+        key[i] = e < p.n_experts ? key_of(f) : 0;
+    }
+    int mine;
+    if constexpr (SIG) {
+        // s is off by less than 2^-21 (e^-l by 2^-22 and |l| 2^-24 of it, which the sum with 1 makes smaller where |l| is large;
+        // a quotient of 2 steps), its sum with the bias by a rounding: order is certain where neighbours lie further apart
+        // than twice that
+        float last = 0.f;
+        bool close = false;
+        mine = largest<L>(key, min(p.top_k + 1, p.n_experts), lane, [&](int j, uint32_t m) {
+            const float f = of_key(m);
+            close |= j > 0 && !(last - f > (1.f + fabsf(f)) * 0x1p-19f);
+            last = f;
+        });
+        if (close) {
+            unsigned long long exact[L];
+#pragma unroll
+            for (int i = 0; i < L; ++i) {
+                const int e = lane + 32 * i;
+                const double s = 1.0 / (1.0 + exp(-(double)l[i]));
+                exact[i] = e < p.n_experts ? key_of(p.bias ? s + (double)p.bias[e] : s) : 0;
+            }
+            mine = largest<L>(exact, p.top_k, lane, [](int, unsigned long long) {});
+        }
+    } else {
+        mine = largest<L>(key, p.top_k, lane, [](int, uint32_t) {});
     }
     const bool on = lane < p.top_k;
+    const float got = on ? logit(p, t, mine) : 0.f;
     if constexpr (SIG) {
-        w = on ? 1.f / (1.f + expf(-logit(p, t, mine))) : 0.f;
+        w = on ? 1.f / (1.f + expf(-got)) : 0.f;
         if (p.renorm) {
             const float s = warp_sum(w);
             w = s == 0.f ? 0.f : w / s;
         }
     } else {
-        w = on ? expf(of_key(got) - top) : 0.f;
+        const float top = __shfl_sync(0xffffffffu, got, 0);
+        float total = 0.f;
+        if (!p.renorm) {
+#pragma unroll
+            for (int i = 0; i < L; ++i)
+                if (lane + 32 * i < p.n_experts) total += expf(l[i] - top);
+        }
+        w = on ? expf(got - top) : 0.f;
         const float s = warp_sum(p.renorm ? w : total);
         w = top == -INFINITY ? 0.f : w / s;                      // every logit is -inf: no weight
     }
@@ -139,6 +169,7 @@ __device__ __forceinline__ int choose(const RouteParams& p, int t, int lane, flo
 }
 
 // Exclusive prefix of v over the CTA's threads; `part`: a word per warp.
+template <int THREADS>
 __device__ __forceinline__ int cta_prefix(int v, int* part) {
     int s = v;
 #pragma unroll
@@ -150,43 +181,48 @@ __device__ __forceinline__ int cta_prefix(int v, int* part) {
     __syncthreads();
     int before = 0;
 #pragma unroll
-    for (int i = 0; i < kRouteWarps; ++i) before += i < (int)(threadIdx.x >> 5) ? part[i] : 0;
+    for (int i = 0; i < THREADS / 32; ++i) before += i < (int)(threadIdx.x >> 5) ? part[i] : 0;
     return before + s - v;
 }
 
 // base[e] = where the CTA's slots of expert e begin: `before` of the CTAs ahead of it, behind all of the experts before e.
-// Thread i has experts 2 i and 2 i + 1. CTA 0 writes the offsets.
-__device__ __forceinline__ void find_bases(const RouteParams& p, const int all[2], const int before[2], int* base, int* part,
+// Thread i has the N experts from N i. CTA 0 writes the offsets.
+template <int THREADS, int N>
+__device__ __forceinline__ void find_bases(const RouteParams& p, const int all[N], const int before[N], int* base, int* part,
                                            bool first) {
-    const int e = 2 * threadIdx.x;
-    const int at = cta_prefix(all[0] + all[1], part);
-    if (e < p.n_experts) {
-        base[e] = at + before[0];
-        if (e + 1 < p.n_experts) base[e + 1] = at + all[0] + before[1];
-        if (first) {
-            p.offsets[e] = at;
-            p.offsets[e + 1] = at + all[0];
-            if (e + 2 == p.n_experts) p.offsets[e + 2] = at + all[0] + all[1];
-        }
+    int sum = 0;
+#pragma unroll
+    for (int i = 0; i < N; ++i) sum += all[i];
+    int at = cta_prefix<THREADS>(sum, part);
+#pragma unroll
+    for (int i = 0; i < N; ++i) {
+        const int e = N * threadIdx.x + i;
+        if (e >= p.n_experts) break;
+        base[e] = at + before[i];
+        if (first) p.offsets[e] = at;
+        at += all[i];
+        if (first && e + 1 == p.n_experts) p.offsets[e + 1] = at;
     }
     __syncthreads();
 }
 
-__host__ __device__ constexpr size_t route_smem(int experts, int slots) {
-    return ((size_t)(kRouteWarps * 2 + 2 * 4) * experts + 63) / 64 * 64 + 64 + (size_t)4 * slots;
+template <bool ONE>
+constexpr size_t route_smem(int experts, int slots) {
+    return ((size_t)(kRouteWarps<ONE> * 2 + 2 * 4) * experts + 127) / 128 * 128 + 128 + (size_t)4 * slots;
 }
 
 // per warp: counts [warps][experts] (16 bits); then the CTA's totals and bases [experts]; a word per warp; the slots
 template <int L, bool SIG, bool ONE>
-__global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams p) {
+__global__ void __launch_bounds__(kRouteWarps<ONE> * 32) route_kernel(const RouteParams p) {
+    constexpr int kWarps = kRouteWarps<ONE>, kThreads = kWarps * 32;
     extern __shared__ __align__(16) uint8_t smem[];
     const int E = p.n_experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
     unsigned short* seen = reinterpret_cast<unsigned short*>(smem);
-    int* total = reinterpret_cast<int*>(smem + (size_t)kRouteWarps * 2 * E);
+    int* total = reinterpret_cast<int*>(smem + (size_t)kWarps * 2 * E);
     int* base = total + E;
-    int* part = reinterpret_cast<int*>(smem + ((size_t)(kRouteWarps * 2 + 8) * E + 63) / 64 * 64);
-    int* slots = part + kRouteWarps;                             // expert << 16 | rank; ONE only
-    for (int i = threadIdx.x; i < kRouteWarps * E / 2; i += kRouteThreads) reinterpret_cast<uint32_t*>(seen)[i] = 0u;
+    int* part = reinterpret_cast<int*>(smem + ((size_t)(kWarps * 2 + 8) * E + 127) / 128 * 128);
+    int* slots = part + 32;                             // expert << 16 | rank; ONE only
+    for (int i = threadIdx.x; i < kWarps * E / 2; i += kThreads) reinterpret_cast<uint32_t*>(seen)[i] = 0u;
     __syncthreads();
     pdl_wait_and_trigger();
     const int t0 = blockIdx.x * p.per_cta, tn = min(p.per_cta, p.tokens - t0);
@@ -210,10 +246,10 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
         __syncwarp();                                            // the counts are whole before the next token's
     }
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += kRouteThreads) {       // counts of the warps before, and the CTA's total
+    for (int e = threadIdx.x; e < E; e += kThreads) {       // counts of the warps before, and the CTA's total
         int n = 0;
 #pragma unroll
-        for (int w = 0; w < kRouteWarps; ++w) {
+        for (int w = 0; w < kWarps; ++w) {
             const int c = seen[(size_t)w * E + e];
             seen[(size_t)w * E + e] = (unsigned short)n;
             n += c;
@@ -226,7 +262,9 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
         const cg::cluster_group cluster = cg::this_cluster();
         cluster.sync();
         int all[2] = {0, 0}, before[2] = {0, 0};
-        for (int c = 0; c < (int)gridDim.x; ++c) {
+        #pragma unroll
+        for (int c = 0; c < kRouteCluster; ++c) {
+            if (c >= (int)gridDim.x) break;
             const int* of = cluster.map_shared_rank(total, c);
 #pragma unroll
             for (int i = 0; i < 2; ++i) {
@@ -235,8 +273,8 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
                 before[i] += c < (int)blockIdx.x ? n : 0;
             }
         }
-        find_bases(p, all, before, base, part, blockIdx.x == 0);
-        for (int i = threadIdx.x; i < tn * p.top_k; i += kRouteThreads) {
+        find_bases<kThreads, 2>(p, all, before, base, part, blockIdx.x == 0);
+        for (int i = threadIdx.x; i < tn * p.top_k; i += kThreads) {
             const int v = slots[i], e = v >> 16;
             const long long s = (long long)t0 * p.top_k + i;
             int at = -1;
@@ -251,7 +289,7 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
     } else {
         __syncthreads();
         // a slot's rank in the CTA; its expert's place follows
-        for (int i = threadIdx.x; i < tn * p.top_k; i += kRouteThreads) {
+        for (int i = threadIdx.x; i < tn * p.top_k; i += kThreads) {
             const long long s = (long long)t0 * p.top_k + i;
             const int e = p.experts[s];
             if (e >= 0) p.places[s] += seen[(size_t)(i / p.top_k / p.per_warp) * E + e];
@@ -259,26 +297,33 @@ __global__ void __launch_bounds__(kRouteThreads) route_kernel(const RouteParams 
     }
 }
 
-// The second launch: every slot's place from its rank in its CTA and the counts of all CTAs.
-__global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteParams p) {
-    __shared__ int base[kRouteMaxExperts], part[kRouteWarps];
+// The second launch: every slot's place from its rank in its CTA and the counts of all CTAs. The counts of an expert are added
+// up by as many threads as there are for each (one thread per expert, going through all CTAs' counts alone: 10 us).
+__global__ void __launch_bounds__(kPlaceThreads) route_place_kernel(const RouteParams p) {
+    __shared__ int sums[2][kPlaceThreads], base[kRouteMaxExperts], part[kPlaceThreads / 32];
     pdl_wait_and_trigger();
-    const int E = p.n_experts;
-    int all[2] = {0, 0}, before[2] = {0, 0};
-    if (2 * (int)threadIdx.x < E) {
-        const bool two = 2 * (int)threadIdx.x + 1 < E;
-        for (int c = 0; c < (int)gridDim.x; ++c) {
-            const int* of = p.counts + (size_t)c * E + 2 * threadIdx.x;
-            const int a = of[0], b = two ? of[1] : 0;
-            all[0] += a;
-            all[1] += b;
-            before[0] += c < (int)blockIdx.x ? a : 0;
-            before[1] += c < (int)blockIdx.x ? b : 0;
+    const int E = p.n_experts, groups = kPlaceThreads / E, g = threadIdx.x / E, e = threadIdx.x - g * E;
+    if (g < groups) {
+        int all = 0, before = 0;
+#pragma unroll 8
+        for (int c = g; c < (int)gridDim.x; c += groups) {
+            const int n = p.counts[(size_t)c * E + e];
+            all += n;
+            before += c < (int)blockIdx.x ? n : 0;
         }
+        sums[0][threadIdx.x] = all;
+        sums[1][threadIdx.x] = before;
     }
-    find_bases(p, all, before, base, part, blockIdx.x == 0);
+    __syncthreads();
+    int all[1] = {0}, before[1] = {0};
+    if ((int)threadIdx.x < E)
+        for (int i = threadIdx.x; i < groups * E; i += E) {
+            all[0] += sums[0][i];
+            before[0] += sums[1][i];
+        }
+    find_bases<kPlaceThreads, 1>(p, all, before, base, part, blockIdx.x == 0);
     const int t0 = blockIdx.x * p.per_cta, tn = min(p.per_cta, p.tokens - t0);
-    for (int i = threadIdx.x; i < tn * p.top_k; i += kRouteThreads) {
+    for (int i = threadIdx.x; i < tn * p.top_k; i += kPlaceThreads) {
         const long long s = (long long)t0 * p.top_k + i;
         const int e = p.experts[s];
         if (e < 0) continue;
@@ -291,26 +336,27 @@ __global__ void __launch_bounds__(kRouteThreads) route_place_kernel(const RouteP
 template <int L, bool SIG>
 int launch_route(RouteParams& p, cudaStream_t st) {
     if (p.tokens <= kRouteClusterTokens) {
+        constexpr int W = kRouteWarps<true>;
         static std::atomic<unsigned long long> done{0};
         const auto fn = route_kernel<L, SIG, true>;
-        const int ctas = p.tokens <= kRouteWarps ? 1 : p.tokens < kRouteWarps * kRouteCluster ? (p.tokens + kRouteWarps - 1) / kRouteWarps
-                                                                                         : kRouteCluster;
+        const int ctas = p.tokens <= W ? 1 : p.tokens < W * kRouteCluster ? (p.tokens + W - 1) / W : kRouteCluster;
         p.per_cta = (p.tokens + ctas - 1) / ctas;
-        p.per_warp = (p.per_cta + kRouteWarps - 1) / kRouteWarps;
-        const size_t most = route_smem(kRouteMaxExperts, kRouteClusterTokens / kRouteCluster * kRouteMaxTopK);
+        p.per_warp = (p.per_cta + W - 1) / W;
+        const size_t most = route_smem<true>(kRouteMaxExperts, kRouteClusterTokens / kRouteCluster * kRouteMaxTopK);
         const int rc = serve_allow_smem((const void*)fn, most, done);
         if (rc) return rc;
-        return serve_launch(fn, p, dim3((unsigned)ctas), kRouteThreads, route_smem(p.n_experts, p.per_cta * p.top_k), st, ctas);
+        return serve_launch(fn, p, dim3((unsigned)ctas), W * 32, route_smem<true>(p.n_experts, p.per_cta * p.top_k), st, ctas);
     }
+    constexpr int W = kRouteWarps<false>;
     static std::atomic<unsigned long long> done{0};
     const auto fn = route_kernel<L, SIG, false>;
     const int ctas = sm_count() < kRouteMaxGrid ? sm_count() : kRouteMaxGrid;
     p.per_cta = (p.tokens + ctas - 1) / ctas;
-    p.per_warp = (p.per_cta + kRouteWarps - 1) / kRouteWarps;
+    p.per_warp = (p.per_cta + W - 1) / W;
     const dim3 grid((unsigned)((p.tokens + p.per_cta - 1) / p.per_cta));
-    int rc = serve_allow_smem((const void*)fn, route_smem(kRouteMaxExperts, 0), done);
-    if (!rc) rc = serve_launch(fn, p, grid, kRouteThreads, route_smem(p.n_experts, 0), st);
-    return rc ? rc : serve_launch(route_place_kernel, p, grid, kRouteThreads, 0, st);
+    int rc = serve_allow_smem((const void*)fn, route_smem<false>(kRouteMaxExperts, 0), done);
+    if (!rc) rc = serve_launch(fn, p, grid, W * 32, route_smem<false>(p.n_experts, 0), st);
+    return rc ? rc : serve_launch(route_place_kernel, p, grid, kPlaceThreads, 0, st);
 }
 
 template <bool SIG>

@@ -11,7 +11,8 @@ RMSNorm, scaled-dot-product attention, SiLU x up, residual adds).
 
 `PagedDecodeModel` is the same step for a batch of sequences of different lengths, as a server runs it: batched GEMVs,
 low-rank adapters per request, rotary positions and cache write in one pass (`serve.qkv_rope_cache`), attention over a
-paged cache (`serve.paged_attention`); lengths live on the device, so one captured graph decodes token after token.
+paged cache (`serve.paged_attention`), blocks of experts (`serve.route`, `serve.expert_matmul`, `serve.block_norm`); lengths
+live on the device, so one captured graph decodes token after token.
 """
 import torch
 import torch.nn.functional as F
@@ -214,16 +215,21 @@ class PagedDecodeModel:
     `max_len` positions (bf16, or float8_e4m3fn with a scale per kv head where cache="fp8"), the first lens[b] of them
     synthetic. step() decodes one token of every sequence at position lens[b], appends it and raises lens[b].
     adapters > 0: that many low-rank adapters of rank `rank` on the qkv, o, gate_up and down projections; self.adapter[b]
-    (int32, -1: none) names the one of sequence b. qk_norm: RMS norm of q and k per head before the rotation. A sequence
-    that is full must be retired by its caller; active[b] = False (self.active) makes row b padding: its cache and length
+    (int32, -1: none) names the one of sequence b. qk_norm: RMS norm of q and k per head before the rotation. experts > 0:
+    each layer's feed-forward block is that many experts of inner size `expert_inter`, weights in `kind` (bf16 or fp8), of
+    which every token takes its top_k (`scoring` as in serve.route); adapters are then on qkv and o, and the residual adds
+    and the norms (with post_norm those of the blocks' outputs too) are serve.block_norm. A sequence that is full must be retired by its caller; active[b] = False (self.active) makes row b padding: its cache and length
     stay, its logits are those of an empty context."""
 
     def __init__(self, lib, model, kind, lens, max_len=1024, page_size=16, cache="bf16", adapters=0, rank=16,
-                 qk_norm=False, layers=None, seed=0, dims=None):
+                 qk_norm=False, layers=None, seed=0, dims=None, experts=0, top_k=2, expert_inter=1024, scoring="softmax",
+                 post_norm=False):
         cfg = dict(MODELS[model])
         cfg.update(dims or {})
         if layers is not None:
             cfg["layers"] = layers
+        if experts and kind not in ("bf16", "fp8"):
+            raise ValueError(f"experts have bf16 or fp8 weights, not {kind}")
         if not lens or max(lens) >= max_len or min(lens) < 0:
             raise ValueError(f"lens must lie in [0, max_len = {max_len}), got {lens}")
         self.lib, self.cfg, self.kind, self.page_size, self.max_len = lib, cfg, kind, page_size, max_len
@@ -233,7 +239,9 @@ class PagedDecodeModel:
         dev = dict(device="cuda", dtype=torch.bfloat16)
         self.embed = (torch.randn(V, H, device="cuda", generator=g) * 0.02).to(torch.bfloat16)
         norm = lambda n: (1.0 + 0.1 * torch.randn(n, device="cuda", generator=g)).to(torch.bfloat16).float()   # noqa: E731
-        sizes = {"qkv": ((nh + 2 * nkv) * hd, H), "o": (H, nh * hd), "gate_up": (2 * I, H), "down": (H, I)}
+        sizes = {"qkv": ((nh + 2 * nkv) * hd, H), "o": (H, nh * hd)}
+        if not experts:
+            sizes.update(gate_up=(2 * I, H), down=(H, I))
         per_seq = -(-max_len // page_size)
         order = torch.randperm(B * per_seq, device="cuda", generator=g)
         self.page_table = order.view(B, per_seq).to(torch.int32)
@@ -254,6 +262,16 @@ class PagedDecodeModel:
             for name in ("k", "v"):
                 x = torch.randn(B * per_seq, page_size, nkv, hd, device="cuda", generator=g)
                 lay[name] = (x if cache == "bf16" else x * 32).to(dtype)
+            if experts:
+                lay["router"] = (torch.randn(experts, H, device="cuda", generator=g) / H ** 0.5).to(torch.bfloat16)
+                for name, n, k in (("experts_gate_up", 2 * expert_inter, H), ("experts_down", H, expert_inter)):
+                    w = torch.randn(experts, n, k, device="cuda", generator=g).mul_(0.02)
+                    if kind == "bf16":
+                        lay[name], lay[name + "_s"] = w.to(torch.bfloat16), None
+                    else:
+                        q, sc = quant.quantize_fp8_rowwise(w.view(experts * n, k))
+                        lay[name], lay[name + "_s"] = q.view(experts, n, k), sc.view(experts, n)
+                lay["post1"], lay["post2"] = (norm(H), norm(H)) if post_norm else (None, None)
             self.layers.append(lay)
         self.norm_f = norm(H)
         self.lm_head = Projection(lib, kind, V, H, g)
@@ -272,6 +290,13 @@ class PagedDecodeModel:
         self.h, self.a, self.o, self.d = (buf(H) for _ in range(4))
         self.qkv, self.gu, self.m, self.logits = buf((nh + 2 * nkv) * hd), buf(2 * I), buf(I), buf(V)
         self.q, self.attn = torch.zeros(B, nh, hd, **dev), torch.zeros(B, nh, hd, **dev)
+        self.experts, self.scoring = experts, scoring
+        if experts:
+            self.routing = serve.routing(lib, B, experts, top_k)
+            self.expert_workspace = serve.expert_workspace(lib)
+            self.router_logits = buf(experts)
+            self.mid = torch.zeros(B * top_k, expert_inter, **dev)
+            self.expert_out = torch.zeros(B * top_k, H, **dev)
 
     def _project(self, lay, name, x, y):
         """y = the projection of every row, plus the row's adapter."""
@@ -282,6 +307,20 @@ class PagedDecodeModel:
     def _rmsnorm(self, w, eps=1e-5):
         self.a.copy_(F.rms_norm(self.h.float(), (self.h.shape[1],), w, eps))
 
+    def _experts(self, lay, next_norm):
+        """The end of the attention block and the whole of the experts' one: h += o, a = norm2(h), each token's experts of a
+        and their weighted sum onto h, a = next_norm(h)."""
+        L, r, w = self.lib, self.routing, self.expert_workspace
+        serve.block_norm(L, self.h, self.o, self.h, out=self.a, post=lay["post1"], pre=lay["norm2"])
+        L.batched("bf16", lay["router"].data_ptr(), None, None, self.a.data_ptr(), None, self.router_logits.data_ptr(),
+                  self.batch, self.experts, self.cfg["hidden"])
+        serve.route(L, self.router_logits, r, scoring=self.scoring, positions=self.positions)
+        serve.expert_matmul(L, lay["experts_gate_up"], self.a, r.offsets, self.mid, w, scales=lay["experts_gate_up_s"],
+                            rows=r.rows, silu=True)
+        serve.expert_matmul(L, lay["experts_down"], self.mid, r.offsets, self.expert_out, w, scales=lay["experts_down_s"])
+        serve.block_norm(L, self.h, self.expert_out, self.h, out=self.a, places=r.places, weights=r.weights,
+                         post=lay["post2"], pre=next_norm)
+
     def step(self):
         """One token of every active sequence: reads self.token, writes self.logits and the argmax of each active row
         into self.token, appends to the cache and raises the lengths."""
@@ -289,8 +328,11 @@ class PagedDecodeModel:
         self.h.copy_(self.embed.index_select(0, self.token))
         torch.where(self.active, self.lens, self.padding, out=self.positions)      # padding rows: position -1, length 0
         torch.add(self.positions, 1, out=self.seen)
-        for lay in self.layers:
-            self._rmsnorm(lay["norm1"])
+        if self.experts:
+            serve.block_norm(self.lib, self.h, out=self.a, pre=self.layers[0]["norm1"])
+        for i, lay in enumerate(self.layers):
+            if not self.experts:
+                self._rmsnorm(lay["norm1"])
             self._project(lay, "qkv", self.a, self.qkv)
             serve.qkv_rope_cache(self.lib, self.qkv, self.positions, self.inv_freq, self.q, lay["k"], lay["v"],
                                  self.page_table, q_norm=lay["q_norm"], k_norm=lay["k_norm"], k_scale=self.k_scale,
@@ -298,13 +340,17 @@ class PagedDecodeModel:
             serve.paged_attention(self.lib, self.q, lay["k"], lay["v"], self.page_table, self.seen, self.attn,
                                   self.workspace, k_scale=self.k_scale, v_scale=self.v_scale)
             self._project(lay, "o", self.attn.view(self.batch, -1), self.o)
+            if self.experts:
+                self._experts(lay, self.layers[i + 1]["norm1"] if i + 1 < len(self.layers) else self.norm_f)
+                continue
             self.h.add_(self.o)
             self._rmsnorm(lay["norm2"])
             self._project(lay, "gate_up", self.a, self.gu)
             torch.mul(F.silu(self.gu[:, :I]), self.gu[:, I:], out=self.m)
             self._project(lay, "down", self.m, self.d)
             self.h.add_(self.d)
-        self._rmsnorm(self.norm_f)
+        if not self.experts:
+            self._rmsnorm(self.norm_f)
         self.lm_head.rows(self.a, self.logits)
         self.token.copy_(torch.where(self.active, torch.argmax(self.logits, 1), self.token))
         self.lens.add_(self.active)

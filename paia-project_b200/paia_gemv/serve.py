@@ -318,7 +318,7 @@ def route(lib, logits, routing, *, scoring="softmax", bias=None, renormalise=Tru
     sum of the chosen (renormalise) or of all; "sigmoid": ordered by sigmoid(l) + bias (fp32 [experts] or None), weights
     sigmoid(l), over the sum of the chosen where renormalise. positions (int32 [tokens], None: all live): rows below 0 are
     padding, with experts and places -1 and no place among the rows."""
-    if _bind is not None and hasattr(_bind, "route") and _bind.route(lib.route_entry, lib.device_entry, logits, routing.ptrs, routing.sizes, scoring, bias,
+    if _bind is not None and _bind.route(lib.route_entry, lib.device_entry, logits, routing.ptrs, routing.sizes, scoring, bias,
                                          renormalise, scale, positions, stream) == 0:
         return routing
     dev, ls = _device(logits, "logits"), _strides(logits)
@@ -364,7 +364,7 @@ def expert_matmul(lib, w, x, offsets, out, workspace, *, scales=None, rows=None,
     makes offsets and rows). w [experts, N, K] bf16, or e4m3 (float8_e4m3fn or its bytes as uint8) with scales fp32
     [experts, N]; x bf16 [rows, K]; rows int32 [M] (None: x[i]); out bf16 [M, N] (apart from x). silu: w[e] holds [gate; up]
     and out [M, N / 2] gets silu(gate x) * (up x). Rows of out that belong to no expert stay as they were."""
-    if _bind is not None and hasattr(_bind, "route") and _bind.expert_matmul(lib.expert_matmul_entry, lib.device_entry, w, x, offsets, out, workspace.ptr,
+    if _bind is not None and _bind.expert_matmul(lib.expert_matmul_entry, lib.device_entry, w, x, offsets, out, workspace.ptr,
                                                  workspace.device, scales, rows, silu, stream) == 0:
         return out
     dev, sw, xs, os = _device(x, "x"), _strides(w), _strides(x), _strides(out)
@@ -411,7 +411,7 @@ def block_norm(lib, h, x=None, h_out=None, *, out=None, places=None, weights=Non
     it is); out[t] = h_out[t] / sqrt(mean h_out[t]^2 + eps) * pre where out and pre (fp32 [hidden]) are given. h, x, h_out,
     out bf16 [.., hidden]; h_out may be h. gate bf16 [hidden], [tokens, 1] or [tokens, hidden]. Without x (and h_out): the
     norm of h alone."""
-    if _bind is not None and hasattr(_bind, "route") and _bind.block_norm(lib.block_norm_entry, lib.device_entry, h, x, h_out, out, places, weights, post,
+    if _bind is not None and _bind.block_norm(lib.block_norm_entry, lib.device_entry, h, x, h_out, out, places, weights, post,
                                               gate, scale, pre, eps, stream) == 0:
         return out if h_out is None else h_out
     dev, hs = _device(h, "h"), _strides(h)
