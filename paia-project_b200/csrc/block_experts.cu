@@ -19,7 +19,7 @@
 //            the last CTA to arrive joins them in the order of K (the same bits whichever it is); no CTA waits for another.
 // Every wait on a barrier is bounded; one that gives up sets code 15 and the CTA stops.
 #include "paia_gemv.h"
-#include "serve_tc5.cuh"
+#include "block_tc5.cuh"
 
 namespace pb2 {
 namespace {

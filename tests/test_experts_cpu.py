@@ -137,7 +137,7 @@ def code(name):
 def test_stream_order():
     """As every serving operator: each kernel waits for the one before it before anything that a caller may have written is
     read, lets the next one start only then, and asks for no load through the read-only path."""
-    for name in ("serve_route.cu", "serve_experts.cu", "serve_norm.cu"):
+    for name in ("block_route.cu", "block_experts.cu", "block_norm.cu"):
         src = code(name)
         kernels = [m.end() for m in re.finditer(r"__global__", src)]
         assert kernels and len(re.findall(r"\bpdl_wait_and_trigger\(\);", src)) == len(kernels), name
@@ -193,7 +193,7 @@ def walk(counts, tokens, row_tiles, units, grid, cg, min_run):
 
 
 def test_tiles_are_divided_once():
-    src = code("serve_experts.cu")
+    src = code("block_experts.cu")
     min_run = int(re.search(r"kExpMinRun = (\d+)", src).group(1))
     rng = random.Random(5)
     for _ in range(300):
@@ -230,3 +230,19 @@ def test_tiles_are_divided_once():
             assert blocks[0][0] == sum(counts[:ex]) and all(a + n == b for (a, n), (b, _) in zip(blocks, blocks[1:]))
             assert sum(n for _, n in blocks) == counts[ex]
         assert len(rows) == sum(c > 0 for c in counts) * row_tiles
+
+
+def test_registers():
+    """ptxas's report: nothing of the products' kernels spills, and a CTA's registers fit the SM at its size."""
+    from test_compile_report import load_reports
+    rows = [r for r in load_reports() if r["file"].startswith("block_")]
+    threads = {0: 384, 1: 384, 2: 896}                           # bf16, split, converted
+    seen = 0
+    for r in rows:
+        m = re.search(r"expert_kernelILi(\d)ELb(\d)ELi(\d)E", r["fn"])
+        if m:
+            seen += 1
+            assert r["regs"] * threads[int(m.group(1))] <= 65536 and r["spill_st"] + r["spill_ld"] <= 64, r
+        if "block_norm_kernel" in r["fn"] or "route_place" in r["fn"]:
+            assert r["spill_st"] == 0 and r["stack"] == 0, r
+    assert seen >= 8
