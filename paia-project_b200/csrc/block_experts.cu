@@ -70,7 +70,7 @@ struct ExpBars {
     uint64_t full[kExpMaxStages], empty[kExpMaxStages], peer[kExpMaxStages];
     uint64_t d[2], d_empty[2], a[4], a_empty[4], drained;
     uint32_t tmem;
-    int dead, last;
+    int dead, last[2];
     int part[32];
 };
 constexpr int kExpExchange = 2 * 4 * 8 * 32 * 4;     // [2][warp][column][lane] floats
@@ -95,6 +95,7 @@ struct ExpRing {
 // One run of units of one tile.
 struct ExpPart {
     int tile, e, row_tile, k0, k1;
+    int turn;                                        // a whole tile begins with this unit of K
     int row0, m;                                     // rows of out
 };
 
@@ -114,7 +115,7 @@ struct ExpWalk {
         // less than a round that keeps most CTAs busy: whole tiles, no joins
         else if (4 * cut >= 3 * g) cut = 0;
         work = cut * p.units;
-        workers = min(g, max(1, work / kExpMinRun));
+        workers = min(g, max(max(cut, 1), work / kExpMinRun));
         at = c < workers ? bound(c) : 0;
         end = c < workers ? bound(c + 1) : 0;
         next_whole = cut + c;
@@ -152,9 +153,16 @@ struct ExpWalk {
         const int per = round_up((all + blocks - 1) / blocks);
         s.row_tile = local / blocks;
         const int b = local - s.row_tile * blocks;
+        // CTAs that begin together would ask for the same place in rows of the same length all along (one token, 8 experts of
+        // 2048 x 4096 in bf16: 29.4 us, so 26.6); those that share rows of W should
+        s.turn = blocks == 1 && s.k1 - s.k0 == p.units ? s.tile * 13 % p.units : 0;
         s.row0 = off[lo] + b * per;
         s.m = min(per, all - b * per);
         return true;
+    }
+    __device__ __forceinline__ int unit(const ExpPart& s, int k) const {
+        k += s.turn;
+        return k < p.units ? k : k - p.units;
     }
     static __device__ __forceinline__ int round_up(int n) { return (n + 16 * CG - 1) & ~(16 * CG - 1); }
 };
@@ -320,8 +328,9 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     const uint32_t bar = bar_full + 8 * at.slot, to = ring + at.slot * stage;
                     bar_expect(bar, n * kExpUnit);
                     for (int u = 0; u < n; ++u) {
-                        if (SILU) tma_4d(to + u * kExpUnit, &p.w, (k + u) * K, y, 0, s.e, bar);
-                        else tma_3d(to + u * kExpUnit, &p.w, (k + u) * K, y, s.e, bar);
+                        const int from = walk.unit(s, k + u) * K;
+                        if (SILU) tma_4d(to + u * kExpUnit, &p.w, from, y, 0, s.e, bar);
+                        else tma_3d(to + u * kExpUnit, &p.w, from, y, s.e, bar);
                     }
                 }
             }
@@ -341,7 +350,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     const int n = XT * min(sub, s.k1 - k);
                     const uint32_t bar = bar_full + 8 * at.slot, to = ring + at.slot * stage + sub * kExpUnit;
                     bar_expect(bar, n * xb);
-                    for (int u = 0; u < n; ++u) tma_2d(to + u * xb, &p.x_map, k * K + K / XT * u, row, bar);
+                    for (int u = 0; u < n; ++u) tma_2d(to + u * xb, &p.x_map, walk.unit(s, k + u / XT) * K + K / XT * (u % XT), row, bar);
                 }
             }
         }
@@ -374,7 +383,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 const int n = XT * min(sub, s.k1 - k);
                 for (int u = 0; u < n; ++u) {
                     const uint32_t to = to0 + at.slot * stage + u * xb;
-                    const int from = k * K + 64 * u;
+                    const int from = walk.unit(s, k + u / XT) * K + 64 * (u % XT);
                     if (plain && from + 64 <= p.k) {
 #pragma unroll
                         for (int i = 0; i < 8; ++i)
@@ -484,18 +493,19 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     for (int i = 0; i < 16; ++i) to[(c + i) * kExpRows] = v[i];
                 }
                 release();
-                __threadfence();
+                // one thread's arrival releases what all of them, ahead of the barrier, have stored, and acquires what the
+                // other parts' threads had
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 if (row == 0) {
                     unsigned int* counter = p.counters + s.tile * CG + rank;
-                    const bool last = atomicAdd(counter, 1u) == (unsigned)(c1 - c0);
+                    unsigned int n;
+                    asm volatile("atom.add.acq_rel.gpu.global.u32 %0, [%1], 1;" : "=r"(n) : "l"(counter) : "memory");
+                    const bool last = n == (unsigned)(c1 - c0);
                     if (last) *counter = 0;
-                    bars.last = last;
+                    bars.last[tile & 1] = last;
                 }
                 asm volatile("bar.sync 1, 128;" ::: "memory");
-                mine = bars.last;
-                __threadfence();
-                asm volatile("bar.sync 1, 128;" ::: "memory");   // bars.last has been read
+                mine = bars.last[tile & 1];
             }
             if (mine) {
                 const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
@@ -510,10 +520,21 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                        for (int o = c0; o <= c1; ++o) {
-                            const float* from = p.parts + ((size_t)(walk.place(o, s.tile) * CG + rank) * cols + C * t) * kExpRows + row;
+                        constexpr int J = CONV ? 1 : 4;          // parts that are on their way together
+                        for (int o = c0; o <= c1; o += J) {
+                            float part[J][16];
 #pragma unroll
-                            for (int i = 0; i < 16; ++i) v[i] += __ldcg(from + i * kExpRows);
+                            for (int j = 0; j < J; ++j) {
+                                if (o + j > c1) continue;
+                                const float* from = p.parts + ((size_t)(walk.place(o + j, s.tile) * CG + rank) * cols + C * t) * kExpRows + row;
+#pragma unroll
+                                for (int i = 0; i < 16; ++i) part[j][i] = __ldcg(from + i * kExpRows);
+                            }
+#pragma unroll
+                            for (int j = 0; j < J; ++j)
+                                if (o + j <= c1)
+#pragma unroll
+                                    for (int i = 0; i < 16; ++i) v[i] += part[j][i];
                         }
                     }
                     if (FMT == kSplit)

@@ -164,7 +164,7 @@ def walk(counts, tokens, row_tiles, units, grid, cg, min_run):
     elif 4 * cut >= 3 * g:
         cut = 0
     work = cut * units
-    workers = min(g, max(1, work // min_run))
+    workers = min(g, max(cut, 1, work // min_run))
     bound = lambda c: c * work // workers                        # noqa: E731
     parts = []
     for c in range(g):
