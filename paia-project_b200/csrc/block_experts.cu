@@ -65,7 +65,8 @@ struct alignas(64) ExpertParams {
     int stages, sub;                                 // ring, units per stage
 };
 
-// Shared memory: ring of stages (their W, then their x), then the silu exchange, the barriers and three words per expert.
+// Shared memory: ring of stages (their W, then their x), then the silu exchange, where the gathered rows begin (a list per
+// gathering warp), the barriers and three words per expert.
 struct ExpBars {
     uint64_t full[kExpMaxStages], empty[kExpMaxStages], peer[kExpMaxStages];
     uint64_t d[2], d_empty[2], a[4], a_empty[4], drained;
@@ -74,7 +75,8 @@ struct ExpBars {
     int part[32];
 };
 constexpr int kExpExchange = 2 * 4 * 8 * 32 * 4;     // [2][warp][column][lane] floats
-constexpr size_t exp_fixed_smem(int experts) { return 1024 + kExpExchange + sizeof(ExpBars) + 12 * (size_t)(experts + 1); }
+constexpr int kExpLists = 4 * 128 * 8;
+constexpr size_t exp_fixed_smem(int experts) { return 1024 + kExpExchange + kExpLists + sizeof(ExpBars) + 12 * (size_t)(experts + 1); }
 
 // A place in a ring.
 struct ExpRing {
@@ -277,7 +279,8 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     const int sub = p.sub, cols = p.tokens * C, xb = cols / CG * 128;    // bytes of one tile of x
     const int stage = sub * (kExpUnit + XT * xb);
     float* exchange = reinterpret_cast<float*>(smem + (size_t)p.stages * stage);
-    ExpBars& bars = *reinterpret_cast<ExpBars*>(reinterpret_cast<uint8_t*>(exchange) + kExpExchange);
+    const __nv_bfloat16** lists = reinterpret_cast<const __nv_bfloat16**>(reinterpret_cast<uint8_t*>(exchange) + kExpExchange);
+    ExpBars& bars = *reinterpret_cast<ExpBars*>(reinterpret_cast<uint8_t*>(lists) + kExpLists);
     int* first = reinterpret_cast<int*>(&bars + 1);
     int* off = first + p.experts + 1;
     volatile int* dead = &bars.dead;
@@ -285,7 +288,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     const uint32_t rank = CG == 1 ? 0 : cluster_rank();
     if (threadIdx.x == 0) {
         for (int s = 0; s < p.stages; ++s) {
-            bar_init(sptr(&bars.full[s]), 1 + (p.rows ? 128 : 1));
+            bar_init(sptr(&bars.full[s]), 1 + (p.rows ? 32 : 1));
             bar_init(sptr(&bars.empty[s]), 1);
             bar_init(sptr(&bars.peer[s]), 1);
         }
@@ -355,50 +358,42 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             }
         }
     } else if (warp >= kExpGather && warp < kExpConverters && p.rows) {
-        // ---- x, gathered: a thread has 16-byte piece `piece` of rows r0 + 16 i
-        const int t = threadIdx.x - kExpGather * 32, r0 = t >> 3, piece = t & 7;
-        const uint32_t to0 = ring + sub * kExpUnit + r0 * 128 + ((piece ^ (r0 & 7)) << 4);
+        // ---- x, gathered: the four warps take the stages in turn, a lane 16-byte piece `piece` of rows r0 + 4 i. (Every lane's
+        // arrival takes its turn at the barrier: with all four warps on each stage, four times as many, a prompt over e4m3
+        // took 396 us, PROMPT now.)
+        const int mine = warp - kExpGather, r0 = lane >> 3, piece = lane & 7;
+        const __nv_bfloat16** list = lists + 128 * mine;         // nullptr: that row is nowhere: zeros
+        int turn = 0;
         while (ok && walk.next(s)) {
-            const int half = CG == 1 ? s.m : walk.round_up(s.m) / 2, skip = (int)rank * half, mine = min(half, s.m - skip);
-            const __nv_bfloat16* src[8];                         // (a row that is not in the block: any)
-            int gone = 0;                                        // bit i: row i is nowhere: zeros
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int r = r0 + 16 * i;
-                int from = 0;
-                if (r < mine) {
-                    from = p.rows[s.row0 + skip + r];
-                    if (from < 0 || from >= p.x_rows) {
-                        serve_error(kErrRouting);
-                        from = 0;
-                        gone |= 1 << i;
-                    }
-                }
-                src[i] = p.x + from * p.x_row + piece * 8;
+            const int half = CG == 1 ? s.m : walk.round_up(s.m) / 2, skip = (int)rank * half, rows = min(half, s.m - skip);
+            bool whole = true;
+            __syncwarp();
+            for (int r = lane; r < ((rows + 3) & ~3); r += 32) {
+                const int from = r < rows ? p.rows[s.row0 + skip + r] : 0;       // (behind the last: any)
+                const bool there = from >= 0 && from < p.x_rows;
+                if (!there) serve_error(kErrRouting);
+                whole &= there;
+                list[r] = there ? p.x + from * p.x_row : nullptr;
             }
-            const bool plain = !__any_sync(0xffffffffu, gone);
-            const int steps = (mine + 15) >> 4;
-            for (int k = s.k0; k < s.k1; k += sub) {
+            whole = __all_sync(0xffffffffu, whole);
+            for (int k = s.k0; k < s.k1; k += sub, at.step(), turn = (turn + 1) & 3) {
+                if (turn != mine) continue;
                 if (at.full && !(ok = __all_sync(0xffffffffu, bar_wait(bar_empty + 8 * at.slot, at.phase ^ 1u, dead)))) break;
                 const int n = XT * min(sub, s.k1 - k);
                 for (int u = 0; u < n; ++u) {
-                    const uint32_t to = to0 + at.slot * stage + u * xb;
-                    const int from = walk.unit(s, k + u / XT) * K + 64 * (u % XT);
-                    if (plain && from + 64 <= p.k) {
-#pragma unroll
-                        for (int i = 0; i < 8; ++i)
-                            if (i < steps) cp16(to + i * 2048, src[i] + from);
-                    } else {
-                        const bool in = from + piece * 8 < p.k;  // zeros behind the end of K
-#pragma unroll
-                        for (int i = 0; i < 8; ++i) {
-                            const bool got = in && !(gone >> i & 1);
-                            if (i < steps) cp16(to + i * 2048, got ? src[i] + from : p.x, got ? 16 : 0);
+                    const uint32_t to = ring + at.slot * stage + sub * kExpUnit + u * xb;
+                    const int from = walk.unit(s, k + u / XT) * K + 64 * (u % XT) + piece * 8;
+                    if (whole && from - piece * 8 + 64 <= p.k) {
+#pragma unroll 4
+                        for (int r = r0; r < rows; r += 4) cp16(to + r * 128 + ((piece ^ (r & 7)) << 4), list[r] + from);
+                    } else {                                     // zeros behind the end of K
+                        for (int r = r0; r < rows; r += 4) {
+                            const bool got = from < p.k && list[r];
+                            cp16(to + r * 128 + ((piece ^ (r & 7)) << 4), got ? list[r] + from : p.x, got ? 16 : 0);
                         }
                     }
                 }
                 cp_arrive(bar_full + 8 * at.slot);
-                at.step();
             }
         }
         cp_commit();
@@ -597,6 +592,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                         tc5_fence_before();
                         __syncwarp();
                         if (lane == 0) bar_arrive(bar_a + 8 * ab);
+                        __syncwarp();
                     }
                     if (++ab == T::kABufs) {
                         ab = 0;
