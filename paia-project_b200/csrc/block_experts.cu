@@ -63,6 +63,7 @@ struct alignas(64) ExpertParams {
     int units, row_tiles;                            // of K; tiles along n
     int tokens;                                      // columns per tile
     int stages, sub;                                 // ring, units per stage
+    int box;                                         // rows of x per copy, where they are in order
 };
 
 // Shared memory: ring of stages (their W, then their x), then the silu exchange, where the gathered rows begin (a list per
@@ -347,13 +348,17 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         // ---- x, rows in order
         if (!p.rows && elect_one()) {
             while (ok && walk.next(s)) {
-                const int row = C * s.row0 + (int)rank * (walk.round_up(s.m) / CG);
+                const int half = walk.round_up(s.m) / CG, row = C * s.row0 + (int)rank * half;
+                const int copies = (C * min(half, max(s.m - (int)rank * half, 1)) + p.box - 1) / p.box;
                 for (int k = s.k0; k < s.k1; k += sub, at.step()) {
                     if (at.full && !wait(bar_empty + 8 * at.slot, at.phase ^ 1u)) break;
                     const int n = XT * min(sub, s.k1 - k);
                     const uint32_t bar = bar_full + 8 * at.slot, to = ring + at.slot * stage + sub * kExpUnit;
-                    bar_expect(bar, n * xb);
-                    for (int u = 0; u < n; ++u) tma_2d(to + u * xb, &p.x_map, walk.unit(s, k + u / XT) * K + K / XT * (u % XT), row, bar);
+                    bar_expect(bar, n * copies * p.box * 128);
+                    for (int u = 0; u < n; ++u) {
+                        const int from = walk.unit(s, k + u / XT) * K + K / XT * (u % XT);
+                        for (int i = 0; i < copies; ++i) tma_2d(to + u * xb + i * p.box * 128, &p.x_map, from, row + i * p.box, bar);
+                    }
                 }
             }
         }
@@ -696,7 +701,7 @@ bool map_operands(ExpertParams& p, const void* x, long long x_row, int x_rows, c
     const cuuint64_t xes = FMT == kSplit ? 1 : 2;
     const cuuint64_t x_dims[2] = {(cuuint64_t)a->K, (cuuint64_t)x_rows};
     const cuuint64_t x_stride[1] = {x_rows > 1 ? (cuuint64_t)x_row * xes : ((cuuint64_t)a->K * xes + 15) / 16 * 16};
-    const cuuint32_t x_box[2] = {(cuuint32_t)(128 / xes), (cuuint32_t)(p.tokens * Exp<FMT, CG>::kCols / CG)};
+    const cuuint32_t x_box[2] = {(cuuint32_t)(128 / xes), (cuuint32_t)p.box};
     return fn(&p.x_map, FMT == kSplit ? CU_TENSOR_MAP_DATA_TYPE_UINT8 : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(x),
               x_dims, x_stride, x_box, one, CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
               CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS;
@@ -714,6 +719,9 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* ter
     p.stages = depth / p.sub < kExpMaxStages ? depth / p.sub : kExpMaxStages;
     if (p.stages < 2) return -2;
     const size_t smem = fixed + (size_t)p.stages * p.sub * unit;
+    // a copy of x brings as many rows as keep the copies few and what they bring in vain little
+    const int x_rows_cta = p.tokens * T::kCols / CG;
+    p.box = x_rows_cta <= 32 ? x_rows_cta : x_rows_cta <= 64 || x_rows_cta % 64 ? 32 : 64;
     p.units = (a->K + T::kK - 1) / T::kK;
     const int rows = CG * (SILU ? 64 : kExpRows);
     p.row_tiles = (p.n + rows - 1) / rows;
@@ -751,8 +759,8 @@ int pick_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* terms
         if (p.tokens <= 128) return launch_experts<kBf16W, SILU, 1>(p, a, terms, st);
         return launch_experts<kBf16W, SILU, 2>(p, a, terms, st);
     }
-    if (p.tokens <= kExpSplitTokens && (size_t)a->M * (4 * (size_t)a->K + 4) <= kExpSplitBytes)
-        return launch_experts<kSplit, SILU, 1>(p, a, terms, st);
+    if (want <= 2 * kExpSplitTokens && (size_t)a->M * (4 * (size_t)a->K + 4) <= kExpSplitBytes)
+        { p.tokens = p.tokens < kExpSplitTokens ? p.tokens : kExpSplitTokens; return launch_experts<kSplit, SILU, 1>(p, a, terms, st); }
     if (p.tokens <= 128) return launch_experts<kConverted, SILU, 1>(p, a, terms, st);
     p.tokens = 192;                                  // (converted W takes columns of tensor memory)
     return launch_experts<kConverted, SILU, 2>(p, a, terms, st);
