@@ -408,9 +408,12 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         // tells the first
         if (elect_one()) {
             const bool leader = rank == 0;
+            // every instruction here takes its latency from the products': places in the ring are kept as they are used
             const bool gathered = p.rows != nullptr;
-            int ab = 0;                                          // e4m3: buffer of converted W, its phase
-            uint32_t ap = 0;
+            const uint32_t lo0 = tc5_operand(ring), lo_step = (uint32_t)stage >> 4, x_off = (uint32_t)(sub * kExpUnit) >> 4,
+                           xb_lo = (uint32_t)xb >> 4, to_empty = bar_empty - bar_full, bar_end = bar_full + 8 * p.stages;
+            uint32_t lo = lo0, bar = bar_full, phase = 0, to_peer = bar_peer - bar_full;
+            uint32_t ab = 0, ap = 0;                             // e4m3: buffer of converted W, its phase
             for (int tile = 0; ok && walk.next(s); ++tile) {
                 const int buf = tile & 1;
                 if (leader && tile >= 2 && !wait(sptr(&bars.d_empty[buf]), (tile / 2 & 1) ^ 1u)) break;
@@ -418,31 +421,32 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 const uint32_t d = tmem + buf * cols;
                 const uint32_t shape = FMT == kSplit ? tc5_e4m3_shape<CG>((4 * s.m + 15) & ~15) : tc5_bf16_shape<CG>(walk.round_up(s.m));
                 uint32_t add = 0;
-                for (int k = s.k0; ok && k < s.k1; k += sub) {
-                    const int n = min(sub, s.k1 - k);
-                    const uint32_t w = ring + at.slot * stage;
-                    uint64_t wo = tc5_operand(w), xo = tc5_operand(w + sub * kExpUnit);
+                for (int left = s.k1 - s.k0; left > 0; left -= sub) {
+                    const int n = min(sub, left);
+                    uint32_t wo = lo, xo = lo + x_off;
                     for (int u = 0; u < n; ++u) {
                         if (CONV || u == 0) {
-                            const int i = CONV ? ab : at.slot;
-                            const uint32_t phase = CONV ? ap : at.phase;
-                            if (!wait((CONV ? bar_a : bar_full) + 8 * i, phase)) break;
+                            const uint32_t there = CONV ? bar_a + 8 * ab : bar, peer = CONV ? bar_peer + 8 * ab : bar + to_peer;
+                            const uint32_t ph = CONV ? ap : phase;
+                            if (!wait(there, ph)) break;
                             if (gathered) async_proxy_fence();
-                            if (CG == 2 && leader && !wait(bar_peer + 8 * i, phase)) break;
-                            if (CG == 2 && !leader) bar_arrive_at(bar_peer + 8 * i, 0);
+                            if (CG == 2 && leader && !wait(peer, ph)) break;
+                            if (CG == 2 && !leader) bar_arrive_at(peer, 0);
                             tc5_fence_after();
                         }
                         if (CG == 1 || leader) {
 #pragma unroll
-                            for (int j = 0; j < XT; ++j, xo += xb >> 4) {
+                            for (int j = 0; j < XT; ++j) {
 #pragma unroll
                                 for (int q = 0; q < 4; ++q) {
-                                    if (FMT == kBf16W) tc5_mma<CG>(d, wo + 2 * q, xo + 2 * q, shape, add);
-                                    else if (FMT == kSplit) tc5_mma_e4m3(d, wo + 2 * q, xo + 2 * q, shape, add);
-                                    else tc5_mma_t<CG>(d, tmem + T::kABase + 64 * ab + 32 * j + 8 * q, xo + 2 * q, shape, add);
-                                    add = 1;
+                                    const uint32_t on = j + q ? 1u : add;
+                                    if (FMT == kBf16W) tc5_mma<CG>(d, wo + 2 * q, xo + 2 * q, shape, on);
+                                    else if (FMT == kSplit) tc5_mma_e4m3(d, wo + 2 * q, xo + 2 * q, shape, on);
+                                    else tc5_mma_t<CG>(d, tmem + T::kABase + 64 * ab + 32 * j + 8 * q, xo + 2 * q, shape, on);
                                 }
+                                xo += xb_lo;
                             }
+                            add = 1;
                             wo += kExpUnit >> 4;
                             if (CONV) tc5_commit<CG>(bar_a_empty + 8 * ab);
                         }
@@ -451,8 +455,15 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                             ap ^= 1u;
                         }
                     }
-                    if (ok && leader) tc5_commit<CG>(bar_empty + 8 * at.slot);
-                    at.step();
+                    if (!ok) break;
+                    if (leader) tc5_commit<CG>(bar + to_empty);
+                    bar += 8;
+                    lo += lo_step;
+                    if (bar == bar_end) {
+                        bar = bar_full;
+                        lo = lo0;
+                        phase ^= 1u;
+                    }
                 }
                 if (ok && leader) tc5_commit<CG>(sptr(&bars.d[buf]));
             }
@@ -717,7 +728,7 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* ter
     // Few tokens: larger stages, for fewer waits.
     p.sub = depth >= 8 ? 2 : 1;
     p.stages = depth / p.sub < kExpMaxStages ? depth / p.sub : kExpMaxStages;
-    if (p.stages < 2) return -2;
+    if (p.stages < 4 && (p.rows || p.stages < 2)) return -2;     // (what the gathering warps' turns rely on)
     const size_t smem = fixed + (size_t)p.stages * p.sub * unit;
     // a copy of x brings as many rows as keep the copies few and what they bring in vain little
     const int x_rows_cta = p.tokens * T::kCols / CG;

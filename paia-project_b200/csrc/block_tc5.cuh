@@ -115,11 +115,10 @@ __device__ __forceinline__ void tc5_commit(uint32_t bar) {
                      :: "r"(bar) : "memory");
 }
 
-// A K-major operand of 64 16-bit values per row in shared memory, rows of 128 bytes with 16-byte pieces XOR-swizzled by
-// row & 7 (1024-byte atoms of 8 rows): a descriptor of its 16 values from byte 0; + 2 for the next 16.
-__device__ __forceinline__ uint64_t tc5_operand(uint32_t addr) {
-    return (uint64_t)(addr >> 4 & 0x3fff) | 1ull << 16 | (uint64_t)(1024 >> 4) << 32 | 1ull << 46 | 2ull << 61;
-}
+// A K-major operand of 128 bytes of K per row in shared memory, rows of 128 bytes with 16-byte pieces XOR-swizzled by row & 7
+// (1024-byte atoms of 8 rows): its descriptor's lower word (+ 2 for the next 32 bytes of K, + n / 16 for n bytes on) and upper.
+__device__ __forceinline__ uint32_t tc5_operand(uint32_t addr) { return (addr >> 4 & 0x3fff) | 1u << 16; }
+#define PB2_TC5_UPPER "1073758272"                   // 1024 >> 4 (bytes between atoms) | 1 << 14 | 2 << 29 (the swizzle)
 // bf16 x bf16 -> fp32, both K-major, 128 CG rows, n columns (a multiple of 16, of 32 for two CTAs, up to 256).
 template <int CG>
 __device__ __forceinline__ uint32_t tc5_bf16_shape(int n) {
@@ -131,29 +130,34 @@ __device__ __forceinline__ uint32_t tc5_e4m3_shape(int n) {
     return 1u << 4 | (uint32_t)(n >> 3) << 17 | (uint32_t)(CG * 128 >> 4) << 24;
 }
 // D (+)= A B of e4m3, 32 of K
-__device__ __forceinline__ void tc5_mma_e4m3(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
-    asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f8f6f4 [%0], %1, %2, %3, p;\n\t}"
-                 :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+__device__ __forceinline__ void tc5_mma_e4m3(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add) {
+    asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 a, {%1, " PB2_TC5_UPPER "};\n\tmov.b64 b, {%2, " PB2_TC5_UPPER "};\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f8f6f4 [%0], a, b, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "r"(b), "r"(shape), "r"(add) : "memory");
 }
 // D (+)= A B, A in shared memory
 template <int CG>
-__device__ __forceinline__ void tc5_mma(uint32_t d, uint64_t a, uint64_t b, uint32_t shape, uint32_t add) {
+__device__ __forceinline__ void tc5_mma(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add) {
     if (CG == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 a, {%1, " PB2_TC5_UPPER "};\n\tmov.b64 b, {%2, " PB2_TC5_UPPER "};\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], a, b, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "r"(b), "r"(shape), "r"(add) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], %1, %2, %3, p;\n\t}"
-                     :: "r"(d), "l"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 a, {%1, " PB2_TC5_UPPER "};\n\tmov.b64 b, {%2, " PB2_TC5_UPPER "};\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], a, b, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "r"(b), "r"(shape), "r"(add) : "memory");
 }
 // D (+)= A B, A in tensor memory (lane = row, a column holds two neighbours along K)
 template <int CG>
-__device__ __forceinline__ void tc5_mma_t(uint32_t d, uint32_t a, uint64_t b, uint32_t shape, uint32_t add) {
+__device__ __forceinline__ void tc5_mma_t(uint32_t d, uint32_t a, uint32_t b, uint32_t shape, uint32_t add) {
     if (CG == 1)
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                     :: "r"(d), "r"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 b, {%2, " PB2_TC5_UPPER "};\n\t"
+                     "tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "r"(b), "r"(shape), "r"(add) : "memory");
     else
-        asm volatile("{\n\t.reg .pred p;\n\tsetp.ne.u32 p, %4, 0;\n\ttcgen05.mma.cta_group::2.kind::f16 [%0], [%1], %2, %3, p;\n\t}"
-                     :: "r"(d), "r"(a), "l"(b), "r"(shape), "r"(add) : "memory");
+        asm volatile("{\n\t.reg .pred p;\n\t.reg .b64 a, b;\n\tsetp.ne.u32 p, %4, 0;\n\tmov.b64 b, {%2, " PB2_TC5_UPPER "};\n\t"
+                     "tcgen05.mma.cta_group::2.kind::f16 [%0], [%1], b, %3, p;\n\t}"
+                     :: "r"(d), "r"(a), "r"(b), "r"(shape), "r"(add) : "memory");
 }
 // 16 columns of the warp's 32 lanes: a row per lane
 __device__ __forceinline__ void tmem_load16(uint32_t addr, float v[16]) {
