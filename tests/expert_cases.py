@@ -90,10 +90,10 @@ def route(logits, top_k, scoring="softmax", bias=None, renormalise=True, scale=1
     score = l.clone() if scoring == "softmax" else 1 / (1 + torch.exp(-l))
     if bias is not None:
         score = score + bias.to(F64)
-    score = torch.where(torch.isnan(score), -torch.inf, score)
-    nan = torch.isnan(l)
-    order = [sorted(range(e), key=lambda j: (bool(nan[i, j]), -float(score[i, j]), j)) for i in range(t)]
-    ids = torch.tensor([o[:top_k] for o in order]).view(t, top_k)
+    nan = torch.isnan(score).cpu()
+    order = torch.sort(torch.where(nan, -torch.inf, score.cpu()), dim=1, descending=True, stable=True).indices
+    last = torch.sort(nan.gather(1, order).int(), dim=1, stable=True).indices
+    ids = order.gather(1, last)[:, :top_k].clone()
     chosen = l.cpu().gather(1, ids)
     if scoring == "softmax":
         top = chosen[:, :1]
@@ -109,12 +109,9 @@ def route(logits, top_k, scoring="softmax", bias=None, renormalise=True, scale=1
     if positions is not None:
         dead = positions.cpu() < 0
         w[dead], ids[dead] = 0, -1
-    places, rows, offsets = torch.full((t, top_k), -1), [], [0]
-    flat = ids.flatten().tolist()
-    for j in range(e):
-        for s, i in enumerate(flat):
-            if i == j:
-                places.view(-1)[s] = len(rows)
-                rows.append(s // top_k)
-        offsets.append(len(rows))
-    return w, ids, places, torch.tensor(rows, dtype=torch.int64), torch.tensor(offsets)
+    flat = ids.flatten()
+    slots = torch.sort(torch.where(flat < 0, e, flat), dim=0, stable=True).indices[:int((flat >= 0).sum())]
+    places = torch.full((t * top_k,), -1)
+    places[slots] = torch.arange(len(slots))
+    offsets = torch.cat([torch.zeros(1, dtype=torch.int64), torch.bincount(flat[flat >= 0], minlength=e).cumsum(0)])
+    return w, ids, places.view(t, top_k), slots // top_k, offsets
