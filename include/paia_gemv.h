@@ -352,10 +352,12 @@ int paia_gemv_route(const paia_gemv_route_args* a, void* stream);
 /* Products of grouped rows with their expert's weights W[e] [N][K]: for i in offsets[e] .. offsets[e + 1] - 1,
  *   out[i] = W[e] x[rows[i]]   (rows NULL: x[i]),  or with silu, W[e] = [gate; up] of N / 2 rows each:  silu(gate x) * (up x).
  * kind 0: W bf16; kind 1: W e4m3 with a fp32 scale per row, W[e][n] = scales[e][n] * stored. Products are exact, sums fp32,
- * out is rounded once to bf16; how K is divided follows from the whole call, and the same call gives the same bits. A NaN or
- * an infinity in a row of x or of W makes what it reaches NaN or infinite and nothing else. Rows of out that belong to no
- * expert stay as they were. An offset below the one before it or outside [0, M] cuts its group short and a row of x outside
- * [0, x_rows) reads as zeros (code 14); a bounded wait inside the kernel that gives up sets code 15. K is a multiple of 8
+ * out is rounded once to bf16. (kind 1 with up to 64 rows per expert on average: x enters as four e4m3 terms, exact down to
+ * 2^-26 of its row's largest; what is off below that is 2^-34 of the largest.) How K is divided follows from the whole call,
+ * and the same call gives the same bits. A NaN or an infinity in a row of x or of W makes what it reaches NaN or infinite and
+ * nothing else. Rows of out that belong to no expert stay as they were. An offset below the one before it or outside [0, M]
+ * cuts its group short and a row of x outside [0, x_rows) reads as zeros (code 14); a bounded wait inside the kernel that
+ * gives up sets code 15, out is then not to be used and the workspace to be zeroed. K is a multiple of 8
  * (kind 1: 16), experts <= 1024, M <= 2^28, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of
  * whole 16 bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed
  * once; every launch leaves it ready for the next, of any sizes; launches that may overlap on the GPU need one each. */
@@ -407,10 +409,10 @@ int paia_gemv_block_norm(const paia_gemv_block_norm_args* a, void* stream);
 int paia_gemv_current_device(void);
 
 /* Device-side error words of the current device: one of the GEMVs, set by kernels whose bounded waits gave up (codes below
- * 10), and one of each serving operator, set by the first bad index that it met in device memory (10 to 14; 15: a bounded wait of
- * paia_gemv_expert_matmul gave up). Returns the
- * first of them that is set (0 = none; -1: they cannot be read); clear != 0 resets that one alone, so calls until 0 return
- * them all. Synchronous; wait for the kernels in question first. */
+ * 10), and one of each serving operator, set by the first bad index that it met in device memory (10 to 14; 15: a
+ * bounded wait of paia_gemv_expert_matmul gave up). Returns the first of them that is set (0 = none; -1: they cannot be
+ * read); clear != 0 resets that one alone, so calls until 0 return them all. Synchronous; wait for the kernels in question
+ * first. */
 int paia_gemv_device_error(int clear);
 
 #ifdef __cplusplus

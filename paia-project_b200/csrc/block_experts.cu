@@ -18,6 +18,10 @@
 //            two rounds, is cut into equal runs of units. A tile cut by a run's end leaves its parts in the workspace and
 //            the last CTA to arrive joins them in the order of K (the same bits whichever it is); no CTA waits for another.
 // Every wait on a barrier is bounded; one that gives up sets code 15 and the CTA stops.
+// Measured: one token's 8 experts of 2048 x 4096 in bf16 26.4 us (5.1 TB/s; 4 of it the launch and what precedes the first
+// row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 82-85 (5.7 TB/s), 64 of 4096 x 1024 for 61 tokens 57-59; 8192 rows, 8
+// experts of 4096 x 14336 in bf16 790 (1.2 PFLOP/s, tensor pipe 79 % busy; in runs of seconds, under the power cap, 950);
+// 16384 rows, 64 experts of 2048 x 4096 in e4m3 350-410 (conversion and its hand-over to the products bound it).
 #include "paia_gemv.h"
 #include "block_tc5.cuh"
 
@@ -365,7 +369,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     } else if (warp >= kExpGather && warp < kExpConverters && p.rows) {
         // ---- x, gathered: the four warps take the stages in turn, a lane 16-byte piece `piece` of rows r0 + 4 i. (Every lane's
         // arrival takes its turn at the barrier: with all four warps on each stage, four times as many, a prompt over e4m3
-        // took 396 us, PROMPT now.)
+        // took 396 us, 379 now.)
         const int mine = warp - kExpGather, r0 = lane >> 3, piece = lane & 7;
         const __nv_bfloat16** list = lists + 128 * mine;         // nullptr: that row is nowhere: zeros
         int turn = 0;
@@ -551,10 +555,11 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     if (FMT == kSplit)
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
+                            // (in this order nothing passes fp32's range that the result does not pass)
                             const float f = t + i < s.m ? p.x_scale[s.row0 + t + i] : 0.f;
-                            v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * f;
+                            v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * scale * f;
                         }
-                    if (FMT != kBf16W)
+                    if (CONV)
 #pragma unroll
                         for (int i = 0; i < W; ++i) v[i] *= scale;
                     __nv_bfloat16* to = p.out + (long long)(s.row0 + t) * p.out_row + n;
@@ -633,10 +638,11 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
 struct SplitParams {
     const __nv_bfloat16* x;
     const int* rows;
+    const int* offsets;
     uint8_t* terms;
     float* scale;
     long long x_row;
-    int k, x_rows;
+    int k, x_rows, experts;
 };
 constexpr int kSplitThreads = 256;
 __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams p) {
@@ -645,7 +651,8 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams 
     const int i = blockIdx.x, from = p.rows ? p.rows[i] : i;
     uint8_t* to = p.terms + (size_t)i * 4 * p.k;
     const bool there = from >= 0 && from < p.x_rows;
-    if (!there && threadIdx.x == 0) serve_error(kErrRouting);
+    // (rows of out that belong to no expert may say anything here)
+    if (!there && threadIdx.x == 0 && i >= p.offsets[0] && i < p.offsets[p.experts]) serve_error(kErrRouting);
     const __nv_bfloat16* x = p.x + (there ? from * p.x_row : 0);
     uint32_t top = 0;                                            // the largest magnitude, as bits
     for (int c = threadIdx.x * 8; there && c < p.k; c += kSplitThreads * 8) {
@@ -741,7 +748,8 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* ter
     long long x_row = p.x_row;
     int x_rows = p.x_rows;
     if (FMT == kSplit) {
-        SplitParams q{p.x, p.rows, terms, reinterpret_cast<float*>(terms + (size_t)a->M * 4 * p.k), p.x_row, p.k, p.x_rows};
+        SplitParams q{p.x, p.rows, p.offsets, terms, reinterpret_cast<float*>(terms + (size_t)a->M * 4 * p.k), p.x_row, p.k, p.x_rows,
+                      p.experts};
         p.x_scale = q.scale;
         p.rows = nullptr;
         x = terms;
@@ -770,8 +778,12 @@ int pick_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* terms
         if (p.tokens <= 128) return launch_experts<kBf16W, SILU, 1>(p, a, terms, st);
         return launch_experts<kBf16W, SILU, 2>(p, a, terms, st);
     }
-    if (want <= 2 * kExpSplitTokens && (size_t)a->M * (4 * (size_t)a->K + 4) <= kExpSplitBytes)
-        { p.tokens = p.tokens < kExpSplitTokens ? p.tokens : kExpSplitTokens; return launch_experts<kSplit, SILU, 1>(p, a, terms, st); }
+    // e4m3: four columns per token where weights are what is waited for, conversion where products are (32 experts of 4096 x
+    // 2048, gathered rows, split / converted: 48 rows each 92 / 104 us, 64: 105 / 111, 96: 139 / 113).
+    if (want <= 2 * kExpSplitTokens && (size_t)a->M * (4 * (size_t)a->K + 4) <= kExpSplitBytes) {
+        p.tokens = p.tokens < kExpSplitTokens ? p.tokens : kExpSplitTokens;
+        return launch_experts<kSplit, SILU, 1>(p, a, terms, st);
+    }
     if (p.tokens <= 128) return launch_experts<kConverted, SILU, 1>(p, a, terms, st);
     p.tokens = 192;                                  // (converted W takes columns of tensor memory)
     return launch_experts<kConverted, SILU, 2>(p, a, terms, st);

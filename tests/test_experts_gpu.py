@@ -202,6 +202,42 @@ def test_rows_of_any_magnitude(L, ws, exponent):
 
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("tokens", [4, 100, 300])
+def test_rows_behind_the_groups_say_anything(L, ws, kind, tokens):
+    """What rows holds for places of no expert is not looked at."""
+    from paia_gemv import serve
+    g = gen(13)
+    off = C.groups([tokens, tokens], DEV) + 2
+    w, s, values = C.weights(2, 64, 128, kind, g, DEV)
+    x = torch.randn(tokens, 128, generator=g, device=DEV).to(C.BF16)
+    rows = torch.full((2 * tokens + 5,), 0x7FFFFFFF, dtype=torch.int32, device=DEV)
+    rows[2:2 * tokens + 2] = torch.arange(2 * tokens, device=DEV, dtype=torch.int32) % tokens
+    out = torch.full((2 * tokens + 5, 64), 7.0, dtype=C.BF16, device=DEV)
+    serve.expert_matmul(L, w, x, off, out, ws, scales=s, rows=rows)
+    live = slice(2, 2 * tokens + 2)
+    want, bound = C.matmul(values, x, off - 2, rows[live], split=kind == "fp8")
+    within(out[live], want, bound)
+    assert bool((out[:2] == 7.0).all()) and bool((out[2 * tokens + 2:] == 7.0).all())
+    assert L.device_error() == 0
+
+
+@pytest.mark.parametrize("xe,we", [(120, -120), (-120, 100), (60, 60)])
+def test_magnitudes_that_cancel(L, ws, xe, we):
+    """Rows of x and scales of W near both ends of fp32's range whose products lie well inside it."""
+    from paia_gemv import serve
+    g = gen(14)
+    for tokens in (3, 100, 200):
+        q = torch.randn(1, 64, 128, generator=g, device=DEV).to(C.E4M3)
+        s = torch.full((1, 64), 2.0 ** we, device=DEV)
+        x = (torch.randn(tokens, 128, generator=g, device=DEV).double() * 2.0 ** xe).to(C.BF16)
+        out = torch.zeros(tokens, 64, dtype=C.BF16, device=DEV)
+        off = C.groups([tokens], DEV)
+        serve.expert_matmul(L, q, x, off, out, ws, scales=s)
+        values = q.to(C.F64) * s.to(C.F64)[:, :, None]
+        within(out, *C.matmul(values, x, off, split=True))
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("tokens", [4, 100, 300])
 def test_bad_rows_and_offsets(L, ws, kind, tokens):
     """A row of x that is nowhere reads as zeros; groups out of order or range are cut short. Code 14 either way."""
     from paia_gemv import serve
