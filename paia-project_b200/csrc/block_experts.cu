@@ -483,6 +483,15 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         int step = 0;                                            // exchanges so far
         for (int tile = 0; ok && walk.next(s); ++tile) {
             const int buf = tile & 1;
+            // what the sums are multiplied by, on its way while they are made
+            const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
+            const int n = SILU ? y + (q & 1) * 32 + lane : y + row;
+            float scale = 1.f, x_scale[2] = {0.f, 0.f};          // of tokens lane and 32 + lane
+            if (FMT != kBf16W && n < p.n) scale = p.scales[s.e * p.scale_expert + n + (SILU && q >= 2 ? p.n : 0)];
+            if (FMT == kSplit)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+                    if (32 * i + lane < s.m) x_scale[i] = p.x_scale[s.row0 + 32 * i + lane];
             if (!(ok = all_of(__all_sync(0xffffffffu, bar_wait(sptr(&bars.d[buf]), tile / 2 & 1, dead))))) break;
             tc5_fence_after();
             const uint32_t d = tmem + buf * cols + ((uint32_t)(q * 32) << 16);
@@ -523,10 +532,6 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 mine = bars.last[tile & 1];
             }
             if (mine) {
-                const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
-                const int n = SILU ? y + (q & 1) * 32 + lane : y + row;
-                float scale = 1.f;
-                if (FMT != kBf16W && n < p.n) scale = p.scales[s.e * p.scale_expert + n + (SILU && q >= 2 ? p.n : 0)];
                 constexpr int W = 16 / C;                        // tokens per step
                 for (int t = 0; t < s.m; t += W) {
                     float v[16];
@@ -556,7 +561,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
                             // (in this order nothing passes fp32's range that the result does not pass)
-                            const float f = t + i < s.m ? p.x_scale[s.row0 + t + i] : 0.f;
+                            const float f = __shfl_sync(0xffffffffu, t < 32 ? x_scale[0] : x_scale[1], t + i & 31);
                             v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * scale * f;
                         }
                     if (CONV)
@@ -570,11 +575,11 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
 #pragma unroll
                         for (int i = 0; i < H; ++i) x[(q * 8 + i) * 32 + lane] = q < 2 ? v[H + i] : v[i];
                         asm volatile("bar.sync %0, 64;" :: "r"(2 + (q & 1)) : "memory");
-                        const float* y = x + (q ^ 2) * 8 * 32 + lane;
+                        const float* other = x + (q ^ 2) * 8 * 32 + lane;
 #pragma unroll
                         for (int i = 0; i < H; ++i) {
                             const int at = i + (q < 2 ? 0 : H);
-                            const float r = q < 2 ? silu_mul(v[i], y[i * 32]) : silu_mul(y[i * 32], v[H + i]);
+                            const float r = q < 2 ? silu_mul(v[i], other[i * 32]) : silu_mul(other[i * 32], v[H + i]);
                             if (t + at < s.m && n < p.n) to[at * p.out_row] = __float2bfloat16_rn(r);
                         }
                     } else {
