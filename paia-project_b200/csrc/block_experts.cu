@@ -733,6 +733,7 @@ bool map_operands(ExpertParams& p, const void* x, long long x_row, int x_rows, c
 template <int FMT, bool SILU, int CG>
 int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* terms, cudaStream_t st) {
     using T = Exp<FMT, CG>;
+    if (p.tokens % (16 * CG)) return -2;                         // a block's rows come in these
     const int unit = kExpUnit + T::kXTiles * (p.tokens * T::kCols / CG * 128);
     const size_t most = max_dyn_smem(), fixed = exp_fixed_smem(a->experts);
     if (most < fixed) return -2;
