@@ -237,7 +237,7 @@ __device__ void list_tiles(const ExpertParams& p, int* off, int* first, int* par
             const int e = 4 * t + i;
             lo[i] = hi[i] = tiles[i] = 0;
             if (e >= p.experts) continue;
-            const int a = p.offsets[e], b = p.offsets[e + 1];
+            const int a = __ldcg(p.offsets + e), b = __ldcg(p.offsets + e + 1);
             lo[i] = min(max(a, 0), p.m);
             hi[i] = max(lo[i], min(max(b, 0), p.m));
             bad |= a != lo[i] || b != hi[i];
@@ -315,7 +315,10 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     if (CG == 1) __syncthreads();
     else cluster_barrier();
     tc5_fence_after();
-    pdl_wait_and_trigger();
+    // Behind split_kernel only what it writes, the terms and their scales, has to be waited for: it lets this kernel start once
+    // it has waited itself, and so once everything ahead of it is done. (Offsets, rows of W and the workspace's counters are
+    // older than it.)
+    if (FMT != kSplit) pdl_wait_and_trigger();
     list_tiles(p, off, first, bars.part);
     const uint32_t tmem = bars.tmem;
     ExpWalk<CG> walk(p, off, first);
@@ -351,6 +354,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     } else if (warp == kExpX) {
         // ---- x, rows in order
         if (!p.rows && elect_one()) {
+            if (FMT == kSplit) pdl_wait_and_trigger();
             while (ok && walk.next(s)) {
                 const int half = walk.round_up(s.m) / CG, row = C * s.row0 + (int)rank * half;
                 const int copies = (C * min(half, max(s.m - (int)rank * half, 1)) + p.box - 1) / p.box;
@@ -479,6 +483,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         }
     } else if (warp >= kExpEpilogue && warp < kExpGather) {
         // ---- results
+        if (FMT == kSplit) pdl_wait_and_trigger();
         const int q = warp - kExpEpilogue, row = q * 32 + lane;
         int step = 0;                                            // exchanges so far
         for (int tile = 0; ok && walk.next(s); ++tile) {

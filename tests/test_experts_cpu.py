@@ -140,7 +140,10 @@ def test_stream_order():
     for name in ("block_route.cu", "block_experts.cu", "block_norm.cu"):
         src = code(name)
         kernels = [m.end() for m in re.finditer(r"__global__", src)]
-        assert kernels and len(re.findall(r"\bpdl_wait_and_trigger\(\);", src)) == len(kernels), name
+        # (expert_kernel behind its own split_kernel waits where it reads what that writes)
+        late = len(re.findall(r"if \(FMT == kSplit\) pdl_wait_and_trigger\(\);", src))
+        assert kernels and len(re.findall(r"\bpdl_wait_and_trigger\(\);", src)) == len(kernels) + late, name
+        assert late == (2 if name == "block_experts.cu" else 0)
         assert "griddepcontrol" not in src and not re.search(r"__ldg|\.nc\b|__restrict", src), name
         for at in kernels:
             head = src[at:][:src[at:].index("pdl_wait_and_trigger();")]
