@@ -355,8 +355,8 @@ int paia_gemv_route(const paia_gemv_route_args* a, void* stream);
  * out is rounded once to bf16. (kind 1 with up to 64 rows per expert on average: x enters as four e4m3 terms, exact down to
  * 2^-26 of its row's largest; what is off below that is 2^-34 of the largest.) How K is divided follows from the whole call,
  * and the same call gives the same bits. A NaN or an infinity in a row of x or of W makes what it reaches NaN or infinite and
- * nothing else. Rows of out that belong to no expert stay as they were. An offset below the one before it or outside [0, M]
- * cuts its group short and a row of x outside [0, x_rows) reads as zeros (code 14); a bounded wait inside the kernel that
+ * nothing else. Rows of out that belong to no expert stay as they were. With an offset below the one before it or outside
+ * [0, M] nothing is computed, a row of x outside [0, x_rows) reads as zeros (code 14); a bounded wait inside the kernel that
  * gives up sets code 15, out is then not to be used and the workspace to be zeroed. K is a multiple of 8
  * (kind 1: 16), experts <= 1024, M <= 2^28, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of
  * whole 16 bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed

@@ -19,7 +19,7 @@
 //            the last CTA to arrive joins them in the order of K (the same bits whichever it is); no CTA waits for another.
 // Every wait on a barrier is bounded; one that gives up sets code 15 and the CTA stops.
 // Measured: one token's 8 experts of 2048 x 4096 in bf16 26.4 us (5.1 TB/s; 4 of it the launch and what precedes the first
-// row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 82-85 (5.7 TB/s), 64 of 4096 x 1024 for 61 tokens 57-59; 8192 rows, 8
+// row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 79 (6.0 TB/s), 64 of 4096 x 1024 for 61 tokens 54; 8192 rows, 8
 // experts of 4096 x 14336 in bf16 790 (1.2 PFLOP/s, tensor pipe 79 % busy; in runs of seconds, under the power cap, 950);
 // 16384 rows, 64 experts of 2048 x 4096 in e4m3 350-410 (conversion and its hand-over to the products bound it).
 #include "paia_gemv.h"
@@ -162,7 +162,7 @@ struct ExpWalk {
         const int b = local - s.row_tile * blocks;
         // CTAs that begin together would ask for the same place in rows of the same length all along (one token, 8 experts of
         // 2048 x 4096 in bf16: 29.4 us, so 26.6); those that share rows of W should
-        s.turn = blocks == 1 && s.k1 - s.k0 == p.units ? s.tile * 13 % p.units : 0;
+        s.turn = blocks == 1 && s.k1 - s.k0 == p.units ? s.tile % p.units * 13 % p.units : 0;
         s.row0 = off[lo] + b * per;
         s.m = min(per, all - b * per);
         return true;
@@ -175,8 +175,8 @@ struct ExpWalk {
 };
 
 // Two e4m3 as bf16, exactly: with a byte of its sign above each (prmt), the exponent's field moves by a shift, and 2^120 makes
-// up for the bias (subnormals among them). Eight instructions on the integer pipe for four values took twice as long as the
-// stream from HBM; these are four.
+// up for the bias (subnormals among them): four instructions on the integer pipe for four values, where byte moves, shifts and
+// masks alone are eight.
 template <int SEL>
 __device__ __forceinline__ uint32_t e4m3x2_bf16(uint32_t w) {
     uint32_t t, r;
@@ -197,7 +197,7 @@ __device__ __forceinline__ void e4m3x16_bf16(uint32_t from, uint32_t r[8], uint3
     }
 }
 // 64 of a row (pieces first .. first + 3 of its eight) once more into the 32 columns at `to`, NaN where they are. Out of the
-// way: with it in the converting loop the loop no longer fitted where instructions are fetched from in time (128 against 123 us).
+// way: in line it kept the converting loop waiting for instructions (150 us, without it 123, at the time).
 __device__ __noinline__ void e4m3_row_with_nan(uint32_t row, uint32_t key, int first, uint32_t to) {
     uint32_t r[32];
 #pragma unroll
@@ -225,8 +225,8 @@ __device__ __forceinline__ bool all_of(bool ok) {
     return r != 0;
 }
 
-// first[e], off[e] (and at off[experts + 1 + e] its end) of every expert, by the first 256 threads; an offset that is out of
-// order or range cuts its group short.
+// first[e], off[e] (and at off[experts + 1 + e] its end) of every expert, by the first 256 threads; offsets that are out of
+// order or range make an empty list (their groups could overlap, and the tiles be more than an int counts).
 __device__ void list_tiles(const ExpertParams& p, int* off, int* first, int* part) {
     const int t = threadIdx.x;
     int lo[4], hi[4], tiles[4], sum = 0;
@@ -237,15 +237,18 @@ __device__ void list_tiles(const ExpertParams& p, int* off, int* first, int* par
             const int e = 4 * t + i;
             lo[i] = hi[i] = tiles[i] = 0;
             if (e >= p.experts) continue;
-            const int a = __ldcg(p.offsets + e), b = __ldcg(p.offsets + e + 1);
-            lo[i] = min(max(a, 0), p.m);
-            hi[i] = max(lo[i], min(max(b, 0), p.m));
-            bad |= a != lo[i] || b != hi[i];
-            tiles[i] = (hi[i] - lo[i] + p.tokens - 1) / p.tokens * p.row_tiles;
-            sum += tiles[i];
+            lo[i] = __ldcg(p.offsets + e);
+            hi[i] = __ldcg(p.offsets + e + 1);
+            bad |= lo[i] < 0 || hi[i] < lo[i] || hi[i] > p.m;
         }
         if (bad) serve_error(kErrRouting);
     }
+    if (!__syncthreads_or(bad) && t < 256)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            tiles[i] = (hi[i] - lo[i] + p.tokens - 1) / p.tokens * p.row_tiles;
+            sum += tiles[i];
+        }
     int s = sum;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {

@@ -239,7 +239,7 @@ def test_magnitudes_that_cancel(L, ws, xe, we):
 @pytest.mark.parametrize("kind", ["bf16", "fp8"])
 @pytest.mark.parametrize("tokens", [4, 100, 300])
 def test_bad_rows_and_offsets(L, ws, kind, tokens):
-    """A row of x that is nowhere reads as zeros; groups out of order or range are cut short. Code 14 either way."""
+    """A row of x that is nowhere reads as zeros; with offsets out of order or range nothing is computed. Code 14 either way."""
     from paia_gemv import serve
     g = gen(10)
     w, s, values = C.weights(2, 64, 128, kind, g, DEV)
@@ -256,12 +256,12 @@ def test_bad_rows_and_offsets(L, ws, kind, tokens):
     assert not out[1:3].any()
     torch.cuda.synchronize()
     assert L.device_error() == 14 and L.device_error() == 0
-    for bad in ([0, tokens + 50, tokens], [-3, 2, tokens], [tokens, 0, 2]):
+    for bad in ([0, tokens + 50, tokens], [-3, 2, tokens], [tokens, 0, 2], [0, 1, tokens + 1], [-2 ** 31, 2 ** 31 - 1, 0]):
         out.fill_(7.0)
         serve.expert_matmul(L, w, x, torch.tensor(bad, dtype=torch.int32, device=DEV), out, ws, scales=s)
         torch.cuda.synchronize()
         assert L.device_error() == 14 and L.device_error() == 0, bad
-        assert torch.isfinite(out.float()).all()
+        assert bool((out == 7.0).all())
 
 
 def test_offsets_past_32_bits(L, ws):
