@@ -32,7 +32,7 @@ constexpr int kExpMaxExperts = 1024;
 constexpr int kExpMaxGrid = 160;                     // the workspace holds two parts per CTA of the largest grid
 constexpr int kExpRows = 128;                        // of W per CTA and tile
 constexpr int kExpUnit = kExpRows * 128;             // bytes of W per unit: 128 of each row
-constexpr int kExpMinRun = 8;                        // units per CTA, at least, where a list is cut
+constexpr int kExpMinRun = 16;                       // units per CTA, at least, where a list is cut
 constexpr int kExpMaxStages = 12;
 constexpr int kExpX = 2, kExpEpilogue = 4, kExpGather = 8, kExpConverters = 12;      // first warps of the roles
 
@@ -122,7 +122,11 @@ struct ExpWalk {
         // less than a round that keeps most CTAs busy: whole tiles, no joins
         else if (4 * cut >= 3 * g) cut = 0;
         work = cut * p.units;
+        // Few tiles: the same number of CTAs for each, so that none has parts of two, and so many that a run is worth its join
+        // (one token, 2 experts of 2048 x 4096 in bf16: equal runs of at least 8 units 16.8 us, 16 13.9, 32 14.0; as here 14.1;
+        // 1 expert of 1024 x 8192: 14.2, 12.0, 12.6; 12.1; 8 of 1024 x 2048: 16.0, 13.7, 12.3; 13.8).
         workers = min(g, max(max(cut, 1), work / kExpMinRun));
+        if (rounds == 0 && cut) workers -= workers % cut;
         at = c < workers ? bound(c) : 0;
         end = c < workers ? bound(c + 1) : 0;
         next_whole = cut + c;

@@ -168,6 +168,8 @@ def walk(counts, tokens, row_tiles, units, grid, cg, min_run):
         cut = 0
     work = cut * units
     workers = min(g, max(cut, 1, work // min_run))
+    if rounds == 0 and cut:
+        workers -= workers % cut
     bound = lambda c: c * work // workers                        # noqa: E731
     parts = []
     for c in range(g):
