@@ -18,6 +18,7 @@
 // second launch places what the first has chosen and counted.
 // Measured: 1 token of 64 experts 3.0 us (2.3 is the launch), 250 of 256 experts under sigmoid 12.4, 8192 of 128 12.8.
 #include <cooperative_groups.h>
+#include <type_traits>
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 
@@ -26,6 +27,9 @@ namespace {
 
 template <bool ONE>
 constexpr int kRouteWarps = ONE ? 16 : 32;           // per CTA of the one-launch form, and of the other
+// A warp's slots of an expert, then those of the CTA's warps before it: 113000 and more where 2^24 tokens like the same one.
+template <bool ONE>
+using RouteCount = std::conditional_t<ONE, unsigned short, int>;
 constexpr int kPlaceThreads = 1024;
 constexpr int kRouteCluster = 8;                     // most CTAs of the one-launch form
 constexpr int kRouteClusterTokens = 256;            // (500 of 256 experts: 13.8 us here, 11 in two launches; 250: 9.2)
@@ -209,26 +213,27 @@ __device__ __forceinline__ void find_bases(const RouteParams& p, const int all[N
 
 template <bool ONE>
 constexpr size_t route_smem(int experts, int slots) {
-    return ((size_t)(kRouteWarps<ONE> * 2 + 2 * 4) * experts + 127) / 128 * 128 + 128 + (size_t)4 * slots;
+    return ((size_t)(kRouteWarps<ONE> * sizeof(RouteCount<ONE>) + 2 * 4) * experts + 127) / 128 * 128 + 128 + (size_t)4 * slots;
 }
 
-// per warp: counts [warps][experts] (16 bits); then the CTA's totals and bases [experts]; a word per warp; the slots
+// per warp: counts [warps][experts]; then the CTA's totals and bases [experts]; a word per warp; the slots
 template <int L, bool SIG, bool ONE>
 __global__ void __launch_bounds__(kRouteWarps<ONE> * 32) route_kernel(const RouteParams p) {
-    constexpr int kWarps = kRouteWarps<ONE>, kThreads = kWarps * 32;
+    using Count = RouteCount<ONE>;
+    constexpr int kWarps = kRouteWarps<ONE>, kThreads = kWarps * 32, kCounts = kWarps * sizeof(Count);
     extern __shared__ __align__(16) uint8_t smem[];
     const int E = p.n_experts, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    unsigned short* seen = reinterpret_cast<unsigned short*>(smem);
-    int* total = reinterpret_cast<int*>(smem + (size_t)kWarps * 2 * E);
+    Count* seen = reinterpret_cast<Count*>(smem);
+    int* total = reinterpret_cast<int*>(smem + (size_t)kCounts * E);
     int* base = total + E;
-    int* part = reinterpret_cast<int*>(smem + ((size_t)(kWarps * 2 + 8) * E + 127) / 128 * 128);
+    int* part = reinterpret_cast<int*>(smem + ((size_t)(kCounts + 8) * E + 127) / 128 * 128);
     int* slots = part + 32;                             // expert << 16 | rank; ONE only
-    for (int i = threadIdx.x; i < kWarps * E / 2; i += kThreads) reinterpret_cast<uint32_t*>(seen)[i] = 0u;
+    for (int i = threadIdx.x; i < kCounts / 4 * E; i += kThreads) reinterpret_cast<uint32_t*>(seen)[i] = 0u;
     __syncthreads();
     pdl_wait_and_trigger();
     const int t0 = blockIdx.x * p.per_cta, tn = min(p.per_cta, p.tokens - t0);
     const int first = min(warp * p.per_warp, tn), last = min(first + p.per_warp, tn);
-    unsigned short* mine = seen + (size_t)warp * E;
+    Count* mine = seen + (size_t)warp * E;
     for (int i = first; i < last; ++i) {
         const int t = t0 + i;
         float w = 0.f;
@@ -252,7 +257,7 @@ __global__ void __launch_bounds__(kRouteWarps<ONE> * 32) route_kernel(const Rout
 #pragma unroll
         for (int w = 0; w < kWarps; ++w) {
             const int c = seen[(size_t)w * E + e];
-            seen[(size_t)w * E + e] = (unsigned short)n;
+            seen[(size_t)w * E + e] = (Count)n;
             n += c;
         }
         total[e] = n;
