@@ -396,6 +396,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 list[r] = there ? p.x + from * p.x_row : nullptr;
             }
             whole = __all_sync(0xffffffffu, whole);
+            __syncwarp();                                        // (a vote orders no memory: each lane reads the others' entries)
             for (int k = s.k0; k < s.k1; k += sub, at.step(), turn = (turn + 1) & 3) {
                 if (turn != mine) continue;
                 if (at.full && !(ok = __all_sync(0xffffffffu, bar_wait(bar_empty + 8 * at.slot, at.phase ^ 1u, dead)))) break;
