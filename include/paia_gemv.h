@@ -323,12 +323,12 @@ int paia_gemv_lora(const paia_gemv_lora_args* a, void* stream);
 /* Token t's experts are the top_k of its `experts` logits (bf16 or fp32), in falling order, ties to the lowest index, NaN
  * last. scoring 0, softmax: ordered by the logits; weights scale e^l_j / sum of e^l over the chosen (renormalise) or over all
  * experts; 0 where every logit is -inf. scoring 1, sigmoid: ordered by s_e + bias[e], s = 1 / (1 + e^-l), in fp64; weights
- * scale s_j, over the sum of the chosen s where renormalise (0 where that sum is 0). Weights are fp32. The chosen (t, j),
- * numbered t top_k + j, are grouped by expert in the order of their numbers: expert e's stand at places offsets[e] ..
- * offsets[e + 1] - 1, places[t][j] is where (t, j) stands and rows[place] its token. A token with pos[t] < 0 is padding: it
- * has ids and places -1, weights 0 and no place. rows behind offsets[experts] stay as they were. experts <= 1024, top_k <=
- * 32, tokens <= 2^24. `workspace`: paia_gemv_route_workspace(experts) bytes, 16-byte aligned, of any content; calls that may
- * overlap on the GPU need one each. */
+ * scale s_j, over the sum of the chosen s where renormalise (0 where every chosen logit is -inf). Weights are fp32. The
+ * chosen (t, j), numbered t top_k + j, are grouped by expert in the order of their numbers: expert e's stand at places
+ * offsets[e] .. offsets[e + 1] - 1, places[t][j] is where (t, j) stands and rows[place] its token. A token with pos[t] < 0 is
+ * padding: it has ids and places -1, weights 0 and no place. rows behind offsets[experts] stay as they were. experts <= 1024,
+ * top_k <= 32, tokens <= 2^24. `workspace`: paia_gemv_route_workspace(experts) bytes, 16-byte aligned, of any content; calls
+ * that may overlap on the GPU need one each. */
 typedef struct paia_gemv_route_args {
     const void* logits;          /* [tokens][experts] */
     const float* bias;           /* [experts] or NULL; scoring 1 only */

@@ -1,9 +1,10 @@
 // Choosing each token's experts and grouping the tokens by expert (paia_gemv_route).
 //
 // softmax: a token's experts are those of its top_k largest logits; weights e^(l - m) over the chosen or over all.
-// sigmoid: ordered by s + bias, s = 1 / (1 + e^-l), as fp64 has it; weights s (/ their sum). fp32 decides where neighbours in
-// the order are further apart than it can be off, which is nearly always; else the token is done again in fp64 (250 tokens
-// of 256 experts, all of them in fp64: 18.4 us). Ties go to the lowest index in both.
+// sigmoid: ordered by s + bias, s = 1 / (1 + e^-l), as fp64 has it; weights s (/ their sum, as far below 0 as the logits may
+// lie: 0 where every chosen one is -inf). fp32 decides the order where neighbours in it are further apart than it can be off,
+// which is nearly always; else the token is done again in fp64 (250 tokens of 256 experts, all of them in fp64: 18.4 us). Ties
+// go to the lowest index in both.
 //
 // The chosen (token, place) pairs, "slots", are grouped by expert in the order of their numbers (token * top_k + place): the
 // same bits on every run, without atomics.
@@ -153,6 +154,13 @@ __device__ __forceinline__ int choose(const RouteParams& p, int t, int lane, flo
     const float got = on ? logit(p, t, mine) : 0.f;
     if constexpr (SIG) {
         w = on ? 1.f / (1.f + expf(-got)) : 0.f;
+        if (__any_sync(0xffffffffu, on && got < -60.f)) {
+            // s leaves fp32's range below -87, its share of the sum does not: s / e^c, with c the largest chosen logit where
+            // that is below 0 (in every token's way this took 1 to 2 us)
+            const float most = of_key(warp_max(on ? key_of(got) : 0u));
+            const float c = p.renorm && most < 0.f && most > -INFINITY ? most : 0.f;
+            if (on && got < 0.f) w = expf(got - c) / (1.f + expf(got));
+        }
         if (p.renorm) {
             const float s = warp_sum(w);
             w = s == 0.f ? 0.f : w / s;

@@ -41,3 +41,32 @@ def test_routes_of_several_tokens_per_warp(L, scoring, tokens, experts, top_k):
     pos[600:700] = -1
     route_case(L, logits, top_k, scoring=scoring)
     route_case(L, logits.to(C.BF16), top_k, scoring=scoring, positions=pos)
+
+
+def routes_far_below_zero(L, logits, bias=None):
+    """Order as C.route has it; shares of the sum by logarithms (e^-l alone is infinite in 64 bits from l = -710 on)."""
+    from paia_gemv import serve
+    r = serve.routing(L, *logits.shape, 8)
+    serve.route(L, logits, r, scoring="sigmoid", bias=bias)
+    ids = C.route(logits, 8, scoring="sigmoid", bias=bias)[1]
+    assert torch.equal(r.experts.cpu().long(), ids)
+    chosen = logits.cpu().double().gather(1, ids)
+    want = torch.softmax(torch.nn.functional.logsigmoid(chosen), 1)
+    want[torch.isneginf(chosen).all(1)] = 0
+    # exponentials of differences up to 200: 2^-16 of a weight (of smaller ones: nothing that fp32 holds)
+    assert bool(((r.weights.cpu().double() - want).abs() <= 2.0 ** -16 * want + 1e-37).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("level", [-85.0, -95.0, -200.0, -700.0])
+def test_sigmoid_weights_of_logits_far_below_zero(L, level, dtype):
+    """s itself leaves fp32's range; over the sum of the chosen it is an ordinary weight."""
+    g = gen(7)
+    logits = (level + 3 * torch.randn(20, 64, generator=g, device=DEV)).clamp(max=-80.0).to(dtype)
+    logits[11] = -float("inf")
+    logits[12, 3] = 1.0
+    routes_far_below_zero(L, logits)
+    route_case(L, logits, 8, scoring="sigmoid", scale=3.0, renormalise=False)
+    bias = torch.where(torch.arange(64, device=DEV) % 4 == 0, 2.0, 0.0)      # the chosen are not those of the largest s
+    near = torch.where(torch.arange(64, device=DEV) % 4 == 0, logits.float(), torch.randn(20, 64, generator=g, device=DEV))
+    routes_far_below_zero(L, near.to(dtype), bias)
