@@ -351,8 +351,8 @@ int paia_gemv_route(const paia_gemv_route_args* a, void* stream);
 
 /* Products of grouped rows with their expert's weights W[e] [N][K]: for i in offsets[e] .. offsets[e + 1] - 1,
  *   out[i] = W[e] x[rows[i]]   (rows NULL: x[i]),  or with silu, W[e] = [gate; up] of N / 2 rows each:  silu(gate x) * (up x).
- * kind 0: W bf16; kind 1: W e4m3 with a fp32 scale per row, W[e][n] = scales[e][n] * stored. Products are exact, sums fp32,
- * out is rounded once to bf16. (kind 1 with up to 64 rows per expert on average: x enters as four e4m3 terms, exact down to
+ * kind 0: W bf16; kind 1: W e4m3 with a fp32 scale per row, W[e][n] = scales[e][n] * stored. Products are exact, sums (of x
+ * with what W stores) fp32, infinite beyond its range; out is rounded once to bf16. (kind 1 with up to 64 rows per expert on average: x enters as four e4m3 terms, exact down to
  * 2^-26 of its row's largest; what is off below that is 2^-34 of the largest.) How K is divided follows from the whole call,
  * and the same call gives the same bits. A NaN or an infinity in a row of x or of W makes what it reaches NaN or infinite and
  * nothing else. Rows of out that belong to no expert stay as they were. With an offset below the one before it or outside

@@ -61,7 +61,7 @@ struct alignas(64) ExpertParams {
     __nv_bfloat16* out;
     unsigned int* counters;                          // one per cut tile and CTA of it: parts that have arrived
     float* parts;                                    // [2 grid][columns][128]
-    const float* x_scale;                            // split: [m], of each row's terms
+    const int* x_power;                              // split: [m], of two, of each row's terms
     long long x_row, out_row, scale_expert;
     int experts, n, m, k, x_rows;                    // n: rows of W_e (silu: of gate)
     int units, row_tiles;                            // of K; tiles along n
@@ -499,12 +499,13 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
             // what the sums are multiplied by, on its way while they are made
             const int y = (s.row_tile * CG + (int)rank) * (SILU ? 64 : kExpRows);
             const int n = SILU ? y + (q & 1) * 32 + lane : y + row;
-            float scale = 1.f, x_scale[2] = {0.f, 0.f};          // of tokens lane and 32 + lane
+            float scale = 1.f;
+            int x_power[2] = {0, 0};                             // of tokens lane and 32 + lane
             if (FMT != kBf16W && n < p.n) scale = p.scales[s.e * p.scale_expert + n + (SILU && q >= 2 ? p.n : 0)];
             if (FMT == kSplit)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
-                    if (32 * i + lane < s.m) x_scale[i] = p.x_scale[s.row0 + 32 * i + lane];
+                    if (32 * i + lane < s.m) x_power[i] = p.x_power[s.row0 + 32 * i + lane];
             if (!(ok = all_of(__all_sync(0xffffffffu, bar_wait(sptr(&bars.d[buf]), tile / 2 & 1, dead))))) break;
             tc5_fence_after();
             const uint32_t d = tmem + buf * cols + ((uint32_t)(q * 32) << 16);
@@ -573,9 +574,12 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     if (FMT == kSplit)
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
-                            // (in this order nothing passes fp32's range that the result does not pass)
-                            const float f = __shfl_sync(0xffffffffu, t < 32 ? x_scale[0] : x_scale[1], t + i & 31);
-                            v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * scale * f;
+                            // x's power of two up to 2^80 or down to 2^-80 ahead of W's scale, the rest behind it: sums lie between
+                            // 2^-34 and 2^37, so that nothing on the way passes fp32's range that the result does not pass
+                            const int power = __shfl_sync(0xffffffffu, t < 32 ? x_power[0] : x_power[1], t + i & 31);
+                            const int ahead = max(-80, min(power, 80));
+                            const float f0 = __int_as_float((ahead + 127) << 23), f1 = __int_as_float((power - ahead + 127) << 23);
+                            v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * f0 * scale * f1;
                         }
                     if (CONV)
 #pragma unroll
@@ -650,15 +654,15 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     }
 }
 
-// x of every row of out, in their order, as four e4m3 terms of 128-byte aligned rows [m][4][k] and a power of two by which
-// they are to be multiplied: v = x / scale lies below 256, and v = t0 + t1 + 2^-16 (t2 + t3), each term the nearest to what is
+// x of every row of out, in their order, as four e4m3 terms [m][4][k] and the exponent of the power of two by which they are to
+// be multiplied: v = x / 2^power lies below 256, and v = t0 + t1 + 2^-16 (t2 + t3), each term the nearest to what is
 // left. A row that holds a NaN or an infinity is NaN, one that is not there zero.
 struct SplitParams {
     const __nv_bfloat16* x;
     const int* rows;
     const int* offsets;
     uint8_t* terms;
-    float* scale;
+    int* power;
     long long x_row;
     int k, x_rows, experts;
 };
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams 
     const bool bad = top >= 0x7f80u;
     const int e = bad || top == 0 ? 7 : max((int)(top >> 7), 1) - 127, f = 7 - e;
     const float f0 = ldexpf(1.f, f / 2), f1 = ldexpf(1.f, f - f / 2);
-    if (threadIdx.x == 0) p.scale[i] = ldexpf(1.f, -f);
+    if (threadIdx.x == 0) p.power[i] = -f;
     for (int c = threadIdx.x * 8; c < p.k; c += kSplitThreads * 8) {
         uint4 v = make_uint4(0, 0, 0, 0);
         if (there) v = *reinterpret_cast<const uint4*>(x + c);
@@ -767,9 +771,9 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* ter
     long long x_row = p.x_row;
     int x_rows = p.x_rows;
     if (FMT == kSplit) {
-        SplitParams q{p.x, p.rows, p.offsets, terms, reinterpret_cast<float*>(terms + (size_t)a->M * 4 * p.k), p.x_row, p.k, p.x_rows,
+        SplitParams q{p.x, p.rows, p.offsets, terms, reinterpret_cast<int*>(terms + (size_t)a->M * 4 * p.k), p.x_row, p.k, p.x_rows,
                       p.experts};
-        p.x_scale = q.scale;
+        p.x_power = q.power;
         p.rows = nullptr;
         x = terms;
         x_row = p.k;

@@ -70,3 +70,27 @@ def test_sigmoid_weights_of_logits_far_below_zero(L, level, dtype):
     bias = torch.where(torch.arange(64, device=DEV) % 4 == 0, 2.0, 0.0)      # the chosen are not those of the largest s
     near = torch.where(torch.arange(64, device=DEV) % 4 == 0, logits.float(), torch.randn(20, 64, generator=g, device=DEV))
     routes_far_below_zero(L, near.to(dtype), bias)
+
+
+# ------------------------------------------------------------------ products
+
+@pytest.mark.parametrize("tokens", [3, 100, 200])
+@pytest.mark.parametrize("xe,we,size", [(-120, 115, 64.0), (120, -147, 0.02), (-126, 120, 100.0), (126, -149, 1.0)])
+def test_magnitudes_beyond_fp32_half_way(L, ws, xe, we, size, tokens):
+    """Rows of x and scales of W so far apart that a sum of W's stored values, times either alone, would leave fp32's range."""
+    from paia_gemv import serve
+    g = gen(15)
+    q = (size * torch.randn(1, 64, 128, generator=g, device=DEV)).clamp(-448, 448).to(C.E4M3)
+    s = torch.full((1, 64), 2.0 ** we, device=DEV)
+    x = (torch.randn(tokens, 128, generator=g, device=DEV).clamp(-3, 3).double() * 2.0 ** xe).to(C.BF16)
+    out = torch.zeros(tokens, 64, dtype=C.BF16, device=DEV)
+    off = C.groups([tokens], DEV)
+    serve.expert_matmul(L, q, x, off, out, ws, scales=s)
+    want, bound = C.matmul(q.to(C.F64) * s.to(C.F64)[:, :, None], x, off)
+    if tokens > 64:
+        # W meets x as bf16, and sums of x with what W stores are fp32's: where products of one sign (or those whose order is
+        # the kernel's own) may add up to 2^128, which they do for x of 2^126, a sum may be infinite or NaN
+        fits = x.to(C.F64).abs() @ q[0].to(C.F64).abs().T < 2.0 ** 128
+        assert bool(fits.all()) == (xe < 126)
+        out, want, bound = out[fits], want[fits], bound[fits]
+    within(out, want, bound)
