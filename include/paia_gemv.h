@@ -352,15 +352,15 @@ int paia_gemv_route(const paia_gemv_route_args* a, void* stream);
 /* Products of grouped rows with their expert's weights W[e] [N][K]: for i in offsets[e] .. offsets[e + 1] - 1,
  *   out[i] = W[e] x[rows[i]]   (rows NULL: x[i]),  or with silu, W[e] = [gate; up] of N / 2 rows each:  silu(gate x) * (up x).
  * kind 0: W bf16; kind 1: W e4m3 with a fp32 scale per row, W[e][n] = scales[e][n] * stored. Products are exact, sums (of x
- * with what W stores) fp32, infinite beyond its range; out is rounded once to bf16. (kind 1 with up to 64 rows per expert on average: x enters as four e4m3 terms, exact down to
- * 2^-26 of its row's largest; what is off below that is 2^-34 of the largest.) How K is divided follows from the whole call,
- * and the same call gives the same bits. A NaN or an infinity in a row of x or of W makes what it reaches NaN or infinite and
- * nothing else. Rows of out that belong to no expert stay as they were. With an offset below the one before it or outside
- * [0, M] nothing is computed, a row of x outside [0, x_rows) reads as zeros (code 14); a bounded wait inside the kernel that
- * gives up sets code 15, out is then not to be used and the workspace to be zeroed. K is a multiple of 8
- * (kind 1: 16), experts <= 1024, M <= 2^28, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of
- * whole 16 bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed
- * once; every launch leaves it ready for the next, of any sizes; launches that may overlap on the GPU need one each. */
+ * with what W stores) fp32, infinite beyond its range; out is rounded once to bf16. (kind 1 with few rows per expert: x enters
+ * as four e4m3 terms; what they leave out of a row is added wherever it may be 2^-18 of a sum.) How K is divided follows from
+ * the whole call, and the same call gives the same bits. A NaN or an infinity in a row of x or of W makes what it reaches NaN
+ * or infinite and nothing else. Rows of out that belong to no expert stay as they were. With an offset below the one before it
+ * or outside [0, M] nothing is computed, a row of x outside [0, x_rows) reads as zeros (code 14); a bounded wait inside the
+ * kernel that gives up sets code 15, out is then not to be used and the workspace to be zeroed. K is a multiple of 8 (kind 1:
+ * 16), experts <= 1024, M <= 2^28, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of whole 16
+ * bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed once; every
+ * launch leaves it ready for the next, of any sizes; launches that may overlap on the GPU need one each. */
 typedef struct paia_gemv_expert_args {
     const void* w;               /* [experts][N][K] */
     const float* scales;         /* [experts][N]; kind 1 only */

@@ -11,7 +11,7 @@
 //            gather of four rows took 58 cycles each). A ring of as many stages of one or more units as shared memory holds.
 //   math     bf16 x bf16 in fp32 accumulators in tensor memory, two tiles' worth, so that one is stored while the next is
 //            summed. e4m3 with few tokens: the bytes as they are, and x as four e4m3 terms (split_kernel), each a column of
-//            its own: x is exact down to 2^-26 of its row's largest, what is off below that is 2^-34 of it. With many: W
+//            its own, exact down to 2^-25 of a row's largest; the rest is added to sums beside which it counts. With many: W
 //            becomes bf16 exactly, in registers, and meets x from tensor memory. Its row's scale is applied to the sum.
 //   split    The launch does not know the groups. All tiles form one list (expert, rows of W, block of tokens) that every
 //            CTA finds from the offsets. Whole rounds of one tile per CTA are taken as they come; what is left over, up to
@@ -22,6 +22,7 @@
 // row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 79 (6.0 TB/s), 64 of 4096 x 1024 for 61 tokens 54; 8192 rows, 8
 // experts of 4096 x 14336 in bf16 790 (1.2 PFLOP/s, tensor pipe 79 % busy; in runs of seconds, under the power cap, 950);
 // 16384 rows, 64 experts of 2048 x 4096 in e4m3 350-410 (conversion and its hand-over to the products bound it).
+#include <type_traits>
 #include "paia_gemv.h"
 #include "block_tc5.cuh"
 
@@ -39,7 +40,9 @@ constexpr int kExpX = 2, kExpEpilogue = 4, kExpGather = 8, kExpConverters = 12; 
 // How W meets x. bf16: both are; split: e4m3 W as it is, x as four e4m3 terms; converted: e4m3 W as bf16.
 enum { kBf16W, kSplit, kConverted };
 constexpr int kExpSplitTokens = 64;                  // per block
-constexpr size_t kExpSplitBytes = 48 << 20;          // of the workspace
+constexpr size_t kExpSplitBytes = 48 << 20;          // of the workspace: 4 K + 4 bytes per row
+// and a word per 256 of K: at most K / 64 + 4 bytes for 4 K of terms, with no more rows than 64 of every expert
+constexpr size_t kExpApartBytes = kExpSplitBytes / 256 + (size_t)4 * kExpSplitTokens * kExpMaxExperts;
 
 // CG CTAs per tile.
 template <int FMT, int CG>
@@ -61,7 +64,13 @@ struct alignas(64) ExpertParams {
     __nv_bfloat16* out;
     unsigned int* counters;                          // one per cut tile and CTA of it: parts that have arrived
     float* parts;                                    // [2 grid][columns][128]
-    const int* x_power;                              // split: [m], of two, of each row's terms
+    // split, by row of out: what its terms are to be multiplied by and what of x they leave out (split_kernel), where x has it
+    const int* x_power;
+    const uint32_t* apart;
+    const int* x_from;
+    const uint8_t* w_at;                             // (W itself; the products read it through the map)
+    long long w_expert, w_row;
+    int words;
     long long x_row, out_row, scale_expert;
     int experts, n, m, k, x_rows;                    // n: rows of W_e (silu: of gate)
     int units, row_tiles;                            // of K; tiles along n
@@ -213,6 +222,87 @@ __device__ __noinline__ void e4m3_row_with_nan(uint32_t row, uint32_t key, int f
         if ((w & 0x7f00) == 0x7f00) r[i] = (r[i] & 0xffffu) | 0x7fff0000u;
     }
     tmem_store32(to, r);
+}
+
+// v's four e4m3 terms, v = t0 + t1 + 2^-16 (t2 + t3), each the nearest to what is left, of two values at once (in the low and the
+// high byte): what is left behind them, times 2^16, stays in a and b.
+__device__ __forceinline__ void split_terms(float& a, float& b, uint16_t term[4]) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+        if (t == 2) { a *= 0x1p16f; b *= 0x1p16f; }
+        uint32_t h;
+        asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(term[t]) : "f"(b), "f"(a));
+        asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(term[t]));
+        const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
+        a -= back.x;
+        b -= back.y;
+    }
+}
+// 2^-power in two factors, since the whole may pass fp32's range
+__device__ __forceinline__ float2 split_factors(int power) {
+    return make_float2(ldexpf(1.f, -power / 2), ldexpf(1.f, -power - -power / 2));
+}
+
+// A sum of terms times 2^power and W's scale: up to 2^80 or down to 2^-80 of the power ahead of the scale, the rest behind it. Sums
+// lie between 2^-34 and 2^37, so that nothing on the way passes fp32's range that the result does not pass.
+__device__ __forceinline__ float scaled_sum(float sum, int power, float scale) {
+    const int ahead = max(-80, min(power, 80));
+    return sum * __int_as_float((ahead + 127) << 23) * scale * __int_as_float((power - ahead + 127) << 23);
+}
+
+// The same for the row x of out's row `at`, whose terms leave something out, and each lane's row n of expert e's W (`on`: there is
+// one): where that may count, it is added, in fp32 and in an order that depends on nothing else. The whole warp takes one row of
+// W at a time, a marked group of 8 along K per lane.
+__device__ __noinline__ float with_rest(const ExpertParams& p, float sum, int code, float scale, int e, int n, bool on, int at) {
+    const int lane = threadIdx.x & 31, words = p.words, power = code >> 8, from = p.x_from ? p.x_from[at] : at;
+    const __nv_bfloat16* x = p.x + from * p.x_row;
+    const uint32_t* apart = p.apart + (size_t)at * words;
+    const float2 f = split_factors(power);
+    // beside a sum of this or more all that the terms leave out is less than 2^-18 of it
+    const float enough = __int_as_float(((code & 255) - 1) << 23);
+    float more = 0.f;                                            // of what has no terms at all
+    for (uint32_t todo = __ballot_sync(0xffffffffu, on && fabsf(sum) < enough); todo; todo &= todo - 1) {
+        const int to = __ffs(todo) - 1;
+        const uint8_t* w = p.w_at + e * p.w_expert + (n - lane + to) * p.w_row;
+        float left = 0.f, apart_left = 0.f;
+        for (int i0 = 0; i0 < words; i0 += 32) {
+            const uint32_t marks = i0 + lane < words ? apart[i0 + lane] : 0u;
+            for (uint32_t some = __ballot_sync(0xffffffffu, marks != 0); some; some &= some - 1) {
+                const int i = __ffs(some) - 1;
+                if (!(__shfl_sync(0xffffffffu, marks, i) >> lane & 1)) continue;
+                const int c = (i0 + i) * 256 + lane * 8;
+                const uint4 v = *reinterpret_cast<const uint4*>(x + c);
+                const uint2 u = *reinterpret_cast<const uint2*>(w + c);
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+                    uint32_t h[2];
+                    uint16_t term[4];
+                    e4m3x4_f16x4(j < 2 ? u.x : u.y, h[0], h[1]);
+                    const float2 by = __half22float2(*reinterpret_cast<const __half2*>(&h[j & 1]));
+                    const float x0 = bf16_lo((&v.x)[j]), x1 = bf16_hi((&v.x)[j]);
+                    float a = x0 * f.x * f.y, b = x1 * f.x * f.y;
+                    // (what has no terms may be infinite, or too small for fp32 beside the row's largest)
+                    const bool none0 = !(fabsf(a) > 0x1p-26f && fabsf(a) < 256.f), none1 = !(fabsf(b) > 0x1p-26f && fabsf(b) < 256.f);
+                    split_terms(a, b, term);
+                    if (none0) apart_left = fmaf(by.x, x0, apart_left);
+                    else left = fmaf(by.x, a, left);
+                    if (none1) apart_left = fmaf(by.y, x1, apart_left);
+                    else left = fmaf(by.y, b, left);
+                }
+            }
+            __syncwarp();
+        }
+#pragma unroll
+        for (int o = 16; o; o >>= 1) {
+            left += __shfl_xor_sync(0xffffffffu, left, o);
+            apart_left += __shfl_xor_sync(0xffffffffu, apart_left, o);
+        }
+        if (lane == to) {
+            sum += left * 0x1p-16f;
+            more = apart_left * scale;
+        }
+    }
+    return scaled_sum(sum, power, scale) + more;
 }
 
 // silu(g) u
@@ -545,7 +635,9 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 mine = bars.last[tile & 1];
             }
-            if (mine) {
+            // (careful: some row of the block has elements that its terms leave out. A loop of its own: with the call in the one
+            // that nearly all blocks take, 61 tokens' way down took 1.7 us more)
+            const auto results = [&](auto careful) {
                 constexpr int W = 16 / C;                        // tokens per step
                 for (int t = 0; t < s.m; t += W) {
                     float v[16];
@@ -554,7 +646,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                        constexpr int J = CONV ? 1 : 4;          // parts that are on their way together
+                        constexpr int J = CONV || decltype(careful)::value ? 1 : 4;      // parts on their way together
                         for (int o = c0; o <= c1; o += J) {
                             float part[J][16];
 #pragma unroll
@@ -571,16 +663,18 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                                     for (int i = 0; i < 16; ++i) v[i] += part[j][i];
                         }
                     }
-                    if (FMT == kSplit)
+                    if (FMT == kSplit) {
+#pragma unroll
+                        for (int i = 0; i < W; ++i) v[i] = v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f);
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
-                            // x's power of two up to 2^80 or down to 2^-80 ahead of W's scale, the rest behind it: sums lie between
-                            // 2^-34 and 2^37, so that nothing on the way passes fp32's range that the result does not pass
-                            const int power = __shfl_sync(0xffffffffu, t < 32 ? x_power[0] : x_power[1], t + i & 31);
-                            const int ahead = max(-80, min(power, 80));
-                            const float f0 = __int_as_float((ahead + 127) << 23), f1 = __int_as_float((power - ahead + 127) << 23);
-                            v[i] = (v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f)) * f0 * scale * f1;
+                            const int code = __shfl_sync(0xffffffffu, t < 32 ? x_power[0] : x_power[1], t + i & 31);
+                            if (decltype(careful)::value && code & 255)
+                                v[i] = with_rest(p, v[i], code, scale, s.e, n + (SILU && q >= 2 ? p.n : 0), n < p.n, s.row0 + t + i);
+                            else
+                                v[i] = scaled_sum(v[i], code >> 8, scale);
                         }
+                    }
                     if (CONV)
 #pragma unroll
                         for (int i = 0; i < W; ++i) v[i] *= scale;
@@ -605,6 +699,10 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                             if (t + i < s.m && n < p.n) to[i * p.out_row] = __float2bfloat16_rn(v[i]);
                     }
                 }
+            };
+            if (mine) {
+                if (FMT == kSplit && __any_sync(0xffffffffu, (x_power[0] | x_power[1]) & 255)) results(std::true_type{});
+                else results(std::false_type{});
             }
             if (whole) release();
         }
@@ -654,71 +752,111 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
     }
 }
 
-// x of every row of out, in their order, as four e4m3 terms [m][4][k] and the exponent of the power of two by which they are to
-// be multiplied: v = x / 2^power lies below 256, and v = t0 + t1 + 2^-16 (t2 + t3), each term the nearest to what is
-// left. A row that holds a NaN or an infinity is NaN, one that is not there zero.
+// x of every row of out, in their order, as four e4m3 terms [m][4][k] and the power of two by which they are to be multiplied:
+// v = x / 2^power lies below 256. From 2^-18 on the terms are v exactly (bf16 has 8 bits, and the last one's is 2^-25 or more,
+// the step of 2^-16 t3); below they leave out up to 2^-26, and of an infinity or NaN all. The groups of 8 along K that have
+// such an element are marked, and where a sum is not large enough beside all that is left out of its row, it is added from x and
+// W themselves (rest_sums). (Without that the smallest elements were lost where W is zero at the largest, and a single infinity
+// made all of a row NaN. Added wherever a row has any: 79 -> 1700 us for 256 rows with a few elements of 4000 times the others.)
 struct SplitParams {
     const __nv_bfloat16* x;
     const int* rows;
     const int* offsets;
     uint8_t* terms;
-    int* power;
+    int* power;                                      // [m] 256 power + q: sums below 2^(q - 128) want what is left out; 0: none
+    uint32_t* apart;                                 // [m][words], a bit per 8 of K
     long long x_row;
-    int k, x_rows, experts;
+    int k, x_rows, experts, words;
 };
 constexpr int kSplitThreads = 256;
 __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams p) {
     __shared__ uint32_t part[kSplitThreads / 32];
+    __shared__ float rests[kSplitThreads / 32];
     pdl_wait_and_trigger();
     const int i = blockIdx.x, from = p.rows ? p.rows[i] : i;
     uint8_t* to = p.terms + (size_t)i * 4 * p.k;
+    uint32_t* apart = p.apart + (size_t)i * p.words;
     const bool there = from >= 0 && from < p.x_rows;
     // (rows of out that belong to no expert may say anything here)
     if (!there && threadIdx.x == 0 && i >= p.offsets[0] && i < p.offsets[p.experts]) serve_error(kErrRouting);
     const __nv_bfloat16* x = p.x + (there ? from * p.x_row : 0);
-    uint32_t top = 0;                                            // the largest magnitude, as bits
-    for (int c = threadIdx.x * 8; there && c < p.k; c += kSplitThreads * 8) {
-        const uint4 v = *reinterpret_cast<const uint4*>(x + c);
+    const auto largest = [&](uint32_t most) {                    // magnitude up to `most` of the row, as bits
+        uint32_t top = 0;
+        for (int c = threadIdx.x * 8; there && c < p.k; c += kSplitThreads * 8) {
+            const uint4 v = *reinterpret_cast<const uint4*>(x + c);
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const uint32_t w = (&v.x)[j] & 0x7fff7fffu;
-            top = max(top, max(w & 0xffffu, w >> 16));
-        }
-    }
-    top = __reduce_max_sync(0xffffffffu, top);
-    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
-    __syncthreads();
-#pragma unroll
-    for (int j = 0; j < kSplitThreads / 32; ++j) top = max(top, part[j]);
-    // 2^e is the largest's power of two; x 2^(7 - e) in two factors, since the whole may pass fp32's range
-    const bool bad = top >= 0x7f80u;
-    const int e = bad || top == 0 ? 7 : max((int)(top >> 7), 1) - 127, f = 7 - e;
-    const float f0 = ldexpf(1.f, f / 2), f1 = ldexpf(1.f, f - f / 2);
-    if (threadIdx.x == 0) p.power[i] = -f;
-    for (int c = threadIdx.x * 8; c < p.k; c += kSplitThreads * 8) {
-        uint4 v = make_uint4(0, 0, 0, 0);
-        if (there) v = *reinterpret_cast<const uint4*>(x + c);
-        uint32_t term[4][2];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            float a = bf16_lo((&v.x)[j]) * f0 * f1, b = bf16_hi((&v.x)[j]) * f0 * f1;
-#pragma unroll
-            for (int t = 0; t < 4; ++t) {
-                if (t == 2) { a *= 0x1p16f; b *= 0x1p16f; }
-                uint16_t q;
-                uint32_t h;
-                asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(q) : "f"(b), "f"(a));
-                asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(q));
-                const float2 back = __half22float2(*reinterpret_cast<const __half2*>(&h));
-                a -= back.x;
-                b -= back.y;
-                if (bad) q = 0x7f7f;
-                term[t][j >> 1] = j & 1 ? term[t][j >> 1] | (uint32_t)q << 16 : q;
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = (&v.x)[j] & 0x7fff7fffu, lo = w & 0xffffu, hi = w >> 16;
+                top = max(top, max(lo <= most ? lo : 0u, hi <= most ? hi : 0u));
             }
         }
+        top = __reduce_max_sync(0xffffffffu, top);
+        __syncthreads();
+        if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
+        __syncthreads();
 #pragma unroll
-        for (int t = 0; t < 4; ++t) *reinterpret_cast<uint2*>(to + (size_t)t * p.k + c) = make_uint2(term[t][0], term[t][1]);
+        for (int j = 0; j < kSplitThreads / 32; ++j) top = max(top, part[j]);
+        return top;
+    };
+    uint32_t top = largest(0x7fffu);
+    if (top >= 0x7f80u) top = largest(0x7f7fu);
+    // the largest's power of two, 2^(power + 7)
+    const int power = top == 0 ? 0 : max((int)(top >> 7), 1) - 134;
+    const float2 f = split_factors(power);
+    // bits of 2^(power - 18): magnitudes from there on, and zeros, have their terms
+    const uint32_t least = power >= -108 ? (uint32_t)(power + 109) << 7 : power >= -115 ? 1u << (power + 115) : 1u;
+    float rest = 0.f;                                            // magnitudes of what this thread's terms leave out
+    for (int c0 = 0; c0 < p.k; c0 += kSplitThreads * 8) {
+        const int c = c0 + threadIdx.x * 8;
+        bool out = false;
+        if (c < p.k) {
+            uint4 v = make_uint4(0, 0, 0, 0);
+            if (there) v = *reinterpret_cast<const uint4*>(x + c);
+            uint32_t low = 0xffffffffu, high = 0u;               // less 1, so that a zero is no small one
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint32_t w = __vsub2((&v.x)[j] & 0x7fff7fffu, 0x00010001u);
+                low = __vminu2(low, w);
+                high = __vmaxs2(high, w);
+            }
+            out = min(low & 0xffffu, low >> 16) < least - 1 || max(high & 0xffffu, high >> 16) >= 0x7f7fu;
+            uint32_t term[4][2];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float x0 = bf16_lo((&v.x)[j]), x1 = bf16_hi((&v.x)[j]);
+                float a = x0 * f.x * f.y, b = x1 * f.x * f.y;
+                if (out) {                                       // (2^-100: what has left fp32's range)
+                    if (a == 0.f && x0 != 0.f) rest += 0x1p-100f;
+                    if (b == 0.f && x1 != 0.f) rest += 0x1p-100f;
+                    if (!(fabsf(a) < 256.f)) { rest = INFINITY; a = 0.f; }
+                    if (!(fabsf(b) < 256.f)) { rest = INFINITY; b = 0.f; }
+                }
+                uint16_t q[4];
+                split_terms(a, b, q);
+                if (out) rest += (fabsf(a) + fabsf(b)) * 0x1p-16f;
+#pragma unroll
+                for (int t = 0; t < 4; ++t) term[t][j >> 1] = j & 1 ? term[t][j >> 1] | (uint32_t)q[t] << 16 : q[t];
+            }
+#pragma unroll
+            for (int t = 0; t < 4; ++t) *reinterpret_cast<uint2*>(to + (size_t)t * p.k + c) = make_uint2(term[t][0], term[t][1]);
+        }
+        const uint32_t marks = __ballot_sync(0xffffffffu, out);
+        const int word = (c0 >> 8) + (threadIdx.x >> 5);
+        if ((threadIdx.x & 31) == 0 && word < p.words) apart[word] = marks;
     }
+    int q = 0;
+    if (__syncthreads_or(rest != 0.f)) {
+#pragma unroll
+        for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+        if ((threadIdx.x & 31) == 0) rests[threadIdx.x >> 5] = rest;
+        __syncthreads();
+        rest = 0.f;
+#pragma unroll
+        for (int j = 0; j < kSplitThreads / 32; ++j) rest += rests[j];
+        // each meets 448 at most; the next power of two above 2^18 times that
+        q = rest == INFINITY ? 255 : ilogbf(rest * (448.f * 0x1p18f)) + 1 + 128;
+    }
+    if (threadIdx.x == 0) p.power[i] = power * 256 + q;
 }
 
 // The maps. W [experts][rows][K]: 128 bytes of 128 rows (silu: of 64 of gate and 64 of up) per copy; rows and K behind the end
@@ -771,9 +909,17 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* ter
     long long x_row = p.x_row;
     int x_rows = p.x_rows;
     if (FMT == kSplit) {
-        SplitParams q{p.x, p.rows, p.offsets, terms, reinterpret_cast<int*>(terms + (size_t)a->M * 4 * p.k), p.x_row, p.k, p.x_rows,
-                      p.experts};
+        // (the powers behind the terms, the marks behind the powers)
+        SplitParams q{p.x, p.rows, p.offsets, terms, reinterpret_cast<int*>(terms + (size_t)a->M * 4 * p.k), nullptr, p.x_row, p.k,
+                      p.x_rows, p.experts, (p.k + 255) / 256};
+        q.apart = reinterpret_cast<uint32_t*>(q.power + a->M);
         p.x_power = q.power;
+        p.apart = q.apart;
+        p.words = q.words;
+        p.x_from = p.rows;
+        p.w_at = static_cast<const uint8_t*>(a->w);
+        p.w_expert = a->w_expert;
+        p.w_row = a->w_row;
         p.rows = nullptr;
         x = terms;
         x_row = p.k;
@@ -824,7 +970,7 @@ int experts_device_error(int clear) { return serve_error_word(clear); }
 using namespace pb2;
 
 extern "C" size_t paia_gemv_expert_workspace(void) {
-    return kExpCounters + kExpParts + kExpSplitBytes;
+    return kExpCounters + kExpParts + kExpSplitBytes + kExpApartBytes;
 }
 
 extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* stream) {

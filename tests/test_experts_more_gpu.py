@@ -94,3 +94,86 @@ def test_magnitudes_beyond_fp32_half_way(L, ws, xe, we, size, tokens):
         assert bool(fits.all()) == (xe < 126)
         out, want, bound = out[fits], want[fits], bound[fits]
     within(out, want, bound)
+
+
+@pytest.mark.parametrize("tokens", [3, 60, 100, 200])
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("gather", [False, True])
+def test_every_finite_x(L, ws, kind, tokens, gather):
+    """Ones on the diagonal of W: out is x to the bit, with rows of values from bf16's smallest to its largest."""
+    from paia_gemv import serve
+    g = gen(tokens)
+    x = torch.randint(0, 0x7F80, (tokens, 512), generator=g, device=DEV)
+    x = (x | torch.randint(0, 2, x.shape, generator=g, device=DEV) << 15).to(torch.int16).view(C.BF16)
+    x[1, 100:] = 0
+    w = torch.eye(512, device=DEV)[None].to(C.E4M3 if kind == "fp8" else C.BF16)
+    s = torch.ones(1, 512, device=DEV) if kind == "fp8" else None
+    rows = torch.randperm(tokens, generator=g, device=DEV).to(torch.int32) if gather else None
+    out = torch.full((tokens, 512), 7.0, dtype=C.BF16, device=DEV)
+    serve.expert_matmul(L, w, x, C.groups([tokens], DEV), out, ws, scales=s, rows=rows)
+    assert torch.equal(out, x if rows is None else x[rows.long()])
+
+
+@pytest.mark.parametrize("tokens", [3, 100, 200])
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+def test_infinities_and_nan_as_the_formula_has_them(L, ws, kind, tokens):
+    """An infinity in x takes the sign of the weight that it meets; with a weight of zero, or another of the other sign, NaN."""
+    from paia_gemv import serve
+    g = gen(16)
+    w, s, values = C.weights(1, 128, 256, kind, g, DEV)
+    w[0, 5, 7] = 0
+    values[0, 5, 7] = 0
+    x = torch.randn(tokens, 256, generator=g, device=DEV).to(C.BF16)
+    inf = float("inf")
+    x[0, 7], x[1, 9], x[2, 3], x[2, 200] = inf, -inf, inf, -inf
+    x[tokens - 1, 255] = float("nan") if tokens > 3 else x[tokens - 1, 255]
+    out = torch.zeros(tokens, 128, dtype=C.BF16, device=DEV)
+    serve.expert_matmul(L, w, x, C.groups([tokens], DEV), out, ws, scales=s)
+    want = x.to(C.F64) @ values[0].T
+    assert bool(torch.isinf(want[:2]).any()) and bool(torch.isnan(want[:3]).any())
+    odd = ~torch.isfinite(want)
+    assert torch.equal(torch.isnan(out), torch.isnan(want)) and torch.equal(out[odd & ~torch.isnan(want)].to(C.F64), want[odd & ~torch.isnan(want)])
+    fine = torch.isfinite(x.float()).all(1)
+    _, bound = C.matmul(values, torch.where(fine[:, None], x, 0.0), C.groups([tokens], DEV))
+    within(out[fine], want[fine], bound[fine])
+
+
+@pytest.mark.parametrize("counts", [[5, 0, 9, 40], [100], [200, 130]], ids=str)
+@pytest.mark.parametrize("n,k", [(200, 48), (200, 528), (64, 16384)])
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+def test_small_elements_whose_large_neighbours_meet_no_weight(L, ws, counts, n, k, silu, gather):
+    """e4m3 rows of W that are zero wherever x is large: the sums are those of what lies 2^-30 to 2^-60 below."""
+    from paia_gemv import serve
+    g, m = gen(k + n), sum(counts)
+    e, off = len(counts), C.groups(counts, DEV)
+    w, s, values = C.weights(e, n, 2 * k, "fp8", g, DEV)
+    w, values = w[:, :, k:], values[:, :, k:]
+    w[:, 1::2, ::3] = 0
+    values[:, 1::2, ::3] = 0
+    x = torch.randn(m, 2 * k, generator=g, device=DEV)[:, :k]
+    x = (x * 2.0 ** (-30 * torch.rand(m, k, generator=g, device=DEV) - 10)).to(C.BF16)
+    x[:, ::3] = (2.0 ** 20 * torch.randn(x[:, ::3].shape, generator=g, device=DEV)).to(C.BF16)
+    x[2] = 0
+    big = torch.zeros(m, 2 * k, dtype=C.BF16, device=DEV)
+    big[:, :k] = x
+    rows = torch.randint(0, m, (m,), generator=g, device=DEV).to(torch.int32) if gather else None
+    out = torch.full((m, n // 2 if silu else n), 7.0, dtype=C.BF16, device=DEV)
+    serve.expert_matmul(L, w, big[:, :k], off, out, ws, scales=s, rows=rows, silu=silu)
+    values = values.contiguous()
+    at = off.tolist()
+    for i in range(e):
+        lo, hi = at[i], at[i + 1]
+        xx = (x[lo:hi] if rows is None else x[rows[lo:hi].long()]).to(C.F64)
+        y = xx @ values[i].T
+        # C.matmul's roundings, and those of up to K products that are added one after another
+        d = (xx.abs() @ values[i].abs().T) * (k / 8 + 64 + k / 2) * C.F32 + 4 * C.F32 * y.abs()
+        if silu:
+            (gate, up), (dg, du) = y.chunk(2, 1), d.chunk(2, 1)
+            half = torch.sigmoid(gate)
+            y = gate * half * up
+            d = 1.1 * dg * (up.abs() + du) + (gate * half).abs() * du + y.abs() * (8 + gate.abs()) * 2 * C.F32
+        within(out[lo:hi], y, d * (1 + C.HALF_BF16) + C.HALF_BF16 * y.abs() + 1e-38)
+    again = torch.zeros_like(out)
+    serve.expert_matmul(L, w, big[:, :k], off, again, ws, scales=s, rows=rows, silu=silu)
+    assert torch.equal(out, again) and L.device_error() == 0
