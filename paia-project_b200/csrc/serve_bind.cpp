@@ -400,7 +400,7 @@ PyObject* block_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
         return none();
     if (a[6] != Py_None) {
         if (!pl.is(a[6], dev, kI32, 2) || !wt.is(a[7], dev, kF32, 2) || pl.n(0) != t || wt.n(0) != t || wt.n(1) != pl.n(1) ||
-            !small(pl.n(1)) || !pl.dense_last() || !wt.dense_last())
+            !small(pl.n(1)) || pl.n(1) < 1 || !pl.dense_last() || !wt.dense_last())
             return none();
         s.places = static_cast<const int*>(pl.ptr());
         s.weights = static_cast<const float*>(wt.ptr());

@@ -430,9 +430,9 @@ def block_norm(lib, h, x=None, h_out=None, *, out=None, places=None, weights=Non
 
     top_k, ps, wts = 0, 0, 0
     if places is not None:
-        if len(places.shape) != 2 or places.shape[0] != t or places.dtype is not _I32 or places.get_device() != dev or (
-                places.stride(1) != 1 and places.shape[1] != 1):
-            _bad("places", places, f"int32 [{t}, top_k], contiguous in its last dimension,")
+        if len(places.shape) != 2 or places.shape[0] != t or places.shape[1] < 1 or places.dtype is not _I32 or (
+                places.get_device() != dev or places.stride(1) != 1 and places.shape[1] != 1):
+            _bad("places", places, f"int32 [{t}, top_k >= 1], contiguous in its last dimension,")
         top_k = places.shape[1]
         if weights is None or weights.shape != places.shape or weights.dtype is not _F32 or weights.get_device() != dev or (
                 weights.stride(1) != 1 and top_k != 1):

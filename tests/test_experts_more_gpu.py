@@ -177,3 +177,15 @@ def test_small_elements_whose_large_neighbours_meet_no_weight(L, ws, counts, n, 
     again = torch.zeros_like(out)
     serve.expert_matmul(L, w, big[:, :k], off, again, ws, scales=s, rows=rows, silu=silu)
     assert torch.equal(out, again) and L.device_error() == 0
+
+
+# ------------------------------------------------------------------ norms
+
+def test_block_of_no_places_is_refused(L):
+    """Places without a column are no call without places, which adds x's own rows."""
+    from paia_gemv import serve
+    h, x = torch.zeros(4, 64, dtype=C.BF16, device=DEV), torch.ones(4, 64, dtype=C.BF16, device=DEV)
+    places, weights = torch.zeros(4, 0, dtype=torch.int32, device=DEV), torch.zeros(4, 0, device=DEV)
+    with pytest.raises(ValueError, match="places"):
+        serve.block_norm(L, h, x, h, places=places, weights=weights)
+    assert not h.any()
