@@ -64,7 +64,9 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const NormPara
     __shared__ float part[2][32];
     pdl_wait_and_trigger();
     const int n = (int)blockDim.x;
-    for (int t = blockIdx.x; t < p.tokens; t += gridDim.x) {
+    // (unsigned: the step behind the last of nearly 2^31 rows passes an int)
+    const unsigned tokens = p.tokens;
+    for (unsigned t = blockIdx.x; t < tokens; t += gridDim.x) {
         uint4 hv[V];
         float y[V][8];
 #pragma unroll
@@ -181,7 +183,7 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const NormPara
             }
         }
         // With both norms each sum's words were read before the other's barrier; a lone one's are still being read.
-        if (!(p.post && p.out) && t + (int)gridDim.x < p.tokens) __syncthreads();
+        if (!(p.post && p.out) && t + gridDim.x < tokens) __syncthreads();
     }
 }
 

@@ -47,3 +47,11 @@ def test_terms_and_marks_fit_the_workspace(L):
     for k in [16 * i for i in range(1, 400)] + [256 * i + d for i in (30, 500, 4095) for d in (-16, 0, 16)] + [1 << 20]:
         m = min(split // (4 * k + 4), tokens * experts)
         assert m * (4 * k + 4) + m * 4 * -(-k // 256) <= room, (k, m)
+
+
+def test_norm_counts_rows_without_passing_an_int():
+    """block_norm_kernel steps by the grid's size from its last row, of up to 2^31 - 1: in an unsigned."""
+    src = code("block_norm.cu")
+    loop = re.search(r"for \((\w+) t = blockIdx\.x; t < (\w+(?:\.\w+)?); t \+= gridDim\.x\)", src)
+    assert loop and loop.group(1) == "unsigned" and re.search(rf"const unsigned {loop.group(2)} = p\.tokens;", src)
+    assert "(int)gridDim.x" not in src[src.index("block_norm_kernel"):src.index("launch_norm")]

@@ -189,3 +189,20 @@ def test_block_of_no_places_is_refused(L):
     with pytest.raises(ValueError, match="places"):
         serve.block_norm(L, h, x, h, places=places, weights=weights)
     assert not h.any()
+
+
+def test_norms_of_nearly_2_31_rows(L):
+    """The most rows that an int counts (one row of h for all of them): the last are reached, and nothing behind."""
+    from paia_gemv import serve
+    tokens = 2 ** 31 - 1
+    g = gen(17)
+    h = torch.randn(1, 8, generator=g, device=DEV).to(C.BF16)
+    pre = 1 + 0.1 * torch.randn(8, generator=g, device=DEV)
+    small = torch.zeros(1, 8, dtype=C.BF16, device=DEV)
+    serve.block_norm(L, h, out=small, pre=pre)
+    within(small, *C.norm(h, pre))
+    out = torch.full((tokens + 1, 8), 7.0, dtype=C.BF16, device=DEV)
+    serve.block_norm(L, h.expand(tokens, 8), out=out[:tokens], pre=pre)
+    assert bool((out[tokens] == 7.0).all())
+    for piece in out[:tokens].split(1 << 28):
+        assert bool((piece == small).all())
