@@ -358,8 +358,8 @@ int paia_gemv_route(const paia_gemv_route_args* a, void* stream);
  * or infinite and nothing else. Rows of out that belong to no expert stay as they were. With an offset below the one before it
  * or outside [0, M] nothing is computed, a row of x outside [0, x_rows) reads as zeros (code 14); a bounded wait inside the
  * kernel that gives up sets code 15, out is then not to be used and the workspace to be zeroed. K is a multiple of 8 (kind 1:
- * 16), experts <= 1024, M <= 2^28, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of whole 16
- * bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed once; every
+ * 16), experts <= 1024, M <= 2^28, N <= 2^30, K <= 2^20. w, x and workspace 16-byte aligned, rows of w and x at strides of
+ * whole 16 bytes. x may not overlap out. `workspace`: paia_gemv_expert_workspace() bytes on the launch's device, zeroed once; every
  * launch leaves it ready for the next, of any sizes; launches that may overlap on the GPU need one each. */
 typedef struct paia_gemv_expert_args {
     const void* w;               /* [experts][N][K] */

@@ -978,7 +978,7 @@ extern "C" int paia_gemv_expert_matmul(const paia_gemv_expert_args* a, void* str
         (a->kind != 0 && a->kind != 1) || (a->silu && a->N % 2))
         return -2;
     const int unit = a->kind == 0 ? 8 : 16;
-    if (a->K % unit || a->K > 1 << 20 || a->M > 1 << 28 || !a->scales != !a->kind) return -2;
+    if (a->K % unit || a->K > 1 << 20 || a->M > 1 << 28 || a->N > 1 << 30 || !a->scales != !a->kind) return -2;
     if (a->M == 0) return 0;
     if (!a->w || !a->offsets || !a->workspace || !a->x || !a->out) return -2;
     if (!aligned_to(a->w, 16) || !aligned_to(a->x, 16) || !aligned_to(a->out, 2) || !aligned_to(a->rows, 4) ||

@@ -49,6 +49,16 @@ def test_terms_and_marks_fit_the_workspace(L):
         assert m * (4 * k + 4) + m * 4 * -(-k // 256) <= room, (k, m)
 
 
+def test_sizes_whose_tiles_pass_an_int_are_refused(L):
+    """Rows of W are counted in tiles of up to 256, and a tile's last rows may lie behind N: both within an int."""
+    from paia_gemv import serve
+    from test_experts_cpu import EXPERTS, packed
+    most = re.search(r"a->N > (\d+) << (\d+)", code("block_experts.cu"))
+    assert most and (int(most.group(1)) << int(most.group(2))) + 2 * 255 < 2 ** 31
+    big = dict(N=2 ** 31 - 200, K=8, w_row=8, w_expert=8 * (2 ** 31 - 200), out_row=2 ** 31 - 200)
+    assert L._lib.paia_gemv_expert_matmul(packed("paia_gemv_expert_args", serve.EXPERTS, EXPERTS, **big), None) == -2
+
+
 def test_norm_counts_rows_without_passing_an_int():
     """block_norm_kernel steps by the grid's size from its last row, of up to 2^31 - 1: in an unsigned."""
     src = code("block_norm.cu")
