@@ -179,6 +179,53 @@ def test_small_elements_whose_large_neighbours_meet_no_weight(L, ws, counts, n, 
     assert torch.equal(out, again) and L.device_error() == 0
 
 
+# More than two rounds of tiles: runs of K that end inside tiles, then whole tiles, three parts and more for every CTA (pair).
+# Units of K: one, three with the last one short, seven.
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("kind,k", [("bf16", 64), ("bf16", 168), ("bf16", 448), ("fp8", 128), ("fp8", 368), ("fp8", 896)])
+@pytest.mark.parametrize("counts,n", [([300, 0, 257, 130], 10496), ([150, 513, 0, 1, 290, 190], 8192), ([256, 256], 19200)],
+                         ids=str)
+def test_many_tiles_of_large_blocks(L, ws, counts, n, kind, k, gather, silu):
+    """Pairs of CTAs, tile after tile."""
+    a = run(L, ws, counts, n, k, kind, silu, gather, tokens=700 if gather else None, seed=k)
+    assert torch.equal(a, run(L, ws, counts, n, k, kind, silu, gather, tokens=700 if gather else None, seed=k))
+    assert not ws.buffer[:1280].any()
+
+
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("kind,k", [("bf16", 168), ("bf16", 448), ("fp8", 368), ("fp8", 896)])
+@pytest.mark.parametrize("counts,n", [([1] * 40, 1536), ([9, 0, 17, 1, 30, 2] * 6, 1664), ([60, 64, 3, 50] * 2, 7296)], ids=str)
+def test_many_tiles_of_small_blocks(L, ws, counts, n, kind, k, gather, silu):
+    """Single CTAs, tile after tile (e4m3: as split terms)."""
+    a = run(L, ws, counts, n, k, kind, silu, gather, tokens=100 if gather else None, seed=k)
+    assert torch.equal(a, run(L, ws, counts, n, k, kind, silu, gather, tokens=100 if gather else None, seed=k))
+    assert not ws.buffer[:1280].any()
+
+
+@pytest.mark.parametrize("kind", ["bf16", "fp8"])
+@pytest.mark.parametrize("k", [1040, 4096])
+def test_one_round_of_whole_tiles(L, ws, kind, k):
+    """Tiles that nearly fill a round are taken whole, each from another place of K on."""
+    run(L, ws, [1] * 8, 2048, k, kind, silu=True, gather=True, tokens=1)
+    run(L, ws, [3, 1, 0, 2, 2, 1, 1, 1, 5], 2048, k, kind)
+
+
+@pytest.mark.parametrize("silu", [False, True])
+@pytest.mark.parametrize("gather", [False, True])
+@pytest.mark.parametrize("experts,rows", [(256, 8), (96, 21), (64, 40)])
+def test_small_blocks_of_converted_weights(L, ws, experts, rows, gather, silu):
+    """e4m3 rows whose terms would not fit the workspace: blocks of 16 to 128 tokens meet converted weights, an odd number of
+    units of K two by two."""
+    counts = [rows + (i % 5) - 2 for i in range(experts)]
+    counts[3], counts[4] = 0, counts[3] + counts[4]
+    k = 7024                                                     # 55 units
+    assert sum(counts) * (4 * k + 4) > 48 << 20
+    a = run(L, ws, counts, 144, k, "fp8", silu, gather, tokens=300 if gather else None)
+    assert torch.equal(a, run(L, ws, counts, 144, k, "fp8", silu, gather, tokens=300 if gather else None))
+
+
 # ------------------------------------------------------------------ norms
 
 def test_block_of_no_places_is_refused(L):
