@@ -22,7 +22,6 @@
 // row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 79 (6.0 TB/s), 64 of 4096 x 1024 for 61 tokens 54; 8192 rows, 8
 // experts of 4096 x 14336 in bf16 790 (1.2 PFLOP/s, tensor pipe 79 % busy; in runs of seconds, under the power cap, 950);
 // 16384 rows, 64 experts of 2048 x 4096 in e4m3 350-410 (conversion and its hand-over to the products bound it).
-#include <type_traits>
 #include "paia_gemv.h"
 #include "block_tc5.cuh"
 
@@ -90,7 +89,9 @@ struct ExpBars {
 };
 constexpr int kExpExchange = 2 * 4 * 8 * 32 * 4;     // [2][warp][column][lane] floats
 constexpr int kExpLists = 4 * 128 * 8;
-constexpr size_t exp_fixed_smem(int experts) { return 1024 + kExpExchange + kExpLists + sizeof(ExpBars) + 12 * (size_t)(experts + 1); }
+constexpr size_t exp_fixed_smem(int experts) {
+    return 1024 + kExpExchange + kExpLists + sizeof(ExpBars) + 12 * (size_t)(experts + 1);
+}
 
 // A place in a ring.
 struct ExpRing {
@@ -122,7 +123,8 @@ struct ExpWalk {
     const int* off;                                  // first row of each expert, then (from experts + 1) its end
     const int* first;                                // first tile of each expert
     int total, cut, work, workers, at, end, next_whole, step;
-    __device__ __forceinline__ ExpWalk(const ExpertParams& p_, const int* off_, const int* first_) : p(p_), off(off_), first(first_) {
+    __device__ __forceinline__ ExpWalk(const ExpertParams& p_, const int* off_, const int* first_)
+        : p(p_), off(off_), first(first_) {
         const int g = (int)gridDim.x / CG, c = (int)blockIdx.x / CG;
         total = first[p.experts];
         int rounds = total / g;
@@ -253,7 +255,7 @@ __device__ __forceinline__ float scaled_sum(float sum, int power, float scale) {
 // The same for the row x of out's row `at`, whose terms leave something out, and each lane's row n of expert e's W (`on`: there is
 // one): where that may count, it is added, in fp32 and in an order that depends on nothing else. The whole warp takes one row of
 // W at a time, a marked group of 8 along K per lane.
-__device__ __noinline__ float with_rest(const ExpertParams& p, float sum, int code, float scale, int e, int n, bool on, int at) {
+__device__ __forceinline__ float with_rest(const ExpertParams& p, float sum, int code, float scale, int e, int n, bool on, int at) {
     const int lane = threadIdx.x & 31, words = p.words, power = code >> 8, from = p.x_from ? p.x_from[at] : at;
     const __nv_bfloat16* x = p.x + from * p.x_row;
     const uint32_t* apart = p.apart + (size_t)at * words;
@@ -282,7 +284,8 @@ __device__ __noinline__ float with_rest(const ExpertParams& p, float sum, int co
                     const float x0 = bf16_lo((&v.x)[j]), x1 = bf16_hi((&v.x)[j]);
                     float a = x0 * f.x * f.y, b = x1 * f.x * f.y;
                     // (what has no terms may be infinite, or too small for fp32 beside the row's largest)
-                    const bool none0 = !(fabsf(a) > 0x1p-26f && fabsf(a) < 256.f), none1 = !(fabsf(b) > 0x1p-26f && fabsf(b) < 256.f);
+                    const bool none0 = !(fabsf(a) > 0x1p-26f && fabsf(a) < 256.f);
+                    const bool none1 = !(fabsf(b) > 0x1p-26f && fabsf(b) < 256.f);
                     split_terms(a, b, term);
                     if (none0) apart_left = fmaf(by.x, x0, apart_left);
                     else left = fmaf(by.x, a, left);
@@ -310,6 +313,53 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
     float r;
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
     return g * r * u;
+}
+// The rows of a block whose terms leave something out, once more, behind the others and over what those have stored.
+// (Out of the way: nearly always there are none, and in the others' loop it took registers, 1.6 us of every call.)
+template <bool SILU>
+__device__ __noinline__ int rows_with_rest(const ExpertParams& p, const ExpWalk<1> walk, const ExpPart s, uint32_t d, float* exchange,
+                                           int step) {
+    const int q = (threadIdx.x >> 5) - kExpEpilogue, lane = threadIdx.x & 31;
+    const int n = s.row_tile * (SILU ? 64 : kExpRows) + (SILU ? q & 1 : q) * 32 + lane, w_n = n + (SILU && q >= 2 ? p.n : 0);
+    const float scale = n < p.n ? p.scales[s.e * p.scale_expert + w_n] : 0.f;
+    const bool whole = s.k0 == 0 && s.k1 == p.units;
+    const int c0 = whole ? 0 : walk.owner(s.tile * p.units), c1 = whole ? 0 : walk.owner((s.tile + 1) * p.units - 1);
+    uint64_t rows = 0;
+    for (int t = 0; t < s.m; t += 32) {
+        const uint32_t some = __ballot_sync(0xffffffffu, t + lane < s.m && p.x_power[s.row0 + t + lane] & 255);
+        rows |= (uint64_t)some << t;
+    }
+#pragma unroll 1
+    for (; rows; rows &= rows - 1) {
+        const int t = __ffsll((long long)rows) - 1, code = p.x_power[s.row0 + t];
+        float v[4] = {0.f, 0.f, 0.f, 0.f};
+        if (whole) {
+            float w[16];                                         // (of 16 columns, as everywhere here)
+            tmem_load16(d + (4 * t & ~15), w);
+#pragma unroll
+            for (int i = 0; i < 16; ++i)
+                if (i >> 2 == (t & 3)) v[i & 3] = w[i];
+        } else {
+#pragma unroll 1
+            for (int o = c0; o <= c1; ++o) {
+                const float* from = p.parts + ((size_t)walk.place(o, s.tile) * 4 * p.tokens + 4 * t) * kExpRows + q * 32 + lane;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) v[i] += __ldcg(from + i * kExpRows);
+            }
+        }
+        const float sum = v[0] + (v[1] + (v[2] + v[3]) * 0x1p-16f);
+        const float r = with_rest(p, sum, code, scale, s.e, w_n, n < p.n, s.row0 + t);
+        __nv_bfloat16* to = p.out + (long long)(s.row0 + t) * p.out_row + n;
+        if (SILU) {                                              // (the barrier also puts the other warp's store ahead of this one)
+            float* x = exchange + (step++ & 1) * (4 * 8 * 32) + lane;
+            if (q >= 2) x[q * 8 * 32] = r;
+            asm volatile("bar.sync %0, 64;" :: "r"(2 + (q & 1)) : "memory");
+            if (q < 2 && n < p.n) *to = __float2bfloat16_rn(silu_mul(r, x[(q ^ 2) * 8 * 32]));
+        } else if (n < p.n) {
+            *to = __float2bfloat16_rn(r);
+        }
+    }
+    return step;
 }
 // Whether `ok` holds in all 128 threads of the barrier (one for every part, so that none of them waits alone).
 __device__ __forceinline__ bool all_of(bool ok) {
@@ -462,7 +512,8 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     bar_expect(bar, n * copies * p.box * 128);
                     for (int u = 0; u < n; ++u) {
                         const int from = walk.unit(s, k + u / XT) * K + K / XT * (u % XT);
-                        for (int i = 0; i < copies; ++i) tma_2d(to + u * xb + i * p.box * 128, &p.x_map, from, row + i * p.box, bar);
+                        for (int i = 0; i < copies; ++i)
+                            tma_2d(to + u * xb + i * p.box * 128, &p.x_map, from, row + i * p.box, bar);
                     }
                 }
             }
@@ -525,7 +576,8 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 if (leader && tile >= 2 && !wait(sptr(&bars.d_empty[buf]), (tile / 2 & 1) ^ 1u)) break;
                 tc5_fence_after();
                 const uint32_t d = tmem + buf * cols;
-                const uint32_t shape = FMT == kSplit ? tc5_e4m3_shape<CG>((4 * s.m + 15) & ~15) : tc5_bf16_shape<CG>(walk.round_up(s.m));
+                const uint32_t shape =
+                    FMT == kSplit ? tc5_e4m3_shape<CG>((4 * s.m + 15) & ~15) : tc5_bf16_shape<CG>(walk.round_up(s.m));
                 uint32_t add = 0;
                 for (int left = s.k1 - s.k0; left > 0; left -= sub) {
                     const int n = min(sub, left);
@@ -635,9 +687,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                 asm volatile("bar.sync 1, 128;" ::: "memory");
                 mine = bars.last[tile & 1];
             }
-            // (careful: some row of the block has elements that its terms leave out. A loop of its own: with the call in the one
-            // that nearly all blocks take, 61 tokens' way down took 1.7 us more)
-            const auto results = [&](auto careful) {
+            if (mine) {
                 constexpr int W = 16 / C;                        // tokens per step
                 for (int t = 0; t < s.m; t += W) {
                     float v[16];
@@ -646,13 +696,14 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                     } else {
 #pragma unroll
                         for (int i = 0; i < 16; ++i) v[i] = 0.f;
-                        constexpr int J = CONV || decltype(careful)::value ? 1 : 4;      // parts on their way together
+                        constexpr int J = CONV ? 1 : 4;          // parts that are on their way together
                         for (int o = c0; o <= c1; o += J) {
                             float part[J][16];
 #pragma unroll
                             for (int j = 0; j < J; ++j) {
                                 if (o + j > c1) continue;
-                                const float* from = p.parts + ((size_t)(walk.place(o + j, s.tile) * CG + rank) * cols + C * t) * kExpRows + row;
+                                const size_t place = walk.place(o + j, s.tile) * CG + rank;
+                                const float* from = p.parts + (place * cols + C * t) * kExpRows + row;
 #pragma unroll
                                 for (int i = 0; i < 16; ++i) part[j][i] = __ldcg(from + i * kExpRows);
                             }
@@ -663,18 +714,12 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                                     for (int i = 0; i < 16; ++i) v[i] += part[j][i];
                         }
                     }
-                    if (FMT == kSplit) {
-#pragma unroll
-                        for (int i = 0; i < W; ++i) v[i] = v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f);
+                    if (FMT == kSplit)
 #pragma unroll
                         for (int i = 0; i < W; ++i) {
-                            const int code = __shfl_sync(0xffffffffu, t < 32 ? x_power[0] : x_power[1], t + i & 31);
-                            if (decltype(careful)::value && code & 255)
-                                v[i] = with_rest(p, v[i], code, scale, s.e, n + (SILU && q >= 2 ? p.n : 0), n < p.n, s.row0 + t + i);
-                            else
-                                v[i] = scaled_sum(v[i], code >> 8, scale);
+                            const int power = __shfl_sync(0xffffffffu, t < 32 ? x_power[0] : x_power[1], t + i & 31) >> 8;
+                            v[i] = scaled_sum(v[4 * i] + (v[4 * i + 1] + (v[4 * i + 2] + v[4 * i + 3]) * 0x1p-16f), power, scale);
                         }
-                    }
                     if (CONV)
 #pragma unroll
                         for (int i = 0; i < W; ++i) v[i] *= scale;
@@ -699,10 +744,9 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
                             if (t + i < s.m && n < p.n) to[i * p.out_row] = __float2bfloat16_rn(v[i]);
                     }
                 }
-            };
-            if (mine) {
-                if (FMT == kSplit && __any_sync(0xffffffffu, (x_power[0] | x_power[1]) & 255)) results(std::true_type{});
-                else results(std::false_type{});
+                if constexpr (FMT == kSplit)
+                    if (__any_sync(0xffffffffu, (x_power[0] | x_power[1]) & 255))
+                        step = rows_with_rest<SILU>(p, walk, s, d, exchange, step);
             }
             if (whole) release();
         }
@@ -714,7 +758,9 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
         const uint32_t to0 = tmem + T::kABase + 32 * half + ((uint32_t)((warp & 3) * 32) << 16);
         int turn = 0, ab = 0;
         uint32_t ap = 1;                                         // the first round of buffers is free
-        const auto wait_all = [&](uint32_t bar, uint32_t phase) { return ok = __all_sync(0xffffffffu, bar_wait(bar, phase, dead)); };
+        const auto wait_all = [&](uint32_t bar, uint32_t phase) {
+            return ok = __all_sync(0xffffffffu, bar_wait(bar, phase, dead));
+        };
         while (ok && walk.next(s))
             for (int k = s.k0; ok && k < s.k1; k += sub, at.step()) {
                 const int n = min(sub, s.k1 - k);
@@ -757,7 +803,8 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
 // the step of 2^-16 t3); below they leave out up to 2^-26, and of an infinity or NaN all. The groups of 8 along K that have
 // such an element are marked, and where a sum is not large enough beside all that is left out of its row, it is added from x and
 // W themselves (rest_sums). (Without that the smallest elements were lost where W is zero at the largest, and a single infinity
-// made all of a row NaN. Added wherever a row has any: 79 -> 1700 us for 256 rows with a few elements of 4000 times the others.)
+// made all of a row NaN. Rows of heavy tails with a few elements of 4000 times the others, 256 of them: 79 us before, 1709 with the
+// rest added to every sum, 404 as here; normal rows with such elements 82.)
 struct SplitParams {
     const __nv_bfloat16* x;
     const int* rows;
@@ -780,83 +827,92 @@ __global__ void __launch_bounds__(kSplitThreads) split_kernel(const SplitParams 
     // (rows of out that belong to no expert may say anything here)
     if (!there && threadIdx.x == 0 && i >= p.offsets[0] && i < p.offsets[p.experts]) serve_error(kErrRouting);
     const __nv_bfloat16* x = p.x + (there ? from * p.x_row : 0);
-    const auto largest = [&](uint32_t most) {                    // magnitude up to `most` of the row, as bits
-        uint32_t top = 0;
-        for (int c = threadIdx.x * 8; there && c < p.k; c += kSplitThreads * 8) {
-            const uint4 v = *reinterpret_cast<const uint4*>(x + c);
-#pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = (&v.x)[j] & 0x7fff7fffu, lo = w & 0xffffu, hi = w >> 16;
-                top = max(top, max(lo <= most ? lo : 0u, hi <= most ? hi : 0u));
-            }
-        }
+    const auto over_cta = [&](uint32_t top) {                    // the largest of all threads'
         top = __reduce_max_sync(0xffffffffu, top);
-        __syncthreads();
         if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = top;
         __syncthreads();
 #pragma unroll
         for (int j = 0; j < kSplitThreads / 32; ++j) top = max(top, part[j]);
         return top;
     };
-    uint32_t top = largest(0x7fffu);
-    if (top >= 0x7f80u) top = largest(0x7f7fu);
+    uint32_t top = 0;                                            // the largest magnitude, as bits
+    for (int c = threadIdx.x * 8; there && c < p.k; c += kSplitThreads * 8) {
+        const uint4 v = *reinterpret_cast<const uint4*>(x + c);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            const uint32_t w = (&v.x)[j] & 0x7fff7fffu;
+            top = max(top, max(w & 0xffffu, w >> 16));
+        }
+    }
+    top = over_cta(top);
+    if (top >= 0x7f80u) {                                        // an infinity or NaN: once more without
+        top = 0;
+#pragma unroll 1
+        for (int c = threadIdx.x; c < p.k; c += kSplitThreads) {
+            const uint32_t w = reinterpret_cast<const uint16_t*>(x)[c] & 0x7fffu;
+            if (w < 0x7f80u) top = max(top, w);
+        }
+        __syncthreads();
+        top = over_cta(top);
+    }
     // the largest's power of two, 2^(power + 7)
     const int power = top == 0 ? 0 : max((int)(top >> 7), 1) - 134;
     const float2 f = split_factors(power);
-    // bits of 2^(power - 18): magnitudes from there on, and zeros, have their terms
-    const uint32_t least = power >= -108 ? (uint32_t)(power + 109) << 7 : power >= -115 ? 1u << (power + 115) : 1u;
-    float rest = 0.f;                                            // magnitudes of what this thread's terms leave out
-    for (int c0 = 0; c0 < p.k; c0 += kSplitThreads * 8) {
-        const int c = c0 + threadIdx.x * 8;
-        bool out = false;
-        if (c < p.k) {
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (there) v = *reinterpret_cast<const uint4*>(x + c);
-            uint32_t low = 0xffffffffu, high = 0u;               // less 1, so that a zero is no small one
+    uint32_t left = 0;                                           // bits of all that this thread's terms leave out
+    for (int c = threadIdx.x * 8; c < p.k; c += kSplitThreads * 8) {
+        uint4 v = make_uint4(0, 0, 0, 0);
+        if (there) v = *reinterpret_cast<const uint4*>(x + c);
+        uint32_t term[4][2];
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const uint32_t w = __vsub2((&v.x)[j] & 0x7fff7fffu, 0x00010001u);
-                low = __vminu2(low, w);
-                high = __vmaxs2(high, w);
-            }
-            out = min(low & 0xffffu, low >> 16) < least - 1 || max(high & 0xffffu, high >> 16) >= 0x7f7fu;
-            uint32_t term[4][2];
+        for (int j = 0; j < 4; ++j) {
+            float a = bf16_lo((&v.x)[j]) * f.x * f.y, b = bf16_hi((&v.x)[j]) * f.x * f.y;
+            uint16_t q[4];
+            split_terms(a, b, q);
+            left |= __float_as_uint(a) | __float_as_uint(b);
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
-                const float x0 = bf16_lo((&v.x)[j]), x1 = bf16_hi((&v.x)[j]);
-                float a = x0 * f.x * f.y, b = x1 * f.x * f.y;
-                if (out) {                                       // (2^-100: what has left fp32's range)
-                    if (a == 0.f && x0 != 0.f) rest += 0x1p-100f;
-                    if (b == 0.f && x1 != 0.f) rest += 0x1p-100f;
-                    if (!(fabsf(a) < 256.f)) { rest = INFINITY; a = 0.f; }
-                    if (!(fabsf(b) < 256.f)) { rest = INFINITY; b = 0.f; }
-                }
-                uint16_t q[4];
-                split_terms(a, b, q);
-                if (out) rest += (fabsf(a) + fabsf(b)) * 0x1p-16f;
-#pragma unroll
-                for (int t = 0; t < 4; ++t) term[t][j >> 1] = j & 1 ? term[t][j >> 1] | (uint32_t)q[t] << 16 : q[t];
-            }
-#pragma unroll
-            for (int t = 0; t < 4; ++t) *reinterpret_cast<uint2*>(to + (size_t)t * p.k + c) = make_uint2(term[t][0], term[t][1]);
+            for (int t = 0; t < 4; ++t) term[t][j >> 1] = j & 1 ? term[t][j >> 1] | (uint32_t)q[t] << 16 : q[t];
         }
-        const uint32_t marks = __ballot_sync(0xffffffffu, out);
+#pragma unroll
+        for (int t = 0; t < 4; ++t) *reinterpret_cast<uint2*>(to + (size_t)t * p.k + c) = make_uint2(term[t][0], term[t][1]);
+    }
+    // (above 2^16 bf16's smallest times 2^-power leave fp32's range, and nothing is left of them to be seen)
+    if (!__syncthreads_or((left & 0x7fffffffu) != 0 || power > 16)) {
+        if (threadIdx.x == 0) p.power[i] = power * 256;
+        return;
+    }
+    // where and how much is left out; no terms for what is infinite or NaN
+    float rest = 0.f;
+#pragma unroll 1
+    for (int c0 = 0; c0 < p.k; c0 += kSplitThreads * 8) {
+        float here = 0.f;
+#pragma unroll 1
+        for (int c = c0 + threadIdx.x * 8, end = min(c + 8, p.k); c < end && there; ++c) {
+            const float v = __bfloat162float(x[c]);
+            float a = v * f.x * f.y, b = 0.f;
+            uint16_t q[4];
+            if (a == 0.f && v != 0.f) here += 0x1p-100f;
+            if (fabsf(a) < 256.f) {
+                split_terms(a, b, q);
+                here += fabsf(a) * 0x1p-16f;
+            } else {
+                here = INFINITY;
+                for (int t = 0; t < 4; ++t) to[(size_t)t * p.k + c] = 0;
+            }
+        }
+        const uint32_t marks = __ballot_sync(0xffffffffu, here != 0.f);
         const int word = (c0 >> 8) + (threadIdx.x >> 5);
         if ((threadIdx.x & 31) == 0 && word < p.words) apart[word] = marks;
+        rest += here;
     }
-    int q = 0;
-    if (__syncthreads_or(rest != 0.f)) {
 #pragma unroll
-        for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
-        if ((threadIdx.x & 31) == 0) rests[threadIdx.x >> 5] = rest;
-        __syncthreads();
-        rest = 0.f;
-#pragma unroll
-        for (int j = 0; j < kSplitThreads / 32; ++j) rest += rests[j];
+    for (int o = 16; o; o >>= 1) rest += __shfl_xor_sync(0xffffffffu, rest, o);
+    if ((threadIdx.x & 31) == 0) rests[threadIdx.x >> 5] = rest;
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        for (int j = 1; j < kSplitThreads / 32; ++j) rest += rests[j];
         // each meets 448 at most; the next power of two above 2^18 times that
-        q = rest == INFINITY ? 255 : ilogbf(rest * (448.f * 0x1p18f)) + 1 + 128;
+        p.power[i] = power * 256 + (rest == 0.f ? 0 : rest == INFINITY ? 255 : ilogbf(rest * (448.f * 0x1p18f)) + 1 + 128);
     }
-    if (threadIdx.x == 0) p.power[i] = power * 256 + q;
 }
 
 // The maps. W [experts][rows][K]: 128 bytes of 128 rows (silu: of 64 of gate and 64 of up) per copy; rows and K behind the end
@@ -933,7 +989,8 @@ int launch_experts(ExpertParams& p, const paia_gemv_expert_args* a, uint8_t* ter
     const int rc = serve_allow_smem((const void*)expert_kernel<FMT, SILU, CG>, most, done);
     if (rc) return rc;
     const int grid = (sm_count() < kExpMaxGrid ? sm_count() : kExpMaxGrid) / CG * CG;
-    return serve_launch(expert_kernel<FMT, SILU, CG>, p, dim3((unsigned)grid), T::kThreads, smem > kSmemAlone ? smem : kSmemAlone, st, CG);
+    return serve_launch(expert_kernel<FMT, SILU, CG>, p, dim3((unsigned)grid), T::kThreads, smem > kSmemAlone ? smem : kSmemAlone,
+                        st, CG);
 }
 
 template <bool SILU>
