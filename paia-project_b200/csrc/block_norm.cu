@@ -127,7 +127,8 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const NormPara
             for (int i = 0; i < V; ++i) {
                 const int c = threadIdx.x + i * n;
                 if (c >= p.vecs) continue;
-                const float4 a = *reinterpret_cast<const float4*>(p.post + 8 * c), b = *reinterpret_cast<const float4*>(p.post + 8 * c + 4);
+                const float4 a = *reinterpret_cast<const float4*>(p.post + 8 * c);
+                const float4 b = *reinterpret_cast<const float4*>(p.post + 8 * c + 4);
                 const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[i][e] = y[i][e] * r * w[e];
@@ -175,7 +176,8 @@ __global__ void __launch_bounds__(kNormThreads) block_norm_kernel(const NormPara
             for (int i = 0; i < V; ++i) {
                 const int c = threadIdx.x + i * n;
                 if (c >= p.vecs) continue;
-                const float4 a = *reinterpret_cast<const float4*>(p.pre + 8 * c), b = *reinterpret_cast<const float4*>(p.pre + 8 * c + 4);
+                const float4 a = *reinterpret_cast<const float4*>(p.pre + 8 * c);
+                const float4 b = *reinterpret_cast<const float4*>(p.pre + 8 * c + 4);
                 const float w[8] = {a.x, a.y, a.z, a.w, b.x, b.y, b.z, b.w};
 #pragma unroll
                 for (int e = 0; e < 8; ++e) y[i][e] = y[i][e] * r * w[e];
@@ -194,7 +196,8 @@ int launch_norm(const NormParams& p, cudaStream_t st) {
     int d = 0, per_sm = 0;
     if (cudaGetDevice(&d) == cudaSuccess && d < 64) per_sm = known[d].load(std::memory_order_relaxed);
     if (!per_sm) {                                   // CTAs of the largest size that an SM holds, smaller ones in proportion
-        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, block_norm_kernel<V, B>, kNormThreads, 0) != cudaSuccess || per_sm < 1) {
+        if (cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, block_norm_kernel<V, B>, kNormThreads, 0) != cudaSuccess ||
+            per_sm < 1) {
             (void)cudaGetLastError();
             per_sm = 1;
         }

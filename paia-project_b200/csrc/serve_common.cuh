@@ -1,4 +1,5 @@
-// Shared by the serving operators (serve_*.cu, block_*.cu): the device error word, PTX helpers and the launch. Like the GEMVs they allocate nothing, never synchronise and launch on the caller's stream.
+// Shared by the serving operators (serve_*.cu, block_*.cu): the device error word, PTX helpers and the launch. Like the GEMVs
+// they allocate nothing, never synchronise and launch on the caller's stream.
 #pragma once
 #include <cuda_bf16.h>
 #include <cuda_fp16.h>

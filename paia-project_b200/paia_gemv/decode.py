@@ -217,9 +217,10 @@ class PagedDecodeModel:
     adapters > 0: that many low-rank adapters of rank `rank` on the qkv, o, gate_up and down projections; self.adapter[b]
     (int32, -1: none) names the one of sequence b. qk_norm: RMS norm of q and k per head before the rotation. experts > 0:
     each layer's feed-forward block is that many experts of inner size `expert_inter`, weights in `kind` (bf16 or fp8), of
-    which every token takes its top_k (`scoring` as in serve.route); adapters are then on qkv and o, and the residual adds
-    and the norms (with post_norm those of the blocks' outputs too) are serve.block_norm. A sequence that is full must be retired by its caller; active[b] = False (self.active) makes row b padding: its cache and length
-    stay, its logits are those of an empty context."""
+    which every token takes its top_k (`scoring` as in serve.route; router logits are bf16 here, as the GEMV writes them);
+    adapters are then on qkv and o, and the residual adds and the norms (with post_norm those of the blocks' outputs too) are
+    serve.block_norm. A sequence that is full must be retired by its caller; active[b] = False (self.active) makes row b
+    padding: its cache and length stay, its logits are those of an empty context."""
 
     def __init__(self, lib, model, kind, lens, max_len=1024, page_size=16, cache="bf16", adapters=0, rank=16,
                  qk_norm=False, layers=None, seed=0, dims=None, experts=0, top_k=2, expert_inter=1024, scoring="softmax",
@@ -287,8 +288,8 @@ class PagedDecodeModel:
         self.padding = torch.full((B,), -1, dtype=torch.int32, device="cuda")
         self.seen = torch.empty(B, dtype=torch.int32, device="cuda")
         buf = lambda n: torch.zeros(B, n, **dev)   # noqa: E731
-        self.h, self.a, self.o, self.d = (buf(H) for _ in range(4))
-        self.qkv, self.gu, self.m, self.logits = buf((nh + 2 * nkv) * hd), buf(2 * I), buf(I), buf(V)
+        self.h, self.a, self.o = (buf(H) for _ in range(3))
+        self.qkv, self.logits = buf((nh + 2 * nkv) * hd), buf(V)
         self.q, self.attn = torch.zeros(B, nh, hd, **dev), torch.zeros(B, nh, hd, **dev)
         self.experts, self.scoring = experts, scoring
         if experts:
@@ -297,6 +298,8 @@ class PagedDecodeModel:
             self.router_logits = buf(experts)
             self.mid = torch.zeros(B * top_k, expert_inter, **dev)
             self.expert_out = torch.zeros(B * top_k, H, **dev)
+        else:
+            self.gu, self.m, self.d = buf(2 * I), buf(I), buf(H)
 
     def _project(self, lay, name, x, y):
         """y = the projection of every row, plus the row's adapter."""
