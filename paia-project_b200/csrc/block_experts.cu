@@ -18,10 +18,11 @@
 //            two rounds, is cut into equal runs of units. A tile cut by a run's end leaves its parts in the workspace and
 //            the last CTA to arrive joins them in the order of K (the same bits whichever it is); no CTA waits for another.
 // Every wait on a barrier is bounded; one that gives up sets code 15 and the CTA stops.
-// Measured: one token's 8 experts of 2048 x 4096 in bf16 26.4 us (5.1 TB/s; 4 of it the launch and what precedes the first
-// row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 79 (6.0 TB/s), 64 of 4096 x 1024 for 61 tokens 54; 8192 rows, 8
-// experts of 4096 x 14336 in bf16 790 (1.2 PFLOP/s, tensor pipe 79 % busy; in runs of seconds, under the power cap, 950);
-// 16384 rows, 64 experts of 2048 x 4096 in e4m3 350-410 (conversion and its hand-over to the products bound it).
+// Measured: one token's 8 experts of 2048 x 4096 in bf16 26.6 us (5.0 TB/s; 4 of it the launch and what precedes the first
+// row), 64 experts of 2048 x 3584 in e4m3 for 32 tokens 79 (6.0 TB/s; 82 in long runs), 64 of 4096 x 1024
+// for 61 tokens 54 (56); 8192 rows, 8 experts of 4096 x 14336 in bf16 775 (1.24 PFLOP/s, tensor pipe 79 % busy; in runs of
+// seconds, under the power cap, 850 to 950); 16384 rows, 64 experts of 2048 x 4096 in e4m3 355-410 (conversion and its hand-over
+// to the products bound it).
 #include "paia_gemv.h"
 #include "block_tc5.cuh"
 

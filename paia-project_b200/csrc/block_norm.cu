@@ -7,9 +7,10 @@
 // Bound: HBM for many rows (each input read once, h' and out written once), latency for few: ids -> rows -> two sums over
 // the CTA. A row is one CTA's; a thread keeps its 16-byte pieces of the row in registers from the first load to the last
 // store, so nothing is read twice.
-// Measured: 1 row of 4096 2.1 us (little more than the launch), 61 rows of 8 summed 4.1, 8192 rows of 3584 with both norms 51
-// (4.6 TB/s; 68 % of the issue slots), 4096 rows of 2 summed 33 (5.1 TB/s). Two or four pieces per thread, or the next row's
-// loads ahead, were no faster: 54, 58 and 49-60 us for the 8192.
+// Measured: 1 row of 4096 2.1 us (little more than the launch), 61 rows of 8 summed 4.2, 8192 rows of 3584 with both norms 51
+// (4.6 TB/s; 64 % of the issue slots: post and pre are read again for every row, 28 KB from the caches beside the 14 of its x and
+// h), 4096 rows of 2 summed 33 (5.1 TB/s). Two or four pieces per thread, or the next row's loads ahead, were no faster: 54, 58
+// and 49-60 us for the 8192.
 #include "paia_gemv.h"
 #include "serve_common.cuh"
 

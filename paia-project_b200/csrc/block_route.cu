@@ -14,10 +14,16 @@
 //           (a token's experts differ, so its lanes count apart): a slot's rank among the warp's. Then a prefix over the
 //           CTA's warps, over the CTAs before, and over the experts before.
 //   place   rank + those three prefixes.
-// Bound: latency for a batch (logits -> top_k dependent selections -> prefixes -> stores), the selections' issue for prompts.
+// Bound: latency for one token (logits -> top_k dependent selections -> prefixes -> stores); for a batch the same on the
+// few SMs of its cluster, 28 % of their issue slots full (256 experts, 8 of them, softmax / sigmoid: 1 token 3.7 / 4.8 us, the 16
+// of one CTA's warps 4.6 / 6.1, 17 in two CTAs 5.1 / 6.6, 128 in eight 6.9 / 8.5, 250, two for a warp, 9.8 / 12.2, and 14.6 where
+// one is done in fp64); for
+// prompts the selections' issue, and in the second launch the counts of all CTAs, which every CTA reads (257 tokens, one expert
+// each: of 64 experts 6.8, of 256 10.9).
 // Up to kRouteClusterTokens tokens one cluster does it all, exchanging counts through distributed shared memory; above, a
 // second launch places what the first has chosen and counted.
-// Measured: 1 token of 64 experts 3.0 us (2.3 is the launch), 250 of 256 experts under sigmoid 12.4, 8192 of 128 12.8.
+// Measured: 1 token of 64 experts 3.1 us (2.3 is the launch), 250 of 256 experts under sigmoid with a bias 12.2 to 14.6, 8192 of
+// 128 13.2, of 1024 113.
 #include <cooperative_groups.h>
 #include <type_traits>
 #include "paia_gemv.h"
@@ -33,7 +39,7 @@ template <bool ONE>
 using RouteCount = std::conditional_t<ONE, unsigned short, int>;
 constexpr int kPlaceThreads = 1024;
 constexpr int kRouteCluster = 8;                     // most CTAs of the one-launch form
-constexpr int kRouteClusterTokens = 256;            // (500 of 256 experts: 13.8 us here, 11 in two launches; 250: 9.2)
+constexpr int kRouteClusterTokens = 256;             // (256 experts, softmax: 256 9.8 us, 257 in two launches 11.4; 500 here 13.8)
 constexpr int kRouteMaxExperts = 1024;
 constexpr int kRouteMaxTopK = 32;
 constexpr int kRouteMaxGrid = 160;                   // the workspace holds the counts of this many CTAs
