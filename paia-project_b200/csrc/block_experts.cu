@@ -315,8 +315,9 @@ __device__ __forceinline__ float silu_mul(float g, float u) {
     asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + __expf(-g)));
     return g * r * u;
 }
-// The rows of a block whose terms leave something out, once more, behind the others and over what those have stored.
-// (Out of the way: nearly always there are none, and in the others' loop it took registers, 1.6 us of every call.)
+
+// The rows of a block whose terms leave something out, once more, behind the others and over what those have stored. (Out of the
+// way: nearly always there are none, and in the others' loop it took registers, 1.6 us of every call.)
 template <bool SILU>
 __device__ __noinline__ int rows_with_rest(const ExpertParams& p, const ExpWalk<1> walk, const ExpPart s, uint32_t d, float* exchange,
                                            int step) {
@@ -333,6 +334,7 @@ __device__ __noinline__ int rows_with_rest(const ExpertParams& p, const ExpWalk<
 #pragma unroll 1
     for (; rows; rows &= rows - 1) {
         const int t = __ffsll((long long)rows) - 1, code = p.x_power[s.row0 + t];
+        __syncwarp();                                            // (what follows wants the whole warp side by side)
         float v[4] = {0.f, 0.f, 0.f, 0.f};
         if (whole) {
             float w[16];                                         // (of 16 columns, as everywhere here)
@@ -351,6 +353,7 @@ __device__ __noinline__ int rows_with_rest(const ExpertParams& p, const ExpWalk<
         const float sum = v[0] + (v[1] + (v[2] + v[3]) * 0x1p-16f);
         const float r = with_rest(p, sum, code, scale, s.e, w_n, n < p.n, s.row0 + t);
         __nv_bfloat16* to = p.out + (long long)(s.row0 + t) * p.out_row + n;
+        __syncwarp();
         if (SILU) {                                              // (the barrier also puts the other warp's store ahead of this one)
             float* x = exchange + (step++ & 1) * (4 * 8 * 32) + lane;
             if (q >= 2) x[q * 8 * 32] = r;
@@ -362,6 +365,7 @@ __device__ __noinline__ int rows_with_rest(const ExpertParams& p, const ExpWalk<
     }
     return step;
 }
+
 // Whether `ok` holds in all 128 threads of the barrier (one for every part, so that none of them waits alone).
 __device__ __forceinline__ bool all_of(bool ok) {
     uint32_t r;
@@ -803,7 +807,7 @@ __global__ void __launch_bounds__(Exp<FMT, CG>::kThreads, 1) expert_kernel(const
 // v = x / 2^power lies below 256. From 2^-18 on the terms are v exactly (bf16 has 8 bits, and the last one's is 2^-25 or more,
 // the step of 2^-16 t3); below they leave out up to 2^-26, and of an infinity or NaN all. The groups of 8 along K that have
 // such an element are marked, and where a sum is not large enough beside all that is left out of its row, it is added from x and
-// W themselves (rest_sums). (Without that the smallest elements were lost where W is zero at the largest, and a single infinity
+// W themselves (rows_with_rest). (Without that the smallest elements were lost where W is zero at the largest, and a single infinity
 // made all of a row NaN. Rows of heavy tails with a few elements of 4000 times the others, 256 of them: 79 us before, 1709 with the
 // rest added to every sum, 404 as here; normal rows with such elements 82.)
 struct SplitParams {

@@ -179,6 +179,37 @@ def test_small_elements_whose_large_neighbours_meet_no_weight(L, ws, counts, n, 
     assert torch.equal(out, again) and L.device_error() == 0
 
 
+@pytest.mark.parametrize("silu", [False, True])
+def test_captured_calls_follow_what_x_holds(L, silu):
+    """e4m3, few rows: a captured call on rows of ordinary values, then of elements that only meet zeros of W beside larger ones,
+    infinities among them, then ordinary ones again: to the bit as calls of their own."""
+    from paia_gemv import serve
+    g = gen(18)
+    space = serve.expert_workspace(L)
+    counts = [7, 0, 30, 1]
+    w, s, values = C.weights(4, 96, 512, "fp8", g, DEV)
+    w[:, 1::2, :8] = 0
+    off, m = C.groups(counts, DEV), sum(counts)
+    plain = torch.randn(m, 512, generator=g, device=DEV).to(C.BF16)
+    wide = (plain.float() * 2.0 ** -30).to(C.BF16)
+    wide[:, :8] = 3.0
+    endless = wide.clone()
+    endless[::3, 100] = float("inf")
+    x, out = plain.clone(), torch.zeros(m, 48 if silu else 96, dtype=C.BF16, device=DEV)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        serve.expert_matmul(L, w, x, off, out, space, scales=s, silu=silu)
+    for now in (plain, wide, endless, plain):
+        x.copy_(now)
+        graph.replay()
+        alone = torch.zeros_like(out)
+        serve.expert_matmul(L, w, now, off, alone, space, scales=s, silu=silu)
+        assert torch.equal(out.view(torch.int16), alone.view(torch.int16))
+        assert bool(torch.isfinite(out).all()) == (now is not endless)
+        if now is wide:                                          # rows that are zero at the large elements
+            assert bool((out[:, 1::2] != 0).any()) and out[:, 1::2].abs().max() < 2.0 ** -20
+
+
 # More than two rounds of tiles: runs of K that end inside tiles, then whole tiles, three parts and more for every CTA (pair).
 # Units of K: one, three with the last one short, seven.
 @pytest.mark.parametrize("silu", [False, True])
